@@ -221,6 +221,41 @@ int tsc_silu(tsc_ctx* ctx, int32_t dtype, const void* x, int64_t numel, void* y)
 /* y = a + b elementwise, fp32 math (elementwise.ts:33-40).  y may alias a. */
 int tsc_add(tsc_ctx* ctx, int32_t dtype, const void* a, const void* b, int64_t numel, void* y);
 
+/* Group norm over the rows of each sample, channels last, with an optional SiLU:
+ *   y = (x - mean) / sqrt(var + eps) * gamma + beta,  then y / (1 + exp(-y)) with apply_silu,
+ * mean and (biased) var over the sample's rows and the C / groups consecutive channels of a group.
+ *   x, y       (N,C) `dtype`, aligned to the element size (16-byte aligned buffers and rows of whole
+ *              16 bytes are fastest); y may be x itself, no other overlap
+ *   cu_rows    device int32 (B+1), non-decreasing: sample b is rows [cu_rows[b], cu_rows[b+1]).
+ *              Values outside [0, N] are clamped; an array that decreases gives undefined values but
+ *              no access out of bounds.  NULL: B samples of N / B rows each.
+ *   gamma/beta (C) `dtype`, NULL = 1 / 0.  groups divides C.
+ *   zero_rest  rows of y outside every sample: 0 = left as they were, 1 = set to zero
+ *   stats      NULL, or device fp32 (B, groups, 2), 8-byte aligned: mean and 1 / sqrt(var + eps) for
+ *              the backward pass (not written for samples without rows)
+ *   workspace  device scratch of tsc_groupnorm_workspace_bytes(..., backward = 0) bytes, 16-byte
+ *              aligned; the context keeps nothing, so calls with scratch of their own may overlap
+ *              and be captured.  -1 from tsc_groupnorm_workspace_bytes: sizes out of range.
+ * fp32 statistics about the data's own means, merged in fp64.  The sums have one fixed order.
+ * No counterpart in the reference's sparse path, whose blocks normalize rows only
+ * (src/sparse/ops/norm.ts:10-140); a SparseTensor's samples are its layout
+ * (src/sparse/sparse_tensor.ts:216-237). */
+int64_t tsc_groupnorm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C,
+                                      int32_t groups, int32_t backward);
+int tsc_groupnorm(tsc_ctx* ctx, int32_t dtype, const void* x, const int32_t* cu_rows, int32_t B,
+                  int64_t N, int32_t C, int32_t groups, const void* gamma, const void* beta,
+                  float eps, int32_t apply_silu, int32_t zero_rest, float* stats, void* workspace,
+                  void* y);
+/* Its gradient: dx (N,C), and dgamma, dbeta (C) summed over all samples in `dtype` (NULL = not
+ * wanted), from dy, the same x, cu_rows, gamma, beta and apply_silu and the stats that
+ * tsc_groupnorm wrote; workspace with backward = 1.  dx must not overlap dy or x.  zero_rest is
+ * about rows of dx. */
+int tsc_groupnorm_backward(tsc_ctx* ctx, int32_t dtype, const void* dy, const void* x,
+                           const int32_t* cu_rows, int32_t B, int64_t N, int32_t C, int32_t groups,
+                           const void* gamma, const void* beta, int32_t apply_silu,
+                           int32_t zero_rest, const float* stats, void* workspace, void* dx,
+                           void* dgamma, void* dbeta);
+
 /* Sparse ResBlock: out = x + conv2(silu(LN(conv1(x)+b1))) + b2, with C=Ci=Co.
  * LN uses eps and gamma/beta (NULL = 1/0).  out must not overlap x (TSC_ERR_INVALID if any
  * byte of the two (N,C) ranges is shared).  The intermediate (N,C)

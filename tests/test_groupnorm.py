@@ -1,0 +1,57 @@
+"""Refusals of group_norm that need no GPU: arguments are checked before any device call."""
+import ctypes
+
+import pytest
+import torch
+
+
+def test_group_norm_refuses_bad_arguments(pkg):
+    x = torch.zeros((10, 12))
+    with pytest.raises(pkg.TscError, match="do not divide"):
+        pkg.group_norm(x, 5)
+    with pytest.raises(pkg.TscError, match="do not divide"):
+        pkg.group_norm(x, 0)
+    with pytest.raises(pkg.TscError, match="do not divide"):
+        pkg.group_norm(torch.zeros((3, 0)), 1)
+    with pytest.raises(pkg.TscError, match=r"\(N, C\) or"):
+        pkg.group_norm(torch.zeros(12), 3)
+    with pytest.raises(pkg.TscError, match="weight and bias"):
+        pkg.group_norm(x, 3, torch.ones(11))
+    with pytest.raises(pkg.TscError, match="weight and bias"):
+        pkg.group_norm(x, 3, torch.ones(12), torch.zeros(12, dtype=torch.float16))
+    with pytest.raises(pkg.TscError, match="out has the wrong"):
+        pkg.group_norm(x, 3, out=torch.zeros((9, 12)))
+    with pytest.raises(pkg.TscError, match="unsupported dtype"):
+        pkg.group_norm(x.double(), 3)
+    with pytest.raises(pkg.TscError, match="not on a GPU"):
+        pkg.group_norm(x, 3)
+
+
+def test_workspace_bytes(pkg):
+    lib = pkg.load_library()
+    f = lib.tsc_groupnorm_workspace_bytes
+    assert f(2, 2, 1000, 64, 32, 0) > 0
+    assert f(2, 2, 1000, 64, 32, 1) >= f(2, 2, 1000, 64, 32, 0) + 8 * 64 * 2
+    for bad in ((3, 1, 10, 64, 32, 0), (0, -1, 10, 64, 32, 0), (0, 1, -1, 64, 32, 0),
+                (0, 1, 10, 64, 0, 0), (0, 1, 10, 64, 30, 0), (0, 1, 2 ** 31, 64, 32, 0),
+                (0, 1, 10, 65537, 1, 0)):
+        assert f(*bad) == -1, bad
+        assert lib.tsc_last_error()
+
+
+def test_null_context(pkg):
+    lib = pkg.load_library()
+    P = ctypes.c_void_p
+    assert lib.tsc_groupnorm(None, 0, P(16), None, 1, 4, 8, 2, None, None, 1e-5, 0, 0, None, P(16),
+                             P(16)) == 1
+    assert b"null context" in lib.tsc_last_error()
+    assert lib.tsc_groupnorm_backward(None, 0, P(16), P(16), None, 1, 4, 8, 2, None, None, 0, 0,
+                                      P(16), P(16), P(64), None, None) == 1
+    assert b"null context" in lib.tsc_last_error()
+
+
+def test_cu_rows_of_a_sparse_tensor(pkg):
+    coords = torch.tensor([[0, 1, 2, 3], [0, 4, 0, 1], [2, 0, 5, 0]], dtype=torch.int32)
+    x = pkg.SparseTensor(torch.zeros((3, 8)), coords)
+    assert x.cu_rows.tolist() == [0, 2, 2, 3] and x.cu_rows.dtype == torch.int32
+    assert x.replace(torch.ones((3, 4))).cu_rows is x.cu_rows

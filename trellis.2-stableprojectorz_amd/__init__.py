@@ -19,17 +19,18 @@ from .sparse_tensor import SparseTensor, Scale, Fraction, SCALE_IDENTITY, comput
 from .conv3d import SparseConv3d, SparseResBlock3d, get_neighbor_map, neighbor_cache_key  # noqa: F401
 from .ops import (NeighborMap, build_neighbor_map, map_conv_order, map_gather_plan,  # noqa: F401
                   sparse_conv3d,
-                  layer_norm, silu, add, sparse_resblock, sparse_subdivide, subdivide_count,
+                  layer_norm, group_norm, silu, add, sparse_resblock, sparse_subdivide, subdivide_count,
                   sparse_linear, sparse_attention, scaled_dot_product_attention)
 from .spatial import SparseSubdivide  # noqa: F401
-from .blocks import SparseLinear, SparseConvNeXtBlock3d  # noqa: F401
+from .blocks import SparseLinear, SparseGroupNorm, SparseConvNeXtBlock3d  # noqa: F401
 from .weights import SafetensorsFile, SafetensorsHeader, TensorEntry, MultiFileLoader  # noqa: F401
 from . import workloads  # noqa: F401
 
 __all__ = [
     "TscError", "SparseTensor", "SparseConv3d", "SparseResBlock3d", "NeighborMap",
-    "build_neighbor_map", "map_conv_order", "map_gather_plan", "sparse_conv3d", "layer_norm", "silu", "add", "sparse_resblock",
-    "sparse_subdivide", "subdivide_count", "SparseSubdivide", "sparse_linear", "SparseLinear",
+    "build_neighbor_map", "map_conv_order", "map_gather_plan", "sparse_conv3d", "layer_norm", "group_norm",
+    "silu", "add", "sparse_resblock",
+    "sparse_subdivide", "subdivide_count", "SparseSubdivide", "sparse_linear", "SparseLinear", "SparseGroupNorm",
     "SparseConvNeXtBlock3d", "sparse_attention", "scaled_dot_product_attention", "SafetensorsFile", "SafetensorsHeader", "TensorEntry", "MultiFileLoader",
     "get_neighbor_map", "neighbor_cache_key", "workloads",
 ]

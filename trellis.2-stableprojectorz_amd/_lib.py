@@ -72,6 +72,11 @@ _SIGNATURES = {
     "tsc_conv_fused_noalloc": (_I32, [_P, _I32, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P,
                                       _P, _F32, _P]),
     "tsc_layernorm": (_I32, [_P, _I32, _P, _I64, _I32, _P, _P, _F32, _I32, _P]),
+    "tsc_groupnorm_workspace_bytes": (_I64, [_I32, _I32, _I64, _I32, _I32, _I32]),
+    "tsc_groupnorm": (_I32, [_P, _I32, _P, _P, _I32, _I64, _I32, _I32, _P, _P, _F32, _I32, _I32, _P,
+                             _P, _P]),
+    "tsc_groupnorm_backward": (_I32, [_P, _I32, _P, _P, _P, _I32, _I64, _I32, _I32, _P, _P, _I32,
+                                      _I32, _P, _P, _P, _P, _P]),
     "tsc_silu": (_I32, [_P, _I32, _P, _I64, _P]),
     "tsc_add": (_I32, [_P, _I32, _P, _P, _I64, _P]),
     "tsc_resblock": (_I32, [_P, _I32, _P, _P, _P, _I64, _I32, _P, _P, _P, _P, _F32, _P, _P, _P]),
@@ -146,6 +151,7 @@ class Context:
         check(self.lib.tsc_ctx_create(device, _P(stream), ctypes.byref(h)))
         self.handle = h
         self._stream = stream
+        self.profiling = False
 
     def bind(self):
         """Point the context at torch's current stream; returns the raw handle."""
@@ -163,6 +169,7 @@ class Context:
     def profile(self, on: bool) -> None:
         """Bracket every kernel this context launches with hipEvents (per-kernel timing)."""
         check(self.lib.tsc_profile_enable(self.handle, int(on)))
+        self.profiling = bool(on)
 
     def profile_results(self) -> dict:
         """{kernel name: (total ms, launches)} over the launches since the last reset."""
@@ -191,3 +198,27 @@ def context(device: int) -> Context:
         with _lock:
             _contexts[device] = ctx
     return ctx
+
+
+_stream_handles: dict[tuple[int, int], ctypes.c_void_p] = {}
+
+
+def stream_handle(device: int):
+    """(library, handle of a context on torch's current stream) for the ops that keep nothing in a
+    context: one per stream, made at its first use and never re-pointed, so that calls from several
+    threads, on several streams or under graph capture (where the device's shared context cannot
+    wait for the stream it was on) do not meet.  While the shared context is profiled it is that one."""
+    import torch
+
+    shared = _contexts.get(device)
+    if shared is not None and shared.profiling:
+        return shared.lib, shared.bind()
+    lib = load_library()
+    stream = torch.cuda.current_stream(device).cuda_stream
+    with _lock:
+        h = _stream_handles.get((device, stream))
+        if h is None:
+            h = _P()
+            check(lib.tsc_ctx_create(device, _P(stream), ctypes.byref(h)))
+            _stream_handles[device, stream] = h
+    return lib, h

@@ -1,0 +1,30 @@
+"""Gradients of the differentiable ops (torch.autograd.Function around two C-ABI calls each).
+
+The backward calls run on the stream that is current there, which is the forward's; their scratch
+comes from torch's allocator, so a training step can be captured into a graph.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+class GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, cu, b, groups, eps, silu):
+        stats = torch.empty((b, groups, 2), dtype=torch.float32, device=x.device)
+        out = ops._group_norm(x, weight, bias, cu, b, groups, eps, silu, None, stats)
+        ctx.save_for_backward(x, weight, bias, cu, stats)
+        ctx.args = (b, groups, silu)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, cu, stats = ctx.saved_tensors
+        b, groups, silu = ctx.args
+        dx, dw, db = ops._group_norm_backward(dy.contiguous(), x, weight, bias, cu, b, groups, silu,
+                                              stats, any(ctx.needs_input_grad[1:3]))
+        return dx, dw, db, None, None, None, None, None

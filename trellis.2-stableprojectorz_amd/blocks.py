@@ -32,6 +32,23 @@ class SparseLinear:
     __call__ = forward
 
 
+class SparseGroupNorm:
+    """Group norm of each sample's voxels, optionally with SiLU (ops.group_norm over x.cu_rows)."""
+
+    def __init__(self, num_groups: int, weight: torch.Tensor | None = None,
+                 bias: torch.Tensor | None = None, eps: float = 1e-5, silu: bool = False):
+        self.num_groups, self.eps, self.silu = num_groups, eps, silu
+        self.weight = None if weight is None else weight.contiguous()
+        self.bias = None if bias is None else bias.contiguous()
+
+    def forward(self, x: SparseTensor) -> SparseTensor:
+        cu = x.cu_rows
+        return x.replace(ops.group_norm(x.feats, self.num_groups, self.weight, self.bias, cu,
+                                        self.eps, self.silu))
+
+    __call__ = forward
+
+
 class SparseConvNeXtBlock3d:
     def __init__(self, conv_weight: torch.Tensor, conv_bias: torch.Tensor | None,
                  linear0_weight: torch.Tensor, linear0_bias: torch.Tensor | None,

@@ -523,6 +523,80 @@ int tsc_layernorm(tsc_ctx* ctx, int32_t dtype, const void* x, int64_t N, int32_t
   return layernorm_launch(ctx, dtype, x, N, C, gamma, beta, eps, apply_silu, y);
 }
 
+static int validate_groupnorm(const char* what, int32_t dtype, int32_t B, int64_t N, int32_t C,
+                              int32_t groups) {
+  if (!elem_size(dtype)) return fail(TSC_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
+  if (N < 0 || N > INT32_MAX || C <= 0 || B < 0 || B > (1 << 20))
+    return fail(TSC_ERR_INVALID, "%s: bad sizes N=%lld C=%d B=%d", what, (long long)N, C, B);
+  if (C > 65536) return fail(TSC_ERR_UNSUPPORTED, "%s: C=%d exceeds 65536", what, C);
+  if (groups <= 0 || C % groups)
+    return fail(TSC_ERR_INVALID, "%s: %d groups do not divide C=%d", what, groups, C);
+  return TSC_OK;
+}
+
+int64_t tsc_groupnorm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C,
+                                      int32_t groups, int32_t backward) {
+  g_err[0] = 0;
+  if (validate_groupnorm("groupnorm_workspace_bytes", dtype, B, N, C, groups)) return -1;
+  return groupnorm_workspace_bytes(dtype, B, N, C, groups, backward);
+}
+
+int tsc_groupnorm(tsc_ctx* ctx, int32_t dtype, const void* x, const int32_t* cu_rows, int32_t B,
+                  int64_t N, int32_t C, int32_t groups, const void* gamma, const void* beta,
+                  float eps, int32_t apply_silu, int32_t zero_rest, float* stats, void* workspace,
+                  void* y) {
+  g_err[0] = 0;
+  int st = check_ctx(ctx);
+  if (!st) st = validate_groupnorm("groupnorm", dtype, B, N, C, groups);
+  if (st) return st;
+  if (!(eps >= 0.f)) return fail(TSC_ERR_INVALID, "groupnorm: eps must be >= 0");
+  if (!cu_rows && B > 0 && N % B)
+    return fail(TSC_ERR_INVALID, "groupnorm: N=%lld rows are not %d equal samples", (long long)N, B);
+  if (B == 0 || N == 0) return TSC_OK;
+  const int es = elem_size(dtype);
+  const size_t bytes = (size_t)N * C * es;
+  if (!x || !y || !workspace) return fail(TSC_ERR_INVALID, "groupnorm: null buffer");
+  if (!aligned(x, es) || !aligned(y, es) || (gamma && !aligned(gamma, es)) ||
+      (beta && !aligned(beta, es)) || !aligned(workspace, 16) || (stats && !aligned(stats, 8)) ||
+      (cu_rows && !aligned(cu_rows, 4)))
+    return fail(TSC_ERR_INVALID, "groupnorm: x, y, gamma and beta must be aligned to their element "
+                                 "size, stats to 8 bytes, workspace to 16");
+  if (x != y && overlaps(x, bytes, y, bytes))
+    return fail(TSC_ERR_INVALID, "groupnorm: y overlaps x without being x");
+  DeviceGuard g(ctx->device);
+  return groupnorm_launch(ctx, dtype, x, cu_rows, B, N, C, groups, gamma, beta, eps, apply_silu,
+                          zero_rest, stats, workspace, y);
+}
+
+int tsc_groupnorm_backward(tsc_ctx* ctx, int32_t dtype, const void* dy, const void* x,
+                           const int32_t* cu_rows, int32_t B, int64_t N, int32_t C, int32_t groups,
+                           const void* gamma, const void* beta, int32_t apply_silu,
+                           int32_t zero_rest, const float* stats, void* workspace, void* dx,
+                           void* dgamma, void* dbeta) {
+  g_err[0] = 0;
+  int st = check_ctx(ctx);
+  if (!st) st = validate_groupnorm("groupnorm_backward", dtype, B, N, C, groups);
+  if (st) return st;
+  if (B == 0 || (!cu_rows && N % B))
+    return fail(TSC_ERR_INVALID, "groupnorm_backward: N=%lld rows are not %d equal samples",
+                (long long)N, B);
+  const int es = elem_size(dtype);
+  const size_t bytes = (size_t)N * C * es;
+  if (!workspace || !stats || (N > 0 && (!dy || !x || !dx)))
+    return fail(TSC_ERR_INVALID, "groupnorm_backward: null buffer");
+  if (!aligned(x, es) || !aligned(dy, es) || !aligned(dx, es) || (gamma && !aligned(gamma, es)) ||
+      (beta && !aligned(beta, es)) || (dgamma && !aligned(dgamma, es)) ||
+      (dbeta && !aligned(dbeta, es)) || !aligned(workspace, 16) || !aligned(stats, 8) ||
+      (cu_rows && !aligned(cu_rows, 4)))
+    return fail(TSC_ERR_INVALID, "groupnorm_backward: x, dy, gamma, beta and the gradients must be "
+                                 "aligned to their element size, stats to 8 bytes, workspace to 16");
+  if (overlaps(dx, bytes, x, bytes) || overlaps(dx, bytes, dy, bytes))
+    return fail(TSC_ERR_INVALID, "groupnorm_backward: dx overlaps x or dy");
+  DeviceGuard g(ctx->device);
+  return groupnorm_backward_launch(ctx, dtype, dy, x, cu_rows, B, N, C, groups, gamma, beta,
+                                   apply_silu, zero_rest, stats, workspace, dx, dgamma, dbeta);
+}
+
 int tsc_silu(tsc_ctx* ctx, int32_t dtype, const void* x, int64_t numel, void* y) {
   g_err[0] = 0;
   int st = check_ctx(ctx);

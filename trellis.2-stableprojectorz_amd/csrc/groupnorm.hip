@@ -1,0 +1,706 @@
+// Group norm over the rows of each sample, channels last, with an optional SiLU, and its gradient.
+//
+//   sample b = rows [cu[b], cu[b+1]) of x (N, C); its group g = channels [g C/G, (g+1) C/G); n values
+//   mean = sum x / n;  var = sum (x - mean)^2 / n;  rstd = 1 / sqrt(var + eps)
+//   xh = (x - mean) rstd;  h = xh gamma + beta;  y = h, or h s with s = 1 / (1 + exp(-h))
+//   dh = dy, or dy s (1 + h (1 - s));  dbeta = sum dh;  dgamma = sum dh xh   (over all samples)
+//   dx = rstd (gamma dh - A / n - xh B / n),  A = sum gamma dh, B = sum gamma dh xh  (sample, group)
+//
+// Bound by memory: the statistics need all of a sample before its first output, so x (and dy) is
+// read twice, the second time from the 256 MB memory-side cache as far as it fits.
+// Two launches each way.  The rows are cut into T tiles and the channels into slabs of whole 16-byte
+// vectors; a block owns one (tile, slab), each thread one vector column of it and every TY-th row.
+// The first kernel leaves one partial result per (tile, sample, granule) - a granule is the largest
+// run of channels that lies in one group and one slab - and each block of the second kernel adds up
+// those of its own groups: a few KB from the L2, and no launch or atomic in between, so that the
+// sums have one order.  Tile t and sample b meet in slot t + b: along the rows one of the two grows
+// at each step, so slots are distinct, and every slot in [0, T + B - 1) is written.
+// Statistics are fp32 (mean, M2) pairs about their own means, merged pairwise, and merged over tiles
+// in fp64 about the first one's mean: no sum of squares of raw values, which would lose a spread
+// that is small beside the mean.
+
+#include <algorithm>
+#include <initializer_list>
+#include <type_traits>
+
+#include "rownorm.h"
+#include "tsc_internal.h"
+
+namespace tsc {
+namespace {
+
+constexpr int kNT = 256;       // threads of a block
+constexpr int kParamCh = 8;    // channels of a block that adds up dgamma and dbeta
+constexpr int kMaxVec = 32;    // vector columns of a slab
+constexpr int kMaxGroups = 256;  // groups that a slab can touch: kMaxVec * 8 channels
+
+struct GnShape {
+  const int32_t* cu;  // null: B samples of N / B rows
+  int64_t N;
+  int32_t B, C, groups, cpg;  // cpg = C / groups
+  int32_t nvec, TX, TY, slabs;
+  int32_t T;           // row tiles
+  int64_t R;           // rows of a tile
+  int32_t gran, NG, GP;  // channels of a granule, granules in all, granules of a group
+};
+
+template <typename T, int VN>
+struct __attribute__((aligned(VN * sizeof(T)))) Pack {
+  T v[VN];
+};
+template <int BYTES>
+struct Word;
+template <>
+struct Word<16> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
+template <>
+struct Word<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
+template <>
+struct Word<4> { typedef uint32_t type; };
+template <>
+struct Word<2> { typedef uint16_t type; };
+
+// Outputs are next read by another layer's kernel; x is what the second pass wants kept.
+template <typename T, int VN>
+__device__ __forceinline__ void store_nt(T* p, const float (&f)[VN]) {
+  Pack<T, VN> o;
+#pragma unroll
+  for (int e = 0; e < VN; ++e) o.v[e] = (T)f[e];
+  typedef typename Word<VN * sizeof(T)>::type W;
+  __builtin_nontemporal_store(__builtin_bit_cast(W, o), (W*)p);
+}
+
+__device__ __forceinline__ void gn_segment(const GnShape& s, int b, int64_t* lo, int64_t* hi) {
+  if (!s.cu) {
+    const int64_t n = s.N / s.B;
+    *lo = b * n;
+    *hi = *lo + n;
+    return;
+  }
+  *lo = min<int64_t>(max<int64_t>(s.cu[b], 0), s.N);
+  *hi = min<int64_t>(max<int64_t>(s.cu[b + 1], *lo), s.N);
+}
+
+// The sample whose slots start tile t: the last one that begins at or before the tile's first row
+// (0 for tile 0, B - 1 past the last tile).  Every lane of the wave takes part.
+__device__ __forceinline__ int first_sample(const GnShape& s, int t) {
+  if (t == 0 || s.B == 1) return 0;
+  if (t >= s.T) return s.B - 1;
+  const int64_t row = t * s.R;
+  if (!s.cu) return (int)min<int64_t>(row / max<int64_t>(s.N / s.B, 1), s.B - 1);
+  int n = 0;
+  for (int b0 = 1; b0 < s.B; b0 += 64) {
+    const int b = b0 + (threadIdx.x & 63);
+    n += __popcll(__builtin_amdgcn_ballot_w64(b < s.B && s.cu[min(b, s.B - 1)] <= row));
+  }
+  return n;
+}
+
+struct Where {
+  int t, slab, col, ty, c0;  // tile, slab, vector column, first row's lane, first channel
+  bool live;
+  int b0, b1;                // samples of the tile's slots
+  int64_t r0, r1;            // its rows
+};
+template <int VN>
+__device__ __forceinline__ Where where(const GnShape& s, int t, int slab) {
+  Where w;
+  w.t = t;
+  w.slab = slab;
+  w.col = threadIdx.x % s.TX;
+  w.ty = threadIdx.x / s.TX;
+  const int vec = slab * s.TX + w.col;
+  w.live = w.ty < s.TY && vec < s.nvec;
+  w.c0 = vec * VN;
+  w.b0 = first_sample(s, t);
+  w.b1 = first_sample(s, t + 1);
+  w.r0 = t * s.R;
+  w.r1 = min<int64_t>(w.r0 + s.R, s.N);
+  return w;
+}
+
+// Zeros for the tile's rows before the first sample and after the last one.
+template <typename T, int VN>
+__device__ __forceinline__ void zero_rest(const GnShape& s, const Where& w, T* y) {
+  if (!s.cu || !w.live) return;
+  int64_t lo, hi, none;
+  gn_segment(s, 0, &lo, &none);
+  gn_segment(s, s.B - 1, &none, &hi);
+  const float z[VN] = {};
+  for (int64_t r = w.r0 + w.ty; r < w.r1; r += s.TY)
+    if (r < lo || r >= hi) store_nt<T, VN>(y + r * s.C + w.c0, z);
+}
+
+// ------------------------------------------------------------------------------- forward
+// Partial statistics: part[slot * NG + granule] = (mean, M2).
+template <typename T, int VN>
+__global__ void __launch_bounds__(kNT)
+    gn_stats_kernel(GnShape s, const T* __restrict__ x, float2* __restrict__ part) {
+  constexpr int KR = 8;  // rows in flight per thread
+  __shared__ float smean[kNT * VN], sm2[kNT * VN], scnt[kNT];
+  const Where w = where<VN>(s, blockIdx.x, blockIdx.y);
+  const int tid = threadIdx.x, SC = s.TX * VN;
+  const int g0 = w.slab * SC / s.gran, ng = min(SC / s.gran, s.NG - g0);
+  for (int b = w.b0; b <= w.b1; ++b) {
+    int64_t lo, hi;
+    gn_segment(s, b, &lo, &hi);
+    lo = max(lo, w.r0);
+    hi = min(hi, w.r1);
+    float2* dst = part + (int64_t)(w.t + b) * s.NG + g0;
+    if (hi <= lo) {  // uniform over the block
+      for (int i = tid; i < ng; i += kNT) dst[i] = make_float2(0.f, 0.f);
+      continue;
+    }
+    float cnt = 0.f, mean[VN], m2[VN];
+#pragma unroll
+    for (int e = 0; e < VN; ++e) mean[e] = m2[e] = 0.f;
+    if (w.live) {
+      const T* p = x + w.c0;
+      auto chunk = [&](int64_t r, int k, auto whole) {  // rows r, r + TY, ..., k of them
+        Pack<T, VN> v[KR];
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (decltype(whole)::value || i < k)
+            v[i] = *(const Pack<T, VN>*)(p + (r + (int64_t)i * s.TY) * s.C);
+        const float kf = decltype(whole)::value ? (float)KR : (float)k, ik = 1.f / kf;
+        const float f = kf / (cnt + kf);
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+          float a = 0.f, q = 0.f;
+#pragma unroll
+          for (int i = 0; i < KR; ++i)
+            if (decltype(whole)::value || i < k) a += (float)v[i].v[e];
+          a *= ik;
+#pragma unroll
+          for (int i = 0; i < KR; ++i)
+            if (decltype(whole)::value || i < k) {
+              const float d = (float)v[i].v[e] - a;
+              q = fmaf(d, d, q);
+            }
+          const float d = a - mean[e];
+          mean[e] = fmaf(d, f, mean[e]);
+          m2[e] += fmaf(d * d, f * cnt, q);
+        }
+        cnt += kf;
+      };
+      int64_t r = lo + w.ty;
+      for (; r + (int64_t)(KR - 1) * s.TY < hi; r += (int64_t)KR * s.TY) chunk(r, KR, std::true_type());
+      if (r < hi) chunk(r, (int)((hi - r + s.TY - 1) / s.TY), std::false_type());
+    }
+    __syncthreads();  // the granules of the sample before have been read
+#pragma unroll
+    for (int e = 0; e < VN; ++e) {
+      smean[tid * VN + e] = mean[e];
+      sm2[tid * VN + e] = m2[e];
+    }
+    scnt[tid] = cnt;
+    __syncthreads();
+    int half = 1;
+    while (2 * half < s.TY) half *= 2;
+    for (; half > 0 && s.TY > 1; half >>= 1) {
+      if (w.ty < half && w.ty + half < s.TY) {
+        const int o = tid + half * s.TX;
+        const float nb = scnt[o];
+        if (nb > 0.f) {
+          const float f = nb / (cnt + nb);
+#pragma unroll
+          for (int e = 0; e < VN; ++e) {
+            const float d = smean[o * VN + e] - mean[e];
+            mean[e] = fmaf(d, f, mean[e]);
+            m2[e] += fmaf(d * d, f * cnt, sm2[o * VN + e]);
+            smean[tid * VN + e] = mean[e];
+            sm2[tid * VN + e] = m2[e];
+          }
+          cnt += nb;
+          scnt[tid] = cnt;
+        }
+      }
+      __syncthreads();
+    }
+    // The first TX threads' channels, in order: one thread joins a granule's.
+    for (int i = tid; i < ng; i += kNT) {
+      const float* mc = smean + i * s.gran;
+      const float* qc = sm2 + i * s.gran;
+      float a = 0.f, q = 0.f;
+      for (int c = 0; c < s.gran; ++c) a += mc[c] - mc[0];
+      a = mc[0] + a / (float)s.gran;
+      for (int c = 0; c < s.gran; ++c) {
+        const float d = mc[c] - a;
+        q += fmaf(d * d, (float)(hi - lo), qc[c]);
+      }
+      dst[i] = make_float2(a, q);
+    }
+  }
+}
+
+// Threads of the block that add up one group's partials: a power of two.
+__device__ __forceinline__ int lanes_per_group(int ng) {
+  int p = kNT;
+  while (p * ng > kNT) p >>= 1;
+  return p;
+}
+
+// Adds a pair of doubles over each run of P threads; the run's first thread returns the sums.
+__device__ __forceinline__ void run_sum(double* sa, double* sb, int P, double* a, double* b) {
+  const int tid = threadIdx.x;
+  sa[tid] = *a;
+  sb[tid] = *b;
+  __syncthreads();
+  for (int half = P / 2; half > 0; half >>= 1) {
+    if ((tid & (P - 1)) < half) {
+      *a += sa[tid + half];
+      *b += sb[tid + half];
+      sa[tid] = *a;
+      sb[tid] = *b;
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int VN>
+__global__ void __launch_bounds__(kNT)
+    gn_apply_kernel(GnShape s, const T* x, const float2* __restrict__ part,
+                    const T* __restrict__ gamma, const T* __restrict__ beta, float eps,
+                    int32_t silu, int32_t rest, float* __restrict__ stats, T* y) {
+  constexpr int KR = 4;
+  __shared__ double sa[kNT], sb[kNT];
+  __shared__ float2 sg[kMaxGroups];
+  const Where w = where<VN>(s, blockIdx.x, blockIdx.y);
+  const int tid = threadIdx.x, SC = s.TX * VN;
+  const int gl = w.slab * SC / s.cpg, gh = (min((w.slab + 1) * SC, s.C) - 1) / s.cpg;
+  const int ng = gh - gl + 1, P = lanes_per_group(ng);
+  for (int b = w.b0; b <= w.b1; ++b) {
+    int64_t lo, hi;
+    gn_segment(s, b, &lo, &hi);
+    const int64_t beg = lo, end = hi;
+    lo = max(lo, w.r0);
+    hi = min(hi, w.r1);
+    if (hi <= lo) continue;
+    {
+      const int t0 = (int)(beg / s.R), nt = (int)((end - 1) / s.R) - t0 + 1;
+      const int g = gl + tid / P, j = tid & (P - 1);
+      double n = 0., d1 = 0., d2 = 0.;
+      float m0 = 0.f;
+      if (g <= gh) {
+        const float2* src = part + (int64_t)(t0 + b) * s.NG + (int64_t)g * s.GP;
+        m0 = src->x;
+        for (int k = 0; k < s.GP; ++k)
+          for (int i = j; i < nt; i += P) {
+            const float2 p = src[(int64_t)i * s.NG + k];
+            const int64_t a0 = max(beg, (t0 + i) * s.R), a1 = min(end, (t0 + i + 1) * s.R);
+            const double c = (double)((a1 - a0) * s.gran), d = (double)p.x - (double)m0;
+            d1 += c * d;
+            d2 += (double)p.y + c * d * d;
+          }
+      }
+      run_sum(sa, sb, P, &d1, &d2);
+      if (g <= gh && j == 0) {
+        n = (double)(end - beg) * s.cpg;
+        const double mean = (double)m0 + d1 / n;
+        const double q = d2 - d1 * d1 / n;
+        const double var = q < 0. ? 0. : q / n;  // NaN stays
+        const float2 r = make_float2((float)mean, (float)(1. / sqrt(var + (double)eps)));
+        sg[g - gl] = r;
+        if (stats && w.r0 <= beg && g * s.cpg >= w.slab * SC)
+          *(float2*)(stats + 2 * ((int64_t)b * s.groups + g)) = r;
+      }
+      __syncthreads();
+    }
+    if (w.live) {
+      float mean[VN], a[VN], c[VN];
+#pragma unroll
+      for (int e = 0; e < VN; ++e) {
+        const float2 m = sg[(w.c0 + e) / s.cpg - gl];
+        mean[e] = m.x;
+        a[e] = m.y * (gamma ? (float)gamma[w.c0 + e] : 1.f);
+        c[e] = beta ? (float)beta[w.c0 + e] : 0.f;
+      }
+      auto chunk = [&](int64_t r, int k, auto whole) {
+        Pack<T, VN> v[KR];
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (decltype(whole)::value || i < k)
+            v[i] = *(const Pack<T, VN>*)(x + (r + (int64_t)i * s.TY) * s.C + w.c0);
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (decltype(whole)::value || i < k) {
+            float o[VN];
+#pragma unroll
+            for (int e = 0; e < VN; ++e) {
+              const float h = fmaf((float)v[i].v[e] - mean[e], a[e], c[e]);
+              o[e] = silu ? h * __builtin_amdgcn_rcpf(1.f + __expf(-h)) : h;
+            }
+            store_nt<T, VN>(y + (r + (int64_t)i * s.TY) * s.C + w.c0, o);
+          }
+      };
+      int64_t r = lo + w.ty;
+      for (; r + (int64_t)(KR - 1) * s.TY < hi; r += (int64_t)KR * s.TY) chunk(r, KR, std::true_type());
+      if (r < hi) chunk(r, (int)((hi - r + s.TY - 1) / s.TY), std::false_type());
+    }
+    __syncthreads();  // sg, sa, sb are free again
+  }
+  if (rest) zero_rest<T, VN>(s, w, y);
+}
+
+// ------------------------------------------------------------------------------- backward
+// dh and xh of one value.
+__device__ __forceinline__ void grad_one(float x, float dy, float mean, float rstd, float gamma,
+                                         float beta, int silu, float* dh, float* xh) {
+  *xh = (x - mean) * rstd;
+  if (silu) {
+    const float h = fmaf(*xh, gamma, beta);
+    const float sg = __builtin_amdgcn_rcpf(1.f + __expf(-h));
+    dy *= sg * fmaf(h, 1.f - sg, 1.f);
+  }
+  *dh = dy;
+}
+
+// The thread's per-channel constants of sample b.
+template <typename T, int VN>
+__device__ __forceinline__ void channel_consts(const GnShape& s, int b, int c0, const float* stats,
+                                               const T* gamma, const T* beta, float (&mean)[VN],
+                                               float (&rstd)[VN], float (&ga)[VN], float (&be)[VN]) {
+#pragma unroll
+  for (int e = 0; e < VN; ++e) {
+    const float2 m = *(const float2*)(stats + 2 * ((int64_t)b * s.groups + (c0 + e) / s.cpg));
+    mean[e] = m.x;
+    rstd[e] = m.y;
+    ga[e] = gamma ? (float)gamma[c0 + e] : 1.f;
+    be[e] = beta ? (float)beta[c0 + e] : 0.f;
+  }
+}
+
+// Sums over a tile's rows of one sample: pc[slot * C + channel] = (sum dh, sum dh xh), and
+// pg[slot * NG + granule] the same weighted with gamma and summed over the granule.
+template <typename T, int VN>
+__global__ void __launch_bounds__(kNT)
+    gn_grad_sums_kernel(GnShape s, const T* __restrict__ dy, const T* __restrict__ x,
+                        const float* __restrict__ stats, const T* __restrict__ gamma,
+                        const T* __restrict__ beta, int32_t silu, float2* __restrict__ pc,
+                        float2* __restrict__ pg) {
+  constexpr int KR = 4;
+  __shared__ float s1[kNT * VN], s2[kNT * VN];
+  const Where w = where<VN>(s, blockIdx.x, blockIdx.y);
+  const int tid = threadIdx.x, SC = s.TX * VN;
+  const int g0 = w.slab * SC / s.gran, ng = min(SC / s.gran, s.NG - g0);
+  const int ch0 = w.slab * SC, nch = min(SC, s.C - ch0);
+  for (int b = w.b0; b <= w.b1; ++b) {
+    int64_t lo, hi;
+    gn_segment(s, b, &lo, &hi);
+    lo = max(lo, w.r0);
+    hi = min(hi, w.r1);
+    float2* dc = pc + (int64_t)(w.t + b) * s.C + ch0;
+    float2* dg = pg + (int64_t)(w.t + b) * s.NG + g0;
+    if (hi <= lo) {
+      for (int i = tid; i < nch; i += kNT) dc[i] = make_float2(0.f, 0.f);
+      for (int i = tid; i < ng; i += kNT) dg[i] = make_float2(0.f, 0.f);
+      continue;
+    }
+    float a1[VN], a2[VN];
+#pragma unroll
+    for (int e = 0; e < VN; ++e) a1[e] = a2[e] = 0.f;
+    if (w.live) {
+      float mean[VN], rstd[VN], ga[VN], be[VN];
+      channel_consts<T, VN>(s, b, w.c0, stats, gamma, beta, mean, rstd, ga, be);
+      auto chunk = [&](int64_t r, int k, auto whole) {
+        Pack<T, VN> vx[KR], vy[KR];
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (decltype(whole)::value || i < k) {
+            const int64_t at = (r + (int64_t)i * s.TY) * s.C + w.c0;
+            vx[i] = *(const Pack<T, VN>*)(x + at);
+            vy[i] = *(const Pack<T, VN>*)(dy + at);
+          }
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (decltype(whole)::value || i < k)
+#pragma unroll
+            for (int e = 0; e < VN; ++e) {
+              float dh, xh;
+              grad_one((float)vx[i].v[e], (float)vy[i].v[e], mean[e], rstd[e], ga[e], be[e], silu,
+                       &dh, &xh);
+              a1[e] += dh;
+              a2[e] = fmaf(dh, xh, a2[e]);
+            }
+      };
+      int64_t r = lo + w.ty;
+      for (; r + (int64_t)(KR - 1) * s.TY < hi; r += (int64_t)KR * s.TY) chunk(r, KR, std::true_type());
+      if (r < hi) chunk(r, (int)((hi - r + s.TY - 1) / s.TY), std::false_type());
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < VN; ++e) {
+      s1[tid * VN + e] = a1[e];
+      s2[tid * VN + e] = a2[e];
+    }
+    __syncthreads();
+    int half = 1;
+    while (2 * half < s.TY) half *= 2;
+    for (; half > 0 && s.TY > 1; half >>= 1) {
+      if (w.ty < half && w.ty + half < s.TY) {
+        const int o = tid + half * s.TX;
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+          a1[e] += s1[o * VN + e];
+          a2[e] += s2[o * VN + e];
+          s1[tid * VN + e] = a1[e];
+          s2[tid * VN + e] = a2[e];
+        }
+      }
+      __syncthreads();
+    }
+    for (int i = tid; i < nch; i += kNT) dc[i] = make_float2(s1[i], s2[i]);
+    for (int i = tid; i < ng; i += kNT) {
+      float u = 0.f, v = 0.f;
+      for (int c = i * s.gran; c < (i + 1) * s.gran; ++c) {
+        const float g = gamma ? (float)gamma[ch0 + c] : 1.f;
+        u = fmaf(g, s1[c], u);
+        v = fmaf(g, s2[c], v);
+      }
+      dg[i] = make_float2(u, v);
+    }
+  }
+}
+
+// dx; the first pblocks blocks add up dgamma and dbeta instead, 8 channels each.
+template <typename T, int VN>
+__global__ void __launch_bounds__(kNT)
+    gn_grad_kernel(GnShape s, const T* dy, const T* x, const float* __restrict__ stats,
+                   const T* __restrict__ gamma, const T* __restrict__ beta, int32_t silu,
+                   int32_t rest, int32_t pblocks, const float2* __restrict__ pc,
+                   const float2* __restrict__ pg, T* dx, T* dgamma, T* dbeta) {
+  constexpr int KR = 2;
+  __shared__ double sa[kNT], sb[kNT];
+  __shared__ float2 sg[kMaxGroups];
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x < pblocks) {
+    const int e = tid % kParamCh, j = tid / kParamCh, c = blockIdx.x * kParamCh + e;
+    double u = 0., v = 0.;
+    if (c < s.C)
+      for (int i = j; i < s.T + s.B - 1; i += kNT / kParamCh) {
+        const float2 p = pc[(int64_t)i * s.C + c];
+        u += (double)p.x;
+        v += (double)p.y;
+      }
+    sa[tid] = u;
+    sb[tid] = v;
+    __syncthreads();
+    for (int half = kNT / 2; half >= kParamCh; half >>= 1) {
+      if (tid < half) {
+        sa[tid] += sa[tid + half];
+        sb[tid] += sb[tid + half];
+      }
+      __syncthreads();
+    }
+    if (tid < kParamCh && c < s.C) {
+      if (dbeta) dbeta[c] = (T)(float)sa[tid];
+      if (dgamma) dgamma[c] = (T)(float)sb[tid];
+    }
+    return;
+  }
+  const int at = blockIdx.x - pblocks;
+  const Where w = where<VN>(s, at % s.T, at / s.T);
+  const int SC = s.TX * VN;
+  const int gl = w.slab * SC / s.cpg, gh = (min((w.slab + 1) * SC, s.C) - 1) / s.cpg;
+  const int ng = gh - gl + 1, P = lanes_per_group(ng);
+  for (int b = w.b0; b <= w.b1; ++b) {
+    int64_t lo, hi;
+    gn_segment(s, b, &lo, &hi);
+    const int64_t beg = lo, end = hi;
+    lo = max(lo, w.r0);
+    hi = min(hi, w.r1);
+    if (hi <= lo) continue;
+    {
+      const int t0 = (int)(beg / s.R), nt = (int)((end - 1) / s.R) - t0 + 1;
+      const int g = gl + tid / P, j = tid & (P - 1);
+      double u = 0., v = 0.;
+      if (g <= gh) {
+        const float2* src = pg + (int64_t)(t0 + b) * s.NG + (int64_t)g * s.GP;
+        for (int k = 0; k < s.GP; ++k)
+          for (int i = j; i < nt; i += P) {
+            const float2 p = src[(int64_t)i * s.NG + k];
+            u += (double)p.x;
+            v += (double)p.y;
+          }
+      }
+      run_sum(sa, sb, P, &u, &v);
+      if (g <= gh && j == 0) {
+        const double n = (double)(end - beg) * s.cpg;
+        sg[g - gl] = make_float2((float)(u / n), (float)(v / n));
+      }
+      __syncthreads();
+    }
+    if (w.live) {
+      float mean[VN], rstd[VN], ga[VN], be[VN], ma[VN], mb[VN];
+      channel_consts<T, VN>(s, b, w.c0, stats, gamma, beta, mean, rstd, ga, be);
+#pragma unroll
+      for (int e = 0; e < VN; ++e) {
+        const float2 m = sg[(w.c0 + e) / s.cpg - gl];
+        ma[e] = m.x;
+        mb[e] = m.y;
+      }
+      auto chunk = [&](int64_t r, int k, auto whole) {
+        Pack<T, VN> vx[KR], vy[KR];
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (decltype(whole)::value || i < k) {
+            const int64_t at = (r + (int64_t)i * s.TY) * s.C + w.c0;
+            vx[i] = *(const Pack<T, VN>*)(x + at);
+            vy[i] = *(const Pack<T, VN>*)(dy + at);
+          }
+#pragma unroll
+        for (int i = 0; i < KR; ++i)
+          if (decltype(whole)::value || i < k) {
+            float o[VN];
+#pragma unroll
+            for (int e = 0; e < VN; ++e) {
+              float dh, xh;
+              grad_one((float)vx[i].v[e], (float)vy[i].v[e], mean[e], rstd[e], ga[e], be[e], silu,
+                       &dh, &xh);
+              o[e] = rstd[e] * (fmaf(ga[e], dh, -ma[e]) - xh * mb[e]);
+            }
+            store_nt<T, VN>(dx + (r + (int64_t)i * s.TY) * s.C + w.c0, o);
+          }
+      };
+      int64_t r = lo + w.ty;
+      for (; r + (int64_t)(KR - 1) * s.TY < hi; r += (int64_t)KR * s.TY) chunk(r, KR, std::true_type());
+      if (r < hi) chunk(r, (int)((hi - r + s.TY - 1) / s.TY), std::false_type());
+    }
+    __syncthreads();
+  }
+  if (rest) zero_rest<T, VN>(s, w, dx);
+}
+
+// ------------------------------------------------------------------------------- host
+int gcd(int a, int b) {
+  while (b) {
+    const int r = a % b;
+    a = b;
+    b = r;
+  }
+  return a;
+}
+
+constexpr int kTargetBlocks = 1024;  // 4 blocks of 256 threads per CU
+
+GnShape gn_shape(const int32_t* cu, int32_t B, int64_t N, int32_t C, int32_t groups, int vn) {
+  GnShape s;
+  s.cu = cu;
+  s.N = N;
+  s.B = B;
+  s.C = C;
+  s.groups = groups;
+  s.cpg = C / groups;
+  s.nvec = C / vn;
+  s.slabs = (s.nvec + kMaxVec - 1) / kMaxVec;
+  s.TX = (s.nvec + s.slabs - 1) / s.slabs;
+  s.slabs = (s.nvec + s.TX - 1) / s.TX;
+  s.TY = kNT / s.TX;
+  const int64_t most = std::max<int64_t>(1, kTargetBlocks / s.slabs);
+  const int64_t want = (N + (int64_t)s.TY * 8 - 1) / ((int64_t)s.TY * 8);
+  s.T = (int32_t)std::max<int64_t>(1, std::min(most, want));
+  s.R = std::max<int64_t>(1, (N + s.T - 1) / s.T);
+  s.T = (int32_t)std::max<int64_t>(1, (N + s.R - 1) / s.R);
+  s.gran = gcd(s.cpg, s.TX * vn);
+  s.NG = C / s.gran;
+  s.GP = s.cpg / s.gran;
+  return s;
+}
+
+// Elements per load: 16 bytes where the rows and every buffer allow it, else 8, else one element.
+int vec_elems(int es, int32_t C, std::initializer_list<const void*> bufs) {
+  for (int bytes = 16; bytes >= 8; bytes /= 2) {
+    bool ok = ((int64_t)C * es) % bytes == 0;
+    for (const void* p : bufs) ok = ok && ((uintptr_t)p % bytes) == 0;
+    if (ok) return bytes / es;
+  }
+  return 1;
+}
+
+// f(T value, integral_constant VN) for the runtime type and vector length.
+template <typename F>
+void by_type(int32_t dtype, int vn, F f) {
+  constexpr std::integral_constant<int, 8> I8{};
+  constexpr std::integral_constant<int, 4> I4{};
+  constexpr std::integral_constant<int, 2> I2{};
+  constexpr std::integral_constant<int, 1> I1{};
+  if (dtype == TSC_F32) {
+    if (vn == 4) f(float(), I4);
+    else if (vn == 2) f(float(), I2);
+    else f(float(), I1);
+  } else if (dtype == TSC_F16) {
+    if (vn == 8) f(_Float16(), I8);
+    else if (vn == 4) f(_Float16(), I4);
+    else f(_Float16(), I1);
+  } else {
+    if (vn == 8) f(__bf16(), I8);
+    else if (vn == 4) f(__bf16(), I4);
+    else f(__bf16(), I1);
+  }
+}
+
+}  // namespace
+
+int64_t groupnorm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C, int32_t groups,
+                                  int32_t backward) {
+  // the buffers' alignment decides the vector length only at the call: the largest of the lengths
+  const int es = dtype == TSC_F32 ? 4 : 2;
+  int64_t most = 0;
+  for (int vn : {16 / es, 8 / es, 1}) {
+    if (C % vn) continue;
+    const GnShape s = gn_shape(nullptr, B, N, C, groups, vn);
+    const int64_t slots = (int64_t)s.T + B;
+    most = std::max(most, slots * 8 * ((int64_t)s.NG + (backward ? C : 0)));
+  }
+  return most;
+}
+
+int groupnorm_launch(tsc_ctx* ctx, int32_t dtype, const void* x, const int32_t* cu, int32_t B,
+                     int64_t N, int32_t C, int32_t groups, const void* gamma, const void* beta,
+                     float eps, int32_t silu, int32_t rest, float* stats, void* ws, void* y) {
+  const int es = dtype == TSC_F32 ? 4 : 2;
+  const int vn = vec_elems(es, C, {x, y});
+  const GnShape s = gn_shape(cu, B, N, C, groups, vn);
+  const dim3 grid((unsigned)s.T, (unsigned)s.slabs);
+  by_type(dtype, vn, [&](auto t, auto v) {
+    using T = decltype(t);
+    constexpr int VN = decltype(v)::value;
+    {
+      ProfScope p(ctx, "groupnorm_stats");
+      gn_stats_kernel<T, VN><<<grid, kNT, 0, ctx->stream>>>(s, (const T*)x, (float2*)ws);
+    }
+    ProfScope p(ctx, silu ? "groupnorm_silu" : "groupnorm");
+    gn_apply_kernel<T, VN><<<grid, kNT, 0, ctx->stream>>>(
+        s, (const T*)x, (const float2*)ws, (const T*)gamma, (const T*)beta, eps, silu, rest,
+        stats, (T*)y);
+  });
+  return check_hip(hipGetLastError(), "groupnorm launch");
+}
+
+int groupnorm_backward_launch(tsc_ctx* ctx, int32_t dtype, const void* dy, const void* x,
+                              const int32_t* cu, int32_t B, int64_t N, int32_t C, int32_t groups,
+                              const void* gamma, const void* beta, int32_t silu, int32_t rest,
+                              const float* stats, void* ws, void* dx, void* dgamma, void* dbeta) {
+  const int es = dtype == TSC_F32 ? 4 : 2;
+  const int vn = vec_elems(es, C, {x, dy, dx});
+  const GnShape s = gn_shape(cu, B, N, C, groups, vn);
+  const int pblocks = dgamma || dbeta ? (C + kParamCh - 1) / kParamCh : 0;
+  float2* pc = (float2*)ws;
+  float2* pg = pc + ((int64_t)s.T + B) * C;
+  by_type(dtype, vn, [&](auto t, auto v) {
+    using T = decltype(t);
+    constexpr int VN = decltype(v)::value;
+    {
+      ProfScope p(ctx, "groupnorm_grad_sums");
+      gn_grad_sums_kernel<T, VN><<<dim3((unsigned)s.T, (unsigned)s.slabs), kNT, 0, ctx->stream>>>(
+          s, (const T*)dy, (const T*)x, stats, (const T*)gamma, (const T*)beta, silu, pc, pg);
+    }
+    ProfScope p(ctx, "groupnorm_grad");
+    gn_grad_kernel<T, VN>
+        <<<(unsigned)(s.T * s.slabs + pblocks), kNT, 0, ctx->stream>>>(
+            s, (const T*)dy, (const T*)x, stats, (const T*)gamma, (const T*)beta, silu, rest,
+            pblocks, pc, pg, (T*)dx, (T*)dgamma, (T*)dbeta);
+  });
+  return check_hip(hipGetLastError(), "groupnorm backward launch");
+}
+
+}  // namespace tsc

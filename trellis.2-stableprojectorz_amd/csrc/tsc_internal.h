@@ -230,6 +230,17 @@ int attention_launch(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, 
                      int64_t total_kv, int32_t H, int32_t D, float scale, int32_t max_seqlen_q,
                      void* out);
 
+// ---- implemented in groupnorm.hip ----
+int64_t groupnorm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C, int32_t groups,
+                                  int32_t backward);
+int groupnorm_launch(tsc_ctx* ctx, int32_t dtype, const void* x, const int32_t* cu, int32_t B,
+                     int64_t N, int32_t C, int32_t groups, const void* gamma, const void* beta,
+                     float eps, int32_t silu, int32_t rest, float* stats, void* ws, void* y);
+int groupnorm_backward_launch(tsc_ctx* ctx, int32_t dtype, const void* dy, const void* x,
+                              const int32_t* cu, int32_t B, int64_t N, int32_t C, int32_t groups,
+                              const void* gamma, const void* beta, int32_t silu, int32_t rest,
+                              const float* stats, void* ws, void* dx, void* dgamma, void* dbeta);
+
 // ---- launchers implemented in rowops.hip ----
 int layernorm_launch(tsc_ctx* ctx, int32_t dtype, const void* x, int64_t N, int32_t C,
                      const void* gamma, const void* beta, float eps, int32_t apply_silu, void* y);

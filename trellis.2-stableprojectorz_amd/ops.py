@@ -253,6 +253,90 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-6, silu:
     return out
 
 
+def _scratch(nbytes: int, dev) -> torch.Tensor:
+    """A call's workspace, from torch's allocator: it is stream-ordered, and a captured graph keeps
+    its own, so calls and graphs share none."""
+    return torch.empty((max(int(nbytes), 16),), dtype=torch.uint8, device=dev)
+
+
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, cu_rows=None,
+               eps: float = 1e-5, silu: bool = False, out=None) -> torch.Tensor:
+    """Group norm over the rows of each sample, channels last (fp32 statistics), optionally fused
+    with SiLU (tsc_groupnorm).
+
+    x (N, C): cu_rows (B+1,) gives the samples' row offsets (host sequence or tensor, as
+    sparse_attention's cu_seqlens; a device tensor is not read back); without it all rows are one
+    sample.  x (B, ..., C): every x[b] is a sample.  weight, bias (C,) in x's dtype.  out may be x.
+    Rows outside every sample are zero in a new result and left as they were in `out`.
+    Differentiable in x, weight and bias (then without `out`; a graph through the gradient itself is
+    not supported)."""
+    if x.dim() < 2:
+        raise TscError(_lib.TSC_ERR_INVALID, "group_norm: x must be (N, C) or (B, ..., C)")
+    c = x.shape[-1]
+    if num_groups <= 0 or c == 0 or c % num_groups:
+        raise TscError(_lib.TSC_ERR_INVALID, f"group_norm: {num_groups} groups do not divide C={c}")
+    for t in (weight, bias):
+        if t is not None and (t.shape != (c,) or t.dtype != x.dtype):
+            raise TscError(_lib.TSC_ERR_INVALID, "group_norm: weight and bias must be (C,) of x's dtype")
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
+        raise TscError(_lib.TSC_ERR_INVALID, "group_norm: out has the wrong shape or dtype")
+    _code(x)
+    dev = _dev(x, weight, bias, out)
+    cu, b = None, 1
+    if x.dim() > 2:
+        if cu_rows is not None:
+            raise TscError(_lib.TSC_ERR_INVALID, "group_norm: cu_rows goes with (N, C) rows")
+        b = x.shape[0]
+    elif cu_rows is not None:
+        _, cu = _cu_seqlens(cu_rows, x.shape[0], dev, "cu_rows")
+        _dev(x, cu)
+        b = cu.numel() - 1
+    if _wants_grad(x, weight, bias):
+        if out is not None:
+            raise TscError(_lib.TSC_ERR_INVALID, "group_norm: out cannot be given where gradients are wanted")
+        from .autograd import GroupNorm
+
+        return GroupNorm.apply(x, weight, bias, cu, b, int(num_groups), float(eps), bool(silu))
+    return _group_norm(x, weight, bias, cu, b, int(num_groups), float(eps), bool(silu), out, None)
+
+
+def _group_norm(x, weight, bias, cu, b, groups, eps, silu, out, stats):
+    c = x.shape[-1]
+    n = x.numel() // c
+    rest = out is None
+    if out is None:
+        out = torch.empty_like(x) if b else torch.zeros_like(x)
+    if n == 0 or b == 0:
+        return out
+    lib, handle = _lib.stream_handle(x.device.index)
+    nbytes = lib.tsc_groupnorm_workspace_bytes(_code(x), b, n, c, groups, 0)
+    ws = _scratch(nbytes, x.device)
+    check(lib.tsc_groupnorm(handle, _code(x), _p(x), _p(cu), b, n, c, groups, _p(weight),
+                                _p(bias), eps, int(silu), int(rest), _p(stats), _p(ws), _p(out)))
+    return out
+
+
+def _group_norm_backward(dy, x, weight, bias, cu, b, groups, silu, stats, want_params):
+    c = x.shape[-1]
+    n = x.numel() // c
+    dx = torch.empty_like(x)
+    dw = torch.empty_like(weight) if want_params and weight is not None else None
+    db = torch.empty_like(bias) if want_params and bias is not None else None
+    if n == 0 or b == 0:
+        return tuple(None if t is None else t.zero_() for t in (dx, dw, db))
+    lib, handle = _lib.stream_handle(x.device.index)
+    nbytes = lib.tsc_groupnorm_workspace_bytes(_code(x), b, n, c, groups, 1)
+    ws = _scratch(nbytes, x.device)
+    check(lib.tsc_groupnorm_backward(handle, _code(x), _p(dy), _p(x), _p(cu), b, n, c,
+                                         groups, _p(weight), _p(bias), int(silu), 1, _p(stats),
+                                         _p(ws), _p(dx), _p(dw), _p(db)))
+    return dx, dw, db
+
+
 def silu(x: torch.Tensor, out=None) -> torch.Tensor:
     dev = _dev(x, out)
     if out is None:

@@ -61,7 +61,7 @@ class SparseTensor:
 
     def __init__(self, feats: torch.Tensor, coords: torch.Tensor, shape=None,
                  scale: Scale | None = None, cache: dict | None = None, layout=None,
-                 spatial_shape=None, batch_size: int | None = None):
+                 spatial_shape=None, batch_size: int | None = None, cu_rows=None):
         if coords.dim() != 2 or coords.shape[1] != 4:
             raise ValueError("coords must be (N,4) [batch,x,y,z]")
         if feats.shape[0] != coords.shape[0]:
@@ -72,6 +72,7 @@ class SparseTensor:
         self._scale = scale or SCALE_IDENTITY
         self._spatial_cache = cache if cache is not None else {}
         self._layout = layout
+        self._cu_rows = cu_rows
         self._batch_size = int(batch_size) if batch_size is not None else None
         if spatial_shape is not None:
             self.register_spatial_cache("shape", [int(v) for v in spatial_shape])
@@ -91,6 +92,15 @@ class SparseTensor:
         if self._layout is None:
             self._layout = compute_layout(self.coords)
         return self._layout
+
+    @property
+    def cu_rows(self) -> torch.Tensor:
+        """Row offsets of the samples, int32 (batch + 1) beside feats: `layout` as group_norm and
+        sparse_attention take it, copied to the device on first use."""
+        if self._cu_rows is None or self._cu_rows.device != self.feats.device:
+            offsets = [0] + [stop for _, stop in self.layout]
+            self._cu_rows = torch.tensor(offsets, dtype=torch.int32, device=self.feats.device)
+        return self._cu_rows
 
     @property
     def batch_size(self) -> int:
@@ -139,7 +149,7 @@ class SparseTensor:
         layout, as the reference's replace (sparse_tensor.ts:112-121)."""
         return SparseTensor(feats, self.coords if coords is None else coords, self._shape,
                             self._scale, self._spatial_cache, self._layout,
-                            batch_size=self._batch_size)
+                            batch_size=self._batch_size, cu_rows=self._cu_rows)
 
     def to(self, device) -> "SparseTensor":
         return SparseTensor(self.feats.to(device), self.coords.to(device), self._shape,
