@@ -322,6 +322,49 @@ int tsc_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, con
                   int64_t total_q, int64_t total_kv, int32_t num_heads, int32_t head_dim,
                   float scale, int32_t max_seqlen_q, void* out);
 
+/* ---- differential attention ---------------------------------------------------------------- */
+/* The difference of two softmax maps over packed sequences, each over half of a head's dimensions:
+ *   q = [q1 | q2], k = [k1 | k2] per head, P_i = softmax_m(q_i[n,h,:] . k_i[m,h,:] * scale)
+ *   out[n,h,:] = sum_m (P1[n,m] - lambda[h] P2[n,m]) v[m,h,:]
+ * for the sequences of tsc_attention, whose tensors these are: q, out (total_q, num_heads, head_dim),
+ * k, v (total_kv, num_heads, head_dim), head_dim 64 or 128 (maps of 32 or 64 dimensions).
+ *   ld_q, ld_k, ld_v  row strides in elements, num_heads * head_dim or more, rows 16-byte aligned (so
+ *     q, k and v may be slices of one fused projection); all other buffers are contiguous
+ *   lambda     device fp32 (num_heads)
+ *   cu_seqlens_q / cu_seqlens_kv, scale, max_seqlen_q  as in tsc_attention, scale <= 0 meaning
+ *     1/sqrt(head_dim / 2).  A sequence without keys gives zeros.
+ *   zero_rest  rows of out (and out2) outside every sequence: 0 = left as they were, 1 = zeroed
+ *   out2, lse  both NULL, or for the backward pass: out2 (total_q, num_heads, head_dim) `dtype` holds
+ *     P2 v, lse fp32 (2, num_heads, total_q) the maps' log2-sum-exps
+ *   workspace  device scratch of tsc_diff_attention_workspace_bytes(..., backward = 0) bytes (few
+ *     queries on many keys are shared out over blocks and joined), 16-byte aligned, NULL if that is
+ *     0.  The context keeps nothing, so calls with scratch of their own may overlap and be captured.
+ * fp32 softmax and accumulation; P is rounded to `dtype` for its product with v.
+ * No counterpart in the reference, whose attention is one map (src/sparse/ops/attention.ts:24-79). */
+int64_t tsc_diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q,
+                                           int64_t total_kv, int32_t num_heads, int32_t head_dim,
+                                           int32_t max_seqlen_q, int32_t backward);
+int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, const void* v,
+                       int64_t ld_q, int64_t ld_k, int64_t ld_v, const float* lambda,
+                       const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv, int32_t B,
+                       int64_t total_q, int64_t total_kv, int32_t num_heads, int32_t head_dim,
+                       float scale, int32_t max_seqlen_q, int32_t zero_rest, void* workspace,
+                       void* out, void* out2, float* lse);
+/* Its gradient from dout (total_q, num_heads, head_dim) and what the forward call was given and
+ * wrote: dq (total_q, ...), dk and dv (total_kv, num_heads, head_dim) `dtype`, dlambda fp32
+ * (num_heads) or NULL.  max_seqlen_kv sizes a grid as max_seqlen_q does; zero_rest is about rows of
+ * dq, dk and dv.  workspace with backward = 1.  The gradients must not overlap an input.  The sums
+ * have one fixed order. */
+int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k,
+                                const void* v, int64_t ld_q, int64_t ld_k, int64_t ld_v,
+                                const float* lambda, const int32_t* cu_seqlens_q,
+                                const int32_t* cu_seqlens_kv, int32_t B, int64_t total_q,
+                                int64_t total_kv, int32_t num_heads, int32_t head_dim, float scale,
+                                int32_t max_seqlen_q, int32_t max_seqlen_kv, int32_t zero_rest,
+                                const void* out, const void* out2, const float* lse,
+                                const void* dout, void* workspace, void* dq, void* dk, void* dv,
+                                float* dlambda);
+
 /* ---- safetensors weight files -------------------------------------------------------------- */
 /* Element types of a safetensors header ("dtype" strings).  F32/F16/BF16 equal TSC_F32/F16/BF16. */
 enum tsc_st_dtype {

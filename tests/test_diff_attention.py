@@ -1,0 +1,59 @@
+"""Refusals of sparse_diff_attention that need no GPU: arguments are checked before any device call."""
+import ctypes
+
+import pytest
+import torch
+
+
+def _t(n, h=2, d=64, dtype=torch.float32):
+    return torch.zeros((n, h, d), dtype=dtype)
+
+
+def test_refusals(pkg):
+    f, q, lam = pkg.sparse_diff_attention, _t(10), torch.zeros(2)
+    with pytest.raises(pkg.TscError, match=r"\(total, H, D\)"):
+        f(q.view(10, 128), q, q, lam, [0, 10])
+    with pytest.raises(pkg.TscError, match=r"\(total, H, D\)"):
+        f(q, _t(7), _t(8), lam, [0, 10], [0, 7])
+    with pytest.raises(pkg.TscError, match=r"\(total, H, D\)"):
+        f(q, _t(10, 1), _t(10, 1), lam, [0, 10])
+    with pytest.raises(pkg.TscError, match="head_dim 96"):
+        f(_t(10, 2, 96), _t(10, 2, 96), _t(10, 2, 96), lam, [0, 10])
+    with pytest.raises(pkg.TscError, match="share a dtype"):
+        f(q, q.half(), q, lam, [0, 10])
+    with pytest.raises(pkg.TscError, match="unsupported dtype"):
+        f(q.double(), q.double(), q.double(), lam, [0, 10])
+    for bad in (torch.zeros(3), torch.zeros((1, 2)), torch.zeros(2, dtype=torch.float16)):
+        with pytest.raises(pkg.TscError, match="lam must be"):
+            f(q, q, q, bad, [0, 10])
+    for scale in (0.0, -1.0, float("nan")):
+        with pytest.raises(pkg.TscError, match="scale"):
+            f(q, q, q, lam, [0, 10], scale=scale)
+    with pytest.raises(pkg.TscError, match="out has the wrong"):
+        f(q, q, q, lam, [0, 10], out=_t(9))
+    with pytest.raises(pkg.TscError, match="contiguous"):
+        f(torch.zeros((10, 64, 2)).transpose(1, 2), q, q, lam, [0, 10])
+    with pytest.raises(pkg.TscError, match="contiguous"):
+        f(q, torch.zeros((1, 2, 64)).expand(10, 2, 64), q, lam, [0, 10])
+    with pytest.raises(pkg.TscError, match="not on a GPU"):
+        f(q, q, q, lam, [0, 10])
+
+
+def test_c_entry_points_without_a_gpu(pkg):
+    lib = pkg.load_library()
+    P = ctypes.c_void_p
+    ws = lib.tsc_diff_attention_workspace_bytes
+    assert ws(2, 1, 1, 40000, 12, 128, 1, 0) > 0  # one query: shared out over the keys
+    assert ws(2, 1, 20000, 20000, 12, 128, 20000, 0) == 0
+    assert ws(2, 1, 100, 100, 12, 128, 100, 1) >= 2 * 12 * 100 * 4
+    assert ws(2, 0, 0, 0, 12, 128, 0, 0) == 0
+    for bad in ((3, 1, 1, 1, 1, 64, 1, 0), (0, 1, 1, 1, 1, 32, 1, 0), (0, -1, 1, 1, 1, 64, 1, 0),
+                (0, 1, 2 ** 31, 1, 1, 64, 1, 0), (0, 1, 1, 1, 0, 64, 1, 0), (0, 1, 1, 1, 1, 64, -1, 0)):
+        assert ws(*bad) == -1 and lib.tsc_last_error(), bad
+    st = lib.tsc_diff_attention(None, 0, P(16), P(16), P(16), 64, 64, 64, P(16), P(16), P(16), 1, 1, 1,
+                                1, 64, 0.0, 1, 0, None, P(16), None, None)
+    assert st == 1 and b"null context" in lib.tsc_last_error()
+    st = lib.tsc_diff_attention_backward(None, 0, P(16), P(16), P(16), 64, 64, 64, P(16), P(16), P(16),
+                                         1, 1, 1, 1, 64, 0.0, 1, 1, 0, P(16), P(16), P(16), P(16),
+                                         P(16), P(16), P(16), P(16), None)
+    assert st == 1 and b"null context" in lib.tsc_last_error()

@@ -20,9 +20,10 @@ from .conv3d import SparseConv3d, SparseResBlock3d, get_neighbor_map, neighbor_c
 from .ops import (NeighborMap, build_neighbor_map, map_conv_order, map_gather_plan,  # noqa: F401
                   sparse_conv3d,
                   layer_norm, group_norm, silu, add, sparse_resblock, sparse_subdivide, subdivide_count,
-                  sparse_linear, sparse_attention, scaled_dot_product_attention)
+                  sparse_linear, sparse_attention, sparse_diff_attention,
+                  scaled_dot_product_attention)
 from .spatial import SparseSubdivide  # noqa: F401
-from .blocks import SparseLinear, SparseGroupNorm, SparseConvNeXtBlock3d  # noqa: F401
+from .blocks import SparseLinear, SparseGroupNorm, SparseDiffAttentionBlock3d, SparseConvNeXtBlock3d  # noqa: F401
 from .weights import SafetensorsFile, SafetensorsHeader, TensorEntry, MultiFileLoader  # noqa: F401
 from . import workloads  # noqa: F401
 
@@ -31,6 +32,7 @@ __all__ = [
     "build_neighbor_map", "map_conv_order", "map_gather_plan", "sparse_conv3d", "layer_norm", "group_norm",
     "silu", "add", "sparse_resblock",
     "sparse_subdivide", "subdivide_count", "SparseSubdivide", "sparse_linear", "SparseLinear", "SparseGroupNorm",
-    "SparseConvNeXtBlock3d", "sparse_attention", "scaled_dot_product_attention", "SafetensorsFile", "SafetensorsHeader", "TensorEntry", "MultiFileLoader",
+    "SparseConvNeXtBlock3d", "SparseDiffAttentionBlock3d", "sparse_attention",
+    "sparse_diff_attention", "scaled_dot_product_attention", "SafetensorsFile", "SafetensorsHeader", "TensorEntry", "MultiFileLoader",
     "get_neighbor_map", "neighbor_cache_key", "workloads",
 ]

@@ -28,3 +28,20 @@ class GroupNorm(torch.autograd.Function):
         dx, dw, db = ops._group_norm_backward(dy.contiguous(), x, weight, bias, cu, b, groups, silu,
                                               stats, any(ctx.needs_input_grad[1:3]))
         return dx, dw, db, None, None, None, None, None
+
+
+class DiffAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, cq, ck, b, scale, max_q, max_kv):
+        out, out2, lse = ops._diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, None, True)
+        ctx.save_for_backward(q, k, v, lam, out, out2, lse, cq, ck)
+        ctx.args = (b, scale, max_q, max_kv)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, lam, out, out2, lse, cq, ck = ctx.saved_tensors
+        grads = ops._diff_attention_backward(do.contiguous(), q, k, v, lam, out, out2, lse, cq, ck,
+                                             *ctx.args)
+        return (*grads, None, None, None, None, None, None)

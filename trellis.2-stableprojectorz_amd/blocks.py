@@ -49,6 +49,34 @@ class SparseGroupNorm:
     __call__ = forward
 
 
+class SparseDiffAttentionBlock3d:
+    """x + out(diff_attention(qkv(group_norm(x)))) over each sample's voxels: group norm, one linear
+    layer for q, k and v (read in place as row slices), differential attention, and the output layer
+    with the skip as its residual.  qkv weight (3 C, C), out weight (C, C), lam float32 (num_heads),
+    C = num_heads * 64 or 128."""
+
+    def __init__(self, num_heads: int, num_groups: int, norm_weight: torch.Tensor | None,
+                 norm_bias: torch.Tensor | None, qkv_weight: torch.Tensor,
+                 qkv_bias: torch.Tensor | None, lam: torch.Tensor, out_weight: torch.Tensor,
+                 out_bias: torch.Tensor | None, eps: float = 1e-5):
+        self.num_heads, self.lam = num_heads, lam
+        self.norm = SparseGroupNorm(num_groups, norm_weight, norm_bias, eps)
+        self.qkv = SparseLinear(qkv_weight, qkv_bias)
+        self.out = SparseLinear(out_weight, out_bias)
+
+    def forward(self, x: SparseTensor) -> SparseTensor:
+        n, c = x.feats.shape
+        cu = x.cu_rows
+        longest = max(stop - start for start, stop in x.layout)
+        qkv = self.qkv(self.norm(x)).feats.view(n, 3, self.num_heads, c // self.num_heads)
+        h = ops.sparse_diff_attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], self.lam, cu,
+                                      max_seqlen_q=longest, max_seqlen_kv=longest)
+        return x.replace(ops.sparse_linear(h.view(n, c), self.out.weight, self.out.bias,
+                                           residual=x.feats))
+
+    __call__ = forward
+
+
 class SparseConvNeXtBlock3d:
     def __init__(self, conv_weight: torch.Tensor, conv_bias: torch.Tensor | None,
                  linear0_weight: torch.Tensor, linear0_bias: torch.Tensor | None,

@@ -746,6 +746,138 @@ int tsc_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, con
                           max_seqlen_q, out);
 }
 
+static int diff_attention_args(tsc_ctx* ctx, const char* what, int32_t dtype, const void* q,
+                               const void* k, const void* v, int64_t ld_q, int64_t ld_k,
+                               int64_t ld_v, const float* lambda, const int32_t* cu_q,
+                               const int32_t* cu_kv, int32_t B, int64_t total_q, int64_t total_kv,
+                               int32_t H, int32_t D, float scale, int32_t max_q, int32_t max_kv,
+                               int32_t rest, DiffAttnArgs* x) {
+  const int es = elem_size(dtype);
+  if (!es) return fail(TSC_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
+  if (D != 64 && D != 128)
+    return fail(TSC_ERR_UNSUPPORTED, "%s: head_dim %d (64 and 128 are supported)", what, D);
+  if (B < 0 || H <= 0 || H > 65535 || B > 65535 || total_q < 0 || total_kv < 0 || max_q < 0 ||
+      max_kv < 0 || total_q > INT32_MAX || total_kv > INT32_MAX)
+    return fail(TSC_ERR_INVALID, "%s: bad sizes B=%d H=%d total_q=%lld total_kv=%lld", what, B, H,
+                (long long)total_q, (long long)total_kv);
+  *x = DiffAttnArgs{dtype, q, k, v, ld_q, ld_k, ld_v, lambda, cu_q, cu_kv, B, total_q, total_kv, H, D,
+                    scale > 0.f ? scale : 1.f / sqrtf((float)D / 2), max_q, max_kv, rest};
+  if (!ctx || B == 0) return TSC_OK;  // the sizes only
+  if (!lambda || !cu_q || !cu_kv || (total_q > 0 && !q) || (total_kv > 0 && (!k || !v)))
+    return fail(TSC_ERR_INVALID, "%s: null buffer", what);
+  const int64_t lds[3] = {ld_q, ld_k, ld_v};
+  const void* bufs[3] = {q, k, v};
+  for (int i = 0; i < 3; ++i) {
+    if (lds[i] < (int64_t)H * D || lds[i] > (1 << 28) || lds[i] * es % 16)
+      return fail(TSC_ERR_INVALID, "%s: row stride %lld of q, k or v (%d * %d or more, whole 16 bytes)",
+                  what, (long long)lds[i], H, D);
+    if (!aligned(bufs[i], 16))
+      return fail(TSC_ERR_INVALID, "%s: q, k and v must be 16-byte aligned", what);
+  }
+  if (!aligned(lambda, 4) || !aligned(cu_q, 4) || !aligned(cu_kv, 4))
+    return fail(TSC_ERR_INVALID, "%s: lambda and cu_seqlens must be 4-byte aligned", what);
+  return TSC_OK;
+}
+
+// Bytes that rows of stride ld reach over.
+static size_t row_span(int64_t rows, int64_t ld, const DiffAttnArgs& x) {
+  return rows > 0 ? ((size_t)(rows - 1) * ld + (size_t)x.H * x.D) * elem_size(x.dtype) : 0;
+}
+
+int64_t tsc_diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q,
+                                           int64_t total_kv, int32_t num_heads, int32_t head_dim,
+                                           int32_t max_seqlen_q, int32_t backward) {
+  g_err[0] = 0;
+  DiffAttnArgs x;
+  if (diff_attention_args(nullptr, "diff_attention_workspace_bytes", dtype, nullptr, nullptr, nullptr,
+                          0, 0, 0, nullptr, nullptr, nullptr, B, total_q, total_kv, num_heads,
+                          head_dim, 0.f, max_seqlen_q, 0, 0, &x))
+    return -1;
+  return diff_attention_workspace_bytes(B, total_q, total_kv, num_heads, head_dim, max_seqlen_q,
+                                        backward);
+}
+
+int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, const void* v,
+                       int64_t ld_q, int64_t ld_k, int64_t ld_v, const float* lambda,
+                       const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv, int32_t B,
+                       int64_t total_q, int64_t total_kv, int32_t num_heads, int32_t head_dim,
+                       float scale, int32_t max_seqlen_q, int32_t zero_rest, void* workspace,
+                       void* out, void* out2, float* lse) {
+  g_err[0] = 0;
+  int st = check_ctx(ctx);
+  if (st) return st;
+  DiffAttnArgs x;
+  st = diff_attention_args(ctx, "diff_attention", dtype, q, k, v, ld_q, ld_k, ld_v, lambda,
+                           cu_seqlens_q, cu_seqlens_kv, B, total_q, total_kv, num_heads, head_dim,
+                           scale, max_seqlen_q, 0, zero_rest, &x);
+  if (st) return st;
+  if (B == 0 || total_q == 0) return TSC_OK;
+  if (!out) return fail(TSC_ERR_INVALID, "diff_attention: null buffer");
+  if ((out2 == nullptr) != (lse == nullptr))
+    return fail(TSC_ERR_INVALID, "diff_attention: out2 and lse go together");
+  const int64_t need = diff_attention_workspace_bytes(B, total_q, total_kv, num_heads, head_dim,
+                                                      max_seqlen_q, 0);
+  if (need > 0 && !workspace) return fail(TSC_ERR_INVALID, "diff_attention: null workspace");
+  if (!aligned(out, 16) || !aligned(out2, 16) || !aligned(lse, 4) || !aligned(workspace, 16))
+    return fail(TSC_ERR_INVALID, "diff_attention: out, out2 and workspace must be 16-byte aligned");
+  const size_t no = row_span(total_q, (int64_t)num_heads * head_dim, x);
+  for (const void* o : {(const void*)out, (const void*)out2})
+    if (o && (overlaps(o, no, q, row_span(total_q, ld_q, x)) ||
+              overlaps(o, no, k, row_span(total_kv, ld_k, x)) ||
+              overlaps(o, no, v, row_span(total_kv, ld_v, x))))
+      return fail(TSC_ERR_INVALID, "diff_attention: out overlaps an input");
+  if (out2 && overlaps(out, no, out2, no))
+    return fail(TSC_ERR_INVALID, "diff_attention: out overlaps out2");
+  DeviceGuard g(ctx->device);
+  return diff_attention_launch(ctx, x, out, out2, lse, workspace);
+}
+
+int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k,
+                                const void* v, int64_t ld_q, int64_t ld_k, int64_t ld_v,
+                                const float* lambda, const int32_t* cu_seqlens_q,
+                                const int32_t* cu_seqlens_kv, int32_t B, int64_t total_q,
+                                int64_t total_kv, int32_t num_heads, int32_t head_dim, float scale,
+                                int32_t max_seqlen_q, int32_t max_seqlen_kv, int32_t zero_rest,
+                                const void* out, const void* out2, const float* lse,
+                                const void* dout, void* workspace, void* dq, void* dk, void* dv,
+                                float* dlambda) {
+  g_err[0] = 0;
+  int st = check_ctx(ctx);
+  if (st) return st;
+  DiffAttnArgs x;
+  st = diff_attention_args(ctx, "diff_attention_backward", dtype, q, k, v, ld_q, ld_k, ld_v, lambda,
+                           cu_seqlens_q, cu_seqlens_kv, B, total_q, total_kv, num_heads, head_dim,
+                           scale, max_seqlen_q, max_seqlen_kv, zero_rest, &x);
+  if (st) return st;
+  if (B == 0 || total_q == 0)
+    return fail(TSC_ERR_INVALID, "diff_attention_backward: no queries (the gradients are zero)");
+  if (!out || !out2 || !lse || !dout || !workspace || !dq || (total_kv > 0 && (!dk || !dv)))
+    return fail(TSC_ERR_INVALID, "diff_attention_backward: null buffer");
+  const void* a16[7] = {out, out2, dout, workspace, dq, dk, dv};
+  for (const void* p : a16)
+    if (!aligned(p, 16))
+      return fail(TSC_ERR_INVALID, "diff_attention_backward: buffers must be 16-byte aligned");
+  if (!aligned(lse, 4) || !aligned(dlambda, 4))
+    return fail(TSC_ERR_INVALID, "diff_attention_backward: lse and dlambda must be 4-byte aligned");
+  const int64_t ld = (int64_t)num_heads * head_dim;
+  const size_t no = row_span(total_q, ld, x), nk = row_span(total_kv, ld, x);
+  const void* ins[6] = {q, k, v, out, out2, dout};
+  const size_t in_bytes[6] = {row_span(total_q, ld_q, x), row_span(total_kv, ld_k, x),
+                              row_span(total_kv, ld_v, x), no, no, no};
+  const void* gs[3] = {dq, dk, dv};
+  const size_t g_bytes[3] = {no, nk, nk};
+  for (int i = 0; i < 3; ++i) {
+    for (int j = 0; j < 6; ++j)
+      if (overlaps(gs[i], g_bytes[i], ins[j], in_bytes[j]))
+        return fail(TSC_ERR_INVALID, "diff_attention_backward: a gradient overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (overlaps(gs[i], g_bytes[i], gs[j], g_bytes[j]))
+        return fail(TSC_ERR_INVALID, "diff_attention_backward: the gradients overlap");
+  }
+  DeviceGuard g(ctx->device);
+  return diff_attention_backward_launch(ctx, x, out, out2, lse, dout, workspace, dq, dk, dv, dlambda);
+}
+
 int tsc_st_open(const char* path, tsc_st** out) {
   g_err[0] = 0;
   if (!path || !out) return fail(TSC_ERR_INVALID, "st_open: null argument");

@@ -1,0 +1,773 @@
+// Differential attention over packed sequences, and its gradient: the difference of two softmax maps,
+// each over half of a head's dimensions.
+//
+//   q = [q1 | q2], k = [k1 | k2] per head (halves of D), z = scale
+//   P1 = softmax(q1 k1^T z), P2 = softmax(q2 k2^T z);   out = (P1 - lambda_h P2) v
+//   n in [cu_q[b], cu_q[b+1]), m in [cu_kv[b], cu_kv[b+1]);  no keys: zeros
+// Gradient, with do = d out, dP = do v^T, r_i = do . (P_i v) per query:
+//   dv = (P1 - lambda P2)^T do;  dS1 = P1 (dP - r1);  dS2 = -lambda P2 (dP - r2)
+//   dq_i = z dS_i k_i;  dk_i = z dS_i^T q_i;  dlambda_h = - sum over queries of r2
+//
+// The tensors are those of tsc_attention (rows of H heads of D = 64 or 128), so a fragment of k or q
+// feeds one map or the other by its dimensions, and one walk over the keys serves both.  The two
+// maps' weighted sums of v stay apart until their denominators are known (6 D flops a pair; the
+// difference itself would need 4 D, and two walks).  For the gradient the forward pass keeps
+// P2 v and the two log-sum-exps, and the probabilities are made again from them.
+//
+// Scores are computed in 32 x 32 tiles whose result layout (lane: one column, 16 rows 8(j/4) +
+// 4(lane/32) + j%4) is the operand layout of the next product, contracted over those rows: transposed
+// (keys x queries) where a wave owns queries (forward, dq), plain (queries x keys) where it owns keys
+// (dk, dv).  The other operand of that product is read transposed from the row-major tile in LDS.
+// All three types run the same code on fragments of 8 elements: one 32x32x16 product in 16 bits,
+// eight 32x32x2 products of the same elements in fp32.  P and dS are rounded to the input type for the
+// second products (as v and k are stored); softmax, sums and accumulators are fp32.
+// No atomics: dq and (dk, dv) come from two kernels, each owning its rows, which costs the scores and
+// dP twice (28 D instead of 20 D flops a pair) and keeps the bits of a result fixed.
+
+#include <float.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attention_common.h"
+#include "tsc_internal.h"
+
+namespace tsc {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ---- fragments: 8 elements of a lane --------------------------------------------------------
+struct F32x8 {
+  float v[8];
+};
+template <typename T>
+struct Frag {
+  typedef u32x4_t type;
+  static __device__ __forceinline__ void mma(const u32x4_t& a, const u32x4_t& b, f32x16_t& c) {
+    Mma<T>::run(a, b, c);
+  }
+  // Elements 8 g .. 8 g + 7 of a score tile.
+  static __device__ __forceinline__ u32x4_t pack(const float* s) {
+    u32x4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = Mma<T>::pack(s[2 * i], s[2 * i + 1]);
+    return r;
+  }
+  static __device__ __forceinline__ u32x4_t load(const T* p) { return *(const u32x4_t*)p; }
+};
+template <>
+struct Frag<float> {
+  typedef F32x8 type;
+  static __device__ __forceinline__ void mma(const F32x8& a, const F32x8& b, f32x16_t& c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[i], b.v[i], c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ F32x8 pack(const float* s) {
+    F32x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = s[i];
+    return r;
+  }
+  static __device__ __forceinline__ F32x8 load(const float* p) {
+    F32x8 r;
+    *(float4*)&r.v[0] = *(const float4*)p;
+    *(float4*)&r.v[4] = *(const float4*)(p + 4);
+    return r;
+  }
+};
+
+// ---- row-major tiles in LDS -----------------------------------------------------------------
+// 16 bits: 16-byte chunks XOR-swizzled by row, so that 16 rows of one chunk column (row fragments)
+// and 64 bytes of 4 consecutive rows (transposed reads) both fall into distinct banks.
+// fp32: rows padded by 4 floats.
+template <typename T, int D>
+struct Tile {
+  static constexpr int CPR = D / 8;  // 16-byte chunks of a row
+  static constexpr int ROWB = 2 * D;
+  static __device__ __forceinline__ int swz(int row) {
+    return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row & 2) << 1) | ((row >> 2) & 3);
+  }
+  static __device__ __forceinline__ void put(unsigned char* t, int row, int c, u32x4_t v) {
+    *(u32x4_t*)(t + row * ROWB + ((c ^ swz(row)) << 4)) = v;
+  }
+  // Dims 16 st + 8 hf .. + 7 of row l32 (r0 a multiple of 16).
+  static __device__ __forceinline__ u32x4_t row(const unsigned char* t, int r0, int l32, int hf, int st) {
+    const int r = r0 + l32;
+    return *(const u32x4_t*)(t + r * ROWB + (((2 * st + hf) ^ swz(r)) << 4));
+  }
+  // Column 32 mt + l32; rows r0 + 16 g + 8 (e / 4) + 4 hf + e % 4, e = 0 .. 7.
+  static __device__ __forceinline__ u32x4_t col(const unsigned char* t, int r0, int lane, int g, int mt) {
+    const int vr = 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int c = 4 * mt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    u32x4_t r;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int rr = r0 + 16 * g + 8 * x + vr;
+      const uint2 h = lds_read_tr(t + rr * ROWB + ((c ^ swz(rr)) << 4) + (lane & 1) * 8);
+      r[2 * x] = h.x;
+      r[2 * x + 1] = h.y;
+    }
+    return r;
+  }
+};
+template <int D>
+struct Tile<float, D> {
+  static constexpr int CPR = D / 4;
+  static constexpr int ROWB = 4 * (D + 4);
+  static __device__ __forceinline__ void put(unsigned char* t, int row, int c, u32x4_t v) {
+    *(u32x4_t*)(t + row * ROWB + 16 * c) = v;
+  }
+  static __device__ __forceinline__ F32x8 row(const unsigned char* t, int r0, int l32, int hf, int st) {
+    return Frag<float>::load((const float*)(t + (r0 + l32) * ROWB) + 16 * st + 8 * hf);
+  }
+  static __device__ __forceinline__ F32x8 col(const unsigned char* t, int r0, int lane, int g, int mt) {
+    F32x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      r.v[e] = ((const float*)(t + (r0 + 16 * g + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * ROWB))
+          [32 * mt + (lane & 31)];
+    return r;
+  }
+};
+
+// Rows on their way from global memory into a tile: ROWS rows by NT threads.
+template <typename T, int D, int ROWS, int NT>
+struct Stage {
+  typedef Tile<T, D> Ti;
+  static constexpr int NL = ROWS * Ti::CPR / NT;
+  static_assert(NL >= 1 && NL * NT == ROWS * Ti::CPR, "tile shape");
+  u32x4_t r[NL];
+  // Rows first .. first + ROWS - 1 of base (row stride ld elements); zeros from row `end` on.
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int first, int end) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int id = threadIdx.x + NT * i, row = first + id / Ti::CPR, c = id % Ti::CPR;
+      r[i] = u32x4_t{0, 0, 0, 0};
+      if (row < end) r[i] = *(const u32x4_t*)((const char*)(base + (int64_t)row * ld) + 16 * c);
+    }
+  }
+  __device__ __forceinline__ void store(unsigned char* t) const {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int id = threadIdx.x + NT * i;
+      Ti::put(t, id / Ti::CPR, id % Ti::CPR, r[i]);
+    }
+  }
+};
+
+__device__ __forceinline__ void clear(f32x16_t& c) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) c[j] = 0.f;
+}
+
+// Writes f times a transposed result (lane: one row; dims 8(j/4) + 4 hf + j%4 of each 32) to that row.
+template <typename T>
+__device__ __forceinline__ void store_dims(T* p, int hf, const f32x16_t& c, float f) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const float a = c[4 * g] * f, b = c[4 * g + 1] * f, d = c[4 * g + 2] * f, e = c[4 * g + 3] * f;
+    if constexpr (sizeof(T) == 4)
+      *(float4*)(p + 8 * g + 4 * hf) = make_float4(a, b, d, e);
+    else
+      *(uint2*)(p + 8 * g + 4 * hf) = make_uint2(Mma<T>::pack(a, b), Mma<T>::pack(d, e));
+  }
+}
+
+// Zeros in head h of the rows [r0, r1), shared by the gx blocks of index bx.
+template <typename T>
+__device__ __forceinline__ void zero_rows(T* p, int64_t r0, int64_t r1, int H, int D, int h, int bx,
+                                          int gx) {
+  const int per = D * (int)sizeof(T) / 16;
+  for (int64_t i = threadIdx.x + (int64_t)bx * blockDim.x; i < (r1 - r0) * per;
+       i += (int64_t)gx * blockDim.x)
+    *(uint4*)((char*)(p + ((r0 + i / per) * H + h) * D) + 16 * (i % per)) = make_uint4(0, 0, 0, 0);
+}
+// ... of the rows outside every sequence, by the blocks of the first and the last sequence.
+template <typename T>
+__device__ __forceinline__ void zero_rest(T* p, const int32_t* cu, int64_t total, int bb, int H, int D,
+                                          int h, int bx, int gx) {
+  int b0, n;
+  if (bb == 0) {
+    segment(cu, 0, total, &b0, &n);
+    zero_rows(p, 0, b0, H, D, h, bx, gx);
+  }
+  if (bb == (int)gridDim.z - 1) {
+    segment(cu, bb, total, &b0, &n);
+    zero_rows(p, b0 + n, total, H, D, h, bx, gx);
+  }
+}
+
+struct DaArgs {
+  const void *q, *k, *v;
+  int64_t ldq, ldk, ldv;
+  const float* lambda;
+  const int32_t *cu_q, *cu_kv;
+  int64_t total_q, total_kv;
+  int32_t H;
+  float sl2;     // scale * log2(e)
+  int32_t rest;  // zero the rows outside every sequence
+  // forward
+  void *out, *out2;  // out2 = P2 v, or null
+  float* lse;        // (2, H, total_q): log2 of the sum of 2^(score sl2), or null
+  int32_t splits;    // parts of the keys, each of its own block
+  float* part;       // splits > 1: (splits, total_q, H, 2, D) weighted sums, then
+                     // (splits, total_q, H, 2, 2) maxima (times sl2) and denominators
+  // backward
+  const void* dout;
+  const float* r12;  // (2, H, total_q)
+  const float* lam_part;
+  int32_t lam_parts;
+  void *dq, *dk, *dv;
+  float* dlambda;
+};
+
+// ------------------------------------------------------------------------------- forward
+constexpr int kNT = 256;  // 4 waves of 32 queries (or keys, in dk / dv)
+constexpr int kBQ = 128;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT) da_forward_kernel(const DaArgs a) {
+  typedef Frag<T> F;
+  typedef typename F::type Fr;
+  typedef Tile<T, D> Ti;
+  constexpr int BK = sizeof(T) == 2 ? 64 : 32;
+  constexpr int KS = D / 16, MT = D / 32;
+  __shared__ __attribute__((aligned(16))) unsigned char kt[BK * Ti::ROWB], vt[BK * Ti::ROWB];
+  int bx, h, bb;
+  block_tile(a.cu_kv, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l32 = lane & 31, hf = lane >> 5;
+  const int sp = bx % a.splits, tile = bx / a.splits, tiles = gridDim.x / a.splits;
+  if (a.rest && sp == 0) {
+    zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, tile, tiles);
+    if (a.out2) zero_rest((T*)a.out2, a.cu_q, a.total_q, bb, a.H, D, h, tile, tiles);
+  }
+  const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
+  const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
+  const int per = ((kv_len + a.splits - 1) / a.splits + BK - 1) / BK * BK;
+  const int k_lo = min((int64_t)per * sp, (int64_t)kv_len), k_hi = min(k_lo + per, kv_len);
+  const float lam = a.lambda[h];
+
+  for (int qt = tile * kBQ; qt < q_len; qt += tiles * kBQ) {
+    const int qi = qt + w * 32 + l32;
+    const int64_t qrow = q0 + min(qi, q_len - 1);
+    Fr qf[KS];
+    {
+      const T* p = (const T*)a.q + qrow * a.ldq + (int64_t)h * D + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) qf[st] = F::load(p + 16 * st);
+    }
+    float m[2], l[2];  // the maximum starts finite: a tile of scores of -inf then adds nothing
+    f32x16_t o[2][MT];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      m[i] = -FLT_MAX;
+      l[i] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) clear(o[i][mt]);
+    }
+    Stage<T, D, BK, kNT> ks, vs;
+    ks.load(kbase, a.ldk, k_lo, k_hi);
+    vs.load(vbase, a.ldv, k_lo, k_hi);
+    for (int kb = k_lo; kb < k_hi; kb += BK) {
+      __syncthreads();
+      ks.store(kt);
+      vs.store(vt);
+      __syncthreads();
+      ks.load(kbase, a.ldk, kb + BK, k_hi);
+      vs.load(vbase, a.ldv, kb + BK, k_hi);
+#pragma unroll
+      for (int sub = 0; sub < BK; sub += 32) {
+        const int k0 = kb + sub;
+        if (k0 >= k_hi) break;
+        Fr pf[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f32x16_t s;
+          clear(s);
+#pragma unroll
+          for (int st = i * KS / 2; st < (i + 1) * KS / 2; ++st) F::mma(Ti::row(kt, sub, l32, hf, st), qf[st], s);
+          float mx = -INFINITY, p[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (k0 + 8 * (j >> 2) + 4 * hf + (j & 3) >= k_hi) s[j] = -INFINITY;
+            mx = fmaxf(mx, s[j]);
+          }
+          mx = pair_max(mx) * a.sl2;
+          if (__builtin_amdgcn_ballot_w64(mx > m[i])) {
+            const float mn = fmaxf(m[i], mx), f = fast_exp2(m[i] - mn);
+            m[i] = mn;
+            l[i] *= f;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[i][mt][j] *= f;
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            p[j] = fast_exp2(fmaf(s[j], a.sl2, -m[i]));
+            l[i] += p[j];
+          }
+          pf[i][0] = F::pack(p);
+          pf[i][1] = F::pack(p + 8);
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const Fr vf = Ti::col(vt, sub, lane, g, mt);
+            F::mma(vf, pf[0][g], o[0][mt]);
+            F::mma(vf, pf[1][g], o[1][mt]);
+          }
+      }
+    }
+    l[0] = pair_sum(l[0]);
+    l[1] = pair_sum(l[1]);
+    if (qi < q_len) {
+      const int64_t at = (int64_t)(q0 + qi) * a.H + h;
+      if (a.splits > 1) {
+        const int64_t rows = a.total_q * a.H;
+        float* po = a.part + ((int64_t)sp * rows + at) * 2 * D;
+        float* ps = a.part + (int64_t)a.splits * rows * 2 * D + ((int64_t)sp * rows + at) * 4;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) store_dims(po + i * D + 32 * mt, hf, o[i][mt], 1.f);
+          if (hf == 0) *(float2*)(ps + 2 * i) = make_float2(m[i], l[i]);
+        }
+      } else {
+        const float i1 = kv_len ? 1.f / l[0] : 0.f, i2 = kv_len ? 1.f / l[1] : 0.f, f2 = lam * i2;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          if (a.out2) store_dims((T*)a.out2 + at * D + 32 * mt, hf, o[1][mt], i2);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[0][mt][j] = fmaf(-f2, o[1][mt][j], o[0][mt][j] * i1);
+          store_dims((T*)a.out + at * D + 32 * mt, hf, o[0][mt], 1.f);
+        }
+        if (a.lse && hf == 0) {
+          a.lse[(int64_t)h * a.total_q + q0 + qi] = kv_len ? m[0] + log2f(l[0]) : INFINITY;
+          a.lse[(int64_t)(a.H + h) * a.total_q + q0 + qi] = kv_len ? m[1] + log2f(l[1]) : INFINITY;
+        }
+      }
+    }
+  }
+}
+
+// Joins the parts of the keys: one wave for a (query, head), D / 64 dims a lane.
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT) da_join_kernel(const DaArgs a, int32_t B) {
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = a.total_q * a.H;
+  if (at >= rows) return;
+  const int lane = threadIdx.x & 63, h = (int)(at % a.H);
+  const int64_t row = at / a.H;
+  // The sequence of the row, and whether it has keys.
+  bool in = false, keys = false;
+  for (int b = lane; b < B; b += 64) {
+    int q0, ql, k0, kl;
+    segment(a.cu_q, b, a.total_q, &q0, &ql);
+    if (row >= q0 && row < (int64_t)q0 + ql) {
+      segment(a.cu_kv, b, a.total_kv, &k0, &kl);
+      in = true;
+      keys = kl > 0;
+    }
+  }
+  if (__builtin_amdgcn_ballot_w64(in) == 0) return;
+  keys = __builtin_amdgcn_ballot_w64(keys) != 0;
+  const float* ps = a.part + (int64_t)a.splits * rows * 2 * D;
+  float m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {0.f, 0.f};
+  float o[2][D / 64] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const float4 st = *(const float4*)(ps + ((int64_t)s * rows + at) * 4);
+    const float sm[2] = {st.x, st.z}, sl[2] = {st.y, st.w};
+    const float* po = a.part + ((int64_t)s * rows + at) * 2 * D;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (!(sl[i] != 0.f)) continue;  // a part without keys
+      const float mn = fmaxf(m[i], sm[i]);
+      const float f = fast_exp2(m[i] - mn), g = fast_exp2(sm[i] - mn);
+      m[i] = mn;
+      l[i] = l[i] * f + sl[i] * g;
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e)
+        o[i][e] = o[i][e] * f + po[i * D + lane + 64 * e] * g;
+    }
+  }
+  const float i1 = keys ? 1.f / l[0] : 0.f, i2 = keys ? 1.f / l[1] : 0.f, lam = a.lambda[h];
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) {
+    const int64_t p = at * D + lane + 64 * e;
+    ((T*)a.out)[p] = (T)(o[0][e] * i1 - lam * (o[1][e] * i2));
+    if (a.out2) ((T*)a.out2)[p] = (T)(o[1][e] * i2);
+  }
+  if (a.lse && lane == 0) {
+    a.lse[(int64_t)h * a.total_q + row] = keys ? m[0] + log2f(l[0]) : INFINITY;
+    a.lse[(int64_t)(a.H + h) * a.total_q + row] = keys ? m[1] + log2f(l[1]) : INFINITY;
+  }
+}
+
+// ------------------------------------------------------------------------------- backward
+// r_i = do . (P_i v) per query, P1 v = out + lambda P2 v; and per block the sum of r2 for dlambda.
+// Block: one head, the rows of one sequence in steps of 256 / (D / 8) per grid column.
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r12, float* lam_part) {
+  constexpr int LPR = D / 8;  // lanes of a row, 8 elements each
+  constexpr int RPB = kNT / LPR;
+  __shared__ float sum[kNT / 64];
+  const int h = blockIdx.y, bb = blockIdx.z, e0 = threadIdx.x % LPR * 8;
+  int q0, q_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  const float lam = a.lambda[h];
+  float acc = 0.f;
+  for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR; r < q_len;
+       r += (int64_t)gridDim.x * RPB) {
+    const int64_t at = ((q0 + r) * a.H + h) * D + e0;
+    const T *d = (const T*)a.dout + at, *o = (const T*)a.out + at, *p = (const T*)a.out2 + at;
+    float r1 = 0.f, r2 = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; c += 16 / sizeof(T)) {
+      const u32x4_t wd = *(const u32x4_t*)(d + c), wo = *(const u32x4_t*)(o + c), wp = *(const u32x4_t*)(p + c);
+#pragma unroll
+      for (int e = 0; e < (int)(16 / sizeof(T)); ++e) {
+        const float x = (float)((const T*)&wd)[e], y = (float)((const T*)&wp)[e];
+        r1 = fmaf(x, (float)((const T*)&wo)[e], r1);
+        r2 = fmaf(x, y, r2);
+      }
+    }
+#pragma unroll
+    for (int off = LPR / 2; off > 0; off >>= 1) {
+      r1 += __shfl_xor(r1, off, 64);
+      r2 += __shfl_xor(r2, off, 64);
+    }
+    if (e0 == 0) {
+      r12[(int64_t)h * a.total_q + q0 + r] = fmaf(lam, r2, r1);
+      r12[(int64_t)(a.H + h) * a.total_q + q0 + r] = r2;
+      acc += r2;
+    }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
+  if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    lam_part[((int64_t)h * gridDim.z + bb) * gridDim.x + blockIdx.x] = sum[0] + sum[1] + sum[2] + sum[3];
+}
+
+// dq of 128 queries; one block of each head also adds up dlambda.
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
+  typedef Frag<T> F;
+  typedef typename F::type Fr;
+  typedef Tile<T, D> Ti;
+  constexpr int BK = 32;
+  constexpr int KS = D / 16, MT = D / 32;
+  __shared__ __attribute__((aligned(16))) unsigned char kt[BK * Ti::ROWB], vt[BK * Ti::ROWB];
+  int bx, h, bb;
+  block_tile(a.cu_kv, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l32 = lane & 31, hf = lane >> 5;
+  if (a.rest) zero_rest((T*)a.dq, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
+  if (bx == 0 && bb == 0 && w == 0 && a.dlambda) {
+    double s = 0.;
+    for (int i = lane; i < a.lam_parts; i += 64) s += (double)a.lam_part[(int64_t)h * a.lam_parts + i];
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if (lane == 0) a.dlambda[h] = (float)-s;
+  }
+  const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
+  const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
+  const float nlam = -a.lambda[h], scale = a.sl2 / kLog2e;
+
+  for (int qt = bx * kBQ; qt < q_len; qt += gridDim.x * kBQ) {
+    const int qi = qt + w * 32 + l32;
+    const int64_t qrow = q0 + min(qi, q_len - 1), stat = (int64_t)h * a.total_q + qrow;
+    const int64_t map2 = (int64_t)a.H * a.total_q;
+    Fr qf[KS], df[KS];
+    {
+      const T* p = (const T*)a.q + qrow * a.ldq + (int64_t)h * D + 8 * hf;
+      const T* d = (const T*)a.dout + (qrow * a.H + h) * D + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        qf[st] = F::load(p + 16 * st);
+        df[st] = F::load(d + 16 * st);
+      }
+    }
+    const float l1 = a.lse[stat], l2 = a.lse[map2 + stat], r1 = a.r12[stat], r2 = a.r12[map2 + stat];
+    f32x16_t acc[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) clear(acc[mt]);
+    Stage<T, D, BK, kNT> ks, vs;
+    ks.load(kbase, a.ldk, 0, kv_len);
+    vs.load(vbase, a.ldv, 0, kv_len);
+    for (int kb = 0; kb < kv_len; kb += BK) {
+      __syncthreads();
+      ks.store(kt);
+      vs.store(vt);
+      __syncthreads();
+      ks.load(kbase, a.ldk, kb + BK, kv_len);
+      vs.load(vbase, a.ldv, kb + BK, kv_len);
+      f32x16_t s1, s2, dp;
+      clear(s1);
+      clear(s2);
+      clear(dp);
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        F::mma(Ti::row(kt, 0, l32, hf, st), qf[st], st < KS / 2 ? s1 : s2);
+        F::mma(Ti::row(vt, 0, l32, hf, st), df[st], dp);
+      }
+      float d1[16], d2[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const bool ok = kb + 8 * (j >> 2) + 4 * hf + (j & 3) < kv_len;
+        const float p1 = ok ? fast_exp2(fmaf(s1[j], a.sl2, -l1)) : 0.f;
+        const float p2 = ok ? fast_exp2(fmaf(s2[j], a.sl2, -l2)) : 0.f;
+        d1[j] = p1 * (dp[j] - r1);
+        d2[j] = p2 * ((dp[j] - r2) * nlam);
+      }
+      const Fr f1[2] = {F::pack(d1), F::pack(d1 + 8)}, f2[2] = {F::pack(d2), F::pack(d2 + 8)};
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          F::mma(Ti::col(kt, 0, lane, g, mt), mt < MT / 2 ? f1[g] : f2[g], acc[mt]);
+    }
+    if (qi < q_len) {
+      T* p = (T*)a.dq + ((int64_t)(q0 + qi) * a.H + h) * D;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) store_dims(p + 32 * mt, hf, acc[mt], scale);
+    }
+  }
+}
+
+// dk and dv of 128 keys.  The sequence ranking of block_tile goes by the queries here.
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
+  typedef Frag<T> F;
+  typedef typename F::type Fr;
+  typedef Tile<T, D> Ti;
+  constexpr int BQ = 32;
+  constexpr int KS = D / 16, MT = D / 32;
+  __shared__ __attribute__((aligned(16))) unsigned char qt[BQ * Ti::ROWB], dt[BQ * Ti::ROWB];
+  __shared__ __attribute__((aligned(16))) float st4[4][BQ];  // log-sum-exps and r of the two maps
+  int bx, h, bb;
+  block_tile(a.cu_q, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l32 = lane & 31, hf = lane >> 5;
+  if (a.rest) {
+    zero_rest((T*)a.dk, a.cu_kv, a.total_kv, bb, a.H, D, h, bx, gridDim.x);
+    zero_rest((T*)a.dv, a.cu_kv, a.total_kv, bb, a.H, D, h, bx, gridDim.x);
+  }
+  const T* qbase = (const T*)a.q + (int64_t)q0 * a.ldq + (int64_t)h * D;
+  const T* dbase = (const T*)a.dout + ((int64_t)q0 * a.H + h) * D;
+  const int64_t ldd = (int64_t)a.H * D;
+  const float lam = a.lambda[h], scale = a.sl2 / kLog2e;
+  // Thread tid < 128 brings statistic tid / 32 of query tid % 32.
+  const float* sbase = (tid & 64 ? a.r12 : a.lse) + ((int64_t)(tid & 32 ? a.H : 0) + h) * a.total_q + q0;
+
+  for (int kt = bx * kBQ; kt < kv_len; kt += gridDim.x * kBQ) {
+    const int ki = kt + w * 32 + l32;
+    const int64_t krow = kv0 + min(ki, kv_len - 1);
+    Fr kf[KS], vf[KS];
+    {
+      const T* p = (const T*)a.k + krow * a.ldk + (int64_t)h * D + 8 * hf;
+      const T* d = (const T*)a.v + krow * a.ldv + (int64_t)h * D + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        kf[st] = F::load(p + 16 * st);
+        vf[st] = F::load(d + 16 * st);
+      }
+    }
+    f32x16_t dk[MT], dv[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      clear(dk[mt]);
+      clear(dv[mt]);
+    }
+    Stage<T, D, BQ, kNT> qs, ds;
+    float sv = 0.f;
+    auto load = [&](int qb) {
+      qs.load(qbase, a.ldq, qb, q_len);
+      ds.load(dbase, ldd, qb, q_len);
+      if (tid < 128) {  // past the last query: P = 2^(0 - inf) = 0
+        const int r = qb + (tid & 31);
+        sv = r < q_len ? sbase[r] : tid < 64 ? INFINITY : 0.f;
+      }
+    };
+    load(0);
+    for (int qb = 0; qb < q_len; qb += BQ) {
+      __syncthreads();
+      qs.store(qt);
+      ds.store(dt);
+      if (tid < 128) st4[tid >> 5][tid & 31] = sv;
+      __syncthreads();
+      load(qb + BQ);
+      f32x16_t s1, s2, dp;
+      clear(s1);
+      clear(s2);
+      clear(dp);
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        F::mma(Ti::row(qt, 0, l32, hf, st), kf[st], st < KS / 2 ? s1 : s2);
+        F::mma(Ti::row(dt, 0, l32, hf, st), vf[st], dp);
+      }
+      float p[16], d1[16], d2[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int r = 8 * (j >> 2) + 4 * hf + (j & 3);
+        const float p1 = fast_exp2(fmaf(s1[j], a.sl2, -st4[0][r]));
+        const float p2 = lam * fast_exp2(fmaf(s2[j], a.sl2, -st4[1][r]));
+        p[j] = p1 - p2;
+        d1[j] = p1 * (dp[j] - st4[2][r]);
+        d2[j] = p2 * (st4[3][r] - dp[j]);
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const Fr pf = F::pack(p + 8 * g), f1 = F::pack(d1 + 8 * g), f2 = F::pack(d2 + 8 * g);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          F::mma(Ti::col(dt, 0, lane, g, mt), pf, dv[mt]);
+          F::mma(Ti::col(qt, 0, lane, g, mt), mt < MT / 2 ? f1 : f2, dk[mt]);
+        }
+      }
+    }
+    if (ki < kv_len) {
+      const int64_t at = ((int64_t)(kv0 + ki) * a.H + h) * D;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        store_dims((T*)a.dk + at + 32 * mt, hf, dk[mt], scale);
+        store_dims((T*)a.dv + at + 32 * mt, hf, dv[mt], 1.f);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------- host
+// Tiles of 128 rows that the grid gives a sequence; the kernels' loops cover longer ones.
+unsigned tiles_of(int64_t longest, int64_t hb) {
+  return (unsigned)std::max<int64_t>(
+      1, std::min<int64_t>(std::min<int64_t>((longest + kBQ - 1) / kBQ, 65535), (INT32_MAX / 16) / hb));
+}
+
+// Parts of the keys: where the query tiles leave CUs idle and there are keys to share.
+int da_splits(int32_t B, int64_t total_kv, int32_t H, int64_t max_q) {
+  const int64_t blocks = (int64_t)tiles_of(max_q, (int64_t)H * B) * H * B;
+  const int64_t keys = total_kv / B;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, keys / 256, 64}));
+}
+
+// Row-dot blocks of a (head, sequence).
+int rowdot_blocks(int64_t max_q) { return (int)std::min<int64_t>(std::max<int64_t>(1, (max_q + 63) / 64), 256); }
+
+template <typename F>
+int by_type(int32_t dtype, int32_t D, F f) {
+  constexpr std::integral_constant<int, 64> D64{};
+  constexpr std::integral_constant<int, 128> D128{};
+  auto dims = [&](auto t) { D == 64 ? f(t, D64) : f(t, D128); };
+  if (dtype == TSC_BF16) dims(__bf16());
+  else if (dtype == TSC_F16) dims(_Float16());
+  else dims(float());
+  return check_hip(hipGetLastError(), "diff_attention launch");
+}
+
+DaArgs da_args(const DiffAttnArgs& x) {
+  DaArgs a = {};
+  a.q = x.q;
+  a.k = x.k;
+  a.v = x.v;
+  a.ldq = x.ldq;
+  a.ldk = x.ldk;
+  a.ldv = x.ldv;
+  a.lambda = x.lambda;
+  a.cu_q = x.cu_q;
+  a.cu_kv = x.cu_kv;
+  a.total_q = x.total_q;
+  a.total_kv = x.total_kv;
+  a.H = x.H;
+  a.sl2 = x.scale * kLog2e;
+  a.rest = x.rest;
+  a.splits = 1;
+  return a;
+}
+
+}  // namespace
+
+int64_t diff_attention_workspace_bytes(int32_t B, int64_t total_q, int64_t total_kv, int32_t H,
+                                       int32_t D, int32_t max_q, int32_t backward) {
+  if (B == 0 || total_q == 0) return 0;
+  if (backward) return 4 * (2 * (int64_t)H * total_q + (int64_t)H * B * rowdot_blocks(max_q));
+  const int s = da_splits(B, total_kv, H, max_q);
+  return s > 1 ? 4 * (int64_t)s * total_q * H * (2 * D + 4) : 0;
+}
+
+int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* out2, float* lse,
+                          void* ws) {
+  const int64_t hb = (int64_t)x.H * x.B;
+  if (hb > (int64_t)(INT32_MAX / 1024))
+    return fail(TSC_ERR_UNSUPPORTED, "diff_attention: %lld (head, sequence) pairs", (long long)hb);
+  DaArgs a = da_args(x);
+  a.out = out;
+  a.out2 = out2;
+  a.lse = lse;
+  a.splits = da_splits(x.B, x.total_kv, x.H, x.max_q);
+  a.part = (float*)ws;
+  const dim3 grid(tiles_of(x.max_q, hb) * a.splits, (unsigned)x.H, (unsigned)x.B);
+  return by_type(x.dtype, x.D, [&](auto t, auto d) {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    {
+      ProfScope p(ctx, "diff_attention");
+      da_forward_kernel<T, D><<<grid, kNT, 0, ctx->stream>>>(a);
+    }
+    if (a.splits > 1) {
+      ProfScope p(ctx, "diff_attention_join");
+      da_join_kernel<T, D><<<(unsigned)((x.total_q * x.H + 3) / 4), kNT, 0, ctx->stream>>>(a, x.B);
+    }
+  });
+}
+
+int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const void* out,
+                                   const void* out2, const float* lse, const void* dout, void* ws,
+                                   void* dq, void* dk, void* dv, float* dlambda) {
+  const int64_t hb = (int64_t)x.H * x.B;
+  if (hb > (int64_t)(INT32_MAX / 1024))
+    return fail(TSC_ERR_UNSUPPORTED, "diff_attention: %lld (head, sequence) pairs", (long long)hb);
+  DaArgs a = da_args(x);
+  a.out = (void*)out;
+  a.out2 = (void*)out2;
+  a.lse = (float*)lse;
+  a.dout = dout;
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.dlambda = dlambda;
+  float* r12 = (float*)ws;
+  float* lam_part = r12 + 2 * (int64_t)x.H * x.total_q;
+  const int rb = rowdot_blocks(x.max_q);
+  a.r12 = r12;
+  a.lam_part = lam_part;
+  a.lam_parts = rb * x.B;
+  return by_type(x.dtype, x.D, [&](auto t, auto d) {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    {
+      ProfScope p(ctx, "diff_attention_rowdot");
+      da_rowdot_kernel<T, D><<<dim3((unsigned)rb, (unsigned)x.H, (unsigned)x.B), kNT, 0, ctx->stream>>>(
+          a, r12, lam_part);
+    }
+    {
+      ProfScope p(ctx, "diff_attention_dkv");
+      da_dkv_kernel<T, D><<<dim3(tiles_of(x.max_kv, hb), (unsigned)x.H, (unsigned)x.B), kNT, 0,
+                            ctx->stream>>>(a);
+    }
+    ProfScope p(ctx, "diff_attention_dq");
+    da_dq_kernel<T, D><<<dim3(tiles_of(x.max_q, hb), (unsigned)x.H, (unsigned)x.B), kNT, 0,
+                         ctx->stream>>>(a);
+  });
+}
+
+}  // namespace tsc

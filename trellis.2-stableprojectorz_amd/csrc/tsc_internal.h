@@ -230,6 +230,28 @@ int attention_launch(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, 
                      int64_t total_kv, int32_t H, int32_t D, float scale, int32_t max_seqlen_q,
                      void* out);
 
+// ---- implemented in diff_attention.hip ----
+struct DiffAttnArgs {
+  int32_t dtype;
+  const void *q, *k, *v;
+  int64_t ldq, ldk, ldv;  // row strides in elements
+  const float* lambda;
+  const int32_t *cu_q, *cu_kv;
+  int32_t B;
+  int64_t total_q, total_kv;
+  int32_t H, D;
+  float scale;
+  int32_t max_q, max_kv;  // longest sequences: they size the grids
+  int32_t rest;
+};
+int64_t diff_attention_workspace_bytes(int32_t B, int64_t total_q, int64_t total_kv, int32_t H,
+                                       int32_t D, int32_t max_q, int32_t backward);
+int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* out2, float* lse,
+                          void* ws);
+int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const void* out,
+                                   const void* out2, const float* lse, const void* dout, void* ws,
+                                   void* dq, void* dk, void* dv, float* dlambda);
+
 // ---- implemented in groupnorm.hip ----
 int64_t groupnorm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C, int32_t groups,
                                   int32_t backward);

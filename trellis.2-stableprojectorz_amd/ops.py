@@ -316,7 +316,7 @@ def _group_norm(x, weight, bias, cu, b, groups, eps, silu, out, stats):
     nbytes = lib.tsc_groupnorm_workspace_bytes(_code(x), b, n, c, groups, 0)
     ws = _scratch(nbytes, x.device)
     check(lib.tsc_groupnorm(handle, _code(x), _p(x), _p(cu), b, n, c, groups, _p(weight),
-                                _p(bias), eps, int(silu), int(rest), _p(stats), _p(ws), _p(out)))
+                            _p(bias), eps, int(silu), int(rest), _p(stats), _p(ws), _p(out)))
     return out
 
 
@@ -331,9 +331,9 @@ def _group_norm_backward(dy, x, weight, bias, cu, b, groups, silu, stats, want_p
     lib, handle = _lib.stream_handle(x.device.index)
     nbytes = lib.tsc_groupnorm_workspace_bytes(_code(x), b, n, c, groups, 1)
     ws = _scratch(nbytes, x.device)
-    check(lib.tsc_groupnorm_backward(handle, _code(x), _p(dy), _p(x), _p(cu), b, n, c,
-                                         groups, _p(weight), _p(bias), int(silu), 1, _p(stats),
-                                         _p(ws), _p(dx), _p(dw), _p(db)))
+    check(lib.tsc_groupnorm_backward(handle, _code(x), _p(dy), _p(x), _p(cu), b, n, c, groups,
+                                     _p(weight), _p(bias), int(silu), 1, _p(stats), _p(ws), _p(dx),
+                                     _p(dw), _p(db)))
     return dx, dw, db
 
 
@@ -525,6 +525,123 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                                 tkv, h, d, float(scale) if scale else 0.0, int(max_seqlen_q),
                                 _p(out)))
     return out.view(tq, h, d)
+
+
+def _head_rows(t: torch.Tensor, name: str) -> int:
+    """Row stride in elements of a (total, H, D) tensor whose rows are contiguous."""
+    _, h, d = t.shape
+    if t.stride(2) != 1 or (h > 1 and t.stride(1) != d) or (t.shape[0] > 1 and t.stride(0) < h * d):
+        raise TscError(_lib.TSC_ERR_INVALID, f"{name}: each row's (H, D) values must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else h * d
+
+
+def sparse_diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
+                          cu_seqlens_q, cu_seqlens_kv=None, scale: float | None = None, out=None,
+                          max_seqlen_q: int | None = None,
+                          max_seqlen_kv: int | None = None) -> torch.Tensor:
+    """Differential attention over packed sequences (tsc_diff_attention):
+
+        out = (softmax(q1 k1^T scale) - lam[h] softmax(q2 k2^T scale)) v,   q = [q1 | q2], k = [k1 | k2]
+
+    q (total_q, H, D), k / v (total_kv, H, D) and the cu_seqlens as in sparse_attention; D is 64 or
+    128, the maps have D/2 dimensions each, and scale defaults to 1/sqrt(D/2).  lam is float32 (H,).
+    Rows may be strided (q = qkv[:, 0] of a (total, 3, H, D) projection).  Few queries on many keys
+    are shared out over the keys.  With device cu_seqlens the longest sequences' lengths only size the
+    grids; pass them where they are known (they default to twice the mean).  Rows outside every
+    sequence are zero in a new result and left as they were in `out`.
+    Differentiable in q, k, v and lam (then without `out`; a graph through the gradient itself is not
+    supported)."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[1:] != q.shape[1:]:
+        raise TscError(_lib.TSC_ERR_INVALID, f"diff_attention: q {tuple(q.shape)}, k {tuple(k.shape)} "
+                                             f"and v {tuple(v.shape)} must be (total, H, D)")
+    tq, h, d = q.shape
+    tkv = k.shape[0]
+    if d not in (64, 128):
+        raise TscError(_lib.TSC_ERR_UNSUPPORTED, f"diff_attention: head_dim {d} (64 and 128 are supported)")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: q, k and v must share a dtype")
+    if lam.shape != (h,) or lam.dtype != torch.float32:
+        raise TscError(_lib.TSC_ERR_INVALID, f"diff_attention: lam must be float32 ({h},)")
+    if scale is not None and not scale > 0:
+        raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: scale must be positive")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
+        raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: out has the wrong shape or dtype")
+    _code(q)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _head_rows(t, name)
+    lam = lam.contiguous()
+    dev = _dev(lam, out)
+    for t in (q, k, v):
+        if not t.is_cuda or t.device.index != dev:
+            raise TscError(_lib.TSC_ERR_INVALID, "tensors are not on one GPU; this path has no CPU fallback")
+    cq_host, cq = _cu_seqlens(cu_seqlens_q, tq, dev, "cu_seqlens_q")
+    if cu_seqlens_kv is None:
+        if tkv != tq:
+            raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: cu_seqlens_kv is needed where k has "
+                                                 "other rows than q")
+        ck_host, ck = cq_host, cq
+    else:
+        ck_host, ck = _cu_seqlens(cu_seqlens_kv, tkv, dev, "cu_seqlens_kv")
+    _dev(cq, ck, lam)
+    if ck.numel() != cq.numel():
+        raise TscError(_lib.TSC_ERR_INVALID, "cu_seqlens_q and cu_seqlens_kv differ in length")
+    b = cq.numel() - 1
+
+    def longest(given, host, total):
+        if given is not None:
+            return max(0, min(int(given), total))
+        if b == 0:
+            return 0
+        return int((host[1:] - host[:-1]).max()) if host is not None else min(total, 2 * -(-total // b))
+
+    args = (cq, ck, b, float(scale) if scale is not None else 0.0,
+            longest(max_seqlen_q, cq_host, tq), longest(max_seqlen_kv, ck_host, tkv))
+    if _wants_grad(q, k, v, lam):
+        if out is not None:
+            raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: out cannot be given where gradients "
+                                                 "are wanted")
+        from .autograd import DiffAttention
+
+        return DiffAttention.apply(q, k, v, lam, *args)
+    return _diff_attention(q, k, v, lam, *args, out, False)[0]
+
+
+def _diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, out, keep):
+    """(out, out2, lse); out2 and lse (None unless keep) are what the backward pass needs."""
+    tq, h, d = q.shape
+    tkv = k.shape[0]
+    rest = out is None
+    if out is None:
+        out = (torch.empty if b else torch.zeros)((tq, h, d), dtype=q.dtype, device=q.device)
+    out2 = torch.empty_like(out) if keep else None
+    lse = torch.empty((2, h, tq), dtype=torch.float32, device=q.device) if keep else None
+    if tq and b:
+        lib, handle = _lib.stream_handle(q.device.index)
+        nbytes = lib.tsc_diff_attention_workspace_bytes(_code(q), b, tq, tkv, h, d, max_q, 0)
+        ws = _scratch(nbytes, q.device) if nbytes else None
+        check(lib.tsc_diff_attention(handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"),
+                                     _head_rows(k, "k"), _head_rows(v, "v"), _p(lam), _p(cq), _p(ck), b,
+                                     tq, tkv, h, d, scale, max_q, int(rest), _p(ws), _p(out), _p(out2),
+                                     _p(lse)))
+    return out, out2, lse
+
+
+def _diff_attention_backward(do, q, k, v, lam, out, out2, lse, cq, ck, b, scale, max_q, max_kv):
+    tq, h, d = q.shape
+    tkv = k.shape[0]
+    alloc = torch.empty if tq and b else torch.zeros
+    dq = alloc((tq, h, d), dtype=q.dtype, device=q.device)
+    dk, dv = (alloc((tkv, h, d), dtype=q.dtype, device=q.device) for _ in range(2))
+    dlam = alloc((h,), dtype=torch.float32, device=q.device)
+    if tq and b:
+        lib, handle = _lib.stream_handle(q.device.index)
+        nbytes = lib.tsc_diff_attention_workspace_bytes(_code(q), b, tq, tkv, h, d, max_q, 1)
+        ws = _scratch(nbytes, q.device)
+        check(lib.tsc_diff_attention_backward(
+            handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"), _head_rows(k, "k"),
+            _head_rows(v, "v"), _p(lam), _p(cq), _p(ck), b, tq, tkv, h, d, scale, max_q, max_kv, 1,
+            _p(out), _p(out2), _p(lse), _p(do), _p(ws), _p(dq), _p(dk), _p(dv), _p(dlam)))
+    return dq, dk, dv, dlam
 
 
 def scaled_dot_product_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
