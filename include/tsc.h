@@ -343,7 +343,8 @@ int tsc_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, con
  * No counterpart in the reference, whose attention is one map (src/sparse/ops/attention.ts:24-79). */
 int64_t tsc_diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q,
                                            int64_t total_kv, int32_t num_heads, int32_t head_dim,
-                                           int32_t max_seqlen_q, int32_t backward);
+                                           int32_t max_seqlen_q, int32_t max_seqlen_kv,
+                                           int32_t backward);
 int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, const void* v,
                        int64_t ld_q, int64_t ld_k, int64_t ld_v, const float* lambda,
                        const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv, int32_t B,

@@ -43,12 +43,13 @@ def test_c_entry_points_without_a_gpu(pkg):
     lib = pkg.load_library()
     P = ctypes.c_void_p
     ws = lib.tsc_diff_attention_workspace_bytes
-    assert ws(2, 1, 1, 40000, 12, 128, 1, 0) > 0  # one query: shared out over the keys
-    assert ws(2, 1, 20000, 20000, 12, 128, 20000, 0) == 0
-    assert ws(2, 1, 100, 100, 12, 128, 100, 1) >= 2 * 12 * 100 * 4
-    assert ws(2, 0, 0, 0, 12, 128, 0, 0) == 0
-    for bad in ((3, 1, 1, 1, 1, 64, 1, 0), (0, 1, 1, 1, 1, 32, 1, 0), (0, -1, 1, 1, 1, 64, 1, 0),
-                (0, 1, 2 ** 31, 1, 1, 64, 1, 0), (0, 1, 1, 1, 0, 64, 1, 0), (0, 1, 1, 1, 1, 64, -1, 0)):
+    assert ws(2, 1, 1, 40000, 12, 128, 1, 40000, 0) > 0  # one query: shared out over the keys
+    assert ws(2, 1, 20000, 20000, 12, 128, 20000, 20000, 0) == 0
+    assert ws(2, 1, 100, 100, 12, 128, 100, 100, 1) >= 2 * 12 * 100 * 4
+    assert ws(2, 0, 0, 0, 12, 128, 0, 0, 0) == 0
+    for bad in ((3, 1, 1, 1, 1, 64, 1, 1, 0), (0, 1, 1, 1, 1, 32, 1, 1, 0), (0, -1, 1, 1, 1, 64, 1, 1, 0),
+                (0, 1, 2 ** 31, 1, 1, 64, 1, 1, 0), (0, 1, 1, 1, 0, 64, 1, 1, 0), (0, 1, 1, 1, 1, 64, -1, 1, 0),
+                (0, 1, 1, 1, 1, 64, 1, -1, 0)):
         assert ws(*bad) == -1 and lib.tsc_last_error(), bad
     st = lib.tsc_diff_attention(None, 0, P(16), P(16), P(16), 64, 64, 64, P(16), P(16), P(16), 1, 1, 1,
                                 1, 64, 0.0, 1, 0, None, P(16), None, None)

@@ -11,7 +11,7 @@ value is below its normal range (half its smallest step):
               it is off by sum |do| times their tolerances
   dS          P (error of dP and r) + (u + e) |dS|; dq, dk: their sums against |k|, |q|, one rounding
   dv          (u + e) (P1 + |lambda| P2)^T |do| (the difference is one rounded number), one rounding
-  dlambda     the sum of r2's errors, 2^-20 of the sum of |r2|
+  dlambda     - sum P2 dP, from unrounded fp32 values: e of the sum of P2 |dP|, and dP's error
 Sums of fp32 products: 2^-20 of the sum of the sizes (fewer than 16 roundings on a term's way through
 the accumulator at equal size; rows here are at most 9000 long)."""
 import math
@@ -94,7 +94,7 @@ def _oracle(q, k, v, do, lam, cq, ck, dtype, scale=None):
             r["dk"][:, c, m] = dS.transpose(1, 2) @ qs[..., m] * z
             t["dk"][:, c, m] = (tS + ACC * dS.abs()).transpose(1, 2) @ qs[..., m].abs() * z
         r["dlam"] -= r2.sum((1, 2))
-        t["dlam"] += e_r2.sum((1, 2)) + ACC * r2.abs().sum((1, 2))
+        t["dlam"] += (P[1] * (E[1] * dP.abs() + e_dP)).sum((1, 2))
     for n in ("dq", "dk", "dv"):
         t[n] += u * r[n].abs() + sub
     return {n: ((r[n], t[n]) if n == "dlam" else (r[n].transpose(0, 1), t[n].transpose(0, 1))) for n in r}

@@ -786,15 +786,16 @@ static size_t row_span(int64_t rows, int64_t ld, const DiffAttnArgs& x) {
 
 int64_t tsc_diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q,
                                            int64_t total_kv, int32_t num_heads, int32_t head_dim,
-                                           int32_t max_seqlen_q, int32_t backward) {
+                                           int32_t max_seqlen_q, int32_t max_seqlen_kv,
+                                           int32_t backward) {
   g_err[0] = 0;
   DiffAttnArgs x;
   if (diff_attention_args(nullptr, "diff_attention_workspace_bytes", dtype, nullptr, nullptr, nullptr,
                           0, 0, 0, nullptr, nullptr, nullptr, B, total_q, total_kv, num_heads,
-                          head_dim, 0.f, max_seqlen_q, 0, 0, &x))
+                          head_dim, 0.f, max_seqlen_q, max_seqlen_kv, 0, &x))
     return -1;
   return diff_attention_workspace_bytes(B, total_q, total_kv, num_heads, head_dim, max_seqlen_q,
-                                        backward);
+                                        max_seqlen_kv, backward);
 }
 
 int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, const void* v,
@@ -816,7 +817,7 @@ int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k
   if ((out2 == nullptr) != (lse == nullptr))
     return fail(TSC_ERR_INVALID, "diff_attention: out2 and lse go together");
   const int64_t need = diff_attention_workspace_bytes(B, total_q, total_kv, num_heads, head_dim,
-                                                      max_seqlen_q, 0);
+                                                      max_seqlen_q, 0, 0);
   if (need > 0 && !workspace) return fail(TSC_ERR_INVALID, "diff_attention: null workspace");
   if (!aligned(out, 16) || !aligned(out2, 16) || !aligned(lse, 4) || !aligned(workspace, 16))
     return fail(TSC_ERR_INVALID, "diff_attention: out, out2 and workspace must be 16-byte aligned");

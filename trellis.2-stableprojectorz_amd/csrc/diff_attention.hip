@@ -216,7 +216,7 @@ struct DaArgs {
   // backward
   const void* dout;
   const float* r12;  // (2, H, total_q)
-  const float* lam_part;
+  float* lam_part;   // (H, B, dk / dv blocks of a sequence)
   int32_t lam_parts;
   void *dq, *dk, *dv;
   float* dlambda;
@@ -409,18 +409,16 @@ __global__ void __launch_bounds__(kNT) da_join_kernel(const DaArgs a, int32_t B)
 }
 
 // ------------------------------------------------------------------------------- backward
-// r_i = do . (P_i v) per query, P1 v = out + lambda P2 v; and per block the sum of r2 for dlambda.
+// r_i = do . (P_i v) per query, P1 v = out + lambda P2 v.
 // Block: one head, the rows of one sequence in steps of 256 / (D / 8) per grid column.
 template <typename T, int D>
-__global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r12, float* lam_part) {
+__global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r12) {
   constexpr int LPR = D / 8;  // lanes of a row, 8 elements each
   constexpr int RPB = kNT / LPR;
-  __shared__ float sum[kNT / 64];
   const int h = blockIdx.y, bb = blockIdx.z, e0 = threadIdx.x % LPR * 8;
   int q0, q_len;
   segment(a.cu_q, bb, a.total_q, &q0, &q_len);
   const float lam = a.lambda[h];
-  float acc = 0.f;
   for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR; r < q_len;
        r += (int64_t)gridDim.x * RPB) {
     const int64_t at = ((q0 + r) * a.H + h) * D + e0;
@@ -444,15 +442,8 @@ __global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r
     if (e0 == 0) {
       r12[(int64_t)h * a.total_q + q0 + r] = fmaf(lam, r2, r1);
       r12[(int64_t)(a.H + h) * a.total_q + q0 + r] = r2;
-      acc += r2;
     }
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
-  if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = acc;
-  __syncthreads();
-  if (threadIdx.x == 0)
-    lam_part[((int64_t)h * gridDim.z + bb) * gridDim.x + blockIdx.x] = sum[0] + sum[1] + sum[2] + sum[3];
 }
 
 // dq of 128 queries; one block of each head also adds up dlambda.
@@ -475,7 +466,7 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
     double s = 0.;
     for (int i = lane; i < a.lam_parts; i += 64) s += (double)a.lam_part[(int64_t)h * a.lam_parts + i];
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-    if (lane == 0) a.dlambda[h] = (float)-s;
+    if (lane == 0) a.dlambda[h] = (float)s;
   }
   const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
   const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
@@ -542,7 +533,8 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
   }
 }
 
-// dk and dv of 128 keys.  The sequence ranking of block_tile goes by the queries here.
+// dk and dv of 128 keys, and the block's part of dlambda = - sum P2 dP, from the unrounded fp32
+// probabilities (do . (P2 v) with P2 v in 16 bits is off by 2^-9 of it).  The sequence ranking of block_tile goes by the queries here.
 template <typename T, int D>
 __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
   typedef Frag<T> F;
@@ -567,6 +559,7 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
   const int64_t ldd = (int64_t)a.H * D;
   const float lam = a.lambda[h], scale = a.sl2 / kLog2e;
   // Thread tid < 128 brings statistic tid / 32 of query tid % 32.
+  float dlam = 0.f;
   const float* sbase = (tid & 64 ? a.r12 : a.lse) + ((int64_t)(tid & 32 ? a.H : 0) + h) * a.total_q + q0;
 
   for (int kt = bx * kBQ; kt < kv_len; kt += gridDim.x * kBQ) {
@@ -615,16 +608,18 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
         F::mma(Ti::row(qt, 0, l32, hf, st), kf[st], st < KS / 2 ? s1 : s2);
         F::mma(Ti::row(dt, 0, l32, hf, st), vf[st], dp);
       }
-      float p[16], d1[16], d2[16];
+      float p[16], d1[16], d2[16], lsum = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int r = 8 * (j >> 2) + 4 * hf + (j & 3);
         const float p1 = fast_exp2(fmaf(s1[j], a.sl2, -st4[0][r]));
-        const float p2 = lam * fast_exp2(fmaf(s2[j], a.sl2, -st4[1][r]));
+        const float q2 = fast_exp2(fmaf(s2[j], a.sl2, -st4[1][r])), p2 = lam * q2;
+        lsum = fmaf(q2, dp[j], lsum);
         p[j] = p1 - p2;
         d1[j] = p1 * (dp[j] - st4[2][r]);
         d2[j] = p2 * (st4[3][r] - dp[j]);
       }
+      if (ki < kv_len) dlam -= lsum;  // lanes past the last key repeat it
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const Fr pf = F::pack(p + 8 * g), f1 = F::pack(d1 + 8 * g), f2 = F::pack(d2 + 8 * g);
@@ -644,6 +639,14 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
       }
     }
   }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) dlam += __shfl_xor(dlam, off, 64);
+  __syncthreads();
+  if (lane == 0) st4[0][w] = dlam;
+  __syncthreads();
+  if (tid == 0)
+    a.lam_part[((int64_t)h * gridDim.z + bb) * gridDim.x + bx] =
+        (st4[0][0] + st4[0][1]) + (st4[0][2] + st4[0][3]);
 }
 
 // ------------------------------------------------------------------------------- host
@@ -660,7 +663,7 @@ int da_splits(int32_t B, int64_t total_kv, int32_t H, int64_t max_q) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, keys / 256, 64}));
 }
 
-// Row-dot blocks of a (head, sequence).
+// Blocks of the r kernel for a (head, sequence).
 int rowdot_blocks(int64_t max_q) { return (int)std::min<int64_t>(std::max<int64_t>(1, (max_q + 63) / 64), 256); }
 
 template <typename F>
@@ -697,9 +700,10 @@ DaArgs da_args(const DiffAttnArgs& x) {
 }  // namespace
 
 int64_t diff_attention_workspace_bytes(int32_t B, int64_t total_q, int64_t total_kv, int32_t H,
-                                       int32_t D, int32_t max_q, int32_t backward) {
+                                       int32_t D, int32_t max_q, int32_t max_kv, int32_t backward) {
   if (B == 0 || total_q == 0) return 0;
-  if (backward) return 4 * (2 * (int64_t)H * total_q + (int64_t)H * B * rowdot_blocks(max_q));
+  const int64_t hb = (int64_t)H * B;
+  if (backward) return 4 * (2 * (int64_t)H * total_q + hb * tiles_of(max_kv, hb));
   const int s = da_splits(B, total_kv, H, max_q);
   return s > 1 ? 4 * (int64_t)s * total_q * H * (2 * D + 4) : 0;
 }
@@ -747,17 +751,16 @@ int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const vo
   a.dlambda = dlambda;
   float* r12 = (float*)ws;
   float* lam_part = r12 + 2 * (int64_t)x.H * x.total_q;
-  const int rb = rowdot_blocks(x.max_q);
   a.r12 = r12;
   a.lam_part = lam_part;
-  a.lam_parts = rb * x.B;
+  a.lam_parts = (int)tiles_of(x.max_kv, hb) * x.B;
   return by_type(x.dtype, x.D, [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     {
       ProfScope p(ctx, "diff_attention_rowdot");
-      da_rowdot_kernel<T, D><<<dim3((unsigned)rb, (unsigned)x.H, (unsigned)x.B), kNT, 0, ctx->stream>>>(
-          a, r12, lam_part);
+      da_rowdot_kernel<T, D><<<dim3((unsigned)rowdot_blocks(x.max_q), (unsigned)x.H, (unsigned)x.B),
+                               kNT, 0, ctx->stream>>>(a, r12);
     }
     {
       ProfScope p(ctx, "diff_attention_dkv");

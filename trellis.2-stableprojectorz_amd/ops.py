@@ -617,7 +617,8 @@ def _diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, out, keep):
     lse = torch.empty((2, h, tq), dtype=torch.float32, device=q.device) if keep else None
     if tq and b:
         lib, handle = _lib.stream_handle(q.device.index)
-        nbytes = lib.tsc_diff_attention_workspace_bytes(_code(q), b, tq, tkv, h, d, max_q, 0)
+        nbytes = lib.tsc_diff_attention_workspace_bytes(_code(q), b, tq, tkv, h, d, max_q, max_kv,
+                                                        0)
         ws = _scratch(nbytes, q.device) if nbytes else None
         check(lib.tsc_diff_attention(handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"),
                                      _head_rows(k, "k"), _head_rows(v, "v"), _p(lam), _p(cq), _p(ck), b,
@@ -635,7 +636,8 @@ def _diff_attention_backward(do, q, k, v, lam, out, out2, lse, cq, ck, b, scale,
     dlam = alloc((h,), dtype=torch.float32, device=q.device)
     if tq and b:
         lib, handle = _lib.stream_handle(q.device.index)
-        nbytes = lib.tsc_diff_attention_workspace_bytes(_code(q), b, tq, tkv, h, d, max_q, 1)
+        nbytes = lib.tsc_diff_attention_workspace_bytes(_code(q), b, tq, tkv, h, d, max_q, max_kv,
+                                                        1)
         ws = _scratch(nbytes, q.device)
         check(lib.tsc_diff_attention_backward(
             handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"), _head_rows(k, "k"),
