@@ -36,6 +36,7 @@ namespace tsc {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.f;  // log2 headroom before a running maximum is raised (16 bits)
 
 // ---- fragments: 8 elements of a lane --------------------------------------------------------
 struct F32x8 {
@@ -353,6 +354,299 @@ __global__ void __launch_bounds__(kNT) da_forward_kernel(const DaArgs a) {
         }
       }
     }
+  }
+}
+
+// 16 bits, whole sequences: the two maps' softmax beside the matrix products.  As in attention.hip's
+// kernel of this kind a step of 32 keys has two phases, pinned in program order:
+//   A  the next step's scores (matrix) beside the rest of this step's exponentials (VALU) and the
+//      transposed reads of v
+//   B  both maps' sums += V^T P^T beside the next step's row maxima, the first half of its
+//      exponentials and the reads of k for the step after
+// The exponentials bound it: twice those of one map, a quarter of the VALU's rate each.
+// A wave has NM maps of its 32 queries: both at D = 64; one at D = 128, where the sums of both would
+// leave one wave per SIMD, whose stalls nothing fills (9000 + 6143 tokens, 12 x 128 bf16: 1500 us).  The
+// two waves of a query tile then meet in LDS at the end.
+// The sums of v are divided by the sum of the rounded P that they were made of.  KEEP (for the backward
+// pass) also adds up the unrounded P: the log-sum-exps have to be those of the fp32 probabilities.
+template <typename T, int D, int NM, int NW, bool KEEP>
+__global__ void __launch_bounds__(64 * NW, 2) da_forward16_kernel(const DaArgs a) {
+  typedef Tile<T, D> Ti;
+  constexpr int BK = 64;             // keys per staged block: two steps of 32
+  constexpr int CPR = Ti::CPR, ROWB = Ti::ROWB;
+  constexpr int KH = D / 32, KS = NM * KH, MT = D / 32;  // k-steps of a map's scores, of the wave's
+  constexpr int NT = 64 * NW, QW = NW * NM / 2, BQ = 32 * QW;  // query tiles of the block
+  constexpr int RI = NT / CPR, NL = BK / RI;  // rows a load of the block covers; loads of a thread
+  constexpr int NA = KS, NB = 2 * MT * NM;    // products of the two phases
+  static_assert(NL >= 1, "tile shape");
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4][BK * ROWB];
+  static_assert(NM == 2 || QW * 32 * D * 4 <= 4 * BK * ROWB, "the second map's sums fit");
+  unsigned char(*kbuf)[BK * ROWB] = lds, (*vbuf)[BK * ROWB] = lds + 2;
+  int bx, h, bb;
+  block_tile(a.cu_kv, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  if (a.rest) {
+    zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
+    if (a.out2) zero_rest((T*)a.out2, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
+  }
+  const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
+  const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
+  const float sl2 = a.sl2;
+
+  for (int qt = bx * BQ; qt < q_len; qt += gridDim.x * BQ) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // nothing derived from it is kept across q tiles
+    const int lane = tid & 63, w = tid >> 6, l32 = lane & 31, hf = lane >> 5;
+    const int map = NM == 2 ? 0 : w / QW, tile = w % QW;  // the wave's first map
+    const int qi = qt + tile * 32 + l32;
+    const int64_t at = (int64_t)(q0 + qi) * a.H + h;
+    if (kv_len == 0) {  // uniform over the block
+      if (map == 0 && qi < q_len) {
+        for (int c = hf; c < CPR; c += 2) {
+          *(uint4*)((T*)a.out + at * D + 8 * c) = make_uint4(0, 0, 0, 0);
+          if (a.out2) *(uint4*)((T*)a.out2 + at * D + 8 * c) = make_uint4(0, 0, 0, 0);
+        }
+        if (a.lse && hf == 0) {
+          a.lse[(int64_t)h * a.total_q + q0 + qi] = INFINITY;
+          a.lse[(int64_t)(a.H + h) * a.total_q + q0 + qi] = INFINITY;
+        }
+      }
+      continue;
+    }
+    const int srow = tid / CPR, sc = tid % CPR;  // staging: chunk sc of rows srow + RI * i
+    const uint32_t kst = (uint32_t)(2 * a.ldk), vst = (uint32_t)(2 * a.ldv);  // row bytes
+    u32x4_t qf[KS];
+    {
+      const T* p = (const T*)a.q + (int64_t)(q0 + min(qi, q_len - 1)) * a.ldq + (int64_t)h * D + map * 16 * KH + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) qf[st] = *(const u32x4_t*)(p + 16 * st);
+    }
+    // Block kb's rows; rows past the last key repeat it, a block past the end is block 0.  The scores
+    // of such keys are masked, and their v is stored as zeros.
+    u32x4_t kr[NL], vr[NL];
+    auto load = [&](const T* base, uint32_t rb, int kb, u32x4_t(&r)[NL]) {
+      if (kb >= kv_len) kb = 0;
+      const char* p = (const char*)base + (int64_t)kb * rb;
+      const uint32_t lim = (uint32_t)min(kv_len - 1 - kb, BK - 1) * rb + 16u * sc;
+      const uint32_t off = (uint32_t)srow * rb + 16u * sc;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) r[i] = *(const u32x4_t*)(p + min(off + (uint32_t)(RI * i) * rb, lim));
+    };
+    auto store = [&](int vb, int kb, auto masked, int v0) {  // v0: first key of the v block
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        if (decltype(masked)::value && v0 + srow + RI * i >= kv_len) vr[i] = u32x4_t{0, 0, 0, 0};
+        Ti::put(vbuf[vb], srow + RI * i, sc, vr[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < NL; ++i) Ti::put(kbuf[kb], srow + RI * i, sc, kr[i]);
+    };
+    constexpr std::true_type Y{};
+    constexpr std::false_type N{};
+    float mc[NM], l[NM], lu[NM], alpha[NM];  // mc: running maxima, times sl2
+    f32x16_t o[NM][MT], sa[NM], sb[NM];
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      mc[i] = -FLT_MAX;
+      l[i] = lu[i] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) clear(o[i][mt]);
+    }
+    u32x4_t kf[KS], vf[2][MT], pf[NM][2];
+    float pr[16 * NM];
+    auto read_k = [&](int buf, int half, int st) { kf[st] = Ti::row(kbuf[buf], half * 32, l32, hf, map * KH + st); };
+    auto read_v = [&](int buf, int half, int n) {
+      vf[n / MT][n % MT] = Ti::col(vbuf[buf], half * 32, lane, n / MT, n % MT);
+    };
+    auto score = [&](const f32x16_t(&s)[NM], int i, int j, auto masked, int k0) {
+      return decltype(masked)::value && k0 + 8 * (j >> 2) + 4 * hf + (j & 3) >= kv_len ? -INFINITY
+                                                                                        : s[i][j];
+    };
+    auto exp_one = [&](const f32x16_t(&s)[NM], int e, auto masked, int k0) {
+      pr[e] = fast_exp2(fmaf(score(s, e / 16, e % 16, masked, k0), sl2, -mc[e / 16]));
+      if (KEEP) lu[e / 16] += pr[e];
+    };
+    auto pack_one = [&](int n) {  // n-th of 8 NM pairs -> rounded P and the denominator
+      const int i = n / 8, e = 2 * (n % 8);
+      const uint32_t p = Mma<T>::pack(pr[2 * n], pr[2 * n + 1]);
+      pf[i][e / 8][(e / 2) % 4] = p;
+      l[i] = Mma<T>::add2(p, l[i]);
+    };
+    auto max_part = [&](const f32x16_t(&s)[NM], int i, int part, float mx, auto masked, int k0) {
+#pragma unroll
+      for (int j = 4 * part; j < 4 * part + 4; ++j) mx = fmaxf(mx, score(s, i, j, masked, k0));
+      return mx;
+    };
+    // Raises map i's running maxima where a score exceeds one by more than 2^kLazy.
+    auto raise = [&](int i, float mx) {
+      mx *= sl2;
+      const bool up = __builtin_amdgcn_ballot_w64(mx > mc[i] + kLazy) != 0;
+      if (up) {
+        const float mn = fmaxf(mc[i], mx);
+        alpha[i] = fast_exp2(mc[i] - mn);
+        mc[i] = mn;
+        if (KEEP) lu[i] *= alpha[i];  // the next exponentials are already added to it
+      }
+      return up;
+    };
+    auto rescale = [&](int i) {
+      l[i] *= alpha[i];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][mt][j] *= alpha[i];
+    };
+    // n-th product of a step's scores: the maps in turn.
+    auto qk = [&](int n, f32x16_t(&s)[NM]) {
+      const int i = n % NM, st = i * KH + n / NM;
+      if (n < NM) clear(s[i]);
+      Mma<T>::run(kf[st], qf[st], s[i]);
+    };
+    auto pv = [&](int n) {
+      const int g = n / (MT * NM), mt = (n / NM) % MT, i = n % NM;
+      Mma<T>::run(vf[g][mt], pf[i][g], o[i][mt]);
+    };
+    auto step = [&](f32x16_t(&cur)[NM], f32x16_t(&nxt)[NM], int vb, int vhalf, int kb, int khalf,
+                    auto masked, int k0, auto stage) {
+      constexpr int EA = 8 * NM / NA;               // exponentials and packed pairs per A group
+      constexpr int VA = (2 * MT + NA - 1) / NA;    // v reads per A group
+#pragma unroll
+      for (int n = 0; n < NA; ++n) {
+        qk(n, nxt);
+#pragma unroll
+        for (int x = 0; x < VA; ++x)
+          if (n * VA + x < 2 * MT) read_v(vb, vhalf, n * VA + x);
+#pragma unroll
+        for (int x = 0; x < EA; ++x) exp_one(cur, 8 * NM + n * EA + x, masked, k0);
+#pragma unroll
+        for (int x = 0; x < EA; ++x) pack_one(n * EA + x);  // those made longest ago first
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      constexpr int KB = (KS + NB - 1) / NB;
+      constexpr int M0 = NB / 8;             // groups before the row maxima (matrix latency)
+      constexpr int MG = NB / 4;             // groups of the row maxima
+      constexpr int E0 = M0 + MG;
+      constexpr int EB = (8 * NM + NB - E0 - 1) / (NB - E0);
+      float mx[NM];
+#pragma unroll
+      for (int n = 0; n < E0; ++n) {
+        pv(n);
+#pragma unroll
+        for (int x = 0; x < KB; ++x)
+          if (n * KB + x < KS) read_k(kb, khalf, n * KB + x);
+        if (n == M0) {
+#pragma unroll
+          for (int i = 0; i < NM; ++i) mx[i] = score(nxt, i, 0, masked, k0 + 32);
+        }
+        if (n >= M0) {
+#pragma unroll
+          for (int x = (n - M0) * 4 * NM / MG; x < (n - M0 + 1) * 4 * NM / MG; ++x)
+            mx[x / 4] = max_part(nxt, x / 4, x % 4, mx[x / 4], masked, k0 + 32);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      bool up[NM];
+#pragma unroll
+      for (int i = 0; i < NM; ++i) up[i] = raise(i, pair_max(mx[i]));
+#pragma unroll
+      for (int n = E0; n < NB; ++n) {
+        pv(n);
+#pragma unroll
+        for (int x = 0; x < KB; ++x)
+          if (n * KB + x < KS) read_k(kb, khalf, n * KB + x);
+#pragma unroll
+        for (int x = 0; x < EB; ++x)
+          if ((n - E0) * EB + x < 8 * NM) exp_one(nxt, (n - E0) * EB + x, masked, k0 + 32);
+        if (decltype(stage)::value && n == NB - NB / 4) store(kb, kb ^ 1, masked, k0 + 32);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < NM; ++i)
+        if (up[i]) rescale(i);
+    };
+    {
+      u32x4_t k1[NL];
+      load(kbase, kst, 0, kr);
+      load(vbase, vst, 0, vr);
+      load(kbase, kst, BK, k1);
+      store(0, 0, Y, 0);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) kr[i] = k1[i];
+      store(0, 1, Y, 0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int st = 0; st < KS; ++st) read_k(0, 0, st);
+#pragma unroll
+    for (int n = 0; n < KS; ++n) qk(n, sa);
+#pragma unroll
+    for (int st = 0; st < KS; ++st) read_k(0, 1, st);
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int part = 0; part < 4; ++part) mx = max_part(sa, i, part, mx, Y, 0);
+      raise(i, pair_max(mx));  // the sums are still zero
+    }
+#pragma unroll
+    for (int e = 0; e < 8 * NM; ++e) exp_one(sa, e, Y, 0);
+    __syncthreads();  // block 0's k has been read by every wave: kbuf[0] may be refilled
+    // Block jb: its v and the next block's k are in LDS; meanwhile the v of the next block and the k of
+    // the one after come in through registers, into the buffers that the block before used.
+    int jb = 0;
+    auto block = [&](auto masked) {
+      const int b = jb & 1, kb = jb * BK;
+      load(vbase, vst, kb + BK, vr);
+      load(kbase, kst, kb + 2 * BK, kr);
+      step(sa, sb, b, 0, b ^ 1, 0, masked, kb, N);
+      step(sb, sa, b, 1, b ^ 1, 1, masked, kb + 32, Y);
+      __syncthreads();
+    };
+    const int nfull = max(0, kv_len / BK - 1), nblk = (kv_len + BK - 1) / BK;
+    for (; jb < nfull; ++jb) block(N);
+    for (; jb < nblk; ++jb) block(Y);
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+      const float inv = 1.f / pair_sum(l[i]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][mt][j] *= inv;
+      if (KEEP) {
+        lu[i] = pair_sum(lu[i]);
+        if (qi < q_len && hf == 0)
+          a.lse[(int64_t)((map + i) * a.H + h) * a.total_q + q0 + qi] = mc[i] + log2f(lu[i]);
+        if (map + i == 1 && qi < q_len)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) store_dims((T*)a.out2 + at * D + 32 * mt, hf, o[i][mt], 1.f);
+      }
+    }
+    const float lam = a.lambda[h];
+    if constexpr (NM == 1) {  // the last block ended with a barrier: its buffers are free
+      float* meet = (float*)lds + tile * 32 * D + lane;
+      if (map == 1)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) meet[(16 * mt + j) * 64] = lam * o[0][mt][j];
+      __syncthreads();
+      if (map == 0)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[0][mt][j] -= meet[(16 * mt + j) * 64];
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[0][mt][j] = fmaf(-lam, o[NM - 1][mt][j], o[0][mt][j]);
+    }
+    if (map == 0 && qi < q_len)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) store_dims((T*)a.out + at * D + 32 * mt, hf, o[0][mt], 1.f);
+    __syncthreads();  // the next q tile of this block stages over these buffers
   }
 }
 
@@ -725,6 +1019,14 @@ int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* 
     constexpr int D = decltype(d)::value;
     {
       ProfScope p(ctx, "diff_attention");
+      if constexpr (sizeof(T) == 2) {
+        if (a.splits == 1) {
+          constexpr int NM = D == 64 ? 2 : 1, NW = 8 / NM;
+          if (a.lse) da_forward16_kernel<T, D, NM, NW, true><<<grid, 64 * NW, 0, ctx->stream>>>(a);
+          else da_forward16_kernel<T, D, NM, NW, false><<<grid, 64 * NW, 0, ctx->stream>>>(a);
+          return;
+        }
+      }
       da_forward_kernel<T, D><<<grid, kNT, 0, ctx->stream>>>(a);
     }
     if (a.splits > 1) {
