@@ -332,7 +332,7 @@ int tsc_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, con
  *     q, k and v may be slices of one fused projection); all other buffers are contiguous
  *   lambda     device fp32 (num_heads)
  *   cu_seqlens_q / cu_seqlens_kv, scale, max_seqlen_q  as in tsc_attention, scale <= 0 meaning
- *     1/sqrt(head_dim / 2).  A sequence without keys gives zeros.
+ *     1/sqrt(head_dim / 2); max_seqlen_kv likewise (it sizes the workspace too: the same values there).  A sequence without keys gives zeros.
  *   zero_rest  rows of out (and out2) outside every sequence: 0 = left as they were, 1 = zeroed
  *   out2, lse  both NULL, or for the backward pass: out2 (total_q, num_heads, head_dim) `dtype` holds
  *     P2 v, lse fp32 (2, num_heads, total_q) the maps' log2-sum-exps
@@ -349,12 +349,11 @@ int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k
                        int64_t ld_q, int64_t ld_k, int64_t ld_v, const float* lambda,
                        const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv, int32_t B,
                        int64_t total_q, int64_t total_kv, int32_t num_heads, int32_t head_dim,
-                       float scale, int32_t max_seqlen_q, int32_t zero_rest, void* workspace,
-                       void* out, void* out2, float* lse);
+                       float scale, int32_t max_seqlen_q, int32_t max_seqlen_kv, int32_t zero_rest,
+                       void* workspace, void* out, void* out2, float* lse);
 /* Its gradient from dout (total_q, num_heads, head_dim) and what the forward call was given and
  * wrote: dq (total_q, ...), dk and dv (total_kv, num_heads, head_dim) `dtype`, dlambda fp32
- * (num_heads) or NULL.  max_seqlen_kv sizes a grid as max_seqlen_q does; zero_rest is about rows of
- * dq, dk and dv.  workspace with backward = 1.  The gradients must not overlap an input.  The sums
+ * (num_heads) or NULL.  zero_rest is about rows of dq, dk and dv.  workspace with backward = 1.  The gradients must not overlap an input.  The sums
  * have one fixed order. */
 int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k,
                                 const void* v, int64_t ld_q, int64_t ld_k, int64_t ld_v,

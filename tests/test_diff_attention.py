@@ -52,7 +52,7 @@ def test_c_entry_points_without_a_gpu(pkg):
                 (0, 1, 1, 1, 1, 64, 1, -1, 0)):
         assert ws(*bad) == -1 and lib.tsc_last_error(), bad
     st = lib.tsc_diff_attention(None, 0, P(16), P(16), P(16), 64, 64, 64, P(16), P(16), P(16), 1, 1, 1,
-                                1, 64, 0.0, 1, 0, None, P(16), None, None)
+                                1, 64, 0.0, 1, 1, 0, None, P(16), None, None)
     assert st == 1 and b"null context" in lib.tsc_last_error()
     st = lib.tsc_diff_attention_backward(None, 0, P(16), P(16), P(16), 64, 64, 64, P(16), P(16), P(16),
                                          1, 1, 1, 1, 64, 0.0, 1, 1, 0, P(16), P(16), P(16), P(16),

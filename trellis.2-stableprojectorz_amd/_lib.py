@@ -90,7 +90,7 @@ _SIGNATURES = {
     "tsc_diff_attention_workspace_bytes": (_I64, [_I32, _I32, _I64, _I64, _I32, _I32, _I32, _I32,
                                                   _I32]),
     "tsc_diff_attention": (_I32, [_P, _I32, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _I32, _I64,
-                                  _I64, _I32, _I32, _F32, _I32, _I32, _P, _P, _P, _P]),
+                                  _I64, _I32, _I32, _F32, _I32, _I32, _I32, _P, _P, _P, _P]),
     "tsc_diff_attention_backward": (_I32, [_P, _I32, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _I32,
                                            _I64, _I64, _I32, _I32, _F32, _I32, _I32, _I32, _P, _P,
                                            _P, _P, _P, _P, _P, _P, _P]),

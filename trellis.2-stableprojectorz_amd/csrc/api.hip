@@ -794,7 +794,7 @@ int64_t tsc_diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t tot
                           0, 0, 0, nullptr, nullptr, nullptr, B, total_q, total_kv, num_heads,
                           head_dim, 0.f, max_seqlen_q, max_seqlen_kv, 0, &x))
     return -1;
-  return diff_attention_workspace_bytes(B, total_q, total_kv, num_heads, head_dim, max_seqlen_q,
+  return diff_attention_workspace_bytes(dtype, B, total_q, total_kv, num_heads, head_dim, max_seqlen_q,
                                         max_seqlen_kv, backward);
 }
 
@@ -802,22 +802,22 @@ int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k
                        int64_t ld_q, int64_t ld_k, int64_t ld_v, const float* lambda,
                        const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv, int32_t B,
                        int64_t total_q, int64_t total_kv, int32_t num_heads, int32_t head_dim,
-                       float scale, int32_t max_seqlen_q, int32_t zero_rest, void* workspace,
-                       void* out, void* out2, float* lse) {
+                       float scale, int32_t max_seqlen_q, int32_t max_seqlen_kv, int32_t zero_rest,
+                       void* workspace, void* out, void* out2, float* lse) {
   g_err[0] = 0;
   int st = check_ctx(ctx);
   if (st) return st;
   DiffAttnArgs x;
   st = diff_attention_args(ctx, "diff_attention", dtype, q, k, v, ld_q, ld_k, ld_v, lambda,
                            cu_seqlens_q, cu_seqlens_kv, B, total_q, total_kv, num_heads, head_dim,
-                           scale, max_seqlen_q, 0, zero_rest, &x);
+                           scale, max_seqlen_q, max_seqlen_kv, zero_rest, &x);
   if (st) return st;
   if (B == 0 || total_q == 0) return TSC_OK;
   if (!out) return fail(TSC_ERR_INVALID, "diff_attention: null buffer");
   if ((out2 == nullptr) != (lse == nullptr))
     return fail(TSC_ERR_INVALID, "diff_attention: out2 and lse go together");
-  const int64_t need = diff_attention_workspace_bytes(B, total_q, total_kv, num_heads, head_dim,
-                                                      max_seqlen_q, 0, 0);
+  const int64_t need = diff_attention_workspace_bytes(dtype, B, total_q, total_kv, num_heads, head_dim,
+                                                      max_seqlen_q, max_seqlen_kv, 0);
   if (need > 0 && !workspace) return fail(TSC_ERR_INVALID, "diff_attention: null workspace");
   if (!aligned(out, 16) || !aligned(out2, 16) || !aligned(lse, 4) || !aligned(workspace, 16))
     return fail(TSC_ERR_INVALID, "diff_attention: out, out2 and workspace must be 16-byte aligned");

@@ -139,19 +139,26 @@ struct Stage {
   static constexpr int NL = ROWS * Ti::CPR / NT;
   static_assert(NL >= 1 && NL * NT == ROWS * Ti::CPR, "tile shape");
   u32x4_t r[NL];
-  // Rows first .. first + ROWS - 1 of base (row stride ld elements); zeros from row `end` on.
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int first, int end) {
+  int last;  // the last row of the tile that there is
+  // Rows first .. first + ROWS - 1 of base (row stride ld elements); nothing if first >= end.
+  // No lane branches: rows from `end` on repeat the last one, and are cleared on their way into LDS (at
+  // the load the compiler would wait for it to do so).
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int first, int end, int tid) {
+    if (first >= end) return;
+    const uint32_t rb = (uint32_t)ld * sizeof(T);
+    const char* p = (const char*)base + (int64_t)first * rb;
+    last = min(end - 1 - first, ROWS - 1);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int id = threadIdx.x + NT * i, row = first + id / Ti::CPR, c = id % Ti::CPR;
-      r[i] = u32x4_t{0, 0, 0, 0};
-      if (row < end) r[i] = *(const u32x4_t*)((const char*)(base + (int64_t)row * ld) + 16 * c);
+      const int id = tid + NT * i;
+      r[i] = *(const u32x4_t*)(p + ((uint32_t)min(id / Ti::CPR, last) * rb + 16u * (id % Ti::CPR)));
     }
   }
-  __device__ __forceinline__ void store(unsigned char* t) const {
+  __device__ __forceinline__ void store(unsigned char* t, int tid) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int id = threadIdx.x + NT * i;
+      const int id = tid + NT * i;
+      if (id / Ti::CPR > last) r[i] = u32x4_t{0, 0, 0, 0};
       Ti::put(t, id / Ti::CPR, id % Ti::CPR, r[i]);
     }
   }
@@ -211,9 +218,8 @@ struct DaArgs {
   // forward
   void *out, *out2;  // out2 = P2 v, or null
   float* lse;        // (2, H, total_q): log2 of the sum of 2^(score sl2), or null
-  int32_t splits;    // parts of the keys, each of its own block
-  float* part;       // splits > 1: (splits, total_q, H, 2, D) weighted sums, then
-                     // (splits, total_q, H, 2, 2) maxima (times sl2) and denominators
+  int32_t splits, part_keys;  // small grids: blocks that share a sequence's keys, keys of each
+  float* part;       // splits > 1: (splits, total_q, H, 2, D) sums, then (splits, total_q, H, 2, 4)
   // backward
   const void* dout;
   const float* r12;  // (2, H, total_q)
@@ -227,12 +233,110 @@ struct DaArgs {
 constexpr int kNT = 256;  // 4 waves of 32 queries (or keys, in dk / dv)
 constexpr int kBQ = 128;
 
+// Small grids share a sequence's keys out over a.splits blocks.  Keys of a part of a sequence: more than
+// part_keys where the splits would not reach over it.
+__device__ __forceinline__ int64_t part_of(const DaArgs& a, int kv_len) {
+  return max((int64_t)a.part_keys, ((int64_t)(kv_len + a.splits - 1) / a.splits + 63) / 64 * 64);
+}
+// Narrows a sequence's keys to those of part sp.
+__device__ __forceinline__ void take_part(const DaArgs& a, int sp, int* kv0, int* kv_len) {
+  const int64_t per = part_of(a, *kv_len);
+  const int lo = (int)min(per * sp, (int64_t)*kv_len);
+  *kv0 += lo;
+  *kv_len = (int)min(per, (int64_t)(*kv_len - lo));
+}
+// Where part sp of a.part has map i of (row, head) number at: D weighted sums, and the maximum (times
+// sl2), the denominator and the sum of the unrounded probabilities.
+__device__ __forceinline__ float* part_sums(const DaArgs& a, int sp, int64_t at, int i, int D) {
+  return a.part + (((int64_t)sp * a.total_q * a.H + at) * 2 + i) * D;
+}
+__device__ __forceinline__ float4* part_stat(const DaArgs& a, int sp, int64_t at, int i, int D) {
+  return (float4*)part_sums(a, a.splits, 0, 0, D) + ((int64_t)sp * a.total_q * a.H + at) * 2 + i;
+}
+
+// One 32-key step of both maps for a wave's 32 queries: k and v in LDS rows r0 .. r0 + 31, the keys
+// k0 .. of which those below k_hi count.
 template <typename T, int D>
-__global__ void __launch_bounds__(kNT) da_forward_kernel(const DaArgs a) {
+__device__ __forceinline__ void forward_step(const unsigned char* kt, const unsigned char* vt, int r0,
+                                             int lane, int k0, int k_hi, float sl2,
+                                             const typename Frag<T>::type (&qf)[D / 16],
+                                             float (&m)[2], float (&l)[2],
+                                             f32x16_t (&o)[2][D / 32]) {
   typedef Frag<T> F;
   typedef typename F::type Fr;
   typedef Tile<T, D> Ti;
-  constexpr int BK = sizeof(T) == 2 ? 64 : 32;
+  constexpr int KS = D / 16, MT = D / 32;
+  const int l32 = lane & 31, hf = lane >> 5;
+  Fr pf[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f32x16_t s;
+    clear(s);
+#pragma unroll
+    for (int st = i * KS / 2; st < (i + 1) * KS / 2; ++st)
+      F::mma(Ti::row(kt, r0, l32, hf, st), qf[st], s);
+    if (k0 + 32 > k_hi)  // uniform
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (k0 + 8 * (j >> 2) + 4 * hf + (j & 3) >= k_hi) s[j] = -INFINITY;
+    float mx = s[0], p[16];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
+    mx = pair_max(mx) * sl2;
+    if (__builtin_amdgcn_ballot_w64(mx > m[i])) {
+      const float mn = fmaxf(m[i], mx), f = fast_exp2(m[i] - mn);
+      m[i] = mn;
+      l[i] *= f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][mt][j] *= f;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      p[j] = fast_exp2(fmaf(s[j], sl2, -m[i]));
+      l[i] += p[j];
+    }
+    pf[i][0] = F::pack(p);
+    pf[i][1] = F::pack(p + 8);
+  }
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const Fr vf = Ti::col(vt, r0, lane, g, mt);
+      F::mma(vf, pf[0][g], o[0][mt]);
+      F::mma(vf, pf[1][g], o[1][mt]);
+    }
+}
+
+// Writes a wave's finished rows: qi the lane's query of q_len, l summed over both halves.
+template <typename T, int D>
+__device__ __forceinline__ void forward_store(const DaArgs& a, int h, int64_t row, int hf, bool keys,
+                                              const float (&m)[2], const float (&l)[2],
+                                              f32x16_t (&o)[2][D / 32]) {
+  const float i1 = keys ? 1.f / l[0] : 0.f, i2 = keys ? 1.f / l[1] : 0.f, f2 = a.lambda[h] * i2;
+  const int64_t at = (row * a.H + h) * D;
+#pragma unroll
+  for (int mt = 0; mt < D / 32; ++mt) {
+    if (a.out2) store_dims((T*)a.out2 + at + 32 * mt, hf, o[1][mt], i2);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[0][mt][j] = fmaf(-f2, o[1][mt][j], o[0][mt][j] * i1);
+    store_dims((T*)a.out + at + 32 * mt, hf, o[0][mt], 1.f);
+  }
+  if (a.lse && hf == 0) {
+    a.lse[(int64_t)h * a.total_q + row] = keys ? m[0] + log2f(l[0]) : INFINITY;
+    a.lse[(int64_t)(a.H + h) * a.total_q + row] = keys ? m[1] + log2f(l[1]) : INFINITY;
+  }
+}
+
+// fp32, whole sequences: a block of 4 waves owns 128 queries and walks the keys in tiles of 32.
+template <int D>
+__global__ void __launch_bounds__(kNT) da_forward32_kernel(const DaArgs a) {
+  typedef float T;
+  typedef Frag<T> F;
+  typedef Tile<T, D> Ti;
+  constexpr int BK = 32;
   constexpr int KS = D / 16, MT = D / 32;
   __shared__ __attribute__((aligned(16))) unsigned char kt[BK * Ti::ROWB], vt[BK * Ti::ROWB];
   int bx, h, bb;
@@ -240,124 +344,175 @@ __global__ void __launch_bounds__(kNT) da_forward_kernel(const DaArgs a) {
   int q0, q_len, kv0, kv_len;
   segment(a.cu_q, bb, a.total_q, &q0, &q_len);
   segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l32 = lane & 31, hf = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l32 = lane & 31, hf = lane >> 5;
+  if (a.rest) {
+    zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
+    if (a.out2) zero_rest((T*)a.out2, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
+  }
+  const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
+  const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
+
+  for (int qt = bx * kBQ; qt < q_len; qt += gridDim.x * kBQ) {
+    const int qi = qt + w * 32 + l32;
+    typename F::type qf[KS];
+    {
+      const T* p = (const T*)a.q + (int64_t)(q0 + min(qi, q_len - 1)) * a.ldq + (int64_t)h * D + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) qf[st] = F::load(p + 16 * st);
+    }
+    float m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {0.f, 0.f};  // a finite start: a tile of scores of -inf
+    f32x16_t o[2][MT];                                     // then adds nothing
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      clear(o[0][mt]);
+      clear(o[1][mt]);
+    }
+    Stage<T, D, BK, kNT> ks, vs;
+    ks.load(kbase, a.ldk, 0, kv_len, tid);
+    vs.load(vbase, a.ldv, 0, kv_len, tid);
+    for (int kb = 0; kb < kv_len; kb += BK) {
+      __syncthreads();
+      ks.store(kt, tid);
+      vs.store(vt, tid);
+      __syncthreads();
+      ks.load(kbase, a.ldk, kb + BK, kv_len, tid);
+      vs.load(vbase, a.ldv, kb + BK, kv_len, tid);
+      forward_step<T, D>(kt, vt, 0, lane, kb, kv_len, a.sl2, qf, m, l, o);
+    }
+    l[0] = pair_sum(l[0]);
+    l[1] = pair_sum(l[1]);
+    if (qi < q_len) forward_store<T, D>(a, h, q0 + qi, hf, kv_len > 0, m, l, o);
+  }
+}
+
+// fp32, small grids: a block owns 32 queries, and its waves and the blocks of a.splits
+// parts share out the keys, 32 at a time.  Each wave brings its own keys through its own piece of LDS,
+// so none waits for another until the end, where their maxima, denominators and sums are joined.
+template <int D>
+__global__ void __launch_bounds__(kNT) da_few32_kernel(const DaArgs a) {
+  typedef float T;
+  typedef Frag<T> F;
+  typedef Tile<T, D> Ti;
+  constexpr int KS = D / 16, MT = D / 32, NW = kNT / 64;
+  constexpr int TB = 32 * Ti::ROWB;  // bytes of a tile
+  __shared__ __attribute__((aligned(16))) unsigned char lds[NW][2 * TB];
+  __shared__ float sm[NW][2][32], sl[NW][2][32];
+  static_assert(2 * 32 * D * 4 <= 4 * TB, "a wave's sums fit into two waves' tiles");
+  int bx, h, bb;
+  block_tile(a.cu_kv, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: its keys are scalars
   const int sp = bx % a.splits, tile = bx / a.splits, tiles = gridDim.x / a.splits;
   if (a.rest && sp == 0) {
     zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, tile, tiles);
     if (a.out2) zero_rest((T*)a.out2, a.cu_q, a.total_q, bb, a.H, D, h, tile, tiles);
   }
+  if (a.splits > 1) {
+    take_part(a, sp, &kv0, &kv_len);
+    if (kv_len == 0) return;  // the join passes over it
+  }
   const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
   const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
-  const int per = ((kv_len + a.splits - 1) / a.splits + BK - 1) / BK * BK;
-  const int k_lo = min((int64_t)per * sp, (int64_t)kv_len), k_hi = min(k_lo + per, kv_len);
-  const float lam = a.lambda[h];
+  unsigned char *kt = lds[w], *vt = lds[w] + TB;
 
-  for (int qt = tile * kBQ; qt < q_len; qt += tiles * kBQ) {
-    const int qi = qt + w * 32 + l32;
-    const int64_t qrow = q0 + min(qi, q_len - 1);
-    Fr qf[KS];
+  for (int qt = tile * 32; qt < q_len; qt += tiles * 32) {
+    const int qi = qt + l32;
+    typename F::type qf[KS];
     {
-      const T* p = (const T*)a.q + qrow * a.ldq + (int64_t)h * D + 8 * hf;
+      const T* p = (const T*)a.q + (int64_t)(q0 + min(qi, q_len - 1)) * a.ldq + (int64_t)h * D + 8 * hf;
 #pragma unroll
       for (int st = 0; st < KS; ++st) qf[st] = F::load(p + 16 * st);
     }
-    float m[2], l[2];  // the maximum starts finite: a tile of scores of -inf then adds nothing
+    float m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {0.f, 0.f};
     f32x16_t o[2][MT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      m[i] = -FLT_MAX;
-      l[i] = 0.f;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) clear(o[i][mt]);
+    for (int mt = 0; mt < MT; ++mt) {
+      clear(o[0][mt]);
+      clear(o[1][mt]);
     }
-    Stage<T, D, BK, kNT> ks, vs;
-    ks.load(kbase, a.ldk, k_lo, k_hi);
-    vs.load(vbase, a.ldv, k_lo, k_hi);
-    for (int kb = k_lo; kb < k_hi; kb += BK) {
-      __syncthreads();
-      ks.store(kt);
-      vs.store(vt);
-      __syncthreads();
-      ks.load(kbase, a.ldk, kb + BK, k_hi);
-      vs.load(vbase, a.ldv, kb + BK, k_hi);
+    // The next keys come in during a step, but at D = 128: no registers are left to hold them, and a
+    // step there takes ten times as long as they do.
+    constexpr bool AHEAD = D == 64;
+    Stage<T, D, 32, 64> ks, vs;
+    int k0 = 32 * w;
+    auto load = [&](int k) {
+      ks.load(kbase, a.ldk, k, kv_len, lane);
+      vs.load(vbase, a.ldv, k, kv_len, lane);
+    };
+    if (AHEAD) load(k0);
+    for (; k0 < kv_len; k0 += 32 * NW) {
+      if (!AHEAD) load(k0);
+      // A wave's LDS operations are carried out in order; the compiler has to keep that order.
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      ks.store(kt, lane);
+      vs.store(vt, lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (AHEAD) load(k0 + 32 * NW);
+      forward_step<T, D>(kt, vt, 0, lane, k0, kv_len, a.sl2, qf, m, l, o);
+    }
 #pragma unroll
-      for (int sub = 0; sub < BK; sub += 32) {
-        const int k0 = kb + sub;
-        if (k0 >= k_hi) break;
-        Fr pf[2][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          f32x16_t s;
-          clear(s);
-#pragma unroll
-          for (int st = i * KS / 2; st < (i + 1) * KS / 2; ++st) F::mma(Ti::row(kt, sub, l32, hf, st), qf[st], s);
-          float mx = -INFINITY, p[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (k0 + 8 * (j >> 2) + 4 * hf + (j & 3) >= k_hi) s[j] = -INFINITY;
-            mx = fmaxf(mx, s[j]);
-          }
-          mx = pair_max(mx) * a.sl2;
-          if (__builtin_amdgcn_ballot_w64(mx > m[i])) {
-            const float mn = fmaxf(m[i], mx), f = fast_exp2(m[i] - mn);
-            m[i] = mn;
-            l[i] *= f;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int j = 0; j < 16; ++j) o[i][mt][j] *= f;
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            p[j] = fast_exp2(fmaf(s[j], a.sl2, -m[i]));
-            l[i] += p[j];
-          }
-          pf[i][0] = F::pack(p);
-          pf[i][1] = F::pack(p + 8);
-        }
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            const Fr vf = Ti::col(vt, sub, lane, g, mt);
-            F::mma(vf, pf[0][g], o[0][mt]);
-            F::mma(vf, pf[1][g], o[1][mt]);
-          }
+    for (int i = 0; i < 2; ++i) {
+      l[i] = pair_sum(l[i]);
+      if (hf == 0) {
+        sm[w][i][l32] = m[i];
+        sl[w][i][l32] = l[i];
       }
     }
-    l[0] = pair_sum(l[0]);
-    l[1] = pair_sum(l[1]);
-    if (qi < q_len) {
+    __syncthreads();  // every wave has left its tiles
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float own = m[i];
+      m[i] = sm[0][i][l32];
+#pragma unroll
+      for (int x = 1; x < NW; ++x) m[i] = fmaxf(m[i], sm[x][i][l32]);
+      l[i] = 0.f;
+#pragma unroll
+      for (int x = 0; x < NW; ++x) l[i] = fmaf(sl[x][i][l32], fast_exp2(sm[x][i][l32] - m[i]), l[i]);
+      const float f = fast_exp2(own - m[i]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][mt][j] *= f;
+    }
+#pragma unroll
+    for (int half = NW / 2; half > 0; half >>= 1) {  // waves half .. 2 half - 1 hand theirs on
+      float* meet = (float*)lds[0] + (w % half) * 2 * 32 * D + lane;
+      if (w >= half && w < 2 * half)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) meet[((i * MT + mt) * 16 + j) * 64] = o[i][mt][j];
+      __syncthreads();
+      if (w < half)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[i][mt][j] += meet[((i * MT + mt) * 16 + j) * 64];
+      __syncthreads();
+    }
+    if (w != 0 || qi >= q_len) continue;
+    if (a.splits == 1) {
+      forward_store<T, D>(a, h, q0 + qi, hf, kv_len > 0, m, l, o);
+    } else {
       const int64_t at = (int64_t)(q0 + qi) * a.H + h;
-      if (a.splits > 1) {
-        const int64_t rows = a.total_q * a.H;
-        float* po = a.part + ((int64_t)sp * rows + at) * 2 * D;
-        float* ps = a.part + (int64_t)a.splits * rows * 2 * D + ((int64_t)sp * rows + at) * 4;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) store_dims(po + i * D + 32 * mt, hf, o[i][mt], 1.f);
-          if (hf == 0) *(float2*)(ps + 2 * i) = make_float2(m[i], l[i]);
-        }
-      } else {
-        const float i1 = kv_len ? 1.f / l[0] : 0.f, i2 = kv_len ? 1.f / l[1] : 0.f, f2 = lam * i2;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          if (a.out2) store_dims((T*)a.out2 + at * D + 32 * mt, hf, o[1][mt], i2);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) o[0][mt][j] = fmaf(-f2, o[1][mt][j], o[0][mt][j] * i1);
-          store_dims((T*)a.out + at * D + 32 * mt, hf, o[0][mt], 1.f);
-        }
-        if (a.lse && hf == 0) {
-          a.lse[(int64_t)h * a.total_q + q0 + qi] = kv_len ? m[0] + log2f(l[0]) : INFINITY;
-          a.lse[(int64_t)(a.H + h) * a.total_q + q0 + qi] = kv_len ? m[1] + log2f(l[1]) : INFINITY;
-        }
+        for (int mt = 0; mt < MT; ++mt) store_dims(part_sums(a, sp, at, i, D) + 32 * mt, hf, o[i][mt], 1.f);
+        if (hf == 0) *part_stat(a, sp, at, i, D) = make_float4(m[i], l[i], l[i], 0.f);
       }
     }
   }
 }
 
-// 16 bits, whole sequences: the two maps' softmax beside the matrix products.  As in attention.hip's
+// 16 bits: the two maps' softmax beside the matrix products.  As in attention.hip's
 // kernel of this kind a step of 32 keys has two phases, pinned in program order:
 //   A  the next step's scores (matrix) beside the rest of this step's exponentials (VALU) and the
 //      transposed reads of v
@@ -387,20 +542,27 @@ __global__ void __launch_bounds__(64 * NW, 2) da_forward16_kernel(const DaArgs a
   int q0, q_len, kv0, kv_len;
   segment(a.cu_q, bb, a.total_q, &q0, &q_len);
   segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
-  if (a.rest) {
-    zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
-    if (a.out2) zero_rest((T*)a.out2, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
+  const int sp = bx % a.splits, qtile = bx / a.splits, qtiles = gridDim.x / a.splits;
+  if (a.rest && sp == 0) {
+    zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, qtile, qtiles);
+    if (a.out2) zero_rest((T*)a.out2, a.cu_q, a.total_q, bb, a.H, D, h, qtile, qtiles);
+  }
+  if (a.splits > 1) {
+    take_part(a, sp, &kv0, &kv_len);
+    if (kv_len == 0) return;  // the join passes over it
   }
   const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
   const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
   const float sl2 = a.sl2;
 
-  for (int qt = bx * BQ; qt < q_len; qt += gridDim.x * BQ) {
+  for (int qt = qtile * BQ; qt < q_len; qt += qtiles * BQ) {
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // nothing derived from it is kept across q tiles
     const int lane = tid & 63, w = tid >> 6, l32 = lane & 31, hf = lane >> 5;
-    const int map = NM == 2 ? 0 : w / QW, tile = w % QW;  // the wave's first map
+    const int map = NM == 2 ? 0 : w & 1, tile = NM == 2 ? w : w >> 1;  // the wave's first map
     const int qi = qt + tile * 32 + l32;
+    // A wave without queries brings its share of the keys and does no more.
+    const bool idle = __builtin_amdgcn_readfirstlane(qt + tile * 32) >= q_len;
     const int64_t at = (int64_t)(q0 + qi) * a.H + h;
     if (kv_len == 0) {  // uniform over the block
       if (map == 0 && qi < q_len) {
@@ -577,6 +739,18 @@ __global__ void __launch_bounds__(64 * NW, 2) da_forward16_kernel(const DaArgs a
       store(0, 1, Y, 0);
     }
     __syncthreads();
+    if (idle) {  // the same copies and barriers
+      __syncthreads();
+      for (int jb = 0; jb * BK < kv_len; ++jb) {
+        load(vbase, vst, jb * BK + BK, vr);
+        load(kbase, kst, jb * BK + 2 * BK, kr);
+        store(~jb & 1, jb & 1, Y, jb * BK + BK);
+        __syncthreads();
+      }
+      if (NM == 1 && a.splits == 1) __syncthreads();
+      if (a.splits == 1) __syncthreads();
+      continue;
+    }
 #pragma unroll
     for (int st = 0; st < KS; ++st) read_k(0, 0, st);
 #pragma unroll
@@ -607,6 +781,20 @@ __global__ void __launch_bounds__(64 * NW, 2) da_forward16_kernel(const DaArgs a
     const int nfull = max(0, kv_len / BK - 1), nblk = (kv_len + BK - 1) / BK;
     for (; jb < nfull; ++jb) block(N);
     for (; jb < nblk; ++jb) block(Y);
+    if (a.splits > 1) {
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        l[i] = pair_sum(l[i]);
+        lu[i] = pair_sum(lu[i]);
+        if (qi < q_len) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            store_dims(part_sums(a, sp, at, map + i, D) + 32 * mt, hf, o[i][mt], 1.f);
+          if (hf == 0) *part_stat(a, sp, at, map + i, D) = make_float4(mc[i], l[i], lu[i], 0.f);
+        }
+      }
+      continue;  // the last block of keys ended with a barrier
+    }
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
       const float inv = 1.f / pair_sum(l[i]);
@@ -653,43 +841,45 @@ __global__ void __launch_bounds__(64 * NW, 2) da_forward16_kernel(const DaArgs a
 // Joins the parts of the keys: one wave for a (query, head), D / 64 dims a lane.
 template <typename T, int D>
 __global__ void __launch_bounds__(kNT) da_join_kernel(const DaArgs a, int32_t B) {
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = a.total_q * a.H;
-  if (at >= rows) return;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= a.total_q * a.H) return;
   const int lane = threadIdx.x & 63, h = (int)(at % a.H);
   const int64_t row = at / a.H;
-  // The sequence of the row, and whether it has keys.
-  bool in = false, keys = false;
+  // The sequence of the row, and its keys.
+  bool in = false;
+  int kv_len = 0;
   for (int b = lane; b < B; b += 64) {
     int q0, ql, k0, kl;
     segment(a.cu_q, b, a.total_q, &q0, &ql);
+    segment(a.cu_kv, b, a.total_kv, &k0, &kl);
     if (row >= q0 && row < (int64_t)q0 + ql) {
-      segment(a.cu_kv, b, a.total_kv, &k0, &kl);
       in = true;
-      keys = kl > 0;
+      kv_len = kl;
     }
   }
-  if (__builtin_amdgcn_ballot_w64(in) == 0) return;
-  keys = __builtin_amdgcn_ballot_w64(keys) != 0;
-  const float* ps = a.part + (int64_t)a.splits * rows * 2 * D;
-  float m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {0.f, 0.f};
-  float o[2][D / 64] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float4 st = *(const float4*)(ps + ((int64_t)s * rows + at) * 4);
-    const float sm[2] = {st.x, st.z}, sl[2] = {st.y, st.w};
-    const float* po = a.part + ((int64_t)s * rows + at) * 2 * D;
+  const uint64_t who = __builtin_amdgcn_ballot_w64(in);
+  if (who == 0) return;
+  kv_len = __shfl(kv_len, __builtin_ctzll(who), 64);
+  const int64_t per = part_of(a, kv_len);
+  const int parts = (int)((kv_len + per - 1) / per);
+  float m[2], l[2] = {0.f, 0.f}, lu[2] = {0.f, 0.f}, o[2][D / 64] = {};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (!(sl[i] != 0.f)) continue;  // a part without keys
-      const float mn = fmaxf(m[i], sm[i]);
-      const float f = fast_exp2(m[i] - mn), g = fast_exp2(sm[i] - mn);
-      m[i] = mn;
-      l[i] = l[i] * f + sl[i] * g;
+  for (int i = 0; i < 2; ++i) {
+    m[i] = -FLT_MAX;
+    for (int p = lane; p < parts; p += 64) m[i] = fmaxf(m[i], part_stat(a, p, at, i, D)->x);
+    for (int off = 32; off > 0; off >>= 1) m[i] = fmaxf(m[i], __shfl_xor(m[i], off, 64));
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {  // independent loads, one order of the sums
+      const float4 st = *part_stat(a, p, at, i, D);
+      const float* po = part_sums(a, p, at, i, D);
+      const float f = fast_exp2(st.x - m[i]);
+      l[i] = fmaf(st.y, f, l[i]);
+      lu[i] = fmaf(st.z, f, lu[i]);
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e)
-        o[i][e] = o[i][e] * f + po[i * D + lane + 64 * e] * g;
+      for (int e = 0; e < D / 64; ++e) o[i][e] = fmaf(po[lane + 64 * e], f, o[i][e]);
     }
   }
-  const float i1 = keys ? 1.f / l[0] : 0.f, i2 = keys ? 1.f / l[1] : 0.f, lam = a.lambda[h];
+  const float i1 = parts ? 1.f / l[0] : 0.f, i2 = parts ? 1.f / l[1] : 0.f, lam = a.lambda[h];
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) {
     const int64_t p = at * D + lane + 64 * e;
@@ -697,8 +887,8 @@ __global__ void __launch_bounds__(kNT) da_join_kernel(const DaArgs a, int32_t B)
     if (a.out2) ((T*)a.out2)[p] = (T)(o[1][e] * i2);
   }
   if (a.lse && lane == 0) {
-    a.lse[(int64_t)h * a.total_q + row] = keys ? m[0] + log2f(l[0]) : INFINITY;
-    a.lse[(int64_t)(a.H + h) * a.total_q + row] = keys ? m[1] + log2f(l[1]) : INFINITY;
+    a.lse[(int64_t)h * a.total_q + row] = parts ? m[0] + log2f(lu[0]) : INFINITY;
+    a.lse[(int64_t)(a.H + h) * a.total_q + row] = parts ? m[1] + log2f(lu[1]) : INFINITY;
   }
 }
 
@@ -754,7 +944,7 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
   int q0, q_len, kv0, kv_len;
   segment(a.cu_q, bb, a.total_q, &q0, &q_len);
   segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l32 = lane & 31, hf = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l32 = lane & 31, hf = lane >> 5;
   if (a.rest) zero_rest((T*)a.dq, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
   if (bx == 0 && bb == 0 && w == 0 && a.dlambda) {
     double s = 0.;
@@ -785,15 +975,15 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) clear(acc[mt]);
     Stage<T, D, BK, kNT> ks, vs;
-    ks.load(kbase, a.ldk, 0, kv_len);
-    vs.load(vbase, a.ldv, 0, kv_len);
+    ks.load(kbase, a.ldk, 0, kv_len, tid);
+    vs.load(vbase, a.ldv, 0, kv_len, tid);
     for (int kb = 0; kb < kv_len; kb += BK) {
       __syncthreads();
-      ks.store(kt);
-      vs.store(vt);
+      ks.store(kt, tid);
+      vs.store(vt, tid);
       __syncthreads();
-      ks.load(kbase, a.ldk, kb + BK, kv_len);
-      vs.load(vbase, a.ldv, kb + BK, kv_len);
+      ks.load(kbase, a.ldk, kb + BK, kv_len, tid);
+      vs.load(vbase, a.ldv, kb + BK, kv_len, tid);
       f32x16_t s1, s2, dp;
       clear(s1);
       clear(s2);
@@ -878,8 +1068,8 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
     Stage<T, D, BQ, kNT> qs, ds;
     float sv = 0.f;
     auto load = [&](int qb) {
-      qs.load(qbase, a.ldq, qb, q_len);
-      ds.load(dbase, ldd, qb, q_len);
+      qs.load(qbase, a.ldq, qb, q_len, tid);
+      ds.load(dbase, ldd, qb, q_len, tid);
       if (tid < 128) {  // past the last query: P = 2^(0 - inf) = 0
         const int r = qb + (tid & 31);
         sv = r < q_len ? sbase[r] : tid < 64 ? INFINITY : 0.f;
@@ -888,8 +1078,8 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
     load(0);
     for (int qb = 0; qb < q_len; qb += BQ) {
       __syncthreads();
-      qs.store(qt);
-      ds.store(dt);
+      qs.store(qt, tid);
+      ds.store(dt, tid);
       if (tid < 128) st4[tid >> 5][tid & 31] = sv;
       __syncthreads();
       load(qb + BQ);
@@ -944,17 +1134,36 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
 }
 
 // ------------------------------------------------------------------------------- host
+constexpr int64_t kCUs = 256;
+
 // Tiles of 128 rows that the grid gives a sequence; the kernels' loops cover longer ones.
 unsigned tiles_of(int64_t longest, int64_t hb) {
   return (unsigned)std::max<int64_t>(
       1, std::min<int64_t>(std::min<int64_t>((longest + kBQ - 1) / kBQ, 65535), (INT32_MAX / 16) / hb));
 }
 
-// Parts of the keys: where the query tiles leave CUs idle and there are keys to share.
-int da_splits(int32_t B, int64_t total_kv, int32_t H, int64_t max_q) {
-  const int64_t blocks = (int64_t)tiles_of(max_q, (int64_t)H * B) * H * B;
-  const int64_t keys = total_kv / B;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, keys / 256, 64}));
+// The forward pass' blocks: query rows of each, and the parts of the keys.
+struct Plan {
+  int rows, splits, part_keys;
+};
+Plan da_plan(int32_t dtype, int32_t B, int64_t total_kv, int32_t H, int64_t max_q, int64_t max_kv) {
+  const int64_t hb = (int64_t)H * B;
+  int64_t blocks = std::max<int64_t>(1, (max_q + kBQ - 1) / kBQ) * hb;
+  Plan p = {kBQ, 1, INT32_MAX};
+  if (blocks >= kCUs) return p;
+  if (dtype == TSC_F32) {
+    p.rows = 32;
+    blocks = std::max<int64_t>(1, (max_q + 31) / 32) * hb;
+    if (blocks >= kCUs) return p;
+  }
+  // Parts of one size, so that long sequences get more of them, and no more blocks than CUs: of n a
+  // sequence's query tiles and heads can have sum ceil(keys / part) <= total / part + B.
+  const int64_t n = kCUs / (blocks / B) - B;
+  if (n <= 0) return p;
+  const int64_t part = std::max<int64_t>(dtype == TSC_F32 ? 256 : 512, ((total_kv + n - 1) / n + 63) / 64 * 64);
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((max_kv + part - 1) / part, kCUs));
+  if (p.splits > 1) p.part_keys = (int)std::min<int64_t>(part, INT32_MAX);
+  return p;
 }
 
 // Blocks of the r kernel for a (head, sequence).
@@ -993,13 +1202,13 @@ DaArgs da_args(const DiffAttnArgs& x) {
 
 }  // namespace
 
-int64_t diff_attention_workspace_bytes(int32_t B, int64_t total_q, int64_t total_kv, int32_t H,
+int64_t diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv, int32_t H,
                                        int32_t D, int32_t max_q, int32_t max_kv, int32_t backward) {
   if (B == 0 || total_q == 0) return 0;
   const int64_t hb = (int64_t)H * B;
   if (backward) return 4 * (2 * (int64_t)H * total_q + hb * tiles_of(max_kv, hb));
-  const int s = da_splits(B, total_kv, H, max_q);
-  return s > 1 ? 4 * (int64_t)s * total_q * H * (2 * D + 4) : 0;
+  const int s = da_plan(dtype, B, total_kv, H, max_q, max_kv).splits;
+  return s > 1 ? 4 * (int64_t)s * total_q * H * 2 * (D + 4) : 0;
 }
 
 int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* out2, float* lse,
@@ -1011,23 +1220,26 @@ int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* 
   a.out = out;
   a.out2 = out2;
   a.lse = lse;
-  a.splits = da_splits(x.B, x.total_kv, x.H, x.max_q);
+  const Plan plan = da_plan(x.dtype, x.B, x.total_kv, x.H, x.max_q, x.max_kv);
+  a.splits = plan.splits;
+  a.part_keys = plan.part_keys;
   a.part = (float*)ws;
-  const dim3 grid(tiles_of(x.max_q, hb) * a.splits, (unsigned)x.H, (unsigned)x.B);
+  const bool few = plan.rows == 32;
+  const unsigned gx = (few ? std::max(1, (x.max_q + 31) / 32) : tiles_of(x.max_q, hb)) * a.splits;
+  const dim3 grid(gx, (unsigned)x.H, (unsigned)x.B);
   return by_type(x.dtype, x.D, [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     {
       ProfScope p(ctx, "diff_attention");
-      if constexpr (sizeof(T) == 2) {
-        if (a.splits == 1) {
-          constexpr int NM = D == 64 ? 2 : 1, NW = 8 / NM;
-          if (a.lse) da_forward16_kernel<T, D, NM, NW, true><<<grid, 64 * NW, 0, ctx->stream>>>(a);
-          else da_forward16_kernel<T, D, NM, NW, false><<<grid, 64 * NW, 0, ctx->stream>>>(a);
-          return;
-        }
+      if constexpr (sizeof(T) == 4) {
+        if (few) da_few32_kernel<D><<<grid, kNT, 0, ctx->stream>>>(a);
+        else da_forward32_kernel<D><<<grid, kNT, 0, ctx->stream>>>(a);
+      } else {
+        constexpr int NM = D == 64 ? 2 : 1, NW = 8 / NM;
+        if (a.lse) da_forward16_kernel<T, D, NM, NW, true><<<grid, 64 * NW, 0, ctx->stream>>>(a);
+        else da_forward16_kernel<T, D, NM, NW, false><<<grid, 64 * NW, 0, ctx->stream>>>(a);
       }
-      da_forward_kernel<T, D><<<grid, kNT, 0, ctx->stream>>>(a);
     }
     if (a.splits > 1) {
       ProfScope p(ctx, "diff_attention_join");

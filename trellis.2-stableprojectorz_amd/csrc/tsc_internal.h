@@ -244,8 +244,9 @@ struct DiffAttnArgs {
   int32_t max_q, max_kv;  // longest sequences: they size the grids
   int32_t rest;
 };
-int64_t diff_attention_workspace_bytes(int32_t B, int64_t total_q, int64_t total_kv, int32_t H,
-                                       int32_t D, int32_t max_q, int32_t max_kv, int32_t backward);
+int64_t diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv,
+                                       int32_t H, int32_t D, int32_t max_q, int32_t max_kv,
+                                       int32_t backward);
 int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* out2, float* lse,
                           void* ws);
 int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const void* out,

@@ -622,8 +622,8 @@ def _diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, out, keep):
         ws = _scratch(nbytes, q.device) if nbytes else None
         check(lib.tsc_diff_attention(handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"),
                                      _head_rows(k, "k"), _head_rows(v, "v"), _p(lam), _p(cq), _p(ck), b,
-                                     tq, tkv, h, d, scale, max_q, int(rest), _p(ws), _p(out), _p(out2),
-                                     _p(lse)))
+                                     tq, tkv, h, d, scale, max_q, max_kv, int(rest), _p(ws), _p(out),
+                                     _p(out2), _p(lse)))
     return out, out2, lse
 
 
