@@ -206,6 +206,28 @@ __device__ __forceinline__ void zero_rest(T* p, const int32_t* cu, int64_t total
   }
 }
 
+// Adds up the 4 waves' sums through LDS (2 N x 4 KB at lds, which every wave has left): wave 0 has them.
+template <int N>
+__device__ __forceinline__ void join_waves(float* lds, int w, int lane, f32x16_t (&c)[N]) {
+  __syncthreads();
+#pragma unroll
+  for (int half = 2; half > 0; half >>= 1) {  // waves half .. 2 half - 1 hand theirs on
+    float* meet = lds + (w % half) * N * 1024 + lane;
+    if (w >= half && w < 2 * half)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) meet[(16 * i + j) * 64] = c[i][j];
+    __syncthreads();
+    if (w < half)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) c[i][j] += meet[(16 * i + j) * 64];
+    __syncthreads();
+  }
+}
+
 struct DaArgs {
   const void *q, *k, *v;
   int64_t ldq, ldk, ldv;
@@ -397,7 +419,6 @@ __global__ void __launch_bounds__(kNT) da_few32_kernel(const DaArgs a) {
   constexpr int TB = 32 * Ti::ROWB;  // bytes of a tile
   __shared__ __attribute__((aligned(16))) unsigned char lds[NW][2 * TB];
   __shared__ float sm[NW][2][32], sl[NW][2][32];
-  static_assert(2 * 32 * D * 4 <= 4 * TB, "a wave's sums fit into two waves' tiles");
   int bx, h, bb;
   block_tile(a.cu_kv, &bx, &h, &bb);
   int q0, q_len, kv0, kv_len;
@@ -477,26 +498,8 @@ __global__ void __launch_bounds__(kNT) da_few32_kernel(const DaArgs a) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[i][mt][j] *= f;
     }
-#pragma unroll
-    for (int half = NW / 2; half > 0; half >>= 1) {  // waves half .. 2 half - 1 hand theirs on
-      float* meet = (float*)lds[0] + (w % half) * 2 * 32 * D + lane;
-      if (w >= half && w < 2 * half)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) meet[((i * MT + mt) * 16 + j) * 64] = o[i][mt][j];
-      __syncthreads();
-      if (w < half)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[i][mt][j] += meet[((i * MT + mt) * 16 + j) * 64];
-      __syncthreads();
-    }
+    join_waves<MT>((float*)lds[0], w, lane, o[0]);
+    join_waves<MT>((float*)lds[0], w, lane, o[1]);
     if (w != 0 || qi >= q_len) continue;
     if (a.splits == 1) {
       forward_store<T, D>(a, h, q0 + qi, hf, kv_len > 0, m, l, o);
@@ -930,21 +933,34 @@ __global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r
   }
 }
 
-// dq of 128 queries; one block of each head also adds up dlambda.
-template <typename T, int D>
+// Both gradient kernels: a block's 4 waves own 32 rows each and share the tiles of the other side; or,
+// where that leaves CUs idle (SHARE), all own the same 32 rows and take the tiles in turn, each through
+// its own piece of LDS, and their sums are joined at the end.
+template <bool SHARE>
+__device__ __forceinline__ void tile_sync() {
+  // A wave's own LDS operations are carried out in order; the compiler has to keep that order.
+  if (SHARE) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  else __syncthreads();
+}
+
+// dq of 128 (32) queries; one block of each head also adds up dlambda.
+template <typename T, int D, bool SHARE>
 __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
   typedef Frag<T> F;
   typedef typename F::type Fr;
   typedef Tile<T, D> Ti;
   constexpr int BK = 32;
   constexpr int KS = D / 16, MT = D / 32;
-  __shared__ __attribute__((aligned(16))) unsigned char kt[BK * Ti::ROWB], vt[BK * Ti::ROWB];
+  constexpr int TB = BK * Ti::ROWB, ROWS = SHARE ? 32 : kBQ, NT = SHARE ? 64 : kNT;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[SHARE ? 4 : 1][2 * TB];
   int bx, h, bb;
   block_tile(a.cu_kv, &bx, &h, &bb);
   int q0, q_len, kv0, kv_len;
   segment(a.cu_q, bb, a.total_q, &q0, &q_len);
   segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l32 = lane & 31, hf = lane >> 5;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = SHARE ? lane : threadIdx.x;
+  unsigned char *kt = lds[SHARE ? w : 0], *vt = kt + TB;
   if (a.rest) zero_rest((T*)a.dq, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
   if (bx == 0 && bb == 0 && w == 0 && a.dlambda) {
     double s = 0.;
@@ -956,8 +972,8 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
   const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
   const float nlam = -a.lambda[h], scale = a.sl2 / kLog2e;
 
-  for (int qt = bx * kBQ; qt < q_len; qt += gridDim.x * kBQ) {
-    const int qi = qt + w * 32 + l32;
+  for (int qt = bx * ROWS; qt < q_len; qt += gridDim.x * ROWS) {
+    const int qi = qt + (SHARE ? 0 : w * 32) + l32;
     const int64_t qrow = q0 + min(qi, q_len - 1), stat = (int64_t)h * a.total_q + qrow;
     const int64_t map2 = (int64_t)a.H * a.total_q;
     Fr qf[KS], df[KS];
@@ -974,16 +990,22 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
     f32x16_t acc[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) clear(acc[mt]);
-    Stage<T, D, BK, kNT> ks, vs;
-    ks.load(kbase, a.ldk, 0, kv_len, tid);
-    vs.load(vbase, a.ldv, 0, kv_len, tid);
-    for (int kb = 0; kb < kv_len; kb += BK) {
-      __syncthreads();
+    Stage<T, D, BK, NT> ks, vs;
+    constexpr int STEP = SHARE ? 4 * BK : BK;
+    constexpr bool AHEAD = !SHARE || sizeof(T) == 2 || D == 64;  // registers for the next tile's rows
+    int kb = SHARE ? w * BK : 0;
+    auto load = [&](int k) {
+      ks.load(kbase, a.ldk, k, kv_len, tid);
+      vs.load(vbase, a.ldv, k, kv_len, tid);
+    };
+    if (AHEAD) load(kb);
+    for (; kb < kv_len; kb += STEP) {
+      if (!AHEAD) load(kb);
+      tile_sync<SHARE>();
       ks.store(kt, tid);
       vs.store(vt, tid);
-      __syncthreads();
-      ks.load(kbase, a.ldk, kb + BK, kv_len, tid);
-      vs.load(vbase, a.ldv, kb + BK, kv_len, tid);
+      tile_sync<SHARE>();
+      if (AHEAD) load(kb + STEP);
       f32x16_t s1, s2, dp;
       clear(s1);
       clear(s2);
@@ -1009,7 +1031,8 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
         for (int mt = 0; mt < MT; ++mt)
           F::mma(Ti::col(kt, 0, lane, g, mt), mt < MT / 2 ? f1[g] : f2[g], acc[mt]);
     }
-    if (qi < q_len) {
+    if (SHARE) join_waves<MT>((float*)lds, w, lane, acc);
+    if (qi < q_len && (!SHARE || w == 0)) {
       T* p = (T*)a.dq + ((int64_t)(q0 + qi) * a.H + h) * D;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) store_dims(p + 32 * mt, hf, acc[mt], scale);
@@ -1017,23 +1040,27 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
   }
 }
 
-// dk and dv of 128 keys, and the block's part of dlambda = - sum P2 dP, from the unrounded fp32
+// dk and dv of 128 (32) keys, and the block's part of dlambda = - sum P2 dP, from the unrounded fp32
 // probabilities (do . (P2 v) with P2 v in 16 bits is off by 2^-9 of it).  The sequence ranking of block_tile goes by the queries here.
-template <typename T, int D>
+template <typename T, int D, bool SHARE>
 __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
   typedef Frag<T> F;
   typedef typename F::type Fr;
   typedef Tile<T, D> Ti;
   constexpr int BQ = 32;
   constexpr int KS = D / 16, MT = D / 32;
-  __shared__ __attribute__((aligned(16))) unsigned char qt[BQ * Ti::ROWB], dt[BQ * Ti::ROWB];
-  __shared__ __attribute__((aligned(16))) float st4[4][BQ];  // log-sum-exps and r of the two maps
+  constexpr int TB = BQ * Ti::ROWB, ROWS = SHARE ? 32 : kBQ, NT = SHARE ? 64 : kNT;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[SHARE ? 4 : 1][2 * TB];
+  __shared__ __attribute__((aligned(16))) float stats[SHARE ? 4 : 1][4][BQ];  // log-sum-exps and r
   int bx, h, bb;
   block_tile(a.cu_q, &bx, &h, &bb);
   int q0, q_len, kv0, kv_len;
   segment(a.cu_q, bb, a.total_q, &q0, &q_len);
   segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l32 = lane & 31, hf = lane >> 5;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = SHARE ? lane : threadIdx.x;
+  unsigned char *qt = lds[SHARE ? w : 0], *dt = qt + TB;
+  float(*st4)[BQ] = stats[SHARE ? w : 0];
   if (a.rest) {
     zero_rest((T*)a.dk, a.cu_kv, a.total_kv, bb, a.H, D, h, bx, gridDim.x);
     zero_rest((T*)a.dv, a.cu_kv, a.total_kv, bb, a.H, D, h, bx, gridDim.x);
@@ -1042,12 +1069,12 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
   const T* dbase = (const T*)a.dout + ((int64_t)q0 * a.H + h) * D;
   const int64_t ldd = (int64_t)a.H * D;
   const float lam = a.lambda[h], scale = a.sl2 / kLog2e;
-  // Thread tid < 128 brings statistic tid / 32 of query tid % 32.
+  // Thread tid < 128 brings statistic tid / 32 of query tid % 32; of one wave, each lane two.
   float dlam = 0.f;
-  const float* sbase = (tid & 64 ? a.r12 : a.lse) + ((int64_t)(tid & 32 ? a.H : 0) + h) * a.total_q + q0;
+  const int64_t sbase = ((int64_t)(tid & 32 ? a.H : 0) + h) * a.total_q + q0;
 
-  for (int kt = bx * kBQ; kt < kv_len; kt += gridDim.x * kBQ) {
-    const int ki = kt + w * 32 + l32;
+  for (int kt = bx * ROWS; kt < kv_len; kt += gridDim.x * ROWS) {
+    const int ki = kt + (SHARE ? 0 : w * 32) + l32;
     const int64_t krow = kv0 + min(ki, kv_len - 1);
     Fr kf[KS], vf[KS];
     {
@@ -1065,24 +1092,28 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
       clear(dk[mt]);
       clear(dv[mt]);
     }
-    Stage<T, D, BQ, kNT> qs, ds;
-    float sv = 0.f;
+    Stage<T, D, BQ, NT> qs, ds;
+    float sv[2] = {0.f, 0.f};
+    constexpr int STEP = SHARE ? 4 * BQ : BQ;
+    constexpr bool AHEAD = !SHARE || sizeof(T) == 2 || D == 64;
     auto load = [&](int qb) {
       qs.load(qbase, a.ldq, qb, q_len, tid);
       ds.load(dbase, ldd, qb, q_len, tid);
-      if (tid < 128) {  // past the last query: P = 2^(0 - inf) = 0
-        const int r = qb + (tid & 31);
-        sv = r < q_len ? sbase[r] : tid < 64 ? INFINITY : 0.f;
-      }
+      const int r = qb + (tid & 31);  // past the last query: P = 2^(0 - inf) = 0
+      if (SHARE || tid < 64) sv[0] = r < q_len ? a.lse[sbase + r] : INFINITY;
+      if (SHARE || (tid >= 64 && tid < 128)) sv[1] = r < q_len ? a.r12[sbase + r] : 0.f;
     };
-    load(0);
-    for (int qb = 0; qb < q_len; qb += BQ) {
-      __syncthreads();
+    int qb = SHARE ? w * BQ : 0;
+    if (AHEAD) load(qb);
+    for (; qb < q_len; qb += STEP) {
+      if (!AHEAD) load(qb);
+      tile_sync<SHARE>();
       qs.store(qt, tid);
       ds.store(dt, tid);
-      if (tid < 128) st4[tid >> 5][tid & 31] = sv;
-      __syncthreads();
-      load(qb + BQ);
+      if (SHARE || tid < 64) st4[(tid >> 5) & 1][tid & 31] = sv[0];
+      if (SHARE || (tid >= 64 && tid < 128)) st4[2 + ((tid >> 5) & 1)][tid & 31] = sv[1];
+      tile_sync<SHARE>();
+      if (AHEAD) load(qb + STEP);
       f32x16_t s1, s2, dp;
       clear(s1);
       clear(s2);
@@ -1114,7 +1145,11 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
         }
       }
     }
-    if (ki < kv_len) {
+    if (SHARE) {
+      join_waves<MT>((float*)lds, w, lane, dk);
+      join_waves<MT>((float*)lds, w, lane, dv);
+    }
+    if (ki < kv_len && (!SHARE || w == 0)) {
       const int64_t at = ((int64_t)(kv0 + ki) * a.H + h) * D;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -1126,20 +1161,30 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) dlam += __shfl_xor(dlam, off, 64);
   __syncthreads();
-  if (lane == 0) st4[0][w] = dlam;
+  if (lane == 0) stats[0][0][w] = dlam;
   __syncthreads();
-  if (tid == 0)
+  if (threadIdx.x == 0)
     a.lam_part[((int64_t)h * gridDim.z + bb) * gridDim.x + bx] =
-        (st4[0][0] + st4[0][1]) + (st4[0][2] + st4[0][3]);
+        (stats[0][0][0] + stats[0][0][1]) + (stats[0][0][2] + stats[0][0][3]);
 }
 
 // ------------------------------------------------------------------------------- host
 constexpr int64_t kCUs = 256;
 
-// Tiles of 128 rows that the grid gives a sequence; the kernels' loops cover longer ones.
-unsigned tiles_of(int64_t longest, int64_t hb) {
+// Tiles of `rows` rows that the grid gives a sequence; the kernels' loops cover longer ones.
+unsigned tiles_of(int64_t longest, int64_t hb, int rows = kBQ) {
   return (unsigned)std::max<int64_t>(
-      1, std::min<int64_t>(std::min<int64_t>((longest + kBQ - 1) / kBQ, 65535), (INT32_MAX / 16) / hb));
+      1, std::min<int64_t>(std::min<int64_t>((longest + rows - 1) / rows, 65535), (INT32_MAX / 16) / hb));
+}
+// Rows of a block of one wave per SIMD: 128, or 32 that its waves share.  Blocks of 32 are a quarter of
+// the work each, and waste less of the last round over the CUs; alone they take longer for the joining
+// and for copies that no other wave shares, measured as 1.1-1.2 times in fp32 and 1.4-1.6 in 16 bits.
+// Gradients, us, blocks of 128 / of 32: fp32 8 x 64, 1024 tokens (64 blocks of 128) 296 / 99, 2048 (128)
+// 573 / 338; bf16 12 x 128, 512 (48) 75 / 46, 1024 (96) 133 / 119, 1536 (144) 187 / 218, 3008 (288) 670 / 603.
+int block_rows(int32_t dtype, int64_t longest, int64_t hb) {
+  const int64_t b = (int64_t)tiles_of(longest, hb) * hb, rounds = (b + kCUs - 1) / kCUs;
+  const int64_t quarters = (4 * b + kCUs - 1) / kCUs;
+  return (dtype == TSC_F32 ? 12 * quarters < 40 * rounds : 15 * quarters < 40 * rounds) ? 32 : kBQ;
 }
 
 // The forward pass' blocks: query rows of each, and the parts of the keys.
@@ -1148,14 +1193,9 @@ struct Plan {
 };
 Plan da_plan(int32_t dtype, int32_t B, int64_t total_kv, int32_t H, int64_t max_q, int64_t max_kv) {
   const int64_t hb = (int64_t)H * B;
-  int64_t blocks = std::max<int64_t>(1, (max_q + kBQ - 1) / kBQ) * hb;
-  Plan p = {kBQ, 1, INT32_MAX};
+  Plan p = {dtype == TSC_F32 ? block_rows(dtype, max_q, hb) : kBQ, 1, INT32_MAX};
+  const int64_t blocks = (int64_t)tiles_of(max_q, hb, p.rows) * hb;
   if (blocks >= kCUs) return p;
-  if (dtype == TSC_F32) {
-    p.rows = 32;
-    blocks = std::max<int64_t>(1, (max_q + 31) / 32) * hb;
-    if (blocks >= kCUs) return p;
-  }
   // Parts of one size, so that long sequences get more of them, and no more blocks than CUs: of n a
   // sequence's query tiles and heads can have sum ceil(keys / part) <= total / part + B.
   const int64_t n = kCUs / (blocks / B) - B;
@@ -1206,7 +1246,7 @@ int64_t diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q
                                        int32_t D, int32_t max_q, int32_t max_kv, int32_t backward) {
   if (B == 0 || total_q == 0) return 0;
   const int64_t hb = (int64_t)H * B;
-  if (backward) return 4 * (2 * (int64_t)H * total_q + hb * tiles_of(max_kv, hb));
+  if (backward) return 4 * (2 * (int64_t)H * total_q + hb * tiles_of(max_kv, hb, block_rows(dtype, max_kv, hb)));
   const int s = da_plan(dtype, B, total_kv, H, max_q, max_kv).splits;
   return s > 1 ? 4 * (int64_t)s * total_q * H * 2 * (D + 4) : 0;
 }
@@ -1224,8 +1264,7 @@ int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* 
   a.splits = plan.splits;
   a.part_keys = plan.part_keys;
   a.part = (float*)ws;
-  const bool few = plan.rows == 32;
-  const unsigned gx = (few ? std::max(1, (x.max_q + 31) / 32) : tiles_of(x.max_q, hb)) * a.splits;
+  const unsigned gx = tiles_of(x.max_q, hb, plan.rows) * a.splits;
   const dim3 grid(gx, (unsigned)x.H, (unsigned)x.B);
   return by_type(x.dtype, x.D, [&](auto t, auto d) {
     using T = decltype(t);
@@ -1233,7 +1272,7 @@ int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* 
     {
       ProfScope p(ctx, "diff_attention");
       if constexpr (sizeof(T) == 4) {
-        if (few) da_few32_kernel<D><<<grid, kNT, 0, ctx->stream>>>(a);
+        if (plan.rows == 32) da_few32_kernel<D><<<grid, kNT, 0, ctx->stream>>>(a);
         else da_forward32_kernel<D><<<grid, kNT, 0, ctx->stream>>>(a);
       } else {
         constexpr int NM = D == 64 ? 2 : 1, NW = 8 / NM;
@@ -1267,7 +1306,10 @@ int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const vo
   float* lam_part = r12 + 2 * (int64_t)x.H * x.total_q;
   a.r12 = r12;
   a.lam_part = lam_part;
-  a.lam_parts = (int)tiles_of(x.max_kv, hb) * x.B;
+  const int rq = block_rows(x.dtype, x.max_q, hb), rk = block_rows(x.dtype, x.max_kv, hb);
+  const dim3 gq(tiles_of(x.max_q, hb, rq), (unsigned)x.H, (unsigned)x.B);
+  const dim3 gk(tiles_of(x.max_kv, hb, rk), (unsigned)x.H, (unsigned)x.B);
+  a.lam_parts = (int)gk.x * x.B;
   return by_type(x.dtype, x.D, [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
@@ -1278,12 +1320,12 @@ int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const vo
     }
     {
       ProfScope p(ctx, "diff_attention_dkv");
-      da_dkv_kernel<T, D><<<dim3(tiles_of(x.max_kv, hb), (unsigned)x.H, (unsigned)x.B), kNT, 0,
-                            ctx->stream>>>(a);
+      if (rk == 32) da_dkv_kernel<T, D, true><<<gk, kNT, 0, ctx->stream>>>(a);
+      else da_dkv_kernel<T, D, false><<<gk, kNT, 0, ctx->stream>>>(a);
     }
     ProfScope p(ctx, "diff_attention_dq");
-    da_dq_kernel<T, D><<<dim3(tiles_of(x.max_q, hb), (unsigned)x.H, (unsigned)x.B), kNT, 0,
-                         ctx->stream>>>(a);
+    if (rq == 32) da_dq_kernel<T, D, true><<<gq, kNT, 0, ctx->stream>>>(a);
+    else da_dq_kernel<T, D, false><<<gq, kNT, 0, ctx->stream>>>(a);
   });
 }
 
