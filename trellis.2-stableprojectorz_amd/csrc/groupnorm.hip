@@ -264,13 +264,35 @@ __device__ __forceinline__ float2 granule(const GnShape& s, int i, int64_t rows,
   return make_float2(a, q);
 }
 
+// How many of rows lo .. hi - 1 are the thread's: lo + ty and every TY-th one from there.
+__device__ __forceinline__ int64_t thread_rows(const GnShape& s, const Where& w, int64_t lo, int64_t hi) {
+  return hi - lo > w.ty ? (hi - lo - w.ty + s.TY - 1) / s.TY : 0;
+}
+
+// The second pass goes from the last rows on: they were read last and are still in the memory-side cache.
+// Its first whole chunk is fetched ahead, before the sums that everything else waits for.
+constexpr int kApplyRows = 4;
+template <typename T, int VN>
+struct ApplyRows {
+  Pack<T, VN> v[kApplyRows];
+  __device__ __forceinline__ void fetch(const T* x, int64_t at, int64_t step) {
+#pragma unroll
+    for (int k = 0; k < kApplyRows; ++k) v[k] = *(const Pack<T, VN>*)(x + at + k * step);
+  }
+  __device__ __forceinline__ void ahead(const GnShape& s, const Where& w, int64_t lo, int64_t hi,
+                                        const T* x) {
+    const int64_t whole = thread_rows(s, w, lo, hi) / kApplyRows * kApplyRows;
+    if (w.live && whole > 0)
+      fetch(x, (lo + w.ty + (whole - kApplyRows) * s.TY) * s.C + w.c0, (int64_t)s.TY * s.C);
+  }
+};
+
 // y of rows lo .. hi - 1 from the groups' (mean, rstd) in sg (group gl first).
 template <typename T, int VN>
 __device__ __forceinline__ void apply_rows(const GnShape& s, const Where& w, int64_t lo, int64_t hi,
                                            const float2* sg, int gl, const T* x,
                                            const T* __restrict__ gamma, const T* __restrict__ beta,
-                                           int32_t silu, T* y) {
-  constexpr int KR = 4;
+                                           int32_t silu, T* y, ApplyRows<T, VN>& rows) {
   if (!w.live) return;
   float mean[VN], a[VN], c[VN];
 #pragma unroll
@@ -280,28 +302,23 @@ __device__ __forceinline__ void apply_rows(const GnShape& s, const Where& w, int
     a[e] = m.y * (gamma ? (float)gamma[w.c0 + e] : 1.f);
     c[e] = beta ? (float)beta[w.c0 + e] : 0.f;
   }
-  auto chunk = [&](int64_t r, int k, auto whole) {
-    Pack<T, VN> v[KR];
+  const int64_t n = thread_rows(s, w, lo, hi), whole = n / kApplyRows * kApplyRows;
+  const int64_t step = (int64_t)s.TY * s.C, at0 = (lo + w.ty) * s.C + w.c0;
+  auto one = [&](int64_t i, const Pack<T, VN>& v) {
+    float o[VN];
 #pragma unroll
-    for (int i = 0; i < KR; ++i)
-      if (decltype(whole)::value || i < k)
-        v[i] = *(const Pack<T, VN>*)(x + (r + (int64_t)i * s.TY) * s.C + w.c0);
-#pragma unroll
-    for (int i = 0; i < KR; ++i)
-      if (decltype(whole)::value || i < k) {
-        float o[VN];
-#pragma unroll
-        for (int e = 0; e < VN; ++e) {
-          const float h = fmaf((float)v[i].v[e] - mean[e], a[e], c[e]);
-          o[e] = silu ? h * __builtin_amdgcn_rcpf(1.f + __expf(-h)) : h;
-        }
-        store_nt<T, VN>(y + (r + (int64_t)i * s.TY) * s.C + w.c0, o);
-      }
+    for (int e = 0; e < VN; ++e) {
+      const float h = fmaf((float)v.v[e] - mean[e], a[e], c[e]);
+      o[e] = silu ? h * __builtin_amdgcn_rcpf(1.f + __expf(-h)) : h;
+    }
+    store_nt<T, VN>(y + at0 + i * step, o);
   };
-  // From the last rows on: they were read last and are still in the memory-side cache.
-  const int64_t n = hi - lo > w.ty ? (hi - lo - w.ty + s.TY - 1) / s.TY : 0, whole = n / KR * KR;
-  if (whole < n) chunk(lo + w.ty + whole * s.TY, (int)(n - whole), std::false_type());
-  for (int64_t i = whole - KR; i >= 0; i -= KR) chunk(lo + w.ty + i * s.TY, KR, std::true_type());
+  for (int64_t i = whole; i > 0; i -= kApplyRows) {
+    if (i < whole) rows.fetch(x, at0 + (i - kApplyRows) * step, step);
+#pragma unroll
+    for (int k = 0; k < kApplyRows; ++k) one(i - kApplyRows + k, rows.v[k]);
+  }
+  for (int64_t i = whole; i < n; ++i) one(i, *(const Pack<T, VN>*)(x + at0 + i * step));
 }
 
 // Partial statistics: part[slot * NG + granule] = (mean, M2).
@@ -321,21 +338,22 @@ __global__ void __launch_bounds__(kNT, 4)
   for (int i = tid; i < ng; i += kNT) dst[i] = granule(s, i, w.hi - w.lo, smean, sm2);
 }
 
-// Threads of the block that add up one group's partials: a power of two.
-__device__ __forceinline__ int lanes_per_group(int ng) {
-  int p = kNT;
-  while (p * ng > kNT) p >>= 1;
-  return p;
+// Columns of threads, a power of two: thread tid adds up group tid % columns, so that neighbors read
+// neighboring partials.
+__device__ __forceinline__ int sum_columns(int ng) {
+  int c = 1;
+  while (c < ng) c <<= 1;
+  return c;
 }
 
-// Adds a pair of doubles over each run of P threads; the run's first thread returns the sums.
-__device__ __forceinline__ void run_sum(double* sa, double* sb, int P, double* a, double* b) {
+// Adds a pair of doubles over the threads of each column; those of the first row have the sums.
+__device__ __forceinline__ void column_sum(double* sa, double* sb, int columns, double* a, double* b) {
   const int tid = threadIdx.x;
   sa[tid] = *a;
   sb[tid] = *b;
   __syncthreads();
-  for (int half = P / 2; half > 0; half >>= 1) {
-    if ((tid & (P - 1)) < half) {
+  for (int half = kNT / 2; half >= columns; half >>= 1) {
+    if (tid < half) {
       *a += sa[tid + half];
       *b += sb[tid + half];
       sa[tid] = *a;
@@ -355,13 +373,15 @@ __global__ void __launch_bounds__(kNT, 4)
   const Where w = where<VN>(s, blockIdx.x, blockIdx.y);
   const int tid = threadIdx.x, SC = s.TX * VN;
   const int gl = w.slab * SC / s.cpg, gh = (min((w.slab + 1) * SC, s.C) - 1) / s.cpg;
-  const int ng = gh - gl + 1, P = lanes_per_group(ng);
+  const int ng = gh - gl + 1, cols = sum_columns(ng), P = kNT / cols;
   if (rest) zero_rest<T, VN>(s, w, y);
   if (w.hi <= w.lo) return;  // uniform over the block
+  ApplyRows<T, VN> rows;
+  rows.ahead(s, w, w.lo, w.hi, x);
   const int64_t beg = w.beg, end = w.end;
   {
     const int t0 = tile_of(s, beg), nt = tile_of(s, end - 1) - t0 + 1;
-    const int g = gl + tid / P, j = tid & (P - 1);
+    const int g = gl + (tid & (cols - 1)), j = tid / cols;
     double n = 0., d1 = 0., d2 = 0.;
     float m0 = 0.f;
     if (g <= gh) {
@@ -377,7 +397,7 @@ __global__ void __launch_bounds__(kNT, 4)
           d2 += (double)p.y + c * d * d;
         }
     }
-    run_sum(sa, sb, P, &d1, &d2);
+    column_sum(sa, sb, cols, &d1, &d2);
     if (g <= gh && j == 0) {
       n = (double)(end - beg) * s.cpg;
       const double mean = (double)m0 + d1 / n;
@@ -390,7 +410,7 @@ __global__ void __launch_bounds__(kNT, 4)
     }
     __syncthreads();
   }
-  apply_rows<T, VN>(s, w, w.lo, w.hi, sg, gl, x, gamma, beta, silu, y);
+  apply_rows<T, VN>(s, w, w.lo, w.hi, sg, gl, x, gamma, beta, silu, y, rows);
 }
 
 // Few rows: a block has a whole sample's rows of one slab, whose groups end in it (GP = 1), and both
@@ -416,7 +436,9 @@ __global__ void __launch_bounds__(kOneNT)
       if (stats) *(float2*)(stats + 2 * ((int64_t)b * s.groups + g0 + i)) = r;
     }
     __syncthreads();
-    apply_rows<T, VN>(s, w, lo, hi, sg, g0, x, gamma, beta, silu, y);
+    ApplyRows<T, VN> rows;
+    rows.ahead(s, w, lo, hi, x);
+    apply_rows<T, VN>(s, w, lo, hi, sg, g0, x, gamma, beta, silu, y, rows);
   }
   w.b = b;
   w.beg = lo;
@@ -598,14 +620,25 @@ __global__ void __launch_bounds__(kNT, 4)
   const Where w = where<VN>(s, at % (s.T + s.B), at / (s.T + s.B));
   const int SC = s.TX * VN;
   const int gl = w.slab * SC / s.cpg, gh = (min((w.slab + 1) * SC, s.C) - 1) / s.cpg;
-  const int ng = gh - gl + 1, P = lanes_per_group(ng);
+  const int ng = gh - gl + 1, cols = sum_columns(ng), P = kNT / cols;
   if (rest) zero_rest<T, VN>(s, w, dx);
   if (w.hi <= w.lo) return;  // uniform over the block
   const int b = w.b;
   const int64_t beg = w.beg, end = w.end, lo = w.lo, hi = w.hi;
+  const int64_t n = thread_rows(s, w, lo, hi), whole = n / KR * KR;
+  const int64_t step = (int64_t)s.TY * s.C, at0 = (lo + w.ty) * s.C + w.c0;
+  Pack<T, VN> vx[KR], vy[KR];  // from the last rows on, the first whole chunk ahead of the sums
+  auto fetch = [&](int64_t i) {
+#pragma unroll
+    for (int k = 0; k < KR; ++k) {
+      vx[k] = *(const Pack<T, VN>*)(x + at0 + (i + k) * step);
+      vy[k] = *(const Pack<T, VN>*)(dy + at0 + (i + k) * step);
+    }
+  };
+  if (w.live && whole > 0) fetch(whole - KR);
   {
     const int t0 = tile_of(s, beg), nt = tile_of(s, end - 1) - t0 + 1;
-    const int g = gl + tid / P, j = tid & (P - 1);
+    const int g = gl + (tid & (cols - 1)), j = tid / cols;
     double u = 0., v = 0.;
     if (g <= gh) {
       const float2* src = pg + (int64_t)(t0 + b) * s.NG + (int64_t)g * s.GP;
@@ -617,7 +650,7 @@ __global__ void __launch_bounds__(kNT, 4)
           v += (double)p.y;
         }
     }
-    run_sum(sa, sb, P, &u, &v);
+    column_sum(sa, sb, cols, &u, &v);
     if (g <= gh && j == 0) {
       const double n = (double)(end - beg) * s.cpg;
       sg[g - gl] = make_float2((float)(u / n), (float)(v / n));
@@ -634,32 +667,23 @@ __global__ void __launch_bounds__(kNT, 4)
       ma[e] = m.x * rstd[e];
       mb[e] = m.y * rstd[e] * rstd[e];
     }
-    auto chunk = [&](int64_t r, int k, auto whole) {
-      Pack<T, VN> vx[KR], vy[KR];
+    auto one = [&](int64_t i, const Pack<T, VN>& px, const Pack<T, VN>& py) {
+      float o[VN];
 #pragma unroll
-      for (int i = 0; i < KR; ++i)
-        if (decltype(whole)::value || i < k) {
-          const int64_t at = (r + (int64_t)i * s.TY) * s.C + w.c0;
-          vx[i] = *(const Pack<T, VN>*)(x + at);
-          vy[i] = *(const Pack<T, VN>*)(dy + at);
-        }
-#pragma unroll
-      for (int i = 0; i < KR; ++i)
-        if (decltype(whole)::value || i < k) {
-          float o[VN];
-#pragma unroll
-          for (int e = 0; e < VN; ++e) {
-            const float xm = (float)vx[i].v[e] - mean[e];
-            const float dh = grad_one(xm, (float)vy[i].v[e], a[e], be[e], silu);
-            o[e] = fmaf(-xm, mb[e], fmaf(a[e], dh, -ma[e]));
-          }
-          store_nt<T, VN>(dx + (r + (int64_t)i * s.TY) * s.C + w.c0, o);
-        }
+      for (int e = 0; e < VN; ++e) {
+        const float xm = (float)px.v[e] - mean[e];
+        const float dh = grad_one(xm, (float)py.v[e], a[e], be[e], silu);
+        o[e] = fmaf(-xm, mb[e], fmaf(a[e], dh, -ma[e]));
+      }
+      store_nt<T, VN>(dx + at0 + i * step, o);
     };
-    // From the last rows on: they were read last and are still in the memory-side cache.
-    const int64_t n = hi - lo > w.ty ? (hi - lo - w.ty + s.TY - 1) / s.TY : 0, whole = n / KR * KR;
-    if (whole < n) chunk(lo + w.ty + whole * s.TY, (int)(n - whole), std::false_type());
-    for (int64_t i = whole - KR; i >= 0; i -= KR) chunk(lo + w.ty + i * s.TY, KR, std::true_type());
+    for (int64_t i = whole; i > 0; i -= KR) {
+      if (i < whole) fetch(i - KR);
+#pragma unroll
+      for (int k = 0; k < KR; ++k) one(i - KR + k, vx[k], vy[k]);
+    }
+    for (int64_t i = whole; i < n; ++i)
+      one(i, *(const Pack<T, VN>*)(x + at0 + i * step), *(const Pack<T, VN>*)(dy + at0 + i * step));
   }
 }
 
