@@ -328,8 +328,8 @@ int tsc_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, con
  *   out[n,h,:] = sum_m (P1[n,m] - lambda[h] P2[n,m]) v[m,h,:]
  * for the sequences of tsc_attention, whose tensors these are: q, out (total_q, num_heads, head_dim),
  * k, v (total_kv, num_heads, head_dim), head_dim 64 or 128 (maps of 32 or 64 dimensions).
- *   ld_q, ld_k, ld_v  row strides in elements, num_heads * head_dim or more, rows 16-byte aligned (so
- *     q, k and v may be slices of one fused projection); all other buffers are contiguous
+ *   ld_q, ld_k, ld_v  row strides in elements, num_heads * head_dim to 2^24, rows 16-byte aligned (so q,
+ *     k and v may be slices of one fused projection); all other buffers are contiguous
  *   lambda     device fp32 (num_heads)
  *   cu_seqlens_q / cu_seqlens_kv, scale, max_seqlen_q  as in tsc_attention, scale <= 0 meaning
  *     1/sqrt(head_dim / 2); max_seqlen_kv likewise (it sizes the workspace too: the same values there).  A sequence without keys gives zeros.
@@ -353,8 +353,8 @@ int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k
                        void* workspace, void* out, void* out2, float* lse);
 /* Its gradient from dout (total_q, num_heads, head_dim) and what the forward call was given and
  * wrote: dq (total_q, ...), dk and dv (total_kv, num_heads, head_dim) `dtype`, dlambda fp32
- * (num_heads) or NULL.  zero_rest is about rows of dq, dk and dv.  workspace with backward = 1.  The gradients must not overlap an input.  The sums
- * have one fixed order. */
+ * (num_heads) or NULL.  zero_rest is about rows of dq, dk and dv.  workspace with backward = 1.  The
+ * gradients must not overlap an input.  The sums have one fixed order. */
 int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k,
                                 const void* v, int64_t ld_q, int64_t ld_k, int64_t ld_v,
                                 const float* lambda, const int32_t* cu_seqlens_q,

@@ -290,6 +290,30 @@ def test_hints_and_offsets(pkg, dev):
     assert torch.equal(got, want["out"])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_hints_below_the_lengths_with_shared_keys(pkg, dev, dtype):
+    """The parts of the keys reach over sequences far longer than max_seqlen_kv says, with idle parts
+    for the short ones; rows behind a wrong max_seqlen_q are still covered."""
+    lq, lkv, h, d = [3, 0, 200, 1], [6000, 100, 2500, 0], 2, 64
+    q, k, v, do, lam = _make(lq, lkv, h, d, dtype, 13)
+    cq, ck = _cu(lq), _cu(lkv)
+    want = _oracle(q, k, v, do, lam, cq, ck, dtype)
+    for mq, mk in ((1, 600), (0, 0), (10 ** 6, 10 ** 6), (None, None)):
+        got = _run(pkg, dev, q, k, v, do, lam, torch.tensor(cq, device=dev), torch.tensor(ck, device=dev),
+                   max_seqlen_q=mq, max_seqlen_kv=mk)
+        for n in got:
+            _close(got[n], want[n], f"{n} ({mq}, {mk})")
+
+
+def test_block_without_gradients(pkg, dev):
+    p, lam = _block(128, 2, torch.bfloat16, 5)
+    d = {k: v.to(dev).requires_grad_() for k, v in p.items()}
+    block = pkg.SparseDiffAttentionBlock3d(2, 16, d["nw"], d["nb"], d["wqkv"], d["bqkv"], lam.to(dev),
+                                           d["wo"], d["bo"])
+    coords = torch.zeros((40, 4), dtype=torch.int32, device=dev)
+    assert not block(pkg.SparseTensor(torch.randn(40, 128, device=dev).bfloat16(), coords)).feats.requires_grad
+
+
 def test_empty_inputs(pkg, dev):
     z = lambda n: torch.zeros((n, 2, 64), device=dev).requires_grad_()
     lam = torch.ones(2, device=dev).requires_grad_()

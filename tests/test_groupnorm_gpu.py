@@ -282,6 +282,26 @@ def test_same_bits_each_time_on_any_stream_and_in_a_graph(pkg, dev):
             assert all(torch.equal(a, e) for a, e in zip(outs, eager)), (rep, i)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("c,groups", [(64, 32), (100, 20), (1024, 8)])
+def test_many_uneven_samples(pkg, dev, dtype, c, groups):
+    """Hundreds of samples, many of them empty, starting and ending at, before and after tile borders
+    (tiles are runs of equal length): every (tile, sample) meeting has its slot."""
+    rng = np.random.default_rng(c)
+    lens = rng.choice([0, 0, 1, 2, 7, 31, 32, 33, 64, 130], 300).tolist() + [900, 0, 0, 512, 0]
+    cu = [5 + v for v in _cu(lens)]
+    x, w, b, dy = _make([cu[-1] + 9], c, dtype, c)
+    r = _oracle(x, groups, w, b, cu, 1e-5, True, dy)
+    leaves = [t.to(dev).requires_grad_() for t in (x, w, b)]
+    y = pkg.group_norm(leaves[0], groups, leaves[1], leaves[2], torch.tensor(cu, device=dev), silu=True)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy.to(dev))
+    assert not y[:5].any() and not y[cu[-1]:].any() and not dx[:5].any() and not dx[cu[-1]:].any()
+    _close(y, r["y"], r["ty"], dtype, "y")
+    _close(dx, r["dx"], r["tdx"], dtype, "dx")
+    _close(dw, r["dw"], r["tdw"], dtype, "dweight")
+    _close(db, r["db"], r["tdb"], dtype, "dbias")
+
+
 def test_device_offsets_are_not_read_back(pkg, dev):
     x, w, b, _ = _make([600], 64, torch.float32, 12)
     xd = x.to(dev)

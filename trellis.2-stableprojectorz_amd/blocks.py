@@ -53,7 +53,8 @@ class SparseDiffAttentionBlock3d:
     """x + out(diff_attention(qkv(group_norm(x)))) over each sample's voxels: group norm, one linear
     layer for q, k and v (read in place as row slices), differential attention, and the output layer
     with the skip as its residual.  qkv weight (3 C, C), out weight (C, C), lam float32 (num_heads),
-    C = num_heads * 64 or 128."""
+    C = num_heads * 64 or 128.  Without gradients: its linear layers have none (group_norm and
+    sparse_diff_attention do, around another library's linear layers)."""
 
     def __init__(self, num_heads: int, num_groups: int, norm_weight: torch.Tensor | None,
                  norm_bias: torch.Tensor | None, qkv_weight: torch.Tensor,
@@ -64,6 +65,7 @@ class SparseDiffAttentionBlock3d:
         self.qkv = SparseLinear(qkv_weight, qkv_bias)
         self.out = SparseLinear(out_weight, out_bias)
 
+    @torch.no_grad()
     def forward(self, x: SparseTensor) -> SparseTensor:
         n, c = x.feats.shape
         cu = x.cu_rows

@@ -768,8 +768,8 @@ static int diff_attention_args(tsc_ctx* ctx, const char* what, int32_t dtype, co
   const int64_t lds[3] = {ld_q, ld_k, ld_v};
   const void* bufs[3] = {q, k, v};
   for (int i = 0; i < 3; ++i) {
-    if (lds[i] < (int64_t)H * D || lds[i] > (1 << 28) || lds[i] * es % 16)
-      return fail(TSC_ERR_INVALID, "%s: row stride %lld of q, k or v (%d * %d or more, whole 16 bytes)",
+    if (lds[i] < (int64_t)H * D || lds[i] > (1 << 24) || lds[i] * es % 16)
+      return fail(TSC_ERR_INVALID, "%s: row stride %lld of q, k or v (%d * %d to 2^24, whole 16 bytes)",
                   what, (long long)lds[i], H, D);
     if (!aligned(bufs[i], 16))
       return fail(TSC_ERR_INVALID, "%s: q, k and v must be 16-byte aligned", what);

@@ -1191,8 +1191,10 @@ int block_rows(int32_t dtype, int64_t longest, int64_t hb) {
 struct Plan {
   int rows, splits, part_keys;
 };
-Plan da_plan(int32_t dtype, int32_t B, int64_t total_kv, int32_t H, int64_t max_q, int64_t max_kv) {
+Plan da_plan(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv, int32_t H, int64_t max_q,
+             int64_t max_kv) {
   const int64_t hb = (int64_t)H * B;
+  max_q = std::max(max_q, (total_q + B - 1) / B);  // whatever the caller thinks: parts x rows of scratch
   Plan p = {dtype == TSC_F32 ? block_rows(dtype, max_q, hb) : kBQ, 1, INT32_MAX};
   const int64_t blocks = (int64_t)tiles_of(max_q, hb, p.rows) * hb;
   if (blocks >= kCUs) return p;
@@ -1247,7 +1249,7 @@ int64_t diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q
   if (B == 0 || total_q == 0) return 0;
   const int64_t hb = (int64_t)H * B;
   if (backward) return 4 * (2 * (int64_t)H * total_q + hb * tiles_of(max_kv, hb, block_rows(dtype, max_kv, hb)));
-  const int s = da_plan(dtype, B, total_kv, H, max_q, max_kv).splits;
+  const int s = da_plan(dtype, B, total_q, total_kv, H, max_q, max_kv).splits;
   return s > 1 ? 4 * (int64_t)s * total_q * H * 2 * (D + 4) : 0;
 }
 
@@ -1260,7 +1262,7 @@ int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* 
   a.out = out;
   a.out2 = out2;
   a.lse = lse;
-  const Plan plan = da_plan(x.dtype, x.B, x.total_kv, x.H, x.max_q, x.max_kv);
+  const Plan plan = da_plan(x.dtype, x.B, x.total_q, x.total_kv, x.H, x.max_q, x.max_kv);
   a.splits = plan.splits;
   a.part_keys = plan.part_keys;
   a.part = (float*)ws;

@@ -8,7 +8,7 @@
 //
 // Bound by memory: the statistics need all of a sample before its first output, so x (and dy) is
 // read twice, the second time from the 256 MB memory-side cache as far as it fits.
-// Two launches each way (one for few rows).  The rows are cut into T tiles and the channels into slabs
+// Two launches each way.  The rows are cut into T tiles and the channels into slabs
 // of whole vectors; a block has one slab of the rows that a tile and a sample share, each thread one
 // vector column and every TY-th row.  The first kernel leaves one partial result per (tile, sample,
 // granule) - a granule is the largest run of channels that lies in one group and one slab - and each
@@ -30,7 +30,6 @@
 namespace tsc {
 namespace {
 
-constexpr int kOneNT = 1024;   // threads of a block that has a sample to itself
 constexpr int kNT = 512;       // threads of a block, two of which fill a CU (128 registers)
 constexpr int kParamCh = 8;    // channels of a block that adds up dgamma and dbeta
 constexpr int kSlab = 256;     // channels of a slab, at most
@@ -164,9 +163,9 @@ __device__ __forceinline__ void pair_up(float (&mean)[VN], float (&m2)[VN], floa
 }
 
 // ------------------------------------------------------------------------------- forward
-// Mean, M2 of rows lo .. hi - 1: of each unit of every vector column, in order, in smean and sm2 (NT VN
-// floats each; scnt: NT).  The block has NT threads and the unit's `rows` columns of w.
-template <typename T, int VN, int NT>
+// Mean and M2 of rows lo .. hi - 1 for each unit (the channels of a granule within a vector) of every
+// vector column, in order, in smean and sm2 (kNT VN floats each; scnt: kNT).
+template <typename T, int VN>
 __device__ __forceinline__ void tile_stats(const GnShape& s, const Where& w, int64_t lo, int64_t hi,
                                            const T* __restrict__ x, float* smean, float* sm2,
                                            float* scnt) {
@@ -213,7 +212,6 @@ __device__ __forceinline__ void tile_stats(const GnShape& s, const Where& w, int
   if (VN >= 4 && s.sub >= 4) pair_up<2>(mean, m2, cnt);
   if (VN >= 8 && s.sub >= 8) pair_up<4>(mean, m2, cnt);
   const int units = VN >> s.lsub;  // unit i is element i * sub
-  __syncthreads();  // the granules of the sample before have been read
 #pragma unroll
   for (int e = 0; e < VN; ++e)
     if ((e & (s.sub - 1)) == 0) {
@@ -334,7 +332,7 @@ __global__ void __launch_bounds__(kNT, 4)
     for (int i = tid; i < ng; i += kNT) dst[i] = make_float2(0.f, 0.f);
     return;
   }
-  tile_stats<T, VN, kNT>(s, w, w.lo, w.hi, x, smean, sm2, scnt);
+  tile_stats<T, VN>(s, w, w.lo, w.hi, x, smean, sm2, scnt);
   for (int i = tid; i < ng; i += kNT) dst[i] = granule(s, i, w.hi - w.lo, smean, sm2);
 }
 
@@ -411,41 +409,6 @@ __global__ void __launch_bounds__(kNT, 4)
     __syncthreads();
   }
   apply_rows<T, VN>(s, w, w.lo, w.hi, sg, gl, x, gamma, beta, silu, y, rows);
-}
-
-// Few rows: a block has a whole sample's rows of one slab, whose groups end in it (GP = 1), and both
-// passes are one launch; the second reads from the L2.
-template <typename T, int VN>
-__global__ void __launch_bounds__(kOneNT)
-    gn_one_kernel(GnShape s, const T* x, const T* __restrict__ gamma, const T* __restrict__ beta,
-                  float eps, int32_t silu, int32_t rest, float* __restrict__ stats, T* y) {
-  __shared__ float smean[kOneNT * VN], sm2[kOneNT * VN], scnt[kOneNT];
-  __shared__ float2 sg[kSlab];
-  const int b = blockIdx.x, tid = threadIdx.x, SC = s.TX * VN;
-  Where w = columns<VN>(s, blockIdx.y);
-  const int g0 = w.slab * SC / s.gran, ng = min(SC / s.gran, s.NG - g0);
-  int64_t lo, hi;
-  gn_segment(s, b, &lo, &hi);
-  if (hi > lo) {
-    tile_stats<T, VN, kOneNT>(s, w, lo, hi, x, smean, sm2, scnt);
-    const float n = (float)((hi - lo) * s.cpg);
-    for (int i = tid; i < ng; i += kOneNT) {
-      const float2 g = granule(s, i, hi - lo, smean, sm2);
-      const float2 r = make_float2(g.x, 1.f / sqrtf(g.y / n + eps));
-      sg[i] = r;
-      if (stats) *(float2*)(stats + 2 * ((int64_t)b * s.groups + g0 + i)) = r;
-    }
-    __syncthreads();
-    ApplyRows<T, VN> rows;
-    rows.ahead(s, w, lo, hi, x);
-    apply_rows<T, VN>(s, w, lo, hi, sg, g0, x, gamma, beta, silu, y, rows);
-  }
-  w.b = b;
-  w.beg = lo;
-  w.end = hi;
-  w.r0 = b == 0 ? 0 : lo;
-  w.r1 = b == s.B - 1 ? s.N : hi;
-  if (rest) zero_rest<T, VN>(s, w, y);
 }
 
 // ------------------------------------------------------------------------------- backward
@@ -697,11 +660,9 @@ int gcd(int a, int b) {
   return a;
 }
 
-constexpr int kOneRows = 16;        // rows per thread up to which one block takes a sample
 constexpr int kTargetBlocks = 512;  // two per CU: few partial sums for every block to add up
 
-GnShape gn_shape(const int32_t* cu, int32_t B, int64_t N, int32_t C, int32_t groups, int vn,
-                 int threads = kNT) {
+GnShape gn_shape(const int32_t* cu, int32_t B, int64_t N, int32_t C, int32_t groups, int vn) {
   GnShape s;
   s.cu = cu;
   s.N = N;
@@ -715,7 +676,7 @@ GnShape gn_shape(const int32_t* cu, int32_t B, int64_t N, int32_t C, int32_t gro
   s.slabs = (s.nvec + cols - 1) / cols;
   s.TX = (s.nvec + s.slabs - 1) / s.slabs;
   s.slabs = (s.nvec + s.TX - 1) / s.TX;
-  s.TY = threads / s.TX;
+  s.TY = kNT / s.TX;
   // No more slots than there is room for at once: 520 blocks instead of 512 for 243547 x 512 bf16 in four
   // samples took 164 us instead of 143.
   const int64_t room = kTargetBlocks / s.slabs, most = std::max<int64_t>({1, room - B, room / 2});
@@ -784,17 +745,11 @@ int groupnorm_launch(tsc_ctx* ctx, int32_t dtype, const void* x, const int32_t* 
                      float eps, int32_t silu, int32_t rest, float* stats, void* ws, void* y) {
   const int es = dtype == TSC_F32 ? 4 : 2;
   const int vn = vec_elems(es, C, {x, y});
-  const GnShape s = gn_shape(cu, B, N, C, groups, vn), one = gn_shape(cu, B, N, C, groups, vn, kOneNT);
+  const GnShape s = gn_shape(cu, B, N, C, groups, vn);
   const dim3 grid((unsigned)(s.T + s.B), (unsigned)s.slabs);
   by_type<8>(dtype, vn, [&](auto t, auto v) {
     using T = decltype(t);
     constexpr int VN = decltype(v)::value;
-    if (s.GP == 1 && N <= kOneRows * (int64_t)one.TY * std::min(B, 16)) {
-      ProfScope p(ctx, silu ? "groupnorm_silu" : "groupnorm");
-      gn_one_kernel<T, VN><<<dim3((unsigned)B, (unsigned)one.slabs), kOneNT, 0, ctx->stream>>>(
-          one, (const T*)x, (const T*)gamma, (const T*)beta, eps, silu, rest, stats, (T*)y);
-      return;
-    }
     {
       ProfScope p(ctx, "groupnorm_stats");
       gn_stats_kernel<T, VN><<<grid, kNT, 0, ctx->stream>>>(s, (const T*)x, (float2*)ws);
