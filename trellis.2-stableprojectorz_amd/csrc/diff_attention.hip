@@ -933,9 +933,11 @@ __global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r
   }
 }
 
-// Both gradient kernels: a block's 4 waves own 32 rows each and share the tiles of the other side; or,
-// where that leaves CUs idle (SHARE), all own the same 32 rows and take the tiles in turn, each through
-// its own piece of LDS, and their sums are joined at the end.
+// Both gradient kernels: a block's waves own 32 rows each and share the tiles of the other side, through
+// two buffers in LDS; or, where that leaves CUs idle (SHARE), all own the same 32 rows and take the
+// tiles in turn, each through its own piece of LDS, and their sums are joined at the end.
+// Two waves per SIMD in 16 bits: with one, whose products, exponentials and LDS reads wait for each
+// other, a step of dk / dv took 6700 cycles at D = 128, 1024 of them in the matrix cores.
 template <bool SHARE>
 __device__ __forceinline__ void tile_sync() {
   // A wave's own LDS operations are carried out in order; the compiler has to keep that order.
@@ -945,14 +947,14 @@ __device__ __forceinline__ void tile_sync() {
 
 // dq of 128 (32) queries; one block of each head also adds up dlambda.
 template <typename T, int D, bool SHARE>
-__global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
+__global__ void __launch_bounds__(kNT, sizeof(T) == 2 && !SHARE ? 2 : 1) da_dq_kernel(const DaArgs a) {
   typedef Frag<T> F;
   typedef typename F::type Fr;
   typedef Tile<T, D> Ti;
   constexpr int BK = 32;
   constexpr int KS = D / 16, MT = D / 32;
   constexpr int TB = BK * Ti::ROWB, ROWS = SHARE ? 32 : kBQ, NT = SHARE ? 64 : kNT;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[SHARE ? 4 : 1][2 * TB];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[SHARE ? 4 : 2][2 * TB];
   int bx, h, bb;
   block_tile(a.cu_kv, &bx, &h, &bb);
   int q0, q_len, kv0, kv_len;
@@ -960,7 +962,6 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
   segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
   const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = SHARE ? lane : threadIdx.x;
-  unsigned char *kt = lds[SHARE ? w : 0], *vt = kt + TB;
   if (a.rest) zero_rest((T*)a.dq, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
   if (bx == 0 && bb == 0 && w == 0 && a.dlambda) {
     double s = 0.;
@@ -999,9 +1000,10 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
       vs.load(vbase, a.ldv, k, kv_len, tid);
     };
     if (AHEAD) load(kb);
-    for (; kb < kv_len; kb += STEP) {
+    for (int buf = 0; kb < kv_len; kb += STEP, buf ^= 1) {
+      unsigned char *kt = lds[SHARE ? w : buf], *vt = kt + TB;
       if (!AHEAD) load(kb);
-      tile_sync<SHARE>();
+      if (SHARE) tile_sync<SHARE>();
       ks.store(kt, tid);
       vs.store(vt, tid);
       tile_sync<SHARE>();
@@ -1015,12 +1017,15 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
         F::mma(Ti::row(kt, 0, l32, hf, st), qf[st], st < KS / 2 ? s1 : s2);
         F::mma(Ti::row(vt, 0, l32, hf, st), df[st], dp);
       }
+      if (kb + BK > kv_len)  // uniform
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (kb + 8 * (j >> 2) + 4 * hf + (j & 3) >= kv_len) s1[j] = s2[j] = -INFINITY;
       float d1[16], d2[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const bool ok = kb + 8 * (j >> 2) + 4 * hf + (j & 3) < kv_len;
-        const float p1 = ok ? fast_exp2(fmaf(s1[j], a.sl2, -l1)) : 0.f;
-        const float p2 = ok ? fast_exp2(fmaf(s2[j], a.sl2, -l2)) : 0.f;
+        const float p1 = fast_exp2(fmaf(s1[j], a.sl2, -l1));
+        const float p2 = fast_exp2(fmaf(s2[j], a.sl2, -l2));
         d1[j] = p1 * (dp[j] - r1);
         d2[j] = p2 * ((dp[j] - r2) * nlam);
       }
@@ -1032,6 +1037,7 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
           F::mma(Ti::col(kt, 0, lane, g, mt), mt < MT / 2 ? f1[g] : f2[g], acc[mt]);
     }
     if (SHARE) join_waves<MT>((float*)lds, w, lane, acc);
+    else __syncthreads();  // the next tile's rows go into these buffers
     if (qi < q_len && (!SHARE || w == 0)) {
       T* p = (T*)a.dq + ((int64_t)(q0 + qi) * a.H + h) * D;
 #pragma unroll
@@ -1041,17 +1047,26 @@ __global__ void __launch_bounds__(kNT) da_dq_kernel(const DaArgs a) {
 }
 
 // dk and dv of 128 (32) keys, and the block's part of dlambda = - sum P2 dP, from the unrounded fp32
-// probabilities (do . (P2 v) with P2 v in 16 bits is off by 2^-9 of it).  The sequence ranking of block_tile goes by the queries here.
-template <typename T, int D, bool SHARE>
-__global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
+// probabilities (do . (P2 v) with P2 v in 16 bits is off by 2^-9 of it).  The sequence ranking of
+// block_tile goes by the queries here.
+// A wave has NM maps of its 32 keys: both, or one where the registers of both (dk, dv, k and v: 192 at
+// D = 128) leave one wave per SIMD.  Then dP is made twice, P1 and P2 are multiplied with do one by one
+// (12 D flops a pair instead of 8 D), and the two waves' parts of dv meet in LDS at the end.
+template <typename T, int D, bool SHARE, int NM>
+__global__ void __launch_bounds__(SHARE ? kNT : 512 / NM, sizeof(T) == 2 && !SHARE ? 2 : 1)
+    da_dkv_kernel(const DaArgs a) {
   typedef Frag<T> F;
   typedef typename F::type Fr;
   typedef Tile<T, D> Ti;
   constexpr int BQ = 32;
-  constexpr int KS = D / 16, MT = D / 32;
-  constexpr int TB = BQ * Ti::ROWB, ROWS = SHARE ? 32 : kBQ, NT = SHARE ? 64 : kNT;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[SHARE ? 4 : 1][2 * TB];
-  __shared__ __attribute__((aligned(16))) float stats[SHARE ? 4 : 1][4][BQ];  // log-sum-exps and r
+  constexpr int KS = D / 16, KH = KS / 2 * NM, MT = D / 32, MH = MT / 2 * NM;  // of the wave's maps
+  constexpr int NW = SHARE ? 4 : 8 / NM, ROWS = SHARE ? 32 : 128, NT = SHARE ? 64 : 64 * NW;
+  constexpr int TB = BQ * Ti::ROWB, MEET = NM == 1 ? 4 * 32 * D * 4 : 0;
+  static_assert(!SHARE || NM == 2, "shared tiles: both maps");
+  constexpr int BUFS = SHARE ? 4 : 2;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[BUFS * 2 * TB > MEET ? BUFS * 2 * TB : MEET];
+  __shared__ __attribute__((aligned(16))) float stats[BUFS][4][BQ];  // log-sum-exps and r
+  __shared__ float lam_sum[NW];
   int bx, h, bb;
   block_tile(a.cu_q, &bx, &h, &bb);
   int q0, q_len, kv0, kv_len;
@@ -1059,8 +1074,7 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
   segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
   const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = SHARE ? lane : threadIdx.x;
-  unsigned char *qt = lds[SHARE ? w : 0], *dt = qt + TB;
-  float(*st4)[BQ] = stats[SHARE ? w : 0];
+  const int map = NM == 1 ? w & 1 : 0, tile = SHARE ? 0 : NM == 1 ? w >> 1 : w;  // first map; key tile
   if (a.rest) {
     zero_rest((T*)a.dk, a.cu_kv, a.total_kv, bb, a.H, D, h, bx, gridDim.x);
     zero_rest((T*)a.dv, a.cu_kv, a.total_kv, bb, a.H, D, h, bx, gridDim.x);
@@ -1074,24 +1088,22 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
   const int64_t sbase = ((int64_t)(tid & 32 ? a.H : 0) + h) * a.total_q + q0;
 
   for (int kt = bx * ROWS; kt < kv_len; kt += gridDim.x * ROWS) {
-    const int ki = kt + (SHARE ? 0 : w * 32) + l32;
+    const int ki = kt + tile * 32 + l32;
     const int64_t krow = kv0 + min(ki, kv_len - 1);
-    Fr kf[KS], vf[KS];
+    Fr kf[KH], vf[KS];
     {
       const T* p = (const T*)a.k + krow * a.ldk + (int64_t)h * D + 8 * hf;
       const T* d = (const T*)a.v + krow * a.ldv + (int64_t)h * D + 8 * hf;
 #pragma unroll
-      for (int st = 0; st < KS; ++st) {
-        kf[st] = F::load(p + 16 * st);
-        vf[st] = F::load(d + 16 * st);
-      }
-    }
-    f32x16_t dk[MT], dv[MT];
+      for (int st = 0; st < KH; ++st) kf[st] = F::load(p + 16 * (map * KH + st));
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      clear(dk[mt]);
-      clear(dv[mt]);
+      for (int st = 0; st < KS; ++st) vf[st] = F::load(d + 16 * st);
     }
+    f32x16_t dk[MH], dv[MT];
+#pragma unroll
+    for (int mt = 0; mt < MH; ++mt) clear(dk[mt]);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) clear(dv[mt]);
     Stage<T, D, BQ, NT> qs, ds;
     float sv[2] = {0.f, 0.f};
     constexpr int STEP = SHARE ? 4 * BQ : BQ;
@@ -1105,67 +1117,97 @@ __global__ void __launch_bounds__(kNT) da_dkv_kernel(const DaArgs a) {
     };
     int qb = SHARE ? w * BQ : 0;
     if (AHEAD) load(qb);
-    for (; qb < q_len; qb += STEP) {
+    for (int buf = 0; qb < q_len; qb += STEP, buf ^= 1) {
+      unsigned char *qt = lds + (SHARE ? w : buf) * 2 * TB, *dt = qt + TB;
+      float(*st4)[BQ] = stats[SHARE ? w : buf];
       if (!AHEAD) load(qb);
-      tile_sync<SHARE>();
+      if (SHARE) tile_sync<SHARE>();
       qs.store(qt, tid);
       ds.store(dt, tid);
       if (SHARE || tid < 64) st4[(tid >> 5) & 1][tid & 31] = sv[0];
       if (SHARE || (tid >= 64 && tid < 128)) st4[2 + ((tid >> 5) & 1)][tid & 31] = sv[1];
       tile_sync<SHARE>();
       if (AHEAD) load(qb + STEP);
-      f32x16_t s1, s2, dp;
-      clear(s1);
-      clear(s2);
+      f32x16_t s[NM], dp;
+#pragma unroll
+      for (int i = 0; i < NM; ++i) clear(s[i]);
       clear(dp);
 #pragma unroll
       for (int st = 0; st < KS; ++st) {
-        F::mma(Ti::row(qt, 0, l32, hf, st), kf[st], st < KS / 2 ? s1 : s2);
         F::mma(Ti::row(dt, 0, l32, hf, st), vf[st], dp);
+        if (st < KH) F::mma(Ti::row(qt, 0, l32, hf, map * KH + st), kf[st], s[st / (KS / 2)]);
       }
-      float p[16], d1[16], d2[16], lsum = 0.f;
+      float p[16], d[NM][16], lsum = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int r = 8 * (j >> 2) + 4 * hf + (j & 3);
-        const float p1 = fast_exp2(fmaf(s1[j], a.sl2, -st4[0][r]));
-        const float q2 = fast_exp2(fmaf(s2[j], a.sl2, -st4[1][r])), p2 = lam * q2;
-        lsum = fmaf(q2, dp[j], lsum);
-        p[j] = p1 - p2;
-        d1[j] = p1 * (dp[j] - st4[2][r]);
-        d2[j] = p2 * (st4[3][r] - dp[j]);
+        if constexpr (NM == 2) {
+          const float p1 = fast_exp2(fmaf(s[0][j], a.sl2, -st4[0][r]));
+          const float q2 = fast_exp2(fmaf(s[1][j], a.sl2, -st4[1][r])), p2 = lam * q2;
+          lsum = fmaf(q2, dp[j], lsum);
+          p[j] = p1 - p2;
+          d[0][j] = p1 * (dp[j] - st4[2][r]);
+          d[1][j] = p2 * (st4[3][r] - dp[j]);
+        } else {
+          p[j] = fast_exp2(fmaf(s[0][j], a.sl2, -st4[map][r]));
+          lsum = fmaf(p[j], dp[j], lsum);
+          d[0][j] = p[j] * (dp[j] - st4[2 + map][r]);
+        }
       }
-      if (ki < kv_len) dlam -= lsum;  // lanes past the last key repeat it
+      if (ki < kv_len && (NM == 2 || map == 1)) dlam -= lsum;  // lanes past the last key repeat it
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const Fr pf = F::pack(p + 8 * g), f1 = F::pack(d1 + 8 * g), f2 = F::pack(d2 + 8 * g);
+        const Fr pf = F::pack(p + 8 * g);
+        Fr df[NM];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) df[i] = F::pack(d[i] + 8 * g);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           F::mma(Ti::col(dt, 0, lane, g, mt), pf, dv[mt]);
-          F::mma(Ti::col(qt, 0, lane, g, mt), mt < MT / 2 ? f1 : f2, dk[mt]);
+          if (mt < MH) F::mma(Ti::col(qt, 0, lane, g, map * MH + mt), df[mt / (MT / 2)], dk[mt]);
         }
       }
     }
     if (SHARE) {
-      join_waves<MT>((float*)lds, w, lane, dk);
+      join_waves<MH>((float*)lds, w, lane, dk);
       join_waves<MT>((float*)lds, w, lane, dv);
+    } else {
+      __syncthreads();  // every wave has left the buffers
+    }
+    if constexpr (NM == 1) {
+      float* meet = (float*)lds + tile * 32 * D + lane;
+      if (map == 1)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) meet[(16 * mt + j) * 64] = lam * dv[mt][j];
+      __syncthreads();
+      if (map == 0)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) dv[mt][j] -= meet[(16 * mt + j) * 64];
+      __syncthreads();
     }
     if (ki < kv_len && (!SHARE || w == 0)) {
       const int64_t at = ((int64_t)(kv0 + ki) * a.H + h) * D;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        store_dims((T*)a.dk + at + 32 * mt, hf, dk[mt], scale);
-        store_dims((T*)a.dv + at + 32 * mt, hf, dv[mt], 1.f);
-      }
+      for (int mt = 0; mt < MH; ++mt)
+        store_dims((T*)a.dk + at + 32 * (map * MH + mt), hf, dk[mt], map == 1 ? -lam * scale : scale);
+      if (map == 0)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) store_dims((T*)a.dv + at + 32 * mt, hf, dv[mt], 1.f);
     }
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) dlam += __shfl_xor(dlam, off, 64);
+  if (lane == 0) lam_sum[w] = dlam;
   __syncthreads();
-  if (lane == 0) stats[0][0][w] = dlam;
-  __syncthreads();
-  if (threadIdx.x == 0)
-    a.lam_part[((int64_t)h * gridDim.z + bb) * gridDim.x + bx] =
-        (stats[0][0][0] + stats[0][0][1]) + (stats[0][0][2] + stats[0][0][3]);
+  if (threadIdx.x == 0) {
+    float t = lam_sum[0];
+    for (int i = 1; i < NW; ++i) t += lam_sum[i];
+    a.lam_part[((int64_t)h * gridDim.z + bb) * gridDim.x + bx] = t;
+  }
 }
 
 // ------------------------------------------------------------------------------- host
@@ -1322,8 +1364,9 @@ int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const vo
     }
     {
       ProfScope p(ctx, "diff_attention_dkv");
-      if (rk == 32) da_dkv_kernel<T, D, true><<<gk, kNT, 0, ctx->stream>>>(a);
-      else da_dkv_kernel<T, D, false><<<gk, kNT, 0, ctx->stream>>>(a);
+      constexpr int NM = sizeof(T) == 2 && D == 128 ? 1 : 2;
+      if (rk == 32) da_dkv_kernel<T, D, true, 2><<<gk, kNT, 0, ctx->stream>>>(a);
+      else da_dkv_kernel<T, D, false, NM><<<gk, 512 / NM, 0, ctx->stream>>>(a);
     }
     ProfScope p(ctx, "diff_attention_dq");
     if (rq == 32) da_dq_kernel<T, D, true><<<gq, kNT, 0, ctx->stream>>>(a);
