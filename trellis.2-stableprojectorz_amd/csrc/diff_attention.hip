@@ -297,10 +297,12 @@ __device__ __forceinline__ void forward_step(const unsigned char* kt, const unsi
 #pragma unroll
     for (int st = i * KS / 2; st < (i + 1) * KS / 2; ++st)
       F::mma(Ti::row(kt, r0, l32, hf, st), qf[st], s);
-    if (k0 + 32 > k_hi)  // uniform
+    if (k0 + 32 > k_hi) {  // uniform; the asm keeps it a branch
+      asm volatile("");
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         if (k0 + 8 * (j >> 2) + 4 * hf + (j & 3) >= k_hi) s[j] = -INFINITY;
+    }
     float mx = s[0], p[16];
 #pragma unroll
     for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
@@ -1017,17 +1019,19 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && !SHARE ? 2 : 1) da_dq_k
         F::mma(Ti::row(kt, 0, l32, hf, st), qf[st], st < KS / 2 ? s1 : s2);
         F::mma(Ti::row(vt, 0, l32, hf, st), df[st], dp);
       }
-      if (kb + BK > kv_len)  // uniform
+      if (kb + BK > kv_len) {  // uniform; the asm keeps it a branch, 48 instructions that no other tile needs
+        asm volatile("");
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (kb + 8 * (j >> 2) + 4 * hf + (j & 3) >= kv_len) s1[j] = s2[j] = -INFINITY;
+      }
       float d1[16], d2[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const float p1 = fast_exp2(fmaf(s1[j], a.sl2, -l1));
         const float p2 = fast_exp2(fmaf(s2[j], a.sl2, -l2));
         d1[j] = p1 * (dp[j] - r1);
-        d2[j] = p2 * ((dp[j] - r2) * nlam);
+        d2[j] = p2 * (dp[j] - r2);
       }
       const Fr f1[2] = {F::pack(d1), F::pack(d1 + 8)}, f2[2] = {F::pack(d2), F::pack(d2 + 8)};
 #pragma unroll
@@ -1041,7 +1045,8 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && !SHARE ? 2 : 1) da_dq_k
     if (qi < q_len && (!SHARE || w == 0)) {
       T* p = (T*)a.dq + ((int64_t)(q0 + qi) * a.H + h) * D;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) store_dims(p + 32 * mt, hf, acc[mt], scale);
+      for (int mt = 0; mt < MT; ++mt)
+        store_dims(p + 32 * mt, hf, acc[mt], mt < MT / 2 ? scale : nlam * scale);
     }
   }
 }
