@@ -356,7 +356,7 @@ __device__ __forceinline__ void forward_store(const DaArgs& a, int h, int64_t ro
 
 // fp32, whole sequences: a block of 4 waves owns 128 queries and walks the keys in tiles of 32.
 template <int D>
-__global__ void __launch_bounds__(kNT) da_forward32_kernel(const DaArgs a) {
+__global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) da_forward32_kernel(const DaArgs a) {
   typedef float T;
   typedef Frag<T> F;
   typedef Tile<T, D> Ti;
