@@ -10,7 +10,10 @@ value is below its normal range (half its smallest step):
   dP, r       fp32 dot products of D terms; r = do . (P v) is taken from outputs rounded to the type, so
               it is off by sum |do| times their tolerances
   dS          P (error of dP and r) + (u + e) |dS|; dq, dk: their sums against |k|, |q|, one rounding
-  dv          (u + e) (P1 + |lambda| P2)^T |do| (the difference is one rounded number), one rounding
+  dv          (u + e) (P1 + |lambda| P2)^T |do|, one rounding.  The kernel rounds the difference of the
+              maps once, or (D = 128 in 16 bits, blocks of 128 keys) P1 and P2 each and takes P2's product
+              with do times lambda: relative errors are at most the same, u (P1 + |lambda| P2); below
+              fp16's normal range the two are off by up to 2^-25 each, that is (1 + |lambda|) 2^-25
   dlambda     - sum P2 dP, from unrounded fp32 values: e of the sum of P2 |dP|, and dP's error
 Sums of fp32 products: 2^-20 of the sum of the sizes (fewer than 16 roundings on a term's way through
 the accumulator at equal size; rows here are at most 9000 long)."""
@@ -82,7 +85,7 @@ def _oracle(q, k, v, do, lam, cq, ck, dtype, scale=None):
             ad * (out.abs() + al * O[1].abs())).sum(2, keepdim=True)
         p = P[0] - lm * P[1]
         r["dv"][:, c] = p.transpose(1, 2) @ ds
-        ep = (u + E[0]) * P[0] + al * (u + E[1]) * P[1] + sub
+        ep = (u + E[0]) * P[0] + al * (u + E[1]) * P[1] + (1 + al) * sub
         t["dv"][:, c] = (ep + ACC * (P[0] + al * P[1])).transpose(1, 2) @ ad
         for i, (m, x, e_r, f_) in enumerate(((slice(0, half), r1, e_r1, 1.0), (slice(half, d), r2, e_r2, -lm))):
             dS = P[i] * (dP - x) * f_

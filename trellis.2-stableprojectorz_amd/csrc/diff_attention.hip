@@ -22,7 +22,8 @@
 // eight 32x32x2 products of the same elements in fp32.  P and dS are rounded to the input type for the
 // second products (as v and k are stored); softmax, sums and accumulators are fp32.
 // No atomics: dq and (dk, dv) come from two kernels, each owning its rows, which costs the scores and
-// dP twice (28 D instead of 20 D flops a pair) and keeps the bits of a result fixed.
+// dP twice (14 D instead of 10 D flops a pair; 18 D where a wave has one map, D = 128 in 16 bits) and
+// keeps the bits of a result fixed.
 
 #include <float.h>
 
@@ -1223,34 +1224,59 @@ unsigned tiles_of(int64_t longest, int64_t hb, int rows = kBQ) {
   return (unsigned)std::max<int64_t>(
       1, std::min<int64_t>(std::min<int64_t>((longest + rows - 1) / rows, 65535), (INT32_MAX / 16) / hb));
 }
-// Rows of a block of one wave per SIMD: 128, or 32 that its waves share.  Blocks of 32 are a quarter of
-// the work each, and waste less of the last round over the CUs; alone they take longer for the joining
-// and for copies that no other wave shares, measured as 1.1-1.2 times in fp32 and 1.4-1.6 in 16 bits.
-// Gradients, us, blocks of 128 / of 32: fp32 8 x 64, 1024 tokens (64 blocks of 128) 296 / 99, 2048 (128)
-// 573 / 338; bf16 12 x 128, 512 (48) 75 / 46, 1024 (96) 133 / 119, 1536 (144) 187 / 218, 3008 (288) 670 / 603.
-int block_rows(int32_t dtype, int64_t longest, int64_t hb) {
+// Rows of a block: 128, or 32 that its waves share.  Blocks of 32 are a quarter of the work each, and
+// waste less of the last round over the CUs, but take longer for the joining and for copies that no other
+// wave shares: `cost` tenths of a quarter of the other's time.  Measured, us, in blocks of 128 / of 32
+// rows (the number of 128): fp32 8 x 64, dk and dv, 1024 tokens (64) 165 / 57, 2900 (184) 459 / 397,
+// 4096 (256) 640 / 722, 5000 (320) 1553 / 1109; bf16 12 x 128, dk and dv, 512 (48) 38 / 27, 768 (72)
+// 49 / 56, 1024 (96) 61 / 67; bf16 16 x 64, dq, 1024 (128) 29 / 23, 1536 (192) 40 / 42, its dk and dv
+// 39 / 41 and 55 / 79.
+constexpr int kCostF32 = 12, kCost16 = 25, kCost16Dq64 = 15;
+int block_rows(int cost, int64_t longest, int64_t hb) {
   const int64_t b = (int64_t)tiles_of(longest, hb) * hb, rounds = (b + kCUs - 1) / kCUs;
-  const int64_t quarters = (4 * b + kCUs - 1) / kCUs;
-  return (dtype == TSC_F32 ? 12 * quarters < 40 * rounds : 15 * quarters < 40 * rounds) ? 32 : kBQ;
+  return cost * ((4 * b + kCUs - 1) / kCUs) < 40 * rounds ? 32 : kBQ;
+}
+int dkv_rows(int32_t dtype, int64_t max_kv, int64_t hb) {
+  return block_rows(dtype == TSC_F32 ? kCostF32 : kCost16, max_kv, hb);
+}
+int dq_rows(int32_t dtype, int32_t D, int64_t max_q, int64_t hb) {
+  return block_rows(dtype == TSC_F32 ? kCostF32 : D == 64 ? kCost16Dq64 : kCost16, max_q, hb);
 }
 
-// The forward pass' blocks: query rows of each, and the parts of the keys.
+// The forward pass' blocks: query rows of each, and the parts of the keys.  Fewer blocks than CUs take
+// the keys in parts, which da_join_kernel adds up, as many as run at once: two blocks of four waves on a
+// CU (one query on 30000 keys, 16 x 64: 36 us, and 50 with one; 128 and 70 on 20000 and 9000: 53, 83), or
+// one of eight at D = 128 in 16 bits.  There up to 32 queries have blocks of 64 rows and four waves (one
+// query on each of 4 sequences, 32071 keys, 12 x 128: 43 us instead of 52; 33 rows: 41 instead of 32), in
+// parts of 1024 keys or more (16 and 9 queries on 20000 and 9000 keys, 8 x 128: 32 us, 39 from 512 on).
+// Grids of kCUs blocks are not split (900 + 700 tokens, 16 x 64, 256 blocks: 25 us, and 55 in two parts).
 struct Plan {
   int rows, splits, part_keys;
 };
-Plan da_plan(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv, int32_t H, int64_t max_q,
-             int64_t max_kv) {
+Plan da_plan(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv, int32_t H, int32_t D,
+             int64_t max_q, int64_t max_kv) {
   const int64_t hb = (int64_t)H * B;
   max_q = std::max(max_q, (total_q + B - 1) / B);  // whatever the caller thinks: parts x rows of scratch
-  Plan p = {dtype == TSC_F32 ? block_rows(dtype, max_q, hb) : kBQ, 1, INT32_MAX};
+  Plan p = {kBQ, 1, INT32_MAX};
+  int64_t slots = kCUs, least = 512;  // blocks that run at once, keys a part has at least
+  if (dtype == TSC_F32) {
+    p.rows = block_rows(kCostF32, max_q, hb);
+    least = 256;
+  } else if (D == 64) {
+    slots = 2 * kCUs;
+  } else if (max_q <= 32) {  // four waves instead of eight
+    p.rows = 64;
+    slots = 2 * kCUs;
+    least = 1024;
+  }
   const int64_t blocks = (int64_t)tiles_of(max_q, hb, p.rows) * hb;
   if (blocks >= kCUs) return p;
-  // Parts of one size, so that long sequences get more of them, and no more blocks than CUs: of n a
-  // sequence's query tiles and heads can have sum ceil(keys / part) <= total / part + B.
-  const int64_t n = kCUs / (blocks / B) - B;
+  // Parts of one size, so that long sequences get more of them, and no more blocks than run at once: of
+  // n a sequence's query tiles and heads can have, sum ceil(keys / part) <= total / part + B.
+  const int64_t n = slots / (blocks / B) - B;
   if (n <= 0) return p;
-  const int64_t part = std::max<int64_t>(dtype == TSC_F32 ? 256 : 512, ((total_kv + n - 1) / n + 63) / 64 * 64);
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((max_kv + part - 1) / part, kCUs));
+  const int64_t part = std::max<int64_t>(least, ((total_kv + n - 1) / n + 63) / 64 * 64);
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((max_kv + part - 1) / part, slots));
   if (p.splits > 1) p.part_keys = (int)std::min<int64_t>(part, INT32_MAX);
   return p;
 }
@@ -1295,8 +1321,8 @@ int64_t diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q
                                        int32_t D, int32_t max_q, int32_t max_kv, int32_t backward) {
   if (B == 0 || total_q == 0) return 0;
   const int64_t hb = (int64_t)H * B;
-  if (backward) return 4 * (2 * (int64_t)H * total_q + hb * tiles_of(max_kv, hb, block_rows(dtype, max_kv, hb)));
-  const int s = da_plan(dtype, B, total_q, total_kv, H, max_q, max_kv).splits;
+  if (backward) return 4 * (2 * (int64_t)H * total_q + hb * tiles_of(max_kv, hb, dkv_rows(dtype, max_kv, hb)));
+  const int s = da_plan(dtype, B, total_q, total_kv, H, D, max_q, max_kv).splits;
   return s > 1 ? 4 * (int64_t)s * total_q * H * 2 * (D + 4) : 0;
 }
 
@@ -1309,7 +1335,7 @@ int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* 
   a.out = out;
   a.out2 = out2;
   a.lse = lse;
-  const Plan plan = da_plan(x.dtype, x.B, x.total_q, x.total_kv, x.H, x.max_q, x.max_kv);
+  const Plan plan = da_plan(x.dtype, x.B, x.total_q, x.total_kv, x.H, x.D, x.max_q, x.max_kv);
   a.splits = plan.splits;
   a.part_keys = plan.part_keys;
   a.part = (float*)ws;
@@ -1324,9 +1350,18 @@ int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* 
         if (plan.rows == 32) da_few32_kernel<D><<<grid, kNT, 0, ctx->stream>>>(a);
         else da_forward32_kernel<D><<<grid, kNT, 0, ctx->stream>>>(a);
       } else {
-        constexpr int NM = D == 64 ? 2 : 1, NW = 8 / NM;
-        if (a.lse) da_forward16_kernel<T, D, NM, NW, true><<<grid, 64 * NW, 0, ctx->stream>>>(a);
-        else da_forward16_kernel<T, D, NM, NW, false><<<grid, 64 * NW, 0, ctx->stream>>>(a);
+        auto run = [&](auto nm, auto nw) {
+          constexpr int NM = decltype(nm)::value, NW = decltype(nw)::value;
+          if (a.lse) da_forward16_kernel<T, D, NM, NW, true><<<grid, 64 * NW, 0, ctx->stream>>>(a);
+          else da_forward16_kernel<T, D, NM, NW, false><<<grid, 64 * NW, 0, ctx->stream>>>(a);
+        };
+        constexpr std::integral_constant<int, 1> I1{};
+        constexpr std::integral_constant<int, 2> I2{};
+        constexpr std::integral_constant<int, 4> I4{};
+        constexpr std::integral_constant<int, 8> I8{};
+        if constexpr (D == 64) run(I2, I4);
+        else if (plan.rows == 64) run(I1, I4);
+        else run(I1, I8);
       }
     }
     if (a.splits > 1) {
@@ -1355,7 +1390,7 @@ int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const vo
   float* lam_part = r12 + 2 * (int64_t)x.H * x.total_q;
   a.r12 = r12;
   a.lam_part = lam_part;
-  const int rq = block_rows(x.dtype, x.max_q, hb), rk = block_rows(x.dtype, x.max_kv, hb);
+  const int rq = dq_rows(x.dtype, x.D, x.max_q, hb), rk = dkv_rows(x.dtype, x.max_kv, hb);
   const dim3 gq(tiles_of(x.max_q, hb, rq), (unsigned)x.H, (unsigned)x.B);
   const dim3 gk(tiles_of(x.max_kv, hb, rk), (unsigned)x.H, (unsigned)x.B);
   a.lam_parts = (int)gk.x * x.B;
