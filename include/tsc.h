@@ -332,10 +332,11 @@ int tsc_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, con
  *     k and v may be slices of one fused projection); all other buffers are contiguous
  *   lambda     device fp32 (num_heads)
  *   cu_seqlens_q / cu_seqlens_kv, scale, max_seqlen_q  as in tsc_attention, scale <= 0 meaning
- *     1/sqrt(head_dim / 2); max_seqlen_kv likewise (it sizes the workspace too: the same values there).  A sequence without keys gives zeros.
- *   zero_rest  rows of out (and out2) outside every sequence: 0 = left as they were, 1 = zeroed
- *   out2, lse  both NULL, or for the backward pass: out2 (total_q, num_heads, head_dim) `dtype` holds
- *     P2 v, lse fp32 (2, num_heads, total_q) the maps' log2-sum-exps
+ *     1/sqrt(head_dim / 2); max_seqlen_kv likewise (both size the workspace too: the same values
+ *     there).  A sequence without keys gives zeros.
+ *   zero_rest  rows of out outside every sequence: 0 = left as they were, 1 = zeroed
+ *   maps, lse  both NULL, or for the backward pass: maps fp32 (total_q, num_heads, 2, head_dim) takes
+ *     P1 v and P2 v, lse fp32 (2, num_heads, total_q) the maps' log2-sum-exps (rows of the sequences)
  *   workspace  device scratch of tsc_diff_attention_workspace_bytes(..., backward = 0) bytes (few
  *     queries on many keys are shared out over blocks and joined), 16-byte aligned, NULL if that is
  *     0.  The context keeps nothing, so calls with scratch of their own may overlap and be captured.
@@ -350,7 +351,7 @@ int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k
                        const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv, int32_t B,
                        int64_t total_q, int64_t total_kv, int32_t num_heads, int32_t head_dim,
                        float scale, int32_t max_seqlen_q, int32_t max_seqlen_kv, int32_t zero_rest,
-                       void* workspace, void* out, void* out2, float* lse);
+                       void* workspace, void* out, float* maps, float* lse);
 /* Its gradient from dout (total_q, num_heads, head_dim) and what the forward call was given and
  * wrote: dq (total_q, ...), dk and dv (total_kv, num_heads, head_dim) `dtype`, dlambda fp32
  * (num_heads) or NULL.  zero_rest is about rows of dq, dk and dv.  workspace with backward = 1.  The
@@ -361,9 +362,8 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
                                 const int32_t* cu_seqlens_kv, int32_t B, int64_t total_q,
                                 int64_t total_kv, int32_t num_heads, int32_t head_dim, float scale,
                                 int32_t max_seqlen_q, int32_t max_seqlen_kv, int32_t zero_rest,
-                                const void* out, const void* out2, const float* lse,
-                                const void* dout, void* workspace, void* dq, void* dk, void* dv,
-                                float* dlambda);
+                                const float* maps, const float* lse, const void* dout,
+                                void* workspace, void* dq, void* dk, void* dv, float* dlambda);
 
 /* ---- safetensors weight files -------------------------------------------------------------- */
 /* Element types of a safetensors header ("dtype" strings).  F32/F16/BF16 equal TSC_F32/F16/BF16. */

@@ -56,5 +56,5 @@ def test_c_entry_points_without_a_gpu(pkg):
     assert st == 1 and b"null context" in lib.tsc_last_error()
     st = lib.tsc_diff_attention_backward(None, 0, P(16), P(16), P(16), 64, 64, 64, P(16), P(16), P(16),
                                          1, 1, 1, 1, 64, 0.0, 1, 1, 0, P(16), P(16), P(16), P(16),
-                                         P(16), P(16), P(16), P(16), None)
+                                         P(16), P(16), P(16), None)
     assert st == 1 and b"null context" in lib.tsc_last_error()

@@ -7,8 +7,8 @@ value is below its normal range (half its smallest step):
               denominator's), and 2^-20 for the exponential and the sums
   P v         each P is rounded to the type once: (u + e) of sum P |v|
   out         that of both maps, and one rounding: u |out|
-  dP, r       fp32 dot products of D terms; r = do . (P v) is taken from outputs rounded to the type, so
-              it is off by sum |do| times their tolerances
+  dP, r       fp32 dot products of D terms; r = do . (P v) is taken from sums in fp32 of the rounded P over
+              the sum of the rounded P: off by sum |do| times (2 u + e) of sum P |v|
   dS          P (error of dP and r) + (u + e) |dS|; dq, dk: their sums against |k|, |q|, one rounding
   dv          (u + e) (P1 + |lambda| P2)^T |do|, one rounding.  The kernel rounds the difference of the
               maps once, or (D = 128 in 16 bits, blocks of 128 keys) P1 and P2 each and takes P2's product
@@ -76,13 +76,10 @@ def _oracle(q, k, v, do, lam, cq, ck, dtype, scale=None):
         r["out"][:, a] = out
         t1 = tO[0] + al * tO[1]
         t["out"][:, a] = t1 + u * out.abs() + sub
-        t_out, t_out2 = t["out"][:, a], tO[1] + u * O[1].abs() + sub
         dP = ds @ vs.transpose(1, 2)
         e_dP = (d + 4) * 2.0 ** -24 * (ad @ av.transpose(1, 2))
         r1, r2 = (ds * O[0]).sum(2, keepdim=True), (ds * O[1]).sum(2, keepdim=True)
-        e_r2 = (ad * t_out2).sum(2, keepdim=True) + ACC * (ad * O[1].abs()).sum(2, keepdim=True)
-        e_r1 = (ad * (t_out + al * t_out2)).sum(2, keepdim=True) + ACC * (
-            ad * (out.abs() + al * O[1].abs())).sum(2, keepdim=True)
+        e_r1, e_r2 = ((ad * (tO[i] + u * (P[i] @ av) + ACC * O[i].abs())).sum(2, keepdim=True) for i in (0, 1))
         p = P[0] - lm * P[1]
         r["dv"][:, c] = p.transpose(1, 2) @ ds
         ep = (u + E[0]) * P[0] + al * (u + E[1]) * P[1] + (1 + al) * sub
@@ -193,6 +190,36 @@ def test_moving_maxima(pkg, dev, dtype, d):
     got = _run(pkg, dev, q, k, v, do, lam, [0, n], None)
     for name in got:
         _close(got[name], want[name], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_peaked_maps_keep_dq(pkg, dev, dtype, d):
+    """Scores of standard deviation 4, where dS = P (dP - r) cancels: an r from rounded outputs would be most of
+    dq's error.  A rounding's mean square is at most (u x)^2 / 3, and those of P, dS and dq are independent:
+      |dq error|^2 <= u^2 / 3 (dq^2 + z^2 sum_m dS^2 k^2 + z^2 (sum_m P k)^2 sum_j do_j^2 sum_m P^2 (v - P v)^2)
+    summed over all values (P's roundings are in the numerator and the denominator of P v, whence v - P v;
+    fp32's own errors are 2^-13 of this).  With r from rounded outputs it would be 1.07."""
+    n, h, half = 700, 4, d // 2
+    q, k, v, do, lam = _make([n], [n], h, d, dtype, 3, spread=2.0)
+    got = _run(pkg, dev, q, k, v, do, lam, [0, n], None)["dq"].double().cpu().transpose(0, 1)
+    Q, K, V, DO = (t.double().transpose(0, 1) for t in (q, k, v, do))
+    z, u = 1 / math.sqrt(half), torch.finfo(dtype).eps / 2
+    err = var = 0.0
+    for i, f in enumerate((torch.ones(h, 1, 1, dtype=torch.float64), -lam.double().view(h, 1, 1))):
+        m = slice(i * half, (i + 1) * half)
+        P = torch.softmax(Q[..., m] @ K[..., m].transpose(1, 2) * z, 2)
+        O = P @ V
+        dS = P * (DO @ V.transpose(1, 2) - (DO * O).sum(2, keepdim=True)) * f
+        dq = dS @ K[..., m] * z
+        err += (got[..., m] - dq).square().sum()
+        p2 = P.square()
+        spread = p2 @ V.square() - 2 * O * (p2 @ V) + O.square() * p2.sum(2, keepdim=True)
+        r = (DO.square() * spread).sum(2, keepdim=True) * (f * z * (P @ K[..., m])).square()
+        var += (dq.square() + z * z * (dS.square() @ K[..., m].square()) + r).sum() * u * u / 3
+    ratio = math.sqrt(err / var)
+    print(f"    peaked maps {dtype} D={d}: dq error {ratio:.3f} of the roundings' bound", flush=True)
+    assert ratio <= 1.0
 
 
 def test_gradient_against_differences(pkg, dev):
@@ -306,6 +333,19 @@ def test_hints_below_the_lengths_with_shared_keys(pkg, dev, dtype):
                    max_seqlen_q=mq, max_seqlen_kv=mk)
         for n in got:
             _close(got[n], want[n], f"{n} ({mq}, {mk})")
+
+
+def test_incoming_gradient_at_an_odd_address(pkg, dev):
+    """The gradient of a result that was joined to one value is a view 2 bytes into a larger one."""
+    lens, h, d, dtype = [40, 9], 2, 64, torch.bfloat16
+    q, k, v, do, lam = _make(lens, lens, h, d, dtype, 4)
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v, lam)]
+    o = pkg.sparse_diff_attention(*leaves, _cu(lens))
+    w = torch.cat([torch.ones(1, dtype=dtype), do.flatten()]).to(dev)
+    got = torch.autograd.grad((torch.cat([o.new_ones(1), o.flatten()]) * w).sum(), leaves)
+    want = torch.autograd.grad(pkg.sparse_diff_attention(*leaves, _cu(lens)), leaves, do.to(dev))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
 
 
 def test_block_without_gradients(pkg, dev):

@@ -33,15 +33,18 @@ class GroupNorm(torch.autograd.Function):
 class DiffAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, cq, ck, b, scale, max_q, max_kv):
-        out, out2, lse = ops._diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, None, True)
-        ctx.save_for_backward(q, k, v, lam, out, out2, lse, cq, ck)
+        out, maps, lse = ops._diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, None, True)
+        ctx.save_for_backward(q, k, v, lam, maps, lse, cq, ck)
         ctx.args = (b, scale, max_q, max_kv)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, lam, out, out2, lse, cq, ck = ctx.saved_tensors
-        grads = ops._diff_attention_backward(do.contiguous(), q, k, v, lam, out, out2, lse, cq, ck,
+        q, k, v, lam, maps, lse, cq, ck = ctx.saved_tensors
+        do = do.contiguous()
+        if do.data_ptr() % 16:  # a view into a larger gradient
+            do = do.clone()
+        grads = ops._diff_attention_backward(do, q, k, v, lam, maps, lse, cq, ck,
                                              *ctx.args)
         return (*grads, None, None, None, None, None, None)

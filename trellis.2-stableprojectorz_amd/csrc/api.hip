@@ -803,7 +803,7 @@ int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k
                        const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv, int32_t B,
                        int64_t total_q, int64_t total_kv, int32_t num_heads, int32_t head_dim,
                        float scale, int32_t max_seqlen_q, int32_t max_seqlen_kv, int32_t zero_rest,
-                       void* workspace, void* out, void* out2, float* lse) {
+                       void* workspace, void* out, float* maps, float* lse) {
   g_err[0] = 0;
   int st = check_ctx(ctx);
   if (st) return st;
@@ -814,23 +814,25 @@ int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k
   if (st) return st;
   if (B == 0 || total_q == 0) return TSC_OK;
   if (!out) return fail(TSC_ERR_INVALID, "diff_attention: null buffer");
-  if ((out2 == nullptr) != (lse == nullptr))
-    return fail(TSC_ERR_INVALID, "diff_attention: out2 and lse go together");
+  if ((maps == nullptr) != (lse == nullptr))
+    return fail(TSC_ERR_INVALID, "diff_attention: maps and lse go together");
   const int64_t need = diff_attention_workspace_bytes(dtype, B, total_q, total_kv, num_heads, head_dim,
                                                       max_seqlen_q, max_seqlen_kv, 0);
   if (need > 0 && !workspace) return fail(TSC_ERR_INVALID, "diff_attention: null workspace");
-  if (!aligned(out, 16) || !aligned(out2, 16) || !aligned(lse, 4) || !aligned(workspace, 16))
-    return fail(TSC_ERR_INVALID, "diff_attention: out, out2 and workspace must be 16-byte aligned");
+  if (!aligned(out, 16) || !aligned(maps, 16) || !aligned(lse, 4) || !aligned(workspace, 16))
+    return fail(TSC_ERR_INVALID, "diff_attention: out, maps and workspace must be 16-byte aligned");
   const size_t no = row_span(total_q, (int64_t)num_heads * head_dim, x);
-  for (const void* o : {(const void*)out, (const void*)out2})
-    if (o && (overlaps(o, no, q, row_span(total_q, ld_q, x)) ||
-              overlaps(o, no, k, row_span(total_kv, ld_k, x)) ||
-              overlaps(o, no, v, row_span(total_kv, ld_v, x))))
+  const size_t nm = (size_t)total_q * num_heads * head_dim * 8;
+  const void* outs[2] = {out, maps};
+  for (int i = 0; i < 2; ++i)
+    if (outs[i] && (overlaps(outs[i], i ? nm : no, q, row_span(total_q, ld_q, x)) ||
+                    overlaps(outs[i], i ? nm : no, k, row_span(total_kv, ld_k, x)) ||
+                    overlaps(outs[i], i ? nm : no, v, row_span(total_kv, ld_v, x))))
       return fail(TSC_ERR_INVALID, "diff_attention: out overlaps an input");
-  if (out2 && overlaps(out, no, out2, no))
-    return fail(TSC_ERR_INVALID, "diff_attention: out overlaps out2");
+  if (maps && overlaps(out, no, maps, nm))
+    return fail(TSC_ERR_INVALID, "diff_attention: out overlaps maps");
   DeviceGuard g(ctx->device);
-  return diff_attention_launch(ctx, x, out, out2, lse, workspace);
+  return diff_attention_launch(ctx, x, out, maps, lse, workspace);
 }
 
 int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k,
@@ -839,7 +841,7 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
                                 const int32_t* cu_seqlens_kv, int32_t B, int64_t total_q,
                                 int64_t total_kv, int32_t num_heads, int32_t head_dim, float scale,
                                 int32_t max_seqlen_q, int32_t max_seqlen_kv, int32_t zero_rest,
-                                const void* out, const void* out2, const float* lse,
+                                const float* maps, const float* lse,
                                 const void* dout, void* workspace, void* dq, void* dk, void* dv,
                                 float* dlambda) {
   g_err[0] = 0;
@@ -852,9 +854,9 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
   if (st) return st;
   if (B == 0 || total_q == 0)
     return fail(TSC_ERR_INVALID, "diff_attention_backward: no queries (the gradients are zero)");
-  if (!out || !out2 || !lse || !dout || !workspace || !dq || (total_kv > 0 && (!dk || !dv)))
+  if (!maps || !lse || !dout || !workspace || !dq || (total_kv > 0 && (!dk || !dv)))
     return fail(TSC_ERR_INVALID, "diff_attention_backward: null buffer");
-  const void* a16[7] = {out, out2, dout, workspace, dq, dk, dv};
+  const void* a16[6] = {maps, dout, workspace, dq, dk, dv};
   for (const void* p : a16)
     if (!aligned(p, 16))
       return fail(TSC_ERR_INVALID, "diff_attention_backward: buffers must be 16-byte aligned");
@@ -862,13 +864,13 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
     return fail(TSC_ERR_INVALID, "diff_attention_backward: lse and dlambda must be 4-byte aligned");
   const int64_t ld = (int64_t)num_heads * head_dim;
   const size_t no = row_span(total_q, ld, x), nk = row_span(total_kv, ld, x);
-  const void* ins[6] = {q, k, v, out, out2, dout};
-  const size_t in_bytes[6] = {row_span(total_q, ld_q, x), row_span(total_kv, ld_k, x),
-                              row_span(total_kv, ld_v, x), no, no, no};
+  const void* ins[5] = {q, k, v, maps, dout};
+  const size_t in_bytes[5] = {row_span(total_q, ld_q, x), row_span(total_kv, ld_k, x),
+                              row_span(total_kv, ld_v, x), (size_t)total_q * ld * 8, no};
   const void* gs[3] = {dq, dk, dv};
   const size_t g_bytes[3] = {no, nk, nk};
   for (int i = 0; i < 3; ++i) {
-    for (int j = 0; j < 6; ++j)
+    for (int j = 0; j < 5; ++j)
       if (overlaps(gs[i], g_bytes[i], ins[j], in_bytes[j]))
         return fail(TSC_ERR_INVALID, "diff_attention_backward: a gradient overlaps an input");
     for (int j = 0; j < i; ++j)
@@ -876,7 +878,7 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
         return fail(TSC_ERR_INVALID, "diff_attention_backward: the gradients overlap");
   }
   DeviceGuard g(ctx->device);
-  return diff_attention_backward_launch(ctx, x, out, out2, lse, dout, workspace, dq, dk, dv, dlambda);
+  return diff_attention_backward_launch(ctx, x, maps, lse, dout, workspace, dq, dk, dv, dlambda);
 }
 
 int tsc_st_open(const char* path, tsc_st** out) {

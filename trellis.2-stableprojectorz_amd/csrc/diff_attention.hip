@@ -12,7 +12,7 @@
 // feeds one map or the other by its dimensions, and one walk over the keys serves both.  The two
 // maps' weighted sums of v stay apart until their denominators are known (6 D flops a pair; the
 // difference itself would need 4 D, and two walks).  For the gradient the forward pass keeps
-// P2 v and the two log-sum-exps, and the probabilities are made again from them.
+// P1 v and P2 v in fp32 and the two log-sum-exps, from which the probabilities are made again.
 //
 // Scores are computed in 32 x 32 tiles whose result layout (lane: one column, 16 rows 8(j/4) +
 // 4(lane/32) + j%4) is the operand layout of the next product, contracted over those rows: transposed
@@ -239,7 +239,8 @@ struct DaArgs {
   float sl2;     // scale * log2(e)
   int32_t rest;  // zero the rows outside every sequence
   // forward
-  void *out, *out2;  // out2 = P2 v, or null
+  void* out;
+  float* maps;       // (total_q, H, 2, D): P1 v, P2 v, or null
   float* lse;        // (2, H, total_q): log2 of the sum of 2^(score sl2), or null
   int32_t splits, part_keys;  // small grids: blocks that share a sequence's keys, keys of each
   float* part;       // splits > 1: (splits, total_q, H, 2, D) sums, then (splits, total_q, H, 2, 4)
@@ -344,7 +345,10 @@ __device__ __forceinline__ void forward_store(const DaArgs& a, int h, int64_t ro
   const int64_t at = (row * a.H + h) * D;
 #pragma unroll
   for (int mt = 0; mt < D / 32; ++mt) {
-    if (a.out2) store_dims((T*)a.out2 + at + 32 * mt, hf, o[1][mt], i2);
+    if (a.maps) {
+      store_dims(a.maps + 2 * at + 32 * mt, hf, o[0][mt], i1);
+      store_dims(a.maps + 2 * at + D + 32 * mt, hf, o[1][mt], i2);
+    }
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[0][mt][j] = fmaf(-f2, o[1][mt][j], o[0][mt][j] * i1);
     store_dims((T*)a.out + at + 32 * mt, hf, o[0][mt], 1.f);
@@ -355,7 +359,9 @@ __device__ __forceinline__ void forward_store(const DaArgs& a, int h, int64_t ro
   }
 }
 
-// fp32, whole sequences: a block of 4 waves owns 128 queries and walks the keys in tiles of 32.
+// fp32, whole sequences: a block of 4 waves owns 128 queries and walks the keys in tiles of 32.  Bound by
+// the fp32 matrix cores: 4096 tokens, 8 x 64, 467 us or 110 TFLOP/s of the 154 a large product reaches.
+// At D = 64 two waves per SIMD fill each other's waits; at D = 128 the registers hold one.
 template <int D>
 __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) da_forward32_kernel(const DaArgs a) {
   typedef float T;
@@ -370,10 +376,7 @@ __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) da_forward32_kernel(cons
   segment(a.cu_q, bb, a.total_q, &q0, &q_len);
   segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l32 = lane & 31, hf = lane >> 5;
-  if (a.rest) {
-    zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
-    if (a.out2) zero_rest((T*)a.out2, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
-  }
+  if (a.rest) zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, bx, gridDim.x);
   const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
   const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
 
@@ -413,6 +416,7 @@ __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) da_forward32_kernel(cons
 // fp32, small grids: a block owns 32 queries, and its waves and the blocks of a.splits
 // parts share out the keys, 32 at a time.  Each wave brings its own keys through its own piece of LDS,
 // so none waits for another until the end, where their maxima, denominators and sums are joined.
+// 1024 tokens, 8 x 64 (256 blocks): 46 us, and 132 in the 64 blocks of 128 queries.
 template <int D>
 __global__ void __launch_bounds__(kNT) da_few32_kernel(const DaArgs a) {
   typedef float T;
@@ -430,10 +434,7 @@ __global__ void __launch_bounds__(kNT) da_few32_kernel(const DaArgs a) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: its keys are scalars
   const int sp = bx % a.splits, tile = bx / a.splits, tiles = gridDim.x / a.splits;
-  if (a.rest && sp == 0) {
-    zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, tile, tiles);
-    if (a.out2) zero_rest((T*)a.out2, a.cu_q, a.total_q, bb, a.H, D, h, tile, tiles);
-  }
+  if (a.rest && sp == 0) zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, tile, tiles);
   if (a.splits > 1) {
     take_part(a, sp, &kv0, &kv_len);
     if (kv_len == 0) return;  // the join passes over it
@@ -526,8 +527,10 @@ __global__ void __launch_bounds__(kNT) da_few32_kernel(const DaArgs a) {
 //      exponentials and the reads of k for the step after
 // The exponentials bound it: twice those of one map, a quarter of the VALU's rate each.
 // A wave has NM maps of its 32 queries: both at D = 64; one at D = 128, where the sums of both would
-// leave one wave per SIMD, whose stalls nothing fills (9000 + 6143 tokens, 12 x 128 bf16: 1500 us).  The
-// two waves of a query tile then meet in LDS at the end.
+// leave one wave per SIMD, whose stalls nothing fills (9000 + 6143 tokens, 12 x 128 bf16: 1500 us that way,
+// 1300 us or 840 TFLOP/s now).  The two waves of a query tile then meet in LDS at the end.
+// Counted there: matrix cores busy 37 % and VALU 48 % of the cycles, the clock down to 1.8 - 2.0 GHz; at
+// D = 64 (36011 queries on 7 x 1374 keys, 16 heads, f16: 470 us) 29 % and 70 %.
 // The sums of v are divided by the sum of the rounded P that they were made of.  KEEP (for the backward
 // pass) also adds up the unrounded P: the log-sum-exps have to be those of the fp32 probabilities.
 template <typename T, int D, int NM, int NW, bool KEEP>
@@ -549,10 +552,7 @@ __global__ void __launch_bounds__(64 * NW, 2) da_forward16_kernel(const DaArgs a
   segment(a.cu_q, bb, a.total_q, &q0, &q_len);
   segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
   const int sp = bx % a.splits, qtile = bx / a.splits, qtiles = gridDim.x / a.splits;
-  if (a.rest && sp == 0) {
-    zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, qtile, qtiles);
-    if (a.out2) zero_rest((T*)a.out2, a.cu_q, a.total_q, bb, a.H, D, h, qtile, qtiles);
-  }
+  if (a.rest && sp == 0) zero_rest((T*)a.out, a.cu_q, a.total_q, bb, a.H, D, h, qtile, qtiles);
   if (a.splits > 1) {
     take_part(a, sp, &kv0, &kv_len);
     if (kv_len == 0) return;  // the join passes over it
@@ -572,10 +572,9 @@ __global__ void __launch_bounds__(64 * NW, 2) da_forward16_kernel(const DaArgs a
     const int64_t at = (int64_t)(q0 + qi) * a.H + h;
     if (kv_len == 0) {  // uniform over the block
       if (map == 0 && qi < q_len) {
-        for (int c = hf; c < CPR; c += 2) {
-          *(uint4*)((T*)a.out + at * D + 8 * c) = make_uint4(0, 0, 0, 0);
-          if (a.out2) *(uint4*)((T*)a.out2 + at * D + 8 * c) = make_uint4(0, 0, 0, 0);
-        }
+        for (int c = hf; c < CPR; c += 2) *(uint4*)((T*)a.out + at * D + 8 * c) = make_uint4(0, 0, 0, 0);
+        if (a.maps)
+          for (int c = hf; c < D / 2; c += 2) *(uint4*)(a.maps + at * 2 * D + 4 * c) = make_uint4(0, 0, 0, 0);
         if (a.lse && hf == 0) {
           a.lse[(int64_t)h * a.total_q + q0 + qi] = INFINITY;
           a.lse[(int64_t)(a.H + h) * a.total_q + q0 + qi] = INFINITY;
@@ -812,9 +811,10 @@ __global__ void __launch_bounds__(64 * NW, 2) da_forward16_kernel(const DaArgs a
         lu[i] = pair_sum(lu[i]);
         if (qi < q_len && hf == 0)
           a.lse[(int64_t)((map + i) * a.H + h) * a.total_q + q0 + qi] = mc[i] + log2f(lu[i]);
-        if (map + i == 1 && qi < q_len)
+        if (qi < q_len)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) store_dims((T*)a.out2 + at * D + 32 * mt, hf, o[i][mt], 1.f);
+          for (int mt = 0; mt < MT; ++mt)
+            store_dims(a.maps + (2 * at + map + i) * D + 32 * mt, hf, o[i][mt], 1.f);
       }
     }
     const float lam = a.lambda[h];
@@ -889,8 +889,12 @@ __global__ void __launch_bounds__(kNT) da_join_kernel(const DaArgs a, int32_t B)
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) {
     const int64_t p = at * D + lane + 64 * e;
-    ((T*)a.out)[p] = (T)(o[0][e] * i1 - lam * (o[1][e] * i2));
-    if (a.out2) ((T*)a.out2)[p] = (T)(o[1][e] * i2);
+    const float o1 = o[0][e] * i1, o2 = o[1][e] * i2;
+    ((T*)a.out)[p] = (T)fmaf(-lam, o2, o1);  // one form, whether the maps are stored or not
+    if (a.maps) {
+      a.maps[at * 2 * D + lane + 64 * e] = o1;
+      a.maps[at * 2 * D + D + lane + 64 * e] = o2;
+    }
   }
   if (a.lse && lane == 0) {
     a.lse[(int64_t)h * a.total_q + row] = parts ? m[0] + log2f(lu[0]) : INFINITY;
@@ -899,8 +903,11 @@ __global__ void __launch_bounds__(kNT) da_join_kernel(const DaArgs a, int32_t B)
 }
 
 // ------------------------------------------------------------------------------- backward
-// r_i = do . (P_i v) per query, P1 v = out + lambda P2 v.
+// r_i = do . (P_i v) per query, from the sums in fp32: dS_i = P_i (dP - r_i) cancels where one key has most
+// of a map, and out's rounding would be most of what is left (scores of standard deviation 4: dq off by 0.0042
+// of its norm in bf16 instead of 0.0028).
 // Block: one head, the rows of one sequence in steps of 256 / (D / 8) per grid column.
+// Bound by memory: 13 us for the 70 MB of 7607 queries, 12 x 128 bf16, 5.4 TB/s.
 template <typename T, int D>
 __global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r12) {
   constexpr int LPR = D / 8;  // lanes of a row, 8 elements each
@@ -908,21 +915,23 @@ __global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r
   const int h = blockIdx.y, bb = blockIdx.z, e0 = threadIdx.x % LPR * 8;
   int q0, q_len;
   segment(a.cu_q, bb, a.total_q, &q0, &q_len);
-  const float lam = a.lambda[h];
   for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR; r < q_len;
        r += (int64_t)gridDim.x * RPB) {
     const int64_t at = ((q0 + r) * a.H + h) * D + e0;
-    const T *d = (const T*)a.dout + at, *o = (const T*)a.out + at, *p = (const T*)a.out2 + at;
-    float r1 = 0.f, r2 = 0.f;
+    const T* d = (const T*)a.dout + at;
+    const float* o = a.maps + 2 * (at - e0) + e0;
+    float x[8], r1 = 0.f, r2 = 0.f;
 #pragma unroll
     for (int c = 0; c < 8; c += 16 / sizeof(T)) {
-      const u32x4_t wd = *(const u32x4_t*)(d + c), wo = *(const u32x4_t*)(o + c), wp = *(const u32x4_t*)(p + c);
+      const u32x4_t w = *(const u32x4_t*)(d + c);
 #pragma unroll
-      for (int e = 0; e < (int)(16 / sizeof(T)); ++e) {
-        const float x = (float)((const T*)&wd)[e], y = (float)((const T*)&wp)[e];
-        r1 = fmaf(x, (float)((const T*)&wo)[e], r1);
-        r2 = fmaf(x, y, r2);
-      }
+      for (int e = 0; e < (int)(16 / sizeof(T)); ++e) x[c + e] = (float)((const T*)&w)[e];
+    }
+#pragma unroll
+    for (int c = 0; c < 8; c += 4) {
+      const float4 y = *(const float4*)(o + c), z = *(const float4*)(o + D + c);
+      r1 = fmaf(x[c + 3], y.w, fmaf(x[c + 2], y.z, fmaf(x[c + 1], y.y, fmaf(x[c], y.x, r1))));
+      r2 = fmaf(x[c + 3], z.w, fmaf(x[c + 2], z.z, fmaf(x[c + 1], z.y, fmaf(x[c], z.x, r2))));
     }
 #pragma unroll
     for (int off = LPR / 2; off > 0; off >>= 1) {
@@ -930,7 +939,7 @@ __global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r
       r2 += __shfl_xor(r2, off, 64);
     }
     if (e0 == 0) {
-      r12[(int64_t)h * a.total_q + q0 + r] = fmaf(lam, r2, r1);
+      r12[(int64_t)h * a.total_q + q0 + r] = r1;
       r12[(int64_t)(a.H + h) * a.total_q + q0 + r] = r2;
     }
   }
@@ -940,7 +949,9 @@ __global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r
 // two buffers in LDS; or, where that leaves CUs idle (SHARE), all own the same 32 rows and take the
 // tiles in turn, each through its own piece of LDS, and their sums are joined at the end.
 // Two waves per SIMD in 16 bits: with one, whose products, exponentials and LDS reads wait for each
-// other, a step of dk / dv took 6700 cycles at D = 128, 1024 of them in the matrix cores.
+// other, the matrix cores were busy 15 % of the time in dk / dv at D = 128, now 37 %.
+// 4096 tokens: 12 x 128 bf16, dk and dv 412 us, dq 213 (750 and 730 TFLOP/s executed); 16 x 64 bf16 206
+// and 155 (670); 8 x 64 fp32 638 and 491 (107 of the 154 that a large product reaches).
 template <bool SHARE>
 __device__ __forceinline__ void tile_sync() {
   // A wave's own LDS operations are carried out in order; the compiler has to keep that order.
@@ -1326,14 +1337,14 @@ int64_t diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q
   return s > 1 ? 4 * (int64_t)s * total_q * H * 2 * (D + 4) : 0;
 }
 
-int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* out2, float* lse,
+int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, float* maps, float* lse,
                           void* ws) {
   const int64_t hb = (int64_t)x.H * x.B;
   if (hb > (int64_t)(INT32_MAX / 1024))
     return fail(TSC_ERR_UNSUPPORTED, "diff_attention: %lld (head, sequence) pairs", (long long)hb);
   DaArgs a = da_args(x);
   a.out = out;
-  a.out2 = out2;
+  a.maps = maps;
   a.lse = lse;
   const Plan plan = da_plan(x.dtype, x.B, x.total_q, x.total_kv, x.H, x.D, x.max_q, x.max_kv);
   a.splits = plan.splits;
@@ -1371,15 +1382,14 @@ int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* 
   });
 }
 
-int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const void* out,
-                                   const void* out2, const float* lse, const void* dout, void* ws,
-                                   void* dq, void* dk, void* dv, float* dlambda) {
+int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const float* maps,
+                                   const float* lse, const void* dout, void* ws, void* dq, void* dk,
+                                   void* dv, float* dlambda) {
   const int64_t hb = (int64_t)x.H * x.B;
   if (hb > (int64_t)(INT32_MAX / 1024))
     return fail(TSC_ERR_UNSUPPORTED, "diff_attention: %lld (head, sequence) pairs", (long long)hb);
   DaArgs a = da_args(x);
-  a.out = (void*)out;
-  a.out2 = (void*)out2;
+  a.maps = (float*)maps;
   a.lse = (float*)lse;
   a.dout = dout;
   a.dq = dq;

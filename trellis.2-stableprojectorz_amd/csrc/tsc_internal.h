@@ -247,11 +247,11 @@ struct DiffAttnArgs {
 int64_t diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv,
                                        int32_t H, int32_t D, int32_t max_q, int32_t max_kv,
                                        int32_t backward);
-int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, void* out2, float* lse,
+int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, float* maps, float* lse,
                           void* ws);
-int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const void* out,
-                                   const void* out2, const float* lse, const void* dout, void* ws,
-                                   void* dq, void* dk, void* dv, float* dlambda);
+int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const float* maps,
+                                   const float* lse, const void* dout, void* ws, void* dq, void* dk,
+                                   void* dv, float* dlambda);
 
 // ---- implemented in groupnorm.hip ----
 int64_t groupnorm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C, int32_t groups,

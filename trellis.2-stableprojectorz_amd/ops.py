@@ -607,13 +607,13 @@ def sparse_diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam
 
 
 def _diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, out, keep):
-    """(out, out2, lse); out2 and lse (None unless keep) are what the backward pass needs."""
+    """(out, maps, lse); maps and lse (None unless keep) are what the backward pass needs."""
     tq, h, d = q.shape
     tkv = k.shape[0]
     rest = out is None
     if out is None:
         out = (torch.empty if b else torch.zeros)((tq, h, d), dtype=q.dtype, device=q.device)
-    out2 = torch.empty_like(out) if keep else None
+    maps = torch.empty((tq, h, 2, d), dtype=torch.float32, device=q.device) if keep else None
     lse = torch.empty((2, h, tq), dtype=torch.float32, device=q.device) if keep else None
     if tq and b:
         lib, handle = _lib.stream_handle(q.device.index)
@@ -623,11 +623,11 @@ def _diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, out, keep):
         check(lib.tsc_diff_attention(handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"),
                                      _head_rows(k, "k"), _head_rows(v, "v"), _p(lam), _p(cq), _p(ck), b,
                                      tq, tkv, h, d, scale, max_q, max_kv, int(rest), _p(ws), _p(out),
-                                     _p(out2), _p(lse)))
-    return out, out2, lse
+                                     _p(maps), _p(lse)))
+    return out, maps, lse
 
 
-def _diff_attention_backward(do, q, k, v, lam, out, out2, lse, cq, ck, b, scale, max_q, max_kv):
+def _diff_attention_backward(do, q, k, v, lam, maps, lse, cq, ck, b, scale, max_q, max_kv):
     tq, h, d = q.shape
     tkv = k.shape[0]
     alloc = torch.empty if tq and b else torch.zeros
@@ -642,7 +642,7 @@ def _diff_attention_backward(do, q, k, v, lam, out, out2, lse, cq, ck, b, scale,
         check(lib.tsc_diff_attention_backward(
             handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"), _head_rows(k, "k"),
             _head_rows(v, "v"), _p(lam), _p(cq), _p(ck), b, tq, tkv, h, d, scale, max_q, max_kv, 1,
-            _p(out), _p(out2), _p(lse), _p(do), _p(ws), _p(dq), _p(dk), _p(dv), _p(dlam)))
+            _p(maps), _p(lse), _p(do), _p(ws), _p(dq), _p(dk), _p(dv), _p(dlam)))
     return dq, dk, dv, dlam
 
 
