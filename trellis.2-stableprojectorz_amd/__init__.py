@@ -11,6 +11,9 @@ is not a Python identifier.
   sparse_linear                                  sparse_unet_vae_decoder.ts:48-78)
   sparse_attention,                              varlen attention (sparse/ops/attention.ts:24-79,
   scaled_dot_product_attention                   dense/ops/attention.ts:36-110)
+  group_norm, SparseGroupNorm                    group norm over each sample's rows, with gradients
+  sparse_diff_attention,                         difference of two softmax maps, with gradients, and
+  SparseDiffAttentionBlock3d                     the block around it
   SafetensorsFile, MultiFileLoader               weight files -> device tensors (weights.ts:58-237)
   workloads                                      seeded synthetic voxel shells
 """

@@ -1,10 +1,15 @@
-"""Sparse decoder blocks around the conv: SparseLinear and the ConvNeXt block.
+"""Sparse blocks around the conv: SparseLinear, the ConvNeXt block, group norm and the block of
+differential attention.
 
   SparseLinear            src/sparse/ops/linear.ts:9-29 (nn.Linear per voxel; the TS port
                           multiplies by the (out,in) weight untransposed)
   SparseConvNeXtBlock3d   src/models/sparse_unet_vae_decoder.ts:48-78 and its use at :119-134:
                           h = conv(x); h = LN(h); h = h W0^T + b0; h = silu(LN(h)); out = x + h W2^T + b2
                           (LayerNorm without affine, eps 1e-6, as the TS block calls it)
+  SparseGroupNorm, SparseDiffAttentionBlock3d
+                          over each sample's voxels; no counterpart in the reference, whose blocks
+                          normalize rows (src/sparse/ops/norm.ts:10-140) and attend with one map
+                          (src/sparse/ops/attention.ts:24-79)
 
 Each step is one C-ABI call: the conv (tsc_conv, map cached on x), tsc_layernorm (SiLU fused into
 the second one), and tsc_linear (hipBLASLt GEMM with the bias epilogue; the second linear takes

@@ -907,7 +907,7 @@ __global__ void __launch_bounds__(kNT) da_join_kernel(const DaArgs a, int32_t B)
 // of a map, and out's rounding would be most of what is left (scores of standard deviation 4: dq off by 0.0042
 // of its norm in bf16 instead of 0.0028).
 // Block: one head, the rows of one sequence in steps of 256 / (D / 8) per grid column.
-// Bound by memory: 13 us for the 70 MB of 7607 queries, 12 x 128 bf16, 5.4 TB/s.
+// Bound by memory: 20 us for the 117 MB of 7607 queries, 12 x 128 bf16, 5.8 TB/s.
 template <typename T, int D>
 __global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r12) {
   constexpr int LPR = D / 8;  // lanes of a row, 8 elements each
