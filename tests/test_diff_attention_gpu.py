@@ -320,11 +320,12 @@ def test_hints_and_offsets(pkg, dev):
     assert torch.equal(got, want["out"])
 
 
+@pytest.mark.parametrize("d,longest", [(64, 200), (128, 200), (128, 100)])
 @pytest.mark.parametrize("dtype", TYPES)
-def test_hints_below_the_lengths_with_shared_keys(pkg, dev, dtype):
+def test_hints_below_the_lengths_with_shared_keys(pkg, dev, dtype, d, longest):
     """The parts of the keys reach over sequences far longer than max_seqlen_kv says, with idle parts
     for the short ones; rows behind a wrong max_seqlen_q are still covered."""
-    lq, lkv, h, d = [3, 0, 200, 1], [6000, 100, 2500, 0], 2, 64
+    lq, lkv, h = [3, 0, longest, 1], [6000, 100, 2500, 0], 2
     q, k, v, do, lam = _make(lq, lkv, h, d, dtype, 13)
     cq, ck = _cu(lq), _cu(lkv)
     want = _oracle(q, k, v, do, lam, cq, ck, dtype)
