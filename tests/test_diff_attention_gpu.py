@@ -192,6 +192,20 @@ def test_moving_maxima(pkg, dev, dtype, d):
         _close(got[name], want[name], name)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lkv,h", [([270, 3, 1], [1, 2, 1], 2), ([5000], [1], 16)])
+def test_one_key_has_no_gradient_in_its_scores(pkg, dev, dtype, d, lq, lkv, h):
+    """The softmax of one score is 1 whatever the score: dq and dk are zeros, not what dP - r rounds to."""
+    q, k, v, do, lam = _make(lq, lkv, h, d, dtype, 6)
+    cq, ck = _cu(lq), _cu(lkv)
+    got = _run(pkg, dev, q, k, v, do, lam, cq, ck)
+    for a, b, c, e in zip(cq, cq[1:], ck, ck[1:]):
+        one = e - c == 1
+        assert bool(got["dq"][a:b].any()) != one and bool(got["dk"][c:e].any()) != one
+    assert got["dv"].any()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("d", [64, 128])
 def test_peaked_maps_keep_dq(pkg, dev, dtype, d):

@@ -985,7 +985,7 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && !SHARE ? 2 : 1) da_dq_k
   }
   const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
   const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
-  const float nlam = -a.lambda[h], scale = a.sl2 / kLog2e;
+  const float nlam = -a.lambda[h], scale = kv_len > 1 ? a.sl2 / kLog2e : 0.f;  // one key: P is constant
 
   for (int qt = bx * ROWS; qt < q_len; qt += gridDim.x * ROWS) {
     const int qi = qt + (SHARE ? 0 : w * 32) + l32;
@@ -1099,7 +1099,7 @@ __global__ void __launch_bounds__(SHARE ? kNT : 512 / NM, sizeof(T) == 2 && !SHA
   const T* qbase = (const T*)a.q + (int64_t)q0 * a.ldq + (int64_t)h * D;
   const T* dbase = (const T*)a.dout + ((int64_t)q0 * a.H + h) * D;
   const int64_t ldd = (int64_t)a.H * D;
-  const float lam = a.lambda[h], scale = a.sl2 / kLog2e;
+  const float lam = a.lambda[h], scale = kv_len > 1 ? a.sl2 / kLog2e : 0.f;  // one key: P is constant
   // Thread tid < 128 brings statistic tid / 32 of query tid % 32; of one wave, each lane two.
   float dlam = 0.f;
   const int64_t sbase = ((int64_t)(tid & 32 ? a.H : 0) + h) * a.total_q + q0;
