@@ -163,6 +163,21 @@ def test_gradient_against_differences(pkg, dev):
         assert abs(got - want) <= tol
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("c,lens", [(32, [1, 0, 40, 1]), (13, [1])])
+def test_group_of_one_value_has_no_gradient(pkg, dev, dtype, silu, c, lens):
+    """Its norm is 0 whatever the value: dx is zero, not what gamma dh - A rounds to."""
+    g = torch.Generator().manual_seed(c)
+    cu = [0, *torch.tensor(lens).cumsum(0).tolist()]
+    x, w, b, dy = (torch.randn(s, generator=g).to(dtype).to(dev) for s in ((cu[-1], c), (c,), (c,), (cu[-1], c)))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(pkg.group_norm(*leaves[:1], c, *leaves[1:], cu_rows=cu, silu=silu), leaves, dy)
+    for lo, hi in zip(cu, cu[1:]):
+        assert bool(dx[lo:hi].any()) == (hi - lo > 1)
+    assert db.any() and bool(dw.any()) == (max(lens) > 1)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_spread_beside_a_large_mean(pkg, dev, dtype):
     """Values near 1000 with a spread of 1 (bf16: 16 steps of 8): the variance must not be lost.  The

@@ -625,12 +625,14 @@ __global__ void __launch_bounds__(kNT, 4)
   if (w.live) {
     // dx = rstd gamma dh - rstd A / n - (x - mean) rstd^2 B / n
     float mean[VN], rstd[VN], a[VN], be[VN], ma[VN], mb[VN];
+    const bool alone = (end - beg) * s.cpg == 1;  // a single value's norm is 0 whatever it is: so is dx
     channel_consts<T, VN>(s, b, w.c0, stats, gamma, beta, mean, rstd, a, be);
 #pragma unroll
     for (int e = 0; e < VN; ++e) {
       const float2 m = sg[(w.c0 + e) / s.cpg - gl];
       ma[e] = m.x * rstd[e];
       mb[e] = m.y * rstd[e] * rstd[e];
+      if (alone) a[e] = ma[e] = 0.f;
     }
     auto one = [&](int64_t i, const Pack<T, VN>& px, const Pack<T, VN>& py) {
       float o[VN];
