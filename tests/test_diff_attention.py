@@ -58,3 +58,23 @@ def test_c_entry_points_without_a_gpu(pkg):
                                          1, 1, 1, 1, 64, 0.0, 1, 1, 0, P(16), P(16), P(16), P(16),
                                          P(16), P(16), P(16), None)
     assert st == 1 and b"null context" in lib.tsc_last_error()
+
+
+def test_fp32_grids_of_128_rows_are_not_split(pkg):
+    """In fp32 only blocks of 32 queries take a sequence's keys in parts.  Grids of 193 to 255 blocks of
+    128 have the other kernel and fewer blocks than CUs: no parts, so no scratch, however uneven the
+    keys are; smaller grids on long keys have parts."""
+    ws = pkg.load_library().tsc_diff_attention_workspace_bytes
+    between = 0
+    for d in (64, 128):
+        for b in range(1, 41):
+            for h in (1, 2, 3, 5, 8, 12, 16, 24):
+                for longest in (1, 64, 100, 128, 300, 640, 1500, 4000):
+                    blocks = -(-longest // 128) * h * b
+                    for total_kv, most in ((2000, 1500), (4000, 3000), (40000, 30000), (90 * b, 90)):
+                        if 192 < blocks < 256:
+                            between += 1
+                            args = (0, b, longest * b, total_kv, h, d, longest, most, 0)
+                            assert ws(*args) == 0, args
+    assert between > 500
+    assert ws(0, 1, 1, 40000, 12, 64, 1, 40000, 0) > 0

@@ -173,6 +173,24 @@ def test_larger_self_attention(pkg, dev, dtype, lq, h):
         _close(got[n][hs] if n == "dlam" else got[n][:, hs], want[n], n)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lkv,h", [([64] * 13, [1500] + [41] * 12, 16), ([100] * 28, [3000] + [37] * 27, 8),
+                                      ([640] + [10] * 7, None, 5)])
+def test_many_uneven_sequences_on_nearly_a_block_per_cu(pkg, dev, dtype, d, lq, lkv, h):
+    """193 to 255 blocks of 128 queries, most of the keys in one sequence: whole sequences in fp32,
+    parts of them where a type's kernel has those.  The first and the last head against the definition."""
+    q, k, v, do, lam = _make(lq, lkv or lq, h, d, dtype, 21 + h)
+    cq = _cu(lq)
+    ck = cq if lkv is None else _cu(lkv)
+    print(f"  diff attention uneven {dtype} D={d} H={h} B={len(lq)}", flush=True)
+    got = _run(pkg, dev, q, k, v, do, lam, cq, ck)
+    hs = [0, h - 1]
+    want = _oracle(*(t[:, hs] for t in (q, k, v, do)), lam[hs], cq, ck, dtype)
+    for n in got:
+        _close(got[n][hs] if n == "dlam" else got[n][:, hs], want[n], n)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("d", [64, 128])
 def test_moving_maxima(pkg, dev, dtype, d):

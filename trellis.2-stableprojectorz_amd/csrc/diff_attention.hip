@@ -1272,6 +1272,7 @@ Plan da_plan(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv, int32_
   int64_t slots = kCUs, least = 512;  // blocks that run at once, keys a part has at least
   if (dtype == TSC_F32) {
     p.rows = block_rows(kCostF32, max_q, hb);
+    if (p.rows == kBQ) return p;  // 193 blocks of 128 and more: that kernel takes whole sequences
     least = 256;
   } else if (D == 64) {
     slots = 2 * kCUs;
