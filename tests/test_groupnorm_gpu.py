@@ -317,6 +317,21 @@ def test_many_uneven_samples(pkg, dev, dtype, c, groups):
     _close(db, r["db"], r["tdb"], dtype, "dbias")
 
 
+def test_samples_times_slabs_past_2_32_threads(pkg, dev):
+    """140000 samples, all but the last empty, and 65 slabs of 64 channels (an odd count: no vectors): 9.1
+    million blocks of 512 threads.  The rows' values and gradients are those of the one sample alone."""
+    n, b, c, groups = 300, 140000, 4097, 17
+    cu = torch.zeros(b + 1, dtype=torch.int32, device=dev)
+    cu[b] = n
+    x, w, bias, dy = (t.to(dev) for t in _make([n], c, torch.bfloat16, 15))
+    leaves = [t.requires_grad_() for t in (x, w, bias)]
+    r = _oracle(x.detach().cpu(), groups, w.detach().cpu(), bias.detach().cpu(), [0, n], 1e-5, True, dy.cpu())
+    y = pkg.group_norm(x, groups, w, bias, cu, silu=True)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    for got, want, size in ((y, "y", "ty"), (dx, "dx", "tdx"), (dw, "dw", "tdw"), (db, "db", "tdb")):
+        _close(got, r[want], r[size], torch.bfloat16, want)
+
+
 def test_device_offsets_are_not_read_back(pkg, dev):
     x, w, b, _ = _make([600], 64, torch.float32, 12)
     xd = x.to(dev)

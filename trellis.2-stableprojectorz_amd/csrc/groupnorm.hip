@@ -545,19 +545,23 @@ __global__ void __launch_bounds__(kNT, 4)
   }
 }
 
-// dx; the first pblocks blocks add up dgamma and dbeta instead, 8 channels each.
+// dx; the first pblocks blocks add up dgamma and dbeta instead, 8 channels each, in the grid's first
+// prows rows, whose other blocks have nothing to do.  A row holds the slots of a slab: along one axis of a
+// launch there may be 2^32 - 1 threads only, which 2^20 samples would pass with 8 slabs.
 template <typename T, int VN>
 __global__ void __launch_bounds__(kNT, 4)
     gn_grad_kernel(GnShape s, const T* dy, const T* x, const float* __restrict__ stats,
                    const T* __restrict__ gamma, const T* __restrict__ beta, int32_t silu,
-                   int32_t rest, int32_t pblocks, const float2* __restrict__ pc,
+                   int32_t rest, int32_t pblocks, int32_t prows, const float2* __restrict__ pc,
                    const float2* __restrict__ pg, T* dx, T* dgamma, T* dbeta) {
   constexpr int KR = 2;
   __shared__ double sa[kNT], sb[kNT];
   __shared__ float2 sg[kSlab];
   const int tid = threadIdx.x;
-  if ((int)blockIdx.x < pblocks) {
-    const int e = tid % kParamCh, j = tid / kParamCh, c = blockIdx.x * kParamCh + e;
+  if ((int)blockIdx.y < prows) {
+    const int pb = blockIdx.y * gridDim.x + blockIdx.x;
+    if (pb >= pblocks) return;  // uniform over the block
+    const int e = tid % kParamCh, j = tid / kParamCh, c = pb * kParamCh + e;
     double u = 0., v = 0.;
     if (c < s.C)
       for (int i = j; i < s.T + s.B; i += kNT / kParamCh) {
@@ -581,8 +585,7 @@ __global__ void __launch_bounds__(kNT, 4)
     }
     return;
   }
-  const int at = blockIdx.x - pblocks;
-  const Where w = where<VN>(s, at % (s.T + s.B), at / (s.T + s.B));
+  const Where w = where<VN>(s, blockIdx.x, blockIdx.y - prows);
   const int SC = s.TX * VN;
   const int gl = w.slab * SC / s.cpg, gh = (min((w.slab + 1) * SC, s.C) - 1) / s.cpg;
   const int ng = gh - gl + 1, cols = sum_columns(ng), P = kNT / cols;
@@ -776,6 +779,7 @@ int groupnorm_backward_launch(tsc_ctx* ctx, int32_t dtype, const void* dy, const
   const int vn = std::min(4, vec_elems(es, C, {x, dy, dx}));
   const GnShape s = gn_shape(cu, B, N, C, groups, vn);
   const int pblocks = dgamma || dbeta ? (C + kParamCh - 1) / kParamCh : 0;
+  const int slots = s.T + s.B, prows = (pblocks + slots - 1) / slots;
   float2* pc = (float2*)ws;
   float2* pg = pc + ((int64_t)s.T + B) * C;
   by_type<4>(dtype, vn, [&](auto t, auto v) {
@@ -783,14 +787,14 @@ int groupnorm_backward_launch(tsc_ctx* ctx, int32_t dtype, const void* dy, const
     constexpr int VN = decltype(v)::value;
     {
       ProfScope p(ctx, "groupnorm_grad_sums");
-      gn_grad_sums_kernel<T, VN><<<dim3((unsigned)(s.T + s.B), (unsigned)s.slabs), kNT, 0, ctx->stream>>>(
+      gn_grad_sums_kernel<T, VN><<<dim3((unsigned)slots, (unsigned)s.slabs), kNT, 0, ctx->stream>>>(
           s, (const T*)dy, (const T*)x, stats, (const T*)gamma, (const T*)beta, silu, pc, pg);
     }
     ProfScope p(ctx, "groupnorm_grad");
     gn_grad_kernel<T, VN>
-        <<<(unsigned)((s.T + s.B) * s.slabs + pblocks), kNT, 0, ctx->stream>>>(
+        <<<dim3((unsigned)slots, (unsigned)(s.slabs + prows)), kNT, 0, ctx->stream>>>(
             s, (const T*)dy, (const T*)x, stats, (const T*)gamma, (const T*)beta, silu, rest,
-            pblocks, pc, pg, (T*)dx, (T*)dgamma, (T*)dbeta);
+            pblocks, prows, pc, pg, (T*)dx, (T*)dgamma, (T*)dbeta);
   });
   return check_hip(hipGetLastError(), "groupnorm backward launch");
 }
