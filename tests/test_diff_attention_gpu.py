@@ -390,6 +390,21 @@ def test_block_without_gradients(pkg, dev):
     assert not block(pkg.SparseTensor(torch.randn(40, 128, device=dev).bfloat16(), coords)).feats.requires_grad
 
 
+def test_a_saved_input_that_is_written_is_refused(pkg, dev):
+    """q, k and v are saved for the gradient: written to through a later call's `out`, it is refused."""
+    q, k, v, do, lam = (t.to(dev) for t in _make([30], [30], 2, 64, torch.float32, 2))
+    for i in range(3):
+        saved = [t.clone() for t in (q, k, v)]
+        o = pkg.sparse_diff_attention(*saved, lam.clone().requires_grad_(), [0, 30])
+        with torch.no_grad():
+            pkg.sparse_diff_attention(q, k, v, lam, [0, 30], out=saved[i])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            o.sum().backward()
+    leaf = torch.zeros_like(q).requires_grad_()
+    with pytest.raises(pkg.TscError, match="gradients"):
+        pkg.sparse_diff_attention(q, k, v, lam, [0, 30], out=leaf)
+
+
 def test_empty_inputs(pkg, dev):
     z = lambda n: torch.zeros((n, 2, 64), device=dev).requires_grad_()
     lam = torch.ones(2, device=dev).requires_grad_()

@@ -402,3 +402,50 @@ def test_refusals_on_the_device(pkg, dev):
     base = torch.zeros(12 * 11, device=dev)
     with pytest.raises(pkg.TscError, match="overlaps"):
         pkg.group_norm(base[:120].view(10, 12), 3, out=base[12:].view(10, 12))
+
+
+def test_a_saved_input_that_is_written_is_refused(pkg, dev):
+    """x is saved for the gradient: once any of the library's operators has written to it through `out`,
+    the gradient is refused, as after torch's own in-place operations."""
+    n, c = 24, 64
+    other = torch.randn((n, c), device=dev)
+    w = torch.ones(c, device=dev, requires_grad=True)
+    lam = torch.ones(1, device=dev)
+    nbr = torch.full((n, 27), -1, dtype=torch.int32, device=dev)
+    wc = torch.zeros((c, 3, 3, 3, c), device=dev)
+
+    def norm(out):
+        pkg.group_norm(other, 8, out=out)
+
+    def attend(out):
+        o = other.view(n, 1, c)
+        pkg.sparse_diff_attention(o, o, o, lam, [0, n], out=out.view(n, 1, c))
+
+    def attend_one_map(out):
+        o = other.view(n, 1, c)
+        pkg.sparse_attention(o, o, o, [0, n], out=out)
+
+    writers = [norm, attend, attend_one_map, lambda out: pkg.layer_norm(other, out=out),
+               lambda out: pkg.silu(other, out=out), lambda out: pkg.add(other, other, out=out),
+               lambda out: pkg.sparse_linear(other, torch.eye(c, device=dev), out=out),
+               lambda out: pkg.sparse_conv3d(other, wc, None, nbr, out=out),
+               lambda out: pkg.sparse_resblock(other, nbr, wc, None, wc, None, out=out)]
+    for i, write in enumerate(writers):
+        x = torch.randn((n, c), device=dev)
+        y = pkg.group_norm(x, 8, w)
+        with torch.no_grad():
+            write(x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    x = torch.randn((n, c), device=dev)
+    y = pkg.group_norm(x, 8, w)
+    with pytest.raises(pkg.TscError):  # refused, so not written
+        pkg.group_norm(other, 8, eps=-1.0, out=x)
+    y.sum().backward()
+    leaf = torch.zeros((n, c), device=dev, requires_grad=True)
+    with pytest.raises(pkg.TscError, match="gradients"):
+        pkg.group_norm(other, 8, out=leaf)
+    with torch.no_grad():
+        pkg.group_norm(other, 8, out=leaf)
+    with torch.inference_mode():
+        pkg.group_norm(other, 8, out=torch.zeros((n, c), device=dev))

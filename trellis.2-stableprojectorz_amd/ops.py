@@ -9,6 +9,7 @@ import ctypes
 from dataclasses import dataclass
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import TscError, check
@@ -41,6 +42,13 @@ def _dev(*ts) -> int:
 
 def _p(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def _wrote(out: torch.Tensor | None) -> None:
+    """Tells autograd that a given `out` gets new values, which it cannot see behind the pointer: a
+    gradient that saved the old ones is refused then, as after any in-place operation."""
+    if out is not None:
+        increment_version(out)
 
 
 @dataclass
@@ -225,6 +233,7 @@ def sparse_conv3d(feats: torch.Tensor, weight: torch.Tensor, bias, nmap, order=N
     if epi == _lib.TSC_EPI_BIAS_RESIDUAL and (residual is None or tuple(residual.shape) != (n, co)):
         raise TscError(_lib.TSC_ERR_INVALID, "residual epilogue needs an (N,Co) residual")
     dev = _dev(feats, weight, bias, nbr, order, residual, ln_weight, ln_bias, out)
+    given = out
     if out is None:
         out = torch.empty((n, co), dtype=feats.dtype, device=feats.device)
     ctx = _lib.context(dev)
@@ -232,10 +241,12 @@ def sparse_conv3d(feats: torch.Tensor, weight: torch.Tensor, bias, nmap, order=N
         check(ctx.lib.tsc_conv_planned(ctx.bind(), _code(feats), _p(feats), _p(weight), _p(bias),
                                        _p(nbr), _p(plan), n, ci, co, epi, _p(residual), _p(ln_weight),
                                        _p(ln_bias), float(eps), _p(out)))
+        _wrote(given)
         return out
     check(ctx.lib.tsc_conv_fused(ctx.bind(), _code(feats), _p(feats), _p(weight), _p(bias), _p(nbr),
                                  _p(order), n, ci, co, epi, _p(residual), _p(ln_weight), _p(ln_bias),
                                  float(eps), _p(out)))
+    _wrote(given)
     return out
 
 
@@ -245,11 +256,13 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-6, silu:
     c = x.shape[-1]
     rows = x.numel() // c if c else 0
     dev = _dev(x, weight, bias, out)
+    given = out
     if out is None:
         out = torch.empty_like(x)
     ctx = _lib.context(dev)
     check(ctx.lib.tsc_layernorm(ctx.bind(), _code(x), _p(x), rows, c,
                                 _p(weight), _p(bias), float(eps), int(silu), _p(out)))
+    _wrote(given)
     return out
 
 
@@ -295,7 +308,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, cu_rows
         _, cu = _cu_seqlens(cu_rows, x.shape[0], dev, "cu_rows")
         _dev(x, cu)
         b = cu.numel() - 1
-    if _wants_grad(x, weight, bias):
+    if _wants_grad(x, weight, bias, out):
         if out is not None:
             raise TscError(_lib.TSC_ERR_INVALID, "group_norm: out cannot be given where gradients are wanted")
         from .autograd import GroupNorm
@@ -317,6 +330,8 @@ def _group_norm(x, weight, bias, cu, b, groups, eps, silu, out, stats):
     ws = _scratch(nbytes, x.device)
     check(lib.tsc_groupnorm(handle, _code(x), _p(x), _p(cu), b, n, c, groups, _p(weight),
                             _p(bias), eps, int(silu), int(rest), _p(stats), _p(ws), _p(out)))
+    if not rest:
+        _wrote(out)
     return out
 
 
@@ -339,10 +354,12 @@ def _group_norm_backward(dy, x, weight, bias, cu, b, groups, silu, stats, want_p
 
 def silu(x: torch.Tensor, out=None) -> torch.Tensor:
     dev = _dev(x, out)
+    given = out
     if out is None:
         out = torch.empty_like(x)
     ctx = _lib.context(dev)
     check(ctx.lib.tsc_silu(ctx.bind(), _code(x), _p(x), x.numel(), _p(out)))
+    _wrote(given)
     return out
 
 
@@ -350,10 +367,12 @@ def add(a: torch.Tensor, b: torch.Tensor, out=None) -> torch.Tensor:
     if a.shape != b.shape or a.dtype != b.dtype:
         raise TscError(_lib.TSC_ERR_INVALID, "add: shapes and dtypes must match")
     dev = _dev(a, b, out)
+    given = out
     if out is None:
         out = torch.empty_like(a)
     ctx = _lib.context(dev)
     check(ctx.lib.tsc_add(ctx.bind(), _code(a), _p(a), _p(b), a.numel(), _p(out)))
+    _wrote(given)
     return out
 
 
@@ -366,11 +385,13 @@ def sparse_resblock(x: torch.Tensor, nmap, w1, b1, w2, b2, ln_weight=None, ln_bi
         if tuple(w.shape) != (c, 3, 3, 3, c) or w.dtype != x.dtype:
             raise TscError(_lib.TSC_ERR_INVALID, "resblock weights must be (C,3,3,3,C) of x's dtype")
     dev = _dev(x, nbr, order, w1, b1, w2, b2, ln_weight, ln_bias, out)
+    given = out
     if out is None:
         out = torch.empty_like(x)
     ctx = _lib.context(dev)
     check(ctx.lib.tsc_resblock(ctx.bind(), _code(x), _p(x), _p(nbr), _p(order), n, c, _p(w1), _p(b1),
                                _p(ln_weight), _p(ln_bias), float(eps), _p(w2), _p(b2), _p(out)))
+    _wrote(given)
     return out
 
 
@@ -442,11 +463,13 @@ def sparse_linear(x: torch.Tensor, weight: torch.Tensor, bias=None, residual=Non
     for t in (weight, bias, residual):
         if t is not None and t.dtype != x.dtype:
             raise TscError(_lib.TSC_ERR_INVALID, "linear: dtype mismatch")
+    given = out
     if out is None:
         out = torch.empty((n, cout), dtype=x.dtype, device=x.device)
     ctx = _lib.context(_dev(x, weight, bias, residual, out))
     check(ctx.lib.tsc_linear(ctx.bind(), _code(x), _p(x), n, cin, _p(weight), _p(bias),
                              _p(residual), cout, _p(out)))
+    _wrote(given)
     return out
 
 
@@ -509,6 +532,7 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if ck.numel() != cq.numel():
         raise TscError(_lib.TSC_ERR_INVALID, "cu_seqlens_q and cu_seqlens_kv differ in length")
     b = cq.numel() - 1
+    given = out
     if out is None:
         # the kernel writes every row inside a query sequence; zero-fill unless they cover all
         covered = cq_host is not None and b > 0 and cq_host[0] == 0 and cq_host[-1] == tq
@@ -524,6 +548,7 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     check(ctx.lib.tsc_attention(ctx.bind(), _code(q), _p(q), _p(k), _p(v), _p(cq), _p(ck), b, tq,
                                 tkv, h, d, float(scale) if scale else 0.0, int(max_seqlen_q),
                                 _p(out)))
+    _wrote(given)
     return out.view(tq, h, d)
 
 
@@ -596,7 +621,7 @@ def sparse_diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam
 
     args = (cq, ck, b, float(scale) if scale is not None else 0.0,
             longest(max_seqlen_q, cq_host, tq), longest(max_seqlen_kv, ck_host, tkv))
-    if _wants_grad(q, k, v, lam):
+    if _wants_grad(q, k, v, lam, out):
         if out is not None:
             raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: out cannot be given where gradients "
                                                  "are wanted")
@@ -624,6 +649,8 @@ def _diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, out, keep):
                                      _head_rows(k, "k"), _head_rows(v, "v"), _p(lam), _p(cq), _p(ck), b,
                                      tq, tkv, h, d, scale, max_q, max_kv, int(rest), _p(ws), _p(out),
                                      _p(maps), _p(lse)))
+        if not rest:
+            _wrote(out)
     return out, maps, lse
 
 
