@@ -55,3 +55,25 @@ def test_cu_rows_of_a_sparse_tensor(pkg):
     x = pkg.SparseTensor(torch.zeros((3, 8)), coords)
     assert x.cu_rows.tolist() == [0, 2, 2, 3] and x.cu_rows.dtype == torch.int32
     assert x.replace(torch.ones((3, 4))).cu_rows is x.cu_rows
+
+
+def test_dual_tensors_are_refused(pkg):
+    """There is no forward-mode derivative: a tangent is refused, not dropped."""
+    import torch.autograd.forward_ad as fa
+
+    with fa.dual_level():
+        def dual(*shape):
+            return fa.make_dual(torch.zeros(shape), torch.ones(shape))
+
+        for args in ((dual(10, 12), 3), (torch.zeros(10, 12), 3, dual(12)),
+                     (torch.zeros(10, 12), 3, None, dual(12))):
+            with pytest.raises(pkg.TscError, match="forward-mode"):
+                pkg.group_norm(*args)
+            with torch.no_grad(), pytest.raises(pkg.TscError, match="forward-mode"):
+                pkg.group_norm(*args)
+        q = torch.zeros((10, 2, 64))
+        args = [q, q, q, torch.zeros(2)]
+        for i in range(4):
+            some = [dual(*t.shape) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises(pkg.TscError, match="forward-mode"):
+                pkg.sparse_diff_attention(*some, [0, 10])

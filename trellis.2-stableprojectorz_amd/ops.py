@@ -9,6 +9,7 @@ import ctypes
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _lib
@@ -276,6 +277,12 @@ def _wants_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+def _no_tangents(what: str, *ts) -> None:
+    """Refuses dual tensors: these ops have no forward-mode derivative, and would drop the tangent."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise TscError(_lib.TSC_ERR_UNSUPPORTED, f"{what}: no forward-mode derivative (dual tensor)")
+
+
 def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, cu_rows=None,
                eps: float = 1e-5, silu: bool = False, out=None) -> torch.Tensor:
     """Group norm over the rows of each sample, channels last (fp32 statistics), optionally fused
@@ -298,6 +305,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, cu_rows
     if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
         raise TscError(_lib.TSC_ERR_INVALID, "group_norm: out has the wrong shape or dtype")
     _code(x)
+    _no_tangents("group_norm", x, weight, bias, out)
     dev = _dev(x, weight, bias, out)
     cu, b = None, 1
     if x.dim() > 2:
@@ -592,6 +600,7 @@ def sparse_diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
         raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: out has the wrong shape or dtype")
     _code(q)
+    _no_tangents("diff_attention", q, k, v, lam, out)
     for name, t in (("q", q), ("k", k), ("v", v)):
         _head_rows(t, name)
     lam = lam.contiguous()
