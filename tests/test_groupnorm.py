@@ -77,3 +77,27 @@ def test_dual_tensors_are_refused(pkg):
             some = [dual(*t.shape) if j == i else t for j, t in enumerate(args)]
             with pytest.raises(pkg.TscError, match="forward-mode"):
                 pkg.sparse_diff_attention(*some, [0, 10])
+
+
+def test_cu_rows_needs_rows_grouped_by_sample(pkg):
+    """Offsets cannot say which rows are a sample's where samples are mixed or out of order."""
+    def tensor(samples, **kw):
+        coords = torch.tensor([[b, i, 0, 0] for i, b in enumerate(samples)], dtype=torch.int32).reshape(-1, 4)
+        return pkg.SparseTensor(torch.zeros((len(samples), 8)), coords, **kw)
+
+    for mixed in ([1, 0, 1, 0], [0, 1, 0, 1], [1, 1, 0, 0], [0, 2, 1, 2], [2, 1, 0]):
+        with pytest.raises(ValueError, match="grouped by sample"):
+            tensor(mixed).cu_rows
+    with pytest.raises(ValueError, match="grouped by sample"):  # a layout of other rows
+        tensor([0, 0, 1], layout=[(0, 1), (1, 3)]).cu_rows
+    with pytest.raises(ValueError, match="grouped by sample"):
+        tensor([0, 0, 1], layout=[(1, 3), (0, 1)]).cu_rows
+    assert tensor([0, 0, 3]).cu_rows.tolist() == [0, 2, 2, 2, 3]
+    assert tensor([]).cu_rows.tolist() == [0, 0]
+    x = tensor([0, 0, 1])
+    assert x.cu_rows.tolist() == [0, 2, 3]
+    other = tensor([0, 1, 1]).coords  # replace keeps the layout; other coordinates are looked at again
+    with pytest.raises(ValueError, match="grouped by sample"):
+        x.replace(torch.zeros((3, 8)), other).cu_rows
+    same = x.replace(torch.zeros((3, 8)), x.coords.clone())
+    assert same.cu_rows.tolist() == [0, 2, 3]

@@ -38,7 +38,8 @@ class SparseLinear:
 
 
 class SparseGroupNorm:
-    """Group norm of each sample's voxels, optionally with SiLU (ops.group_norm over x.cu_rows)."""
+    """Group norm of each sample's voxels, optionally with SiLU (ops.group_norm over x.cu_rows, so
+    x's rows have to be grouped by sample)."""
 
     def __init__(self, num_groups: int, weight: torch.Tensor | None = None,
                  bias: torch.Tensor | None = None, eps: float = 1e-5, silu: bool = False):
@@ -55,10 +56,10 @@ class SparseGroupNorm:
 
 
 class SparseDiffAttentionBlock3d:
-    """x + out(diff_attention(qkv(group_norm(x)))) over each sample's voxels: group norm, one linear
-    layer for q, k and v (read in place as row slices), differential attention, and the output layer
-    with the skip as its residual.  qkv weight (3 C, C), out weight (C, C), lam float32 (num_heads),
-    C = num_heads * 64 or 128.  Without gradients: its linear layers have none (group_norm and
+    """x + out(diff_attention(qkv(group_norm(x)))) over each sample's voxels, x's rows grouped by
+    sample: group norm, one linear layer for q, k and v (read in place as row slices), differential
+    attention, and the output layer with the skip as its residual.  qkv weight (3 C, C), out weight
+    (C, C), lam float32 (num_heads), C = num_heads * 64 or 128.  Without gradients: its linear layers have none (group_norm and
     sparse_diff_attention do, around another library's linear layers)."""
 
     def __init__(self, num_heads: int, num_groups: int, norm_weight: torch.Tensor | None,

@@ -96,9 +96,20 @@ class SparseTensor:
     @property
     def cu_rows(self) -> torch.Tensor:
         """Row offsets of the samples, int32 (batch + 1) beside feats: `layout` as group_norm and
-        sparse_attention take it, copied to the device on first use."""
+        sparse_attention take it, copied to the device on first use.  Rows have to be grouped by sample,
+        in the samples' order (the convs need neither): checked then, a ValueError if they are not.  The
+        first use waits for the device, so it comes before a graph is captured."""
         if self._cu_rows is None or self._cu_rows.device != self.feats.device:
-            offsets = [0] + [stop for _, stop in self.layout]
+            layout, n = self.layout, self.coords.shape[0]
+            offsets = [0] + [stop for _, stop in layout]
+            grouped = offsets[-1] == n and [start for start, _ in layout] == offsets[:-1]
+            if grouped and n:
+                dev = self.coords.device
+                counts = torch.tensor([stop - start for start, stop in layout], device=dev)
+                sample = torch.repeat_interleave(torch.arange(len(layout), device=dev), counts, output_size=n)
+                grouped = bool((self.coords[:, 0] == sample).all().item())
+            if not grouped:
+                raise ValueError("cu_rows: the rows are not grouped by sample (sort them by coords[:, 0])")
             self._cu_rows = torch.tensor(offsets, dtype=torch.int32, device=self.feats.device)
         return self._cu_rows
 
@@ -147,9 +158,10 @@ class SparseTensor:
     def replace(self, feats: torch.Tensor, coords: torch.Tensor | None = None) -> "SparseTensor":
         """New feats (and optionally coords) with this tensor's shape, scale, spatial cache and
         layout, as the reference's replace (sparse_tensor.ts:112-121)."""
+        known = self._cu_rows if coords is None else None
         return SparseTensor(feats, self.coords if coords is None else coords, self._shape,
                             self._scale, self._spatial_cache, self._layout,
-                            batch_size=self._batch_size, cu_rows=self._cu_rows)
+                            batch_size=self._batch_size, cu_rows=known)
 
     def to(self, device) -> "SparseTensor":
         return SparseTensor(self.feats.to(device), self.coords.to(device), self._shape,
