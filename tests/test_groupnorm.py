@@ -101,3 +101,13 @@ def test_cu_rows_needs_rows_grouped_by_sample(pkg):
         x.replace(torch.zeros((3, 8)), other).cu_rows
     same = x.replace(torch.zeros((3, 8)), x.coords.clone())
     assert same.cu_rows.tolist() == [0, 2, 3]
+
+
+def test_cu_rows_has_every_sample_of_a_given_batch_size(pkg):
+    """Empty samples after the last row's count too: the offsets pair with a condition's of the batch."""
+    coords = torch.tensor([[0, 0, 0, 0], [0, 1, 0, 0], [1, 0, 0, 0]], dtype=torch.int32)
+    x = pkg.SparseTensor(torch.zeros((3, 8)), coords, batch_size=4)
+    assert x.cu_rows.tolist() == [0, 2, 3, 3, 3] and x.batch_size == 4
+    assert x.replace(torch.zeros((3, 2))).cu_rows is x.cu_rows
+    none = pkg.SparseTensor(torch.zeros((0, 8)), coords[:0], batch_size=2)
+    assert none.cu_rows.tolist() == [0, 0, 0]

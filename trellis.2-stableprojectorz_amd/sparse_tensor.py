@@ -96,7 +96,8 @@ class SparseTensor:
     @property
     def cu_rows(self) -> torch.Tensor:
         """Row offsets of the samples, int32 (batch + 1) beside feats: `layout` as group_norm and
-        sparse_attention take it, copied to the device on first use.  Rows have to be grouped by sample,
+        sparse_attention take it, with the empty samples that a given batch_size has after the last
+        row's, copied to the device on first use.  Rows have to be grouped by sample,
         in the samples' order (the convs need neither): checked then, a ValueError if they are not.  The
         first use waits for the device, so it comes before a graph is captured."""
         if self._cu_rows is None or self._cu_rows.device != self.feats.device:
@@ -110,6 +111,7 @@ class SparseTensor:
                 grouped = bool((self.coords[:, 0] == sample).all().item())
             if not grouped:
                 raise ValueError("cu_rows: the rows are not grouped by sample (sort them by coords[:, 0])")
+            offsets += [n] * ((self._batch_size or 0) - len(layout))
             self._cu_rows = torch.tensor(offsets, dtype=torch.int32, device=self.feats.device)
         return self._cu_rows
 
