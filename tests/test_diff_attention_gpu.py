@@ -330,6 +330,29 @@ def test_infinite_values(pkg, dev, dtype, d):
     assert not out[34:98].isfinite().any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,h", [([32], 2), ([33, 1, 70], 3), ([700, 900], 16)])
+def test_keys_that_no_query_sees(pkg, dev, dtype, d, lens, h):
+    """A key of -inf in a dimension where every query is positive has scores of -inf, so P = 0 in that
+    map, wherever the queries end in a tile.  One of -30000 there has scores at least 500 below the rest,
+    whose exponential is 0 in fp32 too: the same bits, and finite ones, but for dq in that dimension,
+    where 0 times infinity is NaN."""
+    q, k, v, do, lam = _make(lens, lens, h, d, dtype, 17)
+    cq, half = _cu(lens), d // 2
+    q[..., 0], q[..., half] = q[..., 0].abs() + 0.2, q[..., half].abs() + 0.2
+    rows = [lo + 20 for lo, n in zip(cq, lens) if n > 25]
+    k[rows, :, 0], k[[r + 5 for r in rows], :, half] = -30000.0, -30000.0
+    want = _run(pkg, dev, q, k, v, do, lam, cq, None)
+    k[k == -30000] = -math.inf
+    got = _run(pkg, dev, q, k, v, do, lam, cq, None)
+    got["dq"][..., 0], got["dq"][..., half] = want["dq"][..., 0], want["dq"][..., half]
+    for n in got:
+        print(f"  diff attention unseen keys {dtype} D={d} {lens}: {n} has {int(got[n].isnan().sum())} NaN", flush=True)
+        assert want[n].isfinite().all() and torch.equal(got[n], want[n]), n
+    assert not got["dk"][rows][..., :half].any()
+
+
 def test_hints_and_offsets(pkg, dev):
     """Too small lengths still cover every row; device offsets give the host offsets' bits and are not
     read back."""

@@ -142,8 +142,8 @@ struct Stage {
   u32x4_t r[NL];
   int last;  // the last row of the tile that there is
   // Rows first .. first + ROWS - 1 of base (row stride ld elements); nothing if first >= end.
-  // No lane branches: rows from `end` on repeat the last one, and are cleared on their way into LDS (at
-  // the load the compiler would wait for it to do so).
+  // No lane branches: rows from `end` on repeat the last one, and with CLEAR are cleared on their way into
+  // LDS (at the load the compiler would wait for it to do so).
   __device__ __forceinline__ void load(const T* base, int64_t ld, int first, int end, int tid) {
     if (first >= end) return;
     const uint32_t rb = (uint32_t)ld * sizeof(T);
@@ -155,11 +155,12 @@ struct Stage {
       r[i] = *(const u32x4_t*)(p + ((uint32_t)min(id / Ti::CPR, last) * rb + 16u * (id % Ti::CPR)));
     }
   }
+  template <bool CLEAR = true>
   __device__ __forceinline__ void store(unsigned char* t, int tid) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int id = tid + NT * i;
-      if (id / Ti::CPR > last) r[i] = u32x4_t{0, 0, 0, 0};
+      if (CLEAR && id / Ti::CPR > last) r[i] = u32x4_t{0, 0, 0, 0};
       Ti::put(t, id / Ti::CPR, id % Ti::CPR, r[i]);
     }
   }
@@ -1128,7 +1129,7 @@ __global__ void __launch_bounds__(SHARE ? kNT : 512 / NM, sizeof(T) == 2 && !SHA
     auto load = [&](int qb) {
       qs.load(qbase, a.ldq, qb, q_len, tid);
       ds.load(dbase, ldd, qb, q_len, tid);
-      const int r = qb + (tid & 31);  // past the last query: P = 2^(0 - inf) = 0
+      const int r = qb + (tid & 31);
       if (SHARE || tid < 64) sv[0] = r < q_len ? a.lse[sbase + r] : INFINITY;
       if (SHARE || (tid >= 64 && tid < 128)) sv[1] = r < q_len ? a.r12[sbase + r] : 0.f;
     };
@@ -1139,8 +1140,10 @@ __global__ void __launch_bounds__(SHARE ? kNT : 512 / NM, sizeof(T) == 2 && !SHA
       float(*st4)[BQ] = stats[SHARE ? w : buf];
       if (!AHEAD) load(qb);
       if (SHARE) tile_sync<SHARE>();
-      qs.store(qt, tid);
-      ds.store(dt, tid);
+      // Past the last query P = 2^(score - inf) = 0 and the row there is the last query's once more: a row of
+      // zeros would make NaN of an infinite key, whose scores of -inf are 0 to every query.
+      qs.template store<false>(qt, tid);
+      ds.template store<false>(dt, tid);
       if (SHARE || tid < 64) st4[(tid >> 5) & 1][tid & 31] = sv[0];
       if (SHARE || (tid >= 64 && tid < 128)) st4[2 + ((tid >> 5) & 1)][tid & 31] = sv[1];
       tile_sync<SHARE>();
