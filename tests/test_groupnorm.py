@@ -111,3 +111,8 @@ def test_cu_rows_has_every_sample_of_a_given_batch_size(pkg):
     assert x.replace(torch.zeros((3, 2))).cu_rows is x.cu_rows
     none = pkg.SparseTensor(torch.zeros((0, 8)), coords[:0], batch_size=2)
     assert none.cu_rows.tolist() == [0, 0, 0]
+
+
+def test_workspace_of_no_samples(pkg):
+    f = pkg.load_library().tsc_groupnorm_workspace_bytes
+    assert f(0, 0, 10, 64, 32, 0) == 0 and f(2, 0, 0, 64, 32, 1) == 0

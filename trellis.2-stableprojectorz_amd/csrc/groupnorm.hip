@@ -735,6 +735,7 @@ void by_type(int32_t dtype, int vn, F f) {
 
 int64_t groupnorm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C, int32_t groups,
                                   int32_t backward) {
+  if (B == 0) return 0;
   // the buffers' alignment decides the vector length only at the call: the largest of the lengths
   const int es = dtype == TSC_F32 ? 4 : 2;
   int64_t most = 0;
