@@ -230,7 +230,8 @@ int tsc_add(tsc_ctx* ctx, int32_t dtype, const void* a, const void* b, int64_t n
  *              Values outside [0, N] are clamped; an array that decreases gives undefined values but
  *              no access out of bounds.  NULL: B samples of N / B rows each.
  *   gamma/beta (C) `dtype`, NULL = 1 / 0.  groups divides C.
- *   zero_rest  rows of y outside every sample: 0 = left as they were, 1 = set to zero
+ *   zero_rest  rows of y outside every sample (all of them if B is 0): 0 = left as they were, 1 = set
+ *              to zero
  *   stats      NULL, or device fp32 (B, groups, 2), 8-byte aligned: mean and 1 / sqrt(var + eps) for
  *              the backward pass (not written for samples without rows)
  *   workspace  device scratch of tsc_groupnorm_workspace_bytes(..., backward = 0) bytes, 16-byte
@@ -249,7 +250,7 @@ int tsc_groupnorm(tsc_ctx* ctx, int32_t dtype, const void* x, const int32_t* cu_
 /* Its gradient: dx (N,C), and dgamma, dbeta (C) summed over all samples in `dtype` (NULL = not
  * wanted), from dy, the same x, cu_rows, gamma, beta and apply_silu and the stats that
  * tsc_groupnorm wrote; workspace with backward = 1.  dx must not overlap dy or x.  zero_rest is
- * about rows of dx. */
+ * about rows of dx.  Without samples or rows dgamma and dbeta are zeros. */
 int tsc_groupnorm_backward(tsc_ctx* ctx, int32_t dtype, const void* dy, const void* x,
                            const int32_t* cu_rows, int32_t B, int64_t N, int32_t C, int32_t groups,
                            const void* gamma, const void* beta, int32_t apply_silu,
@@ -334,7 +335,8 @@ int tsc_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, con
  *   cu_seqlens_q / cu_seqlens_kv, scale, max_seqlen_q  as in tsc_attention, scale <= 0 meaning
  *     1/sqrt(head_dim / 2); max_seqlen_kv likewise (both size the workspace too: the same values
  *     there).  A sequence without keys gives zeros.
- *   zero_rest  rows of out outside every sequence: 0 = left as they were, 1 = zeroed
+ *   zero_rest  rows of out outside every sequence (all of them if B is 0): 0 = left as they were,
+ *     1 = zeroed
  *   maps, lse  both NULL, or for the backward pass: maps fp32 (total_q, num_heads, 2, head_dim) takes
  *     P1 v and P2 v, lse fp32 (2, num_heads, total_q) the maps' log2-sum-exps (rows of the sequences)
  *   workspace  device scratch of tsc_diff_attention_workspace_bytes(..., backward = 0) bytes (few
@@ -355,7 +357,8 @@ int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k
 /* Its gradient from dout (total_q, num_heads, head_dim) and what the forward call was given and
  * wrote: dq (total_q, ...), dk and dv (total_kv, num_heads, head_dim) `dtype`, dlambda fp32
  * (num_heads) or NULL.  zero_rest is about rows of dq, dk and dv.  workspace with backward = 1.  The
- * gradients must not overlap an input.  The sums have one fixed order. */
+ * gradients must not overlap an input.  The sums have one fixed order.  Without sequences or queries
+ * dlambda is zero, and so are dk and dv of the sequences' rows. */
 int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k,
                                 const void* v, int64_t ld_q, int64_t ld_k, int64_t ld_v,
                                 const float* lambda, const int32_t* cu_seqlens_q,

@@ -78,3 +78,10 @@ def test_fp32_grids_of_128_rows_are_not_split(pkg):
                             assert ws(*args) == 0, args
     assert between > 500
     assert ws(0, 1, 1, 40000, 12, 64, 1, 40000, 0) > 0
+
+
+def test_scratch_of_a_gradient_without_queries(pkg):
+    """dk, dv and dlambda are written all the same, from a partial sum of each block of keys."""
+    ws = pkg.load_library().tsc_diff_attention_workspace_bytes
+    assert ws(2, 2, 0, 500, 3, 64, 0, 300, 1) > 0 and ws(2, 2, 0, 500, 3, 64, 0, 300, 0) == 0
+    assert ws(2, 0, 10, 10, 3, 64, 10, 10, 1) == 0

@@ -438,6 +438,42 @@ def test_empty_inputs(pkg, dev):
         assert o.shape == q.shape and not o.any() and not any(t.any() for t in g)
 
 
+def test_c_calls_without_sequences_or_queries(pkg, dev):
+    """B = 0: every row is outside, zeroed with zero_rest or left as it was; no queries: dk and dv of the
+    sequences' rows are zeros whatever zero_rest is.  dlambda is zero either way."""
+    import ctypes
+    import sys
+
+    P = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
+    lib, hd = sys.modules["trellis2_amd._lib"].stream_handle(0)
+    n, h, d = 50, 3, 64
+    lam = torch.ones(h, device=dev)
+    for code, dtype in ((0, torch.float32), (1, torch.float16), (2, torch.bfloat16)):
+        x = torch.ones((n, h, d), dtype=dtype, device=dev)
+        for rest in (0, 1):
+            o, dq, dk, dv = (torch.full_like(x, 5.0) for _ in range(4))
+            dl = torch.full_like(lam, 5.0)
+            args = (hd, code, P(x), P(x), P(x), h * d, h * d, h * d, P(lam), None, None, 0, n, n, h, d, 0.0, n, n, rest)
+            assert lib.tsc_diff_attention(*args, None, P(o), None, None) == 0
+            maps, lse = torch.zeros((n, h, 2, d), device=dev), torch.zeros((2, h, n), device=dev)
+            assert lib.tsc_diff_attention_backward(*args, P(maps), P(lse), P(x), None, P(dq), P(dk), P(dv), P(dl)) == 0
+            for t in (o, dq, dk, dv):
+                assert bool((t == 5 * (1 - rest)).all())
+            assert not dl.any()
+            cq = torch.zeros(3, dtype=torch.int32, device=dev)
+            ck = torch.tensor([4, 20, 41], dtype=torch.int32, device=dev)
+            nbytes = lib.tsc_diff_attention_workspace_bytes(code, 2, 0, n, h, d, 0, n, 1)
+            ws = torch.full((nbytes // 4,), 7.0, device=dev)
+            dk, dv, dl = torch.full_like(x, 5.0), torch.full_like(x, 5.0), torch.full_like(lam, 5.0)
+            assert lib.tsc_diff_attention_backward(
+                hd, code, None, P(x), P(x), h * d, h * d, h * d, P(lam), P(cq), P(ck), 2, 0, n, h, d, 0.0, 0, n, rest,
+                None, None, None, P(ws), None, P(dk), P(dv), P(dl)) == 0
+            for t in (dk, dv):
+                assert not t[4:41].any() and bool((t[:4] == 5 * (1 - rest)).all())
+                assert bool((t[41:] == 5 * (1 - rest)).all())
+            assert not dl.any()
+
+
 def test_same_bits_each_time_on_any_stream_and_in_a_graph(pkg, dev):
     """Sums have one order; captured training steps replay to the eager bits with new inputs, with
     eager work in between; two captured graphs share nothing."""

@@ -449,3 +449,40 @@ def test_a_saved_input_that_is_written_is_refused(pkg, dev):
         pkg.group_norm(other, 8, out=leaf)
     with torch.inference_mode():
         pkg.group_norm(other, 8, out=torch.zeros((n, c), device=dev))
+
+
+def test_c_calls_without_samples_or_rows(pkg, dev):
+    """B = 0: every row is outside, zeroed with zero_rest or left as it was, and the parameters' gradients
+    are sums over nothing; the same for N = 0.  Captured and replayed as well."""
+    import ctypes
+    import sys
+
+    P = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
+    mod = sys.modules["trellis2_amd._lib"]
+    lib, h = mod.stream_handle(0)
+    n, c = 1000, 37
+    for code, dtype in ((0, torch.float32), (1, torch.float16), (2, torch.bfloat16)):
+        x = torch.ones((n, c), dtype=dtype, device=dev)
+        for rest in (0, 1):
+            y, dx, dw, db = (torch.full_like(t, 5.0) for t in (x, x, x[0], x[0]))
+            assert lib.tsc_groupnorm(h, code, P(x), None, 0, n, c, 1, None, None, 1e-5, 0, rest, None, None,
+                                     P(y)) == 0
+            assert lib.tsc_groupnorm_backward(h, code, P(x), P(x), None, 0, n, c, 1, None, None, 0, rest, None,
+                                              None, P(dx), P(dw), P(db)) == 0
+            assert bool((y == 5 * (1 - rest)).all()) and bool((dx == 5 * (1 - rest)).all())
+            assert not dw.any() and not db.any()
+        ws, st = torch.zeros(1 << 14, device=dev), torch.zeros(8, device=dev)
+        dw, db = torch.full_like(x[0], 5.0), torch.full_like(x[0], 5.0)
+        assert lib.tsc_groupnorm_backward(h, code, None, None, None, 2, 0, c, 1, None, None, 0, 1, P(st), P(ws),
+                                          None, P(dw), P(db)) == 0
+        assert not dw.any() and not db.any()
+    y = torch.empty((n, c), device=dev)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        assert lib.tsc_groupnorm(mod.stream_handle(0)[1], 0, P(y), None, 0, n, c, 1, None, None, 1e-5, 0, 1, None,
+                                 None, P(y)) == 0
+    for _ in range(3):
+        y.fill_(3.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert not y.any()

@@ -552,10 +552,10 @@ int tsc_groupnorm(tsc_ctx* ctx, int32_t dtype, const void* x, const int32_t* cu_
   if (!(eps >= 0.f)) return fail(TSC_ERR_INVALID, "groupnorm: eps must be >= 0");
   if (!cu_rows && B > 0 && N % B)
     return fail(TSC_ERR_INVALID, "groupnorm: N=%lld rows are not %d equal samples", (long long)N, B);
-  if (B == 0 || N == 0) return TSC_OK;
+  if (N == 0 || (B == 0 && !zero_rest)) return TSC_OK;
   const int es = elem_size(dtype);
   const size_t bytes = (size_t)N * C * es;
-  if (!x || !y || !workspace) return fail(TSC_ERR_INVALID, "groupnorm: null buffer");
+  if (!y || (B > 0 && (!x || !workspace))) return fail(TSC_ERR_INVALID, "groupnorm: null buffer");
   if (!aligned(x, es) || !aligned(y, es) || (gamma && !aligned(gamma, es)) ||
       (beta && !aligned(beta, es)) || !aligned(workspace, 16) || (stats && !aligned(stats, 8)) ||
       (cu_rows && !aligned(cu_rows, 4)))
@@ -564,6 +564,7 @@ int tsc_groupnorm(tsc_ctx* ctx, int32_t dtype, const void* x, const int32_t* cu_
   if (x != y && overlaps(x, bytes, y, bytes))
     return fail(TSC_ERR_INVALID, "groupnorm: y overlaps x without being x");
   DeviceGuard g(ctx->device);
+  if (B == 0) return zero_launch(ctx, y, (int64_t)bytes);  // every row is outside
   return groupnorm_launch(ctx, dtype, x, cu_rows, B, N, C, groups, gamma, beta, eps, apply_silu,
                           zero_rest, stats, workspace, y);
 }
@@ -577,12 +578,12 @@ int tsc_groupnorm_backward(tsc_ctx* ctx, int32_t dtype, const void* dy, const vo
   int st = check_ctx(ctx);
   if (!st) st = validate_groupnorm("groupnorm_backward", dtype, B, N, C, groups);
   if (st) return st;
-  if (B == 0 || (!cu_rows && N % B))
+  if (!cu_rows && B > 0 && N % B)
     return fail(TSC_ERR_INVALID, "groupnorm_backward: N=%lld rows are not %d equal samples",
                 (long long)N, B);
   const int es = elem_size(dtype);
   const size_t bytes = (size_t)N * C * es;
-  if (!workspace || !stats || (N > 0 && (!dy || !x || !dx)))
+  if ((N > 0 && !dx) || (B > 0 && (!workspace || !stats || (N > 0 && (!dy || !x)))))
     return fail(TSC_ERR_INVALID, "groupnorm_backward: null buffer");
   if (!aligned(x, es) || !aligned(dy, es) || !aligned(dx, es) || (gamma && !aligned(gamma, es)) ||
       (beta && !aligned(beta, es)) || (dgamma && !aligned(dgamma, es)) ||
@@ -593,6 +594,12 @@ int tsc_groupnorm_backward(tsc_ctx* ctx, int32_t dtype, const void* dy, const vo
   if (overlaps(dx, bytes, x, bytes) || overlaps(dx, bytes, dy, bytes))
     return fail(TSC_ERR_INVALID, "groupnorm_backward: dx overlaps x or dy");
   DeviceGuard g(ctx->device);
+  if (B == 0) {  // sums over no rows, and every row is outside
+    if (zero_rest) st = zero_launch(ctx, dx, (int64_t)bytes);
+    if (!st && dgamma) st = zero_launch(ctx, dgamma, (int64_t)C * es);
+    if (!st && dbeta) st = zero_launch(ctx, dbeta, (int64_t)C * es);
+    return st;
+  }
   return groupnorm_backward_launch(ctx, dtype, dy, x, cu_rows, B, N, C, groups, gamma, beta,
                                    apply_silu, zero_rest, stats, workspace, dx, dgamma, dbeta);
 }
@@ -812,7 +819,7 @@ int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k
                            cu_seqlens_q, cu_seqlens_kv, B, total_q, total_kv, num_heads, head_dim,
                            scale, max_seqlen_q, max_seqlen_kv, zero_rest, &x);
   if (st) return st;
-  if (B == 0 || total_q == 0) return TSC_OK;
+  if (total_q == 0 || (B == 0 && !zero_rest)) return TSC_OK;
   if (!out) return fail(TSC_ERR_INVALID, "diff_attention: null buffer");
   if ((maps == nullptr) != (lse == nullptr))
     return fail(TSC_ERR_INVALID, "diff_attention: maps and lse go together");
@@ -832,6 +839,7 @@ int tsc_diff_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k
   if (maps && overlaps(out, no, maps, nm))
     return fail(TSC_ERR_INVALID, "diff_attention: out overlaps maps");
   DeviceGuard g(ctx->device);
+  if (B == 0) return zero_launch(ctx, out, (int64_t)no);  // every row is outside
   return diff_attention_launch(ctx, x, out, maps, lse, workspace);
 }
 
@@ -852,9 +860,8 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
                            cu_seqlens_q, cu_seqlens_kv, B, total_q, total_kv, num_heads, head_dim,
                            scale, max_seqlen_q, max_seqlen_kv, zero_rest, &x);
   if (st) return st;
-  if (B == 0 || total_q == 0)
-    return fail(TSC_ERR_INVALID, "diff_attention_backward: no queries (the gradients are zero)");
-  if (!maps || !lse || !dout || !workspace || !dq || (total_kv > 0 && (!dk || !dv)))
+  if ((total_q > 0 && (!maps || !lse || !dout || !dq)) || (total_kv > 0 && (!dk || !dv)) ||
+      (B > 0 && !workspace))
     return fail(TSC_ERR_INVALID, "diff_attention_backward: null buffer");
   const void* a16[6] = {maps, dout, workspace, dq, dk, dv};
   for (const void* p : a16)
@@ -878,6 +885,11 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
         return fail(TSC_ERR_INVALID, "diff_attention_backward: the gradients overlap");
   }
   DeviceGuard g(ctx->device);
+  if (B == 0) {  // every row is outside, and dlambda is a sum over none
+    void* rows[3] = {dq, dk, dv};
+    for (int i = 0; i < 3 && zero_rest && !st; ++i) st = zero_launch(ctx, rows[i], (int64_t)g_bytes[i]);
+    return !st && dlambda ? zero_launch(ctx, dlambda, (int64_t)num_heads * 4) : st;
+  }
   return diff_attention_backward_launch(ctx, x, maps, lse, dout, workspace, dq, dk, dv, dlambda);
 }
 

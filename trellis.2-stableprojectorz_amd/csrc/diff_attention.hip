@@ -1334,8 +1334,8 @@ DaArgs da_args(const DiffAttnArgs& x) {
 
 int64_t diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv, int32_t H,
                                        int32_t D, int32_t max_q, int32_t max_kv, int32_t backward) {
-  if (B == 0 || total_q == 0) return 0;
   const int64_t hb = (int64_t)H * B;
+  if (B == 0 || (total_q == 0 && !backward)) return 0;
   if (backward) return 4 * (2 * (int64_t)H * total_q + hb * tiles_of(max_kv, hb, dkv_rows(dtype, max_kv, hb)));
   const int s = da_plan(dtype, B, total_q, total_kv, H, D, max_q, max_kv).splits;
   return s > 1 ? 4 * (int64_t)s * total_q * H * 2 * (D + 4) : 0;

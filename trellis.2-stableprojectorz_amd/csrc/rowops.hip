@@ -222,6 +222,11 @@ __global__ void __launch_bounds__(256)
   for (; i < n; i += stride) y[i] = (T)((float)a[i] + (float)b[i]);
 }
 
+__global__ void __launch_bounds__(256) zero_kernel(uint16_t* p, int64_t n) {
+  const int64_t stride = (int64_t)gridDim.x * 256;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += stride) p[i] = 0;
+}
+
 inline unsigned ew_grid(int64_t n) {
   int64_t b = (n + 255) / 256;
   if (b > 65536) b = 65536;
@@ -300,6 +305,13 @@ int add_launch(tsc_ctx* ctx, int32_t dtype, const void* a, const void* b, int64_
     default: return fail(TSC_ERR_INVALID, "add: unknown dtype %d", dtype);
   }
   return check_hip(hipGetLastError(), "add launch");
+}
+
+int zero_launch(tsc_ctx* ctx, void* p, int64_t bytes) {
+  if (bytes == 0) return TSC_OK;
+  ProfScope s(ctx, "zero");
+  zero_kernel<<<ew_grid(bytes / 2), 256, 0, ctx->stream>>>((uint16_t*)p, bytes / 2);
+  return check_hip(hipGetLastError(), "zero launch");
 }
 
 }  // namespace tsc

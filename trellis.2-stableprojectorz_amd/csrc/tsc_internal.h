@@ -269,5 +269,7 @@ int layernorm_launch(tsc_ctx* ctx, int32_t dtype, const void* x, int64_t N, int3
                      const void* gamma, const void* beta, float eps, int32_t apply_silu, void* y);
 int silu_launch(tsc_ctx* ctx, int32_t dtype, const void* x, int64_t numel, void* y);
 int add_launch(tsc_ctx* ctx, int32_t dtype, const void* a, const void* b, int64_t numel, void* y);
+// Zeros in an array of 2- or 4-byte values, by a kernel (a captured graph takes no memset).
+int zero_launch(tsc_ctx* ctx, void* p, int64_t bytes);
 
 }  // namespace tsc
