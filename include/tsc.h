@@ -249,8 +249,9 @@ int tsc_groupnorm(tsc_ctx* ctx, int32_t dtype, const void* x, const int32_t* cu_
                   void* y);
 /* Its gradient: dx (N,C), and dgamma, dbeta (C) summed over all samples in `dtype` (NULL = not
  * wanted), from dy, the same x, cu_rows, gamma, beta and apply_silu and the stats that
- * tsc_groupnorm wrote; workspace with backward = 1.  dx must not overlap dy or x.  zero_rest is
- * about rows of dx.  Without samples or rows dgamma and dbeta are zeros. */
+ * tsc_groupnorm wrote; workspace with backward = 1.  The gradients must not overlap each other or an
+ * input (gamma is still read when dgamma is written).  zero_rest is about rows of dx.  Without samples
+ * or rows dgamma and dbeta are zeros. */
 int tsc_groupnorm_backward(tsc_ctx* ctx, int32_t dtype, const void* dy, const void* x,
                            const int32_t* cu_rows, int32_t B, int64_t N, int32_t C, int32_t groups,
                            const void* gamma, const void* beta, int32_t apply_silu,

@@ -474,6 +474,33 @@ def test_c_calls_without_sequences_or_queries(pkg, dev):
             assert not dl.any()
 
 
+def test_c_gradients_over_inputs_are_refused(pkg, dev):
+    """dlambda over lambda above all: other blocks still read lambda when dlambda is written."""
+    import ctypes
+    import sys
+
+    P = lambda t: ctypes.c_void_p(t.data_ptr())
+    lib, hd = sys.modules["trellis2_amd._lib"].stream_handle(0)
+    n, h, d = 40, 2, 64
+    b = {k: torch.ones((n, h, d), device=dev) for k in ("q", "k", "v", "dout", "dq", "dk", "dv")}
+    b.update(lam=torch.ones(h, device=dev), dlam=torch.ones(h, device=dev), lse=torch.ones((2, h, n), device=dev),
+             maps=torch.ones((n, h, 2, d), device=dev))
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    ws = torch.zeros(1 << 14, device=dev)
+
+    def call(**other):
+        x = {k: P(t) for k, t in {**b, **other}.items()}
+        ld = h * d
+        return lib.tsc_diff_attention_backward(
+            hd, 0, x["q"], x["k"], x["v"], ld, ld, ld, x["lam"], P(cu), P(cu), 1, n, n, h, d, 0.0, n, n, 1, x["maps"],
+            x["lse"], x["dout"], P(ws), x["dq"], x["dk"], x["dv"], x["dlam"])
+
+    assert call() == 0
+    for over in ({"dlam": b["lam"]}, {"dlam": b["lse"]}, {"dlam": b["dq"]}, {"dk": b["lse"]}, {"dlam": b["maps"]},
+                 {"dq": b["q"]}, {"dv": b["dk"]}, {"dk": b["dout"]}):
+        assert call(**over) == 1 and b"overlap" in lib.tsc_last_error(), list(over)
+
+
 def test_same_bits_each_time_on_any_stream_and_in_a_graph(pkg, dev):
     """Sums have one order; captured training steps replay to the eager bits with new inputs, with
     eager work in between; two captured graphs share nothing."""

@@ -486,3 +486,28 @@ def test_c_calls_without_samples_or_rows(pkg, dev):
         g.replay()
         torch.cuda.synchronize()
         assert not y.any()
+
+
+def test_c_gradients_over_inputs_are_refused(pkg, dev):
+    """dgamma over gamma above all: blocks that make dx still read gamma when dgamma is written."""
+    import ctypes
+    import sys
+
+    P = lambda t: ctypes.c_void_p(t.data_ptr())
+    lib, h = sys.modules["trellis2_amd._lib"].stream_handle(0)
+    n, c = 64, 32
+    bufs = {k: torch.ones((n, c), device=dev) for k in ("x", "dy", "dx")}
+    bufs.update({k: torch.ones(c, device=dev) for k in ("gamma", "beta", "dgamma", "dbeta")})
+    stats, ws = torch.ones((1, 8, 2), device=dev), torch.zeros(1 << 16, device=dev)
+
+    def call(**other):
+        b = {**bufs, **other}
+        return lib.tsc_groupnorm_backward(h, 0, P(b["dy"]), P(b["x"]), None, 1, n, c, 8, P(b["gamma"]), P(b["beta"]),
+                                          0, 1, P(stats), P(ws), P(b["dx"]), P(b["dgamma"]), P(b["dbeta"]))
+
+    assert call() == 0
+    for over in ({"dgamma": bufs["gamma"]}, {"dbeta": bufs["gamma"]}, {"dbeta": bufs["beta"]},
+                 {"dgamma": bufs["x"][-1]}, {"dbeta": bufs["dy"]}, {"dgamma": bufs["dx"]},
+                 {"dbeta": bufs["dgamma"]}, {"dx": bufs["x"]}, {"dx": bufs["dy"]}, {"gamma": bufs["dx"][3]},
+                 {"dgamma": stats}):
+        assert call(**over) == 1 and b"overlap" in lib.tsc_last_error(), list(over)

@@ -591,8 +591,19 @@ int tsc_groupnorm_backward(tsc_ctx* ctx, int32_t dtype, const void* dy, const vo
       (cu_rows && !aligned(cu_rows, 4)))
     return fail(TSC_ERR_INVALID, "groupnorm_backward: x, dy, gamma, beta and the gradients must be "
                                  "aligned to their element size, stats to 8 bytes, workspace to 16");
-  if (overlaps(dx, bytes, x, bytes) || overlaps(dx, bytes, dy, bytes))
-    return fail(TSC_ERR_INVALID, "groupnorm_backward: dx overlaps x or dy");
+  const size_t row = (size_t)C * es;
+  const void* ins[5] = {x, dy, gamma, beta, stats};
+  const size_t in_bytes[5] = {bytes, bytes, gamma ? row : 0, beta ? row : 0, (size_t)B * groups * 8};
+  const void* gs[3] = {dx, dgamma, dbeta};
+  const size_t g_bytes[3] = {bytes, dgamma ? row : 0, dbeta ? row : 0};
+  for (int i = 0; i < 3; ++i) {
+    for (int j = 0; j < 5; ++j)
+      if (overlaps(gs[i], g_bytes[i], ins[j], in_bytes[j]))
+        return fail(TSC_ERR_INVALID, "groupnorm_backward: a gradient overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (overlaps(gs[i], g_bytes[i], gs[j], g_bytes[j]))
+        return fail(TSC_ERR_INVALID, "groupnorm_backward: the gradients overlap");
+  }
   DeviceGuard g(ctx->device);
   if (B == 0) {  // sums over no rows, and every row is outside
     if (zero_rest) st = zero_launch(ctx, dx, (int64_t)bytes);
@@ -871,13 +882,15 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
     return fail(TSC_ERR_INVALID, "diff_attention_backward: lse and dlambda must be 4-byte aligned");
   const int64_t ld = (int64_t)num_heads * head_dim;
   const size_t no = row_span(total_q, ld, x), nk = row_span(total_kv, ld, x);
-  const void* ins[5] = {q, k, v, maps, dout};
-  const size_t in_bytes[5] = {row_span(total_q, ld_q, x), row_span(total_kv, ld_k, x),
-                              row_span(total_kv, ld_v, x), (size_t)total_q * ld * 8, no};
-  const void* gs[3] = {dq, dk, dv};
-  const size_t g_bytes[3] = {no, nk, nk};
-  for (int i = 0; i < 3; ++i) {
-    for (int j = 0; j < 5; ++j)
+  const void* ins[7] = {q, k, v, maps, dout, lambda, lse};
+  const size_t lam_bytes = (size_t)num_heads * 4;
+  const size_t in_bytes[7] = {row_span(total_q, ld_q, x), row_span(total_kv, ld_k, x),
+                              row_span(total_kv, ld_v, x), (size_t)total_q * ld * 8, no,
+                              lambda ? lam_bytes : 0, (size_t)total_q * num_heads * 8};
+  const void* gs[4] = {dq, dk, dv, dlambda};
+  const size_t g_bytes[4] = {no, nk, nk, dlambda ? lam_bytes : 0};
+  for (int i = 0; i < 4; ++i) {
+    for (int j = 0; j < 7; ++j)
       if (overlaps(gs[i], g_bytes[i], ins[j], in_bytes[j]))
         return fail(TSC_ERR_INVALID, "diff_attention_backward: a gradient overlaps an input");
     for (int j = 0; j < i; ++j)
