@@ -85,3 +85,22 @@ def test_scratch_of_a_gradient_without_queries(pkg):
     ws = pkg.load_library().tsc_diff_attention_workspace_bytes
     assert ws(2, 2, 0, 500, 3, 64, 0, 300, 1) > 0 and ws(2, 2, 0, 500, 3, 64, 0, 300, 0) == 0
     assert ws(2, 0, 10, 10, 3, 64, 10, 10, 1) == 0
+
+
+def test_scratch_of_parts_stays_near_the_inputs(pkg):
+    """Every query has scratch for the longest sequence's parts: at most four times what q, k, v and out
+    take, or 64 MB."""
+    ws = pkg.load_library().tsc_diff_attention_workspace_bytes
+    split = 0
+    for code, size in ((0, 4), (1, 2), (2, 2)):
+        for d in (64, 128):
+            for h in (1, 2, 4, 8):
+                for b in (1, 3, 16, 64, 250):
+                    for longest in (1, 32, 128, 1000):
+                        for kv in (3000, 220000, 4000000):
+                            tq, tkv = b * longest, kv + 148 * (b - 1)
+                            got = ws(code, b, tq, tkv, h, d, longest, kv, 0)
+                            assert got <= max(64 << 20, 8 * (tq + tkv) * h * d * size), (code, d, h, b, longest, kv)
+                            split += got > 0
+    assert split > 200
+    assert ws(1, 64, 8192, 229376, 1, 64, 128, 220000, 0) > 0

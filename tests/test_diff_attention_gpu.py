@@ -391,6 +391,19 @@ def test_hints_below_the_lengths_with_shared_keys(pkg, dev, dtype, d, longest):
             _close(got[n], want[n], f"{n} ({mq}, {mk})")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_parts_held_to_the_scratch_there_is(pkg, dev, dtype, d):
+    """Many short sequences beside a long one: fewer, longer parts of its keys than blocks could run."""
+    lq, lkv, h = [32] * 99 + [1], [97] * 99 + [40000], 1
+    q, k, v, do, lam = _make(lq, lkv, h, d, dtype, 19)
+    cq, ck = _cu(lq), _cu(lkv)
+    got = _run(pkg, dev, q, k, v, do, lam, cq, ck)
+    want = _oracle(q, k, v, do, lam, cq, ck, dtype)
+    for n in got:
+        _close(got[n], want[n], n)
+
+
 def test_incoming_gradient_at_an_odd_address(pkg, dev):
     """The gradient of a result that was joined to one value is a view 2 bytes into a larger one."""
     lens, h, d, dtype = [40, 9], 2, 64, torch.bfloat16

@@ -1264,6 +1264,12 @@ int dq_rows(int32_t dtype, int32_t D, int64_t max_q, int64_t hb) {
 // query on each of 4 sequences, 32071 keys, 12 x 128: 43 us instead of 52; 33 rows: 41 instead of 32), in
 // parts of 1024 keys or more (16 and 9 queries on 20000 and 9000 keys, 8 x 128: 32 us, 39 from 512 on).
 // Grids of kCUs blocks are not split (900 + 700 tokens, 16 x 64, 256 blocks: 25 us, and 55 in two parts).
+// Every query has scratch for as many parts as the longest sequence, so there are no more of them than fit
+// four times what q, k, v and out take, or 64 MB (8192 queries on 64 sequences of which one has 220000 of
+// 229376 keys, 1 x 64 f16: 54 parts in 241 MB, 103 us; 430 in 1.9 GB, 143 us; 14 in 67 MB, 293 us).
+constexpr int64_t kScratchInputs = 4, kScratchLeast = 64 << 20;
+// Scratch of a part: sums of D values and four statistics for each query, head and map.
+int64_t part_bytes(int64_t total_q, int32_t H, int32_t D) { return 4 * total_q * H * 2 * (D + 4); }
 struct Plan {
   int rows, splits, part_keys;
 };
@@ -1291,7 +1297,9 @@ Plan da_plan(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv, int32_
   const int64_t n = slots / (blocks / B) - B;
   if (n <= 0) return p;
   const int64_t part = std::max<int64_t>(least, ((total_kv + n - 1) / n + 63) / 64 * 64);
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((max_kv + part - 1) / part, slots));
+  const int64_t es = dtype == TSC_F32 ? 4 : 2, io = 2 * (total_q + total_kv) * H * D * es;
+  const int64_t room = std::max(kScratchLeast, kScratchInputs * io) / part_bytes(total_q, H, D);
+  p.splits = (int)std::max<int64_t>(1, std::min({(max_kv + part - 1) / part, slots, room}));
   if (p.splits > 1) p.part_keys = (int)std::min<int64_t>(part, INT32_MAX);
   return p;
 }
@@ -1338,7 +1346,7 @@ int64_t diff_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q
   if (B == 0 || (total_q == 0 && !backward)) return 0;
   if (backward) return 4 * (2 * (int64_t)H * total_q + hb * tiles_of(max_kv, hb, dkv_rows(dtype, max_kv, hb)));
   const int s = da_plan(dtype, B, total_q, total_kv, H, D, max_q, max_kv).splits;
-  return s > 1 ? 4 * (int64_t)s * total_q * H * 2 * (D + 4) : 0;
+  return s > 1 ? s * part_bytes(total_q, H, D) : 0;
 }
 
 int diff_attention_launch(tsc_ctx* ctx, const DiffAttnArgs& x, void* out, float* maps, float* lse,
