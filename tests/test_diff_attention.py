@@ -104,3 +104,13 @@ def test_scratch_of_parts_stays_near_the_inputs(pkg):
                             split += got > 0
     assert split > 200
     assert ws(1, 64, 8192, 229376, 1, 64, 128, 220000, 0) > 0
+
+
+def test_scales_beyond_fp32_are_refused(pkg):
+    """The kernels take the scale in fp32, where 0 means the default."""
+    q, lam = _t(10), torch.zeros(2)
+    for scale in (1e-46, 1e39, float("inf")):
+        with pytest.raises(pkg.TscError, match="scale"):
+            pkg.sparse_diff_attention(q, q, q, lam, [0, 10], scale=scale)
+    with pytest.raises(pkg.TscError, match="not on a GPU"):  # this one is taken
+        pkg.sparse_diff_attention(q, q, q, lam, [0, 10], scale=1e-30)

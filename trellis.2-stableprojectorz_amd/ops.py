@@ -595,8 +595,8 @@ def sparse_diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam
         raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: q, k and v must share a dtype")
     if lam.shape != (h,) or lam.dtype != torch.float32:
         raise TscError(_lib.TSC_ERR_INVALID, f"diff_attention: lam must be float32 ({h},)")
-    if scale is not None and not scale > 0:
-        raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: scale must be positive")
+    if scale is not None and not 0 < ctypes.c_float(scale).value < float("inf"):
+        raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: scale must be positive and finite in fp32")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
         raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: out has the wrong shape or dtype")
     _code(q)
