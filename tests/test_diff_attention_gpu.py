@@ -173,6 +173,50 @@ def test_larger_self_attention(pkg, dev, dtype, lq, h):
         _close(got[n][hs] if n == "dlam" else got[n][:, hs], want[n], n)
 
 
+def _two_heads(pkg, dev, lq, lkv, h, d, dtype, seed):
+    """Forward and gradients, the first and the last head against the definition."""
+    q, k, v, do, lam = _make(lq, lkv or lq, h, d, dtype, seed)
+    cq = _cu(lq)
+    ck = cq if lkv is None else _cu(lkv)
+    got = _run(pkg, dev, q, k, v, do, lam, cq, ck)
+    hs = sorted({0, h - 1})
+    want = _oracle(*(t[:, hs] for t in (q, k, v, do)), lam[hs], cq, ck, dtype)
+    for n in got:
+        _close(got[n][hs] if n == "dlam" else got[n][:, hs], want[n], n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("h,n", [(64, 100), (65, 100), (64, 200), (43, 300), (64, 300), (193, 100), (85, 300),
+                                 (64, 500), (257, 100), (64, 600), (107, 300), (96, 500), (77, 640), (577, 70)])
+def test_grids_on_both_sides_of_each_rule(pkg, dev, dtype, d, h, n):
+    """64, 65, 128, 129, 192, 193, 255, 256, 257, 320, 321, 384, 385 and 577 blocks of 128 rows: blocks of 32
+    or of 128 rows, in one or more rounds over the CUs, in each of the three passes."""
+    print(f"  diff attention grid {dtype} D={d} H={h} n={n}", flush=True)
+    _two_heads(pkg, dev, [n], None, h, d, dtype, h + n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lq,h", [([1500, 1300], 12), ([4000], 16), ([300] * 9 + [1, 2500], 5)])
+def test_larger_self_attention_of_64_dimensions(pkg, dev, dtype, lq, h):
+    print(f"  diff attention larger {dtype} D=64 {lq} H={h}", flush=True)
+    _two_heads(pkg, dev, lq, None, h, 64, dtype, h)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lkv,h", [([32], [5000], 2), ([33], [5000], 2), ([1] * 12, [3000] + [0, 1, 63, 64, 65] * 2 + [700], 3),
+                                      ([1, 0, 2] * 7, [40, 900, 0] * 6 + [5000, 3, 1025], 1)])
+def test_parts_of_the_keys_of_many_sequences(pkg, dev, dtype, d, lq, lkv, h):
+    """32 and 33 queries (other blocks at 128 dimensions in 16 bits), and more sequences than are ranked by
+    their keys, most of them with fewer keys than a part."""
+    print(f"  diff attention parts {dtype} D={d} {lq} {lkv}", flush=True)
+    ws = pkg.load_library().tsc_diff_attention_workspace_bytes
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    assert ws(code, len(lq), sum(lq), sum(lkv), h, d, max(lq), max(lkv), 0) > 0
+    _two_heads(pkg, dev, lq, lkv, h, d, dtype, 23 + h)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("lq,lkv,h", [([64] * 13, [1500] + [41] * 12, 16), ([100] * 28, [3000] + [37] * 27, 8),
