@@ -59,8 +59,10 @@ class SparseDiffAttentionBlock3d:
     """x + out(diff_attention(qkv(group_norm(x)))) over each sample's voxels, x's rows grouped by
     sample: group norm, one linear layer for q, k and v (read in place as row slices), differential
     attention, and the output layer with the skip as its residual.  qkv weight (3 C, C), out weight
-    (C, C), lam float32 (num_heads), C = num_heads * 64 or 128.  Without gradients: its linear layers have none (group_norm and
-    sparse_diff_attention do, around another library's linear layers)."""
+    (C, C), lam float32 (num_heads), C = num_heads * 64 or 128.  Attention's result goes to the
+    output layer as it is: no norm per head after the difference, no factor of 1 - lambda's start.
+    Without gradients: its linear layers have none (group_norm and sparse_diff_attention do, around
+    another library's linear layers)."""
 
     def __init__(self, num_heads: int, num_groups: int, norm_weight: torch.Tensor | None,
                  norm_bias: torch.Tensor | None, qkv_weight: torch.Tensor,

@@ -10,8 +10,9 @@
 //
 // The tensors are those of tsc_attention (rows of H heads of D = 64 or 128), so a fragment of k or q
 // feeds one map or the other by its dimensions, and one walk over the keys serves both.  The two
-// maps' weighted sums of v stay apart until their denominators are known (6 D flops a pair; the
-// difference itself would need 4 D, and two walks).  For the gradient the forward pass keeps
+// maps' weighted sums of v stay apart until their denominators are known: 6 D flops a pair.  (A second walk
+// with known denominators would multiply only the difference with v, 2 D instead of 4 D, but make the
+// scores again, 2 D, and the exponentials.)  For the gradient the forward pass keeps
 // P1 v and P2 v in fp32 and the two log-sum-exps, from which the probabilities are made again.
 //
 // Scores are computed in 32 x 32 tiles whose result layout (lane: one column, 16 rows 8(j/4) +
@@ -361,7 +362,7 @@ __device__ __forceinline__ void forward_store(const DaArgs& a, int h, int64_t ro
 }
 
 // fp32, whole sequences: a block of 4 waves owns 128 queries and walks the keys in tiles of 32.  Bound by
-// the fp32 matrix cores: 4096 tokens, 8 x 64, 467 us or 110 TFLOP/s of the 154 a large product reaches.
+// the fp32 matrix cores: 4096 tokens, 8 x 64, 471 us or 109 TFLOP/s of the 154 a large product reaches.
 // At D = 64 two waves per SIMD fill each other's waits; at D = 128 the registers hold one.
 template <int D>
 __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) da_forward32_kernel(const DaArgs a) {
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) da_forward32_kernel(cons
 // fp32, small grids: a block owns 32 queries, and its waves and the blocks of a.splits
 // parts share out the keys, 32 at a time.  Each wave brings its own keys through its own piece of LDS,
 // so none waits for another until the end, where their maxima, denominators and sums are joined.
-// 1024 tokens, 8 x 64 (256 blocks): 46 us, and 132 in the 64 blocks of 128 queries.
+// 1024 tokens, 8 x 64 (256 blocks): 50 us, and 124 in the 64 blocks of 128 queries.
 template <int D>
 __global__ void __launch_bounds__(kNT) da_few32_kernel(const DaArgs a) {
   typedef float T;
@@ -529,9 +530,11 @@ __global__ void __launch_bounds__(kNT) da_few32_kernel(const DaArgs a) {
 // The exponentials bound it: twice those of one map, a quarter of the VALU's rate each.
 // A wave has NM maps of its 32 queries: both at D = 64; one at D = 128, where the sums of both would
 // leave one wave per SIMD, whose stalls nothing fills (9000 + 6143 tokens, 12 x 128 bf16: 1500 us that way,
-// 1300 us or 840 TFLOP/s now).  The two waves of a query tile then meet in LDS at the end.
-// Counted there: matrix cores busy 37 % and VALU 48 % of the cycles, the clock down to 1.8 - 2.0 GHz; at
-// D = 64 (36011 queries on 7 x 1374 keys, 16 heads, f16: 470 us) 29 % and 70 %.
+// 1260 us or 870 TFLOP/s now).  The two waves of a query tile then meet in LDS at the end.
+// Counted there: matrix cores busy 38 % and VALU 50 % of the cycles, the clock down to 1.8 - 2.0 GHz; at
+// D = 64 (36011 queries on 7 x 1374 keys, 16 heads, f16: 455 us) 29 % and 70 %.
+// A wave has 256 registers.  Spilled to scratch: with KEEP 12 at D = 64, at D = 128 2 in blocks of eight
+// waves and 47 in blocks of four; without it 14 in the latter and none in the others.
 // The sums of v are divided by the sum of the rounded P that they were made of.  KEEP (for the backward
 // pass) also adds up the unrounded P: the log-sum-exps have to be those of the fp32 probabilities.
 template <typename T, int D, int NM, int NW, bool KEEP>
@@ -951,8 +954,8 @@ __global__ void __launch_bounds__(kNT) da_rowdot_kernel(const DaArgs a, float* r
 // tiles in turn, each through its own piece of LDS, and their sums are joined at the end.
 // Two waves per SIMD in 16 bits: with one, whose products, exponentials and LDS reads wait for each
 // other, the matrix cores were busy 15 % of the time in dk / dv at D = 128, now 37 %.
-// 4096 tokens: 12 x 128 bf16, dk and dv 412 us, dq 213 (750 and 730 TFLOP/s executed); 16 x 64 bf16 206
-// and 155 (670); 8 x 64 fp32 638 and 491 (107 of the 154 that a large product reaches).
+// 4096 tokens: 12 x 128 bf16, dk and dv 410 us, dq 217 (755 and 715 TFLOP/s executed); 16 x 64 bf16 203
+// and 155 (675 and 665); 8 x 64 fp32 640 and 500 (107 and 103 of the 154 that a large product reaches).
 template <bool SHARE>
 __device__ __forceinline__ void tile_sync() {
   // A wave's own LDS operations are carried out in order; the compiler has to keep that order.
@@ -1069,7 +1072,8 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && !SHARE ? 2 : 1) da_dq_k
 // block_tile goes by the queries here.
 // A wave has NM maps of its 32 keys: both, or one where the registers of both (dk, dv, k and v: 192 at
 // D = 128) leave one wave per SIMD.  Then dP is made twice, P1 and P2 are multiplied with do one by one
-// (12 D flops a pair instead of 8 D), and the two waves' parts of dv meet in LDS at the end.
+// (12 D flops a pair instead of 8 D), and the two waves' parts of dv meet in LDS at the end; 13 of the 256
+// registers are spilled.
 template <typename T, int D, bool SHARE, int NM>
 __global__ void __launch_bounds__(SHARE ? kNT : 512 / NM, sizeof(T) == 2 && !SHARE ? 2 : 1)
     da_dkv_kernel(const DaArgs a) {
@@ -1241,10 +1245,10 @@ unsigned tiles_of(int64_t longest, int64_t hb, int rows = kBQ) {
 // Rows of a block: 128, or 32 that its waves share.  Blocks of 32 are a quarter of the work each, and
 // waste less of the last round over the CUs, but take longer for the joining and for copies that no other
 // wave shares: `cost` tenths of a quarter of the other's time.  Measured, us, in blocks of 128 / of 32
-// rows (the number of 128): fp32 8 x 64, dk and dv, 1024 tokens (64) 165 / 57, 2900 (184) 459 / 397,
-// 4096 (256) 640 / 722, 5000 (320) 1553 / 1109; bf16 12 x 128, dk and dv, 512 (48) 38 / 27, 768 (72)
-// 49 / 56, 1024 (96) 61 / 67; bf16 16 x 64, dq, 1024 (128) 29 / 23, 1536 (192) 40 / 42, its dk and dv
-// 39 / 41 and 55 / 79.
+// rows (the number of 128): fp32 8 x 64, dk and dv, 1024 tokens (64) 164 / 59, 2900 (184) 455 / 388,
+// 4096 (256) 640 / 707, 5000 (320) 1538 / 1088; bf16 12 x 128, dk and dv, 512 (48) 37 / 25, 768 (72)
+// 50 / 54, 1024 (96) 61 / 62, 4096 (384) 408 / 482; bf16 16 x 64, dq, 1024 (128) 29 / 22, 1536 (192)
+// 41 / 41, 4096 (512) 156 / 218, its dk and dv 38 / 39, 54 / 75 and 202 / 432.
 constexpr int kCostF32 = 12, kCost16 = 25, kCost16Dq64 = 15;
 int block_rows(int cost, int64_t longest, int64_t hb) {
   const int64_t b = (int64_t)tiles_of(longest, hb) * hb, rounds = (b + kCUs - 1) / kCUs;
