@@ -594,6 +594,95 @@ def test_same_bits_each_time_on_any_stream_and_in_a_graph(pkg, dev):
                 assert all(torch.equal(a, e) for a, e in zip(outs, eager)), (rep, i)
 
 
+def test_calls_of_several_threads_on_streams_of_their_own(pkg, dev):
+    """Training steps of both operators from four threads at once give the bits of one after the other."""
+    import threading
+
+    cases = []
+    for i in range(4):
+        lq, lkv = ([3, 1, 9], [2500, 40, 900]) if i % 2 else ([300, 41], [300, 41])
+        q, k, v, do, lam = (t.to(dev) for t in _make(lq, lkv, 4, 64, TYPES[i % 3], 30 + i))
+        cq, ck = (torch.tensor(_cu(x), dtype=torch.int32, device=dev) for x in (lq, lkv))
+        cases.append((q, k, v, do, lam, cq, ck))
+
+    def step(q, k, v, do, lam, cq, ck):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+        o = pkg.sparse_diff_attention(*leaves, cq, ck)
+        x = v.detach().flatten(1).requires_grad_()
+        y = pkg.group_norm(x, 8, cu_rows=ck, silu=True)
+        return [o.detach(), y.detach(), *torch.autograd.grad(o, leaves, do),
+                *torch.autograd.grad(y, x, torch.ones_like(y))]
+
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    got[i] = step(*cases[i])
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_captured_step_with_other_offsets(pkg, dev, dtype, d):
+    """The offsets are read on the device: a replay goes by those of its time, parts of the keys included."""
+    tq, tkv, h = 64, 6000, 2
+    q, k, v, do, lam = (t.to(dev) for t in _make([tq], [tkv], h, d, dtype, 31))
+    offsets = [([0, 1, 30, 64], [0, 5000, 5400, 6000]), ([0, 0, 64, 64], [0, 10, 5990, 6000]),
+               ([5, 20, 20, 60], [100, 100, 200, 5999])]
+    cq, ck = (torch.tensor(x, dtype=torch.int32, device=dev) for x in offsets[0])
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+        o = pkg.sparse_diff_attention(*leaves, cq, ck, max_seqlen_q=32, max_seqlen_kv=5000)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step()
+    for a, b in offsets * 2:
+        cq.copy_(torch.tensor(a))
+        ck.copy_(torch.tensor(b))
+        g.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs, want)), (a, b)
+        ref = _oracle(*(t.cpu() for t in (q, k, v, do, lam)), a, b, dtype)
+        for n, t in zip(("out", "dq", "dk", "dv", "dlam"), outs):
+            _close(t, ref[n], n)
+
+
+def test_rows_of_different_strides(pkg, dev):
+    """q out of a projection with other values beside it, k and v out of one for both."""
+    lq, lkv, h, d, dtype = [40, 33], [200, 65], 2, 128, torch.bfloat16
+    q, k, v, do, lam = _make(lq, lkv, h, d, dtype, 32)
+    cq, ck = _cu(lq), _cu(lkv)
+    want = _run(pkg, dev, q, k, v, do, lam, cq, ck)
+    wide = torch.full((sum(lq), h * d + 8), float("nan"), dtype=dtype)
+    wide[:, 8:] = q.flatten(1)
+    wide, kv = wide.to(dev).requires_grad_(), torch.stack([k, v], 1).to(dev).requires_grad_()
+    o = pkg.sparse_diff_attention(wide[:, 8:].unflatten(1, (h, d)), kv[:, 0], kv[:, 1], lam.to(dev), cq, ck)
+    gq, gkv = torch.autograd.grad(o, (wide, kv), do.to(dev))
+    assert torch.equal(o, want["out"]) and torch.equal(gq[:, 8:].unflatten(1, (h, d)), want["dq"])
+    assert torch.equal(gkv[:, 0], want["dk"]) and torch.equal(gkv[:, 1], want["dv"]) and not gq[:, :8].any()
+
+
 def test_more_than_2_31_values(pkg, dev):
     """Keys past the 2^31st element of k and v, their gradients, and zeros before them."""
     h, d, dtype = 16, 128, torch.bfloat16
