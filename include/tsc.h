@@ -258,6 +258,48 @@ int tsc_groupnorm_backward(tsc_ctx* ctx, int32_t dtype, const void* dy, const vo
                            int32_t zero_rest, const float* stats, void* workspace, void* dx,
                            void* dgamma, void* dbeta);
 
+/* Norms of rows: kinds. */
+enum tsc_norm { TSC_NORM_NONE = 0, TSC_NORM_LAYER = 1, TSC_NORM_RMS = 2 };
+/* The norms before and after a transformer block, with its gate, its residual scale and its samples'
+ * modulation, in one pass over the rows (C values each, sample b of the row):
+ *   v = norm(y) * post_weight + post_bias,  r = residual_scale * x + gate[b] * v
+ *   h = (norm(r) * weight + bias) * (1 + scale[b]) + shift[b]
+ * with norm(t) = (t - mean(t)) / sqrt(var(t) + eps) (TSC_NORM_LAYER, biased variance) or
+ * t / sqrt(mean(t^2) + eps) (TSC_NORM_RMS), for y TSC_NORM_NONE too (then without weight and bias).
+ *   x, y, r, h  (N,C) `dtype`, aligned to the element size (16-byte aligned buffers and rows of whole
+ *              16 bytes are fastest), C at most 8192.  y NULL: r = x, and r is NULL too; h NULL: r only.
+ *              r and h may each be x or y itself, but not overlap otherwise
+ *   cu_rows, B, zero_rest  as in tsc_groupnorm (zero_rest is about rows of r and h)
+ *   gate, scale, shift  (B,C) `dtype`, row strides ld_* in elements (at least C), NULL = 1 / 0 / 0
+ *   post_weight, post_bias, weight, bias  (C) `dtype`, NULL = 1 / 0
+ *   stats      NULL, or device fp32 for the backward pass, 8-byte aligned: mean and 1 / sigma of each
+ *              row, (N,2) for y's norm if it has one, then (N,2) for r's if there is an h
+ * fp32 math; r is rounded on its way out only, h is of the unrounded r.  The context keeps nothing.
+ * No counterpart in the reference's sparse path, whose blocks normalize rows without modulation
+ * (src/sparse/ops/norm.ts:10-140). */
+int tsc_gated_norm(tsc_ctx* ctx, int32_t dtype, const void* x, const void* y, const int32_t* cu_rows,
+                   int32_t B, int64_t N, int32_t C, int32_t post_norm, const void* post_weight,
+                   const void* post_bias, const void* gate, int64_t ld_gate, float residual_scale,
+                   int32_t norm, const void* weight, const void* bias, const void* scale,
+                   int64_t ld_scale, const void* shift, int64_t ld_shift, float eps,
+                   int32_t zero_rest, float* stats, void* r, void* h);
+/* Its gradient from dr and dh (NULL = zeros; not both; dr is NULL without y) and what the forward call
+ * was given and its stats: dx, dy (N,C) (dy NULL without y), and in `dtype` dgate, dscale, dshift (B,C)
+ * contiguous, dpost_weight, dpost_bias, dweight, dbias (C) (NULL = not wanted; those of h's norm have to
+ * be NULL without dh, those of y's without y).  workspace: device scratch of
+ * tsc_gated_norm_workspace_bytes, 16-byte aligned (-1: sizes out of range).  The gradients must not
+ * overlap each other or an input.  zero_rest is about rows of dx and dy.  The sums have one fixed order. */
+int64_t tsc_gated_norm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C);
+int tsc_gated_norm_backward(tsc_ctx* ctx, int32_t dtype, const void* x, const void* y,
+                            const int32_t* cu_rows, int32_t B, int64_t N, int32_t C,
+                            int32_t post_norm, const void* post_weight, const void* post_bias,
+                            const void* gate, int64_t ld_gate, float residual_scale, int32_t norm,
+                            const void* weight, const void* bias, const void* scale, int64_t ld_scale,
+                            const void* shift, int64_t ld_shift, float eps, int32_t zero_rest,
+                            const float* stats, const void* dr, const void* dh, void* workspace,
+                            void* dx, void* dy, void* dgate, void* dpost_weight, void* dpost_bias,
+                            void* dscale, void* dshift, void* dweight, void* dbias);
+
 /* Sparse ResBlock: out = x + conv2(silu(LN(conv1(x)+b1))) + b2, with C=Ci=Co.
  * LN uses eps and gamma/beta (NULL = 1/0).  out must not overlap x (TSC_ERR_INVALID if any
  * byte of the two (N,C) ranges is shared).  The intermediate (N,C)

@@ -12,6 +12,8 @@ is not a Python identifier.
   sparse_attention,                              varlen attention (sparse/ops/attention.ts:24-79,
   scaled_dot_product_attention                   dense/ops/attention.ts:36-110)
   group_norm, SparseGroupNorm                    group norm over each sample's rows, with gradients
+  modulated_norm, gated_residual,                norms before and after a block with its samples'
+  gated_residual_norm                            modulation, gate and residual scale, with gradients
   sparse_diff_attention,                         difference of two softmax maps, with gradients, and
   SparseDiffAttentionBlock3d                     the block around it
   SafetensorsFile, MultiFileLoader               weight files -> device tensors (weights.ts:58-237)
@@ -22,7 +24,8 @@ from .sparse_tensor import SparseTensor, Scale, Fraction, SCALE_IDENTITY, comput
 from .conv3d import SparseConv3d, SparseResBlock3d, get_neighbor_map, neighbor_cache_key  # noqa: F401
 from .ops import (NeighborMap, build_neighbor_map, map_conv_order, map_gather_plan,  # noqa: F401
                   sparse_conv3d,
-                  layer_norm, group_norm, silu, add, sparse_resblock, sparse_subdivide, subdivide_count,
+                  layer_norm, group_norm, modulated_norm, gated_residual, gated_residual_norm, silu, add,
+                  sparse_resblock, sparse_subdivide, subdivide_count,
                   sparse_linear, sparse_attention, sparse_diff_attention,
                   scaled_dot_product_attention)
 from .spatial import SparseSubdivide  # noqa: F401
@@ -33,7 +36,7 @@ from . import workloads  # noqa: F401
 __all__ = [
     "TscError", "SparseTensor", "SparseConv3d", "SparseResBlock3d", "NeighborMap",
     "build_neighbor_map", "map_conv_order", "map_gather_plan", "sparse_conv3d", "layer_norm", "group_norm",
-    "silu", "add", "sparse_resblock",
+    "modulated_norm", "gated_residual", "gated_residual_norm", "silu", "add", "sparse_resblock",
     "sparse_subdivide", "subdivide_count", "SparseSubdivide", "sparse_linear", "SparseLinear", "SparseGroupNorm",
     "SparseConvNeXtBlock3d", "SparseDiffAttentionBlock3d", "sparse_attention",
     "sparse_diff_attention", "scaled_dot_product_attention", "SafetensorsFile", "SafetensorsHeader", "TensorEntry", "MultiFileLoader",

@@ -19,6 +19,7 @@ TSC_F32, TSC_F16, TSC_BF16 = 0, 1, 2
 TSC_MAP_DUPLICATE, TSC_MAP_OUT_OF_RANGE = 1, 2
 TSC_MAP_AUTO, TSC_MAP_BITMAP, TSC_MAP_RADIX = 0, 1, 2
 TSC_EPI_BIAS, TSC_EPI_BIAS_RESIDUAL, TSC_EPI_BIAS_LN_SILU = 0, 1, 2
+TSC_NORM_NONE, TSC_NORM_LAYER, TSC_NORM_RMS = 0, 1, 2
 TSC_ST_RAW = -1
 # safetensors header dtype strings in tsc_st_dtype order, with their element sizes
 ST_DTYPES = ("F32", "F16", "BF16", "F64", "I64", "I32", "I16", "I8", "U8", "BOOL", "U16", "U32",
@@ -26,6 +27,9 @@ ST_DTYPES = ("F32", "F16", "BF16", "F64", "I64", "I32", "I16", "I8", "U8", "BOOL
 ST_SIZES = (4, 2, 2, 8, 8, 4, 2, 1, 1, 1, 2, 4, 8, 1, 1)
 
 MAP_METHODS = {"auto": TSC_MAP_AUTO, "bitmap": TSC_MAP_BITMAP, "radix": TSC_MAP_RADIX}
+
+
+NORMS = {None: TSC_NORM_NONE, "layer": TSC_NORM_LAYER, "rms": TSC_NORM_RMS}
 
 
 class TscError(RuntimeError):
@@ -77,6 +81,12 @@ _SIGNATURES = {
                              _P, _P]),
     "tsc_groupnorm_backward": (_I32, [_P, _I32, _P, _P, _P, _I32, _I64, _I32, _I32, _P, _P, _I32,
                                       _I32, _P, _P, _P, _P, _P]),
+    "tsc_gated_norm": (_I32, [_P, _I32, _P, _P, _P, _I32, _I64, _I32, _I32, _P, _P, _P, _I64, _F32, _I32,
+                              _P, _P, _P, _I64, _P, _I64, _F32, _I32, _P, _P, _P]),
+    "tsc_gated_norm_workspace_bytes": (_I64, [_I32, _I32, _I64, _I32]),
+    "tsc_gated_norm_backward": (_I32, [_P, _I32, _P, _P, _P, _I32, _I64, _I32, _I32, _P, _P, _P, _I64,
+                                       _F32, _I32, _P, _P, _P, _I64, _P, _I64, _F32, _I32, _P, _P, _P,
+                                       _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "tsc_silu": (_I32, [_P, _I32, _P, _I64, _P]),
     "tsc_add": (_I32, [_P, _I32, _P, _P, _I64, _P]),
     "tsc_resblock": (_I32, [_P, _I32, _P, _P, _P, _I64, _I32, _P, _P, _P, _P, _F32, _P, _P, _P]),

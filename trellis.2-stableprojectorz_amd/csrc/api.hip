@@ -615,6 +615,145 @@ int tsc_groupnorm_backward(tsc_ctx* ctx, int32_t dtype, const void* dy, const vo
                                    apply_silu, zero_rest, stats, workspace, dx, dgamma, dbeta);
 }
 
+// Checks what both calls are given; `stats` is the forward call's output and the backward call's input.
+static int gated_norm_args(const char* what, const GatedNormArgs& x, const void* h, const float* stats) {
+  const int es = elem_size(x.dtype);
+  if (!es) return fail(TSC_ERR_INVALID, "%s: unknown dtype %d", what, x.dtype);
+  if (x.N < 0 || x.N > INT32_MAX || x.C <= 0 || x.B < 0 || x.B > (1 << 20))
+    return fail(TSC_ERR_INVALID, "%s: bad sizes N=%lld C=%d B=%d", what, (long long)x.N, x.C, x.B);
+  if (x.C > gated_norm_max_channels())
+    return fail(TSC_ERR_UNSUPPORTED, "%s: C=%d exceeds %d", what, x.C, gated_norm_max_channels());
+  if (!x.cu && x.B > 0 && x.N % x.B)
+    return fail(TSC_ERR_INVALID, "%s: N=%lld rows are not %d equal samples", what, (long long)x.N, x.B);
+  if (!(x.eps >= 0.f) || !isfinite(x.eps)) return fail(TSC_ERR_INVALID, "%s: eps must be >= 0 and finite", what);
+  if (!isfinite(x.residual_scale)) return fail(TSC_ERR_INVALID, "%s: residual_scale must be finite", what);
+  if (x.y && (x.post_norm < TSC_NORM_NONE || x.post_norm > TSC_NORM_RMS))
+    return fail(TSC_ERR_INVALID, "%s: unknown post_norm %d", what, x.post_norm);
+  if (x.y ? x.post_norm == TSC_NORM_NONE && (x.post_weight || x.post_bias)
+          : x.post_weight || x.post_bias || x.gate)
+    return fail(TSC_ERR_INVALID, "%s: post_weight and post_bias go with a post_norm, gate with y", what);
+  if (h && x.norm != TSC_NORM_LAYER && x.norm != TSC_NORM_RMS)
+    return fail(TSC_ERR_INVALID, "%s: unknown norm %d", what, x.norm);
+  const void* mods[3] = {x.gate, x.scale, x.shift};
+  const int64_t lds[3] = {x.ld_gate, x.ld_scale, x.ld_shift};
+  for (int i = 0; i < 3; ++i)
+    if (mods[i] && (lds[i] < x.C || lds[i] > INT32_MAX))
+      return fail(TSC_ERR_INVALID, "%s: row stride %lld of gate, scale or shift (C=%d to 2^31 - 1)", what,
+                  (long long)lds[i], x.C);
+  const void* vals[9] = {x.x, x.y, x.post_weight, x.post_bias, x.gate, x.weight, x.bias, x.scale, x.shift};
+  for (const void* p : vals)
+    if (!aligned(p, es)) return fail(TSC_ERR_INVALID, "%s: buffers must be aligned to their element size", what);
+  if (!aligned(stats, 8) || !aligned(x.cu, 4))
+    return fail(TSC_ERR_INVALID, "%s: stats must be aligned to 8 bytes, cu_rows to 4", what);
+  return TSC_OK;
+}
+
+int tsc_gated_norm(tsc_ctx* ctx, int32_t dtype, const void* x, const void* y, const int32_t* cu_rows,
+                   int32_t B, int64_t N, int32_t C, int32_t post_norm, const void* post_weight,
+                   const void* post_bias, const void* gate, int64_t ld_gate, float residual_scale,
+                   int32_t norm, const void* weight, const void* bias, const void* scale,
+                   int64_t ld_scale, const void* shift, int64_t ld_shift, float eps,
+                   int32_t zero_rest, float* stats, void* r, void* h) {
+  g_err[0] = 0;
+  int st = check_ctx(ctx);
+  if (st) return st;
+  const GatedNormArgs a{dtype, x,    y,    cu_rows, B,     N,        C,     post_norm, post_weight, post_bias, gate, ld_gate,
+                        residual_scale, norm, weight, bias, scale, ld_scale, shift, ld_shift,  eps,         zero_rest};
+  st = gated_norm_args("gated_norm", a, h, stats);
+  if (st) return st;
+  if (N == 0 || (B == 0 && !zero_rest)) return TSC_OK;
+  if ((y == nullptr) != (r == nullptr) || (!r && !h) || (B > 0 && !x))
+    return fail(TSC_ERR_INVALID, "gated_norm: null buffer (r goes with y; r or h is written)");
+  const int es = elem_size(dtype);
+  const size_t bytes = (size_t)N * C * es;
+  if (!aligned(r, es) || !aligned(h, es))
+    return fail(TSC_ERR_INVALID, "gated_norm: buffers must be aligned to their element size");
+  const void* outs[2] = {r, h};
+  for (const void* o : outs)
+    if (o)
+      for (const void* in : {x, y})
+        if (in && o != in && overlaps(o, bytes, in, bytes))
+          return fail(TSC_ERR_INVALID, "gated_norm: an output overlaps x or y without being it");
+  if (r && h && overlaps(r, bytes, h, bytes)) return fail(TSC_ERR_INVALID, "gated_norm: r overlaps h");
+  DeviceGuard g(ctx->device);
+  if (B == 0) {  // every row is outside
+    if (r) st = zero_launch(ctx, r, (int64_t)bytes);
+    return !st && h ? zero_launch(ctx, h, (int64_t)bytes) : st;
+  }
+  return gated_norm_launch(ctx, a, stats, r, h);
+}
+
+int64_t tsc_gated_norm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C) {
+  g_err[0] = 0;
+  GatedNormArgs a = {};
+  a.dtype = dtype;
+  a.B = B;
+  a.N = B > 0 && N >= 0 ? N / B * B : N;  // whichever way the rows are cut into samples
+  a.C = C;
+  if (gated_norm_args("gated_norm_workspace_bytes", a, nullptr, nullptr)) return -1;
+  return gated_norm_workspace_bytes(dtype, B, N, C);
+}
+
+int tsc_gated_norm_backward(tsc_ctx* ctx, int32_t dtype, const void* x, const void* y,
+                            const int32_t* cu_rows, int32_t B, int64_t N, int32_t C,
+                            int32_t post_norm, const void* post_weight, const void* post_bias,
+                            const void* gate, int64_t ld_gate, float residual_scale, int32_t norm,
+                            const void* weight, const void* bias, const void* scale, int64_t ld_scale,
+                            const void* shift, int64_t ld_shift, float eps, int32_t zero_rest,
+                            const float* stats, const void* dr, const void* dh, void* workspace,
+                            void* dx, void* dy, void* dgate, void* dpost_weight, void* dpost_bias,
+                            void* dscale, void* dshift, void* dweight, void* dbias) {
+  g_err[0] = 0;
+  int st = check_ctx(ctx);
+  if (st) return st;
+  const GatedNormArgs a{dtype, x,    y,    cu_rows, B,     N,        C,     post_norm, post_weight, post_bias, gate, ld_gate,
+                        residual_scale, norm, weight, bias, scale, ld_scale, shift, ld_shift,  eps,         zero_rest};
+  st = gated_norm_args("gated_norm_backward", a, dh, stats);
+  if (st) return st;
+  if ((N > 0 && (!dx || (y && !dy) || (!dr && !dh) || (B > 0 && !x))) || (B > 0 && !workspace) ||
+      (N > 0 && B > 0 && !stats && (dh || (y && post_norm != TSC_NORM_NONE))))
+    return fail(TSC_ERR_INVALID, "gated_norm_backward: null buffer");
+  if ((!y && (dr || dy || dgate || dpost_weight || dpost_bias)) ||
+      (!dh && (dscale || dshift || dweight || dbias)))
+    return fail(TSC_ERR_INVALID, "gated_norm_backward: gradients of a part that is not there");
+  const int es = elem_size(dtype);
+  const size_t bytes = (size_t)N * C * es, row = (size_t)C * es, mod = (size_t)B * C * es;
+  const void* gs[9] = {dx, dy, dgate, dpost_weight, dpost_bias, dscale, dshift, dweight, dbias};
+  const size_t g_bytes[9] = {bytes, bytes, mod, row, row, mod, mod, row, row};
+  const size_t norms = (dh ? 1 : 0) + (y && post_norm != TSC_NORM_NONE ? 1 : 0);
+  auto span = [&](int64_t ld) { return B > 0 ? ((size_t)(B - 1) * ld + C) * es : 0; };
+  const void* ins[12] = {x, y, dr, dh, gate, scale, shift, post_weight, post_bias, weight, bias, stats};
+  const size_t in_bytes[12] = {bytes, bytes, bytes, bytes, span(ld_gate), span(ld_scale), span(ld_shift),
+                               row, row, row, row, norms * (size_t)N * 8};
+  for (int i = 0; i < 9; ++i) {
+    if (!gs[i]) continue;
+    if (!aligned(gs[i], es))
+      return fail(TSC_ERR_INVALID, "gated_norm_backward: buffers must be aligned to their element size");
+    for (int j = 0; j < 12; ++j)
+      if (ins[j] && overlaps(gs[i], g_bytes[i], ins[j], in_bytes[j]))
+        return fail(TSC_ERR_INVALID, "gated_norm_backward: a gradient overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (gs[j] && overlaps(gs[i], g_bytes[i], gs[j], g_bytes[j]))
+        return fail(TSC_ERR_INVALID, "gated_norm_backward: the gradients overlap");
+  }
+  if (!aligned(dr, es) || !aligned(dh, es) || !aligned(workspace, 16))
+    return fail(TSC_ERR_INVALID, "gated_norm_backward: dr and dh must be aligned to their element size, "
+                                 "workspace to 16 bytes");
+  DeviceGuard g(ctx->device);
+  if (B == 0) {  // sums over no rows, and every row is outside
+    for (int i = 0; i < 9 && !st; ++i)
+      if (gs[i] && (i > 1 || zero_rest)) st = zero_launch(ctx, (void*)gs[i], (int64_t)g_bytes[i]);
+    return st;
+  }
+  if (N == 0) {
+    for (int i = 2; i < 9 && !st; ++i)
+      if (gs[i]) st = zero_launch(ctx, (void*)gs[i], (int64_t)g_bytes[i]);
+    return st;
+  }
+  const GatedNormGrads grads{dx, dy, dgate, dpost_weight, dpost_bias, dscale, dshift, dweight, dbias};
+  return gated_norm_backward_launch(ctx, a, stats, dr, dh, workspace, grads);
+}
+
 int tsc_silu(tsc_ctx* ctx, int32_t dtype, const void* x, int64_t numel, void* y) {
   g_err[0] = 0;
   int st = check_ctx(ctx);

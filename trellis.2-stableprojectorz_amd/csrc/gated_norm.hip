@@ -1,0 +1,799 @@
+// The norms before and after a transformer block, fused with its gate, its residual scale and its
+// samples' modulation, and their gradients.  Per row of C values, sample b of the row:
+//
+//   v = norm(y) pw + pb               the block's output, after its norm (or y itself)
+//   r = rs x + gate_b v               the residual stream
+//   h = (norm(r) w + bias)(1 + scale_b) + shift_b     the next block's input
+//   norm(t) = (t - mean) rstd, rstd = 1 / sqrt(var + eps)   (layer), or t / sqrt(mean(t^2) + eps)  (rms)
+// without y: r = x, and without h: only r.  Gradient, with rh = norm(r), yh = norm(y):
+//   drh = dh (1 + scale) w;   dr += rstd_r (drh - m1 - rh mean(drh rh)),  m1 = mean(drh) (layer) or 0
+//   dx = rs dr;   dyh = gate pw dr;   dy = rstd_y (dyh - m2 - yh mean(dyh yh))
+//   per sample P = sum dh rh, Q = sum dh, P' = sum dr yh, Q' = sum dr:
+//   dscale = w P + bias Q, dshift = Q, dgate = pw P' + pb Q';   dw = sum_b (1 + scale) P,
+//   dbias = sum_b (1 + scale) Q, dpw = sum_b gate P', dpb = sum_b gate Q'
+//
+// Bound by memory: a row stays in registers between its reads and its writes, and what is the same for
+// all rows of a sample (modulation and weights, folded) is in registers for a run of rows.
+// A row belongs to G lanes of a wave (a power of 2, up to C = 1024) or to a whole block; a block has R
+// rows one after the other, through as many samples as those rows touch.  Means and variances are taken
+// in two steps from the registers, so that a spread beside a large mean keeps its bits.  r is not
+// rounded before its own norm, and the gradient makes it again from x and y instead of reading it
+// (the same bytes), so that both are those of the unrounded sum.
+// The samples' sums have one order: a block adds up its rows of a sample in slot t + b of the scratch
+// (block t and sample b; along the rows one of the two grows at each step, so slots are distinct),
+// and a second kernel adds up each sample's slots.
+
+#include <algorithm>
+#include <initializer_list>
+#include <type_traits>
+
+#include "tsc_internal.h"
+
+namespace tsc {
+namespace {
+
+constexpr int kWaveC = 1024;    // widest row of one wave
+constexpr int kMaxC = 8192;     // widest row of a block of 16 waves
+constexpr int kSumCols = 16, kSumRows = 64;  // threads of a block that adds up the slots
+constexpr int kLoopB = 16;      // samples that one block of that kernel walks
+
+struct GnArgs {
+  const void *x, *y;
+  const int32_t* cu;  // null: B samples of `each` rows
+  int64_t N, each, R;
+  int32_t B, C, G, post, norm, rest;
+  const void *pw, *pb, *w, *bias, *gate, *scale, *shift;
+  int64_t ldg, lds, ldt;
+  float rs, eps, inv_c;
+  float2 *ystat, *rstat;  // mean, rstd of each row, or null
+  void *r, *h;
+  // backward
+  const void *dr, *dh;
+  void *dx, *dy;
+  float* part;  // (slots, sums, C)
+  int32_t sums;
+};
+
+template <typename T, int VN>
+struct __attribute__((aligned(VN * sizeof(T)))) Pack {
+  T v[VN];
+};
+
+// The sample of a row and the end of its run of rows with the same sample, both uniform; -1 outside.
+// Every lane of the wave takes part.  `row` < N; the run ends past row whatever cu holds.
+__device__ __forceinline__ int sample_of(const GnArgs& a, int64_t row, int64_t* stop) {
+  if (!a.cu) {
+    const int b = (int)(row / a.each);
+    *stop = (int64_t)(b + 1) * a.each;
+    return b;
+  }
+  const int lane = threadIdx.x & 63;
+  int base = 0, len = a.B + 1, count = 0;  // count: offsets at or below row, searched 64 at a time
+  while (true) {
+    const int stride = (len + 63) / 64, at = lane * stride;
+    const bool in = at < len && (int64_t)a.cu[base + min(at, len - 1)] <= row;
+    const int c = __popcll(__builtin_amdgcn_ballot_w64(in));
+    if (stride == 1) {
+      count = base + c;
+      break;
+    }
+    if (c == 0) {
+      count = base;
+      break;
+    }
+    base += (c - 1) * stride;
+    len = min(stride, len - (c - 1) * stride);
+  }
+  count = __builtin_amdgcn_readfirstlane(count);
+  const int64_t next = count <= a.B ? (int64_t)a.cu[count] : a.N;
+  *stop = min(a.N, max(row + 1, next));
+  return count >= 1 && count <= a.B ? count - 1 : -1;
+}
+
+// A row's lanes: G of a wave, or the block.
+template <int MAXV, bool BLOCK>
+struct Team {
+  int G, lane, first, step;  // lanes of a row, this one's number, first row slot, rows a step covers
+  int phase = 0;
+  __device__ explicit Team(int g) {
+    if (BLOCK) {
+      G = blockDim.x;
+      lane = threadIdx.x;
+      first = 0;
+      step = 1;
+    } else {
+      G = g;
+      lane = threadIdx.x & (g - 1);
+      first = threadIdx.x / g;
+      step = blockDim.x / g;
+    }
+  }
+  // Sums of N values over the row's lanes.
+  template <int N>
+  __device__ __forceinline__ void sum(float (&v)[N]) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+      if (BLOCK || off < G)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off, 64);
+    if constexpr (BLOCK) {  // two rounds of slots, so that one barrier keeps a round from the next
+      __shared__ float meet[2][16][2];
+      static_assert(N <= 2, "slots");
+      const int nw = blockDim.x >> 6, w = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) meet[phase][w][i] = v[i];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float t = 0.f;
+        for (int x = 0; x < nw; ++x) t += meet[phase][x][i];
+        v[i] = t;
+      }
+      phase ^= 1;
+    }
+  }
+};
+
+// The lane's values of a row: vectors lane + G k, k < MAXV.
+template <typename T, int VN, int MAXV>
+struct Cols {
+  Pack<T, VN> v[MAXV];
+  __device__ __forceinline__ void load(const T* row, int lane, int G, int nvec) {
+#pragma unroll
+    for (int k = 0; k < MAXV; ++k)
+      if (lane + G * k < nvec) v[k] = *(const Pack<T, VN>*)(row + (int64_t)(lane + G * k) * VN);
+  }
+};
+template <typename T, int VN, int MAXV>
+__device__ __forceinline__ void store_row(T* row, int lane, int G, int nvec, const float (&f)[MAXV][VN]) {
+#pragma unroll
+  for (int k = 0; k < MAXV; ++k)
+    if (lane + G * k < nvec) {
+      Pack<T, VN> o;
+#pragma unroll
+      for (int e = 0; e < VN; ++e) o.v[e] = (T)f[k][e];
+      *(Pack<T, VN>*)(row + (int64_t)(lane + G * k) * VN) = o;
+    }
+}
+// A vector of C parameters in fp32, `none` where there is none.
+template <typename T, int VN, int MAXV>
+__device__ __forceinline__ void params(const void* p, int64_t at, int lane, int G, int nvec, float none,
+                                       float (&f)[MAXV][VN]) {
+  Cols<T, VN, MAXV> c;
+  if (p) c.load((const T*)p + at, lane, G, nvec);
+#pragma unroll
+  for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+    for (int e = 0; e < VN; ++e) f[k][e] = p && lane + G * k < nvec ? (float)c.v[k].v[e] : none;
+}
+
+// Normalizes t in place; lanes past the row's end hold zeros before and after.
+template <int VN, int MAXV, typename Tm>
+__device__ __forceinline__ float2 normalize(Tm& team, int kind, float inv_c, float eps, int nvec,
+                                            float (&t)[MAXV][VN]) {
+  float mean = 0.f;
+  if (kind == TSC_NORM_LAYER) {
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+      for (int e = 0; e < VN; ++e) s[0] += t[k][e];
+    team.sum(s);
+    mean = s[0] * inv_c;
+  }
+  float q[1] = {0.f};
+#pragma unroll
+  for (int k = 0; k < MAXV; ++k)
+    if (team.lane + team.G * k < nvec)
+#pragma unroll
+      for (int e = 0; e < VN; ++e) {
+        t[k][e] -= mean;
+        q[0] = fmaf(t[k][e], t[k][e], q[0]);
+      }
+  team.sum(q);
+  const float rstd = 1.f / sqrtf(fmaf(q[0], inv_c, eps));
+#pragma unroll
+  for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+    for (int e = 0; e < VN; ++e) t[k][e] *= rstd;
+  return make_float2(mean, rstd);
+}
+
+template <typename T, int VN, int MAXV, bool BLOCK, bool Y, bool H>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256) gated_norm_kernel(const GnArgs a) {
+  Team<MAXV, BLOCK> team(a.G);
+  const int lane = team.lane, G = team.G, C = a.C, nvec = C / VN;
+  const int64_t end = min(a.N, ((int64_t)blockIdx.x + 1) * a.R);
+  for (int64_t row0 = (int64_t)blockIdx.x * a.R; row0 < end;) {
+    int64_t stop;
+    const int b = sample_of(a, row0, &stop);
+    stop = min(stop, end);
+    if (b < 0) {  // outside every sample
+      if (a.rest) {
+        float zero[MAXV][VN] = {};
+        for (int64_t row = row0 + team.first; row < stop; row += team.step) {
+          if (Y) store_row<T, VN, MAXV>((T*)a.r + row * C, lane, G, nvec, zero);
+          if (H) store_row<T, VN, MAXV>((T*)a.h + row * C, lane, G, nvec, zero);
+        }
+      }
+      row0 = stop;
+      continue;
+    }
+    // v's factor and summand with the gate; h's factor and summand with the modulation.
+    float gf[MAXV][VN], gs[MAXV][VN], hf[MAXV][VN], hs[MAXV][VN], t[MAXV][VN];
+    if (Y) {
+      params<T, VN, MAXV>(a.gate, b * a.ldg, lane, G, nvec, 1.f, gf);
+      params<T, VN, MAXV>(a.pb, 0, lane, G, nvec, 0.f, gs);
+      params<T, VN, MAXV>(a.pw, 0, lane, G, nvec, 1.f, t);
+#pragma unroll
+      for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+          if (a.pb) gs[k][e] *= gf[k][e];  // uniform: without one it is 0, whatever the gate
+          gf[k][e] *= t[k][e];
+        }
+    }
+    if (H) {
+      params<T, VN, MAXV>(a.scale, b * a.lds, lane, G, nvec, 0.f, hf);
+      params<T, VN, MAXV>(a.bias, 0, lane, G, nvec, 0.f, hs);
+      params<T, VN, MAXV>(a.shift, b * a.ldt, lane, G, nvec, 0.f, t);
+#pragma unroll
+      for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+          hf[k][e] += 1.f;
+          hs[k][e] = a.bias ? fmaf(hs[k][e], hf[k][e], t[k][e]) : t[k][e];
+        }
+      params<T, VN, MAXV>(a.w, 0, lane, G, nvec, 1.f, t);
+#pragma unroll
+      for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) hf[k][e] *= t[k][e];
+    }
+    Cols<T, VN, MAXV> xn, yn;  // the next row's, on their way
+    int64_t row = row0 + team.first;
+    if (row < stop) {
+      xn.load((const T*)a.x + row * C, lane, G, nvec);
+      if (Y) yn.load((const T*)a.y + row * C, lane, G, nvec);
+    }
+    // Lanes of a wave whose row is past the run still take part in the sums.
+    for (int64_t lead = row0; lead < stop; lead += team.step, row += team.step) {
+      const bool live = row < stop;
+      float x[MAXV][VN], y[MAXV][VN];
+#pragma unroll
+      for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+          const bool in = live && lane + G * k < nvec;
+          x[k][e] = in ? (float)xn.v[k].v[e] : 0.f;
+          if (Y) y[k][e] = in ? (float)yn.v[k].v[e] : 0.f;
+        }
+      if (row + team.step < stop) {
+        xn.load((const T*)a.x + (row + team.step) * C, lane, G, nvec);
+        if (Y) yn.load((const T*)a.y + (row + team.step) * C, lane, G, nvec);
+      }
+      if (Y) {
+        if (a.post != TSC_NORM_NONE) {
+          const float2 st = normalize<VN, MAXV>(team, a.post, a.inv_c, a.eps, nvec, y);
+          if (a.ystat && live && lane == 0) a.ystat[row] = st;
+        }
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k)
+          if (lane + G * k < nvec)
+#pragma unroll
+            for (int e = 0; e < VN; ++e) x[k][e] = fmaf(a.rs, x[k][e], fmaf(gf[k][e], y[k][e], gs[k][e]));
+        if (live) store_row<T, VN, MAXV>((T*)a.r + row * C, lane, G, nvec, x);
+      }
+      if (H) {
+        const float2 st = normalize<VN, MAXV>(team, a.norm, a.inv_c, a.eps, nvec, x);
+        if (a.rstat && live && lane == 0) a.rstat[row] = st;
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+          for (int e = 0; e < VN; ++e) x[k][e] = fmaf(x[k][e], hf[k][e], hs[k][e]);
+        if (live) store_row<T, VN, MAXV>((T*)a.h + row * C, lane, G, nvec, x);
+      }
+    }
+    row0 = stop;
+  }
+}
+
+// Adds up the block's lanes that hold the same columns and leaves the sums of a sample's rows in their slot.
+template <int VN, int MAXV, bool BLOCK>
+__device__ __forceinline__ void flush(const GnArgs& a, const Team<MAXV, BLOCK>& team, int64_t slot, int which,
+                                      float (&s)[MAXV][VN]) {
+  const int nvec = a.C / VN;
+  float* out = a.part + (slot * a.sums + which) * a.C;
+  if constexpr (BLOCK) {
+#pragma unroll
+    for (int k = 0; k < MAXV; ++k)
+      if (team.lane + team.G * k < nvec)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) out[(team.lane + team.G * k) * VN + e] = s[k][e];
+  } else {
+    __shared__ float meet[4][64 * MAXV * VN];
+    for (int off = 32; off >= team.G; off >>= 1)
+#pragma unroll
+      for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) s[k][e] += __shfl_xor(s[k][e], off, 64);
+    const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
+    __syncthreads();  // the last sums have been read
+    if (l < team.G)
+#pragma unroll
+      for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+        for (int e = 0; e < VN; ++e) meet[w][(k * VN + e) * 64 + l] = s[k][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.C; c += 256) {
+      const int vec = c / VN, at = (vec / team.G * VN + c % VN) * 64 + vec % team.G;
+      out[c] = (meet[0][at] + meet[1][at]) + (meet[2][at] + meet[3][at]);
+    }
+  }
+}
+
+template <typename T, int VN, int MAXV, bool BLOCK, bool Y, bool H>
+__global__ void __launch_bounds__(BLOCK ? 1024 : 256) gated_norm_backward_kernel(const GnArgs a) {
+  Team<MAXV, BLOCK> team(a.G);
+  const int lane = team.lane, G = team.G, C = a.C, nvec = C / VN;
+  const int64_t end = min(a.N, ((int64_t)blockIdx.x + 1) * a.R);
+  for (int64_t row0 = (int64_t)blockIdx.x * a.R; row0 < end;) {
+    int64_t stop;
+    const int b = sample_of(a, row0, &stop);
+    stop = min(stop, end);
+    if (b < 0) {
+      if (a.rest) {
+        float zero[MAXV][VN] = {};
+        for (int64_t row = row0 + team.first; row < stop; row += team.step) {
+          store_row<T, VN, MAXV>((T*)a.dx + row * C, lane, G, nvec, zero);
+          if (Y) store_row<T, VN, MAXV>((T*)a.dy + row * C, lane, G, nvec, zero);
+        }
+      }
+      row0 = stop;
+      continue;
+    }
+    float hf[MAXV][VN], gf[MAXV][VN], gs[MAXV][VN];  // (1 + scale) w, gate pw, gate pb
+    {
+      float t[MAXV][VN];
+      if (H) {
+        params<T, VN, MAXV>(a.scale, b * a.lds, lane, G, nvec, 0.f, hf);
+        params<T, VN, MAXV>(a.w, 0, lane, G, nvec, 1.f, t);
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+          for (int e = 0; e < VN; ++e) hf[k][e] = (1.f + hf[k][e]) * t[k][e];
+      }
+      if (Y) {
+        params<T, VN, MAXV>(a.gate, b * a.ldg, lane, G, nvec, 1.f, gf);
+        params<T, VN, MAXV>(a.pw, 0, lane, G, nvec, 1.f, t);
+        params<T, VN, MAXV>(a.pb, 0, lane, G, nvec, 0.f, gs);
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+          for (int e = 0; e < VN; ++e) {
+            if (a.pb) gs[k][e] *= gf[k][e];
+            gf[k][e] *= t[k][e];
+          }
+      }
+    }
+    float P[MAXV][VN] = {}, Q[MAXV][VN] = {}, Py[MAXV][VN] = {}, Qy[MAXV][VN] = {};
+    const int64_t first = row0 + team.first;
+    for (int64_t lead = row0, row = first; lead < stop; lead += team.step, row += team.step) {
+      const bool live = row < stop;
+      Cols<T, VN, MAXV> xc, yc, dhc, drc;
+      float2 ys = make_float2(0.f, 1.f), rst = make_float2(0.f, 1.f);
+      if (live) {
+        if (H) xc.load((const T*)a.x + row * C, lane, G, nvec);
+        if (Y) yc.load((const T*)a.y + row * C, lane, G, nvec);
+        if (H) dhc.load((const T*)a.dh + row * C, lane, G, nvec);
+        if (a.dr) drc.load((const T*)a.dr + row * C, lane, G, nvec);
+        if (Y && a.post != TSC_NORM_NONE) ys = a.ystat[row];
+        if (H) rst = a.rstat[row];
+      }
+      float y[MAXV][VN], x[MAXV][VN], d[MAXV][VN], s2[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < MAXV; ++k) {
+        const bool in = live && lane + G * k < nvec;
+#pragma unroll
+        for (int e = 0; e < VN; ++e) {
+          y[k][e] = Y && in ? ((float)yc.v[k].v[e] - ys.x) * ys.y : 0.f;
+          d[k][e] = 0.f;
+          if (H) {
+            float r = in ? (float)xc.v[k].v[e] : 0.f;
+            if (Y) r = fmaf(a.rs, r, fmaf(gf[k][e], y[k][e], gs[k][e]));
+            x[k][e] = in ? (r - rst.x) * rst.y : 0.f;
+            const float dh = in ? (float)dhc.v[k].v[e] : 0.f;
+            P[k][e] = fmaf(dh, x[k][e], P[k][e]);
+            Q[k][e] += dh;
+            d[k][e] = dh * hf[k][e];
+            s2[0] += d[k][e];
+            s2[1] = fmaf(d[k][e], x[k][e], s2[1]);
+          }
+        }
+      }
+      if (H) {
+        team.sum(s2);
+        const float m1 = a.norm == TSC_NORM_LAYER ? s2[0] * a.inv_c : 0.f, m2 = s2[1] * a.inv_c;
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+          for (int e = 0; e < VN; ++e) d[k][e] = rst.y * (d[k][e] - fmaf(x[k][e], m2, m1));
+      }
+      if (a.dr) {
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+          for (int e = 0; e < VN; ++e)
+            if (live && lane + G * k < nvec) d[k][e] += (float)drc.v[k].v[e];
+      }
+      // d: the gradient of r
+      if (live) {
+        if (Y) {
+#pragma unroll
+          for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+            for (int e = 0; e < VN; ++e) x[k][e] = a.rs * d[k][e];
+          store_row<T, VN, MAXV>((T*)a.dx + row * C, lane, G, nvec, x);
+        } else {
+          store_row<T, VN, MAXV>((T*)a.dx + row * C, lane, G, nvec, d);
+        }
+      }
+      if (Y) {
+        float e2[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k)
+          if (live && lane + G * k < nvec)
+#pragma unroll
+            for (int e = 0; e < VN; ++e) {
+              Py[k][e] = fmaf(d[k][e], y[k][e], Py[k][e]);
+              Qy[k][e] += d[k][e];
+              d[k][e] *= gf[k][e];
+              e2[0] += d[k][e];
+              e2[1] = fmaf(d[k][e], y[k][e], e2[1]);
+            }
+        if (a.post != TSC_NORM_NONE) {
+          team.sum(e2);
+          const float m1 = a.post == TSC_NORM_LAYER ? e2[0] * a.inv_c : 0.f, m2 = e2[1] * a.inv_c;
+#pragma unroll
+          for (int k = 0; k < MAXV; ++k)
+#pragma unroll
+            for (int e = 0; e < VN; ++e) d[k][e] = ys.y * (d[k][e] - fmaf(y[k][e], m2, m1));
+        }
+        if (live) store_row<T, VN, MAXV>((T*)a.dy + row * C, lane, G, nvec, d);
+      }
+    }
+    if (a.sums) {
+      const int64_t slot = (int64_t)blockIdx.x + b;
+      int which = 0;
+      if (H) {
+        flush<VN, MAXV, BLOCK>(a, team, slot, which++, P);
+        flush<VN, MAXV, BLOCK>(a, team, slot, which++, Q);
+      }
+      if (Y) {
+        flush<VN, MAXV, BLOCK>(a, team, slot, which++, Py);
+        if (a.sums > which) flush<VN, MAXV, BLOCK>(a, team, slot, which, Qy);
+      }
+    }
+    row0 = stop;
+  }
+}
+
+struct SumArgs {
+  const float* part;
+  double* total;  // (B, 4, C): what the weights' gradients add up, where blocks have one sample each
+  const int32_t* cu;
+  int64_t N, each, R;
+  int32_t B, C, sums, h, y;  // h, y: whether those parts have sums
+  const void *w, *bias, *scale, *pw, *pb, *gate;
+  int64_t lds, ldg;
+  void *dscale, *dshift, *dgate, *dw, *dbias, *dpw, *dpb;
+};
+
+template <typename T>
+__device__ __forceinline__ float at_or(const void* p, int64_t i, float none) {
+  return p ? (float)((const T*)p)[i] : none;
+}
+template <typename T>
+__device__ __forceinline__ void put(void* p, int64_t i, double v) {
+  if (p) ((T*)p)[i] = (T)(float)v;
+}
+
+// Sums over a sample's slots, 16 columns by 64 slots at a time, merged in fp64.  Grid y = 1: all samples,
+// one after the other, and the weights' gradients; else one sample each, whose parts of those go to `total`.
+template <typename T>
+__global__ void __launch_bounds__(kSumCols* kSumRows) gated_norm_sums_kernel(const SumArgs a) {
+  __shared__ double meet[kSumRows][kSumCols];
+  const int tc = threadIdx.x % kSumCols, tr = threadIdx.x / kSumCols, c = blockIdx.x * kSumCols + tc;
+  const bool in = c < a.C, alone = gridDim.y == 1;
+  double weights[4] = {0., 0., 0., 0.};
+  for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
+    int64_t lo = b * a.each, hi = lo + a.each;
+    if (a.cu) {
+      lo = min<int64_t>(max<int64_t>(a.cu[b], 0), a.N);
+      hi = min<int64_t>(max<int64_t>(a.cu[b + 1], lo), a.N);
+    }
+    const int64_t t0 = lo / a.R, t1 = hi > lo ? (hi - 1) / a.R + 1 : t0;  // blocks of these rows
+    double s[4] = {0., 0., 0., 0.};
+    for (int i = 0; i < a.sums; ++i) {
+      double v = 0.;
+      if (in)
+        for (int64_t t = t0 + tr; t < t1; t += kSumRows) v += (double)a.part[((t + b) * a.sums + i) * a.C + c];
+      __syncthreads();
+      meet[tr][tc] = v;
+      __syncthreads();
+      for (int half = kSumRows / 2; half > 0; half >>= 1) {
+        if (tr < half) meet[tr][tc] += meet[tr + half][tc];
+        __syncthreads();
+      }
+      s[i] = meet[0][tc];
+    }
+    if (!in || tr) continue;
+    const int64_t at = (int64_t)b * a.C + c;
+    int i = 0;
+    double part[4] = {0., 0., 0., 0.};
+    if (a.h) {
+      const double P = s[0], Q = s[1], f = 1. + (double)at_or<T>(a.scale, b * a.lds + c, 0.f);
+      put<T>(a.dscale, at, (double)at_or<T>(a.w, c, 1.f) * P + (a.bias ? (double)at_or<T>(a.bias, c, 0.f) * Q : 0.));
+      put<T>(a.dshift, at, Q);
+      part[0] = f * P;
+      part[1] = f * Q;
+      i = 2;
+    }
+    if (a.y) {
+      const double P = s[i], Q = a.sums > i + 1 ? s[i + 1] : 0., g = at_or<T>(a.gate, b * a.ldg + c, 1.f);
+      put<T>(a.dgate, at, (double)at_or<T>(a.pw, c, 1.f) * P + (a.pb ? (double)at_or<T>(a.pb, c, 0.f) * Q : 0.));
+      part[2] = g * P;
+      part[3] = g * Q;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (alone) weights[j] += part[j];
+      else if (a.total) a.total[((int64_t)b * 4 + j) * a.C + c] = part[j];
+    }
+  }
+  if (alone && in && tr == 0) {
+    put<T>(a.dw, c, weights[0]);
+    put<T>(a.dbias, c, weights[1]);
+    put<T>(a.dpw, c, weights[2]);
+    put<T>(a.dpb, c, weights[3]);
+  }
+}
+
+// The weights' gradients of more than kLoopB samples.
+template <typename T>
+__global__ void __launch_bounds__(kSumCols* kSumRows) gated_norm_weights_kernel(const SumArgs a) {
+  __shared__ double meet[kSumRows][kSumCols];
+  const int tc = threadIdx.x % kSumCols, tr = threadIdx.x / kSumCols, c = blockIdx.x * kSumCols + tc;
+  void* out[4] = {a.dw, a.dbias, a.dpw, a.dpb};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (!out[j]) continue;  // uniform
+    double v = 0.;
+    if (c < a.C)
+      for (int b = tr; b < a.B; b += kSumRows) v += a.total[((int64_t)b * 4 + j) * a.C + c];
+    __syncthreads();
+    meet[tr][tc] = v;
+    __syncthreads();
+    for (int half = kSumRows / 2; half > 0; half >>= 1) {
+      if (tr < half) meet[tr][tc] += meet[tr + half][tc];
+      __syncthreads();
+    }
+    if (c < a.C && tr == 0) put<T>(out[j], c, meet[0][tc]);
+  }
+}
+
+// ------------------------------------------------------------------------------- host
+struct Shape {
+  bool block;
+  int G, threads, rows;  // lanes of a row, threads of a block, rows a step of it covers
+};
+Shape shape_of(int32_t C, int vn, int per_lane) {
+  const int nvec = C / vn;
+  if (C <= kWaveC) {
+    int g = 1;
+    while (g < 64 && g < nvec) g *= 2;
+    return {false, g, 256, 256 / g};
+  }
+  const int lanes = (nvec + per_lane / vn - 1) / (per_lane / vn);
+  const int threads = (lanes + 63) / 64 * 64;
+  return {true, threads, threads, 1};
+}
+// Rows of a block: as many blocks as `most` where there are enough rows.
+int64_t rows_of(const Shape& s, int64_t N, int64_t most) {
+  const int64_t steps = (N + s.rows - 1) / s.rows;
+  return s.rows * std::max<int64_t>(1, (steps + most - 1) / most);
+}
+constexpr int64_t kForwardBlocks = 2048, kBackwardBlocks = 1024;
+
+// A step's rows and with them the slots do not depend on the alignment: the scratch has room for both.
+int64_t slots_of(int32_t dtype, int32_t B, int64_t N, int32_t C) {
+  const int vn = dtype == TSC_F32 ? 4 : 8;
+  int64_t most = 0;
+  for (int v : {vn, 1}) {
+    if (C % v) continue;
+    const int64_t r = rows_of(shape_of(C, v, 8), N, kBackwardBlocks);
+    most = std::max(most, (N + r - 1) / r);
+  }
+  return most + B;
+}
+
+bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+GnArgs args_of(const GatedNormArgs& x) {
+  GnArgs a = {};
+  a.x = x.x;
+  a.y = x.y;
+  a.cu = x.cu;
+  a.N = x.N;
+  a.each = x.cu || x.B == 0 ? 0 : x.N / x.B;
+  a.B = x.B;
+  a.C = x.C;
+  a.post = x.post_norm;
+  a.norm = x.norm;
+  a.rest = x.rest;
+  a.pw = x.post_weight;
+  a.pb = x.post_bias;
+  a.w = x.weight;
+  a.bias = x.bias;
+  a.gate = x.gate;
+  a.scale = x.scale;
+  a.shift = x.shift;
+  a.ldg = x.ld_gate;
+  a.lds = x.ld_scale;
+  a.ldt = x.ld_shift;
+  a.rs = x.residual_scale;
+  a.eps = x.eps;
+  a.inv_c = 1.f / (float)x.C;
+  return a;
+}
+// Whether rows and parameters can be read 16 bytes at a time.
+bool whole_vectors(const GatedNormArgs& x, int vn, std::initializer_list<const void*> rows) {
+  if (x.C % vn) return false;
+  for (const void* p : rows)
+    if (!aligned16(p)) return false;
+  for (const void* p : {x.x, x.y, x.post_weight, x.post_bias, x.weight, x.bias, x.gate, x.scale, x.shift})
+    if (!aligned16(p)) return false;
+  return !((x.gate && x.ld_gate % vn) || (x.scale && x.ld_scale % vn) || (x.shift && x.ld_shift % vn));
+}
+
+// Calls f(type, VN, MAXV, BLOCK) with the kernel's shape: vectors of 16 bytes or single values; 16 (8) values
+// a lane of a wave (of a block).
+template <typename F>
+void by_shape(int32_t dtype, bool vec, bool block, F f) {
+  auto with = [&](auto t, auto vn) {
+    constexpr int VN = decltype(vn)::value;
+    if (block) f(t, vn, std::integral_constant<int, 8 / VN>(), std::true_type());
+    else f(t, vn, std::integral_constant<int, 16 / VN>(), std::false_type());
+  };
+  auto types = [&](auto t) {
+    if (vec) with(t, std::integral_constant<int, 16 / sizeof(decltype(t))>());
+    else with(t, std::integral_constant<int, 1>());
+  };
+  if (dtype == TSC_BF16) types(__bf16());
+  else if (dtype == TSC_F16) types(_Float16());
+  else types(float());
+}
+
+}  // namespace
+
+int32_t gated_norm_max_channels() { return kMaxC; }
+
+int gated_norm_launch(tsc_ctx* ctx, const GatedNormArgs& x, float* stats, void* r, void* h) {
+  GnArgs a = args_of(x);
+  a.r = r;
+  a.h = h;
+  if (stats) {
+    const bool post = x.y && x.post_norm != TSC_NORM_NONE;
+    a.ystat = post ? (float2*)stats : nullptr;
+    a.rstat = h ? (float2*)stats + (post ? x.N : 0) : nullptr;
+  }
+  const int vn = x.dtype == TSC_F32 ? 4 : 8;
+  const bool vec = whole_vectors(x, vn, {r, h});
+  const Shape s = shape_of(x.C, vec ? vn : 1, 8);
+  a.G = s.G;
+  a.R = rows_of(s, x.N, kForwardBlocks);
+  const unsigned grid = (unsigned)((x.N + a.R - 1) / a.R);
+  ProfScope p(ctx, "gated_norm");
+  by_shape(x.dtype, vec, s.block, [&](auto t, auto v, auto m, auto blk) {
+    using T = decltype(t);
+    constexpr int VN = decltype(v)::value, MAXV = decltype(m)::value;
+    constexpr bool BLOCK = decltype(blk)::value;
+    if (x.y && h) gated_norm_kernel<T, VN, MAXV, BLOCK, true, true><<<grid, s.threads, 0, ctx->stream>>>(a);
+    else if (x.y) gated_norm_kernel<T, VN, MAXV, BLOCK, true, false><<<grid, s.threads, 0, ctx->stream>>>(a);
+    else gated_norm_kernel<T, VN, MAXV, BLOCK, false, true><<<grid, s.threads, 0, ctx->stream>>>(a);
+  });
+  return check_hip(hipGetLastError(), "gated_norm launch");
+}
+
+int64_t gated_norm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C) {
+  if (B == 0) return 0;
+  const int64_t part = align_up((size_t)slots_of(dtype, B, N, C) * 4 * C * 4, 16);
+  return part + (B > kLoopB ? (int64_t)B * 4 * C * 8 : 0);
+}
+
+int gated_norm_backward_launch(tsc_ctx* ctx, const GatedNormArgs& x, const float* stats, const void* dr,
+                               const void* dh, void* ws, const GatedNormGrads& g) {
+  GnArgs a = args_of(x);
+  const bool post = x.y && x.post_norm != TSC_NORM_NONE;
+  a.ystat = (float2*)stats;
+  a.rstat = (float2*)stats + (post ? x.N : 0);
+  a.dr = dr;
+  a.dh = dh;
+  a.dx = g.dx;
+  a.dy = g.dy;
+  const bool want_h = dh && (g.dscale || g.dshift || g.dweight || g.dbias);
+  const bool want_y = x.y && (g.dgate || g.dpost_weight || g.dpost_bias);
+  // Either part's sums where any is wanted: the kernel makes them all the same.
+  a.sums = want_h || want_y ? (dh ? 2 : 0) + (x.y ? (x.post_bias ? 2 : 1) : 0) : 0;
+  a.part = (float*)ws;
+  const int vn = x.dtype == TSC_F32 ? 4 : 8;
+  const bool vec = whole_vectors(x, vn, {dr, dh, g.dx, g.dy});
+  const Shape s = shape_of(x.C, vec ? vn : 1, 8);
+  a.G = s.G;
+  a.R = rows_of(s, std::max<int64_t>(x.N, 1), kBackwardBlocks);
+  if (x.N > 0) {
+    const unsigned grid = (unsigned)((x.N + a.R - 1) / a.R);
+    ProfScope p(ctx, "gated_norm_backward");
+    by_shape(x.dtype, vec, s.block, [&](auto t, auto v, auto m, auto blk) {
+      using T = decltype(t);
+      constexpr int VN = decltype(v)::value, MAXV = decltype(m)::value;
+      constexpr bool BLOCK = decltype(blk)::value;
+      auto* st = ctx->stream;
+      if (x.y && dh) gated_norm_backward_kernel<T, VN, MAXV, BLOCK, true, true><<<grid, s.threads, 0, st>>>(a);
+      else if (x.y) gated_norm_backward_kernel<T, VN, MAXV, BLOCK, true, false><<<grid, s.threads, 0, st>>>(a);
+      else gated_norm_backward_kernel<T, VN, MAXV, BLOCK, false, true><<<grid, s.threads, 0, st>>>(a);
+    });
+  }
+  if (a.sums) {
+    SumArgs q = {};
+    q.part = a.part;
+    q.cu = a.cu;
+    q.N = a.N;
+    q.each = a.each;
+    q.R = a.R;
+    q.B = a.B;
+    q.C = a.C;
+    q.sums = a.sums;
+    q.h = dh != nullptr;
+    q.y = x.y != nullptr;
+    q.w = x.weight;
+    q.bias = x.bias;
+    q.scale = x.scale;
+    q.pw = x.post_weight;
+    q.pb = x.post_bias;
+    q.gate = x.gate;
+    q.lds = x.ld_scale;
+    q.ldg = x.ld_gate;
+    q.dscale = g.dscale;
+    q.dshift = g.dshift;
+    q.dgate = g.dgate;
+    q.dw = g.dweight;
+    q.dbias = g.dbias;
+    q.dpw = g.dpost_weight;
+    q.dpb = g.dpost_bias;
+    const bool weights = g.dweight || g.dbias || g.dpost_weight || g.dpost_bias;
+    const bool loop = x.B <= kLoopB;
+    if (!loop && weights)
+      q.total = (double*)((char*)ws + align_up((size_t)slots_of(x.dtype, x.B, x.N, x.C) * 4 * x.C * 4, 16));
+    const unsigned gx = (unsigned)((x.C + kSumCols - 1) / kSumCols);
+    const dim3 grid(gx, loop ? 1u : (unsigned)std::min(x.B, 65535));
+    auto run = [&](auto t) {
+      using T = decltype(t);
+      {
+        ProfScope p(ctx, "gated_norm_sums");
+        gated_norm_sums_kernel<T><<<grid, kSumCols * kSumRows, 0, ctx->stream>>>(q);
+      }
+      if (!loop && weights) {
+        ProfScope p(ctx, "gated_norm_weights");
+        gated_norm_weights_kernel<T><<<gx, kSumCols * kSumRows, 0, ctx->stream>>>(q);
+      }
+    };
+    if (x.dtype == TSC_BF16) run(__bf16());
+    else if (x.dtype == TSC_F16) run(_Float16());
+    else run(float());
+  }
+  return check_hip(hipGetLastError(), "gated_norm_backward launch");
+}
+
+}  // namespace tsc

@@ -264,6 +264,34 @@ int groupnorm_backward_launch(tsc_ctx* ctx, int32_t dtype, const void* dy, const
                               const void* gamma, const void* beta, int32_t silu, int32_t rest,
                               const float* stats, void* ws, void* dx, void* dgamma, void* dbeta);
 
+// ---- implemented in gated_norm.hip ----
+struct GatedNormArgs {
+  int32_t dtype;
+  const void *x, *y;  // y null: r = x
+  const int32_t* cu;  // null: B samples of N / B rows
+  int32_t B;
+  int64_t N;
+  int32_t C, post_norm;
+  const void *post_weight, *post_bias, *gate;
+  int64_t ld_gate;  // row strides of gate, scale and shift in elements
+  float residual_scale;
+  int32_t norm;
+  const void *weight, *bias, *scale;
+  int64_t ld_scale;
+  const void* shift;
+  int64_t ld_shift;
+  float eps;
+  int32_t rest;
+};
+struct GatedNormGrads {
+  void *dx, *dy, *dgate, *dpost_weight, *dpost_bias, *dscale, *dshift, *dweight, *dbias;
+};
+int32_t gated_norm_max_channels();
+int gated_norm_launch(tsc_ctx* ctx, const GatedNormArgs& x, float* stats, void* r, void* h);
+int64_t gated_norm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C);
+int gated_norm_backward_launch(tsc_ctx* ctx, const GatedNormArgs& x, const float* stats, const void* dr,
+                               const void* dh, void* ws, const GatedNormGrads& g);
+
 // ---- launchers implemented in rowops.hip ----
 int layernorm_launch(tsc_ctx* ctx, int32_t dtype, const void* x, int64_t N, int32_t C,
                      const void* gamma, const void* beta, float eps, int32_t apply_silu, void* y);

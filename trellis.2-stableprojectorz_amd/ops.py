@@ -360,6 +360,178 @@ def _group_norm_backward(dy, x, weight, bias, cu, b, groups, silu, stats, want_p
     return dx, dw, db
 
 
+def _modulation(t, name: str, b: int, c: int, dtype):
+    """A (B, C) tensor whose rows may be strided: a gate, a scale or a shift of each sample."""
+    if t is not None and (t.shape != (b, c) or t.dtype != dtype):
+        raise TscError(_lib.TSC_ERR_INVALID, f"{name} must be ({b}, {c}) of x's dtype, got {tuple(t.shape)} {t.dtype}")
+    if t is not None and (t.stride(1) != 1 and c > 1 or t.stride(0) < c and b > 1):
+        raise TscError(_lib.TSC_ERR_INVALID, f"{name}: each sample's {c} values must be contiguous")
+
+
+def _gated_norm_args(what: str, x, y, cu_rows, post, gate, residual_scale, pre, scale, shift, eps, outs):
+    """Checks what the norms around a block are given; (tensors, arguments) of _gated_norm.  post and pre:
+    (kind, weight, bias), kind None where there is none."""
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise TscError(_lib.TSC_ERR_INVALID, f"{what}: x must be (N, C)")
+    n, c = x.shape
+    if y is not None and (y.shape != x.shape or y.dtype != x.dtype):
+        raise TscError(_lib.TSC_ERR_INVALID, f"{what}: y must have x's shape and dtype")
+    for name, (kind, w, b) in (("post_norm", post), ("norm", pre)):
+        if kind not in _lib.NORMS:
+            raise TscError(_lib.TSC_ERR_INVALID, f"{what}: {name} must be 'layer' or 'rms', got {kind!r}")
+        if kind is None and (w is not None or b is not None):
+            raise TscError(_lib.TSC_ERR_INVALID, f"{what}: a weight or bias needs a {name}")
+        for t in (w, b):
+            if t is not None and (t.shape != (c,) or t.dtype != x.dtype):
+                raise TscError(_lib.TSC_ERR_INVALID, f"{what}: weights and biases must be ({c},) of x's dtype")
+    for out in outs:
+        if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
+            raise TscError(_lib.TSC_ERR_INVALID, f"{what}: out has the wrong shape or dtype")
+    _code(x)
+    eps, residual_scale = float(eps), float(residual_scale)
+    if not 0 <= ctypes.c_float(eps).value < float("inf"):
+        raise TscError(_lib.TSC_ERR_INVALID, f"{what}: eps must be >= 0 and finite")
+    if not abs(ctypes.c_float(residual_scale).value) < float("inf"):
+        raise TscError(_lib.TSC_ERR_INVALID, f"{what}: residual_scale must be finite in fp32")
+    tensors = (x, y, post[1], post[2], gate, pre[1], pre[2], scale, shift)
+    _no_tangents(what, *tensors, *outs)
+    if isinstance(cu_rows, torch.Tensor):
+        b = cu_rows.numel() - 1
+    else:
+        b = 1 if cu_rows is None else len(cu_rows) - 1
+    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+        _modulation(t, f"{what}: {name}", b, c, x.dtype)
+    dev = _dev(x, y, *post[1:], *pre[1:], *outs)
+    for t in (gate, scale, shift):
+        if t is not None and (not t.is_cuda or t.device.index != dev):
+            raise TscError(_lib.TSC_ERR_INVALID, "tensors are not on one GPU; this path has no CPU fallback")
+    cu = None
+    if cu_rows is not None:
+        _, cu = _cu_seqlens(cu_rows, n, dev, "cu_rows")
+        _dev(x, cu)
+    if b and c > 8192:
+        raise TscError(_lib.TSC_ERR_UNSUPPORTED, f"{what}: C={c} exceeds 8192")
+    return tensors, (cu, b, _lib.NORMS[post[0]], _lib.NORMS[pre[0]], residual_scale, eps)
+
+
+def modulated_norm(x: torch.Tensor, cu_rows=None, scale=None, shift=None, norm: str = "layer",
+                   weight=None, bias=None, eps: float = 1e-6, out=None) -> torch.Tensor:
+    """The norm before a transformer block, modulated per sample (tsc_gated_norm):
+
+        h = (norm(x) * weight + bias) * (1 + scale[b]) + shift[b]
+
+    x (N, C), C up to 8192; cu_rows (B+1,) gives the samples' row offsets (as in group_norm; without it
+    all rows are one sample).  scale, shift (B, C) may be strided rows, mod[:, i] of a (B, 6, C) tensor.
+    norm "layer" or "rms" over each row; weight, bias (C,).  All in x's dtype.  out may be x.  Rows
+    outside every sample are zero in a new result and left as they were in `out`.
+    Differentiable in all tensors (then without `out`; a graph through the gradient itself is not
+    supported)."""
+    if norm is None:
+        raise TscError(_lib.TSC_ERR_INVALID, "modulated_norm: norm must be 'layer' or 'rms', got None")
+    tensors, args = _gated_norm_args("modulated_norm", x, None, cu_rows, (None, None, None), None, 1.0,
+                                     (norm, weight, bias), scale, shift, eps, (out,))
+    return _gated_norm_entry("modulated_norm", tensors, args, False, True, out)[1]
+
+
+def gated_residual(x: torch.Tensor, y: torch.Tensor, cu_rows=None, gate=None, residual_scale: float = 1.0,
+                   post_norm: str | None = None, post_weight=None, post_bias=None, eps: float = 1e-6,
+                   out=None) -> torch.Tensor:
+    """A block's output y added to the residual stream x (tsc_gated_norm):
+
+        r = residual_scale * x + gate[b] * (norm(y) * post_weight + post_bias)
+
+    x, y (N, C); gate (B, C) of the samples that cu_rows gives, rows may be strided; post_norm None (y as
+    it is), "layer" or "rms".  Otherwise as modulated_norm; out may be x or y."""
+    tensors, args = _gated_norm_args("gated_residual", x, y, cu_rows, (post_norm, post_weight, post_bias),
+                                     gate, residual_scale, (None, None, None), None, None, eps, (out,))
+    return _gated_norm_entry("gated_residual", tensors, args, True, False, out)[0]
+
+
+def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, cu_rows=None, gate=None,
+                        residual_scale: float = 1.0, post_norm: str | None = None, post_weight=None,
+                        post_bias=None, norm: str = "layer", weight=None, bias=None, scale=None,
+                        shift=None, eps: float = 1e-6):
+    """(r, h): gated_residual, and modulated_norm of its result (not rounded in between), in one pass
+    over the rows.  Arguments as theirs."""
+    if norm is None:
+        raise TscError(_lib.TSC_ERR_INVALID, "gated_residual_norm: norm must be 'layer' or 'rms', got None")
+    tensors, args = _gated_norm_args("gated_residual_norm", x, y, cu_rows,
+                                     (post_norm, post_weight, post_bias), gate, residual_scale,
+                                     (norm, weight, bias), scale, shift, eps, ())
+    return _gated_norm_entry("gated_residual_norm", tensors, args, True, True, None)
+
+
+def _gated_norm_entry(what, tensors, args, want_r, want_h, out):
+    if _wants_grad(*tensors, out):
+        if out is not None:
+            raise TscError(_lib.TSC_ERR_INVALID, f"{what}: out cannot be given where gradients are wanted")
+        from .autograd import GatedNorm
+
+        got = GatedNorm.apply(*tensors, args, want_r, want_h)
+        return got if want_r and want_h else (got, got)
+    return _gated_norm(tensors, args, want_r, want_h, out, False)[:2]
+
+
+def _gated_norm_call(tensors, args):
+    """The arguments that both C calls share."""
+    x, y, pw, pb, gate, w, bias, scale, shift = tensors
+    cu, b, post, pre, residual_scale, eps = args
+    n, c = x.shape
+
+    def rows(t):
+        return _p(t), 0 if t is None else t.stride(0) if b > 1 else c
+
+    return (_code(x), _p(x), _p(y), _p(cu), b, n, c, post, _p(pw), _p(pb), *rows(gate), residual_scale,
+            pre, _p(w), _p(bias), *rows(scale), *rows(shift), eps)
+
+
+def _gated_norm(tensors, args, want_r, want_h, out, keep):
+    """(r, h, stats); stats (None unless keep) is what the backward pass needs."""
+    x, y = tensors[:2]
+    n, b, post = x.shape[0], args[1], args[2]
+    new = torch.empty_like if b else torch.zeros_like
+    r = (out if out is not None else new(x)) if want_r else None
+    h = (out if out is not None and not want_r else new(x)) if want_h else None
+    norms = int(want_h) + int(y is not None and post != _lib.TSC_NORM_NONE)
+    stats = torch.empty((norms, n, 2), dtype=torch.float32, device=x.device) if keep else None
+    if n and b:
+        lib, handle = _lib.stream_handle(x.device.index)
+        check(lib.tsc_gated_norm(handle, *_gated_norm_call(tensors, args), int(out is None),
+                                 _p(stats) if norms else None, _p(r), _p(h)))
+        _wrote(out)
+    return r, h, stats
+
+
+def _gated_norm_backward(tensors, args, stats, dr, dh, wanted):
+    """The gradients of `tensors` (None where `wanted` says so)."""
+    x, y, pw, pb, gate, w, bias, scale, shift = tensors
+    b = args[1]
+    n, c = x.shape
+    if n == 0:
+        return [None if t is None else torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
+    dx = torch.empty_like(x)
+    dy = None if y is None else torch.empty_like(x)
+    there = (True, y is not None) + 3 * (y is not None,) + 4 * (dh is not None,)
+
+    def new(i, *shape):
+        t = tensors[i]
+        return torch.empty(shape, dtype=x.dtype, device=x.device) if t is not None and wanted[i] and there[i] else None
+
+    dpw, dpb, dgate, dw, db, dscale, dshift = (new(2, c), new(3, c), new(4, b, c), new(5, c), new(6, c),
+                                               new(7, b, c), new(8, b, c))
+    lib, handle = _lib.stream_handle(x.device.index)
+    nbytes = lib.tsc_gated_norm_workspace_bytes(_code(x), b, n, c)
+    ws = _scratch(nbytes, x.device)
+    check(lib.tsc_gated_norm_backward(handle, *_gated_norm_call(tensors, args), 1, _p(stats), _p(dr),
+                                      _p(dh), _p(ws), _p(dx), _p(dy), _p(dgate), _p(dpw), _p(dpb),
+                                      _p(dscale), _p(dshift), _p(dw), _p(db)))
+    grads = [dx, dy, dpw, dpb, dgate, dw, db, dscale, dshift]
+    for i, t in enumerate(tensors):  # of a part whose output has no gradient
+        if t is not None and wanted[i] and grads[i] is None:
+            grads[i] = torch.zeros(t.shape, dtype=t.dtype, device=t.device)
+    return grads
+
+
 def silu(x: torch.Tensor, out=None) -> torch.Tensor:
     dev = _dev(x, out)
     given = out
