@@ -411,6 +411,53 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
                                 const float* maps, const float* lse, const void* dout,
                                 void* workspace, void* dq, void* dk, void* dv, float* dlambda);
 
+/* ---- window attention ---------------------------------------------------------------------- */
+/* Attention in a sliding window along packed sequences, with a few first tokens that stay visible.
+ * Query i of a sequence of n queries and m keys stands at position p = i + m - n (the queries are the
+ * last of the keys' rows), and sees key j where
+ *   (j < sinks or |p - j| <= window) and (not causal or j <= p)
+ *   out[i,h,:] = softmax_j(q[i,h,:] . k[j,g,:] * scale) v[j,g,:] over those, g = h / (num_heads / num_kv_heads)
+ * A query that sees no key gives zeros.
+ *   q, out (total_q, num_heads, head_dim), k, v (total_kv, num_kv_heads, head_dim): `dtype`; head_dim 64 or
+ *     128, num_kv_heads divides num_heads
+ *   ld_q, ld_k, ld_v  row strides in elements, the row's values to 2^24, rows 16-byte aligned; all other
+ *     buffers are contiguous
+ *   cu_seqlens_q / cu_seqlens_kv, scale, max_seqlen_q, max_seqlen_kv, zero_rest  as in tsc_diff_attention,
+ *     scale <= 0 meaning 1/sqrt(head_dim)
+ *   window, sinks  at least 0 (INT32_MAX: no bound)
+ *   out_lo, lse  both NULL, or for the backward pass: lse fp32 (total_q, num_heads) takes the rows'
+ *     log2-sum-exps, out_lo (as out; NULL for TSC_F32) what out's rounding left
+ *   workspace  device scratch of tsc_window_attention_workspace_bytes(..., backward = 0) bytes, 16-byte
+ *     aligned, NULL if that is 0.  The context keeps nothing.
+ * fp32 softmax and accumulation; P is rounded to `dtype` for its product with v.  Infinities and NaN stay
+ * with the queries that see them.
+ * No counterpart in the reference, whose attention is over whole samples (src/sparse/ops/attention.ts:24-79). */
+int64_t tsc_window_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv,
+                                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                             int32_t window, int32_t sinks, int32_t causal,
+                                             int32_t max_seqlen_q, int32_t max_seqlen_kv,
+                                             int32_t backward);
+int tsc_window_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, const void* v,
+                         int64_t ld_q, int64_t ld_k, int64_t ld_v, const int32_t* cu_seqlens_q,
+                         const int32_t* cu_seqlens_kv, int32_t B, int64_t total_q, int64_t total_kv,
+                         int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+                         int32_t window, int32_t sinks, int32_t causal, int32_t max_seqlen_q,
+                         int32_t max_seqlen_kv, int32_t zero_rest, void* workspace, void* out,
+                         void* out_lo, float* lse);
+/* Its gradient from dout (as out) and what the forward call was given and wrote: dq (total_q, ...), dk and
+ * dv (total_kv, num_kv_heads, head_dim; summed over the heads that share a key head) `dtype`.  workspace
+ * with backward = 1.  The gradients must not overlap an input or each other.  zero_rest is about rows of
+ * dq, dk and dv.  The sums have one fixed order. */
+int tsc_window_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k,
+                                  const void* v, int64_t ld_q, int64_t ld_k, int64_t ld_v,
+                                  const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv, int32_t B,
+                                  int64_t total_q, int64_t total_kv, int32_t num_heads,
+                                  int32_t num_kv_heads, int32_t head_dim, float scale, int32_t window,
+                                  int32_t sinks, int32_t causal, int32_t max_seqlen_q,
+                                  int32_t max_seqlen_kv, int32_t zero_rest, const void* out,
+                                  const void* out_lo, const float* lse, const void* dout,
+                                  void* workspace, void* dq, void* dk, void* dv);
+
 /* ---- safetensors weight files -------------------------------------------------------------- */
 /* Element types of a safetensors header ("dtype" strings).  F32/F16/BF16 equal TSC_F32/F16/BF16. */
 enum tsc_st_dtype {

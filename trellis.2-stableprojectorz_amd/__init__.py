@@ -16,6 +16,8 @@ is not a Python identifier.
   gated_residual_norm                            modulation, gate and residual scale, with gradients
   sparse_diff_attention,                         difference of two softmax maps, with gradients, and
   SparseDiffAttentionBlock3d                     the block around it
+  sparse_window_attention                        sliding window and first tokens that stay visible, shared
+                                                 key heads, with gradients
   SafetensorsFile, MultiFileLoader               weight files -> device tensors (weights.ts:58-237)
   workloads                                      seeded synthetic voxel shells
 """
@@ -26,7 +28,7 @@ from .ops import (NeighborMap, build_neighbor_map, map_conv_order, map_gather_pl
                   sparse_conv3d,
                   layer_norm, group_norm, modulated_norm, gated_residual, gated_residual_norm, silu, add,
                   sparse_resblock, sparse_subdivide, subdivide_count,
-                  sparse_linear, sparse_attention, sparse_diff_attention,
+                  sparse_linear, sparse_attention, sparse_diff_attention, sparse_window_attention,
                   scaled_dot_product_attention)
 from .spatial import SparseSubdivide  # noqa: F401
 from .blocks import SparseLinear, SparseGroupNorm, SparseDiffAttentionBlock3d, SparseConvNeXtBlock3d  # noqa: F401
@@ -39,6 +41,6 @@ __all__ = [
     "modulated_norm", "gated_residual", "gated_residual_norm", "silu", "add", "sparse_resblock",
     "sparse_subdivide", "subdivide_count", "SparseSubdivide", "sparse_linear", "SparseLinear", "SparseGroupNorm",
     "SparseConvNeXtBlock3d", "SparseDiffAttentionBlock3d", "sparse_attention",
-    "sparse_diff_attention", "scaled_dot_product_attention", "SafetensorsFile", "SafetensorsHeader", "TensorEntry", "MultiFileLoader",
+    "sparse_diff_attention", "sparse_window_attention", "scaled_dot_product_attention", "SafetensorsFile", "SafetensorsHeader", "TensorEntry", "MultiFileLoader",
     "get_neighbor_map", "neighbor_cache_key", "workloads",
 ]

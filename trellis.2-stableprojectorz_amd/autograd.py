@@ -72,3 +72,21 @@ class DiffAttention(torch.autograd.Function):
         grads = ops._diff_attention_backward(do, q, k, v, lam, maps, lse, cq, ck,
                                              *ctx.args)
         return (*grads, None, None, None, None, None, None)
+
+
+class WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, args):
+        out, lo, lse = ops._window_attention(q, k, v, args, None, True)
+        ctx.save_for_backward(q, k, v, out, lo, lse, *args[:2])
+        ctx.args = args[2:]
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, out, lo, lse, cq, ck = ctx.saved_tensors
+        do = do.contiguous()
+        if do.data_ptr() % 16:  # a view into a larger gradient
+            do = do.clone()
+        return (*ops._window_attention_backward(do, q, k, v, out, lo, lse, (cq, ck, *ctx.args)), None)

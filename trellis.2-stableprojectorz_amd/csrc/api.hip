@@ -1045,6 +1045,141 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
   return diff_attention_backward_launch(ctx, x, maps, lse, dout, workspace, dq, dk, dv, dlambda);
 }
 
+static int window_attention_sizes(const char* what, const WindowAttnSizes& z) {
+  if (!elem_size(z.dtype)) return fail(TSC_ERR_INVALID, "%s: unknown dtype %d", what, z.dtype);
+  if (z.D != 64 && z.D != 128)
+    return fail(TSC_ERR_UNSUPPORTED, "%s: head_dim %d (64 and 128 are supported)", what, z.D);
+  if (z.B < 0 || z.B > 65535 || z.H <= 0 || z.H > 65535 || z.Hk <= 0 || z.H % z.Hk || z.total_q < 0 ||
+      z.total_kv < 0 || z.max_q < 0 || z.max_kv < 0 || z.total_q > INT32_MAX || z.total_kv > INT32_MAX)
+    return fail(TSC_ERR_INVALID, "%s: bad sizes B=%d H=%d/%d total_q=%lld total_kv=%lld", what, z.B, z.H, z.Hk,
+                (long long)z.total_q, (long long)z.total_kv);
+  if (z.window < 0 || z.sinks < 0)
+    return fail(TSC_ERR_INVALID, "%s: window %d and sinks %d must not be negative", what, z.window, z.sinks);
+  return TSC_OK;
+}
+
+// Bytes that rows of `heads` heads and stride ld reach over.
+static size_t head_span(const WindowAttnSizes& z, int64_t rows, int64_t ld, int32_t heads) {
+  return rows > 0 ? ((size_t)(rows - 1) * ld + (size_t)heads * z.D) * elem_size(z.dtype) : 0;
+}
+
+static int window_attention_args(const char* what, const WindowAttnArgs& x) {
+  const WindowAttnSizes& z = x.z;
+  int st = window_attention_sizes(what, z);
+  if (st || z.B == 0) return st;
+  if (!x.cu_q || !x.cu_kv || (z.total_q > 0 && !x.q) || (z.total_kv > 0 && (!x.k || !x.v)))
+    return fail(TSC_ERR_INVALID, "%s: null buffer", what);
+  const int64_t lds[3] = {x.ldq, x.ldk, x.ldv};
+  const void* bufs[3] = {x.q, x.k, x.v};
+  for (int i = 0; i < 3; ++i) {
+    const int64_t row = (int64_t)(i ? z.Hk : z.H) * z.D;
+    if (lds[i] < row || lds[i] > (1 << 24) || lds[i] * elem_size(z.dtype) % 16)
+      return fail(TSC_ERR_INVALID, "%s: row stride %lld of q, k or v (%lld to 2^24, whole 16 bytes)", what,
+                  (long long)lds[i], (long long)row);
+    if (!aligned(bufs[i], 16)) return fail(TSC_ERR_INVALID, "%s: q, k and v must be 16-byte aligned", what);
+  }
+  if (!aligned(x.cu_q, 4) || !aligned(x.cu_kv, 4))
+    return fail(TSC_ERR_INVALID, "%s: cu_seqlens must be 4-byte aligned", what);
+  return TSC_OK;
+}
+
+int64_t tsc_window_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv,
+                                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                             int32_t window, int32_t sinks, int32_t causal,
+                                             int32_t max_seqlen_q, int32_t max_seqlen_kv,
+                                             int32_t backward) {
+  g_err[0] = 0;
+  const WindowAttnSizes z{dtype, B, total_q, total_kv, num_heads, num_kv_heads, head_dim, window, sinks, causal != 0,
+                          max_seqlen_q, max_seqlen_kv};
+  if (window_attention_sizes("window_attention_workspace_bytes", z)) return -1;
+  return window_attention_workspace_bytes(z, backward);
+}
+
+int tsc_window_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, const void* v,
+                         int64_t ld_q, int64_t ld_k, int64_t ld_v, const int32_t* cu_seqlens_q,
+                         const int32_t* cu_seqlens_kv, int32_t B, int64_t total_q, int64_t total_kv,
+                         int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+                         int32_t window, int32_t sinks, int32_t causal, int32_t max_seqlen_q,
+                         int32_t max_seqlen_kv, int32_t zero_rest, void* workspace, void* out,
+                         void* out_lo, float* lse) {
+  g_err[0] = 0;
+  int st = check_ctx(ctx);
+  if (st) return st;
+  const WindowAttnArgs x{{dtype, B, total_q, total_kv, num_heads, num_kv_heads, head_dim, window, sinks, causal != 0,
+                          max_seqlen_q, max_seqlen_kv},
+                         q, k, v, ld_q, ld_k, ld_v, cu_seqlens_q, cu_seqlens_kv,
+                         scale > 0.f ? scale : 1.f / sqrtf((float)head_dim), zero_rest};
+  st = window_attention_args("window_attention", x);
+  if (st) return st;
+  if (total_q == 0 || (B == 0 && !zero_rest)) return TSC_OK;
+  if (!out) return fail(TSC_ERR_INVALID, "window_attention: null buffer");
+  if (dtype == TSC_F32 ? out_lo != nullptr : (out_lo == nullptr) != (lse == nullptr))
+    return fail(TSC_ERR_INVALID, "window_attention: out_lo goes with lse, and not with fp32");
+  if (window_attention_workspace_bytes(x.z, 0) > 0 && !workspace)
+    return fail(TSC_ERR_INVALID, "window_attention: null workspace");
+  if (!aligned(out, 16) || !aligned(out_lo, 16) || !aligned(lse, 4) || !aligned(workspace, 16))
+    return fail(TSC_ERR_INVALID, "window_attention: out, out_lo and workspace must be 16-byte aligned");
+  const size_t no = head_span(x.z, total_q, (int64_t)num_heads * head_dim, num_heads);
+  for (const void* o : {(const void*)out, (const void*)out_lo})
+    if (o && (overlaps(o, no, q, head_span(x.z, total_q, ld_q, num_heads)) ||
+              overlaps(o, no, k, head_span(x.z, total_kv, ld_k, num_kv_heads)) ||
+              overlaps(o, no, v, head_span(x.z, total_kv, ld_v, num_kv_heads))))
+      return fail(TSC_ERR_INVALID, "window_attention: out overlaps an input");
+  if (out_lo && overlaps(out, no, out_lo, no))
+    return fail(TSC_ERR_INVALID, "window_attention: out overlaps out_lo");
+  DeviceGuard g(ctx->device);
+  if (B == 0) return zero_launch(ctx, out, (int64_t)no);  // every row is outside
+  return window_attention_launch(ctx, x, out, out_lo, lse, workspace);
+}
+
+int tsc_window_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k,
+                                  const void* v, int64_t ld_q, int64_t ld_k, int64_t ld_v,
+                                  const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_kv, int32_t B,
+                                  int64_t total_q, int64_t total_kv, int32_t num_heads,
+                                  int32_t num_kv_heads, int32_t head_dim, float scale, int32_t window,
+                                  int32_t sinks, int32_t causal, int32_t max_seqlen_q,
+                                  int32_t max_seqlen_kv, int32_t zero_rest, const void* out,
+                                  const void* out_lo, const float* lse, const void* dout,
+                                  void* workspace, void* dq, void* dk, void* dv) {
+  g_err[0] = 0;
+  int st = check_ctx(ctx);
+  if (st) return st;
+  const WindowAttnArgs x{{dtype, B, total_q, total_kv, num_heads, num_kv_heads, head_dim, window, sinks, causal != 0,
+                          max_seqlen_q, max_seqlen_kv},
+                         q, k, v, ld_q, ld_k, ld_v, cu_seqlens_q, cu_seqlens_kv,
+                         scale > 0.f ? scale : 1.f / sqrtf((float)head_dim), zero_rest};
+  st = window_attention_args("window_attention_backward", x);
+  if (st) return st;
+  if ((total_q > 0 && (!dq || (B > 0 && (!out || !lse || !dout || !workspace || (dtype != TSC_F32 && !out_lo))))) ||
+      (total_kv > 0 && (!dk || !dv)))
+    return fail(TSC_ERR_INVALID, "window_attention_backward: null buffer");
+  for (const void* p : {out, out_lo, dout, (const void*)workspace, (const void*)dq, (const void*)dk, (const void*)dv})
+    if (!aligned(p, 16)) return fail(TSC_ERR_INVALID, "window_attention_backward: buffers must be 16-byte aligned");
+  if (!aligned(lse, 4)) return fail(TSC_ERR_INVALID, "window_attention_backward: lse must be 4-byte aligned");
+  const size_t no = head_span(x.z, total_q, (int64_t)num_heads * head_dim, num_heads);
+  const size_t nk = head_span(x.z, total_kv, (int64_t)num_kv_heads * head_dim, num_kv_heads);
+  const void* ins[7] = {q, k, v, out, out_lo, dout, lse};
+  const size_t in_bytes[7] = {head_span(x.z, total_q, ld_q, num_heads), head_span(x.z, total_kv, ld_k, num_kv_heads),
+                              head_span(x.z, total_kv, ld_v, num_kv_heads), no, out_lo ? no : 0, no,
+                              (size_t)total_q * num_heads * 4};
+  const void* gs[3] = {dq, dk, dv};
+  const size_t g_bytes[3] = {no, nk, nk};
+  for (int i = 0; i < 3; ++i) {
+    for (int j = 0; j < 7; ++j)
+      if (overlaps(gs[i], g_bytes[i], ins[j], in_bytes[j]))
+        return fail(TSC_ERR_INVALID, "window_attention_backward: a gradient overlaps an input");
+    for (int j = 0; j < i; ++j)
+      if (overlaps(gs[i], g_bytes[i], gs[j], g_bytes[j]))
+        return fail(TSC_ERR_INVALID, "window_attention_backward: the gradients overlap");
+  }
+  DeviceGuard g(ctx->device);
+  if (B == 0) {  // every row is outside
+    for (int i = 0; i < 3 && zero_rest && !st; ++i) st = zero_launch(ctx, (void*)gs[i], (int64_t)g_bytes[i]);
+    return st;
+  }
+  return window_attention_backward_launch(ctx, x, out, out_lo, lse, dout, workspace, dq, dk, dv);
+}
+
 int tsc_st_open(const char* path, tsc_st** out) {
   g_err[0] = 0;
   if (!path || !out) return fail(TSC_ERR_INVALID, "st_open: null argument");

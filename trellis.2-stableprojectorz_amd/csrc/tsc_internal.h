@@ -253,6 +253,29 @@ int diff_attention_backward_launch(tsc_ctx* ctx, const DiffAttnArgs& x, const fl
                                    const float* lse, const void* dout, void* ws, void* dq, void* dk,
                                    void* dv, float* dlambda);
 
+// ---- implemented in window_attention.hip ----
+struct WindowAttnSizes {
+  int32_t dtype, B;
+  int64_t total_q, total_kv;
+  int32_t H, Hk, D;  // query heads, key heads
+  int32_t window, sinks, causal;
+  int32_t max_q, max_kv;  // longest sequences: they size the grids
+};
+struct WindowAttnArgs {
+  WindowAttnSizes z;
+  const void *q, *k, *v;
+  int64_t ldq, ldk, ldv;  // row strides in elements
+  const int32_t *cu_q, *cu_kv;
+  float scale;
+  int32_t rest;
+};
+int64_t window_attention_workspace_bytes(const WindowAttnSizes& z, int32_t backward);
+int window_attention_launch(tsc_ctx* ctx, const WindowAttnArgs& x, void* out, void* out_lo, float* lse,
+                            void* ws);
+int window_attention_backward_launch(tsc_ctx* ctx, const WindowAttnArgs& x, const void* out,
+                                     const void* out_lo, const float* lse, const void* dout, void* ws,
+                                     void* dq, void* dk, void* dv);
+
 // ---- implemented in groupnorm.hip ----
 int64_t groupnorm_workspace_bytes(int32_t dtype, int32_t B, int64_t N, int32_t C, int32_t groups,
                                   int32_t backward);

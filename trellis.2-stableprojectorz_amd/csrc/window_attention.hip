@@ -1,0 +1,943 @@
+// Attention in a sliding window along packed sequences, with a few first tokens that stay visible, and
+// its gradient.
+//
+//   A sequence has n queries and m keys; query i stands at position p = i + m - n among the keys.
+//   It sees key j where (j < sinks or |p - j| <= window) and (not causal or j <= p).
+//   out = softmax(q k^T scale over the keys it sees) v; zeros where it sees none
+// Gradient, with do = d out, dP = do v^T, r = do . out per query:
+//   dv = P^T do;  dS = P (dP - r);  dq = scale dS k;  dk = scale dS^T q
+//
+// G = H / Hk query heads share a key head.  A block's rows are the (query, head of the group) pairs of one
+// key head, row x = query x / G, head x % G: so a key head is read once for its G heads, a single token
+// fills G rows of a tile, and a tile of 128 rows spans 128 / G positions only.
+// The keys of a block's rows are two runs, the sinks and the window of the first to that of the last row
+// (one run where they meet); tiles that all rows see take no mask.
+// In the others a row and a key that do not see each other have P = 0, and dS = 0, by selection.  Their
+// product with a row of v (k; do, q in dk / dv) that holds an infinity or NaN would be NaN still: tiles with
+// masks look for those, take them as zeros, and add what they bring one row at a time with a selection
+// behind the product, so that who does not see them has the bits it would have without them.
+
+#include <float.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attention_tiles.h"
+#include "tsc_internal.h"
+
+namespace tsc {
+namespace {
+
+constexpr int kNT = 256;  // 4 waves of 32 rows (or keys, in dk / dv)
+constexpr int kBQ = 128;
+constexpr int kBK = 32;   // keys of a tile
+
+struct WaArgs {
+  const void *q, *k, *v;
+  int64_t ldq, ldk, ldv;
+  const int32_t *cu_q, *cu_kv;
+  int64_t total_q, total_kv;
+  int32_t Hk, G, shift;  // G = 1 << shift, or shift < 0
+  float sl2;             // scale * log2(e)
+  int32_t window, sinks, causal, rest;
+  // forward
+  void *out, *lo;  // lo: what out's rounding left, in the same type, or null
+  float* lse;      // (total_q, H): log2 of the sum of 2^(score sl2), or null
+  int32_t splits;  // blocks that share a row tile's keys
+  float* part;     // splits > 1: (splits, total_q, H, D) sums, then (splits, total_q, H, 2)
+  // backward
+  const void* dout;
+  const float* r;  // (total_q, H)
+  void *dq, *dk, *dv;
+};
+
+// ---- rows, and what they see ----------------------------------------------------------------
+__device__ __forceinline__ int query_of(const WaArgs& a, int x) {
+  return a.shift >= 0 ? x >> a.shift : (int)((uint32_t)x / (uint32_t)a.G);
+}
+// Element offset of row x of key head h in a tensor of row stride ld.
+__device__ __forceinline__ int64_t row_at(const WaArgs& a, int64_t ld, int h, int x, int D) {
+  const int i = query_of(a, x);
+  return (int64_t)i * ld + (int64_t)(h * a.G + x - i * a.G) * D;
+}
+
+// The keys that a query at position p sees: [lo, hi) and [0, sink).
+struct Seen {
+  int lo, hi, sink;
+};
+__device__ __forceinline__ Seen seen_from(const WaArgs& a, int p, int keys) {
+  Seen s;
+  s.lo = (int)max<int64_t>(0, (int64_t)p - a.window);
+  s.hi = (int)max<int64_t>(s.lo, min<int64_t>(keys, a.causal ? (int64_t)p + 1 : (int64_t)p + a.window + 1));
+  s.sink = max(0, min(min(a.sinks, keys), a.causal ? p + 1 : keys));
+  return s;
+}
+
+// The key tiles of rows at positions p0 to p1.
+struct Walk {
+  int n1, n2;       // tiles of the two runs
+  int end1, lo, hi; // the first run is [0, end1), the second [lo, hi)
+  bool one;         // the sinks and the window are one run
+  Seen first, last; // of p0 and p1
+  __device__ __forceinline__ Walk(const WaArgs& a, int p0, int p1, int keys) {
+    first = seen_from(a, p0, keys);
+    last = seen_from(a, p1, keys);
+    one = first.lo <= last.sink;
+    end1 = one ? max(last.hi, last.sink) : last.sink;
+    lo = first.lo;
+    hi = last.hi;
+    n1 = (end1 + kBK - 1) / kBK;
+    n2 = one || hi <= lo ? 0 : (hi - lo + kBK - 1) / kBK;
+  }
+  __device__ __forceinline__ int tiles() const { return n1 + n2; }
+  __device__ __forceinline__ void tile(int t, int* at, int* end) const {
+    *at = t < n1 ? t * kBK : lo + (t - n1) * kBK;
+    *end = t < n1 ? end1 : hi;
+  }
+  // Whether rows whose bounds are f (first) to l (last) see all of tile t; whether they see any of it.
+  __device__ __forceinline__ bool full(int t, const Seen& f, const Seen& l) const {
+    int at, end;
+    tile(t, &at, &end);
+    if (at + kBK > end) return false;
+    const bool sinks = t < n1 && at + kBK <= f.sink;
+    const bool win = (one || t >= n1) && at >= l.lo && at + kBK <= f.hi;
+    return sinks || win;
+  }
+  __device__ __forceinline__ bool any(int t, const Seen& f, const Seen& l) const {
+    int at, end;
+    tile(t, &at, &end);
+    const bool sinks = t < n1 && at < l.sink;
+    const bool win = (one || t >= n1) && at < l.hi && at + kBK > f.lo;
+    return sinks || win;
+  }
+  // A row's bounds within the run that tile t belongs to.
+  __device__ __forceinline__ Seen in_run(int t, Seen s) const {
+    if (!one) {
+      if (t < n1) s.hi = s.lo;
+      else s.sink = 0;
+    }
+    return s;
+  }
+};
+__device__ __forceinline__ bool sees(const Seen& s, int k) {
+  return (uint32_t)(k - s.lo) < (uint32_t)(s.hi - s.lo) || k < s.sink;
+}
+
+// ---- infinities and NaN where a row sees nothing ---------------------------------------------
+// Not 0 if an element is not finite: whether each half of a word, or a word, has all of its exponent's bits
+// set, by the carry out of them.
+template <typename T>
+__device__ __forceinline__ uint32_t odd(const F32x8& f) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r |= (__float_as_uint(f.v[i]) & 0x7f800000u) + 0x00800000u & 0x80000000u;
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t odd(const u32x4_t& f) {
+  constexpr uint32_t E = std::is_same<T, __bf16>::value ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t L = std::is_same<T, __bf16>::value ? 0x00800080u : 0x04000400u;
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r |= (f[i] & E) + L & 0x80008000u;
+  return r;
+}
+// The elements of a fragment that are finite (or that are not), zeros for the others.
+template <typename T>
+__device__ __forceinline__ F32x8 part(const F32x8& f, bool finite) {
+  F32x8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = ((__float_as_uint(f.v[i]) & 0x7f800000u) != 0x7f800000u) == finite ? f.v[i] : 0.f;
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ u32x4_t part(const u32x4_t& f, bool finite) {
+  constexpr uint32_t E = std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
+  u32x4_t r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t m = ((f[i] & E) != E ? 0xffffu : 0u) | ((f[i] >> 16 & E) != E ? 0xffff0000u : 0u);
+    r[i] = f[i] & (finite ? m : ~m);
+  }
+  return r;
+}
+// Element x of a fragment, zeros in its other places and where `on` is not set.
+__device__ __forceinline__ F32x8 only(const F32x8& f, int x, bool on) {
+  F32x8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = on && i == x ? f.v[i] : 0.f;
+  return r;
+}
+__device__ __forceinline__ u32x4_t only(const u32x4_t& f, int x, bool on) {
+  u32x4_t r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = on && i == x >> 1 ? f[i] & (x & 1 ? 0xffff0000u : 0xffffu) : 0u;
+  return r;
+}
+
+// acc += sum over the 32 rows e of the tile of p[e] row_e, for those e that the lane's column sees.
+// pf: p as two fragments.  With masks: rows that are not finite go in one by one, and only where seen.
+template <typename T, int D, bool MASK, typename S>
+__device__ __forceinline__ void add_rows(const unsigned char* t, int lane, const typename Frag<T>::type (&pf)[2],
+                                         S see, f32x16_t (&acc)[D / 32]) {
+  typedef Frag<T> F;
+  typedef typename F::type Fr;
+  typedef Tile<T, D> Ti;
+  constexpr int MT = D / 32;
+  if constexpr (MASK) {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) bad |= odd<T>(Ti::col(t, 0, lane, g, mt));
+    if (__builtin_amdgcn_ballot_w64(bad != 0)) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) F::mma(part<T>(Ti::col(t, 0, lane, g, mt), true), pf[g], acc[mt]);
+      for (int e = 0; e < 32; ++e) {
+        const int g = e >> 4, x = 4 * ((e >> 3) & 1) + (e & 3);
+        const bool on = (lane >> 5) == ((e >> 2) & 1), seen = see(e);
+        const Fr p = only(g ? pf[1] : pf[0], x, on);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          f32x16_t one;
+          clear(one);
+          const Fr v = only(part<T>(Ti::col(t, 0, lane, g, mt), false), x, on);
+          if (!__builtin_amdgcn_ballot_w64(odd<T>(v) != 0)) continue;
+          F::mma(v, p, one);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[mt][j] += seen ? one[j] : 0.f;
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) F::mma(Ti::col(t, 0, lane, g, mt), pf[g], acc[mt]);
+}
+
+// ------------------------------------------------------------------------------- forward
+// One tile of 32 keys from k0 on, in LDS, for a wave's 32 rows; s: what the lane's row sees of it.
+template <typename T, int D, bool MASK>
+__device__ __forceinline__ void forward_step(const unsigned char* kt, const unsigned char* vt, int lane,
+                                             int k0, const Seen& s, float sl2,
+                                             const typename Frag<T>::type (&qf)[D / 16], float& m,
+                                             float& l, f32x16_t (&o)[D / 32]) {
+  typedef Frag<T> F;
+  typedef Tile<T, D> Ti;
+  constexpr int KS = D / 16, MT = D / 32;
+  const int l32 = lane & 31, hf = lane >> 5;
+  f32x16_t c;
+  clear(c);
+#pragma unroll
+  for (int st = 0; st < KS; ++st) F::mma(Ti::row(kt, 0, l32, hf, st), qf[st], c);
+  if constexpr (MASK) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (!sees(s, k0 + 8 * (j >> 2) + 4 * hf + (j & 3))) c[j] = -INFINITY;
+  }
+  float mx = c[0], p[16];
+#pragma unroll
+  for (int j = 1; j < 16; ++j) mx = fmaxf(mx, c[j]);
+  mx = pair_max(mx) * sl2;
+  if (__builtin_amdgcn_ballot_w64(mx > m)) {
+    const float mn = fmaxf(m, mx), f = fast_exp2(m - mn);
+    m = mn;
+    l *= f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[mt][j] *= f;
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    p[j] = fast_exp2(fmaf(c[j], sl2, -m));
+    l += p[j];
+  }
+  const typename F::type pf[2] = {F::pack(p), F::pack(p + 8)};
+  add_rows<T, D, MASK>(vt, lane, pf, [&](int e) { return sees(s, k0 + e); }, o);
+}
+
+// Writes a wave's finished rows: l summed over both halves, 0 where a row sees no key.
+template <typename T, int D>
+__device__ __forceinline__ void forward_store(const WaArgs& a, int64_t at, int hf, float m, float l,
+                                              f32x16_t (&o)[D / 32]) {
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+  for (int mt = 0; mt < D / 32; ++mt) {
+    T* p = (T*)a.out + at * D + 32 * mt;
+    if (sizeof(T) == 2 && a.lo) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[mt][j] *= inv;
+      store_dims(p, hf, o[mt], 1.f);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[mt][j] -= (float)(T)o[mt][j];
+      store_dims((T*)a.lo + at * D + 32 * mt, hf, o[mt], 1.f);
+    } else {
+      store_dims(p, hf, o[mt], inv);
+    }
+  }
+  if (a.lse && hf == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
+}
+
+// A block of 4 waves owns 128 rows and walks their keys in tiles of 32.
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward_kernel(const WaArgs a) {
+  typedef Frag<T> F;
+  typedef Tile<T, D> Ti;
+  constexpr int KS = D / 16, MT = D / 32;
+  __shared__ __attribute__((aligned(16))) unsigned char kt[kBK * Ti::ROWB], vt[kBK * Ti::ROWB];
+  int bx, h, bb;
+  block_tile(a.cu_kv, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hf = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int H = a.Hk * a.G, n = q_len * a.G, off = kv_len - q_len;
+  if (a.rest) zero_rest((T*)a.out, a.cu_q, a.total_q, bb, H, D, h * a.G, bx, gridDim.x, a.G);
+  const T* qbase = (const T*)a.q + (int64_t)q0 * a.ldq;
+  const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
+  const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
+
+  for (int64_t rt = (int64_t)bx * kBQ; rt < n; rt += (int64_t)gridDim.x * kBQ) {
+    const int x0 = (int)rt, x = min(x0 + w * 32 + l32, n - 1);
+    const bool live = x0 + w * 32 + l32 < n;
+    typename F::type qf[KS];
+    {
+      const T* p = qbase + row_at(a, a.ldq, h, x, D) + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) qf[st] = F::load(p + 16 * st);
+    }
+    const Walk walk(a, query_of(a, x0) + off, query_of(a, min(x0 + kBQ, n) - 1) + off, kv_len);
+    const Seen mine = seen_from(a, query_of(a, x) + off, kv_len);
+    const Seen wf = seen_from(a, query_of(a, min(x0 + w * 32, n - 1)) + off, kv_len);
+    const Seen wl = seen_from(a, query_of(a, min(x0 + w * 32 + 31, n - 1)) + off, kv_len);
+    const bool idle = x0 + w * 32 >= n;
+    float m = -FLT_MAX, l = 0.f;  // a finite start: a tile of scores of -inf then adds nothing
+    f32x16_t o[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) clear(o[mt]);
+    Stage<T, D, kBK, kNT> ks, vs;
+    const int nt = walk.tiles();
+    auto load = [&](int t) {
+      if (t >= nt) return;
+      int at, end;
+      walk.tile(t, &at, &end);
+      ks.load(kbase, a.ldk, at, end, tid);
+      vs.load(vbase, a.ldv, at, end, tid);
+    };
+    load(0);
+    for (int t = 0; t < nt; ++t) {
+      int at, end;
+      walk.tile(t, &at, &end);
+      __syncthreads();
+      ks.template store<false>(kt, tid);
+      vs.template store<false>(vt, tid);
+      __syncthreads();
+      load(t + 1);
+      if (idle || !walk.any(t, wf, wl)) continue;
+      if (walk.full(t, wf, wl)) {
+        forward_step<T, D, false>(kt, vt, lane, at, mine, a.sl2, qf, m, l, o);
+      } else {
+        Seen s = walk.in_run(t, mine);
+        forward_step<T, D, true>(kt, vt, lane, at, s, a.sl2, qf, m, l, o);
+      }
+    }
+    l = pair_sum(l);
+    if (live) forward_store<T, D>(a, q0 * (int64_t)H + row_at(a, H, h, x, 1), hf, m, l, o);
+  }
+}
+
+// Small grids: a block owns 32 rows, and its waves, and the blocks of a.splits parts, share out their key
+// tiles.  Each wave brings its own tiles through its own piece of LDS, so none waits for another until
+// the end, where their maxima, denominators and sums are joined.
+__device__ __forceinline__ float* part_sums(const WaArgs& a, int sp, int64_t at, int D) {
+  return a.part + ((int64_t)sp * a.total_q * a.Hk * a.G + at) * D;
+}
+__device__ __forceinline__ float2* part_stat(const WaArgs& a, int sp, int64_t at, int D) {
+  return (float2*)part_sums(a, a.splits, 0, D) + (int64_t)sp * a.total_q * a.Hk * a.G + at;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT) wa_few_kernel(const WaArgs a) {
+  typedef Frag<T> F;
+  typedef Tile<T, D> Ti;
+  constexpr int KS = D / 16, MT = D / 32, NW = kNT / 64;
+  constexpr int TB = kBK * Ti::ROWB;
+  constexpr int LB = NW * 2 * TB > 2 * MT * 4096 ? NW * 2 * TB : 2 * MT * 4096;  // the joined sums meet there too
+  __shared__ __attribute__((aligned(16))) unsigned char lds[LB];
+  __shared__ float sm[NW][32], sl[NW][32];
+  int bx, h, bb;
+  block_tile(a.cu_kv, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int sp = bx % a.splits, tile = bx / a.splits, tiles = gridDim.x / a.splits;
+  const int H = a.Hk * a.G, n = q_len * a.G, off = kv_len - q_len;
+  if (a.rest && sp == 0) zero_rest((T*)a.out, a.cu_q, a.total_q, bb, H, D, h * a.G, tile, tiles, a.G);
+  const T* qbase = (const T*)a.q + (int64_t)q0 * a.ldq;
+  const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
+  const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
+  unsigned char *kt = lds + w * 2 * TB, *vt = kt + TB;
+
+  for (int64_t rt = (int64_t)tile * 32; rt < n; rt += (int64_t)tiles * 32) {
+    const int x0 = (int)rt, x = min(x0 + l32, n - 1);
+    typename F::type qf[KS];
+    {
+      const T* p = qbase + row_at(a, a.ldq, h, x, D) + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) qf[st] = F::load(p + 16 * st);
+    }
+    const Walk walk(a, query_of(a, x0) + off, query_of(a, min(x0 + 32, n) - 1) + off, kv_len);
+    const Seen mine = seen_from(a, query_of(a, x) + off, kv_len);
+    float m = -FLT_MAX, l = 0.f;
+    f32x16_t o[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) clear(o[mt]);
+    Stage<T, D, kBK, 64> ks, vs;
+    const int nt = walk.tiles(), per = (nt + a.splits - 1) / a.splits;
+    const int stop = min(nt, (sp + 1) * per);
+    auto load = [&](int t) {
+      if (t >= stop) return;
+      int at, end;
+      walk.tile(t, &at, &end);
+      ks.load(kbase, a.ldk, at, end, lane);
+      vs.load(vbase, a.ldv, at, end, lane);
+    };
+    constexpr bool AHEAD = D == 64 || sizeof(T) == 2;  // registers for the next tile's rows
+    int t = sp * per + w;
+    if (AHEAD) load(t);
+    for (; t < stop; t += NW) {
+      if (!AHEAD) load(t);
+      int at, end;
+      walk.tile(t, &at, &end);
+      // A wave's LDS operations are carried out in order; the compiler has to keep that order.
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      ks.template store<false>(kt, lane);
+      vs.template store<false>(vt, lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (AHEAD) load(t + NW);
+      if (walk.full(t, walk.first, walk.last))
+        forward_step<T, D, false>(kt, vt, lane, at, mine, a.sl2, qf, m, l, o);
+      else
+        forward_step<T, D, true>(kt, vt, lane, at, walk.in_run(t, mine), a.sl2, qf, m, l, o);
+    }
+    l = pair_sum(l);
+    if (hf == 0) {
+      sm[w][l32] = m;
+      sl[w][l32] = l;
+    }
+    __syncthreads();  // every wave has left its tiles
+    const float own = m;
+    m = sm[0][l32];
+#pragma unroll
+    for (int y = 1; y < NW; ++y) m = fmaxf(m, sm[y][l32]);
+    l = 0.f;
+#pragma unroll
+    for (int y = 0; y < NW; ++y) l = fmaf(sl[y][l32], fast_exp2(sm[y][l32] - m), l);
+    const float f = fast_exp2(own - m);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[mt][j] *= f;
+    join_waves<MT>((float*)lds, w, lane, o);
+    if (w != 0 || x0 + l32 >= n) continue;
+    const int64_t at = q0 * (int64_t)H + row_at(a, H, h, x, 1);
+    if (a.splits == 1) {
+      forward_store<T, D>(a, at, hf, m, l, o);
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) store_dims(part_sums(a, sp, at, D) + 32 * mt, hf, o[mt], 1.f);
+      if (hf == 0) *part_stat(a, sp, at, D) = make_float2(m, l);
+    }
+  }
+}
+
+// Joins the parts of the keys: one wave for a (query, head), D / 64 dims a lane.  Rows outside every
+// sequence have no parts.
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT) wa_join_kernel(const WaArgs a, int32_t B) {
+  const int H = a.Hk * a.G;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= a.total_q * H) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = at / H;
+  bool in = false;
+  for (int b = lane; b < B; b += 64) {
+    int q0, ql;
+    segment(a.cu_q, b, a.total_q, &q0, &ql);
+    in |= row >= q0 && row < (int64_t)q0 + ql;
+  }
+  if (__builtin_amdgcn_ballot_w64(in) == 0) return;
+  float m = -FLT_MAX, l = 0.f, o[D / 64] = {};
+  for (int p = lane; p < a.splits; p += 64) m = fmaxf(m, part_stat(a, p, at, D)->x);
+  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+#pragma unroll 4
+  for (int p = 0; p < a.splits; ++p) {  // independent loads, one order of the sums
+    const float2 st = *part_stat(a, p, at, D);
+    const float* po = part_sums(a, p, at, D);
+    const float f = fast_exp2(st.x - m);
+    l = fmaf(st.y, f, l);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] = fmaf(po[lane + 64 * e], f, o[e]);
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) {
+    const int64_t p = at * D + lane + 64 * e;
+    const float y = o[e] * inv;
+    ((T*)a.out)[p] = (T)y;
+    if (sizeof(T) == 2 && a.lo) ((T*)a.lo)[p] = (T)(y - (float)(T)y);
+  }
+  if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
+}
+
+// ------------------------------------------------------------------------------- backward
+// r = do . out per (query, head), out with what its rounding left: dS = P (dP - r) cancels where one key
+// has most of a row, and out's rounding would be most of what is left.
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT) wa_rowdot_kernel(const T* dout, const T* out, const T* lo, int64_t rows,
+                                                        float* r) {
+  constexpr int LPR = D / 8;
+  const int64_t row = ((int64_t)blockIdx.x * kNT + threadIdx.x) / LPR;
+  const int e0 = threadIdx.x % LPR * 8;
+  if (row >= rows) return;
+  float t = 0.f;
+#pragma unroll
+  for (int c = 0; c < 8; c += 16 / sizeof(T)) {
+    const u32x4_t x = *(const u32x4_t*)(dout + row * D + e0 + c), y = *(const u32x4_t*)(out + row * D + e0 + c);
+    u32x4_t z = {0, 0, 0, 0};
+    if (sizeof(T) == 2) z = *(const u32x4_t*)(lo + row * D + e0 + c);
+#pragma unroll
+    for (int e = 0; e < (int)(16 / sizeof(T)); ++e)
+      t = fmaf((float)((const T*)&x)[e], (float)((const T*)&y)[e] + (float)((const T*)&z)[e], t);
+  }
+#pragma unroll
+  for (int off = LPR / 2; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
+  if (e0 == 0) r[row] = t;
+}
+
+// Both gradient kernels: a block's waves own 32 rows (keys) each and share the tiles of the other side,
+// through two buffers in LDS; or, where that leaves CUs idle (SHARE), all own the same 32 and take the
+// tiles in turn, each through its own piece of LDS, and their sums are joined at the end.
+template <bool SHARE>
+__device__ __forceinline__ void tile_sync() {
+  if (SHARE) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  else __syncthreads();
+}
+
+template <typename T, int D, bool SHARE>
+__global__ void __launch_bounds__(kNT, 1) wa_dq_kernel(const WaArgs a) {
+  typedef Frag<T> F;
+  typedef typename F::type Fr;
+  typedef Tile<T, D> Ti;
+  constexpr int KS = D / 16, MT = D / 32;
+  constexpr int TB = kBK * Ti::ROWB, ROWS = SHARE ? 32 : kBQ, NT = SHARE ? 64 : kNT, BUFS = SHARE ? 4 : 2;
+  constexpr int LB = !SHARE || BUFS * 2 * TB > 2 * MT * 4096 ? BUFS * 2 * TB : 2 * MT * 4096;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[LB];
+  int bx, h, bb;
+  block_tile(a.cu_kv, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = SHARE ? lane : threadIdx.x;
+  const int H = a.Hk * a.G, n = q_len * a.G, off = kv_len - q_len;
+  if (a.rest) zero_rest((T*)a.dq, a.cu_q, a.total_q, bb, H, D, h * a.G, bx, gridDim.x, a.G);
+  const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
+  const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
+  const float scale = a.sl2 / kLog2e;
+
+  for (int64_t rt = (int64_t)bx * ROWS; rt < n; rt += (int64_t)gridDim.x * ROWS) {
+    const int x0 = (int)rt, xw = SHARE ? x0 : x0 + w * 32, x = min(xw + l32, n - 1);
+    const int64_t at = q0 * (int64_t)H + row_at(a, H, h, x, 1);
+    Fr qf[KS], df[KS];
+    {
+      const T* p = (const T*)a.q + (int64_t)q0 * a.ldq + row_at(a, a.ldq, h, x, D) + 8 * hf;
+      const T* d = (const T*)a.dout + at * D + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        qf[st] = F::load(p + 16 * st);
+        df[st] = F::load(d + 16 * st);
+      }
+    }
+    const float lse = a.lse[at], r = a.r[at];
+    const Walk walk(a, query_of(a, x0) + off, query_of(a, min(x0 + ROWS, n) - 1) + off, kv_len);
+    const Seen mine = seen_from(a, query_of(a, x) + off, kv_len);
+    const Seen wf = seen_from(a, query_of(a, min(xw, n - 1)) + off, kv_len);
+    const Seen wl = seen_from(a, query_of(a, min(xw + 31, n - 1)) + off, kv_len);
+    const bool idle = xw >= n;
+    f32x16_t acc[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) clear(acc[mt]);
+    Stage<T, D, kBK, NT> ks, vs;
+    const int nt = walk.tiles();
+    auto load = [&](int t) {
+      if (t >= nt) return;
+      int k0, end;
+      walk.tile(t, &k0, &end);
+      ks.load(kbase, a.ldk, k0, end, tid);
+      vs.load(vbase, a.ldv, k0, end, tid);
+    };
+    constexpr int STEP = SHARE ? 4 : 1;
+    constexpr bool AHEAD = !SHARE || sizeof(T) == 2 || D == 64;
+    auto step = [&](const unsigned char* kt, const unsigned char* vt, auto masked, int k0, const Seen& s) {
+      constexpr bool MASK = decltype(masked)::value;
+      f32x16_t c, dp;
+      clear(c);
+      clear(dp);
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        F::mma(Ti::row(kt, 0, l32, hf, st), qf[st], c);
+        F::mma(Ti::row(vt, 0, l32, hf, st), df[st], dp);
+      }
+      float d[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        d[j] = fast_exp2(fmaf(c[j], a.sl2, -lse)) * (dp[j] - r);
+        if (MASK && !sees(s, k0 + 8 * (j >> 2) + 4 * hf + (j & 3))) d[j] = 0.f;
+      }
+      const Fr f[2] = {F::pack(d), F::pack(d + 8)};
+      add_rows<T, D, MASK>(kt, lane, f, [&](int e) { return sees(s, k0 + e); }, acc);
+    };
+    int t = SHARE ? w : 0;
+    if (AHEAD) load(t);
+    for (int buf = 0; t < nt; t += STEP, buf ^= 1) {
+      unsigned char *kt = lds + (SHARE ? w : buf) * 2 * TB, *vt = kt + TB;
+      if (!AHEAD) load(t);
+      if (SHARE) tile_sync<SHARE>();
+      ks.template store<false>(kt, tid);
+      vs.template store<false>(vt, tid);
+      tile_sync<SHARE>();
+      if (AHEAD) load(t + STEP);
+      int k0, end;
+      walk.tile(t, &k0, &end);
+      if (idle || !walk.any(t, wf, wl)) continue;
+      if (walk.full(t, wf, wl)) step(kt, vt, std::false_type(), k0, mine);
+      else step(kt, vt, std::true_type(), k0, walk.in_run(t, mine));
+    }
+    if (SHARE) join_waves<MT>((float*)lds, w, lane, acc);
+    else __syncthreads();  // the next tile's rows go into these buffers
+    if (xw + l32 < n && (!SHARE || w == 0)) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) store_dims((T*)a.dq + at * D + 32 * mt, hf, acc[mt], scale);
+    }
+  }
+}
+
+// The rows that see key k: one run [lo, hi).
+struct Rows {
+  int lo, hi;
+};
+__device__ __forceinline__ Rows rows_of(const WaArgs& a, int k, int off, int q_len) {
+  const bool sink = k < a.sinks;
+  int64_t lo = a.causal ? (int64_t)k - off : sink ? 0 : (int64_t)k - a.window - off;
+  int64_t hi = sink ? q_len : (int64_t)k + a.window - off + 1;
+  lo = min<int64_t>(max<int64_t>(lo, 0), q_len);
+  hi = min<int64_t>(max<int64_t>(hi, lo), q_len);
+  return {(int)lo * a.G, (int)hi * a.G};
+}
+
+// dk and dv of 128 (32) keys of a key head, over the rows of all its query heads.
+template <typename T, int D, bool SHARE>
+__global__ void __launch_bounds__(kNT, 1) wa_dkv_kernel(const WaArgs a) {
+  typedef Frag<T> F;
+  typedef typename F::type Fr;
+  typedef Tile<T, D> Ti;
+  constexpr int BQ = 32;
+  constexpr int KS = D / 16, MT = D / 32;
+  constexpr int ROWS = SHARE ? 32 : 128, NT = SHARE ? 64 : kNT, BUFS = SHARE ? 4 : 2;
+  constexpr int TB = BQ * Ti::ROWB;
+  constexpr int LB = !SHARE || BUFS * 2 * TB > 2 * MT * 4096 ? BUFS * 2 * TB : 2 * MT * 4096;
+  constexpr int NL = BQ * Ti::CPR / NT, EPC = 16 / sizeof(T);
+  __shared__ __attribute__((aligned(16))) unsigned char lds[LB];
+  __shared__ __attribute__((aligned(16))) float stats[BUFS][2][BQ];
+  int bx, h, bb;
+  block_tile(a.cu_q, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = SHARE ? lane : threadIdx.x;
+  const int H = a.Hk * a.G, off = kv_len - q_len;
+  if (a.rest) {
+    zero_rest((T*)a.dk, a.cu_kv, a.total_kv, bb, a.Hk, D, h, bx, gridDim.x, 1);
+    zero_rest((T*)a.dv, a.cu_kv, a.total_kv, bb, a.Hk, D, h, bx, gridDim.x, 1);
+  }
+  const T* qbase = (const T*)a.q + (int64_t)q0 * a.ldq;
+  const T* dbase = (const T*)a.dout + (int64_t)q0 * H * D;
+  const float scale = a.sl2 / kLog2e;
+
+  for (int64_t ktile = (int64_t)bx * ROWS; ktile < kv_len; ktile += (int64_t)gridDim.x * ROWS) {
+    const int k0 = (int)ktile, kw = SHARE ? k0 : k0 + w * 32, ki = min(kw + l32, kv_len - 1);
+    const int64_t krow = kv0 + ki;
+    Fr kf[KS], vf[KS];
+    {
+      const T* p = (const T*)a.k + krow * a.ldk + (int64_t)h * D + 8 * hf;
+      const T* d = (const T*)a.v + krow * a.ldv + (int64_t)h * D + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        kf[st] = F::load(p + 16 * st);
+        vf[st] = F::load(d + 16 * st);
+      }
+    }
+    // The rows of the block's keys and of the wave's: along the keys both bounds grow, but for the sinks'.
+    auto span = [&](int first, int last, int* most, int* least) {  // of all keys; that see each of them
+      const Rows f = rows_of(a, first, off, q_len), l = rows_of(a, last, off, q_len);
+      const bool mixed = first < a.sinks && last >= a.sinks;
+      const Rows m = mixed ? rows_of(a, a.sinks, off, q_len) : f;
+      *most = max(l.lo, f.lo);
+      *least = min(min(f.hi, l.hi), m.hi);
+      return Rows{min(f.lo, l.lo), max(max(f.hi, l.hi), f.lo)};
+    };
+    int all_lo, all_hi, wave_lo, wave_hi;
+    const Rows run = span(k0, min(k0 + ROWS, kv_len) - 1, &all_lo, &all_hi);
+    const Rows wrun = span(min(kw, kv_len - 1), min(kw + 31, kv_len - 1), &wave_lo, &wave_hi);
+    const Rows mine = rows_of(a, ki, off, q_len);
+    const bool idle = kw >= kv_len;
+    f32x16_t dk[MT], dv[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      clear(dk[mt]);
+      clear(dv[mt]);
+    }
+    u32x4_t qr[NL], dr[NL];
+    float sv = 0.f;
+    constexpr int STEP = SHARE ? 4 * BQ : BQ;
+    constexpr bool AHEAD = !SHARE || sizeof(T) == 2 || D == 64;
+    // Rows past the last one repeat it: they are masked.
+    auto load = [&](int xb) {
+      if (xb >= run.hi) return;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int id = tid + NT * i, x = min(xb + id / Ti::CPR, run.hi - 1), c = id % Ti::CPR * EPC;
+        const int qi = query_of(a, x);
+        const int64_t hd = (int64_t)(h * a.G + x - qi * a.G) * D + c;
+        qr[i] = *(const u32x4_t*)(qbase + qi * a.ldq + hd);
+        dr[i] = *(const u32x4_t*)(dbase + (int64_t)qi * H * D + hd);
+      }
+      if (tid < 64) {
+        const int x = min(xb + (tid & 31), run.hi - 1);
+        const int64_t at = q0 * (int64_t)H + row_at(a, H, h, x, 1);
+        sv = tid < 32 ? a.lse[at] : a.r[at];
+      }
+    };
+    auto step = [&](const unsigned char* qt, const unsigned char* dt, const float(*st2)[BQ], int xb, auto masked) {
+      constexpr bool MASK = decltype(masked)::value;
+      f32x16_t c, dp;
+      clear(c);
+      clear(dp);
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        F::mma(Ti::row(qt, 0, l32, hf, st), kf[st], c);
+        F::mma(Ti::row(dt, 0, l32, hf, st), vf[st], dp);
+      }
+      auto see = [&](int e) { return (uint32_t)(xb + e - mine.lo) < (uint32_t)(mine.hi - mine.lo); };
+      float p[16], d[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int e = 8 * (j >> 2) + 4 * hf + (j & 3);
+        p[j] = fast_exp2(fmaf(c[j], a.sl2, -st2[0][e]));
+        d[j] = p[j] * (dp[j] - st2[1][e]);
+        if (MASK && !see(e)) p[j] = d[j] = 0.f;
+      }
+      const Fr pf[2] = {F::pack(p), F::pack(p + 8)};
+      add_rows<T, D, MASK>(dt, lane, pf, see, dv);
+      const Fr df[2] = {F::pack(d), F::pack(d + 8)};
+      add_rows<T, D, MASK>(qt, lane, df, see, dk);
+    };
+    int xb = run.lo + (SHARE ? w * BQ : 0);
+    if (AHEAD) load(xb);
+    for (int buf = 0; xb < run.hi; xb += STEP, buf ^= 1) {
+      unsigned char *qt = lds + (SHARE ? w : buf) * 2 * TB, *dt = qt + TB;
+      float(*st2)[BQ] = stats[SHARE ? w : buf];
+      if (!AHEAD) load(xb);
+      if (SHARE) tile_sync<SHARE>();
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int id = tid + NT * i;
+        Ti::put(qt, id / Ti::CPR, id % Ti::CPR, qr[i]);
+        Ti::put(dt, id / Ti::CPR, id % Ti::CPR, dr[i]);
+      }
+      if (tid < 64) st2[tid >> 5][tid & 31] = sv;
+      tile_sync<SHARE>();
+      if (AHEAD) load(xb + STEP);
+      if (idle || xb >= wrun.hi || xb + BQ <= wrun.lo) continue;
+      if (xb >= wave_lo && xb + BQ <= wave_hi) step(qt, dt, st2, xb, std::false_type());
+      else step(qt, dt, st2, xb, std::true_type());
+    }
+    if (SHARE) {
+      join_waves<MT>((float*)lds, w, lane, dk);
+      join_waves<MT>((float*)lds, w, lane, dv);
+    } else {
+      __syncthreads();  // every wave has left the buffers
+    }
+    if (kw + l32 < kv_len && (!SHARE || w == 0)) {
+      const int64_t at = (krow * a.Hk + h) * D;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        store_dims((T*)a.dk + at + 32 * mt, hf, dk[mt], scale);
+        store_dims((T*)a.dv + at + 32 * mt, hf, dv[mt], 1.f);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------- host
+constexpr int64_t kCUs = 256;
+
+// Tiles of `rows` rows that the grid gives a sequence; the kernels' loops cover longer ones.
+unsigned tiles_of(int64_t longest, int64_t hb, int rows) {
+  return (unsigned)std::max<int64_t>(
+      1, std::min<int64_t>(std::min<int64_t>((longest + rows - 1) / rows, 65535), (INT32_MAX / 1024) / hb));
+}
+
+// Blocks of the forward pass: rows of each, and the parts of their keys.
+struct Plan {
+  int rows, splits;
+};
+constexpr int64_t kScratchInputs = 4, kScratchLeast = 64 << 20;
+int64_t part_bytes(int64_t total_q, int32_t H, int32_t D) { return 4 * total_q * H * (D + 2); }
+Plan wa_plan(const WindowAttnSizes& z) {
+  const int64_t hb = (int64_t)z.Hk * z.B, G = z.H / z.Hk;
+  const int64_t max_q = std::max<int64_t>(z.max_q, (z.total_q + z.B - 1) / z.B);
+  Plan p = {kBQ, 1};
+  if ((int64_t)tiles_of(max_q * G, hb, kBQ) * hb >= kCUs) return p;
+  p.rows = 32;
+  const int64_t blocks = (int64_t)tiles_of(max_q * G, hb, 32) * hb;
+  if (blocks >= 2 * kCUs) return p;
+  const int64_t span = std::min<int64_t>(z.max_kv, (z.causal ? 1 : 2) * (int64_t)z.window + 32 + z.sinks);
+  const int64_t es = z.dtype == TSC_F32 ? 4 : 2;
+  const int64_t io = 2 * z.D * es * (z.total_q * z.H + z.total_kv * z.Hk);
+  const int64_t room = std::max(kScratchLeast, kScratchInputs * io) / std::max<int64_t>(1, part_bytes(z.total_q, z.H, z.D));
+  p.splits = (int)std::max<int64_t>(1, std::min({span / 256, 2 * kCUs / blocks, room}));
+  return p;
+}
+
+template <typename F>
+int by_type(int32_t dtype, int32_t D, F f) {
+  constexpr std::integral_constant<int, 64> D64{};
+  constexpr std::integral_constant<int, 128> D128{};
+  auto dims = [&](auto t) { D == 64 ? f(t, D64) : f(t, D128); };
+  if (dtype == TSC_BF16) dims(__bf16());
+  else if (dtype == TSC_F16) dims(_Float16());
+  else dims(float());
+  return check_hip(hipGetLastError(), "window_attention launch");
+}
+
+WaArgs wa_args(const WindowAttnArgs& x) {
+  const WindowAttnSizes& z = x.z;
+  WaArgs a = {};
+  a.q = x.q;
+  a.k = x.k;
+  a.v = x.v;
+  a.ldq = x.ldq;
+  a.ldk = x.ldk;
+  a.ldv = x.ldv;
+  a.cu_q = x.cu_q;
+  a.cu_kv = x.cu_kv;
+  a.total_q = z.total_q;
+  a.total_kv = z.total_kv;
+  a.Hk = z.Hk;
+  a.G = z.H / z.Hk;
+  a.shift = -1;
+  for (int s = 0; s < 16; ++s)
+    if (a.G == 1 << s) a.shift = s;
+  a.sl2 = x.scale * kLog2e;
+  a.window = z.window;
+  a.sinks = z.sinks;
+  a.causal = z.causal;
+  a.rest = x.rest;
+  a.splits = 1;
+  return a;
+}
+int too_many(const WindowAttnSizes& z) {
+  const int64_t hb = (int64_t)z.Hk * z.B, G = z.H / z.Hk;
+  if (hb > (int64_t)(INT32_MAX / 1024))
+    return fail(TSC_ERR_UNSUPPORTED, "window_attention: %lld (key head, sequence) pairs", (long long)hb);
+  if (z.total_q * G > INT32_MAX - 1024)
+    return fail(TSC_ERR_UNSUPPORTED, "window_attention: %lld queries with %lld heads to a key head",
+                (long long)z.total_q, (long long)G);
+  return TSC_OK;
+}
+
+}  // namespace
+
+int64_t window_attention_workspace_bytes(const WindowAttnSizes& z, int32_t backward) {
+  if (z.B == 0 || z.total_q == 0) return 0;
+  if (backward) return 4 * z.total_q * z.H;
+  const int s = wa_plan(z).splits;
+  return s > 1 ? s * part_bytes(z.total_q, z.H, z.D) : 0;
+}
+
+int window_attention_launch(tsc_ctx* ctx, const WindowAttnArgs& x, void* out, void* out_lo, float* lse, void* ws) {
+  const WindowAttnSizes& z = x.z;
+  if (int st = too_many(z)) return st;
+  WaArgs a = wa_args(x);
+  a.out = out;
+  a.lo = out_lo;
+  a.lse = lse;
+  a.part = (float*)ws;
+  const Plan plan = wa_plan(z);
+  a.splits = plan.splits;
+  const int64_t hb = (int64_t)z.Hk * z.B;
+  const dim3 grid(tiles_of((int64_t)z.max_q * a.G, hb, plan.rows) * a.splits, (unsigned)z.Hk, (unsigned)z.B);
+  return by_type(z.dtype, z.D, [&](auto t, auto d) {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    {
+      ProfScope p(ctx, "window_attention");
+      if (plan.rows == 32) wa_few_kernel<T, D><<<grid, kNT, 0, ctx->stream>>>(a);
+      else wa_forward_kernel<T, D><<<grid, kNT, 0, ctx->stream>>>(a);
+    }
+    if (a.splits > 1) {
+      ProfScope p(ctx, "window_attention_join");
+      wa_join_kernel<T, D><<<(unsigned)((z.total_q * z.H + 3) / 4), kNT, 0, ctx->stream>>>(a, z.B);
+    }
+  });
+}
+
+int window_attention_backward_launch(tsc_ctx* ctx, const WindowAttnArgs& x, const void* out, const void* out_lo,
+                                     const float* lse, const void* dout, void* ws, void* dq, void* dk, void* dv) {
+  const WindowAttnSizes& z = x.z;
+  if (int st = too_many(z)) return st;
+  WaArgs a = wa_args(x);
+  a.lse = (float*)lse;
+  a.dout = dout;
+  a.r = (float*)ws;
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  const int64_t hb = (int64_t)z.Hk * z.B, rows = z.total_q * z.H;
+  const bool few_q = (int64_t)tiles_of((int64_t)z.max_q * a.G, hb, kBQ) * hb < kCUs;
+  const bool few_k = (int64_t)tiles_of(z.max_kv, hb, kBQ) * hb < kCUs;
+  const dim3 gq(tiles_of((int64_t)z.max_q * a.G, hb, few_q ? 32 : kBQ), (unsigned)z.Hk, (unsigned)z.B);
+  const dim3 gk(tiles_of(z.max_kv, hb, few_k ? 32 : kBQ), (unsigned)z.Hk, (unsigned)z.B);
+  return by_type(z.dtype, z.D, [&](auto t, auto d) {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    if (rows > 0) {
+      ProfScope p(ctx, "window_attention_rowdot");
+      wa_rowdot_kernel<T, D><<<(unsigned)((rows * (D / 8) + kNT - 1) / kNT), kNT, 0, ctx->stream>>>(
+          (const T*)dout, (const T*)out, (const T*)out_lo, rows, (float*)ws);
+    }
+    {
+      ProfScope p(ctx, "window_attention_dkv");
+      if (few_k) wa_dkv_kernel<T, D, true><<<gk, kNT, 0, ctx->stream>>>(a);
+      else wa_dkv_kernel<T, D, false><<<gk, kNT, 0, ctx->stream>>>(a);
+    }
+    if (rows > 0) {
+      ProfScope p(ctx, "window_attention_dq");
+      if (few_q) wa_dq_kernel<T, D, true><<<gq, kNT, 0, ctx->stream>>>(a);
+      else wa_dq_kernel<T, D, false><<<gq, kNT, 0, ctx->stream>>>(a);
+    }
+  });
+}
+
+}  // namespace tsc

@@ -6,6 +6,7 @@ Inputs must be contiguous tensors on a HIP device (there is no CPU path).
 from __future__ import annotations
 
 import ctypes
+import operator
 from dataclasses import dataclass
 
 import torch
@@ -792,16 +793,8 @@ def sparse_diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam
     if ck.numel() != cq.numel():
         raise TscError(_lib.TSC_ERR_INVALID, "cu_seqlens_q and cu_seqlens_kv differ in length")
     b = cq.numel() - 1
-
-    def longest(given, host, total):
-        if given is not None:
-            return max(0, min(int(given), total))
-        if b == 0:
-            return 0
-        return int((host[1:] - host[:-1]).max()) if host is not None else min(total, 2 * -(-total // b))
-
     args = (cq, ck, b, float(scale) if scale is not None else 0.0,
-            longest(max_seqlen_q, cq_host, tq), longest(max_seqlen_kv, ck_host, tkv))
+            _longest(max_seqlen_q, cq_host, tq, b), _longest(max_seqlen_kv, ck_host, tkv, b))
     if _wants_grad(q, k, v, lam, out):
         if out is not None:
             raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: out cannot be given where gradients "
@@ -852,6 +845,134 @@ def _diff_attention_backward(do, q, k, v, lam, maps, lse, cq, ck, b, scale, max_
             _head_rows(v, "v"), _p(lam), _p(cq), _p(ck), b, tq, tkv, h, d, scale, max_q, max_kv, 1,
             _p(maps), _p(lse), _p(do), _p(ws), _p(dq), _p(dk), _p(dv), _p(dlam)))
     return dq, dk, dv, dlam
+
+
+_NO_BOUND = 2 ** 31 - 1
+
+
+def sparse_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int | None,
+                            cu_seqlens_q, cu_seqlens_kv=None, sinks: int = 0, causal: bool = False,
+                            scale: float | None = None, out=None, max_seqlen_q: int | None = None,
+                            max_seqlen_kv: int | None = None) -> torch.Tensor:
+    """Attention in a sliding window along packed sequences, with a few first tokens that stay visible
+    (tsc_window_attention):
+
+        out[i] = softmax(q[i] k^T scale over the keys that i sees) v
+
+    Query i of a sequence of n queries and m keys stands at position p = i + m - n and sees key j where
+    (j < sinks or |p - j| <= window) and, with causal, j <= p; a query that sees none gives zeros.  window
+    None: no bound.  q (total_q, H, D), k / v (total_kv, Hk, D), each key head shared by H / Hk query heads;
+    D is 64 or 128.  cu_seqlens, scale, max_seqlen_*, strided rows and `out` as in sparse_diff_attention,
+    scale defaulting to 1/sqrt(D).  With fewer queries than keys the queries are the last rows: a token, or
+    a piece of a prompt, on a longer cache.  Few queries on many keys are shared out over the keys.
+    Differentiable in q, k and v (then without `out`; a graph through the gradient itself is not
+    supported)."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2]:
+        raise TscError(_lib.TSC_ERR_INVALID, f"window_attention: q {tuple(q.shape)}, k {tuple(k.shape)} "
+                                             f"and v {tuple(v.shape)} must be (total, heads, D)")
+    tq, h, d = q.shape
+    tkv, hk = k.shape[:2]
+    if hk == 0 or h == 0 or h % hk:
+        raise TscError(_lib.TSC_ERR_INVALID, f"window_attention: {hk} key heads do not divide {h} query heads")
+    if d not in (64, 128):
+        raise TscError(_lib.TSC_ERR_UNSUPPORTED, f"window_attention: head_dim {d} (64 and 128 are supported)")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TscError(_lib.TSC_ERR_INVALID, "window_attention: q, k and v must share a dtype")
+    window = _NO_BOUND if window is None else operator.index(window)
+    sinks = operator.index(sinks)
+    if not 0 <= window <= _NO_BOUND or not 0 <= sinks <= _NO_BOUND:
+        raise TscError(_lib.TSC_ERR_INVALID, f"window_attention: window {window} and sinks {sinks} must be in "
+                                             "[0, 2^31)")
+    if scale is not None and not 0 < ctypes.c_float(scale).value < float("inf"):
+        raise TscError(_lib.TSC_ERR_INVALID, "window_attention: scale must be positive and finite in fp32")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
+        raise TscError(_lib.TSC_ERR_INVALID, "window_attention: out has the wrong shape or dtype")
+    _code(q)
+    _no_tangents("window_attention", q, k, v, out)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _head_rows(t, name)
+    dev = _dev(out)
+    for t in (q, k, v):
+        if not t.is_cuda or dev is not None and t.device.index != dev:
+            raise TscError(_lib.TSC_ERR_INVALID, "tensors are not on one GPU; this path has no CPU fallback")
+        dev = t.device.index
+    cq_host, cq = _cu_seqlens(cu_seqlens_q, tq, dev, "cu_seqlens_q")
+    if cu_seqlens_kv is None:
+        if tkv != tq:
+            raise TscError(_lib.TSC_ERR_INVALID, "window_attention: cu_seqlens_kv is needed where k has "
+                                                 "other rows than q")
+        ck_host, ck = cq_host, cq
+    else:
+        ck_host, ck = _cu_seqlens(cu_seqlens_kv, tkv, dev, "cu_seqlens_kv")
+    for t in (cq, ck):
+        if t.device.index != dev:
+            raise TscError(_lib.TSC_ERR_INVALID, "tensors live on different devices")
+    if ck.numel() != cq.numel():
+        raise TscError(_lib.TSC_ERR_INVALID, "cu_seqlens_q and cu_seqlens_kv differ in length")
+    b = cq.numel() - 1
+    args = (cq, ck, b, float(scale) if scale is not None else 0.0, window, sinks, int(bool(causal)),
+            _longest(max_seqlen_q, cq_host, tq, b), _longest(max_seqlen_kv, ck_host, tkv, b))
+    if _wants_grad(q, k, v, out):
+        if out is not None:
+            raise TscError(_lib.TSC_ERR_INVALID, "window_attention: out cannot be given where gradients "
+                                                 "are wanted")
+        from .autograd import WindowAttention
+
+        return WindowAttention.apply(q, k, v, args)
+    return _window_attention(q, k, v, args, out, False)[0]
+
+
+def _longest(given, host, total: int, b: int) -> int:
+    """The longest sequence's length, as far as it is known: what the caller says, the host's offsets', or
+    twice the mean."""
+    if given is not None:
+        return max(0, min(int(given), total))
+    if b == 0:
+        return 0
+    return int((host[1:] - host[:-1]).max()) if host is not None else min(total, 2 * -(-total // b))
+
+
+def _window_attention(q, k, v, args, out, keep):
+    """(out, lo, lse); lo and lse (None unless keep) are what the backward pass needs."""
+    cq, ck, b, scale, window, sinks, causal, max_q, max_kv = args
+    tq, h, d = q.shape
+    tkv, hk = k.shape[:2]
+    rest = out is None
+    if out is None:
+        out = (torch.empty if b else torch.zeros)((tq, h, d), dtype=q.dtype, device=q.device)
+    lo = torch.empty_like(out) if keep and q.dtype != torch.float32 else None
+    lse = torch.empty((tq, h), dtype=torch.float32, device=q.device) if keep else None
+    if tq and b:
+        lib, handle = _lib.stream_handle(q.device.index)
+        nbytes = lib.tsc_window_attention_workspace_bytes(_code(q), b, tq, tkv, h, hk, d, window, sinks, causal,
+                                                          max_q, max_kv, 0)
+        ws = _scratch(nbytes, q.device) if nbytes else None
+        check(lib.tsc_window_attention(handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"),
+                                       _head_rows(k, "k"), _head_rows(v, "v"), _p(cq), _p(ck), b, tq, tkv, h,
+                                       hk, d, scale, window, sinks, causal, max_q, max_kv, int(rest), _p(ws),
+                                       _p(out), _p(lo), _p(lse)))
+        if not rest:
+            _wrote(out)
+    return out, lo, lse
+
+
+def _window_attention_backward(do, q, k, v, out, lo, lse, args):
+    cq, ck, b, scale, window, sinks, causal, max_q, max_kv = args
+    tq, h, d = q.shape
+    tkv, hk = k.shape[:2]
+    alloc = torch.empty if b else torch.zeros
+    dq = alloc((tq, h, d), dtype=q.dtype, device=q.device)
+    dk, dv = (alloc((tkv, hk, d), dtype=q.dtype, device=q.device) for _ in range(2))
+    if b and (tq or tkv):
+        lib, handle = _lib.stream_handle(q.device.index)
+        nbytes = lib.tsc_window_attention_workspace_bytes(_code(q), b, tq, tkv, h, hk, d, window, sinks, causal,
+                                                          max_q, max_kv, 1)
+        ws = _scratch(nbytes, q.device)
+        check(lib.tsc_window_attention_backward(
+            handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"), _head_rows(k, "k"), _head_rows(v, "v"),
+            _p(cq), _p(ck), b, tq, tkv, h, hk, d, scale, window, sinks, causal, max_q, max_kv, 1, _p(out),
+            _p(lo), _p(lse), _p(do), _p(ws), _p(dq), _p(dk), _p(dv)))
+    return dq, dk, dv
 
 
 def scaled_dot_product_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
