@@ -228,22 +228,31 @@ def context(device: int) -> Context:
 _stream_handles: dict[tuple[int, int], ctypes.c_void_p] = {}
 
 
+try:  # a stream's number without an object around it: 1.5 us less a call
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(device: int) -> int:
+        import torch
+
+        return torch.cuda.current_stream(device).cuda_stream
+
+
 def stream_handle(device: int):
     """(library, handle of a context on torch's current stream) for the ops that keep nothing in a
     context: one per stream, made at its first use and never re-pointed, so that calls from several
     threads, on several streams or under graph capture (where the device's shared context cannot
     wait for the stream it was on) do not meet.  While the shared context is profiled it is that one."""
-    import torch
-
     shared = _contexts.get(device)
     if shared is not None and shared.profiling:
         return shared.lib, shared.bind()
-    lib = load_library()
-    stream = torch.cuda.current_stream(device).cuda_stream
-    with _lock:
-        h = _stream_handles.get((device, stream))
-        if h is None:
-            h = _P()
-            check(lib.tsc_ctx_create(device, _P(stream), ctypes.byref(h)))
-            _stream_handles[device, stream] = h
-    return lib, h
+    stream = _raw_stream(device)
+    h = _stream_handles.get((device, stream))
+    if h is None:
+        lib = load_library()
+        with _lock:
+            h = _stream_handles.get((device, stream))
+            if h is None:
+                h = _P()
+                check(lib.tsc_ctx_create(device, _P(stream), ctypes.byref(h)))
+                _stream_handles[device, stream] = h
+    return _lib, h

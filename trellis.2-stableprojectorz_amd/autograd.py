@@ -32,26 +32,29 @@ class GroupNorm(torch.autograd.Function):
 
 class GatedNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, pw, pb, gate, w, bias, scale, shift, args, want_r, want_h):
-        tensors = (x, y, pw, pb, gate, w, bias, scale, shift)
-        r, h, stats = ops._gated_norm(tensors, args, want_r, want_h, None, True)
+    def forward(ctx, how, *given):
+        args, there, want_r, want_h = how
+        it = iter(given)
+        r, h, stats = ops._gated_norm([next(it) if t else None for t in there], args, want_r, want_h, None, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(*tensors, args[0], stats)
-        ctx.args = (args[1:], want_r, want_h)
+        ctx.save_for_backward(args[0], stats, *given)
+        ctx.how = (args[1:], there, want_r, want_h)
         return (r, h) if want_r and want_h else r if want_r else h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *douts):
-        *tensors, cu, stats = ctx.saved_tensors
-        args, want_r, want_h = ctx.args
+        args, there, want_r, want_h = ctx.how
         douts = [None if d is None else d.contiguous() for d in douts]
         dr = douts[0] if want_r else None
         dh = douts[-1] if want_h else None
         if dr is None and dh is None:
-            return (None,) * 12
-        grads = ops._gated_norm_backward(tensors, (cu, *args), stats, dr, dh, ctx.needs_input_grad[:9])
-        return (*grads, None, None, None)
+            return (None,) * len(ctx.needs_input_grad)
+        cu, stats, *given = ctx.saved_tensors
+        it, wanted = iter(given), iter(ctx.needs_input_grad[1:])
+        grads = ops._gated_norm_backward([next(it) if t else None for t in there], (cu, *args), stats, dr, dh,
+                                         [t and next(wanted) for t in there])
+        return (None, *(g for g, t in zip(grads, there) if t))
 
 
 class DiffAttention(torch.autograd.Function):

@@ -14,7 +14,7 @@
 //
 // Bound by memory: a row stays in registers between its reads and its writes, and what is the same for
 // all rows of a sample (modulation and weights, folded) is in registers for a run of rows.
-// A row belongs to G lanes of a wave (a power of 2, up to C = 1024) or to a whole block; a block has R
+// A row belongs to G lanes of a wave (a power of 2) or to a whole block; a block has R
 // rows one after the other, through as many samples as those rows touch.  Means and variances are taken
 // in two steps from the registers, so that a spread beside a large mean keeps its bits.  r is not
 // rounded before its own norm, and the gradient makes it again from x and y instead of reading it
@@ -32,9 +32,10 @@
 namespace tsc {
 namespace {
 
-constexpr int kWaveC = 1024;    // widest row of one wave
+constexpr int kLaneF = 16, kLaneB = 8;  // most values of a wave's lane, forward and backward: wider rows have a block
+constexpr int kBackThreads = 512;  // threads of a block of the gradient, where a row has lanes of a wave
 constexpr int kMaxC = 8192;     // widest row of a block of 16 waves
-constexpr int kSumCols = 16, kSumRows = 64;  // threads of a block that adds up the slots
+constexpr int kSumCols = 16, kSumRows = 64, kSumWaves = kSumCols * kSumRows / 64;  // of a block that adds up slots
 constexpr int kLoopB = 16;      // samples that one block of that kernel walks
 
 struct GnArgs {
@@ -312,7 +313,8 @@ __device__ __forceinline__ void flush(const GnArgs& a, const Team<MAXV, BLOCK>& 
 #pragma unroll
         for (int e = 0; e < VN; ++e) out[(team.lane + team.G * k) * VN + e] = s[k][e];
   } else {
-    __shared__ float meet[4][64 * MAXV * VN];
+    constexpr int NW = kBackThreads / 64;
+    __shared__ float meet[NW][64 * MAXV * VN];
     for (int off = 32; off >= team.G; off >>= 1)
 #pragma unroll
       for (int k = 0; k < MAXV; ++k)
@@ -326,15 +328,19 @@ __device__ __forceinline__ void flush(const GnArgs& a, const Team<MAXV, BLOCK>& 
 #pragma unroll
         for (int e = 0; e < VN; ++e) meet[w][(k * VN + e) * 64 + l] = s[k][e];
     __syncthreads();
-    for (int c = threadIdx.x; c < a.C; c += 256) {
+    for (int c = threadIdx.x; c < a.C; c += kBackThreads) {
       const int vec = c / VN, at = (vec / team.G * VN + c % VN) * 64 + vec % team.G;
-      out[c] = (meet[0][at] + meet[1][at]) + (meet[2][at] + meet[3][at]);
+      float t = meet[0][at];
+#pragma unroll
+      for (int x = 1; x < NW; ++x) t += meet[x][at];
+      out[c] = t;
     }
   }
 }
 
-template <typename T, int VN, int MAXV, bool BLOCK, bool Y, bool H>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 256) gated_norm_backward_kernel(const GnArgs a) {
+// NT: threads of a block at most.  Rows of more than 4096 values, whose blocks have 1024, spill registers.
+template <typename T, int VN, int MAXV, bool BLOCK, int NT, bool Y, bool H>
+__global__ void __launch_bounds__(NT) gated_norm_backward_kernel(const GnArgs a) {
   Team<MAXV, BLOCK> team(a.G);
   const int lane = team.lane, G = team.G, C = a.C, nvec = C / VN;
   const int64_t end = min(a.N, ((int64_t)blockIdx.x + 1) * a.R);
@@ -378,19 +384,22 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) gated_norm_backward_kernel
       }
     }
     float P[MAXV][VN] = {}, Q[MAXV][VN] = {}, Py[MAXV][VN] = {}, Qy[MAXV][VN] = {};
-    const int64_t first = row0 + team.first;
-    for (int64_t lead = row0, row = first; lead < stop; lead += team.step, row += team.step) {
+    Cols<T, VN, MAXV> xc, yc, dhc, drc;  // the next row's, on their way
+    float2 ysn = make_float2(0.f, 1.f), rsn = make_float2(0.f, 1.f);
+    auto load = [&](int64_t row) {
+      if (row >= stop) return;
+      if (H) xc.load((const T*)a.x + row * C, lane, G, nvec);
+      if (Y) yc.load((const T*)a.y + row * C, lane, G, nvec);
+      if (H) dhc.load((const T*)a.dh + row * C, lane, G, nvec);
+      if (a.dr) drc.load((const T*)a.dr + row * C, lane, G, nvec);
+      if (Y && a.post != TSC_NORM_NONE) ysn = a.ystat[row];
+      if (H) rsn = a.rstat[row];
+    };
+    load(row0 + team.first);
+    for (int64_t lead = row0, row = row0 + team.first; lead < stop; lead += team.step, row += team.step) {
       const bool live = row < stop;
-      Cols<T, VN, MAXV> xc, yc, dhc, drc;
-      float2 ys = make_float2(0.f, 1.f), rst = make_float2(0.f, 1.f);
-      if (live) {
-        if (H) xc.load((const T*)a.x + row * C, lane, G, nvec);
-        if (Y) yc.load((const T*)a.y + row * C, lane, G, nvec);
-        if (H) dhc.load((const T*)a.dh + row * C, lane, G, nvec);
-        if (a.dr) drc.load((const T*)a.dr + row * C, lane, G, nvec);
-        if (Y && a.post != TSC_NORM_NONE) ys = a.ystat[row];
-        if (H) rst = a.rstat[row];
-      }
+      const float2 ys = ysn, rst = rsn;
+      const Cols<T, VN, MAXV> dr = drc;
       float y[MAXV][VN], x[MAXV][VN], d[MAXV][VN], s2[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < MAXV; ++k) {
@@ -412,6 +421,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) gated_norm_backward_kernel
           }
         }
       }
+      load(row + team.step);
       if (H) {
         team.sum(s2);
         const float m1 = a.norm == TSC_NORM_LAYER ? s2[0] * a.inv_c : 0.f, m2 = s2[1] * a.inv_c;
@@ -425,7 +435,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) gated_norm_backward_kernel
         for (int k = 0; k < MAXV; ++k)
 #pragma unroll
           for (int e = 0; e < VN; ++e)
-            if (live && lane + G * k < nvec) d[k][e] += (float)drc.v[k].v[e];
+            if (live && lane + G * k < nvec) d[k][e] += (float)dr.v[k].v[e];
       }
       // d: the gradient of r
       if (live) {
@@ -499,11 +509,37 @@ __device__ __forceinline__ void put(void* p, int64_t i, double v) {
   if (p) ((T*)p)[i] = (T)(float)v;
 }
 
+// Adds up v over a block's rows of threads: in a wave, then over the waves.  Row 0 of threads has the sums.
+template <int N>
+__device__ __forceinline__ void sum_rows(double (&v)[N], double (*meet)[kSumWaves][kSumCols], int tc) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 32; off >= kSumCols; off >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off, 64);
+  __syncthreads();  // the last sums have been read
+  if (lane < kSumCols)
+#pragma unroll
+    for (int i = 0; i < N; ++i) meet[i][w][tc] = v[i];
+  __syncthreads();
+  if (w == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      double t = 0.;
+#pragma unroll
+      for (int x = 0; x < kSumWaves / 4; ++x) t += meet[i][4 * x + lane / kSumCols][tc];
+#pragma unroll
+      for (int off = 32; off >= kSumCols; off >>= 1) t += __shfl_xor(t, off, 64);
+      v[i] = t;
+    }
+}
+
 // Sums over a sample's slots, 16 columns by 64 slots at a time, merged in fp64.  Grid y = 1: all samples,
 // one after the other, and the weights' gradients; else one sample each, whose parts of those go to `total`.
-template <typename T>
+// NS: a.sums.
+template <typename T, int NS>
 __global__ void __launch_bounds__(kSumCols* kSumRows) gated_norm_sums_kernel(const SumArgs a) {
-  __shared__ double meet[kSumRows][kSumCols];
+  __shared__ double meet[NS][kSumWaves][kSumCols];
   const int tc = threadIdx.x % kSumCols, tr = threadIdx.x / kSumCols, c = blockIdx.x * kSumCols + tc;
   const bool in = c < a.C, alone = gridDim.y == 1;
   double weights[4] = {0., 0., 0., 0.};
@@ -514,37 +550,30 @@ __global__ void __launch_bounds__(kSumCols* kSumRows) gated_norm_sums_kernel(con
       hi = min<int64_t>(max<int64_t>(a.cu[b + 1], lo), a.N);
     }
     const int64_t t0 = lo / a.R, t1 = hi > lo ? (hi - 1) / a.R + 1 : t0;  // blocks of these rows
-    double s[4] = {0., 0., 0., 0.};
-    for (int i = 0; i < a.sums; ++i) {
-      double v = 0.;
-      if (in)
-        for (int64_t t = t0 + tr; t < t1; t += kSumRows) v += (double)a.part[((t + b) * a.sums + i) * a.C + c];
-      __syncthreads();
-      meet[tr][tc] = v;
-      __syncthreads();
-      for (int half = kSumRows / 2; half > 0; half >>= 1) {
-        if (tr < half) meet[tr][tc] += meet[tr + half][tc];
-        __syncthreads();
-      }
-      s[i] = meet[0][tc];
-    }
+    double s[NS] = {};
+    if (in)
+#pragma unroll 4
+      for (int64_t t = t0 + tr; t < t1; t += kSumRows)
+#pragma unroll
+        for (int i = 0; i < NS; ++i) s[i] += (double)a.part[((t + b) * NS + i) * a.C + c];
+    sum_rows<NS>(s, meet, tc);
     if (!in || tr) continue;
     const int64_t at = (int64_t)b * a.C + c;
-    int i = 0;
     double part[4] = {0., 0., 0., 0.};
-    if (a.h) {
-      const double P = s[0], Q = s[1], f = 1. + (double)at_or<T>(a.scale, b * a.lds + c, 0.f);
+    if (NS > 1 && a.h) {
+      const double P = s[0], Q = s[NS > 1], f = 1. + (double)at_or<T>(a.scale, b * a.lds + c, 0.f);
       put<T>(a.dscale, at, (double)at_or<T>(a.w, c, 1.f) * P + (a.bias ? (double)at_or<T>(a.bias, c, 0.f) * Q : 0.));
       put<T>(a.dshift, at, Q);
       part[0] = f * P;
       part[1] = f * Q;
-      i = 2;
     }
     if (a.y) {
-      const double P = s[i], Q = a.sums > i + 1 ? s[i + 1] : 0., g = at_or<T>(a.gate, b * a.ldg + c, 1.f);
+      constexpr int A = NS > 2 ? 2 : 0;  // with h's two sums before them
+      const double P = s[A], Q = NS % 2 ? 0. : s[NS - 1];
+      const double gate = at_or<T>(a.gate, b * a.ldg + c, 1.f);
       put<T>(a.dgate, at, (double)at_or<T>(a.pw, c, 1.f) * P + (a.pb ? (double)at_or<T>(a.pb, c, 0.f) * Q : 0.));
-      part[2] = g * P;
-      part[3] = g * Q;
+      part[2] = gate * P;
+      part[3] = gate * Q;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -563,62 +592,60 @@ __global__ void __launch_bounds__(kSumCols* kSumRows) gated_norm_sums_kernel(con
 // The weights' gradients of more than kLoopB samples.
 template <typename T>
 __global__ void __launch_bounds__(kSumCols* kSumRows) gated_norm_weights_kernel(const SumArgs a) {
-  __shared__ double meet[kSumRows][kSumCols];
+  __shared__ double meet[4][kSumWaves][kSumCols];
   const int tc = threadIdx.x % kSumCols, tr = threadIdx.x / kSumCols, c = blockIdx.x * kSumCols + tc;
-  void* out[4] = {a.dw, a.dbias, a.dpw, a.dpb};
+  double v[4] = {0., 0., 0., 0.};
+  if (c < a.C)
+    for (int b = tr; b < a.B; b += kSumRows)
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (!out[j]) continue;  // uniform
-    double v = 0.;
-    if (c < a.C)
-      for (int b = tr; b < a.B; b += kSumRows) v += a.total[((int64_t)b * 4 + j) * a.C + c];
-    __syncthreads();
-    meet[tr][tc] = v;
-    __syncthreads();
-    for (int half = kSumRows / 2; half > 0; half >>= 1) {
-      if (tr < half) meet[tr][tc] += meet[tr + half][tc];
-      __syncthreads();
-    }
-    if (c < a.C && tr == 0) put<T>(out[j], c, meet[0][tc]);
+      for (int j = 0; j < 4; ++j) v[j] += a.total[((int64_t)b * 4 + j) * a.C + c];
+  sum_rows<4>(v, meet, tc);
+  if (c < a.C && tr == 0) {
+    put<T>(a.dw, c, v[0]);
+    put<T>(a.dbias, c, v[1]);
+    put<T>(a.dpw, c, v[2]);
+    put<T>(a.dpb, c, v[3]);
   }
 }
 
 // ------------------------------------------------------------------------------- host
 struct Shape {
   bool block;
+  int vn, maxv;          // values of a vector, vectors of a lane
   int G, threads, rows;  // lanes of a row, threads of a block, rows a step of it covers
 };
-Shape shape_of(int32_t C, int vn, int per_lane) {
+Shape shape_of(int32_t C, int vn, int lane_values, int threads) {
   const int nvec = C / vn;
-  if (C <= kWaveC) {
+  if (C <= 64 * lane_values) {
     int g = 1;
     while (g < 64 && g < nvec) g *= 2;
-    return {false, g, 256, 256 / g};
+    return {false, vn, nvec <= 64 ? 1 : lane_values / vn, g, threads, threads / g};
   }
-  const int lanes = (nvec + per_lane / vn - 1) / (per_lane / vn);
-  const int threads = (lanes + 63) / 64 * 64;
-  return {true, threads, threads, 1};
+  const int maxv = 8 / vn;
+  threads = ((nvec + maxv - 1) / maxv + 63) / 64 * 64;
+  return {true, vn, maxv, threads, threads, 1};
 }
 // Rows of a block: as many blocks as `most` where there are enough rows.
 int64_t rows_of(const Shape& s, int64_t N, int64_t most) {
   const int64_t steps = (N + s.rows - 1) / s.rows;
   return s.rows * std::max<int64_t>(1, (steps + most - 1) / most);
 }
-constexpr int64_t kForwardBlocks = 2048, kBackwardBlocks = 1024;
+constexpr int64_t kForwardBlocks = 2048;
+// Waves of the gradient: as many as run at once (more leave more sums to add up).
+constexpr int64_t kBackwardWaves = 4096;
+int64_t back_blocks(const Shape& s) { return kBackwardWaves * 64 / s.threads; }
 
 // A step's rows and with them the slots do not depend on the alignment: the scratch has room for both.
 int64_t slots_of(int32_t dtype, int32_t B, int64_t N, int32_t C) {
-  const int vn = dtype == TSC_F32 ? 4 : 8;
   int64_t most = 0;
-  for (int v : {vn, 1}) {
-    if (C % v) continue;
-    const int64_t r = rows_of(shape_of(C, v, 8), N, kBackwardBlocks);
+  for (int v : {8, 4, 1}) {
+    if (C % v || (v == 8 && dtype == TSC_F32)) continue;
+    const Shape s = shape_of(C, v, kLaneB, kBackThreads);
+    const int64_t r = rows_of(s, N, back_blocks(s));
     most = std::max(most, (N + r - 1) / r);
   }
   return most + B;
 }
-
-bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
 GnArgs args_of(const GatedNormArgs& x) {
   GnArgs a = {};
@@ -647,27 +674,34 @@ GnArgs args_of(const GatedNormArgs& x) {
   a.inv_c = 1.f / (float)x.C;
   return a;
 }
-// Whether rows and parameters can be read 16 bytes at a time.
-bool whole_vectors(const GatedNormArgs& x, int vn, std::initializer_list<const void*> rows) {
-  if (x.C % vn) return false;
-  for (const void* p : rows)
-    if (!aligned16(p)) return false;
-  for (const void* p : {x.x, x.y, x.post_weight, x.post_bias, x.weight, x.bias, x.gate, x.scale, x.shift})
-    if (!aligned16(p)) return false;
-  return !((x.gate && x.ld_gate % vn) || (x.scale && x.ld_scale % vn) || (x.shift && x.ld_shift % vn));
+// The widest vectors that rows and parameters divide into and are aligned to: 16 bytes, 8 in 16 bits, or one value.
+Shape shape_for(const GatedNormArgs& x, int lane_values, int threads,
+                std::initializer_list<const void*> rows) {
+  const int es = x.dtype == TSC_F32 ? 4 : 2;
+  for (int vn : {8, 4}) {
+    if (x.C % vn || vn * es > 16) continue;
+    bool fits = !((x.gate && x.ld_gate % vn) || (x.scale && x.ld_scale % vn) || (x.shift && x.ld_shift % vn));
+    for (const void* p : rows) fits &= (uintptr_t)p % (vn * es) == 0;
+    for (const void* p : {x.x, x.y, x.post_weight, x.post_bias, x.weight, x.bias, x.gate, x.scale, x.shift})
+      fits &= (uintptr_t)p % (vn * es) == 0;
+    if (fits) return shape_of(x.C, vn, lane_values, threads);
+  }
+  return shape_of(x.C, 1, lane_values, threads);
 }
 
-// Calls f(type, VN, MAXV, BLOCK) with the kernel's shape: vectors of 16 bytes or single values; 16 (8) values
-// a lane of a wave (of a block).
-template <typename F>
-void by_shape(int32_t dtype, bool vec, bool block, F f) {
+// Calls f(type, VN, MAXV, BLOCK) with the kernel's shape.
+template <int LANE, typename F>
+void by_shape(int32_t dtype, const Shape& s, F f) {
   auto with = [&](auto t, auto vn) {
     constexpr int VN = decltype(vn)::value;
-    if (block) f(t, vn, std::integral_constant<int, 8 / VN>(), std::true_type());
-    else f(t, vn, std::integral_constant<int, 16 / VN>(), std::false_type());
+    if (s.block) f(t, vn, std::integral_constant<int, 8 / VN>(), std::true_type());
+    else if (s.maxv == 1) f(t, vn, std::integral_constant<int, 1>(), std::false_type());
+    else f(t, vn, std::integral_constant<int, LANE / VN>(), std::false_type());
   };
   auto types = [&](auto t) {
-    if (vec) with(t, std::integral_constant<int, 16 / sizeof(decltype(t))>());
+    if constexpr (sizeof(decltype(t)) == 2)
+      if (s.vn == 8) return with(t, std::integral_constant<int, 8>());
+    if (s.vn == 4) with(t, std::integral_constant<int, 4>());
     else with(t, std::integral_constant<int, 1>());
   };
   if (dtype == TSC_BF16) types(__bf16());
@@ -688,14 +722,12 @@ int gated_norm_launch(tsc_ctx* ctx, const GatedNormArgs& x, float* stats, void* 
     a.ystat = post ? (float2*)stats : nullptr;
     a.rstat = h ? (float2*)stats + (post ? x.N : 0) : nullptr;
   }
-  const int vn = x.dtype == TSC_F32 ? 4 : 8;
-  const bool vec = whole_vectors(x, vn, {r, h});
-  const Shape s = shape_of(x.C, vec ? vn : 1, 8);
+  const Shape s = shape_for(x, kLaneF, 256, {r, h});
   a.G = s.G;
   a.R = rows_of(s, x.N, kForwardBlocks);
   const unsigned grid = (unsigned)((x.N + a.R - 1) / a.R);
   ProfScope p(ctx, "gated_norm");
-  by_shape(x.dtype, vec, s.block, [&](auto t, auto v, auto m, auto blk) {
+  by_shape<kLaneF>(x.dtype, s, [&](auto t, auto v, auto m, auto blk) {
     using T = decltype(t);
     constexpr int VN = decltype(v)::value, MAXV = decltype(m)::value;
     constexpr bool BLOCK = decltype(blk)::value;
@@ -727,22 +759,29 @@ int gated_norm_backward_launch(tsc_ctx* ctx, const GatedNormArgs& x, const float
   // Either part's sums where any is wanted: the kernel makes them all the same.
   a.sums = want_h || want_y ? (dh ? 2 : 0) + (x.y ? (x.post_bias ? 2 : 1) : 0) : 0;
   a.part = (float*)ws;
-  const int vn = x.dtype == TSC_F32 ? 4 : 8;
-  const bool vec = whole_vectors(x, vn, {dr, dh, g.dx, g.dy});
-  const Shape s = shape_of(x.C, vec ? vn : 1, 8);
+  const Shape s = shape_for(x, kLaneB, kBackThreads, {dr, dh, g.dx, g.dy});
   a.G = s.G;
-  a.R = rows_of(s, std::max<int64_t>(x.N, 1), kBackwardBlocks);
+  a.R = rows_of(s, std::max<int64_t>(x.N, 1), back_blocks(s));
   if (x.N > 0) {
     const unsigned grid = (unsigned)((x.N + a.R - 1) / a.R);
     ProfScope p(ctx, "gated_norm_backward");
-    by_shape(x.dtype, vec, s.block, [&](auto t, auto v, auto m, auto blk) {
+    by_shape<kLaneB>(x.dtype, s, [&](auto t, auto v, auto m, auto blk) {
       using T = decltype(t);
       constexpr int VN = decltype(v)::value, MAXV = decltype(m)::value;
       constexpr bool BLOCK = decltype(blk)::value;
-      auto* st = ctx->stream;
-      if (x.y && dh) gated_norm_backward_kernel<T, VN, MAXV, BLOCK, true, true><<<grid, s.threads, 0, st>>>(a);
-      else if (x.y) gated_norm_backward_kernel<T, VN, MAXV, BLOCK, true, false><<<grid, s.threads, 0, st>>>(a);
-      else gated_norm_backward_kernel<T, VN, MAXV, BLOCK, false, true><<<grid, s.threads, 0, st>>>(a);
+      auto run = [&](auto nt) {
+        constexpr int NT = decltype(nt)::value;
+        auto with = [&](auto y, auto hh) {
+          gated_norm_backward_kernel<T, VN, MAXV, BLOCK, NT, decltype(y)::value, decltype(hh)::value>
+              <<<grid, s.threads, 0, ctx->stream>>>(a);
+        };
+        if (x.y && dh) with(std::true_type(), std::true_type());
+        else if (x.y) with(std::true_type(), std::false_type());
+        else with(std::false_type(), std::true_type());
+      };
+      if constexpr (!BLOCK) run(std::integral_constant<int, kBackThreads>());
+      else if (s.threads <= 512) run(std::integral_constant<int, 512>());
+      else run(std::integral_constant<int, 1024>());
     });
   }
   if (a.sums) {
@@ -782,7 +821,13 @@ int gated_norm_backward_launch(tsc_ctx* ctx, const GatedNormArgs& x, const float
       using T = decltype(t);
       {
         ProfScope p(ctx, "gated_norm_sums");
-        gated_norm_sums_kernel<T><<<grid, kSumCols * kSumRows, 0, ctx->stream>>>(q);
+        auto sums = [&](auto ns) {
+          gated_norm_sums_kernel<T, decltype(ns)::value><<<grid, kSumCols * kSumRows, 0, ctx->stream>>>(q);
+        };
+        if (q.sums == 1) sums(std::integral_constant<int, 1>());
+        else if (q.sums == 2) sums(std::integral_constant<int, 2>());
+        else if (q.sums == 3) sums(std::integral_constant<int, 3>());
+        else sums(std::integral_constant<int, 4>());
       }
       if (!loop && weights) {
         ProfScope p(ctx, "gated_norm_weights");

@@ -43,7 +43,8 @@ def _dev(*ts) -> int:
 
 
 def _p(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    """A buffer's address as the C calls take it (an int where c_void_p is declared)."""
+    return None if t is None else t.data_ptr()
 
 
 def _wrote(out: torch.Tensor | None) -> None:
@@ -280,6 +281,8 @@ def _wants_grad(*ts) -> bool:
 
 def _no_tangents(what: str, *ts) -> None:
     """Refuses dual tensors: these ops have no forward-mode derivative, and would drop the tangent."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual level is open
+        return
     if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
         raise TscError(_lib.TSC_ERR_UNSUPPORTED, f"{what}: no forward-mode derivative (dual tensor)")
 
@@ -363,19 +366,20 @@ def _group_norm_backward(dy, x, weight, bias, cu, b, groups, silu, stats, want_p
 
 def _modulation(t, name: str, b: int, c: int, dtype):
     """A (B, C) tensor whose rows may be strided: a gate, a scale or a shift of each sample."""
-    if t is not None and (t.shape != (b, c) or t.dtype != dtype):
+    if t.shape != (b, c) or t.dtype != dtype:
         raise TscError(_lib.TSC_ERR_INVALID, f"{name} must be ({b}, {c}) of x's dtype, got {tuple(t.shape)} {t.dtype}")
-    if t is not None and (t.stride(1) != 1 and c > 1 or t.stride(0) < c and b > 1):
+    if t.stride(1) != 1 and c > 1 or t.stride(0) < c and b > 1:
         raise TscError(_lib.TSC_ERR_INVALID, f"{name}: each sample's {c} values must be contiguous")
 
 
-def _gated_norm_args(what: str, x, y, cu_rows, post, gate, residual_scale, pre, scale, shift, eps, outs):
+def _gated_norm_args(what: str, x, y, cu_rows, post, gate, residual_scale, pre, scale, shift, eps, out=None):
     """Checks what the norms around a block are given; (tensors, arguments) of _gated_norm.  post and pre:
     (kind, weight, bias), kind None where there is none."""
     if x.dim() != 2 or x.shape[1] == 0:
         raise TscError(_lib.TSC_ERR_INVALID, f"{what}: x must be (N, C)")
     n, c = x.shape
-    if y is not None and (y.shape != x.shape or y.dtype != x.dtype):
+    dtype = x.dtype
+    if y is not None and (y.shape != x.shape or y.dtype != dtype):
         raise TscError(_lib.TSC_ERR_INVALID, f"{what}: y must have x's shape and dtype")
     for name, (kind, w, b) in (("post_norm", post), ("norm", pre)):
         if kind not in _lib.NORMS:
@@ -383,33 +387,34 @@ def _gated_norm_args(what: str, x, y, cu_rows, post, gate, residual_scale, pre, 
         if kind is None and (w is not None or b is not None):
             raise TscError(_lib.TSC_ERR_INVALID, f"{what}: a weight or bias needs a {name}")
         for t in (w, b):
-            if t is not None and (t.shape != (c,) or t.dtype != x.dtype):
+            if t is not None and (t.shape != (c,) or t.dtype != dtype):
                 raise TscError(_lib.TSC_ERR_INVALID, f"{what}: weights and biases must be ({c},) of x's dtype")
-    for out in outs:
-        if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
-            raise TscError(_lib.TSC_ERR_INVALID, f"{what}: out has the wrong shape or dtype")
+    if out is not None and (out.shape != x.shape or out.dtype != dtype):
+        raise TscError(_lib.TSC_ERR_INVALID, f"{what}: out has the wrong shape or dtype")
     _code(x)
     eps, residual_scale = float(eps), float(residual_scale)
-    if not 0 <= ctypes.c_float(eps).value < float("inf"):
+    if not 0 <= eps < 3.4e38:
         raise TscError(_lib.TSC_ERR_INVALID, f"{what}: eps must be >= 0 and finite")
-    if not abs(ctypes.c_float(residual_scale).value) < float("inf"):
+    if not -3.4e38 < residual_scale < 3.4e38:
         raise TscError(_lib.TSC_ERR_INVALID, f"{what}: residual_scale must be finite in fp32")
     tensors = (x, y, post[1], post[2], gate, pre[1], pre[2], scale, shift)
-    _no_tangents(what, *tensors, *outs)
+    _no_tangents(what, *tensors, out)
     if isinstance(cu_rows, torch.Tensor):
         b = cu_rows.numel() - 1
     else:
         b = 1 if cu_rows is None else len(cu_rows) - 1
     for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
-        _modulation(t, f"{what}: {name}", b, c, x.dtype)
-    dev = _dev(x, y, *post[1:], *pre[1:], *outs)
+        if t is not None:
+            _modulation(t, f"{what}: {name}", b, c, dtype)
+    dev = _dev(x, y, *post[1:], *pre[1:], out)
     for t in (gate, scale, shift):
         if t is not None and (not t.is_cuda or t.device.index != dev):
             raise TscError(_lib.TSC_ERR_INVALID, "tensors are not on one GPU; this path has no CPU fallback")
     cu = None
     if cu_rows is not None:
         _, cu = _cu_seqlens(cu_rows, n, dev, "cu_rows")
-        _dev(x, cu)
+        if cu.device.index != dev:
+            raise TscError(_lib.TSC_ERR_INVALID, "tensors live on different devices")
     if b and c > 8192:
         raise TscError(_lib.TSC_ERR_UNSUPPORTED, f"{what}: C={c} exceeds 8192")
     return tensors, (cu, b, _lib.NORMS[post[0]], _lib.NORMS[pre[0]], residual_scale, eps)
@@ -430,7 +435,7 @@ def modulated_norm(x: torch.Tensor, cu_rows=None, scale=None, shift=None, norm: 
     if norm is None:
         raise TscError(_lib.TSC_ERR_INVALID, "modulated_norm: norm must be 'layer' or 'rms', got None")
     tensors, args = _gated_norm_args("modulated_norm", x, None, cu_rows, (None, None, None), None, 1.0,
-                                     (norm, weight, bias), scale, shift, eps, (out,))
+                                     (norm, weight, bias), scale, shift, eps, out)
     return _gated_norm_entry("modulated_norm", tensors, args, False, True, out)[1]
 
 
@@ -444,7 +449,7 @@ def gated_residual(x: torch.Tensor, y: torch.Tensor, cu_rows=None, gate=None, re
     x, y (N, C); gate (B, C) of the samples that cu_rows gives, rows may be strided; post_norm None (y as
     it is), "layer" or "rms".  Otherwise as modulated_norm; out may be x or y."""
     tensors, args = _gated_norm_args("gated_residual", x, y, cu_rows, (post_norm, post_weight, post_bias),
-                                     gate, residual_scale, (None, None, None), None, None, eps, (out,))
+                                     gate, residual_scale, (None, None, None), None, None, eps, out)
     return _gated_norm_entry("gated_residual", tensors, args, True, False, out)[0]
 
 
@@ -458,7 +463,7 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor, cu_rows=None, gate=Non
         raise TscError(_lib.TSC_ERR_INVALID, "gated_residual_norm: norm must be 'layer' or 'rms', got None")
     tensors, args = _gated_norm_args("gated_residual_norm", x, y, cu_rows,
                                      (post_norm, post_weight, post_bias), gate, residual_scale,
-                                     (norm, weight, bias), scale, shift, eps, ())
+                                     (norm, weight, bias), scale, shift, eps)
     return _gated_norm_entry("gated_residual_norm", tensors, args, True, True, None)
 
 
@@ -468,7 +473,8 @@ def _gated_norm_entry(what, tensors, args, want_r, want_h, out):
             raise TscError(_lib.TSC_ERR_INVALID, f"{what}: out cannot be given where gradients are wanted")
         from .autograd import GatedNorm
 
-        got = GatedNorm.apply(*tensors, args, want_r, want_h)
+        there = tuple(t is not None for t in tensors)
+        got = GatedNorm.apply((args, there, want_r, want_h), *(t for t in tensors if t is not None))
         return got if want_r and want_h else (got, got)
     return _gated_norm(tensors, args, want_r, want_h, out, False)[:2]
 
@@ -478,12 +484,9 @@ def _gated_norm_call(tensors, args):
     x, y, pw, pb, gate, w, bias, scale, shift = tensors
     cu, b, post, pre, residual_scale, eps = args
     n, c = x.shape
-
-    def rows(t):
-        return _p(t), 0 if t is None else t.stride(0) if b > 1 else c
-
-    return (_code(x), _p(x), _p(y), _p(cu), b, n, c, post, _p(pw), _p(pb), *rows(gate), residual_scale,
-            pre, _p(w), _p(bias), *rows(scale), *rows(shift), eps)
+    ldg, lds, ldt = (0 if t is None else t.stride(0) if b > 1 else c for t in (gate, scale, shift))
+    return (_code(x), x.data_ptr(), _p(y), _p(cu), b, n, c, post, _p(pw), _p(pb), _p(gate), ldg, residual_scale,
+            pre, _p(w), _p(bias), _p(scale), lds, _p(shift), ldt, eps)
 
 
 def _gated_norm(tensors, args, want_r, want_h, out, keep):
@@ -494,42 +497,36 @@ def _gated_norm(tensors, args, want_r, want_h, out, keep):
     r = (out if out is not None else new(x)) if want_r else None
     h = (out if out is not None and not want_r else new(x)) if want_h else None
     norms = int(want_h) + int(y is not None and post != _lib.TSC_NORM_NONE)
-    stats = torch.empty((norms, n, 2), dtype=torch.float32, device=x.device) if keep else None
+    stats = torch.empty((norms, n, 2), dtype=torch.float32, device=x.device) if keep and norms else None
     if n and b:
         lib, handle = _lib.stream_handle(x.device.index)
-        check(lib.tsc_gated_norm(handle, *_gated_norm_call(tensors, args), int(out is None),
-                                 _p(stats) if norms else None, _p(r), _p(h)))
+        check(lib.tsc_gated_norm(handle, *_gated_norm_call(tensors, args), int(out is None), _p(stats), _p(r),
+                                 _p(h)))
         _wrote(out)
     return r, h, stats
 
 
 def _gated_norm_backward(tensors, args, stats, dr, dh, wanted):
-    """The gradients of `tensors` (None where `wanted` says so)."""
-    x, y, pw, pb, gate, w, bias, scale, shift = tensors
+    """The gradients of `tensors`, None where there is none or `wanted` says so."""
+    x, y = tensors[:2]
     b = args[1]
     n, c = x.shape
     if n == 0:
         return [None if t is None else torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
-    dx = torch.empty_like(x)
-    dy = None if y is None else torch.empty_like(x)
-    there = (True, y is not None) + 3 * (y is not None,) + 4 * (dh is not None,)
-
-    def new(i, *shape):
-        t = tensors[i]
-        return torch.empty(shape, dtype=x.dtype, device=x.device) if t is not None and wanted[i] and there[i] else None
-
-    dpw, dpb, dgate, dw, db, dscale, dshift = (new(2, c), new(3, c), new(4, b, c), new(5, c), new(6, c),
-                                               new(7, b, c), new(8, b, c))
+    # Without dh the norm before the next block has no gradient, and neither has its modulation.
+    grads = [None if t is None or not w else
+             torch.empty(t.shape, dtype=x.dtype, device=x.device) if dh is not None or i < 5 else
+             torch.zeros(t.shape, dtype=x.dtype, device=x.device)
+             for i, (t, w) in enumerate(zip(tensors, wanted))]
+    dx, dy, dpw, dpb, dgate, dw, db, dscale, dshift = grads if dh is not None else grads[:5] + 4 * [None]
+    dx = torch.empty_like(x) if dx is None else dx
+    if y is not None and dy is None:
+        dy = torch.empty_like(x)
     lib, handle = _lib.stream_handle(x.device.index)
-    nbytes = lib.tsc_gated_norm_workspace_bytes(_code(x), b, n, c)
-    ws = _scratch(nbytes, x.device)
+    ws = _scratch(lib.tsc_gated_norm_workspace_bytes(_code(x), b, n, c), x.device)
     check(lib.tsc_gated_norm_backward(handle, *_gated_norm_call(tensors, args), 1, _p(stats), _p(dr),
-                                      _p(dh), _p(ws), _p(dx), _p(dy), _p(dgate), _p(dpw), _p(dpb),
+                                      _p(dh), ws.data_ptr(), dx.data_ptr(), _p(dy), _p(dgate), _p(dpw), _p(dpb),
                                       _p(dscale), _p(dshift), _p(dw), _p(db)))
-    grads = [dx, dy, dpw, dpb, dgate, dw, db, dscale, dshift]
-    for i, t in enumerate(tensors):  # of a part whose output has no gradient
-        if t is not None and wanted[i] and grads[i] is None:
-            grads[i] = torch.zeros(t.shape, dtype=t.dtype, device=t.device)
     return grads
 
 
@@ -889,8 +886,7 @@ def sparse_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
         raise TscError(_lib.TSC_ERR_INVALID, "window_attention: out has the wrong shape or dtype")
     _code(q)
     _no_tangents("window_attention", q, k, v, out)
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _head_rows(t, name)
+    lds = (_head_rows(q, "q"), _head_rows(k, "k"), _head_rows(v, "v"))
     dev = _dev(out)
     for t in (q, k, v):
         if not t.is_cuda or dev is not None and t.device.index != dev:
@@ -911,7 +907,7 @@ def sparse_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
         raise TscError(_lib.TSC_ERR_INVALID, "cu_seqlens_q and cu_seqlens_kv differ in length")
     b = cq.numel() - 1
     args = (cq, ck, b, float(scale) if scale is not None else 0.0, window, sinks, int(bool(causal)),
-            _longest(max_seqlen_q, cq_host, tq, b), _longest(max_seqlen_kv, ck_host, tkv, b))
+            _longest(max_seqlen_q, cq_host, tq, b), _longest(max_seqlen_kv, ck_host, tkv, b), lds)
     if _wants_grad(q, k, v, out):
         if out is not None:
             raise TscError(_lib.TSC_ERR_INVALID, "window_attention: out cannot be given where gradients "
@@ -934,7 +930,7 @@ def _longest(given, host, total: int, b: int) -> int:
 
 def _window_attention(q, k, v, args, out, keep):
     """(out, lo, lse); lo and lse (None unless keep) are what the backward pass needs."""
-    cq, ck, b, scale, window, sinks, causal, max_q, max_kv = args
+    cq, ck, b, scale, window, sinks, causal, max_q, max_kv, lds = args
     tq, h, d = q.shape
     tkv, hk = k.shape[:2]
     rest = out is None
@@ -944,20 +940,20 @@ def _window_attention(q, k, v, args, out, keep):
     lse = torch.empty((tq, h), dtype=torch.float32, device=q.device) if keep else None
     if tq and b:
         lib, handle = _lib.stream_handle(q.device.index)
-        nbytes = lib.tsc_window_attention_workspace_bytes(_code(q), b, tq, tkv, h, hk, d, window, sinks, causal,
-                                                          max_q, max_kv, 0)
+        code = _code(q)
+        nbytes = lib.tsc_window_attention_workspace_bytes(code, b, tq, tkv, h, hk, d, window, sinks, causal, max_q,
+                                                          max_kv, 0)
         ws = _scratch(nbytes, q.device) if nbytes else None
-        check(lib.tsc_window_attention(handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"),
-                                       _head_rows(k, "k"), _head_rows(v, "v"), _p(cq), _p(ck), b, tq, tkv, h,
-                                       hk, d, scale, window, sinks, causal, max_q, max_kv, int(rest), _p(ws),
-                                       _p(out), _p(lo), _p(lse)))
+        check(lib.tsc_window_attention(handle, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), *lds, cq.data_ptr(),
+                                       ck.data_ptr(), b, tq, tkv, h, hk, d, scale, window, sinks, causal, max_q,
+                                       max_kv, int(rest), _p(ws), out.data_ptr(), _p(lo), _p(lse)))
         if not rest:
             _wrote(out)
     return out, lo, lse
 
 
 def _window_attention_backward(do, q, k, v, out, lo, lse, args):
-    cq, ck, b, scale, window, sinks, causal, max_q, max_kv = args
+    cq, ck, b, scale, window, sinks, causal, max_q, max_kv, lds = args
     tq, h, d = q.shape
     tkv, hk = k.shape[:2]
     alloc = torch.empty if b else torch.zeros
@@ -965,13 +961,13 @@ def _window_attention_backward(do, q, k, v, out, lo, lse, args):
     dk, dv = (alloc((tkv, hk, d), dtype=q.dtype, device=q.device) for _ in range(2))
     if b and (tq or tkv):
         lib, handle = _lib.stream_handle(q.device.index)
-        nbytes = lib.tsc_window_attention_workspace_bytes(_code(q), b, tq, tkv, h, hk, d, window, sinks, causal,
-                                                          max_q, max_kv, 1)
-        ws = _scratch(nbytes, q.device)
+        code = _code(q)
+        ws = _scratch(lib.tsc_window_attention_workspace_bytes(code, b, tq, tkv, h, hk, d, window, sinks, causal,
+                                                               max_q, max_kv, 1), q.device)
         check(lib.tsc_window_attention_backward(
-            handle, _code(q), _p(q), _p(k), _p(v), _head_rows(q, "q"), _head_rows(k, "k"), _head_rows(v, "v"),
-            _p(cq), _p(ck), b, tq, tkv, h, hk, d, scale, window, sinks, causal, max_q, max_kv, 1, _p(out),
-            _p(lo), _p(lse), _p(do), _p(ws), _p(dq), _p(dk), _p(dv)))
+            handle, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), *lds, cq.data_ptr(), ck.data_ptr(), b, tq, tkv,
+            h, hk, d, scale, window, sinks, causal, max_q, max_kv, 1, out.data_ptr(), _p(lo), lse.data_ptr(),
+            do.data_ptr(), ws.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()))
     return dq, dk, dv
 
 
