@@ -453,3 +453,22 @@ def test_gradient_of_a_view_and_of_one_leaf(pkg, dev):
     big[5:] = do.to(dev).flatten()
     g, = torch.autograd.grad(o, leaf, big[5:].view(90, 2, 64))
     assert torch.equal(g, want["dq"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lkv,sinks", [([2000], None, 1), ([1500, 0, 7, 40, 900], None, 37), ([900, 700], [1000, 900], 4),
+                                          ([2500, 20], None, 130), ([1200, 600], [1000, 30], 33)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_sinks_with_blocks_of_their_own(pkg, dev, dtype, d, lq, lkv, sinks, causal):
+    """Long sequences, short windows: the rows of the sinks are shared out, and sequences shorter than the
+    sinks, without queries, and lengths given too small still have theirs."""
+    h, hk, window = 4, 2, 20
+    ws = pkg.load_library().tsc_window_attention_workspace_bytes
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    most = (max(lq), max(lkv or lq))
+    sizes = (code, len(lq), sum(lq), sum(lkv or lq), h, hk, d, window)
+    assert ws(*sizes, sinks, int(causal), *most, 1) > ws(*sizes, 0, int(causal), *most, 1)
+    _both(pkg, dev, lq, lkv, h, hk, d, dtype, window, sinks, causal)
+    if lkv is None:
+        _both(pkg, dev, lq, lkv, h, hk, d, dtype, window, sinks, causal, max_seqlen_q=most[0], max_seqlen_kv=3 * sinks)

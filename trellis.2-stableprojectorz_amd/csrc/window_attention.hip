@@ -14,8 +14,8 @@
 // (one run where they meet); tiles that all rows see take no mask.
 // In the others a row and a key that do not see each other have P = 0, and dS = 0, by selection.  Their
 // product with a row of v (k; do, q in dk / dv) that holds an infinity or NaN would be NaN still: tiles with
-// masks look for those, take them as zeros, and add what they bring one row at a time with a selection
-// behind the product, so that who does not see them has the bits it would have without them.
+// masks look for those and take them as zeros, and a wave that met one adds them at the end to those of its
+// rows that see them, so that the others have the bits they would have without them.
 
 #include <float.h>
 
@@ -30,6 +30,7 @@ namespace {
 
 constexpr int kNT = 256;  // 4 waves of 32 rows (or keys, in dk / dv)
 constexpr int kBQ = 128;
+constexpr int kBQ16 = 256;  // rows of a block of the forward pass in 16 bits: 4 waves of 64 (D = 64) or 8 of 32
 constexpr int kBK = 32;   // keys of a tile
 
 struct WaArgs {
@@ -49,6 +50,10 @@ struct WaArgs {
   const void* dout;
   const float* r;  // (total_q, H)
   void *dq, *dk, *dv;
+  int32_t own_sinks;   // dk / dv blocks leave out the sinks, which have blocks and scratch of their own:
+  int32_t sink_keys;   // sinks of a sequence there is scratch for, whole tiles of 32
+  int32_t sink_parts;  // blocks that share a tile's rows
+  float* sink_sums;    // (parts, B, Hk, sink_keys, 2, D): dk without its scale, dv
 };
 
 // ---- rows, and what they see ----------------------------------------------------------------
@@ -73,7 +78,8 @@ __device__ __forceinline__ Seen seen_from(const WaArgs& a, int p, int keys) {
   return s;
 }
 
-// The key tiles of rows at positions p0 to p1.
+// The key tiles, of BK keys, of rows at positions p0 to p1.
+template <int BK>
 struct Walk {
   int n1, n2;       // tiles of the two runs
   int end1, lo, hi; // the first run is [0, end1), the second [lo, hi)
@@ -86,28 +92,30 @@ struct Walk {
     end1 = one ? max(last.hi, last.sink) : last.sink;
     lo = first.lo;
     hi = last.hi;
-    n1 = (end1 + kBK - 1) / kBK;
-    n2 = one || hi <= lo ? 0 : (hi - lo + kBK - 1) / kBK;
+    n1 = (end1 + BK - 1) / BK;
+    n2 = one || hi <= lo ? 0 : (hi - lo + BK - 1) / BK;
   }
   __device__ __forceinline__ int tiles() const { return n1 + n2; }
   __device__ __forceinline__ void tile(int t, int* at, int* end) const {
-    *at = t < n1 ? t * kBK : lo + (t - n1) * kBK;
+    *at = t < n1 ? t * BK : lo + (t - n1) * BK;
     *end = t < n1 ? end1 : hi;
   }
-  // Whether rows whose bounds are f (first) to l (last) see all of tile t; whether they see any of it.
-  __device__ __forceinline__ bool full(int t, const Seen& f, const Seen& l) const {
+  // Whether rows whose bounds are f (first) to l (last) see the first `keys` of tile t, all of which there
+  // are; whether they see any of `keys` keys of it.
+  __device__ __forceinline__ bool full(int t, const Seen& f, const Seen& l, int keys = BK) const {
     int at, end;
     tile(t, &at, &end);
-    if (at + kBK > end) return false;
-    const bool sinks = t < n1 && at + kBK <= f.sink;
-    const bool win = (one || t >= n1) && at >= l.lo && at + kBK <= f.hi;
+    if (at + keys > end) return false;
+    const bool sinks = t < n1 && at + keys <= f.sink;
+    const bool win = (one || t >= n1) && at >= l.lo && at + keys <= f.hi;
     return sinks || win;
   }
-  __device__ __forceinline__ bool any(int t, const Seen& f, const Seen& l) const {
+  __device__ __forceinline__ bool any(int t, const Seen& f, const Seen& l, int from = 0, int keys = BK) const {
     int at, end;
     tile(t, &at, &end);
+    at += from;
     const bool sinks = t < n1 && at < l.sink;
-    const bool win = (one || t >= n1) && at < l.hi && at + kBK > f.lo;
+    const bool win = (one || t >= n1) && at < l.hi && at + keys > f.lo;
     return sinks || win;
   }
   // A row's bounds within the run that tile t belongs to.
@@ -142,90 +150,84 @@ __device__ __forceinline__ uint32_t odd(const u32x4_t& f) {
   for (int i = 0; i < 4; ++i) r |= (f[i] & E) + L & 0x80008000u;
   return r;
 }
-// The elements of a fragment that are finite (or that are not), zeros for the others.
+// A fragment with zeros in the place of what is not finite.
 template <typename T>
-__device__ __forceinline__ F32x8 part(const F32x8& f, bool finite) {
+__device__ __forceinline__ F32x8 finite(const F32x8& f) {
   F32x8 r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r.v[i] = ((__float_as_uint(f.v[i]) & 0x7f800000u) != 0x7f800000u) == finite ? f.v[i] : 0.f;
+  for (int i = 0; i < 8; ++i) r.v[i] = (__float_as_uint(f.v[i]) & 0x7f800000u) != 0x7f800000u ? f.v[i] : 0.f;
   return r;
 }
 template <typename T>
-__device__ __forceinline__ u32x4_t part(const u32x4_t& f, bool finite) {
+__device__ __forceinline__ u32x4_t finite(const u32x4_t& f) {
   constexpr uint32_t E = std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
   u32x4_t r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t m = ((f[i] & E) != E ? 0xffffu : 0u) | ((f[i] >> 16 & E) != E ? 0xffff0000u : 0u);
-    r[i] = f[i] & (finite ? m : ~m);
-  }
-  return r;
-}
-// Element x of a fragment, zeros in its other places and where `on` is not set.
-__device__ __forceinline__ F32x8 only(const F32x8& f, int x, bool on) {
-  F32x8 r;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r.v[i] = on && i == x ? f.v[i] : 0.f;
-  return r;
-}
-__device__ __forceinline__ u32x4_t only(const u32x4_t& f, int x, bool on) {
-  u32x4_t r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = on && i == x >> 1 ? f[i] & (x & 1 ? 0xffff0000u : 0xffffu) : 0u;
+  for (int i = 0; i < 4; ++i)
+    r[i] = f[i] & (((f[i] & E) != E ? 0xffffu : 0u) | ((f[i] >> 16 & E) != E ? 0xffff0000u : 0u));
   return r;
 }
 
-// acc += sum over the 32 rows e of the tile of p[e] row_e, for those e that the lane's column sees.
-// pf: p as two fragments.  With masks: rows that are not finite go in one by one, and only where seen.
-template <typename T, int D, bool MASK, typename S>
+// acc += sum over the 32 rows e of the tile of p[e] row_e; pf: p as two fragments.  With masks, what is not
+// finite is left out, and met is set.
+template <typename T, int D, bool MASK>
 __device__ __forceinline__ void add_rows(const unsigned char* t, int lane, const typename Frag<T>::type (&pf)[2],
-                                         S see, f32x16_t (&acc)[D / 32]) {
+                                         f32x16_t (&acc)[D / 32], bool& met) {
   typedef Frag<T> F;
   typedef typename F::type Fr;
   typedef Tile<T, D> Ti;
   constexpr int MT = D / 32;
-  if constexpr (MASK) {
-    uint32_t bad = 0;
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
+  for (int g = 0; g < 2; ++g) {
+    Fr v[MT];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) bad |= odd<T>(Ti::col(t, 0, lane, g, mt));
-    if (__builtin_amdgcn_ballot_w64(bad != 0)) {
+    for (int mt = 0; mt < MT; ++mt) v[mt] = Ti::col(t, 0, lane, g, mt);
+    if constexpr (MASK) {
+      uint32_t bad = 0;
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
+      for (int mt = 0; mt < MT; ++mt) bad |= odd<T>(v[mt]);
+      if (__builtin_amdgcn_ballot_w64(bad != 0)) {
+        met = true;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) F::mma(part<T>(Ti::col(t, 0, lane, g, mt), true), pf[g], acc[mt]);
-      for (int e = 0; e < 32; ++e) {
-        const int g = e >> 4, x = 4 * ((e >> 3) & 1) + (e & 3);
-        const bool on = (lane >> 5) == ((e >> 2) & 1), seen = see(e);
-        const Fr p = only(g ? pf[1] : pf[0], x, on);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          f32x16_t one;
-          clear(one);
-          const Fr v = only(part<T>(Ti::col(t, 0, lane, g, mt), false), x, on);
-          if (!__builtin_amdgcn_ballot_w64(odd<T>(v) != 0)) continue;
-          F::mma(v, p, one);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) acc[mt][j] += seen ? one[j] : 0.f;
-        }
+        for (int mt = 0; mt < MT; ++mt) v[mt] = finite<T>(v[mt]);
       }
-      return;
     }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) F::mma(v[mt], pf[g], acc[mt]);
   }
+}
+// What such a row brings to a lane that sees it: a weight P > 0 times an infinity or NaN is that; dS of a
+// score that is not finite is 0 or NaN, and makes NaN of it (NANS).
+template <typename T, int D, bool NANS>
+__device__ __forceinline__ void add_odd(const T* row, int hf, bool seen, f32x16_t (&acc)[D / 32]) {
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
+  for (int mt = 0; mt < D / 32; ++mt)
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) F::mma(Ti::col(t, 0, lane, g, mt), pf[g], acc[mt]);
+    for (int j = 0; j < 16; ++j) {
+      const float v = (float)row[32 * mt + 8 * (j >> 2) + 4 * hf + (j & 3)];
+      if (seen && !(fabsf(v) < INFINITY)) acc[mt][j] += NANS ? NAN : v;
+    }
 }
 
 // ------------------------------------------------------------------------------- forward
+// add_odd for the keys of tiles t, t + step, .. below stop.
+template <typename T, int D, bool NANS, int BK>
+__device__ __forceinline__ void add_keys(const Walk<BK>& walk, const Seen& mine, int t, int stop, int step,
+                                         const T* base, int64_t ld, int hf, f32x16_t (&acc)[D / 32]) {
+  for (; t < stop; t += step) {
+    int at, end;
+    walk.tile(t, &at, &end);
+    const Seen s = walk.in_run(t, mine);
+    for (int k = at; k < min(at + BK, end); ++k) add_odd<T, D, NANS>(base + (int64_t)k * ld, hf, sees(s, k), acc);
+  }
+}
+
 // One tile of 32 keys from k0 on, in LDS, for a wave's 32 rows; s: what the lane's row sees of it.
 template <typename T, int D, bool MASK>
 __device__ __forceinline__ void forward_step(const unsigned char* kt, const unsigned char* vt, int lane,
                                              int k0, const Seen& s, float sl2,
                                              const typename Frag<T>::type (&qf)[D / 16], float& m,
-                                             float& l, f32x16_t (&o)[D / 32]) {
+                                             float& l, f32x16_t (&o)[D / 32], bool& met) {
   typedef Frag<T> F;
   typedef Tile<T, D> Ti;
   constexpr int KS = D / 16, MT = D / 32;
@@ -258,12 +260,12 @@ __device__ __forceinline__ void forward_step(const unsigned char* kt, const unsi
     l += p[j];
   }
   const typename F::type pf[2] = {F::pack(p), F::pack(p + 8)};
-  add_rows<T, D, MASK>(vt, lane, pf, [&](int e) { return sees(s, k0 + e); }, o);
+  add_rows<T, D, MASK>(vt, lane, pf, o, met);
 }
 
 // Writes a wave's finished rows: l summed over both halves, 0 where a row sees no key.
 template <typename T, int D>
-__device__ __forceinline__ void forward_store(const WaArgs& a, int64_t at, int hf, float m, float l,
+__device__ __forceinline__ void forward_store(const WaArgs& a, int64_t at, int hf, float l,
                                               f32x16_t (&o)[D / 32]) {
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
@@ -280,12 +282,15 @@ __device__ __forceinline__ void forward_store(const WaArgs& a, int64_t at, int h
       store_dims(p, hf, o[mt], inv);
     }
   }
+}
+__device__ __forceinline__ void store_lse(const WaArgs& a, int64_t at, int hf, float m, float l) {
   if (a.lse && hf == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
-// A block of 4 waves owns 128 rows and walks their keys in tiles of 32.
-template <typename T, int D>
-__global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward_kernel(const WaArgs a) {
+// fp32: a block of 4 waves owns 128 rows and walks their keys in tiles of 32.
+template <int D>
+__global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward32_kernel(const WaArgs a) {
+  typedef float T;
   typedef Frag<T> F;
   typedef Tile<T, D> Ti;
   constexpr int KS = D / 16, MT = D / 32;
@@ -312,12 +317,13 @@ __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward_kernel(const 
 #pragma unroll
       for (int st = 0; st < KS; ++st) qf[st] = F::load(p + 16 * st);
     }
-    const Walk walk(a, query_of(a, x0) + off, query_of(a, min(x0 + kBQ, n) - 1) + off, kv_len);
+    const Walk<kBK> walk(a, query_of(a, x0) + off, query_of(a, min(x0 + kBQ, n) - 1) + off, kv_len);
     const Seen mine = seen_from(a, query_of(a, x) + off, kv_len);
     const Seen wf = seen_from(a, query_of(a, min(x0 + w * 32, n - 1)) + off, kv_len);
     const Seen wl = seen_from(a, query_of(a, min(x0 + w * 32 + 31, n - 1)) + off, kv_len);
     const bool idle = x0 + w * 32 >= n;
     float m = -FLT_MAX, l = 0.f;  // a finite start: a tile of scores of -inf then adds nothing
+    bool met = false;
     f32x16_t o[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) clear(o[mt]);
@@ -341,14 +347,386 @@ __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward_kernel(const 
       load(t + 1);
       if (idle || !walk.any(t, wf, wl)) continue;
       if (walk.full(t, wf, wl)) {
-        forward_step<T, D, false>(kt, vt, lane, at, mine, a.sl2, qf, m, l, o);
+        forward_step<T, D, false>(kt, vt, lane, at, mine, a.sl2, qf, m, l, o, met);
       } else {
-        Seen s = walk.in_run(t, mine);
-        forward_step<T, D, true>(kt, vt, lane, at, s, a.sl2, qf, m, l, o);
+        forward_step<T, D, true>(kt, vt, lane, at, walk.in_run(t, mine), a.sl2, qf, m, l, o, met);
       }
     }
+    if (met) add_keys<T, D, false>(walk, mine, 0, nt, 1, vbase, a.ldv, hf, o);
     l = pair_sum(l);
-    if (live) forward_store<T, D>(a, q0 * (int64_t)H + row_at(a, H, h, x, 1), hf, m, l, o);
+    if (live) {
+      const int64_t at = q0 * (int64_t)H + row_at(a, H, h, x, 1);
+      forward_store<T, D>(a, at, hf, l, o);
+      store_lse(a, at, hf, m, l);
+    }
+  }
+}
+
+// 16 bits: one wave's softmax runs beside its matrix products.  A step of 32 keys has two phases, pinned in
+// program order (left to itself the compiler gathers the products):
+//   A  the next step's scores (matrix) beside the rest of this step's exponentials (VALU) and the transposed
+//      reads of v
+//   B  o += V^T P^T beside the next step's row maxima, the first half of its exponentials and the reads of k
+//      for the step after
+// Blocks of 64 keys come through LDS, k one block ahead of v (three buffers, two).  The longest run of them of
+// which all rows see everything goes so; in the others, at the window's ends, a wave does one thing after the
+// other, puts masks on the scores where it has to, and leaves out the keys of which its rows see nothing.
+// The sums of v are divided by the sum of the rounded P that they were made of.  KEEP (for the backward
+// pass) also adds up the unrounded P: the log-sum-exps have to be those of the fp32 probabilities.
+constexpr float kLazy = 8.f;  // log2 headroom before a running maximum is raised
+template <typename T, int D, int QT, int NW, bool KEEP>
+__global__ void __launch_bounds__(64 * NW, 2) wa_forward16_kernel(const WaArgs a) {
+  typedef Tile<T, D> Ti;
+  constexpr int BK = 64, NT = 64 * NW, BQ = 32 * NW * QT;
+  constexpr int CPR = Ti::CPR, ROWB = Ti::ROWB, KS = D / 16, MT = D / 32;
+  constexpr int RI = NT / CPR, NL = BK / RI;     // rows a load of the block covers; loads of a thread
+  constexpr int NA = KS * QT, NB = 2 * MT * QT;  // products of the two phases
+  static_assert(NL >= 1, "tile shape");
+  __shared__ __attribute__((aligned(16))) unsigned char kbuf[3][BK * ROWB], vbuf[2][BK * ROWB];
+  __shared__ uint32_t odd_in[2][NW];  // whether a wave's share of the v in vbuf holds what is not finite
+  int bx, h, bb;
+  block_tile(a.cu_kv, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  const int H = a.Hk * a.G, n = q_len * a.G, off = kv_len - q_len;
+  if (a.rest) zero_rest((T*)a.out, a.cu_q, a.total_q, bb, H, D, h * a.G, bx, gridDim.x, a.G);
+  const T* kbase = (const T*)a.k + (int64_t)kv0 * a.ldk + (int64_t)h * D;
+  const T* vbase = (const T*)a.v + (int64_t)kv0 * a.ldv + (int64_t)h * D;
+  const float sl2 = a.sl2;
+
+  for (int64_t rt = (int64_t)bx * BQ; rt < n; rt += (int64_t)gridDim.x * BQ) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // nothing derived from it is kept across row tiles
+    const int lane = tid & 63, l32 = lane & 31, hf = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int x0 = (int)rt, xw = x0 + 32 * QT * w;  // first row of the block, of the wave
+    const Walk<BK> walk(a, query_of(a, x0) + off, query_of(a, min(x0 + BQ, n) - 1) + off, kv_len);
+    const int nblk = walk.tiles();
+    const Seen wf = seen_from(a, query_of(a, min(xw, n - 1)) + off, kv_len);
+    const Seen wl = seen_from(a, query_of(a, min(xw + 32 * QT, n) - 1) + off, kv_len);
+    u32x4_t qf[QT][KS];
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      const int x = min(xw + 32 * i + l32, n - 1);
+      const T* p = (const T*)a.q + (int64_t)q0 * a.ldq + row_at(a, a.ldq, h, x, D) + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) qf[i][st] = *(const u32x4_t*)(p + 16 * st);
+    }
+    float mc[QT], l[QT], lu[QT], alpha[QT];  // mc: running maxima, times sl2
+    f32x16_t o[QT][MT], sa[QT], sb[QT];
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      mc[i] = -FLT_MAX;
+      l[i] = lu[i] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) clear(o[i][mt]);
+    }
+    auto row_sees = [&](int i) {  // the lane's row of tile i; made anew where it is needed, not kept in between
+      int x = xw + 32 * i + l32;
+      asm volatile("" : "+v"(x));
+      return seen_from(a, query_of(a, min(x, n - 1)) + off, kv_len);
+    };
+    bool met = false;  // a row of v that is not finite, in a block with masks
+    if (nblk > 0) {    // uniform over the block
+      const int srow = tid / CPR, sc = tid % CPR;  // staging: chunk sc of rows srow + RI * i
+      const uint32_t kst = (uint32_t)(2 * a.ldk), vst = (uint32_t)(2 * a.ldv);  // row bytes
+      // Block t's rows; rows past a run's last key repeat it, a block past the end is block 0: no row sees them.
+      u32x4_t kr[NL], vr[NL];
+      auto load = [&](const T* base, uint32_t rb, int t, u32x4_t(&r)[NL]) {
+        int at, end;
+        walk.tile(t < nblk ? t : 0, &at, &end);
+        const char* p = (const char*)base + (int64_t)at * rb;
+        const uint32_t lim = (uint32_t)min(end - 1 - at, BK - 1) * rb + 16u * sc;
+        const uint32_t o0 = (uint32_t)srow * rb + 16u * sc;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) r[i] = *(const u32x4_t*)(p + min(o0 + (uint32_t)(RI * i) * rb, lim));
+      };
+      int kb = 0;  // the buffer of the current block's k
+      auto later = [&](int by) { return kb + by < 3 ? kb + by : kb + by - 3; };
+      auto store = [&](int t) {  // v of block t + 1, k of block t + 2
+#pragma unroll
+        for (int i = 0; i < NL; ++i) Ti::put(vbuf[~t & 1], srow + RI * i, sc, vr[i]);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) Ti::put(kbuf[later(2)], srow + RI * i, sc, kr[i]);
+      };
+      u32x4_t kf[KS], vf[2][MT], pf[QT][2];
+      float pr[16 * QT];
+      // Tile's row and col with addresses made from one register each: chunk 2 st + hf of row l32 is kfrag ^ 32 st,
+      // and the piece of dim tile mt in rows 8 y + .. is vfrag ^ (64 mt ^ 32 y).
+      const int vr0 = 4 * hf + ((lane & 15) >> 2);
+      int kfrag = l32 * ROWB + ((hf ^ Ti::swz(l32)) << 4);
+      int vfrag = vr0 * ROWB + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ Ti::swz(vr0)) << 4) + (lane & 1) * 8;
+      auto read_k = [&](int buf, int half, int st) {
+        kf[st] = *(const u32x4_t*)(&kbuf[buf][0] + ((kfrag ^ (32 * st)) + half * 32 * ROWB));
+      };
+      auto read_v = [&](int buf, int half, int x) {
+        const int g = x / MT, mt = x % MT;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint2 p = lds_read_tr(&vbuf[buf][0] + ((vfrag ^ (64 * mt ^ 32 * y)) + (half * 32 + 16 * g + 8 * y) * ROWB));
+          vf[g][mt][2 * y] = p.x;
+          vf[g][mt][2 * y + 1] = p.y;
+        }
+      };
+      // Masks the scores of 32 keys of block t, from its key `from` on.
+      auto hide = [&](f32x16_t(&s)[QT], int t, int from, const Seen(&mine)[QT]) {
+        int at, end;
+        walk.tile(t, &at, &end);
+        const int k0 = at + from + 4 * hf;
+        const bool sinks = t < walk.n1 && at + from < wl.sink;  // uniform: most tiles with masks have none
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+          const Seen v = walk.in_run(t, mine[i]);
+          const int lo = k0 - v.lo, sink = v.sink - k0;
+          const uint32_t len = v.hi - v.lo;
+          if (sinks) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int c = 8 * (j >> 2) + (j & 3);
+              if (!((uint32_t)(lo + c) < len || c < sink)) s[i][j] = -INFINITY;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if ((uint32_t)(lo + 8 * (j >> 2) + (j & 3)) >= len) s[i][j] = -INFINITY;
+          }
+        }
+      };
+      auto exp_one = [&](const f32x16_t(&s)[QT], int e) {
+        pr[e] = fast_exp2(fmaf(s[e / 16][e % 16], sl2, -mc[e / 16]));
+        if (KEEP) lu[e / 16] += pr[e];
+      };
+      auto pack_one = [&](int x) {  // x-th of 8 QT pairs -> rounded P and the denominator
+        const int i = x / 8, e = 2 * (x % 8);
+        const uint32_t p = Mma<T>::pack(pr[2 * x], pr[2 * x + 1]);
+        pf[i][e / 8][(e / 2) % 4] = p;
+        l[i] = Mma<T>::add2(p, l[i]);
+      };
+      auto max_part = [&](const f32x16_t(&s)[QT], int i, int part, float mx) {
+#pragma unroll
+        for (int j = 4 * part; j < 4 * part + 4; ++j) mx = fmaxf(mx, s[i][j]);
+        return mx;
+      };
+      // Raises the running maxima of row tile i where a score exceeds one by more than 2^kLazy.
+      auto raise = [&](int i, float mx) {
+        mx *= sl2;
+        const bool up = __builtin_amdgcn_ballot_w64(mx > mc[i] + kLazy) != 0;
+        if (up) {
+          const float mn = fmaxf(mc[i], mx);
+          alpha[i] = fast_exp2(mc[i] - mn);
+          mc[i] = mn;
+          if (KEEP) lu[i] *= alpha[i];  // before the next exponentials are added to it
+        }
+        return up;
+      };
+      auto rescale = [&](int i) {
+        l[i] *= alpha[i];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[i][mt][j] *= alpha[i];
+      };
+      auto qk = [&](int x, f32x16_t(&s)[QT]) {
+        const int st = x / QT, i = x % QT;
+        if (st == 0) clear(s[i]);
+        Mma<T>::run(kf[st], qf[i][st], s[i]);
+      };
+      auto pv = [&](int x) {
+        const int g = x / (MT * QT), mt = (x / QT) % MT, i = x % QT;
+        Mma<T>::run(vf[g][mt], pf[i][g], o[i][mt]);
+      };
+      // One step of the run: the scores of cur, half exponentiated, to the sums, beside those of nxt, whose k is
+      // in kf; then the k of half khalf of buffer kbn.
+      auto step = [&](f32x16_t(&cur)[QT], f32x16_t(&nxt)[QT], int t, int vhalf, int kbn, int khalf, auto stage) {
+        constexpr bool STAGE = decltype(stage)::value;
+        constexpr int EA = (8 * QT + NA - 1) / NA;    // exponentials and packed pairs per A group
+        constexpr int VA = (2 * MT + NA - 1) / NA;    // v reads per A group
+#pragma unroll
+        for (int x = 0; x < NA; ++x) {
+          qk(x, nxt);
+#pragma unroll
+          for (int y = 0; y < VA; ++y)
+            if (x * VA + y < 2 * MT) read_v(t & 1, vhalf, x * VA + y);
+#pragma unroll
+          for (int y = 0; y < EA; ++y)
+            if (x * EA + y < 8 * QT) exp_one(cur, 8 * QT + x * EA + y);
+#pragma unroll
+          for (int y = 0; y < EA; ++y)
+            if (x * EA + y < 8 * QT) pack_one(x * EA + y);  // those made longest ago first
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        constexpr int KB = (KS + NB - 1) / NB;
+        constexpr int M0 = NB / 8 > 0 ? NB / 8 : 1;  // groups before the row maxima (matrix latency)
+        constexpr int MG = NB / 4;                   // groups of the row maxima
+        constexpr int E0 = M0 + MG;
+        constexpr int EB = (8 * QT + NB - E0 - 1) / (NB - E0);
+        float mx[QT];
+#pragma unroll
+        for (int x = 0; x < E0; ++x) {
+          pv(x);
+#pragma unroll
+          for (int y = 0; y < KB; ++y)
+            if (x * KB + y < KS) read_k(kbn, khalf, x * KB + y);
+          if (x == M0) {
+#pragma unroll
+            for (int i = 0; i < QT; ++i) mx[i] = nxt[i][0];
+          }
+          if (x >= M0) {
+#pragma unroll
+            for (int y = (x - M0) * 4 * QT / MG; y < (x - M0 + 1) * 4 * QT / MG; ++y)
+              mx[y / 4] = max_part(nxt, y / 4, y % 4, mx[y / 4]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        bool up[QT];
+#pragma unroll
+        for (int i = 0; i < QT; ++i) up[i] = raise(i, pair_max(mx[i]));
+#pragma unroll
+        for (int x = E0; x < NB; ++x) {
+          pv(x);
+#pragma unroll
+          for (int y = 0; y < KB; ++y)
+            if (x * KB + y < KS) read_k(kbn, khalf, x * KB + y);
+#pragma unroll
+          for (int y = 0; y < EB; ++y)
+            if ((x - E0) * EB + y < 8 * QT) exp_one(nxt, (x - E0) * EB + y);
+          if (STAGE && x == NB - NB / 4) store(t);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < QT; ++i)
+          if (up[i]) rescale(i);
+      };
+      // Scores of half `half` of the k in kbuf[b], and the maxima.
+      auto scores = [&](f32x16_t(&s)[QT], int b, int half) {
+#pragma unroll
+        for (int st = 0; st < KS; ++st) read_k(b, half, st);
+#pragma unroll
+        for (int x = 0; x < NA; ++x) qk(x, s);
+      };
+      auto maxima = [&](f32x16_t(&s)[QT]) {
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+          float mx = s[i][0];
+#pragma unroll
+          for (int part = 0; part < 4; ++part) mx = max_part(s, i, part, mx);
+          if (raise(i, pair_max(mx))) rescale(i);
+        }
+      };
+      // The rest of a step whose first `done` exponentials are made; oddities: masked, and its v is not all finite.
+      auto finish = [&](f32x16_t(&s)[QT], int t, int vhalf, int done, bool oddities) {
+#pragma unroll
+        for (int x = 0; x < 2 * MT; ++x) read_v(t & 1, vhalf, x);
+#pragma unroll
+        for (int e = 0; e < 16 * QT; ++e)
+          if (e >= done) exp_one(s, e);
+#pragma unroll
+        for (int x = 0; x < 8 * QT; ++x) pack_one(x);
+        if (oddities) {
+          met = true;
+#pragma unroll
+          for (int x = 0; x < 2 * MT; ++x) vf[x / MT][x % MT] = finite<T>(vf[x / MT][x % MT]);
+        }
+#pragma unroll
+        for (int x = 0; x < NB; ++x) pv(x);
+      };
+      auto fetch = [&](int t) {  // into registers, while block t is at work
+        load(vbase, vst, t + 1, vr);
+        load(kbase, kst, t + 2, kr);
+      };
+      auto next = [&]() {
+        __syncthreads();
+        kb = later(1);
+      };
+      auto check = [&](int t) {  // the v of block t, in vr
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) bad |= odd<T>(vr[i]);
+        const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+        if (lane == 0) odd_in[t & 1][w] = any;
+      };
+      auto edges = [&](int t, int stop) {  // blocks t .. stop - 1, one thing after the other
+        if (t >= stop) return;
+        Seen mine[QT];
+#pragma unroll
+        for (int i = 0; i < QT; ++i) mine[i] = row_sees(i);
+        for (; t < stop; ++t) {
+          fetch(t);
+          uint32_t bad = 0;
+#pragma unroll
+          for (int x = 0; x < NW; ++x) bad |= odd_in[t & 1][x];
+          bad = __builtin_amdgcn_readfirstlane(bad);
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            if (xw >= n || !walk.any(t, wf, wl, 32 * half, 32)) continue;
+            const bool masked = !walk.full(t, wf, wl);
+            scores(sa, kb, half);
+            if (masked) hide(sa, t, 32 * half, mine);
+            maxima(sa);
+            finish(sa, t, half, 0, masked && bad);
+          }
+          check(t + 1);
+          store(t);
+          next();
+        }
+      };
+      // The longest run of blocks of which every row sees everything: of the window's or of the sinks'.
+      const int t0 = walk.one ? 0 : walk.n1, k0 = walk.one ? 0 : walk.lo;
+      int from = t0 + max(0, walk.last.lo - k0 + BK - 1) / BK, to = t0 + max(0, walk.first.hi - k0) / BK;
+      if (walk.first.sink / BK > to - from) from = 0, to = walk.first.sink / BK;
+      if (to <= from) from = to = nblk;
+      {
+        u32x4_t k1[NL];
+        load(kbase, kst, 0, kr);
+        load(vbase, vst, 0, vr);
+        load(kbase, kst, 1, k1);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          Ti::put(kbuf[0], srow + RI * i, sc, kr[i]);
+          Ti::put(vbuf[0], srow + RI * i, sc, vr[i]);
+          Ti::put(kbuf[1], srow + RI * i, sc, k1[i]);
+        }
+        check(0);
+      }
+      __syncthreads();
+      edges(0, from);
+      if (from < to) {
+        scores(sa, kb, 0);
+        maxima(sa);
+#pragma unroll
+        for (int e = 0; e < 8 * QT; ++e) exp_one(sa, e);
+#pragma unroll
+        for (int st = 0; st < KS; ++st) read_k(kb, 1, st);
+        for (int t = from; t < to - 1; ++t) {
+          asm volatile("" : "+v"(kfrag), "+v"(vfrag));  // no address made from them is kept from block to block
+          fetch(t);
+          step(sa, sb, t, 0, later(1), 0, std::false_type());
+          step(sb, sa, t, 1, later(1), 1, std::true_type());
+          next();
+        }
+        fetch(to - 1);
+        step(sa, sb, to - 1, 0, kb, 1, std::false_type());
+        finish(sb, to - 1, 1, 8 * QT, false);
+        check(to);
+        store(to - 1);
+        next();
+        edges(to, nblk);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+      if (met) add_keys<T, D, false>(walk, row_sees(i), 0, nblk, 1, vbase, a.ldv, hf, o[i]);
+      const int x = xw + 32 * i + l32;
+      l[i] = pair_sum(l[i]);
+      if (KEEP) lu[i] = pair_sum(lu[i]);
+      if (x < n) {
+        const int64_t at = q0 * (int64_t)H + row_at(a, H, h, x, 1);
+        forward_store<T, D>(a, at, hf, l[i], o[i]);
+        if (KEEP) store_lse(a, at, hf, mc[i], lu[i]);
+      }
+    }
+    __syncthreads();  // the next row tile of this block stages over these buffers
   }
 }
 
@@ -394,9 +772,10 @@ __global__ void __launch_bounds__(kNT) wa_few_kernel(const WaArgs a) {
 #pragma unroll
       for (int st = 0; st < KS; ++st) qf[st] = F::load(p + 16 * st);
     }
-    const Walk walk(a, query_of(a, x0) + off, query_of(a, min(x0 + 32, n) - 1) + off, kv_len);
+    const Walk<kBK> walk(a, query_of(a, x0) + off, query_of(a, min(x0 + 32, n) - 1) + off, kv_len);
     const Seen mine = seen_from(a, query_of(a, x) + off, kv_len);
     float m = -FLT_MAX, l = 0.f;
+    bool met = false;
     f32x16_t o[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) clear(o[mt]);
@@ -424,10 +803,11 @@ __global__ void __launch_bounds__(kNT) wa_few_kernel(const WaArgs a) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       if (AHEAD) load(t + NW);
       if (walk.full(t, walk.first, walk.last))
-        forward_step<T, D, false>(kt, vt, lane, at, mine, a.sl2, qf, m, l, o);
+        forward_step<T, D, false>(kt, vt, lane, at, mine, a.sl2, qf, m, l, o, met);
       else
-        forward_step<T, D, true>(kt, vt, lane, at, walk.in_run(t, mine), a.sl2, qf, m, l, o);
+        forward_step<T, D, true>(kt, vt, lane, at, walk.in_run(t, mine), a.sl2, qf, m, l, o, met);
     }
+    if (met) add_keys<T, D, false>(walk, mine, sp * per + w, stop, NW, vbase, a.ldv, hf, o);
     l = pair_sum(l);
     if (hf == 0) {
       sm[w][l32] = m;
@@ -450,7 +830,8 @@ __global__ void __launch_bounds__(kNT) wa_few_kernel(const WaArgs a) {
     if (w != 0 || x0 + l32 >= n) continue;
     const int64_t at = q0 * (int64_t)H + row_at(a, H, h, x, 1);
     if (a.splits == 1) {
-      forward_store<T, D>(a, at, hf, m, l, o);
+      forward_store<T, D>(a, at, hf, l, o);
+      store_lse(a, at, hf, m, l);
     } else {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) store_dims(part_sums(a, sp, at, D) + 32 * mt, hf, o[mt], 1.f);
@@ -568,12 +949,13 @@ __global__ void __launch_bounds__(kNT, 1) wa_dq_kernel(const WaArgs a) {
       }
     }
     const float lse = a.lse[at], r = a.r[at];
-    const Walk walk(a, query_of(a, x0) + off, query_of(a, min(x0 + ROWS, n) - 1) + off, kv_len);
+    const Walk<kBK> walk(a, query_of(a, x0) + off, query_of(a, min(x0 + ROWS, n) - 1) + off, kv_len);
     const Seen mine = seen_from(a, query_of(a, x) + off, kv_len);
     const Seen wf = seen_from(a, query_of(a, min(xw, n - 1)) + off, kv_len);
     const Seen wl = seen_from(a, query_of(a, min(xw + 31, n - 1)) + off, kv_len);
     const bool idle = xw >= n;
     f32x16_t acc[MT];
+    bool met = false;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) clear(acc[mt]);
     Stage<T, D, kBK, NT> ks, vs;
@@ -604,7 +986,7 @@ __global__ void __launch_bounds__(kNT, 1) wa_dq_kernel(const WaArgs a) {
         if (MASK && !sees(s, k0 + 8 * (j >> 2) + 4 * hf + (j & 3))) d[j] = 0.f;
       }
       const Fr f[2] = {F::pack(d), F::pack(d + 8)};
-      add_rows<T, D, MASK>(kt, lane, f, [&](int e) { return sees(s, k0 + e); }, acc);
+      add_rows<T, D, MASK>(kt, lane, f, acc, met);
     };
     int t = SHARE ? w : 0;
     if (AHEAD) load(t);
@@ -622,6 +1004,7 @@ __global__ void __launch_bounds__(kNT, 1) wa_dq_kernel(const WaArgs a) {
       if (walk.full(t, wf, wl)) step(kt, vt, std::false_type(), k0, mine);
       else step(kt, vt, std::true_type(), k0, walk.in_run(t, mine));
     }
+    if (met) add_keys<T, D, true>(walk, mine, SHARE ? w : 0, nt, STEP, kbase, a.ldk, hf, acc);
     if (SHARE) join_waves<MT>((float*)lds, w, lane, acc);
     else __syncthreads();  // the next tile's rows go into these buffers
     if (xw + l32 < n && (!SHARE || w == 0)) {
@@ -644,9 +1027,13 @@ __device__ __forceinline__ Rows rows_of(const WaArgs& a, int k, int off, int q_l
   return {(int)lo * a.G, (int)hi * a.G};
 }
 
-// dk and dv of 128 (32) keys of a key head, over the rows of all its query heads.
-template <typename T, int D, bool SHARE>
+// dk and dv of 128 (32) keys of a key head, over the rows of all its query heads.  Every row sees the sinks: where
+// that is many times what sees another key, they are left to SINKS blocks (32 keys, and of their rows one of
+// sink_parts parts; 15143 tokens, 12 x 128 bf16, window 256, 16 sinks: the first tile's blocks took 28 times
+// the others' rows and 970 of the step's 1374 us).
+template <typename T, int D, bool SHARE, bool SINKS>
 __global__ void __launch_bounds__(kNT, 1) wa_dkv_kernel(const WaArgs a) {
+  static_assert(SHARE || !SINKS, "sinks: 32 keys");
   typedef Frag<T> F;
   typedef typename F::type Fr;
   typedef Tile<T, D> Ti;
@@ -666,16 +1053,21 @@ __global__ void __launch_bounds__(kNT, 1) wa_dkv_kernel(const WaArgs a) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, hf = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = SHARE ? lane : threadIdx.x;
   const int H = a.Hk * a.G, off = kv_len - q_len;
-  if (a.rest) {
+  if (a.rest && !SINKS) {
     zero_rest((T*)a.dk, a.cu_kv, a.total_kv, bb, a.Hk, D, h, bx, gridDim.x, 1);
     zero_rest((T*)a.dv, a.cu_kv, a.total_kv, bb, a.Hk, D, h, bx, gridDim.x, 1);
   }
+  const int part = SINKS ? bx % a.sink_parts : 0, bt = SINKS ? bx / a.sink_parts : bx;
+  const int keys = SINKS ? min(kv_len, a.sinks) : kv_len;  // of this grid
+  const int tiles = SINKS ? a.sink_keys / ROWS : gridDim.x;
+  const int first = a.own_sinks && !SINKS ? a.sinks : 0;
   const T* qbase = (const T*)a.q + (int64_t)q0 * a.ldq;
   const T* dbase = (const T*)a.dout + (int64_t)q0 * H * D;
   const float scale = a.sl2 / kLog2e;
 
-  for (int64_t ktile = (int64_t)bx * ROWS; ktile < kv_len; ktile += (int64_t)gridDim.x * ROWS) {
-    const int k0 = (int)ktile, kw = SHARE ? k0 : k0 + w * 32, ki = min(kw + l32, kv_len - 1);
+  for (int64_t ktile = (int64_t)bt * ROWS; ktile < keys; ktile += (int64_t)tiles * ROWS) {
+    if (ktile + ROWS <= first) continue;
+    const int k0 = max((int)ktile, first), kw = SHARE ? (int)ktile : (int)ktile + w * 32, ki = min(kw + l32, keys - 1);
     const int64_t krow = kv0 + ki;
     Fr kf[KS], vf[KS];
     {
@@ -697,16 +1089,24 @@ __global__ void __launch_bounds__(kNT, 1) wa_dkv_kernel(const WaArgs a) {
       return Rows{min(f.lo, l.lo), max(max(f.hi, l.hi), f.lo)};
     };
     int all_lo, all_hi, wave_lo, wave_hi;
-    const Rows run = span(k0, min(k0 + ROWS, kv_len) - 1, &all_lo, &all_hi);
-    const Rows wrun = span(min(kw, kv_len - 1), min(kw + 31, kv_len - 1), &wave_lo, &wave_hi);
-    const Rows mine = rows_of(a, ki, off, q_len);
-    const bool idle = kw >= kv_len;
+    Rows run = span(k0, (int)min(ktile + ROWS, (int64_t)keys) - 1, &all_lo, &all_hi);
+    const Rows wrun = span(min(max(kw, first), keys - 1), min(max(kw + 31, first), keys - 1), &wave_lo, &wave_hi);
+    Rows mine = rows_of(a, ki, off, q_len);
+    if (ki < first) mine.hi = mine.lo;  // another grid's
+    if (kw < first) wave_hi = wave_lo;
+    const bool idle = kw >= keys || kw + 32 <= first;
+    if (SINKS) {  // a part of the rows, in whole tiles for the four waves
+      const int per = ((run.hi - run.lo + a.sink_parts - 1) / a.sink_parts + 127) / 128 * 128;
+      run.lo = (int)min((int64_t)run.lo + (int64_t)part * per, (int64_t)run.hi);
+      run.hi = (int)min((int64_t)run.lo + per, (int64_t)run.hi);
+    }
     f32x16_t dk[MT], dv[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       clear(dk[mt]);
       clear(dv[mt]);
     }
+    bool met = false;
     u32x4_t qr[NL], dr[NL];
     float sv = 0.f;
     constexpr int STEP = SHARE ? 4 * BQ : BQ;
@@ -748,9 +1148,9 @@ __global__ void __launch_bounds__(kNT, 1) wa_dkv_kernel(const WaArgs a) {
         if (MASK && !see(e)) p[j] = d[j] = 0.f;
       }
       const Fr pf[2] = {F::pack(p), F::pack(p + 8)};
-      add_rows<T, D, MASK>(dt, lane, pf, see, dv);
+      add_rows<T, D, MASK>(dt, lane, pf, dv, met);
       const Fr df[2] = {F::pack(d), F::pack(d + 8)};
-      add_rows<T, D, MASK>(qt, lane, df, see, dk);
+      add_rows<T, D, MASK>(qt, lane, df, dk, met);
     };
     int xb = run.lo + (SHARE ? w * BQ : 0);
     if (AHEAD) load(xb);
@@ -772,20 +1172,57 @@ __global__ void __launch_bounds__(kNT, 1) wa_dkv_kernel(const WaArgs a) {
       if (xb >= wave_lo && xb + BQ <= wave_hi) step(qt, dt, st2, xb, std::false_type());
       else step(qt, dt, st2, xb, std::true_type());
     }
+    if (met)
+      for (int x = max(wrun.lo, run.lo); x < min(wrun.hi, run.hi); ++x) {
+        const bool seen = x >= mine.lo && x < mine.hi;
+        add_odd<T, D, true>(qbase + row_at(a, a.ldq, h, x, D), hf, seen, dk);
+        add_odd<T, D, false>(dbase + row_at(a, (int64_t)H * D, h, x, D), hf, seen, dv);
+      }
     if (SHARE) {
       join_waves<MT>((float*)lds, w, lane, dk);
       join_waves<MT>((float*)lds, w, lane, dv);
     } else {
       __syncthreads();  // every wave has left the buffers
     }
-    if (kw + l32 < kv_len && (!SHARE || w == 0)) {
+    if (kw + l32 < keys && kw + l32 >= first && (!SHARE || w == 0)) {
       const int64_t at = (krow * a.Hk + h) * D;
+      if constexpr (SINKS) {
+        float* p = a.sink_sums + ((((int64_t)part * gridDim.z + bb) * a.Hk + h) * a.sink_keys + ki) * 2 * D;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          store_dims(p + 32 * mt, hf, dk[mt], 1.f);
+          store_dims(p + D + 32 * mt, hf, dv[mt], 1.f);
+        }
+        continue;
+      }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         store_dims((T*)a.dk + at + 32 * mt, hf, dk[mt], scale);
         store_dims((T*)a.dv + at + 32 * mt, hf, dv[mt], 1.f);
       }
     }
+  }
+}
+
+// Adds up the parts of the sinks' gradients: a block for four sinks of a key head, a wave each.
+template <typename T, int D>
+__global__ void __launch_bounds__(kNT) wa_sinks_kernel(const WaArgs a) {
+  const int lane = threadIdx.x & 63, k = blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y, bb = blockIdx.z;
+  int kv0, kv_len;
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  if (k >= min(kv_len, a.sinks)) return;
+  const float scale = a.sl2 / kLog2e;
+  const float* p = a.sink_sums + (((int64_t)bb * a.Hk + h) * a.sink_keys + k) * 2 * D;
+  const int64_t step = (int64_t)gridDim.z * a.Hk * a.sink_keys * 2 * D, at = ((int64_t)(kv0 + k) * a.Hk + h) * D;
+  float s[2 * D / 64] = {};
+#pragma unroll 4
+  for (int i = 0; i < a.sink_parts; ++i)
+#pragma unroll
+    for (int e = 0; e < 2 * D / 64; ++e) s[e] += p[i * step + lane + 64 * e];
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) {
+    ((T*)a.dk)[at + lane + 64 * e] = (T)(s[e] * scale);
+    ((T*)a.dv)[at + lane + 64 * e] = (T)s[D / 64 + e];
   }
 }
 
@@ -800,14 +1237,14 @@ unsigned tiles_of(int64_t longest, int64_t hb, int rows) {
 
 // Blocks of the forward pass: rows of each, and the parts of their keys.
 struct Plan {
-  int rows, splits;
+  int rows, splits;  // 32: wa_few_kernel
 };
 constexpr int64_t kScratchInputs = 4, kScratchLeast = 64 << 20;
 int64_t part_bytes(int64_t total_q, int32_t H, int32_t D) { return 4 * total_q * H * (D + 2); }
 Plan wa_plan(const WindowAttnSizes& z) {
   const int64_t hb = (int64_t)z.Hk * z.B, G = z.H / z.Hk;
   const int64_t max_q = std::max<int64_t>(z.max_q, (z.total_q + z.B - 1) / z.B);
-  Plan p = {kBQ, 1};
+  Plan p = {z.dtype == TSC_F32 ? kBQ : kBQ16, 1};
   if ((int64_t)tiles_of(max_q * G, hb, kBQ) * hb >= kCUs) return p;
   p.rows = 32;
   const int64_t blocks = (int64_t)tiles_of(max_q * G, hb, 32) * hb;
@@ -817,6 +1254,27 @@ Plan wa_plan(const WindowAttnSizes& z) {
   const int64_t io = 2 * z.D * es * (z.total_q * z.H + z.total_kv * z.Hk);
   const int64_t room = std::max(kScratchLeast, kScratchInputs * io) / std::max<int64_t>(1, part_bytes(z.total_q, z.H, z.D));
   p.splits = (int)std::max<int64_t>(1, std::min({span / 256, 2 * kCUs / blocks, room}));
+  return p;
+}
+
+// The blocks that share the rows of a tile of sinks: as many as leave each about the rows of another key, in
+// scratch as above; 1: sinks are keys like others.
+struct SinkPlan {
+  int parts, keys;
+  int64_t bytes;
+};
+SinkPlan sink_plan(const WindowAttnSizes& z) {
+  SinkPlan p = {1, 0, 0};
+  const int64_t sinks = std::min<int64_t>(z.sinks, z.max_kv);
+  const int64_t rows = std::min<int64_t>(z.max_q, (z.causal ? 1 : 2) * (int64_t)z.window + 32);
+  if (z.B == 0 || sinks == 0 || 2 * sinks > z.max_kv || z.max_q < 2 * rows) return p;
+  p.keys = (int)((sinks + 31) / 32 * 32);
+  const int64_t part = (int64_t)z.B * z.Hk * p.keys * 2 * z.D * 4;
+  const int64_t es = z.dtype == TSC_F32 ? 4 : 2;
+  const int64_t io = 2 * z.D * es * (z.total_q * z.H + z.total_kv * z.Hk);
+  p.parts = (int)std::min({z.max_q / rows, (int64_t)64, std::max(kScratchLeast, kScratchInputs * io) / part});
+  if (p.parts < 2) return {1, 0, 0};
+  p.bytes = p.parts * part;
   return p;
 }
 
@@ -871,7 +1329,7 @@ int too_many(const WindowAttnSizes& z) {
 
 int64_t window_attention_workspace_bytes(const WindowAttnSizes& z, int32_t backward) {
   if (z.B == 0 || z.total_q == 0) return 0;
-  if (backward) return 4 * z.total_q * z.H;
+  if (backward) return (int64_t)align_up(4 * z.total_q * z.H, 16) + sink_plan(z).bytes;
   const int s = wa_plan(z).splits;
   return s > 1 ? s * part_bytes(z.total_q, z.H, z.D) : 0;
 }
@@ -894,7 +1352,12 @@ int window_attention_launch(tsc_ctx* ctx, const WindowAttnArgs& x, void* out, vo
     {
       ProfScope p(ctx, "window_attention");
       if (plan.rows == 32) wa_few_kernel<T, D><<<grid, kNT, 0, ctx->stream>>>(a);
-      else wa_forward_kernel<T, D><<<grid, kNT, 0, ctx->stream>>>(a);
+      else if constexpr (sizeof(T) == 4) wa_forward32_kernel<D><<<grid, kNT, 0, ctx->stream>>>(a);
+      else {
+        constexpr int QT = D == 64 ? 2 : 1, NW = kBQ16 / 32 / QT;
+        if (a.lse) wa_forward16_kernel<T, D, QT, NW, true><<<grid, 64 * NW, 0, ctx->stream>>>(a);
+        else wa_forward16_kernel<T, D, QT, NW, false><<<grid, 64 * NW, 0, ctx->stream>>>(a);
+      }
     }
     if (a.splits > 1) {
       ProfScope p(ctx, "window_attention_join");
@@ -919,6 +1382,11 @@ int window_attention_backward_launch(tsc_ctx* ctx, const WindowAttnArgs& x, cons
   const bool few_k = (int64_t)tiles_of(z.max_kv, hb, kBQ) * hb < kCUs;
   const dim3 gq(tiles_of((int64_t)z.max_q * a.G, hb, few_q ? 32 : kBQ), (unsigned)z.Hk, (unsigned)z.B);
   const dim3 gk(tiles_of(z.max_kv, hb, few_k ? 32 : kBQ), (unsigned)z.Hk, (unsigned)z.B);
+  const SinkPlan sinks = rows > 0 ? sink_plan(z) : SinkPlan{1, 0, 0};
+  a.own_sinks = sinks.parts > 1;
+  a.sink_parts = sinks.parts;
+  a.sink_keys = sinks.keys;
+  a.sink_sums = (float*)((char*)ws + align_up(4 * rows, 16));
   return by_type(z.dtype, z.D, [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
@@ -929,8 +1397,14 @@ int window_attention_backward_launch(tsc_ctx* ctx, const WindowAttnArgs& x, cons
     }
     {
       ProfScope p(ctx, "window_attention_dkv");
-      if (few_k) wa_dkv_kernel<T, D, true><<<gk, kNT, 0, ctx->stream>>>(a);
-      else wa_dkv_kernel<T, D, false><<<gk, kNT, 0, ctx->stream>>>(a);
+      if (few_k) wa_dkv_kernel<T, D, true, false><<<gk, kNT, 0, ctx->stream>>>(a);
+      else wa_dkv_kernel<T, D, false, false><<<gk, kNT, 0, ctx->stream>>>(a);
+    }
+    if (a.own_sinks) {
+      ProfScope p(ctx, "window_attention_sinks");
+      const dim3 gs((unsigned)(sinks.keys / 32 * sinks.parts), (unsigned)z.Hk, (unsigned)z.B);
+      wa_dkv_kernel<T, D, true, true><<<gs, kNT, 0, ctx->stream>>>(a);
+      wa_sinks_kernel<T, D><<<dim3((unsigned)(sinks.keys / 4), (unsigned)z.Hk, (unsigned)z.B), kNT, 0, ctx->stream>>>(a);
     }
     if (rows > 0) {
       ProfScope p(ctx, "window_attention_dq");
