@@ -88,6 +88,26 @@ struct Tile {
     }
     return r;
   }
+  // The same with addresses made from one register each, so that a loop keeps that and no more.  row_of: chunk
+  // 2 st + hf of row l32 is at it ^ 32 st; col_of: the piece of dim tile mt in rows 8 x + .. at it ^ (64 mt ^ 32 x).
+  static __device__ __forceinline__ int row_of(int l32, int hf) { return l32 * ROWB + ((hf ^ swz(l32)) << 4); }
+  static __device__ __forceinline__ int col_of(int lane) {
+    const int vr = 4 * (lane >> 5) + ((lane & 15) >> 2);
+    return vr * ROWB + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swz(vr)) << 4) + (lane & 1) * 8;
+  }
+  static __device__ __forceinline__ u32x4_t row_at(const unsigned char* t, int r0, int it, int st) {
+    return *(const u32x4_t*)(t + ((it ^ (32 * st)) + r0 * ROWB));
+  }
+  static __device__ __forceinline__ u32x4_t col_at(const unsigned char* t, int r0, int it, int g, int mt) {
+    u32x4_t r;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const uint2 h = lds_read_tr(t + ((it ^ (64 * mt ^ 32 * x)) + (r0 + 16 * g + 8 * x) * ROWB));
+      r[2 * x] = h.x;
+      r[2 * x + 1] = h.y;
+    }
+    return r;
+  }
 };
 template <int D>
 struct Tile<float, D> {
@@ -105,6 +125,18 @@ struct Tile<float, D> {
     for (int e = 0; e < 8; ++e)
       r.v[e] = ((const float*)(t + (r0 + 16 * g + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * ROWB))
           [32 * mt + (lane & 31)];
+    return r;
+  }
+  static __device__ __forceinline__ int row_of(int l32, int hf) { return l32 * ROWB + 32 * hf; }
+  static __device__ __forceinline__ int col_of(int lane) { return 4 * (lane >> 5) * ROWB + 4 * (lane & 31); }
+  static __device__ __forceinline__ F32x8 row_at(const unsigned char* t, int r0, int it, int st) {
+    return Frag<float>::load((const float*)(t + (it + r0 * ROWB + 64 * st)));
+  }
+  static __device__ __forceinline__ F32x8 col_at(const unsigned char* t, int r0, int it, int g, int mt) {
+    F32x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      r.v[e] = *(const float*)(t + (it + (r0 + 16 * g + 8 * (e >> 2) + (e & 3)) * ROWB + 128 * mt));
     return r;
   }
 };

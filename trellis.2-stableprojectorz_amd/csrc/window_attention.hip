@@ -48,7 +48,7 @@ struct WaArgs {
   float* part;     // splits > 1: (splits, total_q, H, D) sums, then (splits, total_q, H, 2)
   // backward
   const void* dout;
-  const float* r;  // (total_q, H)
+  float* r;        // (total_q, H): do . out
   void *dq, *dk, *dv;
   int32_t own_sinks;   // dk / dv blocks leave out the sinks, which have blocks and scratch of their own:
   int32_t sink_keys;   // sinks of a sequence there is scratch for, whole tiles of 32
@@ -118,6 +118,17 @@ struct Walk {
     const bool win = (one || t >= n1) && at < l.hi && at + keys > f.lo;
     return sinks || win;
   }
+  // The longest run of tiles of which every row sees everything: of the window's, or of the sinks'.
+  __device__ __forceinline__ void longest(int* from, int* to) const {
+    const int t0 = one ? 0 : n1, k0 = one ? 0 : lo;
+    *from = t0 + max(0, last.lo - k0 + BK - 1) / BK;
+    *to = t0 + max(0, first.hi - k0) / BK;
+    if (first.sink / BK > *to - *from) {
+      *from = 0;
+      *to = first.sink / BK;
+    }
+    if (*to <= *from) *from = *to = tiles();
+  }
   // A row's bounds within the run that tile t belongs to.
   __device__ __forceinline__ Seen in_run(int t, Seen s) const {
     if (!one) {
@@ -168,10 +179,10 @@ __device__ __forceinline__ u32x4_t finite(const u32x4_t& f) {
   return r;
 }
 
-// acc += sum over the 32 rows e of the tile of p[e] row_e; pf: p as two fragments.  With masks, what is not
+// acc += sum over the 32 rows e of the tile of p[e] row_e; pf: p as two fragments, col: Tile's col_of.  With masks, what is not
 // finite is left out, and met is set.
 template <typename T, int D, bool MASK>
-__device__ __forceinline__ void add_rows(const unsigned char* t, int lane, const typename Frag<T>::type (&pf)[2],
+__device__ __forceinline__ void add_rows(const unsigned char* t, int col, const typename Frag<T>::type (&pf)[2],
                                          f32x16_t (&acc)[D / 32], bool& met) {
   typedef Frag<T> F;
   typedef typename F::type Fr;
@@ -181,7 +192,7 @@ __device__ __forceinline__ void add_rows(const unsigned char* t, int lane, const
   for (int g = 0; g < 2; ++g) {
     Fr v[MT];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) v[mt] = Ti::col(t, 0, lane, g, mt);
+    for (int mt = 0; mt < MT; ++mt) v[mt] = Ti::col_at(t, 0, col, g, mt);
     if constexpr (MASK) {
       uint32_t bad = 0;
 #pragma unroll
@@ -224,18 +235,17 @@ __device__ __forceinline__ void add_keys(const Walk<BK>& walk, const Seen& mine,
 
 // One tile of 32 keys from k0 on, in LDS, for a wave's 32 rows; s: what the lane's row sees of it.
 template <typename T, int D, bool MASK>
-__device__ __forceinline__ void forward_step(const unsigned char* kt, const unsigned char* vt, int lane,
-                                             int k0, const Seen& s, float sl2,
+__device__ __forceinline__ void forward_step(const unsigned char* kt, const unsigned char* vt, int row, int col,
+                                             int hf, int k0, const Seen& s, float sl2,
                                              const typename Frag<T>::type (&qf)[D / 16], float& m,
                                              float& l, f32x16_t (&o)[D / 32], bool& met) {
   typedef Frag<T> F;
   typedef Tile<T, D> Ti;
   constexpr int KS = D / 16, MT = D / 32;
-  const int l32 = lane & 31, hf = lane >> 5;
   f32x16_t c;
   clear(c);
 #pragma unroll
-  for (int st = 0; st < KS; ++st) F::mma(Ti::row(kt, 0, l32, hf, st), qf[st], c);
+  for (int st = 0; st < KS; ++st) F::mma(Ti::row_at(kt, 0, row, st), qf[st], c);
   if constexpr (MASK) {
 #pragma unroll
     for (int j = 0; j < 16; ++j)
@@ -260,7 +270,7 @@ __device__ __forceinline__ void forward_step(const unsigned char* kt, const unsi
     l += p[j];
   }
   const typename F::type pf[2] = {F::pack(p), F::pack(p + 8)};
-  add_rows<T, D, MASK>(vt, lane, pf, o, met);
+  add_rows<T, D, MASK>(vt, col, pf, o, met);
 }
 
 // Writes a wave's finished rows: l summed over both halves, 0 where a row sees no key.
@@ -336,8 +346,10 @@ __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward32_kernel(cons
       ks.load(kbase, a.ldk, at, end, tid);
       vs.load(vbase, a.ldv, at, end, tid);
     };
+    int row = Ti::row_of(l32, hf), col = Ti::col_of(lane);
     load(0);
     for (int t = 0; t < nt; ++t) {
+      asm volatile("" : "+v"(row), "+v"(col));  // no address made from them is kept from tile to tile
       int at, end;
       walk.tile(t, &at, &end);
       __syncthreads();
@@ -347,9 +359,9 @@ __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward32_kernel(cons
       load(t + 1);
       if (idle || !walk.any(t, wf, wl)) continue;
       if (walk.full(t, wf, wl)) {
-        forward_step<T, D, false>(kt, vt, lane, at, mine, a.sl2, qf, m, l, o, met);
+        forward_step<T, D, false>(kt, vt, row, col, hf, at, mine, a.sl2, qf, m, l, o, met);
       } else {
-        forward_step<T, D, true>(kt, vt, lane, at, walk.in_run(t, mine), a.sl2, qf, m, l, o, met);
+        forward_step<T, D, true>(kt, vt, row, col, hf, at, walk.in_run(t, mine), a.sl2, qf, m, l, o, met);
       }
     }
     if (met) add_keys<T, D, false>(walk, mine, 0, nt, 1, vbase, a.ldv, hf, o);
@@ -452,22 +464,10 @@ __global__ void __launch_bounds__(64 * NW, 2) wa_forward16_kernel(const WaArgs a
       };
       u32x4_t kf[KS], vf[2][MT], pf[QT][2];
       float pr[16 * QT];
-      // Tile's row and col with addresses made from one register each: chunk 2 st + hf of row l32 is kfrag ^ 32 st,
-      // and the piece of dim tile mt in rows 8 y + .. is vfrag ^ (64 mt ^ 32 y).
-      const int vr0 = 4 * hf + ((lane & 15) >> 2);
-      int kfrag = l32 * ROWB + ((hf ^ Ti::swz(l32)) << 4);
-      int vfrag = vr0 * ROWB + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ Ti::swz(vr0)) << 4) + (lane & 1) * 8;
-      auto read_k = [&](int buf, int half, int st) {
-        kf[st] = *(const u32x4_t*)(&kbuf[buf][0] + ((kfrag ^ (32 * st)) + half * 32 * ROWB));
-      };
+      int kfrag = Ti::row_of(l32, hf), vfrag = Ti::col_of(lane);
+      auto read_k = [&](int buf, int half, int st) { kf[st] = Ti::row_at(kbuf[buf], 32 * half, kfrag, st); };
       auto read_v = [&](int buf, int half, int x) {
-        const int g = x / MT, mt = x % MT;
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const uint2 p = lds_read_tr(&vbuf[buf][0] + ((vfrag ^ (64 * mt ^ 32 * y)) + (half * 32 + 16 * g + 8 * y) * ROWB));
-          vf[g][mt][2 * y] = p.x;
-          vf[g][mt][2 * y + 1] = p.y;
-        }
+        vf[x / MT][x % MT] = Ti::col_at(vbuf[buf], 32 * half, vfrag, x / MT, x % MT);
       };
       // Masks the scores of 32 keys of block t, from its key `from` on.
       auto hide = [&](f32x16_t(&s)[QT], int t, int from, const Seen(&mine)[QT]) {
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(64 * NW, 2) wa_forward16_kernel(const WaArgs a
         const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
         if (lane == 0) odd_in[t & 1][w] = any;
       };
-      auto edges = [&](int t, int stop) {  // blocks t .. stop - 1, one thing after the other
+      auto edges = [&](int t, int stop) __attribute__((always_inline)) {  // blocks t .. stop - 1, one thing after the other
         if (t >= stop) return;
         Seen mine[QT];
 #pragma unroll
@@ -671,11 +671,8 @@ __global__ void __launch_bounds__(64 * NW, 2) wa_forward16_kernel(const WaArgs a
           next();
         }
       };
-      // The longest run of blocks of which every row sees everything: of the window's or of the sinks'.
-      const int t0 = walk.one ? 0 : walk.n1, k0 = walk.one ? 0 : walk.lo;
-      int from = t0 + max(0, walk.last.lo - k0 + BK - 1) / BK, to = t0 + max(0, walk.first.hi - k0) / BK;
-      if (walk.first.sink / BK > to - from) from = 0, to = walk.first.sink / BK;
-      if (to <= from) from = to = nblk;
+      int from, to;
+      walk.longest(&from, &to);
       {
         u32x4_t k1[NL];
         load(kbase, kst, 0, kr);
@@ -790,9 +787,10 @@ __global__ void __launch_bounds__(kNT) wa_few_kernel(const WaArgs a) {
       vs.load(vbase, a.ldv, at, end, lane);
     };
     constexpr bool AHEAD = D == 64 || sizeof(T) == 2;  // registers for the next tile's rows
-    int t = sp * per + w;
+    int t = sp * per + w, row = Ti::row_of(l32, hf), col = Ti::col_of(lane);
     if (AHEAD) load(t);
     for (; t < stop; t += NW) {
+      asm volatile("" : "+v"(row), "+v"(col));
       if (!AHEAD) load(t);
       int at, end;
       walk.tile(t, &at, &end);
@@ -803,9 +801,9 @@ __global__ void __launch_bounds__(kNT) wa_few_kernel(const WaArgs a) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       if (AHEAD) load(t + NW);
       if (walk.full(t, walk.first, walk.last))
-        forward_step<T, D, false>(kt, vt, lane, at, mine, a.sl2, qf, m, l, o, met);
+        forward_step<T, D, false>(kt, vt, row, col, hf, at, mine, a.sl2, qf, m, l, o, met);
       else
-        forward_step<T, D, true>(kt, vt, lane, at, walk.in_run(t, mine), a.sl2, qf, m, l, o, met);
+        forward_step<T, D, true>(kt, vt, row, col, hf, at, walk.in_run(t, mine), a.sl2, qf, m, l, o, met);
     }
     if (met) add_keys<T, D, false>(walk, mine, sp * per + w, stop, NW, vbase, a.ldv, hf, o);
     l = pair_sum(l);
@@ -880,30 +878,6 @@ __global__ void __launch_bounds__(kNT) wa_join_kernel(const WaArgs a, int32_t B)
 }
 
 // ------------------------------------------------------------------------------- backward
-// r = do . out per (query, head), out with what its rounding left: dS = P (dP - r) cancels where one key
-// has most of a row, and out's rounding would be most of what is left.
-template <typename T, int D>
-__global__ void __launch_bounds__(kNT) wa_rowdot_kernel(const T* dout, const T* out, const T* lo, int64_t rows,
-                                                        float* r) {
-  constexpr int LPR = D / 8;
-  const int64_t row = ((int64_t)blockIdx.x * kNT + threadIdx.x) / LPR;
-  const int e0 = threadIdx.x % LPR * 8;
-  if (row >= rows) return;
-  float t = 0.f;
-#pragma unroll
-  for (int c = 0; c < 8; c += 16 / sizeof(T)) {
-    const u32x4_t x = *(const u32x4_t*)(dout + row * D + e0 + c), y = *(const u32x4_t*)(out + row * D + e0 + c);
-    u32x4_t z = {0, 0, 0, 0};
-    if (sizeof(T) == 2) z = *(const u32x4_t*)(lo + row * D + e0 + c);
-#pragma unroll
-    for (int e = 0; e < (int)(16 / sizeof(T)); ++e)
-      t = fmaf((float)((const T*)&x)[e], (float)((const T*)&y)[e] + (float)((const T*)&z)[e], t);
-  }
-#pragma unroll
-  for (int off = LPR / 2; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
-  if (e0 == 0) r[row] = t;
-}
-
 // Both gradient kernels: a block's waves own 32 rows (keys) each and share the tiles of the other side,
 // through two buffers in LDS; or, where that leaves CUs idle (SHARE), all own the same 32 and take the
 // tiles in turn, each through its own piece of LDS, and their sums are joined at the end.
@@ -913,8 +887,10 @@ __device__ __forceinline__ void tile_sync() {
   else __syncthreads();
 }
 
+// dq of 128 (32) rows, and r = do . out of each, which dk / dv read after it; out with what its rounding left:
+// dS = P (dP - r) cancels where one key has most of a row, and out's rounding would be most of what is left.
 template <typename T, int D, bool SHARE>
-__global__ void __launch_bounds__(kNT, 1) wa_dq_kernel(const WaArgs a) {
+__global__ void __launch_bounds__(kNT, sizeof(T) == 2 && !SHARE ? 2 : 1) wa_dq_kernel(const WaArgs a) {
   typedef Frag<T> F;
   typedef typename F::type Fr;
   typedef Tile<T, D> Ti;
@@ -948,7 +924,24 @@ __global__ void __launch_bounds__(kNT, 1) wa_dq_kernel(const WaArgs a) {
         df[st] = F::load(d + 16 * st);
       }
     }
-    const float lse = a.lse[at], r = a.r[at];
+    float r = 0.f;
+    {
+      const T* o = (const T*)a.out + at * D + 8 * hf;
+      const T* lo = (const T*)a.lo + at * D + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        const Fr of = F::load(o + 16 * st), lf = F::load((sizeof(T) == 2 ? lo : o) + 16 * st);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float y = (float)((const T*)&of)[e];
+          if (sizeof(T) == 2) y += (float)((const T*)&lf)[e];
+          r = fmaf((float)((const T*)&df[st])[e], y, r);
+        }
+      }
+      r = pair_sum(r);
+      if (hf == 0 && xw + l32 < n && (!SHARE || w == 0)) a.r[at] = r;
+    }
+    const float lse = a.lse[at];
     const Walk<kBK> walk(a, query_of(a, x0) + off, query_of(a, min(x0 + ROWS, n) - 1) + off, kv_len);
     const Seen mine = seen_from(a, query_of(a, x) + off, kv_len);
     const Seen wf = seen_from(a, query_of(a, min(xw, n - 1)) + off, kv_len);
@@ -969,15 +962,16 @@ __global__ void __launch_bounds__(kNT, 1) wa_dq_kernel(const WaArgs a) {
     };
     constexpr int STEP = SHARE ? 4 : 1;
     constexpr bool AHEAD = !SHARE || sizeof(T) == 2 || D == 64;
-    auto step = [&](const unsigned char* kt, const unsigned char* vt, auto masked, int k0, const Seen& s) {
+    int row = Ti::row_of(l32, hf), col = Ti::col_of(lane);
+    auto step = [&](const unsigned char* kt, const unsigned char* vt, auto masked, int k0, const Seen& s) __attribute__((always_inline)) {
       constexpr bool MASK = decltype(masked)::value;
       f32x16_t c, dp;
       clear(c);
       clear(dp);
 #pragma unroll
       for (int st = 0; st < KS; ++st) {
-        F::mma(Ti::row(kt, 0, l32, hf, st), qf[st], c);
-        F::mma(Ti::row(vt, 0, l32, hf, st), df[st], dp);
+        F::mma(Ti::row_at(kt, 0, row, st), qf[st], c);
+        F::mma(Ti::row_at(vt, 0, row, st), df[st], dp);
       }
       float d[16];
 #pragma unroll
@@ -986,24 +980,32 @@ __global__ void __launch_bounds__(kNT, 1) wa_dq_kernel(const WaArgs a) {
         if (MASK && !sees(s, k0 + 8 * (j >> 2) + 4 * hf + (j & 3))) d[j] = 0.f;
       }
       const Fr f[2] = {F::pack(d), F::pack(d + 8)};
-      add_rows<T, D, MASK>(kt, lane, f, acc, met);
+      add_rows<T, D, MASK>(kt, col, f, acc, met);
     };
-    int t = SHARE ? w : 0;
+    int t = SHARE ? w : 0, buf = 0, from, to;
+    walk.longest(&from, &to);
     if (AHEAD) load(t);
-    for (int buf = 0; t < nt; t += STEP, buf ^= 1) {
-      unsigned char *kt = lds + (SHARE ? w : buf) * 2 * TB, *vt = kt + TB;
-      if (!AHEAD) load(t);
-      if (SHARE) tile_sync<SHARE>();
-      ks.template store<false>(kt, tid);
-      vs.template store<false>(vt, tid);
-      tile_sync<SHARE>();
-      if (AHEAD) load(t + STEP);
-      int k0, end;
-      walk.tile(t, &k0, &end);
-      if (idle || !walk.any(t, wf, wl)) continue;
-      if (walk.full(t, wf, wl)) step(kt, vt, std::false_type(), k0, mine);
-      else step(kt, vt, std::true_type(), k0, walk.in_run(t, mine));
-    }
+    // One loop for the tiles with masks and one for those without: with both in one, the registers of its two arms
+    // do not fit.
+    auto tiles = [&](int stop, auto masked) __attribute__((always_inline)) {
+      for (; t < stop; t += STEP, buf ^= 1) {
+        asm volatile("" : "+v"(row), "+v"(col));  // no address made from them is kept from tile to tile
+        unsigned char *kt = lds + (SHARE ? w : buf) * 2 * TB, *vt = kt + TB;
+        if (!AHEAD) load(t);
+        if (SHARE) tile_sync<SHARE>();
+        ks.template store<false>(kt, tid);
+        vs.template store<false>(vt, tid);
+        tile_sync<SHARE>();
+        if (AHEAD) load(t + STEP);
+        int k0, end;
+        walk.tile(t, &k0, &end);
+        if (idle || (decltype(masked)::value && !walk.any(t, wf, wl))) continue;
+        step(kt, vt, masked, k0, decltype(masked)::value ? walk.in_run(t, mine) : mine);
+      }
+    };
+    tiles(from, std::true_type());
+    tiles(to, std::false_type());
+    tiles(nt, std::true_type());
     if (met) add_keys<T, D, true>(walk, mine, SHARE ? w : 0, nt, STEP, kbase, a.ldk, hf, acc);
     if (SHARE) join_waves<MT>((float*)lds, w, lane, acc);
     else __syncthreads();  // the next tile's rows go into these buffers
@@ -1032,7 +1034,7 @@ __device__ __forceinline__ Rows rows_of(const WaArgs& a, int k, int off, int q_l
 // sink_parts parts; 15143 tokens, 12 x 128 bf16, window 256, 16 sinks: the first tile's blocks took 28 times
 // the others' rows and 970 of the step's 1374 us).
 template <typename T, int D, bool SHARE, bool SINKS>
-__global__ void __launch_bounds__(kNT, 1) wa_dkv_kernel(const WaArgs a) {
+__global__ void __launch_bounds__(kNT, sizeof(T) == 2 && D == 64 && !SHARE ? 2 : 1) wa_dkv_kernel(const WaArgs a) {
   static_assert(SHARE || !SINKS, "sinks: 32 keys");
   typedef Frag<T> F;
   typedef typename F::type Fr;
@@ -1094,6 +1096,7 @@ __global__ void __launch_bounds__(kNT, 1) wa_dkv_kernel(const WaArgs a) {
     Rows mine = rows_of(a, ki, off, q_len);
     if (ki < first) mine.hi = mine.lo;  // another grid's
     if (kw < first) wave_hi = wave_lo;
+    if (k0 > ktile) all_hi = all_lo;  // a tile with keys of the other grid
     const bool idle = kw >= keys || kw + 32 <= first;
     if (SINKS) {  // a part of the rows, in whole tiles for the four waves
       const int per = ((run.hi - run.lo + a.sink_parts - 1) / a.sink_parts + 127) / 128 * 128;
@@ -1128,15 +1131,16 @@ __global__ void __launch_bounds__(kNT, 1) wa_dkv_kernel(const WaArgs a) {
         sv = tid < 32 ? a.lse[at] : a.r[at];
       }
     };
-    auto step = [&](const unsigned char* qt, const unsigned char* dt, const float(*st2)[BQ], int xb, auto masked) {
+    int row = Ti::row_of(l32, hf), col = Ti::col_of(lane);
+    auto step = [&](const unsigned char* qt, const unsigned char* dt, const float(*st2)[BQ], int xb, auto masked) __attribute__((always_inline)) {
       constexpr bool MASK = decltype(masked)::value;
       f32x16_t c, dp;
       clear(c);
       clear(dp);
 #pragma unroll
       for (int st = 0; st < KS; ++st) {
-        F::mma(Ti::row(qt, 0, l32, hf, st), kf[st], c);
-        F::mma(Ti::row(dt, 0, l32, hf, st), vf[st], dp);
+        F::mma(Ti::row_at(qt, 0, row, st), kf[st], c);
+        F::mma(Ti::row_at(dt, 0, row, st), vf[st], dp);
       }
       auto see = [&](int e) { return (uint32_t)(xb + e - mine.lo) < (uint32_t)(mine.hi - mine.lo); };
       float p[16], d[16];
@@ -1148,30 +1152,38 @@ __global__ void __launch_bounds__(kNT, 1) wa_dkv_kernel(const WaArgs a) {
         if (MASK && !see(e)) p[j] = d[j] = 0.f;
       }
       const Fr pf[2] = {F::pack(p), F::pack(p + 8)};
-      add_rows<T, D, MASK>(dt, lane, pf, dv, met);
+      add_rows<T, D, MASK>(dt, col, pf, dv, met);
       const Fr df[2] = {F::pack(d), F::pack(d + 8)};
-      add_rows<T, D, MASK>(qt, lane, df, dk, met);
+      add_rows<T, D, MASK>(qt, col, df, dk, met);
     };
-    int xb = run.lo + (SHARE ? w * BQ : 0);
+    int xb = run.lo + (SHARE ? w * BQ : 0), buf = 0;
     if (AHEAD) load(xb);
-    for (int buf = 0; xb < run.hi; xb += STEP, buf ^= 1) {
-      unsigned char *qt = lds + (SHARE ? w : buf) * 2 * TB, *dt = qt + TB;
-      float(*st2)[BQ] = stats[SHARE ? w : buf];
-      if (!AHEAD) load(xb);
-      if (SHARE) tile_sync<SHARE>();
+    // As in dq: tiles with masks, those that all keys see, and again with masks.
+    const int run_lo = SHARE ? wave_lo : all_lo, run_hi = SHARE ? wave_hi : all_hi;
+    auto tiles = [&](auto masked, auto more) __attribute__((always_inline)) {
+      for (; xb < run.hi && more(); xb += STEP, buf ^= 1) {
+        asm volatile("" : "+v"(row), "+v"(col));
+        unsigned char *qt = lds + (SHARE ? w : buf) * 2 * TB, *dt = qt + TB;
+        float(*st2)[BQ] = stats[SHARE ? w : buf];
+        if (!AHEAD) load(xb);
+        if (SHARE) tile_sync<SHARE>();
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int id = tid + NT * i;
-        Ti::put(qt, id / Ti::CPR, id % Ti::CPR, qr[i]);
-        Ti::put(dt, id / Ti::CPR, id % Ti::CPR, dr[i]);
+        for (int i = 0; i < NL; ++i) {
+          const int id = tid + NT * i;
+          Ti::put(qt, id / Ti::CPR, id % Ti::CPR, qr[i]);
+          Ti::put(dt, id / Ti::CPR, id % Ti::CPR, dr[i]);
+        }
+        if (tid < 64) st2[tid >> 5][tid & 31] = sv;
+        tile_sync<SHARE>();
+        if (AHEAD) load(xb + STEP);
+        if (idle || (decltype(masked)::value && (xb >= wrun.hi || xb + BQ <= wrun.lo))) continue;
+        step(qt, dt, st2, xb, masked);
       }
-      if (tid < 64) st2[tid >> 5][tid & 31] = sv;
-      tile_sync<SHARE>();
-      if (AHEAD) load(xb + STEP);
-      if (idle || xb >= wrun.hi || xb + BQ <= wrun.lo) continue;
-      if (xb >= wave_lo && xb + BQ <= wave_hi) step(qt, dt, st2, xb, std::false_type());
-      else step(qt, dt, st2, xb, std::true_type());
-    }
+    };
+    auto full = [&] { return xb >= run_lo && xb + BQ <= min(run_hi, run.hi); };
+    tiles(std::true_type(), [&] { return !full(); });
+    tiles(std::false_type(), full);
+    tiles(std::true_type(), [&] { return true; });
     if (met)
       for (int x = max(wrun.lo, run.lo); x < min(wrun.hi, run.hi); ++x) {
         const bool seen = x >= mine.lo && x < mine.hi;
@@ -1257,8 +1269,9 @@ Plan wa_plan(const WindowAttnSizes& z) {
   return p;
 }
 
-// The blocks that share the rows of a tile of sinks: as many as leave each about the rows of another key, in
-// scratch as above; 1: sinks are keys like others.
+// The blocks that share the rows of a tile of sinks: a block on each CU, of four waves' tiles of rows at least, in
+// scratch as above; 1: sinks are keys like others, whose blocks would not have twice the rows of another's.
+// (16384 tokens, 12 x 128 bf16, 4 sinks: 45 us in 30 parts, 54 in 7.)
 struct SinkPlan {
   int parts, keys;
   int64_t bytes;
@@ -1272,7 +1285,8 @@ SinkPlan sink_plan(const WindowAttnSizes& z) {
   const int64_t part = (int64_t)z.B * z.Hk * p.keys * 2 * z.D * 4;
   const int64_t es = z.dtype == TSC_F32 ? 4 : 2;
   const int64_t io = 2 * z.D * es * (z.total_q * z.H + z.total_kv * z.Hk);
-  p.parts = (int)std::min({z.max_q / rows, (int64_t)64, std::max(kScratchLeast, kScratchInputs * io) / part});
+  const int64_t blocks = (int64_t)p.keys / 32 * z.Hk * z.B, most = (int64_t)z.max_q * (z.H / z.Hk) / 128;
+  p.parts = (int)std::min({std::max<int64_t>(2, kCUs / blocks), most, std::max(kScratchLeast, kScratchInputs * io) / part});
   if (p.parts < 2) return {1, 0, 0};
   p.bytes = p.parts * part;
   return p;
@@ -1372,6 +1386,8 @@ int window_attention_backward_launch(tsc_ctx* ctx, const WindowAttnArgs& x, cons
   if (int st = too_many(z)) return st;
   WaArgs a = wa_args(x);
   a.lse = (float*)lse;
+  a.out = (void*)out;
+  a.lo = (void*)out_lo;
   a.dout = dout;
   a.r = (float*)ws;
   a.dq = dq;
@@ -1391,9 +1407,9 @@ int window_attention_backward_launch(tsc_ctx* ctx, const WindowAttnArgs& x, cons
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     if (rows > 0) {
-      ProfScope p(ctx, "window_attention_rowdot");
-      wa_rowdot_kernel<T, D><<<(unsigned)((rows * (D / 8) + kNT - 1) / kNT), kNT, 0, ctx->stream>>>(
-          (const T*)dout, (const T*)out, (const T*)out_lo, rows, (float*)ws);
+      ProfScope p(ctx, "window_attention_dq");
+      if (few_q) wa_dq_kernel<T, D, true><<<gq, kNT, 0, ctx->stream>>>(a);
+      else wa_dq_kernel<T, D, false><<<gq, kNT, 0, ctx->stream>>>(a);
     }
     {
       ProfScope p(ctx, "window_attention_dkv");
@@ -1405,11 +1421,6 @@ int window_attention_backward_launch(tsc_ctx* ctx, const WindowAttnArgs& x, cons
       const dim3 gs((unsigned)(sinks.keys / 32 * sinks.parts), (unsigned)z.Hk, (unsigned)z.B);
       wa_dkv_kernel<T, D, true, true><<<gs, kNT, 0, ctx->stream>>>(a);
       wa_sinks_kernel<T, D><<<dim3((unsigned)(sinks.keys / 4), (unsigned)z.Hk, (unsigned)z.B), kNT, 0, ctx->stream>>>(a);
-    }
-    if (rows > 0) {
-      ProfScope p(ctx, "window_attention_dq");
-      if (few_q) wa_dq_kernel<T, D, true><<<gq, kNT, 0, ctx->stream>>>(a);
-      else wa_dq_kernel<T, D, false><<<gq, kNT, 0, ctx->stream>>>(a);
     }
   });
 }
