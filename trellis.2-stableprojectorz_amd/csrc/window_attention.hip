@@ -1029,6 +1029,22 @@ __device__ __forceinline__ Rows rows_of(const WaArgs& a, int k, int off, int q_l
   return {(int)lo * a.G, (int)hi * a.G};
 }
 
+// The rows that see any of the keys first .. last, and those, [lo, hi), that see each of them.  Along the keys both
+// bounds grow, but for the sinks'.
+struct Spans {
+  Rows any;
+  int lo, hi;
+};
+__device__ __forceinline__ Spans spans_of(const WaArgs& a, int first, int last, int off, int q_len) {
+  const Rows f = rows_of(a, first, off, q_len), l = rows_of(a, last, off, q_len);
+  const Rows m = first < a.sinks && last >= a.sinks ? rows_of(a, a.sinks, off, q_len) : f;
+  Spans s;
+  s.any = {min(f.lo, l.lo), max(max(f.hi, l.hi), f.lo)};
+  s.lo = max(l.lo, f.lo);
+  s.hi = min(min(f.hi, l.hi), m.hi);
+  return s;
+}
+
 // dk and dv of 128 (32) keys of a key head, over the rows of all its query heads.  Every row sees the sinks: where
 // that is many times what sees another key, they are left to SINKS blocks (32 keys, and of their rows one of
 // sink_parts parts; 15143 tokens, 12 x 128 bf16, window 256, 16 sinks: the first tile's blocks took 28 times
@@ -1081,22 +1097,14 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && D == 64 && !SHARE ? 2 :
         vf[st] = F::load(d + 16 * st);
       }
     }
-    // The rows of the block's keys and of the wave's: along the keys both bounds grow, but for the sinks'.
-    auto span = [&](int first, int last, int* most, int* least) {  // of all keys; that see each of them
-      const Rows f = rows_of(a, first, off, q_len), l = rows_of(a, last, off, q_len);
-      const bool mixed = first < a.sinks && last >= a.sinks;
-      const Rows m = mixed ? rows_of(a, a.sinks, off, q_len) : f;
-      *most = max(l.lo, f.lo);
-      *least = min(min(f.hi, l.hi), m.hi);
-      return Rows{min(f.lo, l.lo), max(max(f.hi, l.hi), f.lo)};
-    };
-    int all_lo, all_hi, wave_lo, wave_hi;
-    Rows run = span(k0, (int)min(ktile + ROWS, (int64_t)keys) - 1, &all_lo, &all_hi);
-    const Rows wrun = span(min(max(kw, first), keys - 1), min(max(kw + 31, first), keys - 1), &wave_lo, &wave_hi);
+    Spans all = spans_of(a, k0, (int)min(ktile + ROWS, (int64_t)keys) - 1, off, q_len);
+    Spans own = spans_of(a, min(max(kw, first), keys - 1), min(max(kw + 31, first), keys - 1), off, q_len);
+    Rows run = all.any;
+    const Rows wrun = own.any;
     Rows mine = rows_of(a, ki, off, q_len);
     if (ki < first) mine.hi = mine.lo;  // another grid's
-    if (kw < first) wave_hi = wave_lo;
-    if (k0 > ktile) all_hi = all_lo;  // a tile with keys of the other grid
+    if (kw < first) own.hi = own.lo;
+    if (k0 > ktile) all.hi = all.lo;  // a tile with keys of the other grid
     const bool idle = kw >= keys || kw + 32 <= first;
     if (SINKS) {  // a part of the rows, in whole tiles for the four waves
       const int per = ((run.hi - run.lo + a.sink_parts - 1) / a.sink_parts + 127) / 128 * 128;
@@ -1159,7 +1167,7 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && D == 64 && !SHARE ? 2 :
     int xb = run.lo + (SHARE ? w * BQ : 0), buf = 0;
     if (AHEAD) load(xb);
     // As in dq: tiles with masks, those that all keys see, and again with masks.
-    const int run_lo = SHARE ? wave_lo : all_lo, run_hi = SHARE ? wave_hi : all_hi;
+    const int run_lo = SHARE ? own.lo : all.lo, run_hi = SHARE ? own.hi : all.hi;
     auto tiles = [&](auto masked, auto more) __attribute__((always_inline)) {
       for (; xb < run.hi && more(); xb += STEP, buf ^= 1) {
         asm volatile("" : "+v"(row), "+v"(col));
@@ -1213,6 +1221,172 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && D == 64 && !SHARE ? 2 :
         store_dims((T*)a.dv + at + 32 * mt, hf, dv[mt], 1.f);
       }
     }
+  }
+}
+
+// dk and dv of 128 keys at D = 128 in 16 bits: two waves to 32 keys.  With the sums of both gradients, k and v a wave
+// has the registers of its SIMD for itself, and the matrix cores wait for its exponentials and LDS reads (16384
+// tokens, 12 x 128, window 256 / 1024: 321 / 903 us).  Here one wave makes the scores, P and dv, and hands P on
+// through LDS, in fp32; the other makes dP and, a tile of rows later, dS and dk.  The same products, 16 a tile for
+// each, and none is made twice.  Tiles of 32 rows come through three buffers (q, read a tile later) and two.
+template <typename T>
+__global__ void __launch_bounds__(512, 2) wa_dkv_pair_kernel(const WaArgs a) {
+  constexpr int D = 128, KS = D / 16, MT = D / 32, BQ = 32, ROWS = 128;
+  typedef Frag<T> F;
+  typedef Tile<T, D> Ti;
+  constexpr int TB = BQ * Ti::ROWB;
+  static_assert(BQ * Ti::CPR == 512, "a chunk a thread");
+  __shared__ __attribute__((aligned(16))) unsigned char qbuf[3][TB], dbuf[2][TB];
+  __shared__ __attribute__((aligned(16))) float pbuf[2][4][16 * 64];
+  __shared__ __attribute__((aligned(16))) float stats[3][2][BQ];
+  int bx, h, bb;
+  block_tile(a.cu_q, &bx, &h, &bb);
+  int q0, q_len, kv0, kv_len;
+  segment(a.cu_q, bb, a.total_q, &q0, &q_len);
+  segment(a.cu_kv, bb, a.total_kv, &kv0, &kv_len);
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hf = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), pair = w & 3;
+  const bool of_k = w >= 4;  // the wave of dP and dk
+  const int H = a.Hk * a.G, off = kv_len - q_len, first = a.own_sinks ? a.sinks : 0;
+  if (a.rest) {
+    zero_rest((T*)a.dk, a.cu_kv, a.total_kv, bb, a.Hk, D, h, bx, gridDim.x, 1);
+    zero_rest((T*)a.dv, a.cu_kv, a.total_kv, bb, a.Hk, D, h, bx, gridDim.x, 1);
+  }
+  const T* qbase = (const T*)a.q + (int64_t)q0 * a.ldq;
+  const T* dbase = (const T*)a.dout + (int64_t)q0 * H * D;
+  const float scale = a.sl2 / kLog2e;
+
+  for (int64_t ktile = (int64_t)bx * ROWS; ktile < kv_len; ktile += (int64_t)gridDim.x * ROWS) {
+    if (ktile + ROWS <= first) continue;
+    const int k0 = max((int)ktile, first), kw = (int)ktile + pair * 32, ki = min(kw + l32, kv_len - 1);
+    const int64_t krow = kv0 + ki;
+    u32x4_t kv[KS];  // k of the wave's keys, or v
+    {
+      const T* p = (of_k ? (const T*)a.v + krow * a.ldv : (const T*)a.k + krow * a.ldk) + (int64_t)h * D + 8 * hf;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) kv[st] = F::load(p + 16 * st);
+    }
+    const Spans all = spans_of(a, k0, (int)min(ktile + ROWS, (int64_t)kv_len) - 1, off, q_len);
+    Spans own = spans_of(a, min(max(kw, first), kv_len - 1), min(max(kw + 31, first), kv_len - 1), off, q_len);
+    if (kw < first) own.hi = own.lo;
+    Rows mine = rows_of(a, ki, off, q_len);
+    if (ki < first) mine.hi = mine.lo;  // another grid's
+    const Rows run = all.any;
+    const bool idle = kw >= kv_len || kw + 32 <= first;
+    const int nt = (run.hi - run.lo + BQ - 1) / BQ;
+    f32x16_t acc[MT], dp;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) clear(acc[mt]);
+    bool met = false;
+    u32x4_t qr, dr;
+    float sv = 0.f;
+    auto load = [&](int i) {  // rows past the last one repeat it: they are masked
+      const int x = min(run.lo + BQ * i + tid / Ti::CPR, run.hi - 1), qi = query_of(a, x);
+      const int64_t hd = (int64_t)(h * a.G + x - qi * a.G) * D + tid % Ti::CPR * 8;
+      qr = *(const u32x4_t*)(qbase + qi * a.ldq + hd);
+      dr = *(const u32x4_t*)(dbase + (int64_t)qi * H * D + hd);
+      if (tid < 64) {
+        const int64_t at = q0 * (int64_t)H + row_at(a, H, h, min(run.lo + BQ * i + (tid & 31), run.hi - 1), 1);
+        sv = tid < 32 ? a.lse[at] : a.r[at];
+      }
+    };
+    auto at_work = [&](int i) {
+      const int xb = run.lo + BQ * i;
+      return i >= 0 && i < nt && !idle && xb < own.any.hi && xb + BQ > own.any.lo;
+    };
+    auto masked = [&](int i) { return run.lo + BQ * i < own.lo || run.lo + BQ * i + BQ > own.hi; };
+    auto see = [&](int i, int e) { return (uint32_t)(run.lo + BQ * i + e - mine.lo) < (uint32_t)(mine.hi - mine.lo); };
+    int row = Ti::row_of(l32, hf), col = Ti::col_of(lane);
+    // acc += rows of t weighted with s (rounded to T), what is not finite left out of tiles with masks.
+    auto add = [&](const unsigned char* t, const float(&s)[16], bool mask) __attribute__((always_inline)) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const u32x4_t sf = F::pack(s + 8 * g);
+        u32x4_t v[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) v[mt] = Ti::col_at(t, 0, col, g, mt);
+        if (mask) {
+          uint32_t bad = 0;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) bad |= odd<T>(v[mt]);
+          if (__builtin_amdgcn_ballot_w64(bad != 0)) {
+            met = true;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) v[mt] = finite<T>(v[mt]);
+          }
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) F::mma(v[mt], sf, acc[mt]);
+      }
+    };
+    if (nt > 0) load(0);
+    for (int i = 0; i <= nt; ++i) {
+      asm volatile("" : "+v"(row), "+v"(col));  // no address made from them is kept from tile to tile
+      if (i < nt) {
+        Ti::put(qbuf[i % 3], tid / Ti::CPR, tid % Ti::CPR, qr);
+        Ti::put(dbuf[i & 1], tid / Ti::CPR, tid % Ti::CPR, dr);
+        if (tid < 64) stats[i % 3][tid >> 5][tid & 31] = sv;
+      }
+      // What a buffer held before was last read one barrier ago at least: q and r of tile i - 3 and d and P of tile
+      // i - 2 in step i - 2 or (P) i - 1, whose readers have passed the last barrier or will pass this one first.
+      __syncthreads();
+      if (i + 1 < nt) load(i + 1);
+      if (!of_k) {
+        if (!at_work(i)) continue;
+        f32x16_t c;
+        clear(c);
+#pragma unroll
+        for (int st = 0; st < KS; ++st) F::mma(Ti::row_at(qbuf[i % 3], 0, row, st), kv[st], c);
+        const bool mask = masked(i);
+        float p[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) p[j] = fast_exp2(fmaf(c[j], a.sl2, -stats[i % 3][0][8 * (j >> 2) + 4 * hf + (j & 3)]));
+        if (mask) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (!see(i, 8 * (j >> 2) + 4 * hf + (j & 3))) p[j] = 0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(float4*)&pbuf[i & 1][pair][(g * 64 + lane) * 4] = make_float4(p[4 * g], p[4 * g + 1], p[4 * g + 2], p[4 * g + 3]);
+        add(dbuf[i & 1], p, mask);
+      } else {
+        if (at_work(i - 1)) {
+          const bool mask = masked(i - 1);
+          float d[16];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4 p = *(const float4*)&pbuf[(i - 1) & 1][pair][(g * 64 + lane) * 4];
+            d[4 * g] = p.x, d[4 * g + 1] = p.y, d[4 * g + 2] = p.z, d[4 * g + 3] = p.w;
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) d[j] *= dp[j] - stats[(i + 2) % 3][1][8 * (j >> 2) + 4 * hf + (j & 3)];
+          if (mask) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (!see(i - 1, 8 * (j >> 2) + 4 * hf + (j & 3))) d[j] = 0.f;
+          }
+          add(qbuf[(i + 2) % 3], d, mask);
+        }
+        if (at_work(i)) {
+          clear(dp);
+#pragma unroll
+          for (int st = 0; st < KS; ++st) F::mma(Ti::row_at(dbuf[i & 1], 0, row, st), kv[st], dp);
+        }
+      }
+    }
+    if (met)
+      for (int x = own.any.lo; x < own.any.hi; ++x) {
+        const bool seen = x >= mine.lo && x < mine.hi;
+        if (of_k) add_odd<T, D, true>(qbase + row_at(a, a.ldq, h, x, D), hf, seen, acc);
+        else add_odd<T, D, false>(dbase + row_at(a, (int64_t)H * D, h, x, D), hf, seen, acc);
+      }
+    if (kw + l32 < kv_len && kw + l32 >= first) {
+      T* p = (T*)(of_k ? a.dk : a.dv) + (krow * a.Hk + h) * D;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) store_dims(p + 32 * mt, hf, acc[mt], of_k ? scale : 1.f);
+    }
+    __syncthreads();  // the next keys' rows go into these buffers
   }
 }
 
@@ -1414,6 +1588,7 @@ int window_attention_backward_launch(tsc_ctx* ctx, const WindowAttnArgs& x, cons
     {
       ProfScope p(ctx, "window_attention_dkv");
       if (few_k) wa_dkv_kernel<T, D, true, false><<<gk, kNT, 0, ctx->stream>>>(a);
+      else if constexpr (sizeof(T) == 2 && D == 128) wa_dkv_pair_kernel<T><<<gk, 512, 0, ctx->stream>>>(a);
       else wa_dkv_kernel<T, D, false, false><<<gk, kNT, 0, ctx->stream>>>(a);
     }
     if (a.own_sinks) {
