@@ -738,7 +738,7 @@ __device__ __forceinline__ float2* part_stat(const WaArgs& a, int sp, int64_t at
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kNT) wa_few_kernel(const WaArgs a) {
+__global__ void __launch_bounds__(kNT, D == 64 || sizeof(T) == 2 ? 2 : 1) wa_few_kernel(const WaArgs a) {
   typedef Frag<T> F;
   typedef Tile<T, D> Ti;
   constexpr int KS = D / 16, MT = D / 32, NW = kNT / 64;
@@ -786,25 +786,31 @@ __global__ void __launch_bounds__(kNT) wa_few_kernel(const WaArgs a) {
       ks.load(kbase, a.ldk, at, end, lane);
       vs.load(vbase, a.ldv, at, end, lane);
     };
-    constexpr bool AHEAD = D == 64 || sizeof(T) == 2;  // registers for the next tile's rows
-    int t = sp * per + w, row = Ti::row_of(l32, hf), col = Ti::col_of(lane);
+    constexpr bool AHEAD = sizeof(T) == 2 && D == 64;  // registers for the next tile's rows
+    int t = sp * per + w, row = Ti::row_of(l32, hf), col = Ti::col_of(lane), from, to;
+    walk.longest(&from, &to);
     if (AHEAD) load(t);
-    for (; t < stop; t += NW) {
-      asm volatile("" : "+v"(row), "+v"(col));
-      if (!AHEAD) load(t);
-      int at, end;
-      walk.tile(t, &at, &end);
-      // A wave's LDS operations are carried out in order; the compiler has to keep that order.
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      ks.template store<false>(kt, lane);
-      vs.template store<false>(vt, lane);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if (AHEAD) load(t + NW);
-      if (walk.full(t, walk.first, walk.last))
-        forward_step<T, D, false>(kt, vt, row, col, hf, at, mine, a.sl2, qf, m, l, o, met);
-      else
-        forward_step<T, D, true>(kt, vt, row, col, hf, at, walk.in_run(t, mine), a.sl2, qf, m, l, o, met);
-    }
+    // One loop for the tiles with masks and one for those without: with both in one, the registers of its two arms
+    // do not fit.
+    auto tiles = [&](int end_t, auto masked) __attribute__((always_inline)) {
+      for (; t < end_t; t += NW) {
+        asm volatile("" : "+v"(row), "+v"(col));  // no address made from them is kept from tile to tile
+        if (!AHEAD) load(t);
+        int at, end;
+        walk.tile(t, &at, &end);
+        // A wave's LDS operations are carried out in order; the compiler has to keep that order.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        ks.template store<false>(kt, lane);
+        vs.template store<false>(vt, lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (AHEAD) load(t + NW);
+        constexpr bool MASK = decltype(masked)::value;
+        forward_step<T, D, MASK>(kt, vt, row, col, hf, at, MASK ? walk.in_run(t, mine) : mine, a.sl2, qf, m, l, o, met);
+      }
+    };
+    tiles(min(from, stop), std::true_type());
+    tiles(min(to, stop), std::false_type());
+    tiles(stop, std::true_type());
     if (met) add_keys<T, D, false>(walk, mine, sp * per + w, stop, NW, vbase, a.ldv, hf, o);
     l = pair_sum(l);
     if (hf == 0) {
@@ -890,7 +896,7 @@ __device__ __forceinline__ void tile_sync() {
 // dq of 128 (32) rows, and r = do . out of each, which dk / dv read after it; out with what its rounding left:
 // dS = P (dP - r) cancels where one key has most of a row, and out's rounding would be most of what is left.
 template <typename T, int D, bool SHARE>
-__global__ void __launch_bounds__(kNT, sizeof(T) == 2 && !SHARE ? 2 : 1) wa_dq_kernel(const WaArgs a) {
+__global__ void __launch_bounds__(kNT, D == 64 || (sizeof(T) == 2 && !SHARE) ? 2 : 1) wa_dq_kernel(const WaArgs a) {
   typedef Frag<T> F;
   typedef typename F::type Fr;
   typedef Tile<T, D> Ti;
@@ -961,7 +967,7 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && !SHARE ? 2 : 1) wa_dq_k
       vs.load(vbase, a.ldv, k0, end, tid);
     };
     constexpr int STEP = SHARE ? 4 : 1;
-    constexpr bool AHEAD = !SHARE || sizeof(T) == 2 || D == 64;
+    constexpr bool AHEAD = !SHARE || sizeof(T) == 2;
     int row = Ti::row_of(l32, hf), col = Ti::col_of(lane);
     auto step = [&](const unsigned char* kt, const unsigned char* vt, auto masked, int k0, const Seen& s) __attribute__((always_inline)) {
       constexpr bool MASK = decltype(masked)::value;
@@ -985,8 +991,7 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && !SHARE ? 2 : 1) wa_dq_k
     int t = SHARE ? w : 0, buf = 0, from, to;
     walk.longest(&from, &to);
     if (AHEAD) load(t);
-    // One loop for the tiles with masks and one for those without: with both in one, the registers of its two arms
-    // do not fit.
+    // As in wa_few_kernel: tiles with masks, those without, and again with masks.
     auto tiles = [&](int stop, auto masked) __attribute__((always_inline)) {
       for (; t < stop; t += STEP, buf ^= 1) {
         asm volatile("" : "+v"(row), "+v"(col));  // no address made from them is kept from tile to tile
@@ -1050,7 +1055,7 @@ __device__ __forceinline__ Spans spans_of(const WaArgs& a, int first, int last, 
 // sink_parts parts; 15143 tokens, 12 x 128 bf16, window 256, 16 sinks: the first tile's blocks took 28 times
 // the others' rows and 970 of the step's 1374 us).
 template <typename T, int D, bool SHARE, bool SINKS>
-__global__ void __launch_bounds__(kNT, sizeof(T) == 2 && D == 64 && !SHARE ? 2 : 1) wa_dkv_kernel(const WaArgs a) {
+__global__ void __launch_bounds__(kNT, D == 64 && (sizeof(T) == 2 || SHARE) ? 2 : 1) wa_dkv_kernel(const WaArgs a) {
   static_assert(SHARE || !SINKS, "sinks: 32 keys");
   typedef Frag<T> F;
   typedef typename F::type Fr;
@@ -1121,7 +1126,7 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && D == 64 && !SHARE ? 2 :
     u32x4_t qr[NL], dr[NL];
     float sv = 0.f;
     constexpr int STEP = SHARE ? 4 * BQ : BQ;
-    constexpr bool AHEAD = !SHARE || sizeof(T) == 2 || D == 64;
+    constexpr bool AHEAD = !SHARE || sizeof(T) == 2;
     // Rows past the last one repeat it: they are masked.
     auto load = [&](int xb) {
       if (xb >= run.hi) return;
@@ -1166,7 +1171,7 @@ __global__ void __launch_bounds__(kNT, sizeof(T) == 2 && D == 64 && !SHARE ? 2 :
     };
     int xb = run.lo + (SHARE ? w * BQ : 0), buf = 0;
     if (AHEAD) load(xb);
-    // As in dq: tiles with masks, those that all keys see, and again with masks.
+    // As there: tiles with masks, those that all keys see, and again with masks.
     const int run_lo = SHARE ? own.lo : all.lo, run_hi = SHARE ? own.hi : all.hi;
     auto tiles = [&](auto masked, auto more) __attribute__((always_inline)) {
       for (; xb < run.hi && more(); xb += STEP, buf ^= 1) {
@@ -1431,7 +1436,10 @@ Plan wa_plan(const WindowAttnSizes& z) {
   const int64_t hb = (int64_t)z.Hk * z.B, G = z.H / z.Hk;
   const int64_t max_q = std::max<int64_t>(z.max_q, (z.total_q + z.B - 1) / z.B);
   Plan p = {z.dtype == TSC_F32 ? kBQ : kBQ16, 1};
-  if ((int64_t)tiles_of(max_q * G, hb, kBQ) * hb >= kCUs) return p;
+  // Blocks of 32 rows, whose waves share their keys, while there are too few of the wide ones.  Measured, us, wide /
+  // 32 rows, window 256: 12 x 128 bf16, 2048 tokens 50 / 37, 3000 42 / 53; 16 x 64, 2048 tokens 38 / 30, 3000 37 / 43.
+  const int64_t wide = z.dtype != TSC_F32 && z.D == 64 ? 320 : kCUs;
+  if ((int64_t)tiles_of(max_q * G, hb, kBQ) * hb >= wide) return p;
   p.rows = 32;
   const int64_t blocks = (int64_t)tiles_of(max_q * G, hb, 32) * hb;
   if (blocks >= 2 * kCUs) return p;
