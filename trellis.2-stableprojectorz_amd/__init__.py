@@ -18,6 +18,7 @@ is not a Python identifier.
   SparseDiffAttentionBlock3d                     the block around it
   sparse_window_attention                        sliding window and first tokens that stay visible, shared
                                                  key heads, with gradients
+  SparseModulatedBlock3d                         the modulated transformer block around them
   SafetensorsFile, MultiFileLoader               weight files -> device tensors (weights.ts:58-237)
   workloads                                      seeded synthetic voxel shells
 """
@@ -31,7 +32,8 @@ from .ops import (NeighborMap, build_neighbor_map, map_conv_order, map_gather_pl
                   sparse_linear, sparse_attention, sparse_diff_attention, sparse_window_attention,
                   scaled_dot_product_attention)
 from .spatial import SparseSubdivide  # noqa: F401
-from .blocks import SparseLinear, SparseGroupNorm, SparseDiffAttentionBlock3d, SparseConvNeXtBlock3d  # noqa: F401
+from .blocks import (SparseLinear, SparseGroupNorm, SparseDiffAttentionBlock3d,  # noqa: F401
+                     SparseModulatedBlock3d, SparseConvNeXtBlock3d)
 from .weights import SafetensorsFile, SafetensorsHeader, TensorEntry, MultiFileLoader  # noqa: F401
 from . import workloads  # noqa: F401
 
@@ -40,7 +42,7 @@ __all__ = [
     "build_neighbor_map", "map_conv_order", "map_gather_plan", "sparse_conv3d", "layer_norm", "group_norm",
     "modulated_norm", "gated_residual", "gated_residual_norm", "silu", "add", "sparse_resblock",
     "sparse_subdivide", "subdivide_count", "SparseSubdivide", "sparse_linear", "SparseLinear", "SparseGroupNorm",
-    "SparseConvNeXtBlock3d", "SparseDiffAttentionBlock3d", "sparse_attention",
+    "SparseConvNeXtBlock3d", "SparseDiffAttentionBlock3d", "SparseModulatedBlock3d", "sparse_attention",
     "sparse_diff_attention", "sparse_window_attention", "scaled_dot_product_attention", "SafetensorsFile", "SafetensorsHeader", "TensorEntry", "MultiFileLoader",
     "get_neighbor_map", "neighbor_cache_key", "workloads",
 ]

@@ -1,15 +1,15 @@
-"""Sparse blocks around the conv: SparseLinear, the ConvNeXt block, group norm and the block of
-differential attention.
+"""Sparse blocks around the conv: SparseLinear, the ConvNeXt block, group norm, the block of
+differential attention and the modulated block of window attention.
 
   SparseLinear            src/sparse/ops/linear.ts:9-29 (nn.Linear per voxel; the TS port
                           multiplies by the (out,in) weight untransposed)
   SparseConvNeXtBlock3d   src/models/sparse_unet_vae_decoder.ts:48-78 and its use at :119-134:
                           h = conv(x); h = LN(h); h = h W0^T + b0; h = silu(LN(h)); out = x + h W2^T + b2
                           (LayerNorm without affine, eps 1e-6, as the TS block calls it)
-  SparseGroupNorm, SparseDiffAttentionBlock3d
+  SparseGroupNorm, SparseDiffAttentionBlock3d, SparseModulatedBlock3d
                           over each sample's voxels; no counterpart in the reference, whose blocks
-                          normalize rows (src/sparse/ops/norm.ts:10-140) and attend with one map
-                          (src/sparse/ops/attention.ts:24-79)
+                          normalize rows without modulation (src/sparse/ops/norm.ts:10-140) and attend
+                          with one map over whole samples (src/sparse/ops/attention.ts:24-79)
 
 Each step is one C-ABI call: the conv (tsc_conv, map cached on x), tsc_layernorm (SiLU fused into
 the second one), and tsc_linear (hipBLASLt GEMM with the bias epilogue; the second linear takes
@@ -83,6 +83,55 @@ class SparseDiffAttentionBlock3d:
                                       max_seqlen_q=longest, max_seqlen_kv=longest)
         return x.replace(ops.sparse_linear(h.view(n, c), self.out.weight, self.out.bias,
                                            residual=x.feats))
+
+    __call__ = forward
+
+
+class SparseModulatedBlock3d:
+    """A transformer block over each sample's voxels, in the order in which they stand (along a curve, register
+    tokens first), modulated per sample by mod = (shift1, scale1, gate1, shift2, scale2, gate2), (B, 6, C):
+
+        x = x + gate1 * out(window_attention(qkv(norm(x) * (1 + scale1) + shift1)))
+        x = x + gate2 * mlp2(silu(mlp1(norm(x) * (1 + scale2) + shift2)))
+
+    norm "layer" or "rms" without affine; post_norm, if given, normalizes what the gates take.  The residual
+    add, the gate and the second norm are one pass.  qkv weight ((num_heads + 2 num_kv_heads) D, C), read in
+    place as row slices, D 64 or 128; out weight (C, num_heads D).  Without gradients: its linear layers
+    have none (the norms and the attention do, around another library's linear layers)."""
+
+    def __init__(self, num_heads: int, window: int | None, qkv_weight: torch.Tensor,
+                 qkv_bias: torch.Tensor | None, out_weight: torch.Tensor, out_bias: torch.Tensor | None,
+                 mlp1_weight: torch.Tensor, mlp1_bias: torch.Tensor | None, mlp2_weight: torch.Tensor,
+                 mlp2_bias: torch.Tensor | None, num_kv_heads: int | None = None, sinks: int = 0,
+                 causal: bool = False, norm: str = "layer", post_norm: str | None = None,
+                 eps: float = 1e-6):
+        self.num_heads, self.num_kv_heads = num_heads, num_kv_heads or num_heads
+        self.window, self.sinks, self.causal = window, sinks, causal
+        self.norm, self.post_norm, self.eps = norm, post_norm, eps
+        self.qkv, self.out = SparseLinear(qkv_weight, qkv_bias), SparseLinear(out_weight, out_bias)
+        self.mlp1, self.mlp2 = SparseLinear(mlp1_weight, mlp1_bias), SparseLinear(mlp2_weight, mlp2_bias)
+
+    @torch.no_grad()
+    def forward(self, x: SparseTensor, mod: torch.Tensor) -> SparseTensor:
+        cu = x.cu_rows
+        b, c = cu.numel() - 1, x.feats.shape[1]
+        if mod.shape != (b, 6, c):
+            raise ValueError(f"mod must be ({b}, 6, {c}), got {tuple(mod.shape)}")
+        shift1, scale1, gate1, shift2, scale2, gate2 = mod.unbind(1)
+        longest = max(stop - start for start, stop in x.layout)
+        h = ops.modulated_norm(x.feats, cu, scale1, shift1, self.norm, eps=self.eps)
+        qkv = ops.sparse_linear(h, self.qkv.weight, self.qkv.bias)
+        hq, hk = self.num_heads, self.num_kv_heads
+        qkv = qkv.view(qkv.shape[0], hq + 2 * hk, -1)
+        a = ops.sparse_window_attention(qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:], self.window, cu,
+                                        sinks=self.sinks, causal=self.causal, max_seqlen_q=longest,
+                                        max_seqlen_kv=longest)
+        a = ops.sparse_linear(a.flatten(1), self.out.weight, self.out.bias)
+        r, h = ops.gated_residual_norm(x.feats, a, cu, gate1, post_norm=self.post_norm, norm=self.norm,
+                                       scale=scale2, shift=shift2, eps=self.eps)
+        h = ops.sparse_linear(h, self.mlp1.weight, self.mlp1.bias)
+        h = ops.sparse_linear(ops.silu(h, out=h), self.mlp2.weight, self.mlp2.bias)
+        return x.replace(ops.gated_residual(r, h, cu, gate2, post_norm=self.post_norm, eps=self.eps, out=h))
 
     __call__ = forward
 
