@@ -31,30 +31,36 @@ class GroupNorm(torch.autograd.Function):
 
 
 class GatedNorm(torch.autograd.Function):
+    """Takes (tensors, args, want_r, want_h) of ops._gated_norm, and of the tensors those that are there."""
+
     @staticmethod
     def forward(ctx, how, *given):
-        args, there, want_r, want_h = how
-        it = iter(given)
-        r, h, stats = ops._gated_norm([next(it) if t else None for t in there], args, want_r, want_h, None, True)
+        tensors, args, want_r, want_h = how
+        r, h, stats = ops._gated_norm(tensors, args, want_r, want_h, None, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(args[0], stats, *given)
-        ctx.how = (args[1:], there, want_r, want_h)
+        ctx.how = args[1:], [t is not None for t in tensors], want_r, want_h
         return (r, h) if want_r and want_h else r if want_r else h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *douts):
         args, there, want_r, want_h = ctx.how
-        douts = [None if d is None else d.contiguous() for d in douts]
         dr = douts[0] if want_r else None
         dh = douts[-1] if want_h else None
         if dr is None and dh is None:
             return (None,) * len(ctx.needs_input_grad)
+        dr = None if dr is None else dr.contiguous()
+        dh = None if dh is None else dh.contiguous()
         cu, stats, *given = ctx.saved_tensors
-        it, wanted = iter(given), iter(ctx.needs_input_grad[1:])
-        grads = ops._gated_norm_backward([next(it) if t else None for t in there], (cu, *args), stats, dr, dh,
-                                         [t and next(wanted) for t in there])
-        return (None, *(g for g, t in zip(grads, there) if t))
+        if not all(there):
+            it, wanted = iter(given), iter(ctx.needs_input_grad[1:])
+            given = [next(it) if t else None for t in there]
+            wanted = [t and next(wanted) for t in there]
+        else:
+            wanted = ctx.needs_input_grad[1:]
+        grads = ops._gated_norm_backward(given, (cu, *args), stats, dr, dh, wanted)
+        return (None, *[g for g, t in zip(grads, there) if t])
 
 
 class DiffAttention(torch.autograd.Function):

@@ -372,24 +372,31 @@ def _modulation(t, name: str, b: int, c: int, dtype):
         raise TscError(_lib.TSC_ERR_INVALID, f"{name}: each sample's {c} values must be contiguous")
 
 
-def _gated_norm_args(what: str, x, y, cu_rows, post, gate, residual_scale, pre, scale, shift, eps, out=None):
-    """Checks what the norms around a block are given; (tensors, arguments) of _gated_norm.  post and pre:
-    (kind, weight, bias), kind None where there is none."""
-    if x.dim() != 2 or x.shape[1] == 0:
-        raise TscError(_lib.TSC_ERR_INVALID, f"{what}: x must be (N, C)")
-    n, c = x.shape
-    dtype = x.dtype
-    if y is not None and (y.shape != x.shape or y.dtype != dtype):
-        raise TscError(_lib.TSC_ERR_INVALID, f"{what}: y must have x's shape and dtype")
-    for name, (kind, w, b) in (("post_norm", post), ("norm", pre)):
-        if kind not in _lib.NORMS:
-            raise TscError(_lib.TSC_ERR_INVALID, f"{what}: {name} must be 'layer' or 'rms', got {kind!r}")
-        if kind is None and (w is not None or b is not None):
+def _norm_kind(what: str, name: str, part, c: int, dtype) -> int:
+    """The C value of a norm (kind, weight, bias), kind None where there is none."""
+    kind, w, b = part
+    if kind not in _lib.NORMS:
+        raise TscError(_lib.TSC_ERR_INVALID, f"{what}: {name} must be 'layer' or 'rms', got {kind!r}")
+    if w is not None or b is not None:
+        if kind is None:
             raise TscError(_lib.TSC_ERR_INVALID, f"{what}: a weight or bias needs a {name}")
         for t in (w, b):
             if t is not None and (t.shape != (c,) or t.dtype != dtype):
                 raise TscError(_lib.TSC_ERR_INVALID, f"{what}: weights and biases must be ({c},) of x's dtype")
-    if out is not None and (out.shape != x.shape or out.dtype != dtype):
+    return _lib.NORMS[kind]
+
+
+def _gated_norm_args(what: str, x, y, cu_rows, post, gate, residual_scale, pre, scale, shift, eps, out=None):
+    """Checks what the norms around a block are given; (tensors, arguments) of _gated_norm.  post and pre:
+    (kind, weight, bias), kind None where there is none."""
+    shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    if len(shape) != 2 or shape[1] == 0:
+        raise TscError(_lib.TSC_ERR_INVALID, f"{what}: x must be (N, C)")
+    n, c = shape
+    if y is not None and (y.shape != shape or y.dtype != dtype):
+        raise TscError(_lib.TSC_ERR_INVALID, f"{what}: y must have x's shape and dtype")
+    kinds = _norm_kind(what, "post_norm", post, c, dtype), _norm_kind(what, "norm", pre, c, dtype)
+    if out is not None and (out.shape != shape or out.dtype != dtype):
         raise TscError(_lib.TSC_ERR_INVALID, f"{what}: out has the wrong shape or dtype")
     code = _code(x)
     eps, residual_scale = float(eps), float(residual_scale)
@@ -403,22 +410,25 @@ def _gated_norm_args(what: str, x, y, cu_rows, post, gate, residual_scale, pre, 
         b = cu_rows.numel() - 1
     else:
         b = 1 if cu_rows is None else len(cu_rows) - 1
+    lds = []
     for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
         if t is not None:
             _modulation(t, f"{what}: {name}", b, c, dtype)
-    dev = _dev(x, y, *post[1:], *pre[1:], out)
+        lds.append(0 if t is None else t.stride(0) if b > 1 else c)
+    for t in (x, y, post[1], post[2], pre[1], pre[2], out):
+        if t is not None and (t.get_device() != dev or dev < 0 or not t.is_contiguous()):
+            _dev(x, y, *post[1:], *pre[1:], out)  # says what it is
     for t in (gate, scale, shift):
-        if t is not None and (not t.is_cuda or t.device.index != dev):
+        if t is not None and t.get_device() != dev:
             raise TscError(_lib.TSC_ERR_INVALID, "tensors are not on one GPU; this path has no CPU fallback")
     cu = None
     if cu_rows is not None:
         _, cu = _cu_seqlens(cu_rows, n, dev, "cu_rows")
-        if cu.device.index != dev:
+        if cu.get_device() != dev:
             raise TscError(_lib.TSC_ERR_INVALID, "tensors live on different devices")
     if b and c > 8192:
         raise TscError(_lib.TSC_ERR_UNSUPPORTED, f"{what}: C={c} exceeds 8192")
-    lds = tuple(0 if t is None else t.stride(0) if b > 1 else c for t in (gate, scale, shift))
-    return tensors, (cu, b, _lib.NORMS[post[0]], _lib.NORMS[pre[0]], residual_scale, eps, code, lds)
+    return tensors, (cu, b, *kinds, residual_scale, eps, code, lds, dev)
 
 
 def modulated_norm(x: torch.Tensor, cu_rows=None, scale=None, shift=None, norm: str = "layer",
@@ -474,8 +484,7 @@ def _gated_norm_entry(what, tensors, args, want_r, want_h, out):
             raise TscError(_lib.TSC_ERR_INVALID, f"{what}: out cannot be given where gradients are wanted")
         from .autograd import GatedNorm
 
-        there = tuple(t is not None for t in tensors)
-        got = GatedNorm.apply((args, there, want_r, want_h), *(t for t in tensors if t is not None))
+        got = GatedNorm.apply((tensors, args, want_r, want_h), *[t for t in tensors if t is not None])
         return got if want_r and want_h else (got, got)
     return _gated_norm(tensors, args, want_r, want_h, out, False)[:2]
 
@@ -483,7 +492,7 @@ def _gated_norm_entry(what, tensors, args, want_r, want_h, out):
 def _gated_norm_call(tensors, args):
     """The arguments that both C calls share."""
     x, y, pw, pb, gate, w, bias, scale, shift = tensors
-    cu, b, post, pre, residual_scale, eps, code, lds = args
+    cu, b, post, pre, residual_scale, eps, code, lds, _ = args
     n, c = x.shape
     return (code, x.data_ptr(), _p(y), _p(cu), b, n, c, post, _p(pw), _p(pb), _p(gate), lds[0], residual_scale,
             pre, _p(w), _p(bias), _p(scale), lds[1], _p(shift), lds[2], eps)
@@ -499,7 +508,7 @@ def _gated_norm(tensors, args, want_r, want_h, out, keep):
     norms = int(want_h) + int(y is not None and post != _lib.TSC_NORM_NONE)
     stats = x.new_empty((norms, n, 2), dtype=torch.float32) if keep and norms else None
     if n and b:
-        lib, handle = _lib.stream_handle(x.device.index)
+        lib, handle = _lib.stream_handle(args[8])
         check(lib.tsc_gated_norm(handle, *_gated_norm_call(tensors, args), int(out is None), _p(stats), _p(r),
                                  _p(h)))
         _wrote(out)
@@ -525,7 +534,7 @@ def _gated_norm_backward(tensors, args, stats, dr, dh, wanted):
     dx = torch.empty_like(x) if dx is None else dx
     if y is not None and dy is None:
         dy = torch.empty_like(x)
-    lib, handle = _lib.stream_handle(x.device.index)
+    lib, handle = _lib.stream_handle(args[8])
     ws = new((max(lib.tsc_gated_norm_workspace_bytes(args[6], b, n, c), 16),), dtype=torch.uint8)
     check(lib.tsc_gated_norm_backward(handle, *_gated_norm_call(tensors, args), 1, _p(stats), _p(dr),
                                       _p(dh), ws.data_ptr(), dx.data_ptr(), _p(dy), _p(dgate), _p(dpw), _p(dpb),
@@ -660,13 +669,13 @@ def _cu_seqlens(cu, total: int, dev: int, what: str):
     A host sequence is checked non-decreasing within [0, total] and copied to the device.  A
     device tensor is taken as given (host None): reading it would synchronize the stream, and the
     kernels clamp every offset into [0, total], so a malformed array cannot read out of bounds."""
-    import numpy as np
-
     if isinstance(cu, torch.Tensor) and cu.is_cuda:
         if cu.dim() != 1 or cu.numel() < 1:
             raise TscError(_lib.TSC_ERR_INVALID, f"{what} must be a 1-D (B+1,) sequence")
         d = cu if cu.dtype == torch.int32 and cu.is_contiguous() else cu.to(torch.int32).contiguous()
         return None, d
+    import numpy as np
+
     host = (cu.detach().to("cpu", torch.int64).numpy() if isinstance(cu, torch.Tensor)
             else np.asarray(cu, np.int64))
     if host.ndim != 1 or host.size < 1:
@@ -887,14 +896,12 @@ def sparse_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
         raise TscError(_lib.TSC_ERR_INVALID, "window_attention: scale must be positive and finite in fp32")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
         raise TscError(_lib.TSC_ERR_INVALID, "window_attention: out has the wrong shape or dtype")
-    _code(q)
+    code = _code(q)
     _no_tangents("window_attention", q, k, v, out)
     lds = (_head_rows(q, "q"), _head_rows(k, "k"), _head_rows(v, "v"))
-    dev = _dev(out)
-    for t in (q, k, v):
-        if not t.is_cuda or dev is not None and t.device.index != dev:
-            raise TscError(_lib.TSC_ERR_INVALID, "tensors are not on one GPU; this path has no CPU fallback")
-        dev = t.device.index
+    dev = q.get_device()
+    if out is not None and _dev(out) != dev or dev < 0 or k.get_device() != dev or v.get_device() != dev:
+        raise TscError(_lib.TSC_ERR_INVALID, "tensors are not on one GPU; this path has no CPU fallback")
     cq_host, cq = _cu_seqlens(cu_seqlens_q, tq, dev, "cu_seqlens_q")
     if cu_seqlens_kv is None:
         if tkv != tq:
@@ -903,14 +910,13 @@ def sparse_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
         ck_host, ck = cq_host, cq
     else:
         ck_host, ck = _cu_seqlens(cu_seqlens_kv, tkv, dev, "cu_seqlens_kv")
-    for t in (cq, ck):
-        if t.device.index != dev:
-            raise TscError(_lib.TSC_ERR_INVALID, "tensors live on different devices")
+    if cq.get_device() != dev or ck.get_device() != dev:
+        raise TscError(_lib.TSC_ERR_INVALID, "tensors live on different devices")
     if ck.numel() != cq.numel():
         raise TscError(_lib.TSC_ERR_INVALID, "cu_seqlens_q and cu_seqlens_kv differ in length")
     b = cq.numel() - 1
     args = (cq, ck, b, float(scale) if scale is not None else 0.0, window, sinks, int(bool(causal)),
-            _longest(max_seqlen_q, cq_host, tq, b), _longest(max_seqlen_kv, ck_host, tkv, b), lds)
+            _longest(max_seqlen_q, cq_host, tq, b), _longest(max_seqlen_kv, ck_host, tkv, b), lds, code, dev)
     if _wants_grad(q, k, v, out):
         if out is not None:
             raise TscError(_lib.TSC_ERR_INVALID, "window_attention: out cannot be given where gradients "
@@ -933,7 +939,7 @@ def _longest(given, host, total: int, b: int) -> int:
 
 def _window_attention(q, k, v, args, out, keep):
     """(out, lo, lse); lo and lse (None unless keep) are what the backward pass needs."""
-    cq, ck, b, scale, window, sinks, causal, max_q, max_kv, lds = args
+    cq, ck, b, scale, window, sinks, causal, max_q, max_kv, lds, code, dev = args
     tq, h, d = q.shape
     tkv, hk = k.shape[:2]
     rest = out is None
@@ -942,8 +948,7 @@ def _window_attention(q, k, v, args, out, keep):
     lo = torch.empty_like(out) if keep and q.dtype != torch.float32 else None
     lse = q.new_empty((tq, h), dtype=torch.float32) if keep else None
     if tq and b:
-        lib, handle = _lib.stream_handle(q.device.index)
-        code = _code(q)
+        lib, handle = _lib.stream_handle(dev)
         nbytes = lib.tsc_window_attention_workspace_bytes(code, b, tq, tkv, h, hk, d, window, sinks, causal, max_q,
                                                           max_kv, 0)
         ws = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
@@ -956,14 +961,13 @@ def _window_attention(q, k, v, args, out, keep):
 
 
 def _window_attention_backward(do, q, k, v, out, lo, lse, args):
-    cq, ck, b, scale, window, sinks, causal, max_q, max_kv, lds = args
+    cq, ck, b, scale, window, sinks, causal, max_q, max_kv, lds, code, dev = args
     tq, h, d = q.shape
     tkv, hk = k.shape[:2]
     new = q.new_empty if b else q.new_zeros
     dq, dk, dv = new((tq, h, d)), new((tkv, hk, d)), new((tkv, hk, d))
     if b and (tq or tkv):
-        lib, handle = _lib.stream_handle(q.device.index)
-        code = _code(q)
+        lib, handle = _lib.stream_handle(dev)
         nbytes = lib.tsc_window_attention_workspace_bytes(code, b, tq, tkv, h, hk, d, window, sinks, causal, max_q,
                                                           max_kv, 1)
         ws = new((max(nbytes, 16),), dtype=torch.uint8)
