@@ -430,7 +430,7 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
  *   workspace  device scratch of tsc_window_attention_workspace_bytes(..., backward = 0) bytes, 16-byte
  *     aligned, NULL if that is 0.  The context keeps nothing.
  * fp32 softmax and accumulation; P is rounded to `dtype` for its product with v.  Infinities and NaN stay
- * with the queries that see them.
+ * with the queries that see them; a query whose scores are all -inf gives NaN.
  * No counterpart in the reference, whose attention is over whole samples (src/sparse/ops/attention.ts:24-79). */
 int64_t tsc_window_attention_workspace_bytes(int32_t dtype, int32_t B, int64_t total_q, int64_t total_kv,
                                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,

@@ -375,3 +375,50 @@ def test_wide_rows_and_c_refusals(pkg, dev):
         pkg.modulated_norm(buf[:128].view(4, 32), out=buf[4:132].view(4, 32))
     assert not pkg.modulated_norm(x, [0]).any()  # no samples: zeros
     assert pkg.modulated_norm(x[:0], [0, 0]).shape == (0, 32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", [100, 1536])
+def test_one_tensor_in_several_places(pkg, dev, dtype, c):
+    """x as y, and one modulation as gate, scale and shift: outputs as of copies, gradients summed over the places."""
+    t, d = _make([70, 30], c, dtype, 53, None)
+    t = {k: x.to(dev) for k, x in t.items()}
+    t["y"] = t["x"].clone()
+    t["scale"] = t["shift"] = t["gate"]
+    d = [x.to(dev) for x in d.values()]
+
+    def run(x, y, gate, scale, shift):
+        o = pkg.gated_residual_norm(x, y, [0, 70, 100], gate, weight=t["w"], bias=t["b"], scale=scale, shift=shift)
+        return o, torch.autograd.grad(o, list({id(a): a for a in (x, y, gate, scale, shift)}.values()), d)
+
+    names = ("x", "y", "gate", "scale", "shift")
+    apart, parts = run(*(t[k].clone().requires_grad_() for k in names))
+    x, m = t["x"].clone().requires_grad_(), t["gate"].clone().requires_grad_()
+    once, (dx, dm) = run(x, x, m, m, m)
+    assert torch.equal(once[0], apart[0]) and torch.equal(once[1], apart[1])
+    for got, of in ((dx, parts[:2]), (dm, parts[2:])):
+        size = sum(p.double().abs() for p in of)
+        # an addition in the type less than there are places, of half a step of at most the sum of the sizes each
+        eps = torch.finfo(dtype).eps
+        bound = (len(of) - 1) * eps / 2 * size * (1 + eps) + (2.0 ** -24 if dtype == torch.float16 else 0.0)
+        assert ((got.double() - sum(p.double() for p in of)).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype,c", [(torch.bfloat16, 8192), (torch.float16, 1000)])
+def test_more_than_two_to_the_31_values(pkg, dev, dtype, c):
+    """The last rows of a matrix of more than 2^31 values have what they have by themselves."""
+    n = 2 ** 31 // c + 5000
+    g = torch.Generator(device=dev).manual_seed(59)
+    x, y, dr, dh = (torch.randn((n, c), generator=g, device=dev, dtype=dtype) for _ in range(4))
+    m = (0.3 * torch.randn((2, 3, c), generator=g, device=dev)).to(dtype)
+    print(f"  {n} x {c} {dtype}", flush=True)
+
+    def run(rows, cu, mod):
+        leaves = [t[rows].detach().requires_grad_() for t in (x, y)]
+        r, h = pkg.gated_residual_norm(*leaves, cu, mod[:, 0], 0.5, "rms", scale=mod[:, 1], shift=mod[:, 2])
+        return (r.detach(), h.detach(), *torch.autograd.grad([r, h], leaves, [dr[rows], dh[rows]]))
+
+    all_rows = run(slice(None), [0, 3000, n], m)
+    last = run(slice(n - 900, n), [0, 900], m[1:])
+    for a, b in zip(all_rows, last):
+        assert torch.equal(a[-900:], b)

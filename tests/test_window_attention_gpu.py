@@ -472,3 +472,107 @@ def test_sinks_with_blocks_of_their_own(pkg, dev, dtype, d, lq, lkv, sinks, caus
     _both(pkg, dev, lq, lkv, h, hk, d, dtype, window, sinks, causal)
     if lkv is None:
         _both(pkg, dev, lq, lkv, h, hk, d, dtype, window, sinks, causal, max_seqlen_q=most[0], max_seqlen_kv=3 * sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lkv,h,hk", [([200], None, 2, 2), ([2500], None, 16, 16), ([1, 1], [3000, 40], 2, 1)])
+def test_scores_that_are_all_minus_infinity(pkg, dev, dtype, d, lq, lkv, h, hk):
+    """A softmax of nothing but -inf is NaN, in whichever blocks and parts the row is; of no keys at all it is
+    zeros; and rows that see other keys as well have what they have without those."""
+    q, k, v, do = _make(lq, lkv or lq, h, hk, d, dtype, 23)
+    cq, ck = _cu(lq), _cu(lkv or lq)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    print(f"  scores of -inf {dtype} D={d} {lq} {lkv}", flush=True)
+    if lkv is None:
+        k[100, :, 3] = -math.inf
+        got = {n: x.cpu() for n, x in _run(pkg, dev, q, k, v, do, 0, cq, ck, causal=True).items()}
+        others = torch.arange(sum(lq)) != 100
+        for n in got:  # query 100 sees key 100 alone, and nobody else does
+            assert got[n][100].isnan().all() and got[n][others].isfinite().all(), n
+        got = _run(pkg, dev, q, k, v, do, 5, cq, ck, causal=True)
+        assert got["out"].isfinite().all() and got["dv"].isfinite().all()
+        assert not got["dv"][100].any()
+    else:
+        k[:, :, 3] = -math.inf
+        got = pkg.sparse_window_attention(*(t.to(dev) for t in (q, k, v)), 5000, cq, ck)
+        assert got.isnan().all()
+        k[2500, :, 3] = 1.0  # the one key with a weight
+        got = pkg.sparse_window_attention(*(t.to(dev) for t in (q, k, v)), 5000, cq, ck)
+        alone = v[2500].repeat_interleave(h // hk, 0)
+        # its weight p may be a rounding of the score away from 1, and p v / p is three operations; in 16 bits p is 1
+        assert ((got[0].cpu().double() - alone.double()).abs() <= 4 * 2.0 ** -23 * alone.double().abs()).all()
+        assert got[1].isnan().all()
+    got = pkg.sparse_window_attention(q.to(dev), k[:0].to(dev), v[:0].to(dev), 5, cq, [0] * len(cq))
+    assert not got.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_one_tensor_as_all_inputs(pkg, dev, dtype, d):
+    """q, k and v in the same memory: the gradient is the sum of the three."""
+    q, _, _, do = _make([300], [300], 3, 3, d, dtype, 31)
+    one = q.to(dev).requires_grad_()
+    o = pkg.sparse_window_attention(one, one, one, 30, [0, 300], sinks=2)
+    g, = torch.autograd.grad(o, one, do.to(dev))
+    parts = _run(pkg, dev, q, q, q, do, 30, [0, 300], None, sinks=2)
+    assert torch.equal(o.detach(), parts["out"])
+    size = parts["dq"].double().abs() + parts["dk"].double().abs() + parts["dv"].double().abs()
+    total = parts["dq"].double() + parts["dk"].double() + parts["dv"].double()
+    # two additions in the type, of half a step of at most the sum of the sizes each
+    assert ((g.double() - total).abs() <= 2 * torch.finfo(dtype).eps / 2 * size * (1 + torch.finfo(dtype).eps)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("h,n", [(106, 300), (108, 300), (319, 70), (321, 70)])
+def test_grids_about_320_tiles(pkg, dev, dtype, h, n):
+    """Both sides of the rule for blocks of 256 rows at 64 dimensions in 16 bits."""
+    q, k, v, do = _make([n], [n], h, h, 64, dtype, h + n)
+    print(f"  window attention grid {dtype} H={h} n={n}", flush=True)
+    got = _run(pkg, dev, q, k, v, do, 60, [0, n], None, sinks=3)
+    hs = [0, h - 1]
+    want = _oracle(*(t[:, hs] for t in (q, k, v, do)), [0, n], [0, n], dtype, 60, 3)
+    for name in got:
+        check(got[name][:, hs], want[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_wide_row_strides(pkg, dev, dtype, d):
+    """Rows 2^24 values apart: offsets past 2^32 bytes and, within a tile, past 2^30; one value more is refused."""
+    n, h, ld = 220, 2, 1 << 24
+    q, k, v, do = _make([n], [n], h, h, d, dtype, 37)
+    print(f"  wide strides {dtype} D={d}", flush=True)
+    buf = torch.empty((n, ld), dtype=dtype, device=dev)
+    got = []
+    for t in (q, k, v):
+        view = buf[:, len(got) * h * d:(len(got) + 1) * h * d]
+        view.copy_(t.view(n, -1))
+        got.append(view.unflatten(1, (h, d)))
+    want = _run(pkg, dev, q, k, v, do, 50, [0, n], None, sinks=1)
+    leaves = [t.detach().requires_grad_() for t in got]
+    o = pkg.sparse_window_attention(*leaves, 50, [0, n], sinks=1)
+    assert torch.equal(o.detach(), want["out"])
+    for g, name in zip(torch.autograd.grad(o, leaves, do.to(dev)), ("dq", "dk", "dv")):
+        assert torch.equal(g, want[name]), name
+    far = torch.as_strided(buf, (2, h, d), (ld + 16, d, 1))
+    with pytest.raises(pkg.TscError, match="row stride"):
+        pkg.sparse_window_attention(far, far, far, 5, [0, 2])
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_more_than_two_to_the_31_values(pkg, dev, dtype, d):
+    """A million and more tokens: the last ones, of a second sequence, against the definition on what they see."""
+    h, n = 16, 2 ** 31 // (16 * d) + 5000
+    g = torch.Generator(device=dev).manual_seed(41)
+    q, k, v, do = (torch.randn((n, h, d), generator=g, device=dev, dtype=dtype) for _ in range(4))
+    got = {}
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = pkg.sparse_window_attention(*leaves, 40, [0, 3000, n])
+    got["out"] = o.detach()
+    got["dq"], got["dk"], got["dv"] = torch.autograd.grad(o, leaves, do)
+    tail, hs = 400, [0, h - 1]
+    want = _oracle(*(t[-tail:, hs].detach().cpu() for t in (q, k, v, do)), [0, tail], [0, tail], dtype, 40)
+    print(f"  {n} tokens {dtype} D={d}", flush=True)
+    for name in got:  # the cut row sees less; rows 80 on neither see it nor are seen through it
+        check(got[name][-tail + 80:, hs], tuple(x[80:] for x in want[name]), name)

@@ -141,6 +141,7 @@ struct Walk {
 __device__ __forceinline__ bool sees(const Seen& s, int k) {
   return (uint32_t)(k - s.lo) < (uint32_t)(s.hi - s.lo) || k < s.sink;
 }
+__device__ __forceinline__ bool sees_any(const Seen& s) { return s.hi > s.lo || s.sink > 0; }
 
 // ---- infinities and NaN where a row sees nothing ---------------------------------------------
 // Not 0 if an element is not finite: whether each half of a word, or a word, has all of its exponent's bits
@@ -273,11 +274,16 @@ __device__ __forceinline__ void forward_step(const unsigned char* kt, const unsi
   add_rows<T, D, MASK>(vt, col, pf, o, met);
 }
 
-// Writes a wave's finished rows: l summed over both halves, 0 where a row sees no key.
+// 1 / l; l = 0: the row sees no key, and gets zeros, or its scores are all -inf, of which a softmax is NaN.
+__device__ __forceinline__ float inverse(float l, bool some) { return l > 0.f || l != l ? 1.f / l : some ? NAN : 0.f; }
+__device__ __forceinline__ float row_lse(float m, float l, bool some) {
+  return l == 0.f ? (some ? NAN : INFINITY) : m + log2f(l);
+}
+// Writes a wave's finished rows: l summed over both halves; some: the row sees a key.
 template <typename T, int D>
-__device__ __forceinline__ void forward_store(const WaArgs& a, int64_t at, int hf, float l,
+__device__ __forceinline__ void forward_store(const WaArgs& a, int64_t at, int hf, float l, bool some,
                                               f32x16_t (&o)[D / 32]) {
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const float inv = inverse(l, some);
 #pragma unroll
   for (int mt = 0; mt < D / 32; ++mt) {
     T* p = (T*)a.out + at * D + 32 * mt;
@@ -293,8 +299,8 @@ __device__ __forceinline__ void forward_store(const WaArgs& a, int64_t at, int h
     }
   }
 }
-__device__ __forceinline__ void store_lse(const WaArgs& a, int64_t at, int hf, float m, float l) {
-  if (a.lse && hf == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
+__device__ __forceinline__ void store_lse(const WaArgs& a, int64_t at, int hf, float m, float l, bool some) {
+  if (a.lse && hf == 0) a.lse[at] = row_lse(m, l, some);
 }
 
 // fp32: a block of 4 waves owns 128 rows and walks their keys in tiles of 32.
@@ -368,8 +374,8 @@ __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward32_kernel(cons
     l = pair_sum(l);
     if (live) {
       const int64_t at = q0 * (int64_t)H + row_at(a, H, h, x, 1);
-      forward_store<T, D>(a, at, hf, l, o);
-      store_lse(a, at, hf, m, l);
+      forward_store<T, D>(a, at, hf, l, sees_any(mine), o);
+      store_lse(a, at, hf, m, l, sees_any(mine));
     }
   }
 }
@@ -713,14 +719,15 @@ __global__ void __launch_bounds__(64 * NW, 2) wa_forward16_kernel(const WaArgs a
     }
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-      if (met) add_keys<T, D, false>(walk, row_sees(i), 0, nblk, 1, vbase, a.ldv, hf, o[i]);
+      const Seen mine = row_sees(i);
+      if (met) add_keys<T, D, false>(walk, mine, 0, nblk, 1, vbase, a.ldv, hf, o[i]);
       const int x = xw + 32 * i + l32;
       l[i] = pair_sum(l[i]);
       if (KEEP) lu[i] = pair_sum(lu[i]);
       if (x < n) {
         const int64_t at = q0 * (int64_t)H + row_at(a, H, h, x, 1);
-        forward_store<T, D>(a, at, hf, l[i], o[i]);
-        if (KEEP) store_lse(a, at, hf, mc[i], lu[i]);
+        forward_store<T, D>(a, at, hf, l[i], sees_any(mine), o[i]);
+        if (KEEP) store_lse(a, at, hf, mc[i], lu[i], sees_any(mine));
       }
     }
     __syncthreads();  // the next row tile of this block stages over these buffers
@@ -834,12 +841,13 @@ __global__ void __launch_bounds__(kNT, D == 64 || sizeof(T) == 2 ? 2 : 1) wa_few
     if (w != 0 || x0 + l32 >= n) continue;
     const int64_t at = q0 * (int64_t)H + row_at(a, H, h, x, 1);
     if (a.splits == 1) {
-      forward_store<T, D>(a, at, hf, l, o);
-      store_lse(a, at, hf, m, l);
+      forward_store<T, D>(a, at, hf, l, sees_any(mine), o);
+      store_lse(a, at, hf, m, l, sees_any(mine));
     } else {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) store_dims(part_sums(a, sp, at, D) + 32 * mt, hf, o[mt], 1.f);
-      if (hf == 0) *part_stat(a, sp, at, D) = make_float2(m, l);
+      // A part without a weight of a row that sees a key has its maximum at -inf: the join tells such a row by it.
+      if (hf == 0) *part_stat(a, sp, at, D) = make_float2(l == 0.f && sees_any(mine) ? -INFINITY : m, l);
     }
   }
 }
@@ -861,6 +869,7 @@ __global__ void __launch_bounds__(kNT) wa_join_kernel(const WaArgs a, int32_t B)
   }
   if (__builtin_amdgcn_ballot_w64(in) == 0) return;
   float m = -FLT_MAX, l = 0.f, o[D / 64] = {};
+  bool some = false;
   for (int p = lane; p < a.splits; p += 64) m = fmaxf(m, part_stat(a, p, at, D)->x);
   for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
 #pragma unroll 4
@@ -868,11 +877,12 @@ __global__ void __launch_bounds__(kNT) wa_join_kernel(const WaArgs a, int32_t B)
     const float2 st = *part_stat(a, p, at, D);
     const float* po = part_sums(a, p, at, D);
     const float f = fast_exp2(st.x - m);
+    some |= st.x == -INFINITY;
     l = fmaf(st.y, f, l);
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) o[e] = fmaf(po[lane + 64 * e], f, o[e]);
   }
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const float inv = inverse(l, some);
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) {
     const int64_t p = at * D + lane + 64 * e;
@@ -880,7 +890,7 @@ __global__ void __launch_bounds__(kNT) wa_join_kernel(const WaArgs a, int32_t B)
     ((T*)a.out)[p] = (T)y;
     if (sizeof(T) == 2 && a.lo) ((T*)a.lo)[p] = (T)(y - (float)(T)y);
   }
-  if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
+  if (a.lse && lane == 0) a.lse[at] = row_lse(m, l, some);
 }
 
 // ------------------------------------------------------------------------------- backward
