@@ -22,6 +22,11 @@
 // The samples' sums have one order: a block adds up its rows of a sample in slot t + b of the scratch
 // (block t and sample b; along the rows one of the two grows at each step, so slots are distinct),
 // and a second kernel adds up each sample's slots.
+//
+// Measured (us; TB/s of what each pass has to read and write; a copy of 1 GiB reaches 5.1): forward, r and h of 243547 x
+// 512 bf16 186 (5.35), of 64304 x 1024 111 (4.8), h of 15143 x 1536 22 (4.2); gradient, both norms, of 243547 x 512 bf16
+// 339 (4.4) with the sums' kernel, of 60000 x 1024 fp32 357 (4.1), of 60000 x 1536 bf16 320 (3.4): with the sums of both
+// norms two waves a SIMD are left to wait for memory and for each row's two reductions.
 
 #include <algorithm>
 #include <initializer_list>
@@ -32,10 +37,18 @@
 namespace tsc {
 namespace {
 
-constexpr int kLaneF = 16, kLaneB = 8;  // most values of a wave's lane, forward and backward: wider rows have a block
-constexpr int kBackThreads = 512;  // threads of a block of the gradient, where a row has lanes of a wave
+// Most values of a wave's lane, forward and backward: wider rows have a block.  (64304 x 1024 bf16 with 16 in the
+// gradient 278 us, 253 in blocks; 60000 x 1024 fp32 776, 357: its registers spill.)
+constexpr int kLaneF = 16, kLaneB = 8;
+// Threads of a block of the gradient, where a row has lanes of a wave: its waves add up their sums in LDS.  (400000 x 256
+// bf16 in 256 threads 316 us, in 512 301.)
+constexpr int kBackThreads = 512;
 constexpr int kMaxC = 8192;     // widest row of a block of 16 waves
 constexpr int kSumCols = 16, kSumRows = 64, kSumWaves = kSumCols * kSumRows / 64;  // of a block that adds up slots
+// Rows on their way where a block of 16-byte vectors has both norms' gradients and two waves a SIMD: of few bytes each.
+// us, bf16, 1 / 2 / 3 / 4: 60000 x 1536 314 / 277 / 267 / 273, 30000 x 4096 403 / 353 / 341 / 348.  Others have more waves
+// (modulated_norm, 60000 x 1536: 149 with 1, 175 with 3) or no registers (16000 x 8192: 634, 1258).
+constexpr int kAhead = 3;
 constexpr int kLoopB = 16;      // samples that one block of that kernel walks
 
 struct GnArgs {
@@ -341,6 +354,7 @@ __device__ __forceinline__ void flush(const GnArgs& a, const Team<MAXV, BLOCK>& 
 // NT: threads of a block at most.  Rows of more than 4096 values, whose blocks have 1024, spill registers.
 template <typename T, int VN, int MAXV, bool BLOCK, int NT, bool Y, bool H>
 __global__ void __launch_bounds__(NT) gated_norm_backward_kernel(const GnArgs a) {
+  constexpr int AHEAD = sizeof(T) == 2 && VN == 8 && BLOCK && NT == 512 && Y && H ? kAhead : 1;  // rows on their way
   Team<MAXV, BLOCK> team(a.G);
   const int lane = team.lane, G = team.G, C = a.C, nvec = C / VN;
   const int64_t end = min(a.N, ((int64_t)blockIdx.x + 1) * a.R);
@@ -384,35 +398,36 @@ __global__ void __launch_bounds__(NT) gated_norm_backward_kernel(const GnArgs a)
       }
     }
     float P[MAXV][VN] = {}, Q[MAXV][VN] = {}, Py[MAXV][VN] = {}, Qy[MAXV][VN] = {};
-    Cols<T, VN, MAXV> xc, yc, dhc, drc;  // the next row's, on their way
-    float2 ysn = make_float2(0.f, 1.f), rsn = make_float2(0.f, 1.f);
-    auto load = [&](int64_t row) {
+    struct Ahead {  // a row's, on their way
+      Cols<T, VN, MAXV> x, y, dh, dr;
+      float2 ys = make_float2(0.f, 1.f), rs = make_float2(0.f, 1.f);
+    } ahead[AHEAD];
+    auto load = [&](Ahead& n, int64_t row) {
       if (row >= stop) return;
-      if (H) xc.load((const T*)a.x + row * C, lane, G, nvec);
-      if (Y) yc.load((const T*)a.y + row * C, lane, G, nvec);
-      if (H) dhc.load((const T*)a.dh + row * C, lane, G, nvec);
-      if (a.dr) drc.load((const T*)a.dr + row * C, lane, G, nvec);
-      if (Y && a.post != TSC_NORM_NONE) ysn = a.ystat[row];
-      if (H) rsn = a.rstat[row];
+      if (H) n.x.load((const T*)a.x + row * C, lane, G, nvec);
+      if (Y) n.y.load((const T*)a.y + row * C, lane, G, nvec);
+      if (H) n.dh.load((const T*)a.dh + row * C, lane, G, nvec);
+      if (a.dr) n.dr.load((const T*)a.dr + row * C, lane, G, nvec);
+      if (Y && a.post != TSC_NORM_NONE) n.ys = a.ystat[row];
+      if (H) n.rs = a.rstat[row];
     };
-    load(row0 + team.first);
-    for (int64_t lead = row0, row = row0 + team.first; lead < stop; lead += team.step, row += team.step) {
+    auto step = [&](Ahead& n, int64_t row) __attribute__((always_inline)) {
       const bool live = row < stop;
-      const float2 ys = ysn, rst = rsn;
-      const Cols<T, VN, MAXV> dr = drc;
+      const float2 ys = n.ys, rst = n.rs;
+      const Cols<T, VN, MAXV> dr = n.dr;
       float y[MAXV][VN], x[MAXV][VN], d[MAXV][VN], s2[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < MAXV; ++k) {
         const bool in = live && lane + G * k < nvec;
 #pragma unroll
         for (int e = 0; e < VN; ++e) {
-          y[k][e] = Y && in ? ((float)yc.v[k].v[e] - ys.x) * ys.y : 0.f;
+          y[k][e] = Y && in ? ((float)n.y.v[k].v[e] - ys.x) * ys.y : 0.f;
           d[k][e] = 0.f;
           if (H) {
-            float r = in ? (float)xc.v[k].v[e] : 0.f;
+            float r = in ? (float)n.x.v[k].v[e] : 0.f;
             if (Y) r = fmaf(a.rs, r, fmaf(gf[k][e], y[k][e], gs[k][e]));
             x[k][e] = in ? (r - rst.x) * rst.y : 0.f;
-            const float dh = in ? (float)dhc.v[k].v[e] : 0.f;
+            const float dh = in ? (float)n.dh.v[k].v[e] : 0.f;
             P[k][e] = fmaf(dh, x[k][e], P[k][e]);
             Q[k][e] += dh;
             d[k][e] = dh * hf[k][e];
@@ -421,7 +436,7 @@ __global__ void __launch_bounds__(NT) gated_norm_backward_kernel(const GnArgs a)
           }
         }
       }
-      load(row + team.step);
+      load(n, row + AHEAD * team.step);
       if (H) {
         team.sum(s2);
         const float m1 = a.norm == TSC_NORM_LAYER ? s2[0] * a.inv_c : 0.f, m2 = s2[1] * a.inv_c;
@@ -472,6 +487,13 @@ __global__ void __launch_bounds__(NT) gated_norm_backward_kernel(const GnArgs a)
         }
         if (live) store_row<T, VN, MAXV>((T*)a.dy + row * C, lane, G, nvec, d);
       }
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) load(ahead[i], row0 + team.first + i * team.step);
+    for (int64_t lead = row0; lead < stop; lead += AHEAD * team.step) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (i == 0 || lead + i * team.step < stop) step(ahead[i], lead + team.first + i * team.step);
     }
     if (a.sums) {
       const int64_t slot = (int64_t)blockIdx.x + b;
@@ -630,10 +652,21 @@ int64_t rows_of(const Shape& s, int64_t N, int64_t most) {
   const int64_t steps = (N + s.rows - 1) / s.rows;
   return s.rows * std::max<int64_t>(1, (steps + most - 1) / most);
 }
-constexpr int64_t kForwardBlocks = 2048;
-// Waves of the gradient: as many as run at once (more leave more sums to add up).
-constexpr int64_t kBackwardWaves = 4096;
-int64_t back_blocks(const Shape& s) { return kBackwardWaves * 64 / s.threads; }
+// Blocks of the forward pass: enough that those at work at one time are near each other in memory, and rows enough in
+// each for its sample's parameters.  us, r and h of bf16: 243547 x 512 in 2048 blocks 213, 8192 186, 16384 202;
+// 60000 x 1536 (rows of a block) in 2048 164, 4096 160; 16000 x 8192 in 2048 264, 4096 292; 64304 x 1024 (two vectors a
+// lane) in 2048 114, 4096 111.
+int64_t forward_blocks(const Shape& s, int64_t N) {
+  if (!s.block) return s.maxv == 1 ? 8192 : 4096;
+  return std::min<int64_t>(4096, std::max<int64_t>(1, N / 8));
+}
+// Waves of a CU in the gradient, by its registers: with the sums of r's norm and of y's (176 to 256), of one (92 to 128).
+constexpr int kBothWaves = 8, kOneWaves = 16;
+// Blocks of the gradient: as many as run at once; more of them leave more sums to add up.  us, both norms, bf16: 64304 x
+// 1024 253 with 8 waves a CU, 319 with 12 or 16; 60000 x 1536 374, 393, 454; 243547 x 512 339, 339, 355.
+int64_t back_blocks(const Shape& s, bool both) {
+  return 256 * std::max(1, (both ? kBothWaves : kOneWaves) * 64 / s.threads);
+}
 
 // A step's rows and with them the slots do not depend on the alignment: the scratch has room for both.
 int64_t slots_of(int32_t dtype, int32_t B, int64_t N, int32_t C) {
@@ -641,7 +674,7 @@ int64_t slots_of(int32_t dtype, int32_t B, int64_t N, int32_t C) {
   for (int v : {8, 4, 1}) {
     if (C % v || (v == 8 && dtype == TSC_F32)) continue;
     const Shape s = shape_of(C, v, kLaneB, kBackThreads);
-    const int64_t r = rows_of(s, N, back_blocks(s));
+    const int64_t r = rows_of(s, N, back_blocks(s, false));
     most = std::max(most, (N + r - 1) / r);
   }
   return most + B;
@@ -724,7 +757,7 @@ int gated_norm_launch(tsc_ctx* ctx, const GatedNormArgs& x, float* stats, void* 
   }
   const Shape s = shape_for(x, kLaneF, 256, {r, h});
   a.G = s.G;
-  a.R = rows_of(s, x.N, kForwardBlocks);
+  a.R = rows_of(s, x.N, forward_blocks(s, x.N));
   const unsigned grid = (unsigned)((x.N + a.R - 1) / a.R);
   ProfScope p(ctx, "gated_norm");
   by_shape<kLaneF>(x.dtype, s, [&](auto t, auto v, auto m, auto blk) {
@@ -761,7 +794,7 @@ int gated_norm_backward_launch(tsc_ctx* ctx, const GatedNormArgs& x, const float
   a.part = (float*)ws;
   const Shape s = shape_for(x, kLaneB, kBackThreads, {dr, dh, g.dx, g.dy});
   a.G = s.G;
-  a.R = rows_of(s, std::max<int64_t>(x.N, 1), back_blocks(s));
+  a.R = rows_of(s, std::max<int64_t>(x.N, 1), back_blocks(s, x.y && dh));
   if (x.N > 0) {
     const unsigned grid = (unsigned)((x.N + a.R - 1) / a.R);
     ProfScope p(ctx, "gated_norm_backward");
