@@ -303,7 +303,8 @@ __device__ __forceinline__ void store_lse(const WaArgs& a, int64_t at, int hf, f
   if (a.lse && hf == 0) a.lse[at] = row_lse(m, l, some);
 }
 
-// fp32: a block of 4 waves owns 128 rows and walks their keys in tiles of 32.
+// fp32: a block of 4 waves owns 128 rows and walks their keys in tiles of 32.  Bound by the fp32 products (151 TFLOP/s at
+// most): 3500 tokens of 12 x 128, window 256, 215 us, 50 TFLOP/s of the pairs that are seen.
 template <int D>
 __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward32_kernel(const WaArgs a) {
   typedef float T;
@@ -389,6 +390,12 @@ __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward32_kernel(cons
 // Blocks of 64 keys come through LDS, k one block ahead of v (three buffers, two).  The longest run of them of
 // which all rows see everything goes so; in the others, at the window's ends, a wave does one thing after the
 // other, puts masks on the scores where it has to, and leaves out the keys of which its rows see nothing.
+// Blocks of 256 rows: 16384 tokens of 12 x 128 bf16, window 512, take 171 us, in blocks of 128, of which LDS leaves one a CU,
+// 220.  Masks inside the pipelined steps, or two halves of a block at once at the ends, spill 100 registers and more.
+// Measured: 9000 + 6143 tokens, 12 x 128 bf16, window 512, 160 us, 580 of the 1117 TFLOP/s of a large product by the pairs
+// that are seen (of a tile a fifth is not): matrix cores busy 24 %, VALU 31 %; 20011 + 4097 tokens, 16 / 4 x 64 f16, window
+// 1023, causal, 160 us, 610 TFLOP/s, VALU 52 %.  What is left waits: a step's products for the exponentials before them, and
+// the blocks at the ends, a third of the steps there, do one thing after the other.
 // The sums of v are divided by the sum of the rounded P that they were made of.  KEEP (for the backward
 // pass) also adds up the unrounded P: the log-sum-exps have to be those of the fp32 probabilities.
 constexpr float kLazy = 8.f;  // log2 headroom before a running maximum is raised
@@ -736,7 +743,9 @@ __global__ void __launch_bounds__(64 * NW, 2) wa_forward16_kernel(const WaArgs a
 
 // Small grids: a block owns 32 rows, and its waves, and the blocks of a.splits parts, share out their key
 // tiles.  Each wave brings its own tiles through its own piece of LDS, so none waits for another until
-// the end, where their maxima, denominators and sums are joined.
+// the end, where their maxima, denominators and sums are joined.  Bound by latency: a wave's tile is loaded, brought
+// through LDS and multiplied before the next.  One token each on 33 to 20011 keys (16 / 4 x 128 bf16, window 4095, 52 MB):
+// 18 us, 2.9 TB/s, and 5 for the join; 311 + 1 + 150 tokens of 8 x 64 fp32 12 us.
 __device__ __forceinline__ float* part_sums(const WaArgs& a, int sp, int64_t at, int D) {
   return a.part + ((int64_t)sp * a.total_q * a.Hk * a.G + at) * D;
 }
@@ -793,7 +802,9 @@ __global__ void __launch_bounds__(kNT, D == 64 || sizeof(T) == 2 ? 2 : 1) wa_few
       ks.load(kbase, a.ldk, at, end, lane);
       vs.load(vbase, a.ldv, at, end, lane);
     };
-    constexpr bool AHEAD = sizeof(T) == 2 && D == 64;  // registers for the next tile's rows
+    // Whether there are registers for the next tile's rows.  (us, with / without: 16 x 64 bf16, 2048 tokens 20.6 / 21.8;
+    // 12 x 128 36.9 / 35.1; one token on 33 to 20011 keys, 16 / 4 x 64 fp32 27.1 / 24.9.)
+    constexpr bool AHEAD = sizeof(T) == 2 && D == 64;
     int t = sp * per + w, row = Ti::row_of(l32, hf), col = Ti::col_of(lane), from, to;
     walk.longest(&from, &to);
     if (AHEAD) load(t);
@@ -905,6 +916,9 @@ __device__ __forceinline__ void tile_sync() {
 
 // dq of 128 (32) rows, and r = do . out of each, which dk / dv read after it; out with what its rounding left:
 // dS = P (dP - r) cancels where one key has most of a row, and out's rounding would be most of what is left.
+// 15143 tokens of 12 x 128 bf16, window 256: 182 us, 500 MB from the L2s at 3.2 TB/s, matrix cores busy 18 %, VALU 27 %,
+// waves waiting 47 %: two of 256 registers a SIMD (15 spilled), each with its products and its exponentials in turn.  r in a
+// kernel of its own: 30 us less here, 25 there, and a launch more.
 template <typename T, int D, bool SHARE>
 __global__ void __launch_bounds__(kNT, D == 64 || (sizeof(T) == 2 && !SHARE) ? 2 : 1) wa_dq_kernel(const WaArgs a) {
   typedef Frag<T> F;
@@ -977,7 +991,9 @@ __global__ void __launch_bounds__(kNT, D == 64 || (sizeof(T) == 2 && !SHARE) ? 2
       vs.load(vbase, a.ldv, k0, end, tid);
     };
     constexpr int STEP = SHARE ? 4 : 1;
-    constexpr bool AHEAD = !SHARE || sizeof(T) == 2;
+    // The next tile's rows on their way.  With SHARE the registers for them spill: both gradients, 1000 tokens of 12 x 128
+    // bf16 78 us, 73 without; 8 / 2 x 64 fp32 149, 117.
+    constexpr bool AHEAD = !SHARE;
     int row = Ti::row_of(l32, hf), col = Ti::col_of(lane);
     auto step = [&](const unsigned char* kt, const unsigned char* vt, auto masked, int k0, const Seen& s) __attribute__((always_inline)) {
       constexpr bool MASK = decltype(masked)::value;
@@ -1063,7 +1079,8 @@ __device__ __forceinline__ Spans spans_of(const WaArgs& a, int first, int last, 
 // dk and dv of 128 (32) keys of a key head, over the rows of all its query heads.  Every row sees the sinks: where
 // that is many times what sees another key, they are left to SINKS blocks (32 keys, and of their rows one of
 // sink_parts parts; 15143 tokens, 12 x 128 bf16, window 256, 16 sinks: the first tile's blocks took 28 times
-// the others' rows and 970 of the step's 1374 us).
+// the others' rows and 970 of the step's 1374 us; now 30 and 4 for adding up the parts).  Spills up to 18 registers at
+// D = 64 and two waves a SIMD.
 template <typename T, int D, bool SHARE, bool SINKS>
 __global__ void __launch_bounds__(kNT, D == 64 && (sizeof(T) == 2 || SHARE) ? 2 : 1) wa_dkv_kernel(const WaArgs a) {
   static_assert(SHARE || !SINKS, "sinks: 32 keys");
@@ -1136,7 +1153,7 @@ __global__ void __launch_bounds__(kNT, D == 64 && (sizeof(T) == 2 || SHARE) ? 2 
     u32x4_t qr[NL], dr[NL];
     float sv = 0.f;
     constexpr int STEP = SHARE ? 4 * BQ : BQ;
-    constexpr bool AHEAD = !SHARE || sizeof(T) == 2;
+    constexpr bool AHEAD = !SHARE;  // as there
     // Rows past the last one repeat it: they are masked.
     auto load = [&](int xb) {
       if (xb >= run.hi) return;
@@ -1244,6 +1261,8 @@ __global__ void __launch_bounds__(kNT, D == 64 && (sizeof(T) == 2 || SHARE) ? 2 
 // tokens, 12 x 128, window 256 / 1024: 321 / 903 us).  Here one wave makes the scores, P and dv, and hands P on
 // through LDS, in fp32; the other makes dP and, a tile of rows later, dS and dk.  The same products, 16 a tile for
 // each, and none is made twice.  Tiles of 32 rows come through three buffers (q, read a tile later) and two.
+// Measured: 274 / 692 us there (64 rows a tile, which spill 72 registers: 338 / 799); 275 for 9000 + 6143 tokens, window 256,
+// matrix cores busy 15 %, VALU 39 %, waiting 41 %: a barrier a tile, and both waves of a pair wait for the longer half.
 template <typename T>
 __global__ void __launch_bounds__(512, 2) wa_dkv_pair_kernel(const WaArgs a) {
   constexpr int D = 128, KS = D / 16, MT = D / 32, BQ = 32, ROWS = 128;
@@ -1453,11 +1472,13 @@ Plan wa_plan(const WindowAttnSizes& z) {
   p.rows = 32;
   const int64_t blocks = (int64_t)tiles_of(max_q * G, hb, 32) * hb;
   if (blocks >= 2 * kCUs) return p;
+  // Parts of 512 keys at least, four tiles a wave.  (us, 256 / 512 / 1024: one token on 33 to 20011 keys, 16 / 4 x 128 bf16,
+  // window 4095: 23.2 / 21.1 / 23.1; x 64 fp32 25.0 / 25.0 / 33.7; 1000 tokens of 8 / 2 x 64 fp32, window 256: 25 / 20 / 20.)
   const int64_t span = std::min<int64_t>(z.max_kv, (z.causal ? 1 : 2) * (int64_t)z.window + 32 + z.sinks);
   const int64_t es = z.dtype == TSC_F32 ? 4 : 2;
   const int64_t io = 2 * z.D * es * (z.total_q * z.H + z.total_kv * z.Hk);
   const int64_t room = std::max(kScratchLeast, kScratchInputs * io) / std::max<int64_t>(1, part_bytes(z.total_q, z.H, z.D));
-  p.splits = (int)std::max<int64_t>(1, std::min({span / 256, 2 * kCUs / blocks, room}));
+  p.splits = (int)std::max<int64_t>(1, std::min({span / 512, 2 * kCUs / blocks, room}));
   return p;
 }
 
@@ -1586,8 +1607,12 @@ int window_attention_backward_launch(tsc_ctx* ctx, const WindowAttnArgs& x, cons
   a.dk = dk;
   a.dv = dv;
   const int64_t hb = (int64_t)z.Hk * z.B, rows = z.total_q * z.H;
-  const bool few_q = (int64_t)tiles_of((int64_t)z.max_q * a.G, hb, kBQ) * hb < kCUs;
-  const bool few_k = (int64_t)tiles_of(z.max_kv, hb, kBQ) * hb < kCUs;
+  // SHARE where blocks of 128 would leave CUs idle; in 16 bits where they would half of them, a wave's own tiles being quick
+  // and the joint at the end not.  Both gradients, us, 128 / 32: 192 tiles of 12 x 128 bf16, 2048 tokens 81 / 119; 128 of
+  // 16 x 64, 1000 tokens 49 / 68; 96 of 12 x 128, 1000 tokens 80 / 72; fp32, 8 / 2 x 64, 2048 tokens 154 / 133.
+  const int64_t few = z.dtype == TSC_F32 ? kCUs : kCUs / 2;
+  const bool few_q = (int64_t)tiles_of((int64_t)z.max_q * a.G, hb, kBQ) * hb < few;
+  const bool few_k = (int64_t)tiles_of(z.max_kv, hb, kBQ) * hb < few;
   const dim3 gq(tiles_of((int64_t)z.max_q * a.G, hb, few_q ? 32 : kBQ), (unsigned)z.Hk, (unsigned)z.B);
   const dim3 gk(tiles_of(z.max_kv, hb, few_k ? 32 : kBQ), (unsigned)z.Hk, (unsigned)z.B);
   const SinkPlan sinks = rows > 0 ? sink_plan(z) : SinkPlan{1, 0, 0};
