@@ -39,13 +39,13 @@ class GatedNorm(torch.autograd.Function):
         r, h, stats = ops._gated_norm(tensors, args, want_r, want_h, None, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(args[0], stats, *given)
-        ctx.how = args[1:], [t is not None for t in tensors], want_r, want_h
+        ctx.how = args[1:], [t is not None for t in tensors], want_r, want_h, None if stats is None else stats.shape
         return (r, h) if want_r and want_h else r if want_r else h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *douts):
-        args, there, want_r, want_h = ctx.how
+        args, there, want_r, want_h, stats_shape = ctx.how
         dr = douts[0] if want_r else None
         dh = douts[-1] if want_h else None
         if dr is None and dh is None:
@@ -59,7 +59,7 @@ class GatedNorm(torch.autograd.Function):
             wanted = [t and next(wanted) for t in there]
         else:
             wanted = ctx.needs_input_grad[1:]
-        grads = ops._gated_norm_backward(given, (cu, *args), stats, dr, dh, wanted)
+        grads = ops._gated_norm_backward(given, (cu, *args), stats, stats_shape, dr, dh, wanted)
         return (None, *[g for g, t in zip(grads, there) if t])
 
 
@@ -85,10 +85,10 @@ class DiffAttention(torch.autograd.Function):
 
 class WindowAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, args):
-        out, lo, lse = ops._window_attention(q, k, v, args, None, True)
+    def forward(ctx, q, k, v, lds, args):
+        out, lo, lse = ops._window_attention(q, k, v, lds, args, None, True)
         ctx.save_for_backward(q, k, v, out, lo, lse, *args[:2])
-        ctx.args = args[2:]
+        ctx.kv_shape, ctx.args = k.shape, args[2:]
         return out
 
     @staticmethod
@@ -98,4 +98,5 @@ class WindowAttention(torch.autograd.Function):
         do = do.contiguous()
         if do.data_ptr() % 16:  # a view into a larger gradient
             do = do.clone()
-        return (*ops._window_attention_backward(do, q, k, v, out, lo, lse, (cq, ck, *ctx.args)), None)
+        grads = ops._window_attention_backward(do, q, k, v, out, lo, lse, ctx.kv_shape, (cq, ck, *ctx.args))
+        return (*grads, None, None)

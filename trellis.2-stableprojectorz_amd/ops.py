@@ -287,6 +287,20 @@ def _no_tangents(what: str, *ts) -> None:
         raise TscError(_lib.TSC_ERR_UNSUPPORTED, f"{what}: no forward-mode derivative (dual tensor)")
 
 
+def _restored(t, shape, dtype, dev: int, align: int = 1, strided=None):
+    """A tensor that autograd saved, as the C calls take it: contiguous, or with rows that `strided` finds fit,
+    and aligned.  Hooks on saved tensors (offloading, say) may give back the values in another layout than the
+    forward call's."""
+    if t is None:
+        return None
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
+        raise TscError(_lib.TSC_ERR_INVALID, f"a saved tensor of {tuple(shape)} {dtype} on GPU {dev} came back as "
+                                             f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    if not t.is_contiguous() and (strided is None or not strided(t)):
+        t = t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % align else t
+
+
 def group_norm(x: torch.Tensor, num_groups: int, weight=None, bias=None, cu_rows=None,
                eps: float = 1e-5, silu: bool = False, out=None) -> torch.Tensor:
     """Group norm over the rows of each sample, channels last (fp32 statistics), optionally fused
@@ -364,11 +378,17 @@ def _group_norm_backward(dy, x, weight, bias, cu, b, groups, silu, stats, want_p
     return dx, dw, db
 
 
+def _strided_rows(t) -> bool:
+    """Whether a (B, C) tensor's rows are contiguous and apart."""
+    b, c = t.shape
+    return not (t.stride(1) != 1 and c > 1 or t.stride(0) < c and b > 1)
+
+
 def _modulation(t, name: str, b: int, c: int, dtype):
     """A (B, C) tensor whose rows may be strided: a gate, a scale or a shift of each sample."""
     if t.shape != (b, c) or t.dtype != dtype:
         raise TscError(_lib.TSC_ERR_INVALID, f"{name} must be ({b}, {c}) of x's dtype, got {tuple(t.shape)} {t.dtype}")
-    if t.stride(1) != 1 and c > 1 or t.stride(0) < c and b > 1:
+    if not _strided_rows(t):
         raise TscError(_lib.TSC_ERR_INVALID, f"{name}: each sample's {c} values must be contiguous")
 
 
@@ -410,11 +430,9 @@ def _gated_norm_args(what: str, x, y, cu_rows, post, gate, residual_scale, pre, 
         b = cu_rows.numel() - 1
     else:
         b = 1 if cu_rows is None else len(cu_rows) - 1
-    lds = []
     for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
         if t is not None:
             _modulation(t, f"{what}: {name}", b, c, dtype)
-        lds.append(0 if t is None else t.stride(0) if b > 1 else c)
     for t in (x, y, post[1], post[2], pre[1], pre[2], out):
         if t is not None and (t.get_device() != dev or dev < 0 or not t.is_contiguous()):
             _dev(x, y, *post[1:], *pre[1:], out)  # says what it is
@@ -428,7 +446,7 @@ def _gated_norm_args(what: str, x, y, cu_rows, post, gate, residual_scale, pre, 
             raise TscError(_lib.TSC_ERR_INVALID, "tensors live on different devices")
     if b and c > 8192:
         raise TscError(_lib.TSC_ERR_UNSUPPORTED, f"{what}: C={c} exceeds 8192")
-    return tensors, (cu, b, *kinds, residual_scale, eps, code, lds, dev)
+    return tensors, (cu, b, *kinds, residual_scale, eps, code, dev)
 
 
 def modulated_norm(x: torch.Tensor, cu_rows=None, scale=None, shift=None, norm: str = "layer",
@@ -492,8 +510,10 @@ def _gated_norm_entry(what, tensors, args, want_r, want_h, out):
 def _gated_norm_call(tensors, args):
     """The arguments that both C calls share."""
     x, y, pw, pb, gate, w, bias, scale, shift = tensors
-    cu, b, post, pre, residual_scale, eps, code, lds, _ = args
+    cu, b, post, pre, residual_scale, eps, code, _ = args
     n, c = x.shape
+    # Of these tensors: the gradient's may have other strides than the forward call's.
+    lds = [0 if t is None else t.stride(0) if b > 1 else c for t in (gate, scale, shift)]
     return (code, x.data_ptr(), _p(y), _p(cu), b, n, c, post, _p(pw), _p(pb), _p(gate), lds[0], residual_scale,
             pre, _p(w), _p(bias), _p(scale), lds[1], _p(shift), lds[2], eps)
 
@@ -508,18 +528,24 @@ def _gated_norm(tensors, args, want_r, want_h, out, keep):
     norms = int(want_h) + int(y is not None and post != _lib.TSC_NORM_NONE)
     stats = x.new_empty((norms, n, 2), dtype=torch.float32) if keep and norms else None
     if n and b:
-        lib, handle = _lib.stream_handle(args[8])
+        lib, handle = _lib.stream_handle(args[7])
         check(lib.tsc_gated_norm(handle, *_gated_norm_call(tensors, args), int(out is None), _p(stats), _p(r),
                                  _p(h)))
         _wrote(out)
     return r, h, stats
 
 
-def _gated_norm_backward(tensors, args, stats, dr, dh, wanted):
+def _gated_norm_backward(tensors, args, stats, stats_shape, dr, dh, wanted):
     """The gradients of `tensors`, None where there is none or `wanted` says so."""
-    x, y = tensors[:2]
-    b = args[1]
-    n, c = x.shape
+    like = dr if dh is None else dh
+    shape, dtype, b, dev = like.shape, like.dtype, args[1], args[7]
+    n, c = shape
+    x, y = (_restored(t, shape, dtype, dev) for t in tensors[:2])
+    pw, pb, w, bias = (_restored(tensors[i], (c,), dtype, dev) for i in (2, 3, 5, 6))
+    gate, scale, shift = (_restored(tensors[i], (b, c), dtype, dev, 1, _strided_rows) for i in (4, 7, 8))
+    tensors = (x, y, pw, pb, gate, w, bias, scale, shift)
+    stats = _restored(stats, stats_shape, torch.float32, dev, 8)
+    args = (_restored(args[0], (b + 1,), torch.int32, dev), *args[1:])
     if n == 0:
         return [None if t is None else torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
     # Without dh the norm before the next block has no gradient, and neither has its modulation.
@@ -534,7 +560,7 @@ def _gated_norm_backward(tensors, args, stats, dr, dh, wanted):
     dx = torch.empty_like(x) if dx is None else dx
     if y is not None and dy is None:
         dy = torch.empty_like(x)
-    lib, handle = _lib.stream_handle(args[8])
+    lib, handle = _lib.stream_handle(args[7])
     ws = new((max(lib.tsc_gated_norm_workspace_bytes(args[6], b, n, c), 16),), dtype=torch.uint8)
     check(lib.tsc_gated_norm_backward(handle, *_gated_norm_call(tensors, args), 1, _p(stats), _p(dr),
                                       _p(dh), ws.data_ptr(), dx.data_ptr(), _p(dy), _p(dgate), _p(dpw), _p(dpb),
@@ -742,10 +768,16 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     return out.view(tq, h, d)
 
 
+def _strided_heads(t: torch.Tensor) -> bool:
+    """Whether each row's (H, D) values are contiguous and the rows apart."""
+    n, h, d = t.shape
+    return not (t.stride(2) != 1 or (h > 1 and t.stride(1) != d) or (n > 1 and t.stride(0) < h * d))
+
+
 def _head_rows(t: torch.Tensor, name: str) -> int:
     """Row stride in elements of a (total, H, D) tensor whose rows are contiguous."""
     _, h, d = t.shape
-    if t.stride(2) != 1 or (h > 1 and t.stride(1) != d) or (t.shape[0] > 1 and t.stride(0) < h * d):
+    if not _strided_heads(t):
         raise TscError(_lib.TSC_ERR_INVALID, f"{name}: each row's (H, D) values must be contiguous")
     return t.stride(0) if t.shape[0] > 1 else h * d
 
@@ -898,7 +930,7 @@ def sparse_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
         raise TscError(_lib.TSC_ERR_INVALID, "window_attention: out has the wrong shape or dtype")
     code = _code(q)
     _no_tangents("window_attention", q, k, v, out)
-    lds = (_head_rows(q, "q"), _head_rows(k, "k"), _head_rows(v, "v"))
+    lds = _head_rows(q, "q"), _head_rows(k, "k"), _head_rows(v, "v")
     dev = q.get_device()
     if out is not None and _dev(out) != dev or dev < 0 or k.get_device() != dev or v.get_device() != dev:
         raise TscError(_lib.TSC_ERR_INVALID, "tensors are not on one GPU; this path has no CPU fallback")
@@ -916,15 +948,15 @@ def sparse_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
         raise TscError(_lib.TSC_ERR_INVALID, "cu_seqlens_q and cu_seqlens_kv differ in length")
     b = cq.numel() - 1
     args = (cq, ck, b, float(scale) if scale is not None else 0.0, window, sinks, int(bool(causal)),
-            _longest(max_seqlen_q, cq_host, tq, b), _longest(max_seqlen_kv, ck_host, tkv, b), lds, code, dev)
+            _longest(max_seqlen_q, cq_host, tq, b), _longest(max_seqlen_kv, ck_host, tkv, b), code, dev)
     if _wants_grad(q, k, v, out):
         if out is not None:
             raise TscError(_lib.TSC_ERR_INVALID, "window_attention: out cannot be given where gradients "
                                                  "are wanted")
         from .autograd import WindowAttention
 
-        return WindowAttention.apply(q, k, v, args)
-    return _window_attention(q, k, v, args, out, False)[0]
+        return WindowAttention.apply(q, k, v, lds, args)
+    return _window_attention(q, k, v, lds, args, out, False)[0]
 
 
 def _longest(given, host, total: int, b: int) -> int:
@@ -937,9 +969,9 @@ def _longest(given, host, total: int, b: int) -> int:
     return int((host[1:] - host[:-1]).max()) if host is not None else min(total, 2 * -(-total // b))
 
 
-def _window_attention(q, k, v, args, out, keep):
-    """(out, lo, lse); lo and lse (None unless keep) are what the backward pass needs."""
-    cq, ck, b, scale, window, sinks, causal, max_q, max_kv, lds, code, dev = args
+def _window_attention(q, k, v, lds, args, out, keep):
+    """(out, lo, lse); lo and lse (None unless keep) are what the backward pass needs.  lds: row strides of q, k, v."""
+    cq, ck, b, scale, window, sinks, causal, max_q, max_kv, code, dev = args
     tq, h, d = q.shape
     tkv, hk = k.shape[:2]
     rest = out is None
@@ -960,10 +992,22 @@ def _window_attention(q, k, v, args, out, keep):
     return out, lo, lse
 
 
-def _window_attention_backward(do, q, k, v, out, lo, lse, args):
-    cq, ck, b, scale, window, sinks, causal, max_q, max_kv, lds, code, dev = args
-    tq, h, d = q.shape
-    tkv, hk = k.shape[:2]
+def _aligned_heads(t: torch.Tensor) -> bool:
+    """... and whole 16 bytes apart."""
+    return _strided_heads(t) and t.stride(0) * t.element_size() % 16 == 0
+
+
+def _window_attention_backward(do, q, k, v, out, lo, lse, kv_shape, args):
+    """(dq, dk, dv); kv_shape: k's and v's."""
+    cq, ck, b, scale, window, sinks, causal, max_q, max_kv, code, dev = args
+    shape, dtype = do.shape, do.dtype
+    tq, h, d = shape
+    tkv, hk = kv_shape[:2]
+    q = _restored(q, shape, dtype, dev, 16, _aligned_heads)
+    k, v = (_restored(t, kv_shape, dtype, dev, 16, _aligned_heads) for t in (k, v))
+    out, lo = (_restored(t, shape, dtype, dev, 16) for t in (out, lo))
+    lse = _restored(lse, (tq, h), torch.float32, dev)
+    cq, ck = (_restored(t, (b + 1,), torch.int32, dev) for t in (cq, ck))
     new = q.new_empty if b else q.new_zeros
     dq, dk, dv = new((tq, h, d)), new((tkv, hk, d)), new((tkv, hk, d))
     if b and (tq or tkv):
@@ -972,9 +1016,10 @@ def _window_attention_backward(do, q, k, v, out, lo, lse, args):
                                                           max_kv, 1)
         ws = new((max(nbytes, 16),), dtype=torch.uint8)
         check(lib.tsc_window_attention_backward(
-            handle, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), *lds, cq.data_ptr(), ck.data_ptr(), b, tq, tkv,
-            h, hk, d, scale, window, sinks, causal, max_q, max_kv, 1, out.data_ptr(), _p(lo), lse.data_ptr(),
-            do.data_ptr(), ws.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()))
+            handle, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), _head_rows(q, "q"), _head_rows(k, "k"),
+            _head_rows(v, "v"), cq.data_ptr(), ck.data_ptr(), b, tq, tkv, h, hk, d, scale, window, sinks, causal,
+            max_q, max_kv, 1, out.data_ptr(), _p(lo), lse.data_ptr(), do.data_ptr(), ws.data_ptr(), dq.data_ptr(),
+            dk.data_ptr(), dv.data_ptr()))
     return dq, dk, dv
 
 
