@@ -2,6 +2,7 @@
 save_on_cpu) give back the values in another layout: the C calls are recorded on the CPU, and what each would
 read, by the pointer and the row stride that it is given, is compared with the values that were saved."""
 import ctypes
+import importlib
 
 import numpy as np
 import pytest
@@ -129,3 +130,49 @@ def test_other_types_and_shapes_are_refused(pkg, record, layout):
         with pytest.raises(pkg.TscError, match="came back as"):
             o.sum().backward()
     assert not backward
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_group_norm(pkg, record, monkeypatch, layout):
+    n, c, groups = 12, 32, 4
+    x = torch.randn((n, c)).requires_grad_()
+    seen = []
+
+    def at_call(name, a):
+        if name == "tsc_groupnorm":
+            stats = np.ctypeslib.as_array((ctypes.c_float * (2 * groups * 2)).from_address(a[13]))
+            stats[:] = np.arange(stats.size)
+        if name != "tsc_groupnorm_backward":
+            return
+        seen.append(name)
+        assert torch.equal(_read(a[3], n, c, c), x.detach())
+        assert torch.equal(_read(a[13], 2, 2 * groups, 2 * groups).flatten(), torch.arange(4.0 * groups))
+
+    record(at_call)
+    monkeypatch.setattr(pkg.ops, "_dev", lambda *ts: 0)
+    _step(x, lambda: [pkg.group_norm(x, groups, cu_rows=[0, 5, 12])], layout, seen)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_diff_attention(pkg, record, layout):
+    n, h, d = 12, 2, 64
+    qkv = torch.randn((n, 3, h, d)).requires_grad_()
+    lam, cu = torch.rand(h), torch.tensor([0, 5, 12], dtype=torch.int32)
+    seen, sizes = [], {20: 2 * n * h * d, 21: 2 * h * n}  # maps, lse
+
+    def at_call(name, a):
+        if name == "tsc_diff_attention":
+            for at, size in sizes.items():
+                values = np.ctypeslib.as_array((ctypes.c_float * size).from_address(a[at + 2]))
+                values[:] = np.arange(size)
+        if name != "tsc_diff_attention_backward":
+            return
+        seen.append(name)
+        for i in range(3):
+            assert torch.equal(_read(a[2 + i], n, h * d, a[5 + i]), qkv.detach()[:, i].flatten(1)), "qkv"[i]
+        for at, size in sizes.items():
+            assert torch.equal(_read(a[at], 1, size, size)[0], torch.arange(float(size)))
+
+    record(at_call)
+    f = importlib.import_module(pkg.__name__ + ".autograd").DiffAttention
+    _step(qkv, lambda: [f.apply(qkv[:, 0], qkv[:, 1], qkv[:, 2], lam, cu, cu, 2, 0.0, 7, 7)], layout, seen)

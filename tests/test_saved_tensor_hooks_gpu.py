@@ -82,3 +82,20 @@ def test_norms(pkg, dev, dtype, hook, c, op):
         def call():
             return pkg.gated_residual_norm(x, y, cu, mod[:, 2], 0.5, "layer", w, b, scale=mod[:, 4], shift=mod[:, 3])
     _same(leaves, call, d[:1 if op != "grn" else 2], HOOKS[hook])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hook", HOOKS)
+def test_group_norm_and_diff_attention(pkg, dev, dtype, hook):
+    g = torch.Generator().manual_seed(71)
+    n, h, d = 51, 2, 64
+    cu = torch.tensor([0, 20, 51], dtype=torch.int32, device=dev)
+
+    def leaf(*shape):
+        return torch.randn(shape, generator=g).to(dtype).to(dev).requires_grad_()
+
+    x, w, b, dy = leaf(n, 96), leaf(96), leaf(96), leaf(n, 96).detach()
+    _same([x, w, b], lambda: [pkg.group_norm(x, 8, w, b, cu, silu=True)], [dy], HOOKS[hook])
+    qkv, do = leaf(n, 3, h, d), leaf(n, h, d).detach()
+    lam = torch.rand(h, generator=g).to(dev).requires_grad_()
+    _same([qkv, lam], lambda: [pkg.sparse_diff_attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], lam, cu)], [do], HOOKS[hook])

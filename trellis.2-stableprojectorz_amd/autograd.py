@@ -68,7 +68,7 @@ class DiffAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, lam, cq, ck, b, scale, max_q, max_kv):
         out, maps, lse = ops._diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, None, True)
         ctx.save_for_backward(q, k, v, lam, maps, lse, cq, ck)
-        ctx.args = (b, scale, max_q, max_kv)
+        ctx.total_kv, ctx.args = k.shape[0], (b, scale, max_q, max_kv)
         return out
 
     @staticmethod
@@ -78,7 +78,7 @@ class DiffAttention(torch.autograd.Function):
         do = do.contiguous()
         if do.data_ptr() % 16:  # a view into a larger gradient
             do = do.clone()
-        grads = ops._diff_attention_backward(do, q, k, v, lam, maps, lse, cq, ck,
+        grads = ops._diff_attention_backward(do, q, k, v, lam, maps, lse, ctx.total_kv, cq, ck,
                                              *ctx.args)
         return (*grads, None, None, None, None, None, None)
 

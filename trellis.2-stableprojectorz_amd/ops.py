@@ -362,7 +362,10 @@ def _group_norm(x, weight, bias, cu, b, groups, eps, silu, out, stats):
 
 
 def _group_norm_backward(dy, x, weight, bias, cu, b, groups, silu, stats, want_params):
-    c = x.shape[-1]
+    c, dtype, dev = dy.shape[-1], dy.dtype, dy.get_device()
+    x = _restored(x, dy.shape, dtype, dev)
+    weight, bias = (_restored(t, (c,), dtype, dev) for t in (weight, bias))
+    cu, stats = _restored(cu, (b + 1,), torch.int32, dev), _restored(stats, (b, groups, 2), torch.float32, dev, 8)
     n = x.numel() // c
     dx = torch.empty_like(x)
     dw = torch.empty_like(weight) if want_params and weight is not None else None
@@ -774,6 +777,11 @@ def _strided_heads(t: torch.Tensor) -> bool:
     return not (t.stride(2) != 1 or (h > 1 and t.stride(1) != d) or (n > 1 and t.stride(0) < h * d))
 
 
+def _aligned_heads(t: torch.Tensor) -> bool:
+    """... and whole 16 bytes apart."""
+    return _strided_heads(t) and t.stride(0) * t.element_size() % 16 == 0
+
+
 def _head_rows(t: torch.Tensor, name: str) -> int:
     """Row stride in elements of a (total, H, D) tensor whose rows are contiguous."""
     _, h, d = t.shape
@@ -869,9 +877,14 @@ def _diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, out, keep):
     return out, maps, lse
 
 
-def _diff_attention_backward(do, q, k, v, lam, maps, lse, cq, ck, b, scale, max_q, max_kv):
-    tq, h, d = q.shape
-    tkv = k.shape[0]
+def _diff_attention_backward(do, q, k, v, lam, maps, lse, tkv, cq, ck, b, scale, max_q, max_kv):
+    shape, dtype, dev = do.shape, do.dtype, do.get_device()
+    tq, h, d = shape
+    q = _restored(q, shape, dtype, dev, 16, _aligned_heads)
+    k, v = (_restored(t, (tkv, h, d), dtype, dev, 16, _aligned_heads) for t in (k, v))
+    lam, lse = _restored(lam, (h,), torch.float32, dev), _restored(lse, (2, h, tq), torch.float32, dev)
+    maps = _restored(maps, (tq, h, 2, d), torch.float32, dev, 16)
+    cq, ck = (_restored(t, (b + 1,), torch.int32, dev) for t in (cq, ck))
     alloc = torch.empty if tq and b else torch.zeros
     dq = alloc((tq, h, d), dtype=q.dtype, device=q.device)
     dk, dv = (alloc((tkv, h, d), dtype=q.dtype, device=q.device) for _ in range(2))
@@ -990,11 +1003,6 @@ def _window_attention(q, k, v, lds, args, out, keep):
         if not rest:
             _wrote(out)
     return out, lo, lse
-
-
-def _aligned_heads(t: torch.Tensor) -> bool:
-    """... and whole 16 bytes apart."""
-    return _strided_heads(t) and t.stride(0) * t.element_size() % 16 == 0
 
 
 def _window_attention_backward(do, q, k, v, out, lo, lse, kv_shape, args):
