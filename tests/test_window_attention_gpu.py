@@ -576,3 +576,38 @@ def test_more_than_two_to_the_31_values(pkg, dev, dtype, d):
     print(f"  {n} tokens {dtype} D={d}", flush=True)
     for name in got:  # the cut row sees less; rows 80 on neither see it nor are seen through it
         check(got[name][-tail + 80:, hs], tuple(x[80:] for x in want[name]), name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_infinities_and_nan_in_wide_grids(pkg, dev, dtype, d, causal):
+    """The same with 320 tiles of 128 rows and of 128 keys, which the wide kernels of all three passes take, and a
+    window with tiles that all rows of a block see: at a block's ends, within its run, at a window's edge."""
+    window, sinks, n, h = 400, 2, 2500, 16
+    base = _make([n], [n], h, h, d, dtype, 73)
+    kw = dict(sinks=sinks, causal=causal)
+    print(f"  infinities and NaN {dtype} D={d} n={n} causal={causal}", flush=True)
+    want = {x: t.cpu() for x, t in _run(pkg, dev, *base, window, [0, n], None, **kw).items()}
+    see = _sees(n, n, window, sinks, causal)
+    for what, row, value in ((2, 1100, math.inf), (2, 1279, math.nan), (2, 1, -math.inf), (1, 1021, math.nan), (1, 1500, math.inf),
+                             (0, 1290, math.inf), (0, 1400, math.nan), (0, 2499, -math.inf), (3, 1150, math.inf), (3, 640, math.nan)):
+        t = [x.clone() for x in base]
+        t[what][row, :, 3] = value
+        got = {x: y.cpu() for x, y in _run(pkg, dev, *t, window, [0, n], None, **kw).items()}
+        if what in (1, 2):
+            queries = see[:, row]
+            keys = see[queries].any(0)
+        else:
+            queries = torch.zeros(n, dtype=torch.bool)
+            queries[row] = True
+            keys = see[row]
+        for name in got:
+            hit = queries if name in ("out", "dq") else keys
+            other = (got[name][~hit] != want[name][~hit]).flatten(1).any(1).sum().item()
+            print(f"    {'qkvd'[what]}[{row}] = {value}: {name} of {int((~hit).sum())} other rows, {other} CHANGED", flush=True)
+            assert torch.equal(got[name][~hit], want[name][~hit])
+        if what == 2:
+            assert not got["out"][queries][..., 3].isfinite().any()
+        if what == 3:
+            assert not got["dv"][row].isfinite()[..., 3].any() and torch.equal(got["out"], want["out"])

@@ -521,12 +521,13 @@ __global__ void __launch_bounds__(64 * NW, 2) wa_forward16_kernel(const WaArgs a
         for (int j = 4 * part; j < 4 * part + 4; ++j) mx = fmaxf(mx, s[i][j]);
         return mx;
       };
-      // Raises the running maxima of row tile i where a score exceeds one by more than 2^kLazy.
+      // Raises the running maxima of row tile i where a score exceeds one by more than 2^kLazy: those alone, so that
+      // a row's bits do not depend on the scores of the rows beside it.
       auto raise = [&](int i, float mx) {
         mx *= sl2;
-        const bool up = __builtin_amdgcn_ballot_w64(mx > mc[i] + kLazy) != 0;
+        const bool over = mx > mc[i] + kLazy, up = __builtin_amdgcn_ballot_w64(over) != 0;
         if (up) {
-          const float mn = fmaxf(mc[i], mx);
+          const float mn = over ? mx : mc[i];
           alpha[i] = fast_exp2(mc[i] - mn);
           mc[i] = mn;
           if (KEEP) lu[i] *= alpha[i];  // before the next exponentials are added to it
