@@ -288,9 +288,8 @@ def _no_tangents(what: str, *ts) -> None:
 
 
 def _restored(t, shape, dtype, dev: int, align: int = 1, strided=None):
-    """A tensor that autograd saved, as the C calls take it: contiguous, or with rows that `strided` finds fit,
-    and aligned.  Hooks on saved tensors (offloading, say) may give back the values in another layout than the
-    forward call's."""
+    """A tensor that a hook on saved tensors (offloading, say) gave back, as the C calls take it: contiguous, or
+    with rows that `strided` finds fit, and aligned, whatever its layout is."""
     if t is None:
         return None
     if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
@@ -361,12 +360,14 @@ def _group_norm(x, weight, bias, cu, b, groups, eps, silu, out, stats):
     return out
 
 
-def _group_norm_backward(dy, x, weight, bias, cu, b, groups, silu, stats, want_params):
-    c, dtype, dev = dy.shape[-1], dy.dtype, dy.get_device()
-    x = _restored(x, dy.shape, dtype, dev)
-    weight, bias = (_restored(t, (c,), dtype, dev) for t in (weight, bias))
-    cu, stats = _restored(cu, (b + 1,), torch.int32, dev), _restored(stats, (b, groups, 2), torch.float32, dev, 8)
-    n = x.numel() // c
+def _group_norm_backward(dy, x, weight, bias, cu, b, groups, silu, stats, want_params, moved):
+    c = dy.shape[-1]
+    n = dy.numel() // c
+    if moved:
+        dtype, dev = dy.dtype, dy.get_device()
+        x = _restored(x, dy.shape, dtype, dev)
+        weight, bias = (_restored(t, (c,), dtype, dev) for t in (weight, bias))
+        cu, stats = _restored(cu, (b + 1,), torch.int32, dev), _restored(stats, (b, groups, 2), torch.float32, dev, 8)
     dx = torch.empty_like(x)
     dw = torch.empty_like(weight) if want_params and weight is not None else None
     db = torch.empty_like(bias) if want_params and bias is not None else None
@@ -538,17 +539,21 @@ def _gated_norm(tensors, args, want_r, want_h, out, keep):
     return r, h, stats
 
 
-def _gated_norm_backward(tensors, args, stats, stats_shape, dr, dh, wanted):
-    """The gradients of `tensors`, None where there is none or `wanted` says so."""
-    like = dr if dh is None else dh
-    shape, dtype, b, dev = like.shape, like.dtype, args[1], args[7]
-    n, c = shape
-    x, y = (_restored(t, shape, dtype, dev) for t in tensors[:2])
-    pw, pb, w, bias = (_restored(tensors[i], (c,), dtype, dev) for i in (2, 3, 5, 6))
-    gate, scale, shift = (_restored(tensors[i], (b, c), dtype, dev, 1, _strided_rows) for i in (4, 7, 8))
-    tensors = (x, y, pw, pb, gate, w, bias, scale, shift)
-    stats = _restored(stats, stats_shape, torch.float32, dev, 8)
-    args = (_restored(args[0], (b + 1,), torch.int32, dev), *args[1:])
+def _gated_norm_backward(tensors, args, stats, dr, dh, wanted, moved):
+    """The gradients of `tensors`, None where there is none or `wanted` says so.  moved: tensors, args[0] and stats
+    may have other layouts than in the forward call, for stats of the shape `moved`."""
+    b = args[1]
+    n, c = (dr if dh is None else dh).shape
+    if moved is not None:
+        like, dev = dr if dh is None else dh, args[7]
+        dtype = like.dtype
+        x, y = (_restored(t, like.shape, dtype, dev) for t in tensors[:2])
+        pw, pb, w, bias = (_restored(tensors[i], (c,), dtype, dev) for i in (2, 3, 5, 6))
+        gate, scale, shift = (_restored(tensors[i], (b, c), dtype, dev, 1, _strided_rows) for i in (4, 7, 8))
+        tensors = (x, y, pw, pb, gate, w, bias, scale, shift)
+        stats = _restored(stats, moved, torch.float32, dev, 8)
+        args = (_restored(args[0], (b + 1,), torch.int32, dev), *args[1:])
+    x, y = tensors[:2]
     if n == 0:
         return [None if t is None else torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
     # Without dh the norm before the next block has no gradient, and neither has its modulation.
@@ -877,14 +882,15 @@ def _diff_attention(q, k, v, lam, cq, ck, b, scale, max_q, max_kv, out, keep):
     return out, maps, lse
 
 
-def _diff_attention_backward(do, q, k, v, lam, maps, lse, tkv, cq, ck, b, scale, max_q, max_kv):
-    shape, dtype, dev = do.shape, do.dtype, do.get_device()
-    tq, h, d = shape
-    q = _restored(q, shape, dtype, dev, 16, _aligned_heads)
-    k, v = (_restored(t, (tkv, h, d), dtype, dev, 16, _aligned_heads) for t in (k, v))
-    lam, lse = _restored(lam, (h,), torch.float32, dev), _restored(lse, (2, h, tq), torch.float32, dev)
-    maps = _restored(maps, (tq, h, 2, d), torch.float32, dev, 16)
-    cq, ck = (_restored(t, (b + 1,), torch.int32, dev) for t in (cq, ck))
+def _diff_attention_backward(do, q, k, v, lam, maps, lse, cq, ck, moved, tkv, b, scale, max_q, max_kv):
+    tq, h, d = do.shape
+    if moved:
+        dtype, dev = do.dtype, do.get_device()
+        q = _restored(q, do.shape, dtype, dev, 16, _aligned_heads)
+        k, v = (_restored(t, (tkv, h, d), dtype, dev, 16, _aligned_heads) for t in (k, v))
+        lam, lse = _restored(lam, (h,), torch.float32, dev), _restored(lse, (2, h, tq), torch.float32, dev)
+        maps = _restored(maps, (tq, h, 2, d), torch.float32, dev, 16)
+        cq, ck = (_restored(t, (b + 1,), torch.int32, dev) for t in (cq, ck))
     alloc = torch.empty if tq and b else torch.zeros
     dq = alloc((tq, h, d), dtype=q.dtype, device=q.device)
     dk, dv = (alloc((tkv, h, d), dtype=q.dtype, device=q.device) for _ in range(2))
@@ -1005,17 +1011,20 @@ def _window_attention(q, k, v, lds, args, out, keep):
     return out, lo, lse
 
 
-def _window_attention_backward(do, q, k, v, out, lo, lse, kv_shape, args):
-    """(dq, dk, dv); kv_shape: k's and v's."""
+def _window_attention_backward(do, q, k, v, out, lo, lse, lds, moved, args):
+    """(dq, dk, dv).  moved: the saved tensors may have other layouts than in the forward call, k and v of the
+    shape `moved`."""
     cq, ck, b, scale, window, sinks, causal, max_q, max_kv, code, dev = args
-    shape, dtype = do.shape, do.dtype
-    tq, h, d = shape
-    tkv, hk = kv_shape[:2]
-    q = _restored(q, shape, dtype, dev, 16, _aligned_heads)
-    k, v = (_restored(t, kv_shape, dtype, dev, 16, _aligned_heads) for t in (k, v))
-    out, lo = (_restored(t, shape, dtype, dev, 16) for t in (out, lo))
-    lse = _restored(lse, (tq, h), torch.float32, dev)
-    cq, ck = (_restored(t, (b + 1,), torch.int32, dev) for t in (cq, ck))
+    if moved is not None:
+        shape, dtype = do.shape, do.dtype
+        q = _restored(q, shape, dtype, dev, 16, _aligned_heads)
+        k, v = (_restored(t, moved, dtype, dev, 16, _aligned_heads) for t in (k, v))
+        out, lo = (_restored(t, shape, dtype, dev, 16) for t in (out, lo))
+        lse = _restored(lse, shape[:2], torch.float32, dev)
+        cq, ck = (_restored(t, (b + 1,), torch.int32, dev) for t in (cq, ck))
+        lds = _head_rows(q, "q"), _head_rows(k, "k"), _head_rows(v, "v")
+    tq, h, d = q.shape
+    tkv, hk = k.shape[:2]
     new = q.new_empty if b else q.new_zeros
     dq, dk, dv = new((tq, h, d)), new((tkv, hk, d)), new((tkv, hk, d))
     if b and (tq or tkv):
@@ -1024,10 +1033,9 @@ def _window_attention_backward(do, q, k, v, out, lo, lse, kv_shape, args):
                                                           max_kv, 1)
         ws = new((max(nbytes, 16),), dtype=torch.uint8)
         check(lib.tsc_window_attention_backward(
-            handle, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), _head_rows(q, "q"), _head_rows(k, "k"),
-            _head_rows(v, "v"), cq.data_ptr(), ck.data_ptr(), b, tq, tkv, h, hk, d, scale, window, sinks, causal,
-            max_q, max_kv, 1, out.data_ptr(), _p(lo), lse.data_ptr(), do.data_ptr(), ws.data_ptr(), dq.data_ptr(),
-            dk.data_ptr(), dv.data_ptr()))
+            handle, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), *lds, cq.data_ptr(), ck.data_ptr(), b, tq, tkv,
+            h, hk, d, scale, window, sinks, causal, max_q, max_kv, 1, out.data_ptr(), _p(lo), lse.data_ptr(),
+            do.data_ptr(), ws.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()))
     return dq, dk, dv
 
 
