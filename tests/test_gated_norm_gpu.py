@@ -422,3 +422,39 @@ def test_more_than_two_to_the_31_values(pkg, dev, dtype, c):
     last = run(slice(n - 900, n), [0, 900], m[1:])
     for a, b in zip(all_rows, last):
         assert torch.equal(a[-900:], b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("samples", [2, 20])
+@pytest.mark.parametrize("post,norm", [(1, 2), (2, 1)])
+def test_c_gradients_of_parameters_that_are_not_given(pkg, dev, dtype, samples, post, norm):
+    """The C call's NULL for a weight, bias, gate, scale or shift means ones or zeros, and its gradient may be wanted all
+    the same: the bits that explicit ones and zeros have."""
+    n, c = 40 * samples, 72
+    g = torch.Generator().manual_seed(79)
+    x, y, dr, dh = (torch.randn((n, c), generator=g).to(dtype).to(dev) for _ in range(4))
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    lib, handle = pkg.ops._lib.stream_handle(0)
+
+    def run(pw, pb, gate, w, b, scale, shift):
+        p = [None if t is None else t.data_ptr() for t in (pw, pb, gate, w, b, scale, shift)]
+        args = (handle, code, x.data_ptr(), y.data_ptr(), None, samples, n, c, post, p[0], p[1], p[2], c, 0.5, norm, p[3],
+                p[4], p[5], c, p[6], c, 1e-6, 1)
+        stats = torch.empty((2, n, 2), device=dev)
+        r, h, dx, dy = (torch.full_like(x, float("nan")) for _ in range(4))
+        grads = {k: torch.full((c,) if k in ("dpw", "dpb", "dw", "db") else (samples, c), float("nan"), dtype=dtype, device=dev)
+                 for k in ("dgate", "dpw", "dpb", "dscale", "dshift", "dw", "db")}
+        assert lib.tsc_gated_norm(*args, stats.data_ptr(), r.data_ptr(), h.data_ptr()) == 0
+        ws = torch.empty((lib.tsc_gated_norm_workspace_bytes(code, samples, n, c),), dtype=torch.uint8, device=dev)
+        assert lib.tsc_gated_norm_backward(*args, stats.data_ptr(), dr.data_ptr(), dh.data_ptr(), ws.data_ptr(),
+                                           dx.data_ptr(), dy.data_ptr(), *(t.data_ptr() for t in grads.values())) == 0
+        return {"r": r, "h": h, "dx": dx, "dy": dy, **grads}
+
+    one, zero = torch.ones(c, dtype=dtype, device=dev), torch.zeros(c, dtype=dtype, device=dev)
+    ones, zeros = torch.ones((samples, c), dtype=dtype, device=dev), torch.zeros((samples, c), dtype=dtype, device=dev)
+    want = run(one, zero, ones, one, zero, zeros, zeros)
+    for name, got in (("none", run(None, None, None, None, None, None, None)),
+                      ("weights", run(one, None, None, one, None, None, None)),
+                      ("modulation", run(None, None, ones, None, None, zeros, zeros))):
+        for k in want:
+            assert torch.equal(got[k], want[k]), (name, k)

@@ -789,8 +789,9 @@ int gated_norm_backward_launch(tsc_ctx* ctx, const GatedNormArgs& x, const float
   a.dy = g.dy;
   const bool want_h = dh && (g.dscale || g.dshift || g.dweight || g.dbias);
   const bool want_y = x.y && (g.dgate || g.dpost_weight || g.dpost_bias);
-  // Either part's sums where any is wanted: the kernel makes them all the same.
-  a.sums = want_h || want_y ? (dh ? 2 : 0) + (x.y ? (x.post_bias ? 2 : 1) : 0) : 0;
+  // Either part's sums where any is wanted: the kernel makes them all the same.  Q' is for the bias, its own gradient
+  // and its part of the gate's.
+  a.sums = want_h || want_y ? (dh ? 2 : 0) + (x.y ? (x.post_bias || g.dpost_bias ? 2 : 1) : 0) : 0;
   a.part = (float*)ws;
   const Shape s = shape_for(x, kLaneB, kBackThreads, {dr, dh, g.dx, g.dy});
   a.G = s.G;
