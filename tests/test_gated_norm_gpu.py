@@ -458,3 +458,15 @@ def test_c_gradients_of_parameters_that_are_not_given(pkg, dev, dtype, samples, 
                       ("modulation", run(None, None, ones, None, None, zeros, zeros))):
         for k in want:
             assert torch.equal(got[k], want[k]), (name, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("op,c,lens", [("grn", 1536, [1500]), ("grn", 1536, [1, 0, 2, 0, 3, 2594, 0]), ("grn", 1000, [3, 0, 1, 5] * 330),
+                                       ("grn", 1000, [1990, 7, 1993]), ("grn", 1025, [2, 1] * 420 + [940]), ("grn", 8192, [301, 0, 401]),
+                                       ("mn", 1536, [3, 0, 1, 5, 2] * 235), ("gr", 1536, [1400, 2, 1198])])
+def test_rows_of_blocks(pkg, dev, dtype, op, c, lens):
+    """Rows wider than a wave's, several to each block: the rows ahead come round, three and other numbers of them, and
+    the sums of a block's rows have many samples, a part of one, or both."""
+    most = 256 * max(1, (8 if op == "grn" else 16) * 64 // (-(-c // 512) * 64))  # blocks at 8 values a lane
+    assert sum(lens) > most
+    _both(pkg, dev, op, lens, c, dtype, "layer", "rms", rs=0.75)
