@@ -268,7 +268,7 @@ enum tsc_norm { TSC_NORM_NONE = 0, TSC_NORM_LAYER = 1, TSC_NORM_RMS = 2 };
  * t / sqrt(mean(t^2) + eps) (TSC_NORM_RMS), for y TSC_NORM_NONE too (then without weight and bias).
  *   x, y, r, h  (N,C) `dtype`, aligned to the element size (16-byte aligned buffers and rows of whole
  *              16 bytes are fastest), C at most 8192.  y NULL: r = x, and r is NULL too; h NULL: r only.
- *              r and h may each be x or y itself, but not overlap otherwise
+ *              r and h may each be x or y itself, but overlap neither otherwise, nor each other, nor a parameter
  *   cu_rows, B, zero_rest  as in tsc_groupnorm (zero_rest is about rows of r and h)
  *   gate, scale, shift  (B,C) `dtype`, row strides ld_* in elements (at least C), NULL = 1 / 0 / 0
  *   post_weight, post_bias, weight, bias  (C) `dtype`, NULL = 1 / 0

@@ -470,3 +470,26 @@ def test_rows_of_blocks(pkg, dev, dtype, op, c, lens):
     most = 256 * max(1, (8 if op == "grn" else 16) * 64 // (-(-c // 512) * 64))  # blocks at 8 values a lane
     assert sum(lens) > most
     _both(pkg, dev, op, lens, c, dtype, "layer", "rms", rs=0.75)
+
+
+def test_outputs_over_parameters_are_refused(pkg, dev):
+    """Blocks read them while others write their rows."""
+    n, c = 40, 32
+    buf = torch.zeros((n + 9, c), device=dev)
+    x, out, outside = torch.ones((n, c), device=dev), buf[2:2 + n], buf[2 + n:]
+    cu = [0, 20, n]
+    for kw in ({"scale": out[38:]}, {"shift": buf[:3][1:]}, {"weight": out[0]}, {"bias": out[-1]}):
+        with pytest.raises(pkg.TscError, match="overlaps a parameter"):
+            pkg.modulated_norm(x, cu, out=out, **kw)
+    for kw in ({"gate": out[5::20][:2]}, {"post_weight": out[0]}, {"post_bias": out[7]}):
+        with pytest.raises(pkg.TscError, match="overlaps a parameter"):
+            pkg.gated_residual(x, x, cu, post_norm="layer", out=out, **kw)
+    offsets = out.view(torch.int32).flatten()[:3]
+    with pytest.raises(pkg.TscError, match="overlaps a parameter"):
+        pkg.modulated_norm(x, offsets, out=out)
+    assert pkg.modulated_norm(x, cu, outside[:2], outside[2:4], weight=outside[4], bias=outside[5], out=out) is out
+    lib, handle = pkg.ops._lib.stream_handle(0)
+    for stats in (x, out, outside):
+        st = lib.tsc_gated_norm(handle, 0, x.data_ptr(), None, None, 1, n, c, 0, None, None, None, 0, 1.0, 1, outside.data_ptr(),
+                                None, None, 0, None, 0, 1e-6, 0, stats.data_ptr(), None, out.data_ptr())
+        assert st == 1 and b"overlaps" in lib.tsc_last_error()

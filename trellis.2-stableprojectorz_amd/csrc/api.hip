@@ -675,6 +675,23 @@ int tsc_gated_norm(tsc_ctx* ctx, int32_t dtype, const void* x, const void* y, co
         if (in && o != in && overlaps(o, bytes, in, bytes))
           return fail(TSC_ERR_INVALID, "gated_norm: an output overlaps x or y without being it");
   if (r && h && overlaps(r, bytes, h, bytes)) return fail(TSC_ERR_INVALID, "gated_norm: r overlaps h");
+  // Blocks read the parameters while others write their rows.
+  const size_t row = (size_t)C * es;
+  const size_t st_bytes = (size_t)((h ? 1 : 0) + (y && post_norm != TSC_NORM_NONE ? 1 : 0)) * N * 8;
+  auto span = [&](int64_t ld) { return B > 0 ? ((size_t)(B - 1) * ld + C) * es : 0; };
+  const void* params[8] = {gate, scale, shift, post_weight, post_bias, weight, bias, cu_rows};
+  const size_t p_bytes[8] = {span(ld_gate), span(ld_scale), span(ld_shift), row, row, row, row, ((size_t)B + 1) * 4};
+  const void* written[3] = {r, h, stats};
+  const size_t w_bytes[3] = {bytes, bytes, st_bytes};
+  for (int i = 0; i < 3; ++i) {
+    if (!written[i]) continue;
+    for (int j = 0; j < 8; ++j)
+      if (params[j] && overlaps(written[i], w_bytes[i], params[j], p_bytes[j]))
+        return fail(TSC_ERR_INVALID, "gated_norm: an output overlaps a parameter");
+    for (const void* o : {x, y, (const void*)r, (const void*)h})
+      if (i == 2 && o && overlaps(stats, st_bytes, o, bytes))
+        return fail(TSC_ERR_INVALID, "gated_norm: stats overlaps a matrix");
+  }
   DeviceGuard g(ctx->device);
   if (B == 0) {  // every row is outside
     if (r) st = zero_launch(ctx, r, (int64_t)bytes);
