@@ -426,7 +426,8 @@ int tsc_diff_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, cons
  *     scale <= 0 meaning 1/sqrt(head_dim)
  *   window, sinks  at least 0 (INT32_MAX: no bound)
  *   out_lo, lse  both NULL, or for the backward pass: lse fp32 (total_q, num_heads) takes the rows'
- *     log2-sum-exps, out_lo (as out; NULL for TSC_F32) what out's rounding left
+ *     log2-sum-exps, out_lo (as out; NULL for TSC_F32) what out's rounding left.  out, out_lo and lse
+ *     must not overlap each other or an input
  *   workspace  device scratch of tsc_window_attention_workspace_bytes(..., backward = 0) bytes, 16-byte
  *     aligned, NULL if that is 0.  The context keeps nothing.
  * fp32 softmax and accumulation; P is rounded to `dtype` for its product with v.  Infinities and NaN stay

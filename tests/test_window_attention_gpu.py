@@ -611,3 +611,17 @@ def test_infinities_and_nan_in_wide_grids(pkg, dev, dtype, d, causal):
             assert not got["out"][queries][..., 3].isfinite().any()
         if what == 3:
             assert not got["dv"][row].isfinite()[..., 3].any() and torch.equal(got["out"], want["out"])
+
+
+def test_outputs_over_offsets_and_statistics_are_refused(pkg, dev):
+    n, h, d = 40, 2, 64
+    x, out = torch.ones((n, h, d), device=dev), torch.zeros((n, h, d), device=dev)
+    with pytest.raises(pkg.TscError, match="out overlaps an input"):
+        pkg.sparse_window_attention(x, x, x, 4, out.view(torch.int32).flatten()[5:8], out=out)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    lib, handle = pkg.ops._lib.stream_handle(0)
+    for lse in (x, out, cu):
+        p = x.data_ptr()
+        st = lib.tsc_window_attention(handle, 0, p, p, p, h * d, h * d, h * d, cu.data_ptr(), cu.data_ptr(), 1, n, n, h, h, d,
+                                      0.0, 4, 0, 0, n, n, 0, None, out.data_ptr(), None, lse.data_ptr())
+        assert st == 1 and b"overlap" in lib.tsc_last_error()

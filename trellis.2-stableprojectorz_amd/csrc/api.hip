@@ -1137,13 +1137,20 @@ int tsc_window_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void*
   if (!aligned(out, 16) || !aligned(out_lo, 16) || !aligned(lse, 4) || !aligned(workspace, 16))
     return fail(TSC_ERR_INVALID, "window_attention: out, out_lo and workspace must be 16-byte aligned");
   const size_t no = head_span(x.z, total_q, (int64_t)num_heads * head_dim, num_heads);
-  for (const void* o : {(const void*)out, (const void*)out_lo})
-    if (o && (overlaps(o, no, q, head_span(x.z, total_q, ld_q, num_heads)) ||
-              overlaps(o, no, k, head_span(x.z, total_kv, ld_k, num_kv_heads)) ||
-              overlaps(o, no, v, head_span(x.z, total_kv, ld_v, num_kv_heads))))
+  const size_t n_cu = ((size_t)B + 1) * 4;
+  const void* outs[3] = {out, out_lo, lse};
+  const size_t o_bytes[3] = {no, no, (size_t)total_q * num_heads * 4};
+  for (int i = 0; i < 3; ++i) {
+    if (!outs[i]) continue;
+    if (overlaps(outs[i], o_bytes[i], q, head_span(x.z, total_q, ld_q, num_heads)) ||
+        overlaps(outs[i], o_bytes[i], k, head_span(x.z, total_kv, ld_k, num_kv_heads)) ||
+        overlaps(outs[i], o_bytes[i], v, head_span(x.z, total_kv, ld_v, num_kv_heads)) ||
+        (B > 0 && (overlaps(outs[i], o_bytes[i], cu_seqlens_q, n_cu) || overlaps(outs[i], o_bytes[i], cu_seqlens_kv, n_cu))))
       return fail(TSC_ERR_INVALID, "window_attention: out overlaps an input");
-  if (out_lo && overlaps(out, no, out_lo, no))
-    return fail(TSC_ERR_INVALID, "window_attention: out overlaps out_lo");
+    for (int j = 0; j < i; ++j)
+      if (outs[j] && overlaps(outs[i], o_bytes[i], outs[j], o_bytes[j]))
+        return fail(TSC_ERR_INVALID, "window_attention: the outputs overlap");
+  }
   DeviceGuard g(ctx->device);
   if (B == 0) return zero_launch(ctx, out, (int64_t)no);  // every row is outside
   return window_attention_launch(ctx, x, out, out_lo, lse, workspace);
