@@ -49,6 +49,27 @@ def test_block(pkg, dev, dtype, heads, kv_heads, causal, post):
         block(x, mod[:, :5])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens", [[0], [0, 0], [1], [0, 1]])
+def test_block_of_one_row_or_none(pkg, dev, dtype, lens):
+    heads, kv_heads, d = 2, 1, 64
+    c = heads * d
+    x, mod, g = _tokens(pkg, dev, lens, c, dtype, 3)
+    w = [_weight(g, dtype, dev, (heads + 2 * kv_heads) * d, c), _weight(g, dtype, dev, c, c),
+         _weight(g, dtype, dev, 2 * c, c), _weight(g, dtype, dev, c, 2 * c)]
+    block = pkg.SparseModulatedBlock3d(heads, 30, w[0], None, w[1], None, w[2], None, w[3], None, num_kv_heads=kv_heads)
+    got = block(x, mod)
+    assert got.feats.shape == x.feats.shape and got.feats.dtype == dtype
+    if sum(lens):  # one row attends to itself alone: its v, for both heads
+        m = mod[-1:]
+        h = pkg.modulated_norm(x.feats, None, m[:, 1], m[:, 0])
+        v = pkg.sparse_linear(h, w[0], None)[:, -d:]
+        a = pkg.sparse_linear(torch.cat([v, v], 1).contiguous(), w[1], None)
+        r, h = pkg.gated_residual_norm(x.feats, a, None, m[:, 2], scale=m[:, 4], shift=m[:, 3])
+        f = pkg.sparse_linear(pkg.silu(pkg.sparse_linear(h, w[2], None)), w[3], None)
+        assert torch.equal(got.feats, pkg.gated_residual(r, f, None, m[:, 5]))
+
+
 def _reference(x, mod, w1, w2, cu, heads, window, sinks):
     """The same step in fp64, from its definition."""
     def norm(t):

@@ -122,7 +122,7 @@ class SparseModulatedBlock3d:
         h = ops.modulated_norm(x.feats, cu, scale1, shift1, self.norm, eps=self.eps)
         qkv = ops.sparse_linear(h, self.qkv.weight, self.qkv.bias)
         hq, hk = self.num_heads, self.num_kv_heads
-        qkv = qkv.view(qkv.shape[0], hq + 2 * hk, -1)
+        qkv = qkv.unflatten(1, (hq + 2 * hk, qkv.shape[1] // (hq + 2 * hk)))
         a = ops.sparse_window_attention(qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:], self.window, cu,
                                         sinks=self.sinks, causal=self.causal, max_seqlen_q=longest,
                                         max_seqlen_kv=longest)
