@@ -376,7 +376,7 @@ int tsc_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void* k, con
  *     k and v may be slices of one fused projection); all other buffers are contiguous
  *   lambda     device fp32 (num_heads)
  *   cu_seqlens_q / cu_seqlens_kv, scale, max_seqlen_q  as in tsc_attention, scale <= 0 meaning
- *     1/sqrt(head_dim / 2); max_seqlen_kv likewise (both size the workspace too: the same values
+ *     1/sqrt(head_dim / 2), scale log2(e) finite in fp32; max_seqlen_kv likewise (both size the workspace too: the same values
  *     there).  A sequence without keys gives zeros.
  *   zero_rest  rows of out outside every sequence (all of them if B is 0): 0 = left as they were,
  *     1 = zeroed

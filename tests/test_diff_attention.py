@@ -114,3 +114,14 @@ def test_scales_beyond_fp32_are_refused(pkg):
             pkg.sparse_diff_attention(q, q, q, lam, [0, 10], scale=scale)
     with pytest.raises(pkg.TscError, match="not on a GPU"):  # this one is taken
         pkg.sparse_diff_attention(q, q, q, lam, [0, 10], scale=1e-30)
+
+
+def test_scales_whose_powers_of_two_overflow_are_refused(pkg):
+    """Scores are multiplied with scale log2(e), which fp32 has to hold: 2^128 / log2(e) is 2.3587e38."""
+    f, q = pkg.sparse_diff_attention, _t(10)
+    for scale in (2.36e38, 3.4e38):
+        with pytest.raises(pkg.TscError, match="scale"):
+            f(q, q, q, torch.zeros(2), [0, 10], scale=scale)
+    for scale in (2.35e38, 1e-45):
+        with pytest.raises(pkg.TscError, match="not on"):
+            f(q, q, q, torch.zeros(2), [0, 10], scale=scale)

@@ -83,3 +83,14 @@ def test_scratch_of_parts_stays_near_the_inputs(pkg):
                                 assert 0 <= got <= max(64 << 20, 8 * d * size * (tq * h + tkv * hk))
                                 split += got > 0
     assert split > 200
+
+
+def test_scales_whose_powers_of_two_overflow_are_refused(pkg):
+    """Scores are multiplied with scale log2(e), which fp32 has to hold: 2^128 / log2(e) is 2.3587e38."""
+    f, q = pkg.sparse_window_attention, _t(10)
+    for scale in (2.36e38, 3.4e38):
+        with pytest.raises(pkg.TscError, match="scale"):
+            f(q, q, q, 4, [0, 10], scale=scale)
+    for scale in (2.35e38, 1e-45):
+        with pytest.raises(pkg.TscError, match="not on"):
+            f(q, q, q, 4, [0, 10], scale=scale)

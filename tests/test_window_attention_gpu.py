@@ -625,3 +625,29 @@ def test_outputs_over_offsets_and_statistics_are_refused(pkg, dev):
         st = lib.tsc_window_attention(handle, 0, p, p, p, h * d, h * d, h * d, cu.data_ptr(), cu.data_ptr(), 1, n, n, h, h, d,
                                       0.0, 4, 0, 0, n, n, 0, None, out.data_ptr(), None, lse.data_ptr())
         assert st == 1 and b"overlap" in lib.tsc_last_error()
+
+
+def test_c_scales(pkg, dev):
+    """NaN, infinity and what overflows once it is multiplied with log2(e) are refused; 0 and less mean the default."""
+    n, h, d = 40, 2, 64
+    x = torch.randn((n, h, d), generator=torch.Generator().manual_seed(83)).to(dev)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    lib, handle = pkg.ops._lib.stream_handle(0)
+    p = x.data_ptr()
+    out, dq, dk, dv = (torch.full_like(x, 7.0) for _ in range(4))
+    lse = torch.zeros((n, h), device=dev)
+    ws = torch.empty((lib.tsc_window_attention_workspace_bytes(0, 1, n, n, h, h, d, 4, 0, 0, n, n, 1),), dtype=torch.uint8,
+                     device=dev)
+
+    def run(scale):
+        a = (handle, 0, p, p, p, h * d, h * d, h * d, cu.data_ptr(), cu.data_ptr(), 1, n, n, h, h, d, scale, 4, 0, 0, n, n, 0)
+        return (lib.tsc_window_attention(*a, None, out.data_ptr(), None, lse.data_ptr()),
+                lib.tsc_window_attention_backward(*a, out.data_ptr(), None, lse.data_ptr(), p, ws.data_ptr(), dq.data_ptr(),
+                                                  dk.data_ptr(), dv.data_ptr()))
+
+    for scale in (float("nan"), float("inf"), 3e38):
+        assert run(scale) == (1, 1) and b"scale" in lib.tsc_last_error()
+    assert bool((out == 7).all())
+    for scale in (0.0, -1.0, float("-inf")):
+        assert run(scale) == (0, 0)
+        assert torch.equal(out, pkg.sparse_window_attention(x, x, x, 4, cu))

@@ -115,6 +115,9 @@ static bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
   return na && nb && x < y + nb && y < x + na;
 }
 
+// A scale above 0 (others mean the default) whose product with log2(e) fp32 does not hold, or NaN.
+static bool bad_scale(float scale) { return !(scale <= 0.f) && !isfinite(scale * 1.44269504f); }
+
 static int elem_size(int32_t dtype) {
   switch (dtype) {
     case TSC_F32: return 4;
@@ -934,6 +937,7 @@ static int diff_attention_args(tsc_ctx* ctx, const char* what, int32_t dtype, co
       max_kv < 0 || total_q > INT32_MAX || total_kv > INT32_MAX)
     return fail(TSC_ERR_INVALID, "%s: bad sizes B=%d H=%d total_q=%lld total_kv=%lld", what, B, H,
                 (long long)total_q, (long long)total_kv);
+  if (bad_scale(scale)) return fail(TSC_ERR_INVALID, "%s: scale and scale * log2(e) must be finite in fp32", what);
   *x = DiffAttnArgs{dtype, q, k, v, ld_q, ld_k, ld_v, lambda, cu_q, cu_kv, B, total_q, total_kv, H, D,
                     scale > 0.f ? scale : 1.f / sqrtf((float)D / 2), max_q, max_kv, rest};
   if (!ctx || B == 0) return TSC_OK;  // the sizes only
@@ -1126,6 +1130,7 @@ int tsc_window_attention(tsc_ctx* ctx, int32_t dtype, const void* q, const void*
                           max_seqlen_q, max_seqlen_kv},
                          q, k, v, ld_q, ld_k, ld_v, cu_seqlens_q, cu_seqlens_kv,
                          scale > 0.f ? scale : 1.f / sqrtf((float)head_dim), zero_rest};
+  if (bad_scale(scale)) return fail(TSC_ERR_INVALID, "window_attention: scale and scale * log2(e) must be finite in fp32");
   st = window_attention_args("window_attention", x);
   if (st) return st;
   if (total_q == 0 || (B == 0 && !zero_rest)) return TSC_OK;
@@ -1172,6 +1177,7 @@ int tsc_window_attention_backward(tsc_ctx* ctx, int32_t dtype, const void* q, co
                           max_seqlen_q, max_seqlen_kv},
                          q, k, v, ld_q, ld_k, ld_v, cu_seqlens_q, cu_seqlens_kv,
                          scale > 0.f ? scale : 1.f / sqrtf((float)head_dim), zero_rest};
+  if (bad_scale(scale)) return fail(TSC_ERR_INVALID, "window_attention_backward: scale and scale * log2(e) must be finite in fp32");
   st = window_attention_args("window_attention_backward", x);
   if (st) return st;
   if ((total_q > 0 && (!dq || (B > 0 && (!out || !lse || !dout || !workspace || (dtype != TSC_F32 && !out_lo))))) ||

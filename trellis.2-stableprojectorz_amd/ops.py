@@ -795,6 +795,11 @@ def _head_rows(t: torch.Tensor, name: str) -> int:
     return t.stride(0) if t.shape[0] > 1 else h * d
 
 
+def _scale_fits(scale) -> bool:
+    """The kernels take scores to powers of two: it is scale log2(e) that fp32 has to hold."""
+    return 0 < ctypes.c_float(scale).value and ctypes.c_float(scale * 1.4426950408889634).value < float("inf")
+
+
 def sparse_diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
                           cu_seqlens_q, cu_seqlens_kv=None, scale: float | None = None, out=None,
                           max_seqlen_q: int | None = None,
@@ -822,8 +827,9 @@ def sparse_diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam
         raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: q, k and v must share a dtype")
     if lam.shape != (h,) or lam.dtype != torch.float32:
         raise TscError(_lib.TSC_ERR_INVALID, f"diff_attention: lam must be float32 ({h},)")
-    if scale is not None and not 0 < ctypes.c_float(scale).value < float("inf"):
-        raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: scale must be positive and finite in fp32")
+    if scale is not None and not _scale_fits(scale):
+        raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: scale must be positive and finite in fp32, and so "
+                                             "its product with log2(e)")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
         raise TscError(_lib.TSC_ERR_INVALID, "diff_attention: out has the wrong shape or dtype")
     _code(q)
@@ -943,8 +949,9 @@ def sparse_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
     if not 0 <= window <= _NO_BOUND or not 0 <= sinks <= _NO_BOUND:
         raise TscError(_lib.TSC_ERR_INVALID, f"window_attention: window {window} and sinks {sinks} must be in "
                                              "[0, 2^31)")
-    if scale is not None and not 0 < ctypes.c_float(scale).value < float("inf"):
-        raise TscError(_lib.TSC_ERR_INVALID, "window_attention: scale must be positive and finite in fp32")
+    if scale is not None and not _scale_fits(scale):
+        raise TscError(_lib.TSC_ERR_INVALID, "window_attention: scale must be positive and finite in fp32, and so "
+                                             "its product with log2(e)")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
         raise TscError(_lib.TSC_ERR_INVALID, "window_attention: out has the wrong shape or dtype")
     code = _code(q)
