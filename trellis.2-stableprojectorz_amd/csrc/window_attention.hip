@@ -522,12 +522,14 @@ __global__ void __launch_bounds__(64 * NW, 2) wa_forward16_kernel(const WaArgs a
         return mx;
       };
       // Raises the running maxima of row tile i where a score exceeds one by more than 2^kLazy: those alone, so that
-      // a row's bits do not depend on the scores of the rows beside it.
+      // a row's bits do not depend on the scores of the rows beside it.  (The others' as -inf: with the comparison kept for
+      // a selection, 29 registers spill where KEEP has 64 dimensions.)
       auto raise = [&](int i, float mx) {
         mx *= sl2;
-        const bool over = mx > mc[i] + kLazy, up = __builtin_amdgcn_ballot_w64(over) != 0;
+        mx = mx > mc[i] + kLazy ? mx : -INFINITY;
+        const bool up = __builtin_amdgcn_ballot_w64(mx > mc[i]) != 0;
         if (up) {
-          const float mn = over ? mx : mc[i];
+          const float mn = fmaxf(mc[i], mx);
           alpha[i] = fast_exp2(mc[i] - mn);
           mc[i] = mn;
           if (KEEP) lu[i] *= alpha[i];  // before the next exponentials are added to it
