@@ -651,3 +651,21 @@ def test_c_scales(pkg, dev):
     for scale in (0.0, -1.0, float("-inf")):
         assert run(scale) == (0, 0)
         assert torch.equal(out, pkg.sparse_window_attention(x, x, x, 4, cu))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,h,hk", [(128, 12, 12), (64, 16, 4)])
+@pytest.mark.parametrize("lens", [[30] * 120 + [0] * 3 + [1] * 40 + [257], [600, 1, 1, 1, 1, 1, 1, 1], [1] * 700])
+@pytest.mark.parametrize("window,sinks,causal", [(10, 3, False), (200, 40, True)])
+def test_many_short_sequences(pkg, dev, dtype, d, h, hk, lens, window, sinks, causal):
+    """Grids of wide blocks most of whose rows, or most of which, have nothing to do; the first and the last key head."""
+    q, k, v, do = _make(lens, lens, h, hk, d, dtype, 89 + len(lens))
+    cq = _cu(lens)
+    print(f"  window attention short {dtype} D={d} {len(lens)} sequences H={h}/{hk} w={window} {causal}", flush=True)
+    got = _run(pkg, dev, q, k, v, do, window, cq, None, sinks=sinks, causal=causal)
+    g = h // hk
+    ks = [0, hk - 1]
+    qs = [x * g + i for x in ks for i in range(g)]
+    want = _oracle(q[:, qs], k[:, ks], v[:, ks], do[:, qs], cq, cq, dtype, window, sinks, causal)
+    for n in got:
+        check(got[n][:, qs if n in ("out", "dq") else ks], want[n], n)
