@@ -669,3 +669,28 @@ def test_many_short_sequences(pkg, dev, dtype, d, h, hk, lens, window, sinks, ca
     want = _oracle(q[:, qs], k[:, ks], v[:, ks], do[:, qs], cq, cq, dtype, window, sinks, causal)
     for n in got:
         check(got[n][:, qs if n in ("out", "dq") else ks], want[n], n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_tokens_of_several_objects_on_a_cache_with_room(pkg, dev, dtype, d):
+    """A cache of three sequences that grow in place: the unused rows behind each one's keys are a sequence without a
+    query, and whatever they hold stays out."""
+    h, hk, window, sinks, room = 8, 2, 50, 3, (400, 130, 40)
+    start = _cu(room)
+    _, k, v, _ = _make(room, room, h, hk, d, dtype, 97)
+    cache = [torch.full(t.shape, float("nan"), dtype=dtype, device=dev) for t in (k, v)]
+    cq = torch.tensor([0, 1, 1, 2, 2, 3, 3], dtype=torch.int32, device=dev)
+    for step, lens in enumerate(([1, 1, 1], [64, 129, 40], [399, 130, 0], [400, 0, 33])):
+        for a, n in zip(start, lens):
+            for to, of in zip(cache, (k, v)):
+                to[a:a + n] = of[a:a + n].to(dev)
+        q = _make([3], [0], h, hk, d, dtype, 101 + step)[0]
+        ck = torch.tensor([0] + [x for a, b, n in zip(start, start[1:], lens) for x in (a + n, b)], dtype=torch.int32, device=dev)
+        got = pkg.sparse_window_attention(q.to(dev), *cache, window, cq, ck, sinks=sinks, causal=True, max_seqlen_q=1,
+                                          max_seqlen_kv=max(lens))
+        keys = [torch.cat([t[a:a + n] for a, n in zip(start, lens)]) for t in (k, v)]
+        want = _oracle(q, *keys, torch.zeros_like(q), [0, 1, 2, 3], _cu(lens), dtype, window, sinks, True)["out"]
+        check(got, want, f"{lens}")
+        for t in cache:
+            t.fill_(float("nan"))
