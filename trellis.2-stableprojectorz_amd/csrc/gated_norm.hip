@@ -23,10 +23,13 @@
 // (block t and sample b; along the rows one of the two grows at each step, so slots are distinct),
 // and a second kernel adds up each sample's slots.
 //
-// Measured (us; TB/s of what each pass has to read and write; a copy of 1 GiB reaches 5.1): forward, r and h of 243547 x
-// 512 bf16 186 (5.35), of 64304 x 1024 111 (4.8), h of 15143 x 1536 22 (4.2); gradient, both norms, of 243547 x 512 bf16
-// 339 (4.4) with the sums' kernel, of 60000 x 1024 fp32 357 (4.1), of 60000 x 1536 bf16 320 (3.4): with the sums of both
-// norms two waves a SIMD are left to wait for memory and for each row's two reductions.
+// Measured (each kernel by itself in a trace, us; TB/s of what the pass has to read and write; a copy of 1 GiB reaches
+// 5.1), bf16 in two samples with a norm after (rms) and a norm before (layer), weights and biases of both: forward, r and h,
+// 243547 x 512 206 (4.8), 64304 x 1024 133 (4.0), 60000 x 1536 170 (4.3); gradient and, behind the +, the kernel of its sums,
+// 243547 x 512 321 (4.7) + 10, 64304 x 1024 174 (4.5) + 28, 60000 x 1024 fp32 324 (4.6) + 30, 60000 x 1536 297 (3.7) + 20: with the
+// sums of both norms two waves a SIMD are left to wait for memory and for each row's two reductions.  Without weights and
+// biases, and without a norm after: r and h of 64304 x 1024 110 (4.8), h of 15143 x 1536 23 (4.1).  The kernel figures at the
+// constants are of the same inputs unless they say otherwise.
 
 #include <algorithm>
 #include <initializer_list>
@@ -38,16 +41,16 @@ namespace tsc {
 namespace {
 
 // Most values of a wave's lane, forward and backward: wider rows have a block.  (64304 x 1024 bf16 with 16 in the
-// gradient 278 us, 253 in blocks; 60000 x 1024 fp32 776, 357: its registers spill.)
+// gradient 199 + 9 us, in blocks 174 + 28; 60000 x 1024 fp32 667 + 10, its registers spill, and 324 + 30.)
 constexpr int kLaneF = 16, kLaneB = 8;
 // Threads of a block of the gradient, where a row has lanes of a wave: its waves add up their sums in LDS.  (400000 x 256
-// bf16 in 256 threads 316 us, in 512 301.)
+// bf16 in 256 threads 273 + 19 us, in 512 275 + 10.)
 constexpr int kBackThreads = 512;
 constexpr int kMaxC = 8192;     // widest row of a block of 16 waves
 constexpr int kSumCols = 16, kSumRows = 64, kSumWaves = kSumCols * kSumRows / 64;  // of a block that adds up slots
 // Rows on their way where a block of 16-byte vectors has both norms' gradients and two waves a SIMD: of few bytes each.
-// us, bf16, 1 / 2 / 3 / 4: 60000 x 1536 314 / 277 / 267 / 273, 30000 x 4096 403 / 353 / 341 / 348.  Others have more waves
-// (modulated_norm, 60000 x 1536: 149 with 1, 175 with 3) or no registers (16000 x 8192: 634, 1258).
+// us, bf16, 1 / 2 / 3 / 4: 60000 x 1536 350 / 325 / 297 / 316, 30000 x 4096 491 / 431 / 398 / 407.  Others have more waves
+// (modulated_norm, 60000 x 1536: 131 with 1, 163 with 3) or no registers (16000 x 8192: 745, 1398).
 constexpr int kAhead = 3;
 constexpr int kLoopB = 16;      // samples that one block of that kernel walks
 
@@ -214,6 +217,8 @@ __device__ __forceinline__ float2 normalize(Tm& team, int kind, float inv_c, flo
   return make_float2(mean, rstd);
 }
 
+// A row's block is bounded by the widest rows' 1024 threads whatever its own: rows in single values, of widths that nothing
+// wider divides or that are not aligned, spill for it (88 to 90 registers with both parts), and fp32 ones of both parts 6.
 template <typename T, int VN, int MAXV, bool BLOCK, bool Y, bool H>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 256) gated_norm_kernel(const GnArgs a) {
   Team<MAXV, BLOCK> team(a.G);
@@ -351,7 +356,9 @@ __device__ __forceinline__ void flush(const GnArgs& a, const Team<MAXV, BLOCK>& 
   }
 }
 
-// NT: threads of a block at most.  Rows of more than 4096 values, whose blocks have 1024, spill registers.
+// NT: threads of a block at most.  Rows of more than 4096 values, whose blocks have 1024 threads of 128 registers, spill:
+// with both norms 55 registers in 16 bits, 103 in fp32, 192 in single values; so do single values with both norms at 512
+// threads, 28 to 36.
 template <typename T, int VN, int MAXV, bool BLOCK, int NT, bool Y, bool H>
 __global__ void __launch_bounds__(NT) gated_norm_backward_kernel(const GnArgs a) {
   constexpr int AHEAD = sizeof(T) == 2 && VN == 8 && BLOCK && NT == 512 && Y && H ? kAhead : 1;  // rows on their way
@@ -653,17 +660,18 @@ int64_t rows_of(const Shape& s, int64_t N, int64_t most) {
   return s.rows * std::max<int64_t>(1, (steps + most - 1) / most);
 }
 // Blocks of the forward pass: enough that those at work at one time are near each other in memory, and rows enough in
-// each for its sample's parameters.  us, r and h of bf16: 243547 x 512 in 2048 blocks 213, 8192 186, 16384 202;
-// 60000 x 1536 (rows of a block) in 2048 164, 4096 160; 16000 x 8192 in 2048 264, 4096 292; 64304 x 1024 (two vectors a
-// lane) in 2048 114, 4096 111.
+// each for its sample's parameters.  us, r and h of bf16: 243547 x 512 in 2048 blocks 210, 8192 206, 16384 233; 60000 x
+// 1536 (rows of a block) in 2048 177, 4096 170, 8192 172; 16000 x 8192 in 2000 340, 4096 371.  64304 x 1024 (two vectors a lane) in
+// 2048 119, 4096 133; without weights, biases and a norm after (timed among others, not in a trace) 110, 108.
 int64_t forward_blocks(const Shape& s, int64_t N) {
   if (!s.block) return s.maxv == 1 ? 8192 : 4096;
   return std::min<int64_t>(4096, std::max<int64_t>(1, N / 8));
 }
 // Waves of a CU in the gradient, by its registers: with the sums of r's norm and of y's (176 to 256), of one (92 to 128).
 constexpr int kBothWaves = 8, kOneWaves = 16;
-// Blocks of the gradient: as many as run at once; more of them leave more sums to add up.  us, both norms, bf16: 64304 x
-// 1024 253 with 8 waves a CU, 319 with 12 or 16; 60000 x 1536 374, 393, 454; 243547 x 512 339, 339, 355.
+// Blocks of the gradient: as many as run at once; more of them leave more sums to add up.  us, both norms and the sums' kernel,
+// bf16, with 8 / 12 / 16 waves a CU: 64304 x 1024 174 + 28, 214 + 47, 228 + 58; 60000 x 1536 297 + 20, 307 + 36, 348 + 37; 243547 x
+// 512 321 + 10, 319 + 10, 321 + 24.
 int64_t back_blocks(const Shape& s, bool both) {
   return 256 * std::max(1, (both ? kBothWaves : kOneWaves) * 64 / s.threads);
 }

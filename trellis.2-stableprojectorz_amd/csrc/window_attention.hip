@@ -303,8 +303,10 @@ __device__ __forceinline__ void store_lse(const WaArgs& a, int64_t at, int hf, f
   if (a.lse && hf == 0) a.lse[at] = row_lse(m, l, some);
 }
 
-// fp32: a block of 4 waves owns 128 rows and walks their keys in tiles of 32.  Bound by the fp32 products (151 TFLOP/s at
-// most): 3500 tokens of 12 x 128, window 256, 215 us, 50 TFLOP/s of the pairs that are seen.
+// fp32: a block of 4 waves owns 128 rows and walks their keys in tiles of 32.  3500 tokens of 12 x 128, window 256: 226 us, 47
+// of the 151 TFLOP/s of a large product by the pairs that are seen (80 % of a tile's).  Matrix cores busy 32 %, VALU 10 %,
+// waves waiting 22 %: a wave has its SIMD for itself at D = 128 (416 registers), so 336 blocks take two rounds over the CUs of
+// which the second fills a third, and in a wave products, exponentials and two barriers a tile follow one another.
 template <int D>
 __global__ void __launch_bounds__(kNT, D == 64 ? 2 : 1) wa_forward32_kernel(const WaArgs a) {
   typedef float T;
@@ -747,8 +749,8 @@ __global__ void __launch_bounds__(64 * NW, 2) wa_forward16_kernel(const WaArgs a
 // Small grids: a block owns 32 rows, and its waves, and the blocks of a.splits parts, share out their key
 // tiles.  Each wave brings its own tiles through its own piece of LDS, so none waits for another until
 // the end, where their maxima, denominators and sums are joined.  Bound by latency: a wave's tile is loaded, brought
-// through LDS and multiplied before the next.  One token each on 33 to 20011 keys (16 / 4 x 128 bf16, window 4095, 52 MB):
-// 18 us, 2.9 TB/s, and 5 for the join; 311 + 1 + 150 tokens of 8 x 64 fp32 12 us.
+// through LDS and multiplied before the next.  One token each on 33 to 20011 keys (16 / 4 x 128 bf16, window 4095, 53 MB):
+// 17 us, 3.3 TB/s, and 4 for the join; 311 + 1 + 150 tokens of 8 x 64 fp32 12 us.
 __device__ __forceinline__ float* part_sums(const WaArgs& a, int sp, int64_t at, int D) {
   return a.part + ((int64_t)sp * a.total_q * a.Hk * a.G + at) * D;
 }
@@ -919,7 +921,7 @@ __device__ __forceinline__ void tile_sync() {
 
 // dq of 128 (32) rows, and r = do . out of each, which dk / dv read after it; out with what its rounding left:
 // dS = P (dP - r) cancels where one key has most of a row, and out's rounding would be most of what is left.
-// 15143 tokens of 12 x 128 bf16, window 256: 182 us, 500 MB from the L2s at 3.2 TB/s, matrix cores busy 18 %, VALU 27 %,
+// 15143 tokens of 12 x 128 bf16, window 256: 182 us, 500 MB to the L2s and 3.2 TB/s with its writes, matrix cores busy 18 %, VALU 27 %,
 // waves waiting 47 %: two of 256 registers a SIMD (15 spilled), each with its products and its exponentials in turn.  r in a
 // kernel of its own: 30 us less here, 25 there, and a launch more.
 template <typename T, int D, bool SHARE>
@@ -1082,8 +1084,8 @@ __device__ __forceinline__ Spans spans_of(const WaArgs& a, int first, int last, 
 // dk and dv of 128 (32) keys of a key head, over the rows of all its query heads.  Every row sees the sinks: where
 // that is many times what sees another key, they are left to SINKS blocks (32 keys, and of their rows one of
 // sink_parts parts; 15143 tokens, 12 x 128 bf16, window 256, 16 sinks: the first tile's blocks took 28 times
-// the others' rows and 970 of the step's 1374 us; now 30 and 4 for adding up the parts).  Spills up to 18 registers at
-// D = 64 and two waves a SIMD.
+// the others' rows and 970 of the step's 1374 us; now 32 and 4 for adding up the parts).  Spills up to 18 registers at
+// D = 64 and two waves a SIMD, up to 27 in fp32 at D = 128 and one.
 template <typename T, int D, bool SHARE, bool SINKS>
 __global__ void __launch_bounds__(kNT, D == 64 && (sizeof(T) == 2 || SHARE) ? 2 : 1) wa_dkv_kernel(const WaArgs a) {
   static_assert(SHARE || !SINKS, "sinks: 32 keys");
@@ -1487,7 +1489,7 @@ Plan wa_plan(const WindowAttnSizes& z) {
 
 // The blocks that share the rows of a tile of sinks: a block on each CU, of four waves' tiles of rows at least, in
 // scratch as above; 1: sinks are keys like others, whose blocks would not have twice the rows of another's.
-// (16384 tokens, 12 x 128 bf16, 4 sinks: 45 us in 30 parts, 54 in 7.)
+// (16384 tokens, 12 x 128 bf16, window 256, 4 sinks: 30 us in 21 parts, 39 in 30, 52 in 7, and 4 to 5 to add them up.)
 struct SinkPlan {
   int parts, keys;
   int64_t bytes;
