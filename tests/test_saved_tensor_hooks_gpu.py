@@ -99,3 +99,31 @@ def test_group_norm_and_diff_attention(pkg, dev, dtype, hook):
     qkv, do = leaf(n, 3, h, d), leaf(n, h, d).detach()
     lam = torch.rand(h, generator=g).to(dev).requires_grad_()
     _same([qkv, lam], lambda: [pkg.sparse_diff_attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], lam, cu)], [do], HOOKS[hook])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_checkpointed_step(pkg, dev, dtype):
+    """Recomputed in the backward pass, which hands its tensors to the gradients through hooks."""
+    from torch.utils.checkpoint import checkpoint
+
+    g = torch.Generator().manual_seed(73)
+    n, h, d = 90, 2, 64
+    c = h * d
+    cu = torch.tensor([0, 50, 90], dtype=torch.int32, device=dev)
+
+    def leaf(*shape):
+        return torch.randn(shape, generator=g).to(dtype).to(dev).requires_grad_()
+
+    x, mod, w = leaf(n, c), leaf(2, 6, c), leaf(3 * c, c)
+    dr, dh = leaf(n, c).detach(), leaf(n, c).detach()
+
+    def block(x, mod, w):
+        qkv = torch.nn.functional.linear(pkg.modulated_norm(x, cu, mod[:, 1], mod[:, 0]), w / c ** 0.5).view(n, 3, h, d)
+        a = pkg.sparse_window_attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], 20, cu, sinks=2)
+        return pkg.gated_residual_norm(x, a.flatten(1), cu, mod[:, 2], scale=mod[:, 4], shift=mod[:, 3])
+
+    leaves = [x, mod, w]
+    want = torch.autograd.grad(block(*leaves), leaves, [dr, dh])
+    got = torch.autograd.grad(checkpoint(block, *leaves, use_reentrant=False), leaves, [dr, dh])
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
